@@ -86,8 +86,8 @@ def draw(rng):
         if op in ("attention", "mass"):  # products of 32-bit values cost more
             return max(slots * size / (1 << 28), slots * c["tokens"] * group * c["width"] / (8e8 if c["type"] == "fp32" else 8e9))
         if op == "append":
-            return c["batch"] * c["tokens"] * c["heads"] * size / (1 << 25)
-        return slots * size / (3 << 26 if op == "evict" else 1 << 29)
+            return c["batch"] * c["tokens"] * (c["heads"] + 2 * kv) * (c["width"] * 4 + size) / 150e6
+        return slots * size / (150e6 if op == "evict" else 500e6)
 
     while costs() > 1:  # no more than the largest listed cases
         big = max((x for x in (("batch", "tokens") if op == "append" else ("batch", "layers", "longest")) if x in c), key=lambda x: c[x])
