@@ -294,6 +294,132 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
                           int64_t ldq, float *E, int64_t lde, uint8_t *IDX, int64_t ldi, void *workspace, size_t workspace_bytes,
                           void *stream);
 
+/* ---------------------------------------------------------------- key/value cache operators --------------------- */
+
+/* What a decoder runs between its projections, on a cache of keys and values that holds `batch` sequences in `slots`
+ * slots each: write new tokens behind a sequence, let a tree of drafted tokens attend, take the accepted ones into the
+ * sequence, add up how much attention each slot drew, and keep the slots that drew most. (ggml builds the first two
+ * from RMS_NORM, MUL, ROPE, SET_ROWS and FLASH_ATTN_EXT nodes; it has no op for the others.)
+ *
+ * Sequence b is as long as the device array lens[b] says, and every call reads the lengths on the device, so that a
+ * captured graph stays valid while sequences grow. A call adds n_b tokens to sequence b: n_b = counts[b] where `counts`
+ * is given (0 <= counts[b] <= tokens), else `tokens`; token t of the call has slot lens[b] + t. Rows of tokens t >= n_b
+ * are neither read nor written. A sequence with lens[b] < 0, n_b out of its range or lens[b] + n_b > slots is left
+ * alone, outputs included (p8_tree_accept: reported as nothing accepted), and p8_device_error reports bit 6 (64).
+ *
+ * Layouts: element (layer, b, h, slot, d) of the keys is k[layer * k_stride[0] + b * k_stride[1] + h * k_stride[2] +
+ * slot * k_stride[3] + d], of the values alike. width is 64 or 128; every base address and every stride that is used
+ * (its dimension is above 1) is a multiple of 16 bytes. Query heads: `heads` is a multiple of the cache's heads, query
+ * head i reads cache head i / (heads / kv heads). Strides are in elements. */
+typedef enum p8_kv_type { P8_KV_F32 = 0, P8_KV_F16 = 1, P8_KV_BF16 = 2 } p8_kv_type;
+#define P8_TREE_MAX 64   /* tokens of one sequence in a tree attention, mass or accept call */
+#define P8_BATCH_MAX 4096
+typedef struct p8_kv {
+    void *k, *v;
+    int64_t type;                      /* p8_kv_type of k and v */
+    int64_t layers, batch, heads, slots, width;
+    int64_t k_stride[4], v_stride[4];  /* layer, sequence, head, slot */
+} p8_kv;
+
+/* New tokens into one layer's cache (layers = 1): q, k, v f32 as the projections leave them, element (b, t, h, d) at
+ * b * stride[0] + t * stride[1] + h * stride[2] + d. Per head and token: x' = x / sqrt(mean(x^2) + eps) * norm (where
+ * q_norm / k_norm [width] is given), then the halves rotate by the token's position p = pos[b * tokens + t]:
+ *     y[i] = x'[i] cos[p][i] - x'[i + width/2] sin[p][i],  y[i + width/2] = x'[i + width/2] cos[p][i] + x'[i] sin[p][i]
+ * with cos / sin f32 [positions][width / 2]. Rotated keys and plain values are rounded once to the cache's type and
+ * written to the tokens' slots, rotated queries to q_out (the cache's type). Any number of tokens. A token whose
+ * position is outside [0, positions) is left out and sets bit 6. */
+typedef struct p8_kv_append_args {
+    const float *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t tokens, heads;
+    const int32_t *lens, *counts, *pos;   /* [batch], [batch] or NULL, [batch][tokens] */
+    const float *cos, *sin;
+    int64_t positions;
+    const float *q_norm, *k_norm;         /* [width] or NULL */
+    double eps;
+    void *q_out;
+    int64_t q_out_stride[3];
+} p8_kv_append_args;
+p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream);
+
+/* Attention of 1..P8_TREE_MAX tokens per sequence over one layer's cache (layers = 1), the tokens' own keys and values
+ * already in their slots. Token t sees every slot before lens[b] and drafted token j < n_b where bit j of
+ * mask[b * mask_stride + t] is set (mask NULL: j <= t, a chain). out = softmax(scale q k^T) v over what it sees, in q's
+ * type (the cache's); lse [batch][tokens][heads] f32 (or NULL) the natural log of the sum of exponentials. A token that
+ * sees nothing gets 0 and -infinity. What a token does not see does not reach it, whatever its bits (infinities and NaN
+ * included). Products and sums in fp32 (16-bit types: the weights are rounded to the type before they multiply v).
+ * Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
+typedef struct p8_tree_attn_args {
+    const void *q;
+    int64_t q_stride[3];                  /* sequence, token, head */
+    int64_t tokens, heads;
+    const int32_t *lens, *counts;
+    const uint64_t *mask;
+    int64_t mask_stride;                  /* 0 (one tree for all sequences) or tokens */
+    double scale;
+    void *out;
+    int64_t out_stride[3];
+    float *lse;
+} p8_tree_attn_args;
+size_t p8_tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads);
+p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The attention weight that each slot drew, added up over tokens and the query heads of its cache head. The n_b tokens
+ * are a chain behind the sequence (one decoded token, the end of a prompt, or an accepted path whose keys
+ * p8_tree_accept has moved into place): token i sees slots <= lens[b] + i, and its query and lse rows are those of row
+ * r = rows[b * tokens + i] (rows NULL: r = i) of a p8_tree_attn call. With w the sum of exp(scale q . k - lse):
+ *     out[b][h][j] = mass[b][h][j] + w for j < lens[b],  = w for the slots of the n_b tokens, untouched behind them.
+ * Strides of mass and out: sequence, head; out may be mass (in place). A row that is out of [0, tokens) counts for
+ * nothing and sets bit 6; a row with lse = -infinity counts for nothing. Deterministic. */
+typedef struct p8_attn_mass_args {
+    const void *q;
+    int64_t q_stride[3];
+    int64_t tokens, heads;
+    const float *lse;                     /* [batch][tokens][heads] */
+    const int32_t *lens, *counts, *rows;
+    double scale;
+    const float *mass;
+    int64_t mass_stride[2];
+    float *out;
+    int64_t out_stride[2];
+} p8_attn_mass_args;
+p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream);
+
+/* Shorten every sequence with more than `budget` slots to `budget`, per layer and head: the first `sinks` slots, the
+ * last `recent` slots and, of those between, the ones with the largest mass (ties: the lowest slot; NaN counts as
+ * -infinity), in their order. Keys, values and mass [layer][b][h] of the kept slots are written to the first slots of
+ * dst and mass_out, which are either the same buffers as src and mass (in place) or do not overlap them; a shorter
+ * sequence is kept whole. new_lens[b] = min(lens[b], budget), kept [layers][batch][heads][budget] the kept slots (-1
+ * behind new_lens[b]). sinks + recent <= budget <= the slots of dst and of src; new_lens must not be lens. Mass
+ * strides: layer, sequence, head. A sequence with lens[b] outside [0, slots] is left alone, its new_lens and kept too,
+ * and sets bit 6. */
+typedef struct p8_kv_evict_args {
+    const float *mass;
+    int64_t mass_stride[3];
+    float *mass_out;
+    int64_t mass_out_stride[3];
+    const int32_t *lens;
+    int32_t *new_lens, *kept;
+    int64_t budget, sinks, recent;
+} p8_kv_evict_args;
+p8_status p8_kv_evict(const p8_kv *src, const p8_kv *dst, const p8_kv_evict_args *a, void *stream);
+
+/* Greedy verification of a drafted tree: token 0 is the root (the last known token), parents[b][t] the node that token
+ * t hangs on (a child comes after its parent), target[b][t] the model's choice after node t. From the root the path
+ * goes on to the lowest child whose token is the target's at the node it has reached. The path's keys and values are
+ * moved, in all layers, from slots lens[b] + path[i] to lens[b] + i. path [batch][tokens] (-1 behind the path),
+ * accepted[b] its length, next_token[b] the target at its end, new_lens[b] = lens[b] + accepted[b]; n_b = 0: nothing
+ * accepted, next_token -1. new_lens must not be lens. */
+typedef struct p8_tree_accept_args {
+    const int64_t *tokens, *target;       /* [batch][ntokens] */
+    const int32_t *parents;
+    int64_t ntokens;
+    const int32_t *lens, *counts;
+    int32_t *path, *accepted, *new_lens;
+    int64_t *next_token;
+} p8_tree_accept_args;
+p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream);
+
 /* ---------------------------------------------------------------- model files (GGUF) ---------------------------- */
 
 /* A GGUF file holding a Pingala-8 ("VR native") model, opened and checked as llama_model_loader::vr_native_init does
@@ -315,8 +441,9 @@ p8_status p8_gguf_linear_info(const p8_gguf *g, int64_t i, const char **name, in
 p8_status p8_gguf_load_linear(p8_gguf *g, int64_t i, uint8_t *out, size_t out_cap, size_t *out_n);
 
 /* Non-zero if a kernel since the last call gave up (that launch's results are invalid), then clears the word. Bits:
- * 4 GEMM pipeline wait timed out, 8 row-parallel exchange wait timed out, 16 exchange entry with a foreign tag (1, 2
- * and 32 are unused). Synchronises the device. */
+ * 4 GEMM pipeline wait timed out, 8 row-parallel exchange wait timed out, 16 exchange entry with a foreign tag, 64 a
+ * cache operator met a length, count, position or row out of range and left it out, 128 a tree attention or mass
+ * pipeline wait timed out (1, 2 and 32 are unused). Synchronises the device. */
 int p8_device_error(void);
 
 const char *p8_status_str(p8_status s);

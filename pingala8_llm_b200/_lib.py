@@ -99,6 +99,12 @@ _SIGS = {
     "p8_chain_run": (C.c_int, [_vp, _vp, _sz, _vp]),
     "p8_chain_destroy": (C.c_int, [_vp]),
     "p8_chain_trace": (C.c_int, [_vp, _vp, _sz]),
+    "p8_kv_append": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
+    "p8_tree_attn_workspace": (_sz, [C.c_char_p, _i64, _i64]),
+    "p8_tree_attn": (C.c_int, [C.c_char_p, C.c_char_p, _vp, _sz, _vp]),
+    "p8_attn_mass": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
+    "p8_kv_evict": (C.c_int, [C.c_char_p, C.c_char_p, C.c_char_p, _vp]),
+    "p8_tree_accept": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
     "p8_device_error": (C.c_int, []),
     "p8_status_str": (C.c_char_p, [C.c_int]),
     "p8_build_info": (C.c_char_p, []),

@@ -13,6 +13,7 @@ using namespace p8;
 
 namespace p8 {
 unsigned int read_and_clear_device_error();
+unsigned int read_and_clear_cache_error();
 }
 
 namespace {
@@ -366,7 +367,7 @@ p8_status p8_chain_trace(p8_chain *c, uint64_t *dev_buf, size_t words) {
 }
 
 /* 1 if a kernel since the last call gave up on a bounded wait (results of that launch are invalid). Synchronous. */
-int p8_device_error(void) { return (int)read_and_clear_device_error(); }
+int p8_device_error(void) { return (int)(read_and_clear_device_error() | read_and_clear_cache_error()); }
 
 const char *p8_build_info(void) { return "pingala8_b200 sm_100a (tcgen05/TMA), C ABI v1"; }
 

@@ -1,0 +1,590 @@
+// p8_cache.cu -- key/value cache operators: append (norm, rotation, write), eviction, tree acceptance, and the C ABI
+// entry points of all five (the attention and mass kernels are in p8_tree_attn.cuh).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <mutex>
+
+#include "p8_device.cuh"
+#include "p8_internal.h"
+
+namespace p8 {
+
+// The operators' own error word (bits 64 and 128 of p8_device_error).
+__device__ unsigned int g_cache_error = 0;
+constexpr unsigned int kErrRange = 64u;
+
+unsigned int read_and_clear_cache_error() {
+    unsigned int v = 0, z = 0;
+    cudaMemcpyFromSymbol(&v, g_cache_error, sizeof(v));
+    cudaMemcpyToSymbol(g_cache_error, &z, sizeof(z));
+    return v;
+}
+
+namespace {
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Length of sequence b and its tokens in this call; false where they are out of range.
+__device__ __forceinline__ bool seq_range(const int *lens, const int *counts, int b, int tokens, int64_t slots, int &len, int &n) {
+    len = lens[b];
+    n = counts ? counts[b] : tokens;
+    return len >= 0 && n >= 0 && n <= tokens && (int64_t)len + n <= slots;
+}
+
+// four consecutive values, rounded to the cache's type
+__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
+    union { T t[4]; uint2 u; } r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.t[i] = from_f<T>(v[i]);
+    *reinterpret_cast<uint2 *>(p) = r.u;
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// append: y = rotate(norm(x)) per head of a token. A group of D / 8 lanes holds one head's row, lane l the values
+// 4l..4l+3 of both halves, so a rotation pair is in one lane, the sum of squares is a butterfly over the group, and
+// every access is 8 or 16 bytes wide. Bound by memory on a prompt, by its one launch on a token.
+struct AppendArgs {
+    const float *x[3];          // q, k, v
+    long long xs[3][3];
+    void *y[3];                 // q_out, cache k, cache v
+    long long ys[3][3];         // sequence, token (slot for the cache), head
+    const int *lens, *counts, *pos;
+    const float *cos, *sin, *qn, *kn;
+    long long positions, slots;
+    int tokens, heads, kvh, batch;
+    float eps;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a) {
+    constexpr int L = D / 8, RPB = 256 / L;
+    const int rows = a.heads + 2 * a.kvh;
+    const long long id = (long long)blockIdx.x * RPB + threadIdx.x / L;
+    const int l = threadIdx.x % L;
+    const long long tok = id / rows;
+    if (tok >= (long long)a.batch * a.tokens) return;  // a whole group of lanes leaves
+    const int r = (int)(id - tok * rows), b = (int)(tok / a.tokens), t = (int)(tok - (long long)b * a.tokens);
+    int len, n;
+    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
+        if (t == 0 && r == 0 && l == 0) atomicOr(&g_cache_error, kErrRange);
+        return;
+    }
+    if (t >= n) return;
+    const int p = a.pos[tok];
+    if (p < 0 || p >= a.positions) {
+        if (r == 0 && l == 0) atomicOr(&g_cache_error, kErrRange);
+        return;
+    }
+    const int which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2;
+    const int h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
+    const float *x = a.x[which] + b * a.xs[which][0] + t * a.xs[which][1] + h * a.xs[which][2] + 4 * l;
+    float u[4], w[4];
+    *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(x);
+    *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(x + D / 2);
+    if (which < 2) {
+        float c[4], s[4];
+        *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(a.cos + (long long)p * (D / 2) + 4 * l);
+        *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(a.sin + (long long)p * (D / 2) + 4 * l);
+        const float *g = which == 0 ? a.qn : a.kn;
+        if (g) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ss += u[i] * u[i] + w[i] * w[i];
+            const unsigned int group = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << (threadIdx.x % 32 / L * L);
+#pragma unroll
+            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(group, ss, m);
+            const float rs = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u[i] = u[i] * rs * g[4 * l + i];
+                w[i] = w[i] * rs * g[4 * l + i + D / 2];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x0 = u[i], x1 = w[i];
+            u[i] = x0 * c[i] - x1 * s[i];
+            w[i] = x1 * c[i] + x0 * s[i];
+        }
+    }
+    T *y = static_cast<T *>(a.y[which]) + b * a.ys[which][0] + (which == 0 ? t : len + t) * a.ys[which][1] + h * a.ys[which][2] + 4 * l;
+    store4(y, u);
+    store4(y + D / 2, w);
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// eviction, step 1: the kept slots of one (layer, sequence, head). Radix select on an order-preserving 32-bit key in
+// three digits of 11, 11 and 10 bits finds the smallest kept key; then every warp walks a contiguous part of the
+// slots, so that the kept ones come out in order and, among equal keys, the lowest slots win.
+struct EvictArgs {
+    const float *mass;
+    float *mass_out;
+    long long ms[3], mos[3];
+    const int *lens;
+    int *new_lens, *kept;
+    const char *src[2];
+    char *dst[2];
+    long long ss[2][4], ds[2][4];  // bytes: layer, sequence, head, slot
+    long long slots;
+    int batch, heads, budget, sinks, recent, row_bytes;
+};
+
+__device__ __forceinline__ uint32_t mass_key(float m) {  // larger mass, larger key; NaN as -infinity, -0 as +0
+    if (isnan(m)) m = -INFINITY;
+    m += 0.0f;
+    const uint32_t u = __float_as_uint(m);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
+    __shared__ int hist[2048];
+    __shared__ int wsum[32], weq[32];
+    __shared__ int s_digit, s_above;
+    const int row = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    const int len = a.lens[b];
+    if (len < 0 || len > a.slots) {
+        if (tid == 0) atomicOr(&g_cache_error, kErrRange);
+        return;
+    }
+    if (layer == 0 && h == 0 && tid == 0) a.new_lens[b] = min(len, a.budget);
+    int *kept = a.kept + (long long)row * a.budget;
+    if (len <= a.budget) {
+        for (int i = tid; i < a.budget; i += 1024) kept[i] = i < len ? i : -1;
+        return;
+    }
+    const float *m = a.mass + layer * a.ms[0] + b * a.ms[1] + h * a.ms[2];
+    const int need = a.budget - a.sinks - a.recent, lo = a.sinks, hi = len - a.recent, n = hi - lo;
+    for (int i = tid; i < a.sinks; i += 1024) kept[i] = i;
+    for (int i = tid; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
+    if (need == 0) return;
+    uint32_t prefix = 0, fixed = 0;  // the threshold key's known bits, and which they are
+    int left = need;                 // kept among the keys that share them
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+        hist[tid] = 0;
+        hist[tid + 1024] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += 1024) {
+            const uint32_t k = mass_key(m[lo + i]);
+            if ((k & fixed) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+        }
+        __syncthreads();
+        // thread t holds bins 2t' and 2t'+1 counted from the top; a scan over them finds the digit where `left` falls
+        const int hi_bin = bins - 1 - 2 * tid, lo_bin = hi_bin - 1;
+        const int c0 = hi_bin > 0 ? hist[hi_bin] : 0, c1 = hi_bin > 0 ? hist[lo_bin] : 0;
+        int sum = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) wsum[warp] = sum;
+        __syncthreads();
+        int base = 0;
+        for (int w = 0; w < warp; ++w) base += wsum[w];
+        const int before = base + sum - c0 - c1;
+        if (before < left && left <= before + c0) { s_digit = hi_bin; s_above = before; }
+        if (before + c0 < left && left <= before + c0 + c1) { s_digit = lo_bin; s_above = before + c0; }
+        __syncthreads();
+        prefix |= (uint32_t)s_digit << shift;
+        fixed |= (uint32_t)(bins - 1) << shift;
+        left -= s_above;
+        __syncthreads();
+    }
+    // keys above `prefix` are kept, and the first `left` of those equal to it
+    const int seg = ((n + 31) / 32 + 31) / 32 * 32, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
+    int gt = 0, eq = 0;
+    for (int i = s0 + lane; i < s1; i += 32) {
+        const uint32_t k = mass_key(m[lo + i]);
+        gt += k > prefix;
+        eq += k == prefix;
+    }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) { wsum[warp] = gt; weq[warp] = eq; }
+    __syncthreads();
+    int gt0 = 0, eq0 = 0;
+    for (int w = 0; w < warp; ++w) { gt0 += wsum[w]; eq0 += weq[w]; }
+    int at = a.sinks + gt0 + min(eq0, left);
+    for (int i0 = s0; i0 < s1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < s1 ? mass_key(m[lo + i]) : 0u;
+        const bool e = i < s1 && k == prefix;
+        const unsigned int em = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1u;
+        const bool keep = i < s1 && (k > prefix || (e && eq0 + __popc(em & below) < left));
+        const unsigned int km = __ballot_sync(0xffffffffu, keep);
+        if (keep) kept[at + __popc(km & below)] = lo + i;
+        at += __popc(km);
+        eq0 += __popc(em);
+    }
+}
+
+// step 2, into other buffers: every row moves on its own, 16 bytes a thread.
+__global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
+    const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    const int len = a.lens[b];
+    if (len < 0 || len > a.slots) return;
+    const int keep = min(len, a.budget), per = a.row_bytes / 16, rows = 256 / per;
+    const int *kept = a.kept + (long long)row * a.budget;
+    const char *s0 = a.src[0] + layer * a.ss[0][0] + b * a.ss[0][1] + h * a.ss[0][2], *s1 = a.src[1] + layer * a.ss[1][0] + b * a.ss[1][1] + h * a.ss[1][2];
+    char *d0 = a.dst[0] + layer * a.ds[0][0] + b * a.ds[0][1] + h * a.ds[0][2], *d1 = a.dst[1] + layer * a.ds[1][0] + b * a.ds[1][1] + h * a.ds[1][2];
+    const int unit = 16 * (threadIdx.x % per);
+    const int first = blockIdx.x * rows * 4 + threadIdx.x / per;
+    uint4 x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int i = first + j * rows;
+        if (i < keep) {
+            const long long s = kept[i];
+            x[j] = *reinterpret_cast<const uint4 *>(s0 + s * a.ss[0][3] + unit);
+            y[j] = *reinterpret_cast<const uint4 *>(s1 + s * a.ss[1][3] + unit);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int i = first + j * rows;
+        if (i < keep) {
+            *reinterpret_cast<uint4 *>(d0 + i * a.ds[0][3] + unit) = x[j];
+            *reinterpret_cast<uint4 *>(d1 + i * a.ds[1][3] + unit) = y[j];
+        }
+    }
+    for (int i = blockIdx.x * rows * 4 + threadIdx.x; i < min(keep, (int)(blockIdx.x + 1) * rows * 4); i += 256)
+        a.mass_out[layer * a.mos[0] + b * a.mos[1] + h * a.mos[2] + i] = a.mass[layer * a.ms[0] + b * a.ms[1] + h * a.ms[2] + kept[i]];
+}
+
+// step 2 in place: kept[i] >= i, so a block that goes up through a range of the row's bytes (64 of them: its columns
+// belong to no other block), reads a chunk of sources before it writes their destinations, and reads the next chunk
+// (sources at or behind every destination written so far) meanwhile, loses nothing. blockIdx.z 0 / 1: keys / values,
+// 2: the masses.
+template <typename U>
+__device__ __forceinline__ void evict_slide(const char *base, long long stride, int per, int keep, const int *kept) {
+    constexpr int kRows = 4;
+    const int lanes = 256 / per, unit = threadIdx.x % per, r0 = threadIdx.x / per;
+    char *p = const_cast<char *>(base) + (long long)unit * sizeof(U);
+    U cur[kRows];
+    int src[kRows], nxt[kRows];
+    U ahead[kRows];
+    const int step = lanes * kRows;
+    auto fetch = [&](int i0, U (&v)[kRows], int (&s)[kRows]) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const int i = i0 + j * lanes + r0;
+            s[j] = i < keep ? kept[i] : -1;
+            if (s[j] > i) v[j] = *reinterpret_cast<const U *>(p + s[j] * stride);
+        }
+    };
+    fetch(0, cur, src);
+    for (int i0 = 0; i0 < keep; i0 += step) {
+        fetch(i0 + step, ahead, nxt);
+        __syncthreads();  // every thread has read this chunk and the next
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const int i = i0 + j * lanes + r0;
+            if (src[j] > i) *reinterpret_cast<U *>(p + i * stride) = cur[j];
+            cur[j] = ahead[j];
+            src[j] = nxt[j];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
+    const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    const int len = a.lens[b];
+    if (len <= a.budget || len > a.slots) return;
+    const int *kept = a.kept + (long long)row * a.budget;
+    const int z = blockIdx.z;
+    if (z == 2) {
+        if (blockIdx.x == 0)
+            evict_slide<float>(reinterpret_cast<const char *>(a.mass + layer * a.ms[0] + b * a.ms[1] + h * a.ms[2]), 4, 1, a.budget, kept);
+        return;
+    }
+    evict_slide<uint4>(a.src[z] + layer * a.ss[z][0] + b * a.ss[z][1] + h * a.ss[z][2] + 64 * blockIdx.x, a.ss[z][3], 4, a.budget, kept);
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// acceptance: one block per (layer, sequence, keys or values). Each finds the path on its own (the first warp, two
+// nodes a lane, one ballot per step: cheaper than a launch between the walk and the moves), then moves the rows of all
+// heads in chunks, reading a chunk before writing it: path[i] >= i and the chunks go up, so no source is lost.
+struct AcceptArgs {
+    const long long *tokens, *target;
+    const int *parents, *lens, *counts;
+    int *path, *accepted, *new_lens;
+    long long *next;
+    char *kv[2];
+    long long st[2][4];  // bytes
+    long long slots;
+    int T, batch, heads, row_bytes;
+};
+
+__global__ void __launch_bounds__(256) k_tree_accept(const AcceptArgs a) {
+    __shared__ int path[P8_TREE_MAX];
+    __shared__ int s_n;
+    const int b = blockIdx.x % a.batch, z = blockIdx.x / a.batch % 2, layer = blockIdx.x / a.batch / 2;
+    const int tid = threadIdx.x;
+    const bool report = layer == 0 && z == 0;
+    int len, n;
+    const bool ok = seq_range(a.lens, a.counts, b, a.T, a.slots, len, n);
+    if (tid < 32) {
+        const long long at = (long long)b * a.T;
+        int par[2];
+        bool fits[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int c = tid + 32 * k;
+            par[k] = -1;
+            fits[k] = false;
+            if (ok && c > 0 && c < n) {
+                par[k] = a.parents[at + c];
+                fits[k] = par[k] >= 0 && par[k] < c && a.tokens[at + c] == a.target[at + par[k]];
+            }
+        }
+        int cur = 0, cnt = ok && n > 0 ? 1 : 0;
+        if (tid == 0) path[0] = 0;
+        while (cnt) {
+            const unsigned int m0 = __ballot_sync(0xffffffffu, fits[0] && par[0] == cur);
+            const unsigned int m1 = __ballot_sync(0xffffffffu, fits[1] && par[1] == cur);
+            if (!(m0 | m1)) break;
+            cur = m0 ? __ffs(m0) - 1 : 31 + __ffs(m1);  // parents come first, so cur grows and the walk ends
+            if (tid == 0) path[cnt] = cur;
+            ++cnt;
+        }
+        __syncwarp();
+        if (tid == 0) s_n = cnt;
+        if (report) {
+            for (int t = tid; t < a.T; t += 32) a.path[at + t] = t < cnt ? path[t] : -1;
+            if (tid == 0) {
+                a.accepted[b] = cnt;
+                a.new_lens[b] = len + cnt;
+                a.next[b] = cnt ? a.target[at + cur] : -1;
+                if (!ok) atomicOr(&g_cache_error, kErrRange);
+            }
+        }
+    }
+    __syncthreads();
+    const int cnt = s_n, per = a.row_bytes / 16, items = (cnt - 1) * a.heads * per;
+    char *base = a.kv[z] + layer * a.st[z][0] + b * a.st[z][1] + len * a.st[z][3];
+    for (int i0 = 0; i0 < items; i0 += 1024) {
+        uint4 v[4];
+        char *to[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * 256 + tid;
+            to[j] = nullptr;
+            if (i < items) {
+                const int unit = i % per, h = i / per % a.heads, r = i / per / a.heads + 1;
+                char *p = base + h * a.st[z][2] + 16 * unit;
+                if (path[r] != r) {
+                    v[j] = *reinterpret_cast<const uint4 *>(p + path[r] * a.st[z][3]);
+                    to[j] = p + r * a.st[z][3];
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (to[j]) *reinterpret_cast<uint4 *>(to[j]) = v[j];
+    }
+}
+
+#include "p8_tree_attn.cuh"
+
+// ----------------------------------------------------------------------------------------------------------------
+// host side: argument checks (nothing below them touches the device before they pass) and launches
+int elem_size(int64_t type) { return type == P8_KV_F32 ? 4 : 2; }
+bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+// strides (elements) of the dimensions that are used, as multiples of 16 bytes
+bool strides_ok(const int64_t *st, const int64_t *dims, int n, int es) {
+    for (int i = 0; i < n; ++i)
+        if (dims[i] > 1 && (st[i] * es) % 16) return false;
+    return true;
+}
+
+bool kv_ok(const p8_kv *c, bool values = true) {
+    if (!c || !c->k || (values && !c->v) || !al16(c->k) || !al16(c->v)) return false;
+    if (c->type != P8_KV_F32 && c->type != P8_KV_F16 && c->type != P8_KV_BF16) return false;
+    if (c->width != 64 && c->width != 128) return false;
+    if (c->layers < 1 || c->batch < 1 || c->batch > P8_BATCH_MAX || c->heads < 1 || c->slots < 1 || c->slots > INT32_MAX - 4096) return false;
+    if (c->heads > 65535 || c->layers > 65535 || c->layers * c->batch * c->heads > (int64_t(1) << 30)) return false;
+    const int64_t dims[4] = {c->layers, c->batch, c->heads, c->slots};
+    const int es = elem_size(c->type);
+    return strides_ok(c->k_stride, dims, 4, es) && (!values || strides_ok(c->v_stride, dims, 4, es));
+}
+bool heads_ok(const p8_kv *c, int64_t heads) { return heads >= c->heads && heads % c->heads == 0 && heads <= 65535; }
+
+p8_status launched() { return cudaGetLastError() == cudaSuccess ? P8_OK : P8_ERR_CUDA; }
+
+template <typename T>
+void run_append(const p8_kv *c, const AppendArgs &a, cudaStream_t st) {
+    const long long rows = (long long)a.batch * a.tokens * (a.heads + 2 * a.kvh), per = 256 / (c->width / 8);
+    const unsigned int grid = (unsigned int)((rows + per - 1) / per);
+    if (c->width == 128) k_kv_append<T, 128><<<grid, 256, 0, st>>>(a);
+    else k_kv_append<T, 64><<<grid, 256, 0, st>>>(a);
+}
+
+// whether two strided views (three outer dimensions, `last` elements inside) can share bytes
+void span(const void *base, const int64_t *st, const int64_t *dims, int n, int es, int64_t last, uintptr_t &lo, uintptr_t &hi) {
+    int64_t neg = 0, pos = last;
+    for (int i = 0; i < n; ++i) (st[i] < 0 ? neg : pos) += st[i] * (dims[i] - 1);
+    lo = (uintptr_t)base + (uintptr_t)(neg * es);
+    hi = (uintptr_t)base + (uintptr_t)(pos * es);
+}
+bool overlap(const void *x, const int64_t *xs, const int64_t *xd, int xe, int64_t xl, const void *y, const int64_t *ys, const int64_t *yd, int ye,
+             int64_t yl, int n = 3) {
+    uintptr_t x0, x1, y0, y1;
+    span(x, xs, xd, n, xe, xl, x0, x1);
+    span(y, ys, yd, n, ye, yl, y0, y1);
+    return x0 < y1 && y0 < x1;
+}
+}  // namespace
+}  // namespace p8
+
+using namespace p8;
+
+extern "C" {
+
+p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream) {
+    if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
+    if (!a->q || !a->k || !a->v || !a->q_out || !a->lens || !a->pos || !a->cos || !a->sin || a->tokens < 0 || a->positions < 1) return P8_ERR_ARG;
+    if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->q_out) || !al16(a->cos) || !al16(a->sin) || !(a->eps >= 0.0)) return P8_ERR_ARG;
+    if (a->tokens > c->slots || c->batch * a->tokens * (a->heads + 2 * c->heads) > (int64_t(1) << 34)) return P8_ERR_ARG;
+    const int es = elem_size(c->type);
+    const int64_t dq[3] = {c->batch, a->tokens, a->heads}, dk[3] = {c->batch, a->tokens, c->heads};
+    if (!strides_ok(a->q_stride, dq, 3, 4) || !strides_ok(a->k_stride, dk, 3, 4) || !strides_ok(a->v_stride, dk, 3, 4) ||
+        !strides_ok(a->q_out_stride, dq, 3, es))
+        return P8_ERR_ARG;
+    if (a->tokens == 0) return P8_OK;
+    AppendArgs k;
+    const float *x[3] = {a->q, a->k, a->v};
+    const int64_t *xs[3] = {a->q_stride, a->k_stride, a->v_stride};
+    for (int i = 0; i < 3; ++i) {
+        k.x[i] = x[i];
+        for (int j = 0; j < 3; ++j) k.xs[i][j] = xs[i][j];
+    }
+    k.y[0] = a->q_out; k.y[1] = c->k; k.y[2] = c->v;
+    for (int j = 0; j < 3; ++j) k.ys[0][j] = a->q_out_stride[j];
+    const int64_t *cs[2] = {c->k_stride, c->v_stride};
+    for (int i = 0; i < 2; ++i) { k.ys[1 + i][0] = cs[i][1]; k.ys[1 + i][1] = cs[i][3]; k.ys[1 + i][2] = cs[i][2]; }
+    k.lens = a->lens; k.counts = a->counts; k.pos = a->pos;
+    k.cos = a->cos; k.sin = a->sin; k.qn = a->q_norm; k.kn = a->k_norm;
+    k.positions = a->positions; k.slots = c->slots;
+    k.tokens = (int)a->tokens; k.heads = (int)a->heads; k.kvh = (int)c->heads; k.batch = (int)c->batch;
+    k.eps = (float)a->eps;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (c->type == P8_KV_F32) run_append<float>(c, k, st);
+    else if (c->type == P8_KV_F16) run_append<__half>(c, k, st);
+    else run_append<__nv_bfloat16>(c, k, st);
+    return launched();
+}
+
+size_t p8_tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {
+    if (!kv_ok(c) || c->layers != 1 || tokens < 1 || tokens > P8_TREE_MAX || !heads_ok(c, heads)) return 0;
+    return tree_attn_workspace(c, tokens, heads);
+}
+
+p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
+    if (!a->q || !a->out || !a->lens || a->tokens < 1 || a->tokens > P8_TREE_MAX || !al16(a->q) || !al16(a->out)) return P8_ERR_ARG;
+    if (!isfinite(a->scale) || (a->mask && a->mask_stride != 0 && a->mask_stride != a->tokens)) return P8_ERR_ARG;
+    const int es = elem_size(c->type);
+    const int64_t dq[3] = {c->batch, a->tokens, a->heads};
+    if (!strides_ok(a->q_stride, dq, 3, es) || !strides_ok(a->out_stride, dq, 3, es)) return P8_ERR_ARG;
+    const int64_t dkv[3] = {c->batch, c->heads, c->slots};
+    if (overlap(a->out, a->out_stride, dq, es, c->width, a->q, a->q_stride, dq, es, c->width) ||
+        overlap(a->out, a->out_stride, dq, es, c->width, c->k, c->k_stride + 1, dkv, es, c->width) ||
+        overlap(a->out, a->out_stride, dq, es, c->width, c->v, c->v_stride + 1, dkv, es, c->width))
+        return P8_ERR_ARG;
+    const size_t need = tree_attn_workspace(c, a->tokens, a->heads);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return P8_ERR_WORKSPACE;
+    return launch_tree_attn(c, a, workspace, (cudaStream_t)stream);
+}
+
+p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream) {
+    if (!kv_ok(c, false) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
+    if (!a->q || !a->lse || !a->lens || !a->mass || !a->out || a->tokens < 1 || a->tokens > P8_TREE_MAX || !al16(a->q)) return P8_ERR_ARG;
+    if (!isfinite(a->scale)) return P8_ERR_ARG;
+    const int64_t dq[3] = {c->batch, a->tokens, a->heads};
+    if (!strides_ok(a->q_stride, dq, 3, elem_size(c->type))) return P8_ERR_ARG;
+    const int64_t dm[3] = {c->batch, c->heads, c->slots}, m3[3] = {a->mass_stride[0], a->mass_stride[1], 1}, o3[3] = {a->out_stride[0], a->out_stride[1], 1};
+    const bool same = a->mass == a->out && m3[0] == o3[0] && m3[1] == o3[1];
+    if (!same && overlap(a->mass, m3, dm, 4, 1, a->out, o3, dm, 4, 1)) return P8_ERR_ARG;
+    return launch_attn_mass(c, a, (cudaStream_t)stream);
+}
+
+p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a, void *stream) {
+    if (!kv_ok(s) || !kv_ok(d) || !a || !a->mass || !a->mass_out || !a->lens || !a->new_lens || !a->kept || a->new_lens == a->lens) return P8_ERR_ARG;
+    if (s->type != d->type || s->width != d->width || s->layers != d->layers || s->batch != d->batch || s->heads != d->heads) return P8_ERR_ARG;
+    if (a->budget < 1 || a->sinks < 0 || a->recent < 0 || a->sinks > a->budget || a->recent > a->budget - a->sinks || a->budget > d->slots ||
+        a->budget > s->slots)
+        return P8_ERR_ARG;
+    const int es = elem_size(s->type);
+    const int64_t dims[4] = {s->layers, s->batch, s->heads, s->slots}, ddims[4] = {s->layers, s->batch, s->heads, a->budget};
+    // in place: all three buffers and their strides the same; else no overlap at all
+    bool same = s->k == d->k && s->v == d->v && a->mass == a->mass_out;
+    for (int i = 0; i < 4; ++i) same = same && s->k_stride[i] == d->k_stride[i] && s->v_stride[i] == d->v_stride[i];
+    for (int i = 0; i < 3; ++i) same = same && a->mass_stride[i] == a->mass_out_stride[i];
+    if (!same) {
+        const int64_t m4[4] = {a->mass_stride[0], a->mass_stride[1], a->mass_stride[2], 1}, o4[4] = {a->mass_out_stride[0], a->mass_out_stride[1], a->mass_out_stride[2], 1};
+        const void *from[3] = {s->k, s->v, a->mass}, *to[3] = {d->k, d->v, a->mass_out};
+        const int64_t *fs[3] = {s->k_stride, s->v_stride, m4}, *ts[3] = {d->k_stride, d->v_stride, o4};
+        for (int i = 0; i < 3; ++i)
+            for (int j = 0; j < 3; ++j)
+                if (overlap(from[i], fs[i], dims, i < 2 ? es : 4, i < 2 ? s->width : 1, to[j], ts[j], ddims, j < 2 ? es : 4, j < 2 ? s->width : 1, 4))
+                    return P8_ERR_ARG;
+    }
+    EvictArgs k;
+    k.mass = a->mass; k.mass_out = a->mass_out;
+    for (int i = 0; i < 3; ++i) { k.ms[i] = a->mass_stride[i]; k.mos[i] = a->mass_out_stride[i]; }
+    k.lens = a->lens; k.new_lens = a->new_lens; k.kept = a->kept;
+    k.src[0] = (const char *)s->k; k.src[1] = (const char *)s->v; k.dst[0] = (char *)d->k; k.dst[1] = (char *)d->v;
+    for (int i = 0; i < 4; ++i) {
+        k.ss[0][i] = s->k_stride[i] * es; k.ss[1][i] = s->v_stride[i] * es;
+        k.ds[0][i] = d->k_stride[i] * es; k.ds[1][i] = d->v_stride[i] * es;
+    }
+    k.slots = s->slots; k.batch = (int)s->batch; k.heads = (int)s->heads;
+    k.budget = (int)a->budget; k.sinks = (int)a->sinks; k.recent = (int)a->recent; k.row_bytes = (int)s->width * es;
+    const int64_t rows = s->layers * s->batch * s->heads;
+    if (rows > 65535) return P8_ERR_UNSUPPORTED;
+    cudaStream_t st = (cudaStream_t)stream;
+    k_evict_select<<<(unsigned int)rows, 1024, 0, st>>>(k);
+    if (same) {
+        k_evict_slide<<<dim3((unsigned int)(k.row_bytes / 64), (unsigned int)rows, 3), 256, 0, st>>>(k);
+    } else {
+        const int chunk = 4 * (256 / (k.row_bytes / 16));
+        k_evict_copy<<<dim3((unsigned int)((a->budget + chunk - 1) / chunk), (unsigned int)rows), 256, 0, st>>>(k);
+    }
+    return launched();
+}
+
+p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream) {
+    if (!kv_ok(c) || !a || !a->tokens || !a->target || !a->parents || !a->lens || !a->path || !a->accepted || !a->new_lens || !a->next_token)
+        return P8_ERR_ARG;
+    if (a->ntokens < 1 || a->ntokens > P8_TREE_MAX || a->new_lens == a->lens) return P8_ERR_ARG;
+    const int es = elem_size(c->type);
+    AcceptArgs k;
+    k.tokens = (const long long *)a->tokens; k.target = (const long long *)a->target; k.next = (long long *)a->next_token;
+    k.parents = a->parents; k.lens = a->lens; k.counts = a->counts;
+    k.path = a->path; k.accepted = a->accepted; k.new_lens = a->new_lens;
+    k.kv[0] = (char *)c->k; k.kv[1] = (char *)c->v;
+    for (int i = 0; i < 4; ++i) { k.st[0][i] = c->k_stride[i] * es; k.st[1][i] = c->v_stride[i] * es; }
+    k.slots = c->slots; k.T = (int)a->ntokens; k.batch = (int)c->batch; k.heads = (int)c->heads; k.row_bytes = (int)c->width * es;
+    k_tree_accept<<<(unsigned int)(c->layers * c->batch * 2), 256, 0, (cudaStream_t)stream>>>(k);
+    return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,621 @@
+"""Key/value cache operators against their definitions in 64 bits.
+
+Tolerances. u = eps / 2 is the error of one rounding to the tensors' type, e = 2^-23 that of one fp32 operation (a full
+step: tensor cores may truncate). A score is a dot product of D terms: off by at most ds = (D + 16) e A, A = scale sum
+|q||k| (16: the scale, the split of 32-bit operands into two pieces and the exponent's argument, with room); its
+exponential is then off by a factor 1 +- 2 ds (its own score's and the running maximum's or lse's), 4 e for the exponential
+itself. A sum of L weighted values of independent errors grows as sqrt(L): 8 sqrt(L) e, with a constant 64 for the sums
+inside a tile and the joining of parts. So
+    |o - o*| <= (u_p + 2 ds + (68 + 8 sqrt(L)) e) sum p |v| + u |o*|     u_p = u: 16-bit types round p before p v
+    |lse - lse*| <= ds + (68 + 8 sqrt(L)) e + e |lse*|
+and likewise for the masses, whose terms are exponentials. Whole numbers and moved rows have to be equal.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA GPU", allow_module_level=True)
+
+import pingala8_llm_b200 as p8  # noqa: E402
+from pingala8_llm_b200 import cache  # noqa: E402
+
+E = 2.0 ** -23
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+INF, NAN = math.inf, math.nan
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def u_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def visible(mask, lens, counts, T, cap):
+    """[B, T, cap] from bits [T] or [B, T] (None: a chain)"""
+    B = len(lens)
+    see = torch.zeros(B, T, cap, dtype=torch.bool, device="cuda")
+    for b in range(B):
+        see[b, :, : lens[b]] = True
+        for t in range(T):
+            bits = (1 << (t + 1)) - 1 if mask is None else int(mask[b, t] if mask.dim() == 2 else mask[t])
+            for j in range(min(counts[b], T)):
+                see[b, t, lens[b] + j] = (bits >> j) & 1
+    return see
+
+
+def attend(q, k, v, see, scale):
+    """(o, lse, bound of o, bound of lse) in 64 bits; what is not seen has no part in it"""
+    B, T, H, D = q.shape
+    G = H // k.shape[1]
+    o, lse = torch.zeros(B, T, H, D, dtype=torch.float64, device="cuda"), torch.full((B, T, H), -INF, dtype=torch.float64, device="cuda")
+    to, tl = torch.zeros_like(o), torch.zeros_like(lse)
+    u = u_of(q.dtype)
+    for b in range(B):
+        live = see[b].any(0)  # slots that some token sees
+        s0 = see[b][:, live]
+        for h in range(H):
+            kk, vv, qq = k[b, h // G][live].double(), v[b, h // G][live].double(), q[b, :, h].double()
+            if not kk.shape[0]:
+                continue
+            for t in range(T):
+                m = s0[t]
+                if not m.any():
+                    continue
+                K, V = kk[m], vv[m]
+                s = (K @ qq[t]) * scale
+                lse[b, t, h] = torch.logsumexp(s, 0)
+                p = torch.softmax(s, 0)
+                o[b, t, h] = p @ V
+                ds = (D + 16) * E * float((K.abs() @ qq[t].abs()).max()) * abs(scale)
+                acc = (68 + 8 * math.sqrt(K.shape[0])) * E
+                to[b, t, h] = ((u if q.dtype != torch.float32 else 0.0) + 2 * ds + acc) * (p @ V.abs()) + u * o[b, t, h].abs()
+                tl[b, t, h] = ds + acc + E * lse[b, t, h].abs()
+    return o, lse, to, tl
+
+
+def close(got, want, tol, what=""):
+    got = got.double()
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]), what
+    assert not torch.isnan(got).any(), what
+    d = (got - want)[~inf].abs() - tol[~inf]
+    assert d.numel() == 0 or float(d.max()) <= 0, f"{what}: {float(d.max())} over the bound"
+
+
+def tree_masks(g, B, T):
+    par = torch.tensor([[-1] + [int(torch.randint(max(0, t - 9), t, (1,), device="cuda", generator=g)) for t in range(1, T)] for _ in range(B)])
+    return cache.tree_plan(par)[0].cuda()
+
+
+def ended(bits=0):
+    torch.cuda.synchronize()
+    assert p8.device_error() == bits
+
+
+# (types, B, T, H, Hkv, D, lens, mask)
+SHAPES = [
+    (1, 1, 1, 1, 64, [0], "chain"),
+    (1, 1, 8, 2, 128, [1], "chain"),
+    (1, 1, 32, 8, 128, [127], "chain"),
+    (2, 2, 8, 8, 64, [126, 128], "chain"),
+    (3, 5, 14, 2, 128, [0, 63, 300], "tree"),
+    (1, 12, 32, 8, 128, [517], "tree"),
+    (2, 33, 16, 4, 64, [255, 1000], "tree"),
+    (1, 64, 32, 8, 128, [1234], "tree"),
+    (1, 64, 24, 3, 64, [64], "shared"),
+    (2, 64, 5, 1, 128, [3, 2000], "tree"),
+    (5, 3, 4, 4, 128, [0, 1, 127, 129, 700], "shared"),
+]
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("B,T,H,hk,D,lens,kind", SHAPES)
+def test_tree_attention(dt, B, T, H, hk, D, lens, kind):
+    g, dtype = gen(B * 1000 + T), TYPES[dt]
+    cap = max(lens) + T + 3
+    k, v = randn(g, B, hk, cap, D, dtype=dtype), randn(g, B, hk, cap, D, dtype=dtype)
+    q = randn(g, B, T, H, D, dtype=dtype, scale=1.5)
+    mask = None if kind == "chain" else tree_masks(g, B, T) if kind == "tree" else tree_masks(g, 1, T)[0].contiguous()
+    out, lse = cache.tree_attention(q, k, v, ints(*lens), mask=mask)
+    ended()
+    o, l, to, tl = attend(q, k, v, visible(mask, lens, [T] * B, T, cap), D ** -0.5)
+    close(out, o, to, "out")
+    close(lse, l, tl, "lse")
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("T,H,hk,D,length", [(1, 8, 2, 128, 40001), (40, 8, 2, 128, 9001), (7, 6, 1, 64, 20000)])
+def test_tree_attention_long(dt, T, H, hk, D, length):
+    g, dtype = gen(length), TYPES[dt]
+    cap = length + T
+    k, v = randn(g, 1, hk, cap, D, dtype=dtype), randn(g, 1, hk, cap, D, dtype=dtype)
+    v += 0.5  # a mean that the average keeps
+    q = randn(g, 1, T, H, D, dtype=dtype, scale=1.5)
+    out, lse = cache.tree_attention(q, k, v, ints(length))
+    ended()
+    o, l, to, tl = attend(q, k, v, visible(None, [length], [T], T, cap), D ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("scale,shift", [(0.0, 0.0), (-0.3, 0.0), (4.0, 0.0), (0.09, 30.0)])
+def test_scales_and_far_scores(dt, scale, shift):
+    """no scale, a negative one, scores up to hundreds (one key takes all), and a maximum that grows tile by tile"""
+    g, dtype = gen(11), TYPES[dt]
+    B, T, H, hk, D, n = 1, 3, 4, 2, 64, 600
+    k, v = randn(g, B, hk, n + T, D, dtype=dtype), randn(g, B, hk, n + T, D, dtype=dtype)
+    if shift:
+        k = (k.float() + torch.linspace(-1, 1, n + T, device="cuda")[:, None]).to(dtype)
+    q = (randn(g, B, T, H, D) + (shift / 10)).to(dtype)
+    out, lse = cache.tree_attention(q, k, v, ints(n), scale=scale)
+    ended()
+    o, l, to, tl = attend(q, k, v, visible(None, [n], [T], T, n + T), scale)
+    close(out, o, to)
+    close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_is_not_seen_does_not_reach_a_token(dt, D):
+    """infinities and NaN behind the sequence, and in drafted tokens that others do not see"""
+    g, dtype = gen(5), TYPES[dt]
+    B, T, H, hk, n = 2, 6, 8, 2, [130, 61]
+    cap = 260
+    k, v = randn(g, B, hk, cap, D, dtype=dtype), randn(g, B, hk, cap, D, dtype=dtype)
+    q = randn(g, B, T, H, D, dtype=dtype)
+    mask = torch.tensor([1, 3, 5, 1 | 8, 1 | 2 | 16, 0], device="cuda")  # nobody sees token 5; token 5 sees the sequence alone
+    k2, v2 = k.clone(), v.clone()
+    for b in range(B):
+        for x, bad in ((k2, (NAN, INF, -INF)), (v2, (INF, NAN, -INF))):
+            x[b, :, n[b] + T:] = bad[0]
+            x[b, :, n[b] + 5] = bad[1]
+            x[b, 0, n[b] + 5, 3] = bad[2]
+    want = cache.tree_attention(q, k, v, ints(*n), mask=mask)
+    got = cache.tree_attention(q, k2, v2, ints(*n), mask=mask)
+    ended()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # token 2's own value is infinite: its row says so, the rows that do not see it are as before
+    v2[0, :, n[0] + 2, 7] = INF
+    v2[1, :, n[1] + 2, 9] = NAN
+    got = cache.tree_attention(q, k2, v2, ints(*n), mask=mask)
+    ended()
+    others = [0, 1, 3, 4, 5]
+    assert torch.equal(got[0][:, others], want[0][:, others]) and torch.equal(got[1], want[1])
+    assert bool((got[0][0, 2, :, 7] == INF).all()) and bool(got[0][1, 2, :, 9].isnan().all())
+    rest = got[0][:, 2].clone()
+    rest[0, :, 7], rest[1, :, 9] = 0, 0
+    full = want[0][:, 2].clone()
+    full[0, :, 7], full[1, :, 9] = 0, 0
+    assert torch.equal(rest, full)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+def test_tokens_that_see_nothing(dt):
+    g, dtype = gen(6), TYPES[dt]
+    k, v = randn(g, 1, 2, 16, 128, dtype=dtype), randn(g, 1, 2, 16, 128, dtype=dtype)
+    q = randn(g, 1, 4, 4, 128, dtype=dtype)
+    mask = torch.tensor([0, 2, 0, 5], device="cuda")
+    out, lse = cache.tree_attention(q, k, v, ints(0), mask=mask)
+    ended()
+    assert bool((out[0, [0, 2]] == 0).all()) and bool((lse[0, [0, 2]] == -INF).all())
+    o, l, to, tl = attend(q, k, v, visible(mask, [0], [4], 4, 16), 128 ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+def test_layouts(dt):
+    """slots before heads, queries inside a wider row, an output with gaps; nothing beside the output is written"""
+    g, dtype = gen(7), TYPES[dt]
+    B, T, H, hk, D, n = 2, 5, 6, 2, 64, [70, 200]
+    cap = 220
+    k = randn(g, B, cap, hk, D, dtype=dtype).transpose(1, 2)
+    v = randn(g, hk, B, cap, 2 * D, dtype=dtype).transpose(0, 1)[..., :D]
+    q = randn(g, B, T, 3 * H, D, dtype=dtype)[:, :, H:2 * H]
+    big = torch.full((B, T, H, 2 * D), 5.0, dtype=dtype, device="cuda")
+    mask = tree_masks(g, B, T)
+    out, lse = cache.tree_attention(q, k, v, ints(*n), mask=mask, out=big[..., :D])
+    ended()
+    o, l, to, tl = attend(q, k, v, visible(mask, n, [T] * B, T, cap), D ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+    assert bool((big[..., D:] == 5).all())
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+def test_padded_batches_and_lengths_out_of_range(dt):
+    g, dtype = gen(8), TYPES[dt]
+    B, T, H, hk, D, cap = 6, 9, 4, 2, 128, 150
+    k, v = randn(g, B, hk, cap, D, dtype=dtype), randn(g, B, hk, cap, D, dtype=dtype)
+    q = randn(g, B, T, H, D, dtype=dtype)
+    q[0, 4:] = NAN
+    lens, counts = [100, 0, 30, cap - 3, -1, 20], [4, 9, 0, 4, 2, 10]  # the last three do not fit
+    mask = tree_masks(g, B, T)
+    out, lse = torch.full_like(q, 7.0), torch.full((B, T, H), 9.0, device="cuda")
+    mass = torch.full((B, hk, cap), 3.0, device="cuda")
+    cache.tree_attention(q, k, v, ints(*lens), mask=mask, counts=ints(*counts), out=out, lse=lse)
+    ended(64)
+    ok = [0, 1]
+    see = visible(mask[ok], [lens[b] for b in ok], [counts[b] for b in ok], T, cap)
+    o, l, to, tl = attend(q[ok], k[ok], v[ok], see, D ** -0.5)
+    for i, b in enumerate(ok):
+        n = counts[b]
+        close(out[b, :n], o[i, :n], to[i, :n])
+        close(lse[b, :n], l[i, :n], tl[i, :n])
+        assert bool((out[b, n:] == 7).all()) and bool((lse[b, n:] == 9).all())
+    assert bool((out[2:] == 7).all()) and bool((lse[2:] == 9).all())
+    cache.attention_mass(torch.zeros_like(q), lse, k, ints(*lens), mass, counts=ints(*counts))
+    ended(64)
+    assert bool((mass[2:] == 3).all()) and bool((mass[0, :, 104:] == 3).all()) and bool((mass[0, :, :104] != 3).all())
+
+
+def test_offsets_beyond_32_bits():
+    """two cache heads that lie more than 2^32 bytes and 2^31 elements apart"""
+    g = gen(9)
+    n, D, far = 300, 128, (1 << 31) + 4096
+    buf = torch.empty(far + 400 * D, dtype=torch.bfloat16, device="cuda")
+    k = torch.as_strided(buf, (1, 2, 400, D), (2 * far, far, D, 1))
+    k.copy_(randn(g, 1, 2, 400, D))
+    q = randn(g, 1, 3, 4, D, dtype=torch.bfloat16)
+    out, lse = cache.tree_attention(q, k, k, ints(n))
+    mass = torch.zeros(1, 2, 400, device="cuda")
+    cache.attention_mass(q, lse, k, ints(n), mass)
+    want, wl = cache.tree_attention(q, k.contiguous(), k.contiguous(), ints(n))
+    m2 = cache.attention_mass(q, lse, k.contiguous(), ints(n), torch.zeros_like(mass))
+    ended()
+    assert torch.equal(out, want) and torch.equal(lse, wl) and torch.equal(mass, m2)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("B,T,H,hk,D,lens,path", [
+    (1, 1, 1, 1, 64, [0], False), (1, 1, 14, 2, 64, [1000], False), (2, 6, 32, 8, 128, [127, 129], True), (1, 64, 8, 2, 128, [900], False),
+    (3, 33, 9, 3, 64, [0, 300, 128], True), (1, 64, 40, 5, 128, [77], True), (2, 64, 5, 1, 64, [4000, 5], False)])
+def test_attention_mass(dt, B, T, H, hk, D, lens, path):
+    g, dtype = gen(T * 7 + B), TYPES[dt]
+    cap, G, scale = max(lens) + T + 9, H // hk, D ** -0.5
+    k = randn(g, B, hk, cap, D, dtype=dtype)
+    k[:, :, max(lens) + T:] = NAN
+    q = randn(g, B, T, H, D, dtype=dtype, scale=1.5)
+    lse = randn(g, B, T, H, scale=0.3) + math.log(max(lens) + 1) + 1
+    lse[0, T // 2, 0] = -INF
+    mass = torch.rand(B, hk, cap, device="cuda", generator=g)
+    n = [max(1, T - 3 * b) for b in range(B)]
+    rows = torch.stack([torch.randperm(T, device="cuda", generator=g) for _ in range(B)]).int() if path else None
+    out = torch.full_like(mass, 8.0)
+    got = cache.attention_mass(q, lse, k, ints(*lens), mass, rows=rows, counts=ints(*n), out=out)
+    again = cache.attention_mass(q, lse, k, ints(*lens), mass.clone(), rows=rows, counts=ints(*n))
+    ended()
+    assert got is out
+    for b in range(B):
+        end = lens[b] + n[b]
+        assert bool((out[b, :, end:] == 8).all()) and torch.equal(again[b, :, end:], mass[b, :, end:])
+        assert torch.equal(again[b, :, :end], out[b, :, :end])
+        r = rows[b, :n[b]].long() if path else torch.arange(n[b], device="cuda")
+        for h in range(hk):
+            kk, qq = k[b, h, :end].double(), q[b, r, h * G:(h + 1) * G].double()
+            e = torch.exp(qq @ kk.T * scale - lse[b, r, h * G:(h + 1) * G].double()[..., None])
+            e[lse[b, r, h * G:(h + 1) * G] == -INF] = 0
+            late = torch.arange(end, device="cuda")[None, :] > lens[b] + torch.arange(n[b], device="cuda")[:, None]
+            e = e.masked_fill(late[:, None, :], 0)
+            a = (qq.abs() @ kk.abs().T) * scale
+            off = e * ((D + 16) * E * a + 4 * E + E * (qq @ kk.T * scale - lse[b, r, h * G:(h + 1) * G].double()[..., None]).abs().nan_to_num(0, 0, 0))
+            base = torch.where(torch.arange(end, device="cuda") < lens[b], mass[b, h, :end].double(), 0.0)
+            want = base + e.sum((0, 1))
+            tol = off.sum((0, 1)) + (n[b] * G + 2) * E * want
+            close(out[b, h, :end], want, tol)
+
+
+def test_mass_of_an_attention_call_adds_up_to_its_rows():
+    """over all slots, the weights of a token's heads sum to one each"""
+    g = gen(12)
+    B, T, H, hk, D, lens = 2, 5, 8, 2, 128, [700, 45]
+    k, v = randn(g, B, hk, 720, D, dtype=torch.float16), randn(g, B, hk, 720, D, dtype=torch.float16)
+    q = randn(g, B, T, H, D, dtype=torch.float16)
+    _, lse = cache.tree_attention(q, k, v, ints(*lens))
+    mass = cache.attention_mass(q, lse, k, ints(*lens), torch.zeros(B, hk, 720, device="cuda"))
+    ended()
+    # 720 fp32 sums of at most T * H / hk terms, each weight off by (D + 16) E A (A <= 0.09 * 128 * 25 for these values)
+    assert float((mass.sum(-1) - T * H / hk).abs().max()) < T * H / hk * ((D + 16) * E * 288 + 720 * E)
+
+
+def test_mass_rows_out_of_range():
+    g = gen(13)
+    k, q = randn(g, 1, 1, 40, 64), randn(g, 1, 3, 2, 64)
+    lse = torch.full((1, 3, 2), 3.0, device="cuda")
+    a = cache.attention_mass(q, lse, k, ints(20), torch.zeros(1, 1, 40, device="cuda"), rows=ints(1, 3, -1)[None].contiguous())
+    ended(64)
+    b = cache.attention_mass(q, lse, k, ints(20), torch.zeros(1, 1, 40, device="cuda"), rows=ints(1, 0, 0)[None].contiguous(), counts=ints(1))
+    ended()
+    assert torch.equal(a[..., :21], b[..., :21]) and bool((a[..., 21:] == 0).all())
+
+
+def evict_ref(m, n, budget, sinks, recent):
+    """kept slots of one sequence and head"""
+    if n <= budget:
+        return list(range(n))
+    mid = list(range(sinks, n - recent))
+    key = [(-INF if math.isnan(x) else x) for x in m]
+    mid.sort(key=lambda j: (-key[j], j))
+    return sorted(list(range(sinks)) + mid[: budget - sinks - recent] + list(range(n - recent, n)))
+
+
+MASSES = ["random", "ties", "odd", "zero", "skewed"]
+
+
+def masses(g, kind, *shape):
+    m = torch.rand(*shape, device="cuda", generator=g)
+    if kind == "ties":
+        m = (m * 4).floor() / 4
+    elif kind == "zero":
+        m = torch.where(m < 0.5, torch.zeros_like(m), -torch.zeros_like(m))
+    elif kind == "skewed":
+        m = 1 + m * 2.0 ** -20
+    elif kind == "odd":
+        m = torch.where(m < 0.1, torch.full_like(m, NAN), torch.where(m < 0.2, torch.full_like(m, -INF), torch.where(m > 0.9, torch.full_like(m, INF), 0.5 - m)))
+    return m
+
+
+@pytest.mark.parametrize("kind", MASSES)
+@pytest.mark.parametrize("dt,layers,B,hk,D,lens,cap,budget,sinks,recent", [
+    ("bf16", None, 1, 2, 64, [40], 40, 8, 0, 0), ("fp32", 2, 3, 2, 128, [0, 90, 33], 97, 33, 4, 8), ("fp16", 3, 2, 1, 128, [2500, 2049], 2600, 2048, 4, 64),
+    ("bf16", 1, 2, 3, 128, [5000, 4000], 5001, 1, 0, 0), ("fp32", None, 2, 1, 64, [300, 300], 300, 64, 32, 32), ("fp16", None, 1, 2, 64, [70000], 70001, 9999, 3, 100),
+    ("bf16", None, 1, 1, 64, [20000], 20000, 1500, 0, 1500)])
+def test_evict(kind, dt, layers, B, hk, D, lens, cap, budget, sinks, recent):
+    g, dtype = gen(budget + D), TYPES[dt]
+    lead = (B, hk) if layers is None else (layers, B, hk)
+    k, v = randn(g, *lead, cap, D, dtype=dtype), randn(g, *lead, cap, D, dtype=dtype)
+    m = masses(g, kind, *lead, cap)
+    ko, vo = torch.full((*lead, budget + 1, D), 3.0, dtype=dtype, device="cuda"), torch.full((*lead, budget + 1, D), 4.0, dtype=dtype, device="cuda")
+    mo = torch.full((*lead, budget + 1), 5.0, device="cuda")
+    new, kept = cache.kv_evict(k, v, m, ints(*lens), budget, sinks, recent, k_out=ko, v_out=vo, mass_out=mo)
+    ki, vi, mi = k.clone(), v.clone(), m.clone()
+    new2, kept2 = cache.kv_evict(ki, vi, mi, ints(*lens), budget, sinks, recent)
+    ended()
+    assert new.tolist() == [min(n, budget) for n in lens] == new2.tolist() and torch.equal(kept, kept2)
+    bits = lambda x: x.view(torch.int32)  # noqa: E731
+    mc = m.reshape(-1, B, hk, cap).cpu()
+    for l in range(mc.shape[0]):
+        for b in range(B):
+            for h in range(hk):
+                at = (b, h) if layers is None else (l, b, h)
+                want = evict_ref(mc[l, b, h].tolist(), lens[b], budget, sinks, recent)
+                assert kept[at].tolist() == want + [-1] * (budget - len(want))
+                n = len(want)
+                w = torch.tensor(want, device="cuda", dtype=torch.int64)
+                for x, y, z, fill in ((k, ko, ki, 3), (v, vo, vi, 4)):
+                    assert torch.equal(y[at][:n], x[at][w]) and bool((y[at][n:] == fill).all())
+                    assert torch.equal(z[at][:n], x[at][w]) and torch.equal(z[at][n:], x[at][n:])
+                assert torch.equal(bits(mo[at][:n]), bits(m[at][w])) and bool((mo[at][n:] == 5).all())
+                assert torch.equal(bits(mi[at][:n]), bits(m[at][w])) and torch.equal(bits(mi[at][n:]), bits(m[at][n:]))
+
+
+def test_evict_leaves_sequences_out_of_range():
+    g = gen(3)
+    k, v, m = randn(g, 3, 2, 50, 64), randn(g, 3, 2, 50, 64), torch.rand(3, 2, 50, device="cuda", generator=g)
+    new, kept = ints(7, 7, 7), torch.full((3, 2, 10), 7, dtype=torch.int32, device="cuda")
+    k0 = k.clone()
+    cache.kv_evict(k, v, m, ints(51, 30, -2), 10, new_lens=new, kept=kept)
+    ended(64)
+    assert new.tolist() == [7, 10, 7] and bool((kept[[0, 2]] == 7).all()) and torch.equal(k[[0, 2]], k0[[0, 2]])
+
+
+def accept_ref(tokens, parents, target, n):
+    if n == 0:
+        return []
+    path = [0]
+    while True:
+        kids = [c for c in range(1, n) if parents[c] == path[-1] and c > path[-1] and tokens[c] == target[path[-1]]]
+        if not kids:
+            return path
+        path.append(kids[0])
+
+
+@pytest.mark.parametrize("dt,layers,B,T,hk,D,vocab", [("fp16", 36, 1, 8, 2, 128, 2), ("fp32", None, 5, 64, 3, 64, 3), ("bf16", 2, 9, 33, 1, 128, 2),
+                                                      ("fp32", 1, 3, 1, 8, 128, 4), ("bf16", None, 2, 64, 8, 64, 1)])
+def test_tree_accept(dt, layers, B, T, hk, D, vocab):
+    """few different tokens, so that paths are long and children share a token; vocab 1 accepts a whole path"""
+    g, dtype = gen(T + B), TYPES[dt]
+    lens = [(37 * b) % 90 for b in range(B)]
+    counts = [max(0, T - 2 * b) for b in range(B)]
+    cap = 100 + T
+    lead = () if layers is None else (layers,)
+    k, v = randn(g, *lead, B, hk, cap, D, dtype=dtype), randn(g, *lead, B, hk, cap, D, dtype=dtype)
+    tokens, target = (torch.randint(0, vocab, (B, T), device="cuda", generator=g) for _ in range(2))
+    par = [[-1] + [int(torch.randint(max(-1, t - 4), t, (1,), device="cuda", generator=g)) for t in range(1, T)] for _ in range(B)]
+    k0, v0 = k.clone(), v.clone()
+    got = cache.tree_accept(tokens, torch.tensor(par, dtype=torch.int32, device="cuda"), target, k, v, ints(*lens), counts=ints(*counts))
+    ended()
+    for b in range(B):
+        path = accept_ref(tokens[b].tolist(), par[b], target[b].tolist(), counts[b])
+        assert got.path[b].tolist() == path + [-1] * (T - len(path))
+        assert int(got.accepted[b]) == len(path) and int(got.new_lens[b]) == lens[b] + len(path)
+        assert int(got.next_token[b]) == (int(target[b, path[-1]]) if path else -1)
+        if path:
+            src, dst = [lens[b] + c for c in path], slice(lens[b], lens[b] + len(path))
+            k0[..., b, :, dst, :] = k0[..., b, :, src, :].clone()
+            v0[..., b, :, dst, :] = v0[..., b, :, src, :].clone()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+def test_accept_out_of_range_accepts_nothing():
+    k = torch.zeros(3, 1, 10, 64, device="cuda")
+    t = torch.zeros(3, 4, dtype=torch.int64, device="cuda")
+    par = torch.tensor([[-1, 0, 1, 2]] * 3, dtype=torch.int32, device="cuda")
+    got = cache.tree_accept(t, par, t, k, k.clone(), ints(7, 6, -1))
+    ended(64)
+    assert got.accepted.tolist() == [0, 4, 0] and got.new_lens.tolist() == [7, 10, -1] and got.next_token.tolist() == [-1, 0, -1]
+    assert got.path[0].tolist() == [-1] * 4
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("B,T,H,hk,D,norm", [(1, 1, 32, 8, 128, True), (3, 7, 6, 2, 64, True), (2, 130, 4, 4, 128, False), (1, 1, 1, 1, 64, False)])
+def test_append(dt, B, T, H, hk, D, norm):
+    """y = x cos -+ x' sin of x = u w / sqrt(mean u^2 + eps): a few fp32 roundings of each product, then one to the type"""
+    g, dtype = gen(D + T), TYPES[dt]
+    cap, P = 40 + T, 500
+    x = randn(g, B * T, (H + 2 * hk) * D, scale=2.0)
+    q, k, v = (y.unflatten(1, (-1, D)).unflatten(0, (B, T)) for y in x.split([H * D, hk * D, hk * D], dim=1))
+    lens, counts = [(11 * b) % 40 for b in range(B)], [T - b for b in range(B)]
+    pos = torch.randint(0, P, (B, T), device="cuda", generator=g).int()
+    ang = torch.rand(P, D // 2, device="cuda", generator=g, dtype=torch.float64) * 7
+    cos, sin = torch.cos(ang).float(), torch.sin(ang).float()
+    qn, kn = (1 + randn(g, D, scale=0.1) if norm else None for _ in range(2))
+    kc = torch.full((B, cap, hk, D), 3.0, dtype=dtype, device="cuda").transpose(1, 2)
+    vc = torch.full((B, hk, cap, D), 4.0, dtype=dtype, device="cuda")
+    qo = torch.full((B, T, H, D), 5.0, dtype=dtype, device="cuda")
+    cache.kv_append(q, k, v, kc, vc, ints(*lens), pos, cos, sin, q_norm=qn, k_norm=kn, eps=1e-5, counts=ints(*counts), q_out=qo)
+    ended()
+    u = u_of(dtype)
+
+    def turned(y, w):
+        y = y.double()
+        if w is not None:
+            y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+        c, s = cos[pos.long()].double()[:, :, None], sin[pos.long()].double()[:, :, None]
+        a, b = y[..., : D // 2], y[..., D // 2:]
+        z = torch.cat([a * c - b * s, b * c + a * s], -1)
+        # D + 8 roundings of the norm's sum and scale (half of them in the root), 4 of the rotation
+        big = torch.cat([(a * c).abs() + (b * s).abs()] * 2, -1) + torch.cat([(b * c).abs() + (a * s).abs()] * 2, -1)
+        return z, u * z.abs() + ((D + 8) * E if w is not None else 0) * big + 4 * E * big
+
+    for b in range(B):
+        n, L = counts[b], lens[b]
+        wq, tq = turned(q, qn)
+        wk, tk = turned(k, kn)
+        close(qo[b, :n], wq[b, :n], tq[b, :n])
+        close(kc[b, :, L:L + n], wk[b, :n].transpose(0, 1), tk[b, :n].transpose(0, 1))
+        assert torch.equal(vc[b, :, L:L + n], v[b, :n].transpose(0, 1).to(dtype))
+        assert bool((qo[b, n:] == 5).all()) and bool((kc[b, :, L + n:] == 3).all()) and bool((vc[b, :, :L] == 4).all()) and bool((kc[b, :, :L] == 3).all())
+
+
+def test_append_leaves_out_what_is_out_of_range():
+    g = gen(2)
+    x = randn(g, 4, 3, 2, 64)
+    kc, vc = torch.zeros(4, 2, 10, 64, device="cuda"), torch.zeros(4, 2, 10, 64, device="cuda")
+    t = torch.ones(5, 32, device="cuda")
+    pos = torch.tensor([[0, 5, -1], [0, 1, 2], [0, 1, 2], [0, 1, 2]], dtype=torch.int32, device="cuda")
+    q = cache.kv_append(x, x, x, kc, vc, ints(0, 8, -1, 7), pos, t, t, q_out=torch.zeros_like(x))
+    ended(64)
+    written = kc.ne(0).any(-1).all(1)
+    assert written.tolist() == [[True] + [False] * 9, [False] * 10, [False] * 10, [False] * 7 + [True] * 3]
+    assert bool((q[0, 0] != 0).any()) and bool((q[0, 1:] == 0).all()) and bool((q[1:3] == 0).all())
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+def test_graphs_that_share_a_workspace_and_sequences_that_grow(dt):
+    """two captured calls on one workspace, replayed in turn with other lengths, give what eager calls give"""
+    g, dtype = gen(14), TYPES[dt]
+    B, T, H, hk, D, cap = 2, 4, 8, 2, 128, 3000
+    k, v = randn(g, B, hk, cap, D, dtype=dtype), randn(g, B, hk, cap, D, dtype=dtype)
+    q = [randn(g, B, T, H, D, dtype=dtype) for _ in range(2)]
+    lens, mask = ints(100, 1), tree_masks(g, B, T)
+    ws = torch.empty(cache.attention_workspace_size(k, T, H), dtype=torch.uint8, device="cuda")
+    outs = [(torch.empty_like(q[0]), torch.empty(B, T, H, device="cuda")) for _ in range(2)]
+    mass = torch.zeros(B, hk, cap, device="cuda")
+    graphs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(2):
+            cache.tree_attention(q[i], k, v, lens, mask=mask, out=outs[i][0], lse=outs[i][1], workspace=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            cache.tree_attention(q[i], k, v, lens, mask=mask, out=outs[i][0], lse=outs[i][1], workspace=ws)
+            cache.attention_mass(q[i], outs[i][1], k, lens, mass)
+        graphs.append(gr)
+    for a, b in ((100, 1), (2990, 0), (0, 1500), (640, 2996)):
+        lens.copy_(ints(a, b))
+        mass.zero_()
+        want, total = [], torch.zeros_like(mass)
+        for i in range(2):
+            want.append(cache.tree_attention(q[i], k, v, lens, mask=mask))
+            cache.attention_mass(q[i], want[i][1], k, lens, total)
+        for gr in graphs:
+            gr.replay()
+        ended()
+        for i in range(2):
+            assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
+        assert torch.equal(mass, total)
+
+
+def test_another_stream_and_two_calls_at_once():
+    g = gen(15)
+    B, T, H, hk, D, cap = 1, 8, 32, 8, 128, 20000
+    k, v = randn(g, B, hk, cap, D, dtype=torch.bfloat16), randn(g, B, hk, cap, D, dtype=torch.bfloat16)
+    q = [randn(g, B, T, H, D, dtype=torch.bfloat16) for _ in range(2)]
+    lens = ints(cap - T)
+    want = [cache.tree_attention(x, k, v, lens) for x in q]
+    torch.cuda.synchronize()
+    st = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = [cache.tree_attention(x, k, v, lens, stream=s) for x, s in zip(q, st)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ended()
+
+
+def test_python_refusals():
+    k = torch.zeros(2, 2, 16, 64, device="cuda")
+    q, lens, m = torch.zeros(2, 3, 4, 64, device="cuda"), ints(4, 5), torch.zeros(2, 2, 16, device="cuda")
+    t = torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    lse = torch.zeros(2, 3, 4, device="cuda")
+    bad = [
+        lambda: cache.tree_attention(q.half(), k, k.clone(), lens),
+        lambda: cache.tree_attention(q[:, :, :3], k, k, lens),
+        lambda: cache.tree_attention(q[..., :32], k, k, lens),
+        lambda: cache.tree_attention(q, k, k.half(), lens),
+        lambda: cache.tree_attention(q, k, k, lens.long()),
+        lambda: cache.tree_attention(q, k, k, lens.cpu()),
+        lambda: cache.tree_attention(q, k, k, lens, mask=t[:, :2]),
+        lambda: cache.tree_attention(q, k, k, lens, mask=t.int()),
+        lambda: cache.tree_attention(q.transpose(1, 3), k, k, lens),
+        lambda: cache.tree_attention(torch.zeros(2, 65, 4, 64, device="cuda"), k, k, lens),
+        lambda: cache.tree_attention(q, k, k, lens, out=q.half()),
+        lambda: cache.attention_mass(q, lse[:, :2], k, lens, m),
+        lambda: cache.attention_mass(q, lse, k, lens, m[..., :10]),
+        lambda: cache.attention_mass(q, lse, k, lens, m.double()),
+        lambda: cache.kv_evict(k, k, m, lens, 4, k_out=k.clone()),
+        lambda: cache.kv_evict(k, k, m[..., :4], lens, 4),
+        lambda: cache.kv_evict(k, k, m, lens, 4, kept=torch.zeros(2, 2, 5, dtype=torch.int32, device="cuda")),
+        lambda: cache.tree_accept(t.int(), t.int(), t, k, k, lens),
+        lambda: cache.tree_accept(t, t, t, k, k, lens),
+        lambda: cache.kv_append(q, q[:, :, :2], q[:, :, :2], k, k, lens, t, k[0, 0], k[0, 0]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    status = [
+        (lambda: cache.tree_attention(q, k, k, lens, out=q), -1),
+        (lambda: cache.tree_attention(torch.zeros(2 * 3 * 4 * 64 + 1, device="cuda")[1:].view(2, 3, 4, 64), k, k, lens), -1),
+        (lambda: cache.kv_evict(k, k.clone(), m, lens, 0), -1),
+        (lambda: cache.kv_evict(k, k.clone(), m, lens, 17), -1),
+        (lambda: cache.kv_evict(k, k.clone(), m, lens, 4, sinks=3, recent=2), -1),
+        (lambda: cache.kv_evict(k, k.clone(), m, lens, 4, new_lens=lens), -1),
+        (lambda: cache.kv_evict(k, k.clone(), m, lens, 4, k_out=k[:, :, 4:], v_out=k.clone(), mass_out=m.clone()[..., 4:]), None),
+    ]
+    for i, (call, code) in enumerate(status):
+        with pytest.raises((p8.P8Error, ValueError)) as e:
+            call()
+        assert code is None or e.value.status == code, i
+    ended()
