@@ -1,5 +1,6 @@
 // p8_cache.cu -- key/value cache operators: append (norm, rotation, write), eviction, tree acceptance, and the C ABI
 // entry points of all five (the attention and mass kernels are in p8_tree_attn.cuh).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -7,7 +8,8 @@
 #include <stdint.h>
 #include <string.h>
 
-#include <mutex>
+#include <algorithm>
+#include <atomic>
 
 #include "p8_device.cuh"
 #include "p8_internal.h"
@@ -16,7 +18,7 @@ namespace p8 {
 
 // The operators' own error word (bits 64 and 128 of p8_device_error).
 __device__ unsigned int g_cache_error = 0;
-constexpr unsigned int kErrRange = 64u;
+constexpr unsigned int kErrRange = 64u, kErrWait = 128u;
 
 unsigned int read_and_clear_cache_error() {
     unsigned int v = 0, z = 0;
@@ -411,7 +413,7 @@ bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 // strides (elements) of the dimensions that are used, as multiples of 16 bytes
 bool strides_ok(const int64_t *st, const int64_t *dims, int n, int es) {
     for (int i = 0; i < n; ++i)
-        if (dims[i] > 1 && (st[i] * es) % 16) return false;
+        if (dims[i] > 1 && (st[i] <= 0 || (st[i] * es) % 16)) return false;
     return true;
 }
 

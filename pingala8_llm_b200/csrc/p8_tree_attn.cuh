@@ -14,6 +14,7 @@ struct AttnArgs {
     float *mass_out;
     long long ms[2], mos[2];
     int batch, tokens, heads, kvh, group;
+    int g0, gc, more;  // mass: the query heads g0 .. g0 + gc - 1 of each group; more: added to what `out` has
     float scale;
 };
 
@@ -132,7 +133,951 @@ __global__ void __launch_bounds__(128) k_attn_mass_plain(const AttnArgs a) {
     }
 }
 
-size_t tree_attn_workspace(const p8_kv *, int64_t, int64_t) { return 0; }
+// ================================================================================================================
+// 16-bit caches: tcgen05
+// ================================================================================================================
+// A unit is (sequence, cache head, block of query rows); its slots are cut into tiles of 128. All tiles of all units
+// form one list, sequence by sequence, and every CTA takes an equal contiguous share of it, so that the SMs finish
+// together whatever the lengths are, and one long sequence still fills them. A unit that lies in one share is finished
+// there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
+constexpr int kTile = 128;
+
+struct Share {
+    long long pos, end;  // the CTA's tiles
+    long long off;       // of pos, within sequence b
+    int b;
+};
+
+struct Walk {            // a CTA's way through its share, one segment (the tiles of one unit) at a time
+    const AttnArgs &a;
+    int rblock;
+    long long pos, end, off;
+    int b, len, n, nt, units, u, ta, tb;
+    bool opens;          // the segment is the share's first
+    __device__ Walk(const AttnArgs &a_, int rb, const Share &s) : a(a_), rblock(rb), pos(s.pos), end(s.end), off(s.off), b(s.b) {
+        opens = true;
+        if (pos < end) load();
+    }
+    __device__ void load() {
+        if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
+        nt = n ? (len + n + kTile - 1) / kTile : 0;
+        units = n ? a.kvh * ((n * a.group + rblock - 1) / rblock) : 0;
+    }
+    __device__ bool next() {
+        if (pos >= end) return false;
+        while (off >= (long long)units * nt) {
+            off -= (long long)units * nt;
+            ++b;
+            load();
+        }
+        u = (int)(off / nt);
+        ta = (int)(off - (long long)u * nt);
+        tb = (int)min((long long)nt, ta + (end - pos));
+        return true;
+    }
+    __device__ void advance() {
+        pos += tb - ta;
+        off += tb - ta;
+        opens = false;
+    }
+    __device__ int blocks() const { return units / a.kvh; }
+    __device__ int head() const { return u / blocks(); }
+    __device__ int row0() const { return u % blocks() * rblock; }
+    __device__ bool whole() const { return ta == 0 && tb == nt; }
+};
+
+__device__ __forceinline__ long long seq_tiles(const AttnArgs &a, int rblock, int b, bool *bad) {
+    int len, n;
+    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
+        *bad = true;
+        return 0;
+    }
+    return n ? (long long)a.kvh * ((n * a.group + rblock - 1) / rblock) * ((len + n + kTile - 1) / kTile) : 0;
+}
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ long long warp_scan(long long v, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+// tiles of all sequences (whole warp)
+__device__ __forceinline__ long long all_tiles(const AttnArgs &a, int rblock, int lane, bool *bad) {
+    long long total = 0;
+    for (int b = lane; b < a.batch; b += 32) total += seq_tiles(a, rblock, b, bad);
+    return warp_sum(total);
+}
+// the share of one CTA (whole warp)
+__device__ __forceinline__ Share find_share(const AttnArgs &a, int rblock, int lane, int cta, int ctas) {
+    bool bad = false;
+    const long long total = all_tiles(a, rblock, lane, &bad);
+    if (bad && cta == 0) atomicOr(&g_cache_error, kErrRange);
+    const long long each = (total + ctas - 1) / ctas;
+    Share s;
+    s.pos = min(total, cta * each);
+    s.end = min(total, s.pos + each);
+    s.b = 0;
+    s.off = 0;
+    long long run = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const long long mine = b0 + lane < a.batch ? seq_tiles(a, rblock, b0 + lane, &bad) : 0;
+        const long long incl = run + warp_scan(mine, lane);
+        const unsigned int hit = __ballot_sync(0xffffffffu, incl > s.pos);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            s.b = b0 + l;
+            s.off = s.pos - __shfl_sync(0xffffffffu, incl - mine, l);
+            break;
+        }
+        run = __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return s;
+}
+
+// Waits give up after two seconds (the kernel's results are then invalid and bit 128 is set); from then on every wait
+// of the CTA returns at once, so that all roles run through to the end and meet there.
+struct Waits {
+    volatile int *gave_up;
+    __device__ void operator()(uint64_t *bar, uint32_t parity) const {
+        if (mbar_try_wait(bar, parity) || *gave_up) return;
+        unsigned long long t0, t;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+        for (uint32_t i = 1;; ++i) {
+            if (mbar_try_wait(bar, parity)) return;
+            if ((i & 63) == 0) {
+                asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+                if (*gave_up || t - t0 > 2000000000ull) break;
+            }
+        }
+        *gave_up = 1;
+        atomicOr(&g_cache_error, kErrWait);
+    }
+};
+
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+                 : "memory");
+}
+// Shared-memory operand of 128-byte rows in the 128-byte swizzle (what the tensor map's loads leave; a stage is `rows`
+// rows per 64 columns). Rows as the outer extent (Q, K): groups of 8 rows 1024 bytes apart. Rows as the summed one (V):
+// the same bytes read the other way, the next 64 columns a whole stage part (16 KB) on.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_cols(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <typename T> struct Half16;  // what differs between the two 16-bit types
+template <> struct Half16<__nv_bfloat16> {
+    static constexpr bool bf16 = true;
+    // The weights p = 2^(s - m + kLift) are rounded to the type. The running maximum m is only raised when the new one
+    // is kSlack above it, which saves most passes over the accumulator; p then stays below 2^(kLift + kSlack).
+    static constexpr float kLift = 0.f, kSlack = 8.f;
+    static constexpr uint32_t kExp = 0x7F80u;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+template <> struct Half16<__half> {
+    static constexpr bool bf16 = false;
+    // fp16 ends at 2^-24: lifted by 2^10, weights keep their 11 bits down to 2^-24 of the largest (and stay below 2^15)
+    static constexpr float kLift = 10.f, kSlack = 5.f;
+    static constexpr uint32_t kExp = 0x7C00u;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_of(int n, bool b_cols) {  // f32 accumulator, M = 128
+    const uint32_t f = Half16<T>::bf16 ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((b_cols ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(da), "l"(db),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(ta), "l"(db),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+#define P8_R32(v) "=r"((v)[0]), "=r"((v)[1]), "=r"((v)[2]), "=r"((v)[3]), "=r"((v)[4]), "=r"((v)[5]), "=r"((v)[6]), "=r"((v)[7]), "=r"((v)[8]), \
+    "=r"((v)[9]), "=r"((v)[10]), "=r"((v)[11]), "=r"((v)[12]), "=r"((v)[13]), "=r"((v)[14]), "=r"((v)[15]), "=r"((v)[16]), "=r"((v)[17]), \
+    "=r"((v)[18]), "=r"((v)[19]), "=r"((v)[20]), "=r"((v)[21]), "=r"((v)[22]), "=r"((v)[23]), "=r"((v)[24]), "=r"((v)[25]), "=r"((v)[26]), \
+    "=r"((v)[27]), "=r"((v)[28]), "=r"((v)[29]), "=r"((v)[30]), "=r"((v)[31])
+// 32 lanes x 32 columns of 32 bits; the values are there after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : P8_R32(v)
+        : "r"(at)
+        : "memory");
+}
+#undef P8_R32
+#define P8_RW8(v, o) "+r"((v)[o]), "+r"((v)[o + 1]), "+r"((v)[o + 2]), "+r"((v)[o + 3]), "+r"((v)[o + 4]), "+r"((v)[o + 5]), "+r"((v)[o + 6]), "+r"((v)[o + 7])
+// the wait names the registers, so that nothing that reads them moves ahead of it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : P8_RW8(v, 0), P8_RW8(v, 8), P8_RW8(v, 16), P8_RW8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_waited(uint32_t (&v)[32]) { asm volatile("" : P8_RW8(v, 0), P8_RW8(v, 8), P8_RW8(v, 16), P8_RW8(v, 24)::"memory"); }
+#undef P8_RW8
+#define P8_R16(v, o) "r"((v)[o]), "r"((v)[o + 1]), "r"((v)[o + 2]), "r"((v)[o + 3]), "r"((v)[o + 4]), "r"((v)[o + 5]), "r"((v)[o + 6]), "r"((v)[o + 7]), \
+    "r"((v)[o + 8]), "r"((v)[o + 9]), "r"((v)[o + 10]), "r"((v)[o + 11]), "r"((v)[o + 12]), "r"((v)[o + 13]), "r"((v)[o + 14]), "r"((v)[o + 15])
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+        P8_R16(v, 0), P8_R16(v, 16)
+        : "memory");
+}
+#undef P8_R16
+__device__ __forceinline__ void tmem_st2(uint32_t at, float x, float y) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ float2 tmem_ld2(uint32_t at) {
+    float2 v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];\n tcgen05.wait::ld.sync.aligned;" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Q rows [row0, row0 + tiles * 128) of a unit into swizzled shared memory, 16 bytes a thread and step; rows behind the
+// last are zero. flip: the sign bits (a negative scale is taken as its magnitude and -q).
+template <typename T, int D>
+__device__ __forceinline__ void load_q(char *sq, const AttnArgs &a, int b, int h, int row0, int rows, int tiles, uint32_t flip, int tid, int threads) {
+    constexpr int C = D / 8;
+    const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
+    for (int i = tid; i < tiles * 128 * C; i += threads) {
+        const int c = i % C, r = i / C, row = row0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < rows) {
+            const int t = row / a.group, g = row - t * a.group;
+            v = *reinterpret_cast<const uint4 *>(q + t * a.qs[1] + (long long)(h * a.group + g) * a.qs[2] + c * 8);
+            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        }
+        char *at = sq + (r / 128) * (128 * D * 2) + (c / 8) * 16384 + (r % 128) * 128 + (((c % 8) ^ (r % 8)) * 16);
+        *reinterpret_cast<uint4 *>(at) = v;
+    }
+}
+
+// The tree attention kernel. Ten warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
+// brings tiles of K and V into a ring by TMA, one that issues the MMAs. Two streams of work alternate, one per softmax
+// group, so that the tensor cores compute one stream's scores while the other's are exponentiated:
+//   TWO = false (at most 128 query rows): both streams have the same rows, and the tiles alternate between them; their
+//                accumulators are joined at the segment's end.
+//   TWO = true: stream s has rows 128 s .. of a block of 256, both take every tile (one copy of K and V for 256 rows).
+// Step i of a segment is stream i % 2 on tile i (TWO: i / 2):  S = Q K^T (128 x 128, TMEM) -> softmax group: mask,
+// running maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). The next S of a
+// stream is issued once its P V is done.
+// Bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.7 k cycles, the MMAs 1 k per
+// stream's step, the exponentials (128 x 128 at 16 a cycle) another 1 k.
+template <int D, bool TWO>
+struct TcShape {
+    static constexpr int kStage = kTile * D * 2;
+    static constexpr int kQ = (TWO ? 2 : 1) * 128 * D * 2;
+    static constexpr int kStages = D == 64 ? 10 : TWO ? 5 : 6;
+    static constexpr int kRows = TWO ? 256 : 128;
+    static constexpr int kSmem = 1024 + kQ + kStages * kStage;
+};
+
+template <typename T, int D, bool TWO>
+__global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                                                         float *part_o, float2 *part_ml) {
+    using S_ = TcShape<D, TWO>;
+    using H = Half16<T>;
+    constexpr int NST = S_::kStages, kBoxes = D / 64;
+    extern __shared__ char dyn[];
+    char *sq = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = sq + S_::kQ;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2], b_p[2], b_pv[2], b_q, b_seg;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_gave_up;
+    __shared__ Share s_share;
+    __shared__ unsigned long long s_bad[2];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const Waits wait{&s_gave_up};
+    if (warp == 0) {
+        const Share s = find_share(a, S_::kRows, lane, blockIdx.x, gridDim.x);
+        if (lane == 0) s_share = s;
+    } else if (warp == 9) {
+        tmem_alloc(&s_tmem, 512);
+    } else if (tid == 256) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(b_empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_s + i, 1);
+            mbar_init(b_p + i, 128);
+            mbar_init(b_pv + i, 1);
+            s_bad[i] = 0;
+        }
+        mbar_init(&b_q, 256);
+        mbar_init(&b_seg, 256);
+        s_gave_up = 0;
+        fence_mbar_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    Walk w(a, S_::kRows, s_share);
+
+    if (warp == 8) {  // ---------------------------------------------------------------- loads
+        uint32_t n = 0;
+        auto load = [&](const CUtensorMap *m, int tile) {
+            const int st = n % NST;
+            wait(b_empty + st, (n / NST & 1) ^ 1);
+            if (lane == 0) {
+                mbar_expect_tx(b_full + st, S_::kStage);
+#pragma unroll
+                for (int x = 0; x < kBoxes; ++x) tma_load(ring + st * S_::kStage + x * 16384, m, 64 * x, tile * kTile, w.head(), w.b, b_full + st);
+            }
+            ++n;
+        };
+        while (w.next()) {
+            const int nt = w.tb - w.ta;
+            if (TWO) {
+                for (int t = 0; t < nt; ++t) {
+                    load(&mk, w.ta + t);
+                    load(&mv, w.ta + t);
+                }
+            } else {  // in the order of use: K0 K1 V0 K2 V1 ...
+                load(&mk, w.ta);
+                if (nt > 1) load(&mk, w.ta + 1);
+                for (int t = 0; t < nt; ++t) {
+                    load(&mv, w.ta + t);
+                    if (t + 2 < nt) load(&mk, w.ta + t + 2);
+                }
+            }
+            w.advance();
+        }
+        // nothing may be in flight into this CTA's shared memory when it ends
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+    } else if (warp == 9) {  // ----------------------------------------------------------- MMAs
+        uint32_t base = 0, seg = 0, c_p[2] = {0, 0}, c_pv[2] = {0, 0};
+        constexpr uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(D, true);
+        while (w.next()) {
+            const int ns = (w.tb - w.ta) * (TWO ? 2 : 1);
+            wait(&b_q, seg & 1);
+            tc_fence_after();
+            auto scores = [&](int i) {
+                const int s = i & 1;
+                const uint32_t at = base + (TWO ? 2 * (i / 2) : i < 2 ? i : 2 * i - 1), st = at % NST;
+                wait(b_full + st, at / NST & 1);
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t qa = smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0), ka = smem_u32(ring + st * S_::kStage);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t o = (kk / 4) * 16384 + (kk % 4) * 32;
+                        mma_ss(tmem + 128 * s, desc_rows(qa + o), desc_rows(ka + o), id_s, kk != 0);
+                    }
+                    if (!TWO || s == 1) umma_commit(b_empty + st);
+                    umma_commit(b_s + s);
+                }
+                __syncwarp();
+            };
+            scores(0);
+            if (ns > 1) scores(1);
+            for (int i = 0; i < ns; ++i) {
+                const int s = i & 1;
+                const uint32_t at = base + (TWO ? 2 * (i / 2) + 1 : i + min(i + 2, ns)), st = at % NST;
+                wait(b_p + s, c_p[s]++ & 1);
+                wait(b_full + st, at / NST & 1);
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t va = smem_u32(ring + st * S_::kStage);
+#pragma unroll
+                    for (int kk = 0; kk < kTile / 16; ++kk)
+                        mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, desc_cols(va + kk * 2048), id_o, i >= 2 || kk != 0);
+                    if (!TWO || s == 1) umma_commit(b_empty + st);
+                    umma_commit(b_pv + s);
+                }
+                __syncwarp();
+                if (i + 2 < ns) {
+                    wait(b_pv + s, c_pv[s] & 1);  // P is read: its columns may hold the next scores
+                    scores(i + 2);
+                }
+                ++c_pv[s];
+            }
+            base += 2 * (w.tb - w.ta);
+            ++seg;
+            w.advance();
+        }
+    } else {  // -------------------------------------------------------------------------- softmax
+        const int s = warp / 4, r = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, tS = tmem + 128 * s + lanes, tO = tmem + 256 + 128 * s + lanes;
+        const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // scores in base 2; 0 as a number that vanishes beside them
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+        uint32_t base = 0, seg = 0, c_s = 0, c_pv = 0;
+        while (w.next()) {
+            const int ns = (w.tb - w.ta) * (TWO ? 2 : 1), h = w.head(), row0 = w.row0(), rows = w.n * a.group;
+            const int row = row0 + (TWO ? 128 * s : 0) + r;
+            const bool live = row < rows;
+            const bool warp_live = row0 + (TWO ? 128 * s : 0) + (warp & 3) * 32 < rows;
+            load_q<T, D>(sq, a, w.b, h, row0, rows, TWO ? 2 : 1, flip, tid, 256);
+            fence_proxy_async();
+            mbar_arrive(&b_q);
+            unsigned long long sees = 0;
+            if (live) {
+                const int t = row / a.group;
+                sees = a.mask ? a.mask[w.b * a.mask_stride + t] : ~0ull >> (63 - t);
+                if (w.n < 64) sees &= (1ull << w.n) - 1;
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int i = s; i < ns; i += 2) {
+                const int tile = w.ta + (TWO ? i / 2 : i), key0 = tile * kTile;
+                const bool tail = key0 + kTile > w.len;
+                wait(b_s + s, c_s++ & 1);
+                tc_fence_after();
+                if (warp_live) {
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) tmem_ld32(tS + 32 * j, x[j]);
+                    tmem_wait_ld(x[0]);
+#pragma unroll
+                    for (int j = 1; j < 4; ++j) tmem_waited(x[j]);
+                    if (tail) {
+                        const int off = w.len - key0;  // the tile's columns before it are the sequence's
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int o = off - 32 * j;  // bit k of `see`: column 32 j + k
+                            uint32_t see = o >= 32 ? ~0u : o > 0 ? (1u << o) - 1 : 0u;
+                            if (o < 32 && o > -64) see |= o >= 0 ? (uint32_t)sees << o : (uint32_t)(sees >> -o);
+                            if (!live) see = 0;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (!(see >> k & 1)) x[j][k] = 0xFF800000u;
+                        }
+                    }
+                    float top = __uint_as_float(x[0][0]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(x[j][k]));
+                    top = top == -INFINITY ? m : fmaxf(m, top * c);
+                    if (m == -INFINITY) m = top;  // nothing summed so far
+                    const bool raise = top > m + H::kSlack;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float f = raise ? ex2(m - top) : 1.f;
+                        if (raise) m = top;
+                        l *= f;
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j) {
+                            uint32_t o[32];
+                            tmem_ld32(tO + 32 * j, o);
+                            tmem_wait_ld(o);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st32(tO + 32 * j, o);
+                        }
+                    }
+                    const float sub = m == -INFINITY ? 0.f : H::kLift - m;
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const float p0 = ex2(fmaf(__uint_as_float(x[j + k / 16][2 * (k % 16)]), c, sub));
+                            const float p1 = ex2(fmaf(__uint_as_float(x[j + k / 16][2 * (k % 16) + 1]), c, sub));
+                            l4[k & 1] += p0;
+                            l4[2 + (k & 1)] += p1;
+                            p[k] = H::pack(p0, p1);
+                        }
+                        tmem_st32(tS + 16 * j, p);
+                    }
+                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    tmem_wait_st();
+                }
+                if (tail && (!TWO || s == 0)) {
+                    // Weights are 0 where a row does not see a slot, but 0 times an infinity is not: rows of V behind the
+                    // drafted tokens become zero, and so do a drafted token's infinities and NaN, which reach the rows
+                    // that do see it at the segment's end.
+                    const uint32_t at = base + (TWO ? 2 * (i / 2) + 1 : i + min(i + 2, ns)), st = at % NST;
+                    wait(b_full + st, at / NST & 1);
+                    const int first = max(0, w.len - key0), real = w.len + w.n - key0;
+                    for (int k = r; k < (kTile - first) * (D / 8); k += 128) {
+                        const int y = first + k / (D / 8), ch = k % (D / 8);
+                        uint4 *v = reinterpret_cast<uint4 *>(ring + st * S_::kStage + (ch / 8) * 16384 + y * 128 + ((ch % 8) ^ (y % 8)) * 16);
+                        if (y >= real) {
+                            *v = make_uint4(0, 0, 0, 0);
+                        } else {
+                            uint32_t q[4] = {v->x, v->y, v->z, v->w};
+                            bool bad = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if ((q[e] & H::kExp) == H::kExp) { q[e] &= 0xFFFF0000u; bad = true; }
+                                if ((q[e] >> 16 & H::kExp) == H::kExp) { q[e] &= 0x0000FFFFu; bad = true; }
+                            }
+                            if (bad) {
+                                *v = make_uint4(q[0], q[1], q[2], q[3]);
+                                atomicOr(&s_bad[seg & 1], 1ull << (key0 + y - w.len));
+                            }
+                        }
+                    }
+                    fence_proxy_async();
+                }
+                tc_fence_before();
+                mbar_arrive(b_p + s);
+                ++c_pv;
+            }
+            const int mine = (ns - s + 1) / 2;
+            if (mine > 0) wait(b_pv + s, (c_pv - 1) & 1);
+            tc_fence_after();
+            if (!TWO) {  // the stream's statistics for the other group, over its scores, which are done with
+                tmem_st2(tS, m, l);
+                tmem_wait_st();
+                tc_fence_before();
+            }
+            mbar_arrive(&b_seg);
+            wait(&b_seg, seg & 1);
+            tc_fence_after();
+            if (tid == 0) s_bad[(seg + 1) & 1] = 0;
+            const unsigned long long bad = s_bad[seg & 1] & sees;
+            // out = sum over this thread's streams of f O, in columns [x0, x1)
+            float f0 = 1.f, f1 = 0.f;
+            int x0 = 0, x1 = D;
+            bool both = false;
+            if (!TWO) {
+                const float2 o = tmem_ld2(tmem + 128 * (s ^ 1) + lanes);
+                const float m0 = s ? o.x : m, m1 = s ? m : o.x, l0 = s ? o.y : l, l1 = s ? l : o.y;
+                both = ns > 1;
+                const float top = fmaxf(m0, m1);
+                f0 = m0 == top ? 1.f : ex2(m0 - top);
+                f1 = !both ? 0.f : m1 == top ? 1.f : ex2(m1 - top);
+                m = top;
+                l = l0 * f0 + (both ? l1 * f1 : 0.f);
+                x0 = s * (D / 2);
+                x1 = x0 + D / 2;
+            }
+            if (warp_live) {
+                const bool whole = w.whole();
+                const int t = row / a.group, head = h * a.group + row % a.group;
+                const long long pr = ((long long)blockIdx.x * 2 + (w.opens ? 0 : 1)) * S_::kRows + (TWO ? 128 * s : 0) + r;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                T *out = static_cast<T *>(a.out) + w.b * a.os[0] + t * a.os[1] + (long long)head * a.os[2];
+                float *po = part_o + pr * D;
+                const uint32_t t0 = tmem + 256 + lanes + (TWO ? 128 * s : 0);
+#pragma unroll
+                for (int j = 0; j < (TWO ? D : D / 2) / 32; ++j) {
+                    uint32_t o[32];
+                    tmem_ld32(t0 + x0 + 32 * j, o);
+                    tmem_wait_ld(o);
+                    if (!TWO) {
+                        uint32_t o1[32];
+                        if (both) {
+                            tmem_ld32(t0 + 128 + x0 + 32 * j, o1);
+                            tmem_wait_ld(o1);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            float y = __uint_as_float(o[k]) * f0;
+                            if (both) y = fmaf(__uint_as_float(o1[k]), f1, y);
+                            o[k] = __float_as_uint(y);
+                        }
+                    }
+                    if (live) {
+                        for (unsigned long long rest = bad; rest; rest &= rest - 1) {
+                            const T *v = static_cast<const T *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)(w.len + __ffsll(rest) - 1) * a.vs[2] + x0 + 32 * j;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                const float y = to_f(v[k]);
+                                if (!isfinite(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+                            }
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int k = 0; k < 32; k += 8) {
+                                uint32_t q[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    q[e] = H::pack(__uint_as_float(o[k + 2 * e]) * inv, __uint_as_float(o[k + 2 * e + 1]) * inv);
+                                *reinterpret_cast<uint4 *>(out + x0 + 32 * j + k) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(po + x0 + 32 * j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        }
+                    }
+                }
+                if (live && x0 == 0) {
+                    if (!whole) part_ml[pr] = make_float2(m, l);
+                    else if (a.lse) a.lse[((long long)w.b * a.tokens + t) * a.heads + head] = l == 0.f ? -INFINITY : (m - H::kLift + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+            tc_fence_before();
+            base += 2 * (w.tb - w.ta);
+            ++seg;
+            w.advance();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// Adds up a unit's parts: one warp per query row; lanes find the largest maximum, then every lane sums its columns over
+// the parts in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, int rblock, int ctas, float lift, const float *part_o, const float2 *part_ml) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x % 32;
+    const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+    if (id >= (long long)a.batch * a.tokens * a.heads) return;
+    const int head = (int)(id % a.heads), t = (int)(id / a.heads % a.tokens), b = (int)(id / a.heads / a.tokens);
+    int len, n;
+    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n) || t >= n) return;
+    bool bad = false;
+    long long total = 0, before = 0;
+    for (int x = lane; x < a.batch; x += 32) {
+        const long long k = seq_tiles(a, rblock, x, &bad);
+        total += k;
+        before += x < b ? k : 0;
+    }
+    total = warp_sum(total);
+    before = warp_sum(before);
+    const long long each = (total + ctas - 1) / ctas;
+    const int blocks = (n * a.group + rblock - 1) / rblock, nt = (len + n + kTile - 1) / kTile;
+    const int h = head / a.group, row = t * a.group + head % a.group;
+    const long long u0 = before + (long long)(h * blocks + row / rblock) * nt, u1 = u0 + nt;
+    const int c0 = (int)(u0 / each), c1 = (int)((u1 - 1) / each);
+    if (c0 == c1) return;  // finished by that CTA
+    auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each != u0 ? 1 : 0)) * rblock + row % rblock; };
+    float m = -INFINITY;
+    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[at(c)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, acc[D / 32] = {};
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+        const float2 ml = part_ml[at(c)];
+        const float f = ml.x == m ? 1.f : ex2(ml.x - m);
+        l = fmaf(ml.y, f, l);
+        const float *p = part_o + at(c) * D + lane * (D / 32);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) acc[k] = fmaf(p[k], f, acc[k]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *out = static_cast<T *>(a.out) + b * a.os[0] + t * a.os[1] + (long long)head * a.os[2] + lane * (D / 32);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) out[k] = from_f<T>(acc[k] * inv);
+    if (a.lse && lane == 0) a.lse[((long long)b * a.tokens + t) * a.heads + head] = l == 0.f ? -INFINITY : (m - lift + log2f(l)) * 0.6931471805599453f;
+}
+
+// The mass kernel: S^T = K Q^T, a tile's 128 slots as the TMEM lanes and the query rows as its columns, so that a thread
+// holds one slot and its sum over rows needs no other thread. Two softmax groups take tiles in turn. Keys come through
+// a TMA ring, the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows
+// (32 KB a tile: 1.4 k cycles at 1/148 of the bandwidth), by the exponentials (8 cycles a row and tile) beyond.
+template <int D, int ROWS>
+struct MassShape {
+    static constexpr int kStage = kTile * D * 2;
+    static constexpr int kQ = ROWS * D * 2;
+    static constexpr int kStages = D == 64 ? 6 : ROWS == 256 ? 5 : 2;
+    static constexpr int kSmem = 1024 + kQ + kStages * kStage;
+};
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
+    using S_ = MassShape<D, ROWS>;
+    constexpr int NST = S_::kStages, kBoxes = D / 64, C = D / 8, kAtom = ROWS * 128;
+    extern __shared__ char dyn[];
+    char *sq = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = sq + S_::kQ;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2], b_free[2], b_q, b_seg;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_gave_up;
+    __shared__ Share s_share;
+    __shared__ alignas(16) float s_nl[ROWS];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const Waits wait{&s_gave_up};
+    if (warp == 0) {
+        const Share s = find_share(a, 1 << 30, lane, blockIdx.x, gridDim.x);
+        if (lane == 0) s_share = s;
+    } else if (warp == 9) {
+        tmem_alloc(&s_tmem, 512);
+    } else if (tid == 256) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(b_empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_s + i, 1);
+            mbar_init(b_free + i, 128);
+        }
+        mbar_init(&b_q, 256);
+        mbar_init(&b_seg, 256);
+        s_gave_up = 0;
+        fence_mbar_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    Walk w(a, 1 << 30, s_share);
+
+    if (warp == 8) {  // ---------------------------------------------------------------- loads
+        uint32_t n = 0;
+        while (w.next()) {
+            for (int t = w.ta; t < w.tb; ++t, ++n) {
+                const int st = n % NST;
+                wait(b_empty + st, (n / NST & 1) ^ 1);
+                if (lane == 0) {
+                    mbar_expect_tx(b_full + st, S_::kStage);
+#pragma unroll
+                    for (int x = 0; x < kBoxes; ++x) tma_load(ring + st * S_::kStage + x * 16384, &mk, 64 * x, t * kTile, w.u, w.b, b_full + st);
+                }
+            }
+            w.advance();
+        }
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+    } else if (warp == 9) {  // ----------------------------------------------------------- MMAs
+        uint32_t n = 0, seg = 0, c_free[2] = {0, 0};
+        while (w.next()) {
+            const int rows = w.n * a.gc;
+            wait(&b_q, seg & 1);
+            tc_fence_after();
+            for (int t = w.ta; t < w.tb; ++t, ++n) {
+                const int st = n % NST, s = (t - w.ta) & 1;
+                wait(b_full + st, n / NST & 1);
+                for (int r0 = 0; r0 < rows; r0 += 256) {
+                    wait(b_free + s, (c_free[s]++ & 1) ^ 1);
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t ka = smem_u32(ring + st * S_::kStage), qa = smem_u32(sq) + r0 * 128;
+                        const uint32_t id = idesc_of<T>((min(rows - r0, 256) + 15) / 16 * 16, false);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            mma_ss(tmem + 256 * s, desc_rows(ka + (kk / 4) * 16384 + (kk % 4) * 32), desc_rows(qa + (kk / 4) * kAtom + (kk % 4) * 32), id, kk != 0);
+                        if (r0 + 256 >= rows) umma_commit(b_empty + st);
+                        umma_commit(b_s + s);
+                    }
+                    __syncwarp();
+                }
+            }
+            ++seg;
+            w.advance();
+        }
+    } else {  // -------------------------------------------------------------------------- sums
+        const int s = warp / 4, r = tid & 127;
+        const uint32_t tS = tmem + 256 * s + ((uint32_t)(warp & 3) << 21);
+        const float c = a.scale * 1.4426950408889634f;
+        uint32_t seg = 0, c_s = 0;
+        while (w.next()) {
+            const int rows = w.n * a.gc, h = w.u;
+            for (int i = tid; i < (rows + 15) / 16 * 16 * C; i += 256) {
+                const int ch = i % C, row = i / C;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                float nl = -INFINITY;
+                if (row < rows) {
+                    const int k = row / a.gc, head = h * a.group + a.g0 + row - k * a.gc;
+                    const int src = a.rows ? a.rows[(long long)w.b * a.tokens + k] : k;
+                    if (src < 0 || src >= a.tokens) {
+                        if (ch == 0) atomicOr(&g_cache_error, kErrRange);
+                    } else {
+                        const float lse = a.lse_in[((long long)w.b * a.tokens + src) * a.heads + head];
+                        if (lse != -INFINITY) {
+                            nl = lse * -1.4426950408889634f;
+                            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + w.b * a.qs[0] + src * a.qs[1] + (long long)head * a.qs[2] + ch * 8);
+                        }
+                    }
+                }
+                *reinterpret_cast<uint4 *>(sq + (ch / 8) * kAtom + row * 128 + (((ch % 8) ^ (row % 8)) * 16)) = v;
+                if (ch == 0) s_nl[row] = nl;
+            }
+            fence_proxy_async();
+            mbar_arrive(&b_q);
+            wait(&b_q, seg & 1);  // s_nl is there
+            const float *min_ = a.mass + w.b * a.ms[0] + h * a.ms[1];
+            float *mout = a.mass_out + w.b * a.mos[0] + h * a.mos[1];
+            for (int t = w.ta + s; t < w.tb; t += 2) {
+                const int key = t * kTile + r, late = key - w.len;
+                const bool tail = t * kTile + kTile > w.len;
+                float before = 0.f;
+                if (late < 0) before = min_[key];
+                else if (a.more && late < w.n) before = mout[key];
+                const int from = late > 0 ? (late < w.n ? late * a.gc : rows) : 0;  // the first row that sees the slot
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int r0 = 0; r0 < rows; r0 += 256) {
+                    wait(b_s + s, c_s++ & 1);
+                    tc_fence_after();
+                    const int cnt = min(rows - r0, 256);
+#pragma unroll 1
+                    for (int j = 0; j < cnt; j += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(tS + j, x);
+                        tmem_wait_ld(x);
+                        const float4 *nl = reinterpret_cast<const float4 *>(s_nl + r0 + j);
+                        if (tail || j + 32 > cnt) {
+                            const int lo = from - r0 - j, hi = cnt - j;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                const float p = ex2(fmaf(__uint_as_float(x[k]), c, k < hi ? s_nl[r0 + j + k] : 0.f));
+                                sum[k & 3] += k >= lo && k < hi ? p : 0.f;
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const float4 n4 = nl[k];
+                                sum[0] += ex2(fmaf(__uint_as_float(x[4 * k]), c, n4.x));
+                                sum[1] += ex2(fmaf(__uint_as_float(x[4 * k + 1]), c, n4.y));
+                                sum[2] += ex2(fmaf(__uint_as_float(x[4 * k + 2]), c, n4.z));
+                                sum[3] += ex2(fmaf(__uint_as_float(x[4 * k + 3]), c, n4.w));
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    mbar_arrive(b_free + s);
+                }
+                if (late < w.n) mout[key] = before + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            }
+            mbar_arrive(&b_seg);  // both groups have seen all of the segment's scores: its query rows are done with
+            wait(&b_seg, seg & 1);
+            ++seg;
+            w.advance();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// host side
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {  // from the driver, so that the library does not link against it
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+// 64 columns x 128 slots of one head, in the 128-byte swizzle; slots behind the last read as zero
+bool cache_map(CUtensorMap *m, const p8_kv *c, const void *base, const int64_t *st) {
+    const EncodeTiled f = encode_tiled();
+    if (!f) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c->width, (cuuint64_t)c->slots, (cuuint64_t)c->heads, (cuuint64_t)c->batch};
+    // the stride of a dimension of one is never used, but has to be a valid one
+    const cuuint64_t row = (cuuint64_t)c->width * 2;
+    const cuuint64_t strides[3] = {c->slots > 1 ? (cuuint64_t)st[3] * 2 : row, c->heads > 1 ? (cuuint64_t)st[2] * 2 : row, c->batch > 1 ? (cuuint64_t)st[1] * 2 : row};
+    const cuuint32_t box[4] = {64, kTile, 1, 1}, one[4] = {1, 1, 1, 1};
+    return f(m, c->type == P8_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool TWO>
+void allow_attn() {
+    cudaFuncSetAttribute(k_tree_attn_tc<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<D, TWO>::kSmem);
+}
+template <typename T, int D>
+void allow() {
+    allow_attn<T, D, false>();
+    allow_attn<T, D, true>();
+    cudaFuncSetAttribute(k_attn_mass_tc<T, D, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 256>::kSmem);
+    cudaFuncSetAttribute(k_attn_mass_tc<T, D, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 512>::kSmem);
+}
+// SM count of the current device; the first call on a device raises the kernels' shared-memory limits there
+int sm_count() {
+    static std::atomic<int> n[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int v = n[dev].load(std::memory_order_acquire);
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
+        allow<__half, 64>();
+        allow<__half, 128>();
+        allow<__nv_bfloat16, 64>();
+        allow<__nv_bfloat16, 128>();
+        n[dev].store(v, std::memory_order_release);
+    }
+    return v;
+}
+
+bool two_tiles(int64_t rows) { return rows > 128; }
+// CTAs of a call: no more than there can be tiles
+int tc_ctas(const p8_kv *c, int64_t rows, int rblock) {
+    const int64_t tiles = c->batch * c->heads * ((rows + rblock - 1) / rblock) * ((c->slots + kTile - 1) / kTile);
+    return (int)std::min<int64_t>(sm_count(), tiles);
+}
+
+size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {
+    if (c->type == P8_KV_F32) return 0;
+    // two parts a CTA, each with the rows' two statistics
+    const int64_t rows = tokens * (heads / c->heads);
+    const int R = two_tiles(rows) ? 256 : 128;
+    return (size_t)2 * tc_ctas(c, rows, R) * R * ((size_t)c->width * 4 + 8);
+}
+
+template <typename T, int D, bool TWO>
+p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
+    constexpr int R = TcShape<D, TWO>::kRows;
+    CUtensorMap mk, mv;
+    if (!cache_map(&mk, c, c->k, c->k_stride) || !cache_map(&mv, c, c->v, c->v_stride)) return P8_ERR_CUDA;
+    const int ctas = tc_ctas(c, (int64_t)a.tokens * a.group, R);
+    float *po = static_cast<float *>(ws);
+    float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * R * D);
+    k_tree_attn_tc<T, D, TWO><<<ctas, 320, TcShape<D, TWO>::kSmem, st>>>(a, mk, mv, po, ml);
+    if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned int)(((long long)a.batch * a.tokens * a.heads + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_attn_join<T, D>, a, R, ctas, Half16<T>::kLift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+}
+template <typename T, int D>
+p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
+    return two_tiles((int64_t)a.tokens * a.group) ? run_tc<T, D, true>(c, a, ws, st) : run_tc<T, D, false>(c, a, ws, st);
+}
+template <typename T, int D>
+p8_status run_mass_tc(const p8_kv *c, AttnArgs a, cudaStream_t st) {
+    CUtensorMap mk;
+    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
+    const int ctas = tc_ctas(c, 1, 1 << 30), most = 512 / a.tokens;
+    for (a.g0 = 0; a.g0 < a.group; a.g0 += a.gc) {  // at most 512 rows a launch; the later ones add to the first one's sums
+        a.gc = std::min(most, a.group - a.g0);
+        a.more = a.g0 > 0;
+        if (a.more) {
+            a.mass = a.mass_out;
+            for (int i = 0; i < 2; ++i) a.ms[i] = a.mos[i];
+        }
+        if (a.tokens * a.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(a, mk);
+        else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(a, mk);
+        if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
+    }
+    return P8_OK;
+}
+template <typename T>
+p8_status run16(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cudaStream_t st) {
+    if (c->width == 128) return mass ? run_mass_tc<T, 128>(c, a, st) : run_tc<T, 128>(c, a, ws, st);
+    return mass ? run_mass_tc<T, 64>(c, a, st) : run_tc<T, 64>(c, a, ws, st);
+}
 
 template <typename T>
 void run_attn(const p8_kv *c, const AttnArgs &a, bool mass, cudaStream_t st) {
@@ -156,20 +1101,20 @@ void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, in
     x.group = (int)(heads / c->heads);
 }
 
-p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, cudaStream_t st) {
-    if (c->type == P8_KV_F32) run_attn<float>(c, x, mass, st);
-    else if (c->type == P8_KV_F16) run_attn<__half>(c, x, mass, st);
-    else run_attn<__nv_bfloat16>(c, x, mass, st);
+p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
+    if (c->type == P8_KV_F16) return run16<__half>(c, x, mass, ws, st);
+    if (c->type == P8_KV_BF16) return run16<__nv_bfloat16>(c, x, mass, ws, st);
+    run_attn<float>(c, x, mass, st);
     return cudaGetLastError() == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 
-p8_status launch_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *, cudaStream_t st) {
+p8_status launch_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *ws, cudaStream_t st) {
     AttnArgs x;
     base_args(x, c, a->q, a->q_stride, a->tokens, a->heads);
     x.lens = a->lens; x.counts = a->counts; x.mask = (const unsigned long long *)a->mask; x.mask_stride = a->mask_stride;
     x.scale = (float)a->scale; x.out = a->out; x.lse = a->lse;
     for (int i = 0; i < 3; ++i) x.os[i] = a->out_stride[i];
-    return launch_attn(c, x, false, st);
+    return launch_attn(c, x, false, ws, st);
 }
 
 p8_status launch_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, cudaStream_t st) {
@@ -178,5 +1123,5 @@ p8_status launch_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, cudaStrea
     x.lens = a->lens; x.counts = a->counts; x.rows = a->rows; x.lse_in = a->lse; x.scale = (float)a->scale;
     x.mass = a->mass; x.mass_out = a->out;
     for (int i = 0; i < 2; ++i) { x.ms[i] = a->mass_stride[i]; x.mos[i] = a->out_stride[i]; }
-    return launch_attn(c, x, true, st);
+    return launch_attn(c, x, true, nullptr, st);
 }
