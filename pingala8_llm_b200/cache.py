@@ -20,7 +20,6 @@ Every call goes through the C ABI of libpingala8_b200.so on the tensors' device,
 given; there is no CPU path and no gradient. Lengths, counts, positions and rows that are out of range leave their
 sequence or token out and set bit 64 of device_error().
 """
-import ctypes as C
 import struct
 from collections import namedtuple
 
@@ -41,74 +40,101 @@ _ACCEPT = struct.Struct("=10q")
 Accepted = namedtuple("Accepted", "path accepted next_token new_lens")
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _refuse(what):
+    raise ValueError(what)
 
 
-def _kv(k, v, layers):
-    """the packed p8_kv of a cache, and (layers, batch, heads, slots, width)"""
-    _need(k.is_cuda and k.dtype in _TYPES, "the cache must be float32, float16 or bfloat16 CUDA tensors")
-    nd = k.dim()
-    _need(nd == 4 or (layers and nd == 5), "the cache must be [batch, kv heads, slots, width]" + (" or [layers, ...] of it" if layers else ""))
-    ks = k.stride()
-    _need(ks[-1] == 1, "the cache's last dimension must have unit stride")
-    shape = tuple(k.shape) if nd == 5 else (1, *k.shape)
-    if nd == 4:
-        ks = (0, *ks)
-    vp, vs = 0, ks
+# A decode step makes several of these calls per layer, and their checks are most of a small call's time on the host:
+# each is one comparison of what torch hands out cheapest, and words are put together only for an error.
+def _kv(k, v):
+    """(packed p8_kv, shape) of one layer's cache"""
+    if not k.is_cuda or k.dtype not in _TYPES:
+        _refuse("the cache must be float32, float16 or bfloat16 CUDA tensors")
+    shape = k.shape
+    if len(shape) != 4:
+        _refuse(f"the cache must be [batch, kv heads, slots, width], not {list(shape)}")
+    a, b, c, d = vs = k.stride()
+    vp = 0
     if v is not None:
-        _need(v.shape == k.shape and v.dtype == k.dtype and v.device == k.device, "keys and values must have one shape, type and device")
+        if v.shape != shape or v.dtype is not k.dtype or v.get_device() != k.get_device():
+            _refuse("keys and values must have one shape, type and device")
         vs = v.stride()
-        _need(vs[-1] == 1, "the cache's last dimension must have unit stride")
-        if nd == 4:
-            vs = (0, *vs)
         vp = v.data_ptr()
-    return _KV.pack(k.data_ptr(), vp, _TYPES[k.dtype], *shape, *ks[:4], *vs[:4]), shape
+    if d != 1 or vs[3] != 1:
+        _refuse("the cache's last dimension must have unit stride")
+    return _KV.pack(k.data_ptr(), vp, _TYPES[k.dtype], 1, *shape, 0, a, b, c, 0, vs[0], vs[1], vs[2]), shape
 
 
-def _ints(t, shape, dtype, dev, name):
-    _need(t.dtype == dtype and tuple(t.shape) == shape and t.is_contiguous() and t.device == dev, f"{name} must be contiguous {dtype} {list(shape)} on the cache's device")
-    return t.data_ptr()
+def _kv_layers(k, v):
+    """(packed p8_kv, shape with layers) of a cache with or without a layer dimension"""
+    if k.dim() == 4:
+        kv, shape = _kv(k, v)
+        return kv, (1, *shape)
+    if not k.is_cuda or k.dtype not in _TYPES:
+        _refuse("the cache must be float32, float16 or bfloat16 CUDA tensors")
+    shape = k.shape
+    if len(shape) != 5:
+        _refuse(f"the cache must be [batch, kv heads, slots, width] or [layers, batch, kv heads, slots, width], not {list(shape)}")
+    if v.shape != shape or v.dtype is not k.dtype or v.get_device() != k.get_device():
+        _refuse("keys and values must have one shape, type and device")
+    ks, vs = k.stride(), v.stride()
+    if ks[4] != 1 or vs[4] != 1:
+        _refuse("the cache's last dimension must have unit stride")
+    return _KV.pack(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], *shape, *ks[:4], *vs[:4]), shape
+
+
+def _flat(t, shape, dtype, dev, name):
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(f"{name} must be contiguous {dtype} {list(shape)} on the cache's device")
 
 
 def _rows(t, shape, dtype, dev, name):
     """pointer and the three outer strides of [batch, tokens, heads, width]"""
-    _need(t.dtype == dtype and tuple(t.shape) == shape and t.device == dev, f"{name} must be {dtype} {list(shape)} on the cache's device")
-    st = t.stride()
-    _need(st[3] == 1, f"{name}'s last dimension must have unit stride")
-    return t.data_ptr(), st[0], st[1], st[2]
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev:
+        a, b, c, d = t.stride()
+        if d == 1:
+            return t.data_ptr(), a, b, c
+    _refuse(f"{name} must be {dtype} {list(shape)} with unit stride in its last dimension, on the cache's device")
 
 
-class _On:
-    """Makes the tensors' device (and, where the caller gave one, the stream) current, for the launch and for what the
-    call allocates."""
+def _query(q, k, shape):
+    """pointer and strides of q [batch, tokens, heads, width] beside a cache of this shape, tokens, heads"""
+    if q.dim() != 4:
+        _refuse("q must be [batch, tokens, heads, width]")
+    _, T, H, _ = q.shape
+    if not 1 <= T <= TREE_MAX or H % shape[1] or not H:
+        _refuse(f"1 to {TREE_MAX} tokens, and query heads in whole groups")
+    return _rows(q, (shape[0], T, H, shape[3]), k.dtype, k.get_device(), "q"), T, H
 
-    def __init__(self, dev, stream):
-        self.dev, self.stream, self.ctx = dev, stream, None
 
-    def __enter__(self):
-        if self.stream is not None:
-            _need(self.stream.device == self.dev, "the stream must belong to the cache's device")
-            self.ctx = torch.cuda.stream(self.stream)
-        elif torch.cuda.current_device() != self.dev.index:
-            self.ctx = torch.cuda.device(self.dev)
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return C.c_void_p(torch._C._cuda_getCurrentRawStream(self.dev.index))
+_here = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    def __exit__(self, *e):
-        if self.ctx is not None:
-            self.ctx.__exit__(*e)
+
+def _on(dev, stream, call, *args):
+    """call(*args) with the tensors' device, and the stream where the caller gave one, current: for the launch, and for
+    what the call allocates"""
+    if stream is not None:
+        if stream.device.index != dev:
+            _refuse("the stream must belong to the cache's device")
+        with torch.cuda.stream(stream):
+            return call(*args)
+    if _here() != dev:
+        with torch.cuda.device(dev):
+            return call(*args)
+    return call(*args)
 
 
 def tree_plan(parents):
     """Ancestor bits and depths of drafted trees: parents int [tokens] or [batch, tokens] (parents[t] < t is the token
     that t hangs on, -1 for a root) -> (mask int64, depth int32) of the same shape. Bit j of mask[t]: t is j or hangs on
     it. Torch operations on the tensor's own device; for a fixed tree it is done once."""
-    _need(parents.dtype in (torch.int32, torch.int64) and parents.dim() in (1, 2), "parents must be int32 or int64 [tokens] or [batch, tokens]")
+    if parents.dtype not in (torch.int32, torch.int64) or parents.dim() not in (1, 2):
+        _refuse("parents must be int32 or int64 [tokens] or [batch, tokens]")
     n = parents.shape[-1]
-    _need(1 <= n <= TREE_MAX, f"a tree has 1 to {TREE_MAX} tokens")
+    if not 1 <= n <= TREE_MAX:
+        _refuse(f"a tree has 1 to {TREE_MAX} tokens")
     t = torch.arange(n, device=parents.device)
     root = parents < 0
     mask = (torch.ones_like(t) << t).expand(parents.shape).clone()
@@ -130,28 +156,28 @@ def kv_append(q, k, v, k_cache, v_cache, lens, pos, cos, sin, q_norm=None, k_nor
 
     pos int32 [batch, tokens]: each token's row of cos / sin float32 [positions, width / 2] (rotate-half form). q_norm,
     k_norm float32 [width]: RMSNorm per head before the rotation. Any number of tokens up to the cache's slots."""
-    kv, (_, B, hk, _, D) = _kv(k_cache, v_cache, False)
-    dev = k_cache.device
-    _need(q.dim() == 4 and cos.dim() == 2, "q must be [batch, tokens, heads, width], cos [positions, width / 2]")
-    T, H = q.shape[1], q.shape[2]
-    f32 = torch.float32
-    qp = _rows(q, (B, T, H, D), f32, dev, "q")
-    kp = _rows(k, (B, T, hk, D), f32, dev, "k")
-    vp = _rows(v, (B, T, hk, D), f32, dev, "v")
+    kv, (B, hk, _, D) = _kv(k_cache, v_cache)
+    dev = k_cache.get_device()
+    if q.dim() != 4 or cos.dim() != 2:
+        _refuse("q must be [batch, tokens, heads, width], cos [positions, width / 2]")
+    _, T, H, _ = q.shape
     P = cos.shape[0]
-    i32 = torch.int32
-    cp, sp = _ints(cos, (P, D // 2), f32, dev, "cos"), _ints(sin, (P, D // 2), f32, dev, "sin")
-    lp, pp = _ints(lens, (B,), i32, dev, "lens"), _ints(pos, (B, T), i32, dev, "pos")
-    np_ = _ints(counts, (B,), i32, dev, "counts") if counts is not None else 0
-    qn = _ints(q_norm, (D,), f32, dev, "q_norm") if q_norm is not None else 0
-    kn = _ints(k_norm, (D,), f32, dev, "k_norm") if k_norm is not None else 0
-    with _On(dev, stream) as st:
+    f32, i32 = torch.float32, torch.int32
+    qp, q0, q1, q2 = _rows(q, (B, T, H, D), f32, dev, "q")
+    kp, k0, k1, k2 = _rows(k, (B, T, hk, D), f32, dev, "k")
+    vp, v0, v1, v2 = _rows(v, (B, T, hk, D), f32, dev, "v")
+    tail = (_flat(lens, (B,), i32, dev, "lens"), 0 if counts is None else _flat(counts, (B,), i32, dev, "counts"), _flat(pos, (B, T), i32, dev, "pos"),
+            _flat(cos, (P, D // 2), f32, dev, "cos"), _flat(sin, (P, D // 2), f32, dev, "sin"), P,
+            0 if q_norm is None else _flat(q_norm, (D,), f32, dev, "q_norm"), 0 if k_norm is None else _flat(k_norm, (D,), f32, dev, "k_norm"), eps)
+
+    def call(q_out):
         if q_out is None:
-            q_out = (torch.empty if counts is None else torch.zeros)(B, T, H, D, dtype=k_cache.dtype, device=dev)
-        op = _rows(q_out, (B, T, H, D), k_cache.dtype, dev, "q_out")
-        a = _APPEND.pack(qp[0], kp[0], vp[0], *qp[1:], *kp[1:], *vp[1:], T, H, lp, np_, pp, cp, sp, P, qn, kn, float(eps), *op)
-        check(lib().p8_kv_append(kv, a, st), "p8_kv_append")
-    return q_out
+            q_out = (torch.empty if counts is None else torch.zeros)(B, T, H, D, dtype=k_cache.dtype, device=k_cache.device)
+        a = _APPEND.pack(qp, kp, vp, q0, q1, q2, k0, k1, k2, v0, v1, v2, T, H, *tail, *_rows(q_out, (B, T, H, D), k_cache.dtype, dev, "q_out"))
+        check(lib().p8_kv_append(kv, a, _raw_stream(dev)), "p8_kv_append")
+        return q_out
+
+    return _on(dev, stream, call, q_out)
 
 
 def tree_attention(q, k_cache, v_cache, lens, mask=None, counts=None, scale=None, out=None, lse=None, workspace=None, stream=None):
@@ -161,41 +187,38 @@ def tree_attention(q, k_cache, v_cache, lens, mask=None, counts=None, scale=None
     tokens whose bits mask[t] has (int64 [tokens] or [batch, tokens], as tree_plan makes it; None: a chain). Returns
     (out like q, lse float32 [batch, tokens, heads]): the softmax average of the values and the natural log of the sum
     of exponentials; 0 and -inf for a token that sees nothing. scale: 1 / sqrt(width) unless given."""
-    kv, (_, B, hk, _, D) = _kv(k_cache, v_cache, False)
-    dev = k_cache.device
-    _need(q.dim() == 4, "q must be [batch, tokens, heads, width]")
-    T, H = q.shape[1], q.shape[2]
-    qp = _rows(q, (B, T, H, D), k_cache.dtype, dev, "q")
-    _need(1 <= T <= TREE_MAX and H % hk == 0 and H > 0, f"1 to {TREE_MAX} tokens, and query heads in whole groups")
-    i32 = torch.int32
-    lp = _ints(lens, (B,), i32, dev, "lens")
-    np_ = _ints(counts, (B,), i32, dev, "counts") if counts is not None else 0
-    mp, ms = 0, 0
+    kv, shape = _kv(k_cache, v_cache)
+    B = shape[0]
+    dev = k_cache.get_device()
+    (qp, q0, q1, q2), T, H = _query(q, k_cache, shape)
+    lp = _flat(lens, (B,), torch.int32, dev, "lens")
+    np_ = 0 if counts is None else _flat(counts, (B,), torch.int32, dev, "counts")
+    mp = ms = 0
     if mask is not None:
         ms = T if mask.dim() == 2 else 0
-        mp = _ints(mask, (B, T) if ms else (T,), torch.int64, dev, "mask")
-    if scale is None:
-        scale = D ** -0.5
-    with _On(dev, stream) as st:
+        mp = _flat(mask, (B, T) if ms else (T,), torch.int64, dev, "mask")
+
+    def call(out, lse, workspace):
         new = torch.empty if counts is None else torch.zeros
         if out is None:
-            out = new(B, T, H, D, dtype=q.dtype, device=dev)
+            out = new(q.shape, dtype=q.dtype, device=q.device)
         if lse is None:
-            lse = new(B, T, H, dtype=torch.float32, device=dev)
-        op = _rows(out, (B, T, H, D), q.dtype, dev, "out")
-        ep = _ints(lse, (B, T, H), torch.float32, dev, "lse")
+            lse = new((B, T, H), dtype=torch.float32, device=q.device)
         if workspace is None:
-            workspace = torch.empty(lib().p8_tree_attn_workspace(kv, T, H), dtype=torch.uint8, device=dev)
-        _need(workspace.device == dev and workspace.is_contiguous(), "workspace must be contiguous on the cache's device")
-        a = _ATTN.pack(*qp, T, H, lp, np_, mp, ms, float(scale), *op, ep)
-        check(lib().p8_tree_attn(kv, a, C.c_void_p(workspace.data_ptr()), workspace.numel() * workspace.element_size(), st), "p8_tree_attn")
-    return out, lse
+            workspace = torch.empty(lib().p8_tree_attn_workspace(kv, T, H), dtype=torch.uint8, device=q.device)
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            _refuse("workspace must be contiguous on the cache's device")
+        a = _ATTN.pack(qp, q0, q1, q2, T, H, lp, np_, mp, ms, shape[3] ** -0.5 if scale is None else scale,
+                       *_rows(out, q.shape, q.dtype, dev, "out"), _flat(lse, (B, T, H), torch.float32, dev, "lse"))
+        check(lib().p8_tree_attn(kv, a, workspace.data_ptr(), workspace.nbytes, _raw_stream(dev)), "p8_tree_attn")
+        return out, lse
+
+    return _on(dev, stream, call, out, lse, workspace)
 
 
 def attention_workspace_size(k_cache, tokens, heads):
     """workspace bytes of tree_attention on this cache, for callers that keep their own"""
-    kv, _ = _kv(k_cache, k_cache, False)
-    return int(lib().p8_tree_attn_workspace(kv, tokens, heads))
+    return int(lib().p8_tree_attn_workspace(_kv(k_cache, k_cache)[0], tokens, heads))
 
 
 def attention_mass(q, lse, k_cache, lens, mass, rows=None, counts=None, scale=None, out=None, stream=None):
@@ -205,27 +228,28 @@ def attention_mass(q, lse, k_cache, lens, mass, rows=None, counts=None, scale=No
     q, lse: as in the tree_attention call. rows int32 [batch, tokens]: the tokens' rows in q and lse (the accepted path,
     once tree_accept has moved its keys into place); None: 0, 1, 2, ... counts: how many tokens. The tokens' own slots
     start at 0. In place unless out is given."""
-    kv, (_, B, hk, S, D) = _kv(k_cache, None, False)
-    dev = k_cache.device
-    _need(q.dim() == 4, "q must be [batch, tokens, heads, width]")
-    T, H = q.shape[1], q.shape[2]
-    qp = _rows(q, (B, T, H, D), k_cache.dtype, dev, "q")
-    _need(1 <= T <= TREE_MAX and H % hk == 0 and H > 0, f"1 to {TREE_MAX} tokens, and query heads in whole groups")
+    kv, shape = _kv(k_cache, None)
+    B = shape[0]
+    dev = k_cache.get_device()
+    (qp, q0, q1, q2), T, H = _query(q, k_cache, shape)
     i32, f32 = torch.int32, torch.float32
-    lp = _ints(lens, (B,), i32, dev, "lens")
-    ep = _ints(lse, (B, T, H), f32, dev, "lse")
-    np_ = _ints(counts, (B,), i32, dev, "counts") if counts is not None else 0
-    rp = _ints(rows, (B, T), i32, dev, "rows") if rows is not None else 0
     if out is None:
         out = mass
+    ms = []
     for t in (mass, out):
-        _need(t.dtype == f32 and tuple(t.shape) == (B, hk, S) and t.stride(2) == 1 and t.device == dev, "mass and out must be float32 [batch, kv heads, slots] with unit slot stride on the cache's device")
-    if scale is None:
-        scale = D ** -0.5
-    with _On(dev, stream) as st:
-        a = _MASS.pack(*qp, T, H, ep, lp, np_, rp, float(scale), mass.data_ptr(), mass.stride(0), mass.stride(1), out.data_ptr(), out.stride(0), out.stride(1))
-        check(lib().p8_attn_mass(kv, a, st), "p8_attn_mass")
-    return out
+        st = t.stride()
+        if t.dtype is not f32 or t.shape != shape[:3] or st[2] != 1 or t.get_device() != dev:
+            _refuse("mass and out must be float32 [batch, kv heads, slots] with unit slot stride on the cache's device")
+        ms += (t.data_ptr(), st[0], st[1])
+    a = _MASS.pack(qp, q0, q1, q2, T, H, _flat(lse, (B, T, H), f32, dev, "lse"), _flat(lens, (B,), i32, dev, "lens"),
+                   0 if counts is None else _flat(counts, (B,), i32, dev, "counts"), 0 if rows is None else _flat(rows, (B, T), i32, dev, "rows"),
+                   shape[3] ** -0.5 if scale is None else scale, *ms)
+
+    def call():
+        check(lib().p8_attn_mass(kv, a, _raw_stream(dev)), "p8_attn_mass")
+        return out
+
+    return _on(dev, stream, call)
 
 
 def kv_evict(k_cache, v_cache, mass, lens, budget, sinks=0, recent=0, k_out=None, v_out=None, mass_out=None, new_lens=None, kept=None, stream=None):
@@ -235,34 +259,40 @@ def kv_evict(k_cache, v_cache, mass, lens, budget, sinks=0, recent=0, k_out=None
     Cache [layers, batch, kv heads, slots, width] or without layers, mass float32 of its first dimensions. The kept
     slots go to the front of k_out, v_out and mass_out (other buffers, budget slots or more; give all three), or of the
     cache itself. Returns (new_lens int32 [batch], kept int32 [..., kv heads, budget]: the kept slots, -1 behind them)."""
-    kv, (N, B, hk, S, D) = _kv(k_cache, v_cache, True)
-    dev = k_cache.device
+    kv, (N, B, hk, S, D) = _kv_layers(k_cache, v_cache)
+    dev = k_cache.get_device()
     place = k_out is None
-    _need((v_out is None) == place and (mass_out is None) == place, "give k_out, v_out and mass_out together")
+    if (v_out is None) != place or (mass_out is None) != place:
+        _refuse("give k_out, v_out and mass_out together")
     if place:
         kv2, S2, mass_out = kv, S, mass
     else:
-        _need(k_out.dim() == k_cache.dim() and k_out.dtype == k_cache.dtype and k_out.device == dev, "k_out must have the cache's dimensions, type and device")
-        kv2, shape = _kv(k_out, v_out, True)
+        if k_out.dim() != k_cache.dim() or k_out.dtype is not k_cache.dtype:
+            _refuse("k_out must have the cache's dimensions and type")
+        kv2, shape = _kv_layers(k_out, v_out)
         S2 = shape[3]
-        _need(shape == (N, B, hk, S2, D), "k_out must have the cache's shape but for its slots")
+        if tuple(shape) != (N, B, hk, S2, D) or k_out.get_device() != dev:
+            _refuse("k_out must have the cache's shape but for its slots, on its device")
     budget = int(budget)
     lead = k_cache.shape[:-2]
     ms = []
     for t, s in ((mass, S), (mass_out, S2)):
-        _need(t.dtype == torch.float32 and tuple(t.shape) == (*lead, s) and t.stride(-1) == 1 and t.device == dev, "mass must be float32 [.., kv heads, slots] of the cache with unit slot stride")
         st = t.stride()
-        ms.append((st[0], st[1], st[2]) if len(lead) == 3 else (0, st[0], st[1]))
-    i32 = torch.int32
-    lp = _ints(lens, (B,), i32, dev, "lens")
-    with _On(dev, stream) as st:
+        if t.dtype is not torch.float32 or t.shape != (*lead, s) or st[-1] != 1 or t.get_device() != dev:
+            _refuse("mass must be float32 [.., kv heads, slots] of the cache with unit slot stride, on its device")
+        ms += (t.data_ptr(), *(st[:3] if len(lead) == 3 else (0, *st[:2])))
+    lp = _flat(lens, (B,), torch.int32, dev, "lens")
+
+    def call(new_lens, kept):
         if new_lens is None:
             new_lens = torch.empty_like(lens)
         if kept is None:
-            kept = torch.empty(*lead, max(budget, 0), dtype=i32, device=dev)
-        a = _EVICT.pack(mass.data_ptr(), *ms[0], mass_out.data_ptr(), *ms[1], lp, _ints(new_lens, (B,), i32, dev, "new_lens"), _ints(kept, (*lead, budget), i32, dev, "kept"), budget, int(sinks), int(recent))
-        check(lib().p8_kv_evict(kv, kv2, a, st), "p8_kv_evict")
-    return new_lens, kept
+            kept = torch.empty(*lead, max(budget, 0), dtype=torch.int32, device=k_cache.device)
+        a = _EVICT.pack(*ms, lp, _flat(new_lens, (B,), torch.int32, dev, "new_lens"), _flat(kept, (*lead, budget), torch.int32, dev, "kept"), budget, sinks, recent)
+        check(lib().p8_kv_evict(kv, kv2, a, _raw_stream(dev)), "p8_kv_evict")
+        return new_lens, kept
+
+    return _on(dev, stream, call, new_lens, kept)
 
 
 def tree_accept(tokens, parents, target, k_cache, v_cache, lens, counts=None, path=None, accepted=None, next_token=None, new_lens=None, stream=None):
@@ -273,24 +303,27 @@ def tree_accept(tokens, parents, target, k_cache, v_cache, lens, counts=None, pa
 
     Returns Accepted(path int32 [batch, tokens] (-1 behind it), accepted int32 [batch] its length, next_token int64
     [batch] the target at its end, new_lens int32 [batch])."""
-    kv, (_, B, _, _, _) = _kv(k_cache, v_cache, True)
-    dev = k_cache.device
-    _need(tokens.dim() == 2 and 1 <= tokens.shape[1] <= TREE_MAX, f"tokens must be [batch, 1 to {TREE_MAX}]")
+    kv, (_, B, _, _, _) = _kv_layers(k_cache, v_cache)
+    dev = k_cache.get_device()
+    if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= TREE_MAX:
+        _refuse(f"tokens must be [batch, 1 to {TREE_MAX}]")
     T = tokens.shape[1]
     i32, i64 = torch.int32, torch.int64
-    tp, gp, pp = _ints(tokens, (B, T), i64, dev, "tokens"), _ints(target, (B, T), i64, dev, "target"), _ints(parents, (B, T), i32, dev, "parents")
-    lp = _ints(lens, (B,), i32, dev, "lens")
-    np_ = _ints(counts, (B,), i32, dev, "counts") if counts is not None else 0
-    with _On(dev, stream) as st:
+    head = (_flat(tokens, (B, T), i64, dev, "tokens"), _flat(target, (B, T), i64, dev, "target"), _flat(parents, (B, T), i32, dev, "parents"), T,
+            _flat(lens, (B,), i32, dev, "lens"), 0 if counts is None else _flat(counts, (B,), i32, dev, "counts"))
+
+    def call(path, accepted, next_token, new_lens):
         if path is None:
-            path = torch.empty(B, T, dtype=i32, device=dev)
+            path = torch.empty((B, T), dtype=i32, device=k_cache.device)
         if accepted is None:
-            accepted = torch.empty(B, dtype=i32, device=dev)
+            accepted = torch.empty_like(lens)
         if next_token is None:
-            next_token = torch.empty(B, dtype=i64, device=dev)
+            next_token = torch.empty(B, dtype=i64, device=k_cache.device)
         if new_lens is None:
-            new_lens = torch.empty(B, dtype=i32, device=dev)
-        a = _ACCEPT.pack(tp, gp, pp, T, lp, np_, _ints(path, (B, T), i32, dev, "path"), _ints(accepted, (B,), i32, dev, "accepted"),
-                         _ints(new_lens, (B,), i32, dev, "new_lens"), _ints(next_token, (B,), i64, dev, "next_token"))
-        check(lib().p8_tree_accept(kv, a, st), "p8_tree_accept")
-    return Accepted(path, accepted, next_token, new_lens)
+            new_lens = torch.empty_like(lens)
+        a = _ACCEPT.pack(*head, _flat(path, (B, T), i32, dev, "path"), _flat(accepted, (B,), i32, dev, "accepted"),
+                         _flat(new_lens, (B,), i32, dev, "new_lens"), _flat(next_token, (B,), i64, dev, "next_token"))
+        check(lib().p8_tree_accept(kv, a, _raw_stream(dev)), "p8_tree_accept")
+        return Accepted(path, accepted, next_token, new_lens)
+
+    return _on(dev, stream, call, path, accepted, next_token, new_lens)
