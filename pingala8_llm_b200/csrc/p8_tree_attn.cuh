@@ -18,129 +18,14 @@ struct AttnArgs {
     float scale;
 };
 
-// One block per (sequence, cache head, eight query rows): a running maximum and sum over tiles of 32 slots, products on
-// the CUDA cores. Simple, and right for every type.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_tree_attn_plain(const AttnArgs a) {
-    constexpr int R = 8, KT = 32;
-    __shared__ float sq[R][D], sk[KT][D + 1], sp[R][KT], sv[KT][D];
-    __shared__ float s_m[R], s_l[R], s_c[R];
-    const int b = blockIdx.z, h = blockIdx.y, r0 = blockIdx.x * R, tid = threadIdx.x;
-    int len, n;
-    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
-        if (r0 == 0 && h == 0 && tid == 0) atomicOr(&g_cache_error, kErrRange);
-        return;
-    }
-    const int rows = n * a.group;
-    if (r0 >= rows) return;
-    for (int i = tid; i < R * D; i += 128) {
-        const int r = r0 + i / D;
-        sq[i / D][i % D] = r < rows ? to_f(static_cast<const T *>(a.q)[b * a.qs[0] + r / a.group * a.qs[1] + (h * a.group + r % a.group) * a.qs[2] + i % D]) : 0.f;
-    }
-    if (tid < R) { s_m[tid] = -INFINITY; s_l[tid] = 0.f; }
-    float acc[R] = {};
-    const int end = len + n;
-    const T *K = static_cast<const T *>(a.k) + b * a.ks[0] + h * a.ks[1], *V = static_cast<const T *>(a.v) + b * a.vs[0] + h * a.vs[1];
-    for (int j0 = 0; j0 < end; j0 += KT) {
-        __syncthreads();
-        for (int i = tid; i < KT * D; i += 128) {
-            const int j = j0 + i / D;
-            sk[i / D][i % D] = j < end ? to_f(K[j * a.ks[2] + i % D]) : 0.f;
-            sv[i / D][i % D] = j < end ? to_f(V[j * a.vs[2] + i % D]) : 0.f;
-        }
-        __syncthreads();
-        const int j = j0 + tid % KT;
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-            const int r = tid / KT * 2 + rr, t = (r0 + r) / a.group;
-            float s = 0.f;
-            for (int d = 0; d < D; ++d) s += sq[r][d] * sk[tid % KT][d];
-            bool see = r0 + r < rows && j < end;
-            if (see && j >= len) see = a.mask ? (a.mask[b * a.mask_stride + t] >> (j - len)) & 1 : j - len <= t;
-            s = see ? s * a.scale : -INFINITY;
-            float top = s;
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-            const float m0 = s_m[r], m1 = fmaxf(m0, top);
-            const float p = see ? expf(s - m1) : -1.f;
-            float sum = see ? p : 0.f;
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            __syncwarp();
-            sp[r][tid % KT] = p;
-            if (tid % KT == 0) {
-                s_c[r] = m1 == -INFINITY ? 1.f : expf(m0 - m1);
-                s_l[r] = s_l[r] * s_c[r] + sum;
-                s_m[r] = m1;
-            }
-        }
-        __syncthreads();
-        for (int r = 0; r < R; ++r) {
-            if (tid < D) {
-                float x = acc[r] * s_c[r];
-                for (int i = 0; i < KT; ++i)
-                    if (sp[r][i] >= 0.f || isnan(sp[r][i])) x += sp[r][i] * sv[i][tid];
-                acc[r] = x;
-            }
-        }
-    }
-    __syncthreads();
-    for (int r = 0; r < R && r0 + r < rows; ++r) {
-        const int t = (r0 + r) / a.group, i = h * a.group + (r0 + r) % a.group;
-        if (tid < D) static_cast<T *>(a.out)[b * a.os[0] + t * a.os[1] + i * a.os[2] + tid] = from_f<T>(s_m[r] == -INFINITY ? 0.f : acc[r] / s_l[r]);
-        if (a.lse && tid == 0) a.lse[((long long)b * a.tokens + t) * a.heads + i] = s_m[r] == -INFINITY ? -INFINITY : s_m[r] + logf(s_l[r]);
-    }
-}
-
-// One thread per slot: the query rows pass through shared memory, the slot's key stays in registers as it was read.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_attn_mass_plain(const AttnArgs a) {
-    __shared__ float sq[8][D], sl[8];
-    __shared__ int st[8];
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-    int len, n;
-    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
-        if (blockIdx.x == 0 && h == 0 && tid == 0) atomicOr(&g_cache_error, kErrRange);
-        return;
-    }
-    const int end = len + n;
-    const T *K = static_cast<const T *>(a.k) + b * a.ks[0] + h * a.ks[1];
-    for (int j0 = blockIdx.x * 128; j0 < end; j0 += gridDim.x * 128) {
-        const int j = j0 + tid;
-        float w = 0.f;
-        for (int r0 = 0; r0 < n * a.group; r0 += 8) {
-            __syncthreads();
-            for (int i = tid; i < 8 * D; i += 128) {
-                const int r = r0 + i / D, t = r / a.group;
-                int src = -1;
-                if (r < n * a.group) src = a.rows ? a.rows[b * a.tokens + t] : t;
-                if (src < -1 || src >= a.tokens || (src < 0 && r < n * a.group)) { atomicOr(&g_cache_error, kErrRange); src = -1; }
-                const int hq = h * a.group + r % a.group;
-                sq[i / D][i % D] = src >= 0 ? to_f(static_cast<const T *>(a.q)[b * a.qs[0] + src * a.qs[1] + hq * a.qs[2] + i % D]) : 0.f;
-                if (i % D == 0) {
-                    sl[i / D] = src >= 0 ? a.lse_in[((long long)b * a.tokens + src) * a.heads + hq] : -INFINITY;
-                    st[i / D] = t;
-                }
-            }
-            __syncthreads();
-            if (j < end)
-                for (int r = 0; r < 8; ++r) {
-                    if (sl[r] == -INFINITY || j > len + st[r]) continue;
-                    float s = 0.f;
-                    for (int d = 0; d < D; ++d) s += sq[r][d] * to_f(K[j * a.ks[2] + d]);
-                    w += expf(s * a.scale - sl[r]);
-                }
-        }
-        if (j < end) a.mass_out[b * a.mos[0] + h * a.mos[1] + j] = (j < len ? a.mass[b * a.ms[0] + h * a.ms[1] + j] : 0.f) + w;
-    }
-}
-
-// ================================================================================================================
-// 16-bit caches: tcgen05
-// ================================================================================================================
-// A unit is (sequence, cache head, block of query rows); its slots are cut into tiles of 128. All tiles of all units
+// A unit is (sequence, cache head, block of query rows); its slots are cut into tiles. All tiles of all units
 // form one list, sequence by sequence, and every CTA takes an equal contiguous share of it, so that the SMs finish
 // together whatever the lengths are, and one long sequence still fills them. A unit that lies in one share is finished
 // there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
-constexpr int kTile = 128;
+constexpr int kTile = 128;  // of a 16-bit cache; 64 of a 32-bit one (as many bytes)
+struct Cut {                // how a kernel cuts its work: query rows of a unit, slots of a tile
+    int rblock, tile;
+};
 
 struct Share {
     long long pos, end;  // the CTA's tiles
@@ -150,18 +35,18 @@ struct Share {
 
 struct Walk {            // a CTA's way through its share, one segment (the tiles of one unit) at a time
     const AttnArgs &a;
-    int rblock;
+    const Cut cut;
     long long pos, end, off;
     int b, len, n, nt, units, u, ta, tb;
     bool opens;          // the segment is the share's first
-    __device__ Walk(const AttnArgs &a_, int rb, const Share &s) : a(a_), rblock(rb), pos(s.pos), end(s.end), off(s.off), b(s.b) {
+    __device__ Walk(const AttnArgs &a_, Cut c, const Share &s) : a(a_), cut(c), pos(s.pos), end(s.end), off(s.off), b(s.b) {
         opens = true;
         if (pos < end) load();
     }
     __device__ void load() {
         if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
-        nt = n ? (len + n + kTile - 1) / kTile : 0;
-        units = n ? a.kvh * ((n * a.group + rblock - 1) / rblock) : 0;
+        nt = n ? (len + n + cut.tile - 1) / cut.tile : 0;
+        units = n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) : 0;
     }
     __device__ bool next() {
         if (pos >= end) return false;
@@ -182,17 +67,17 @@ struct Walk {            // a CTA's way through its share, one segment (the tile
     }
     __device__ int blocks() const { return units / a.kvh; }
     __device__ int head() const { return u / blocks(); }
-    __device__ int row0() const { return u % blocks() * rblock; }
+    __device__ int row0() const { return u % blocks() * cut.rblock; }
     __device__ bool whole() const { return ta == 0 && tb == nt; }
 };
 
-__device__ __forceinline__ long long seq_tiles(const AttnArgs &a, int rblock, int b, bool *bad) {
+__device__ __forceinline__ long long seq_tiles(const AttnArgs &a, Cut cut, int b, bool *bad) {
     int len, n;
     if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
         *bad = true;
         return 0;
     }
-    return n ? (long long)a.kvh * ((n * a.group + rblock - 1) / rblock) * ((len + n + kTile - 1) / kTile) : 0;
+    return n ? (long long)a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) * ((len + n + cut.tile - 1) / cut.tile) : 0;
 }
 __device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
@@ -208,15 +93,15 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {  // incl
     return v;
 }
 // tiles of all sequences (whole warp)
-__device__ __forceinline__ long long all_tiles(const AttnArgs &a, int rblock, int lane, bool *bad) {
+__device__ __forceinline__ long long all_tiles(const AttnArgs &a, Cut cut, int lane, bool *bad) {
     long long total = 0;
-    for (int b = lane; b < a.batch; b += 32) total += seq_tiles(a, rblock, b, bad);
+    for (int b = lane; b < a.batch; b += 32) total += seq_tiles(a, cut, b, bad);
     return warp_sum(total);
 }
 // the share of one CTA (whole warp)
-__device__ __forceinline__ Share find_share(const AttnArgs &a, int rblock, int lane, int cta, int ctas) {
+__device__ __forceinline__ Share find_share(const AttnArgs &a, Cut cut, int lane, int cta, int ctas) {
     bool bad = false;
-    const long long total = all_tiles(a, rblock, lane, &bad);
+    const long long total = all_tiles(a, cut, lane, &bad);
     if (bad && cta == 0) atomicOr(&g_cache_error, kErrRange);
     const long long each = (total + ctas - 1) / ctas;
     Share s;
@@ -226,7 +111,7 @@ __device__ __forceinline__ Share find_share(const AttnArgs &a, int rblock, int l
     s.off = 0;
     long long run = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const long long mine = b0 + lane < a.batch ? seq_tiles(a, rblock, b0 + lane, &bad) : 0;
+        const long long mine = b0 + lane < a.batch ? seq_tiles(a, cut, b0 + lane, &bad) : 0;
         const long long incl = run + warp_scan(mine, lane);
         const unsigned int hit = __ballot_sync(0xffffffffu, incl > s.pos);
         if (hit) {
@@ -413,7 +298,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, S_::kRows, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, Cut{S_::kRows, kTile}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
@@ -438,7 +323,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    Walk w(a, S_::kRows, s_share);
+    Walk w(a, Cut{S_::kRows, kTile}, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
@@ -739,7 +624,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
 // Adds up a unit's parts: one warp per query row; lanes find the largest maximum, then every lane sums its columns over
 // the parts in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, int rblock, int ctas, float lift, const float *part_o, const float2 *part_ml) {
+__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x % 32;
     const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
@@ -750,19 +635,19 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, int rblock,
     bool bad = false;
     long long total = 0, before = 0;
     for (int x = lane; x < a.batch; x += 32) {
-        const long long k = seq_tiles(a, rblock, x, &bad);
+        const long long k = seq_tiles(a, cut, x, &bad);
         total += k;
         before += x < b ? k : 0;
     }
     total = warp_sum(total);
     before = warp_sum(before);
     const long long each = (total + ctas - 1) / ctas;
-    const int blocks = (n * a.group + rblock - 1) / rblock, nt = (len + n + kTile - 1) / kTile;
+    const int blocks = (n * a.group + cut.rblock - 1) / cut.rblock, nt = (len + n + cut.tile - 1) / cut.tile;
     const int h = head / a.group, row = t * a.group + head % a.group;
-    const long long u0 = before + (long long)(h * blocks + row / rblock) * nt, u1 = u0 + nt;
+    const long long u0 = before + (long long)(h * blocks + row / cut.rblock) * nt, u1 = u0 + nt;
     const int c0 = (int)(u0 / each), c1 = (int)((u1 - 1) / each);
     if (c0 == c1) return;  // finished by that CTA
-    auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each != u0 ? 1 : 0)) * rblock + row % rblock; };
+    auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each != u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
     float m = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[at(c)].x);
 #pragma unroll
@@ -810,7 +695,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, 1 << 30, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, Cut{1 << 30, kTile}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
@@ -832,7 +717,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    Walk w(a, 1 << 30, s_share);
+    Walk w(a, Cut{1 << 30, kTile}, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
@@ -961,6 +846,447 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
+// ================================================================================================================
+// 32-bit caches: products of 32-bit values on the tensor cores
+// ================================================================================================================
+// x = hi + lo, both TF32 (8 + 11 bits): x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y|, three mma.sync products with
+// fp32 sums. (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
+// more shared-memory traffic than the products take. From registers the split costs three integer or fp32 operations.)
+__device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
+}
+__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+struct Frag {  // a 16 x 8 left operand in two pieces
+    uint32_t hi[4], lo[4];
+    __device__ __forceinline__ Frag(float x0, float x1, float x2, float x3) {
+        split(x0, hi[0], lo[0]);
+        split(x1, hi[1], lo[1]);
+        split(x2, hi[2], lo[2]);
+        split(x3, hi[3], lo[3]);
+    }
+};
+__device__ __forceinline__ void mma_split(float (&c)[4], const Frag &a, float b0, float b1) {
+    uint32_t h0, l0, h1, l1;
+    split(b0, h0, l0);
+    split(b1, h1, l1);
+    mma8(c, a.hi[0], a.hi[1], a.hi[2], a.hi[3], l0, l1);
+    mma8(c, a.lo[0], a.lo[1], a.lo[2], a.lo[3], h0, h1);
+    mma8(c, a.hi[0], a.hi[1], a.hi[2], a.hi[3], h0, h1);
+}
+constexpr int kTile32 = 64;
+// A stage holds 64 slots in parts of 32 columns as the tensor map's loads leave them: 128-byte rows, the 16-byte pieces
+// exchanged by the row's last three bits.
+__device__ __forceinline__ float4 stage32(const char *st, int slot, int col4) {  // columns 4 col4 ..
+    return *reinterpret_cast<const float4 *>(st + (col4 / 8) * 8192 + slot * 128 + ((col4 % 8) ^ (slot % 8)) * 16);
+}
+// Query rows: 16-byte pieces exchanged between the halves of 128 bytes in every other row (two rows are read at a time).
+template <int D>
+__device__ __forceinline__ float4 *query32(char *sq, int row, int col4) {
+    return reinterpret_cast<float4 *>(sq + row * (D * 4) + (col4 ^ ((row & 1) << 2)) * 16);
+}
+
+// RT row tiles of 16 x 8 / RT groups of slots: warp w has row tile w % RT and the slots of group w / RT in every tile,
+// with its own running maximum, sum and accumulator; the groups are joined at the segment's end. No barrier but the
+// ring's in between. Within the products the columns of K (and the slots in S and P) are taken in the order in which a
+// lane finds them in 16 consecutive bytes: the sums do not depend on it.
+// Bound by K and V from HBM for up to 16 rows, by the products beyond.
+template <int D, int RT>
+struct F32Shape {
+    static constexpr int kStage = kTile32 * D * 4;
+    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kQ = RT * 16 * D * 4, kJoin = (8 - RT) * 16 * D * 4;
+    static constexpr int kSmem = 1024 + kQ + kJoin + kStages * kStage;
+};
+
+template <int D, int RT>
+__global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                                                          float *part_o, float2 *part_ml) {
+    using S_ = F32Shape<D, RT>;
+    constexpr int NST = S_::kStages, KG = 8 / RT, NK = kTile32 / 8 / KG, R = RT * 16;  // NK: groups of eight slots of a warp
+    extern __shared__ char dyn[];
+    char *ring = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *sq = ring + NST * S_::kStage, *join = sq + S_::kQ;
+    __shared__ uint64_t b_full[NST], b_empty[NST];
+    __shared__ int s_gave_up;
+    __shared__ Share s_share;
+    __shared__ float2 s_ml[8][16];
+    __shared__ unsigned long long s_bad;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const Waits wait{&s_gave_up};
+    const Cut cut{R, kTile32};
+    if (warp == 0) {
+        const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
+        if (lane == 0) s_share = s;
+    } else if (tid == 256) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(b_empty + i, 8);
+        }
+        s_gave_up = 0;
+        s_bad = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    Walk w(a, cut, s_share);
+    if (warp == 8) {  // loads
+        uint32_t n = 0;
+        while (w.next()) {
+            for (int t = w.ta; t < w.tb; ++t)
+                for (int z = 0; z < 2; ++z, ++n) {
+                    const int st = n % NST;
+                    wait(b_empty + st, (n / NST & 1) ^ 1);
+                    if (lane == 0) {
+                        mbar_expect_tx(b_full + st, S_::kStage);
+#pragma unroll
+                        for (int x = 0; x < D / 32; ++x)
+                            tma_load(ring + st * S_::kStage + x * 8192, z ? &mv : &mk, 32 * x, t * kTile32, w.head(), w.b, b_full + st);
+                    }
+                }
+            w.advance();
+        }
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        return;
+    }
+    const int rt = warp % RT, kg = warp / RT, g = lane / 4, t = lane % 4;
+    const float c = a.scale * 1.4426950408889634f;
+    uint32_t n = 0;
+    while (w.next()) {
+        const int h = w.head(), row0 = w.row0(), rows = w.n * a.group;
+        const float *q = static_cast<const float *>(a.q) + w.b * a.qs[0];
+        for (int i = tid; i < R * (D / 4); i += 256) {
+            const int col4 = i % (D / 4), r = i / (D / 4), row = row0 + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < rows) {
+                const int tok = row / a.group;
+                v = *reinterpret_cast<const float4 *>(q + tok * a.qs[1] + (long long)(h * a.group + row - tok * a.group) * a.qs[2] + 4 * col4);
+                v.x *= c; v.y *= c; v.z *= c; v.w *= c;  // scores in base 2
+            }
+            *query32<D>(sq, r, col4) = v;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const bool warp_live = row0 + 16 * rt < rows;
+        unsigned long long sees[2] = {0, 0};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 32][4][4] = {};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int row = row0 + 16 * rt + g + 8 * y;
+            if (row < rows) {
+                const int tok = row / a.group;
+                sees[y] = a.mask ? a.mask[w.b * a.mask_stride + tok] : ~0ull >> (63 - tok);
+                if (w.n < 64) sees[y] &= (1ull << w.n) - 1;
+            }
+        }
+        for (int tile = w.ta; tile < w.tb; ++tile) {
+            const int key0 = tile * kTile32 + kg * NK * 8;  // the warp's first slot
+            const bool tail = key0 + NK * 8 > w.len;
+            float s[NK][4] = {};
+            const int sk = n % NST;
+            wait(b_full + sk, n / NST & 1);
+            ++n;
+            if (warp_live) {
+                const char *st = ring + sk * S_::kStage;
+                const int slot = kg * NK * 8 + (g >> 1) + ((g & 1) << 2);
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const float4 q0 = *query32<D>(sq, 16 * rt + g, 4 * d + t), q1 = *query32<D>(sq, 16 * rt + g + 8, 4 * d + t);
+                    const Frag fa(q0.x, q1.x, q0.y, q1.y), fb(q0.z, q1.z, q0.w, q1.w);
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) {
+                        const float4 k = stage32(st, slot + 8 * j, 4 * d + t);
+                        mma_split(s[j], fa, k.x, k.y);
+                        mma_split(s[j], fb, k.z, k.w);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_empty + sk);
+            if (warp_live) {  // s[j][2 y + e]: row g + 8 y, slot key0 + 8 j + t + 4 e
+                if (tail) {
+#pragma unroll
+                    for (int j = 0; j < NK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = key0 + 8 * j + t + 4 * (e & 1) - w.len, row = row0 + 16 * rt + g + 8 * (e >> 1);
+                            if (row >= rows || (at >= 0 && (at >= w.n || !(sees[e >> 1] >> at & 1)))) s[j][e] = -INFINITY;
+                        }
+                }
+                float f[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float top = s[0][2 * y];
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) top = fmaxf(top, fmaxf(s[j][2 * y], s[j][2 * y + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    top = fmaxf(top, m[y]);
+                    f[y] = top == m[y] ? 1.f : ex2(m[y] - top);
+                    m[y] = top;
+                    const float sub = top == -INFINITY ? 0.f : top;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) {
+                        s[j][2 * y] = ex2(s[j][2 * y] - sub);
+                        s[j][2 * y + 1] = ex2(s[j][2 * y + 1] - sub);
+                        sum += s[j][2 * y] + s[j][2 * y + 1];
+                    }
+                    l[y] = l[y] * f[y] + sum;
+                }
+                if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[x][i][0] *= f[0];
+                            o[x][i][1] *= f[0];
+                            o[x][i][2] *= f[1];
+                            o[x][i][3] *= f[1];
+                        }
+                }
+            }
+            const int sv = n % NST;
+            wait(b_full + sv, n / NST & 1);
+            ++n;
+            if (warp_live) {
+                const char *st = ring + sv * S_::kStage;
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    const Frag p(s[j][0], s[j][2], s[j][1], s[j][3]);
+                    const int slot = kg * NK * 8 + 8 * j + t, at = key0 + 8 * j + t - w.len;
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x) {
+                        const int col4 = 8 * x + (g >> 1) + ((g & 1) << 2);
+                        float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
+                        if (tail) {  // a weight of 0 times an infinity is not 0: what no row sees, and a drafted token's infinities and NaN, leave here
+                            float *both[2] = {&u.x, &v.x};
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int k = at + 4 * y;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (k >= 0 && (k >= w.n || !isfinite(both[y][i]))) {
+                                        if (k < w.n) atomicOr(&s_bad, 1ull << k);
+                                        both[y][i] = 0.f;
+                                    }
+                            }
+                        }
+                        mma_split(o[x][0], p, u.x, v.x);
+                        mma_split(o[x][1], p, u.y, v.y);
+                        mma_split(o[x][2], p, u.z, v.z);
+                        mma_split(o[x][3], p, u.w, v.w);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_empty + sv);
+        }
+        // o[x][i][2 y + e]: row g + 8 y, column 32 x + 16 e + 4 t + i
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+        }
+        if (KG > 1 && kg > 0 && warp_live) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                if (t == 0) s_ml[warp][g + 8 * y] = make_float2(m[y], l[y]);
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float4 *>(join + (((warp - RT) * 16 + g + 8 * y) * D + 32 * x + 16 * e + 4 * t) * 4) =
+                            make_float4(o[x][0][2 * y + e], o[x][1][2 * y + e], o[x][2][2 * y + e], o[x][3][2 * y + e]);
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (kg == 0 && warp_live) {
+            const bool whole = w.whole();
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int row = row0 + 16 * rt + g + 8 * y;
+                float top = m[y];
+#pragma unroll
+                for (int k = 1; k < KG; ++k) top = fmaxf(top, s_ml[k * RT + rt][g + 8 * y].x);
+                const float f0 = m[y] == top ? 1.f : ex2(m[y] - top);
+                float f[KG], sum = l[y] * f0;
+#pragma unroll
+                for (int k = 1; k < KG; ++k) {
+                    const float2 ml = s_ml[k * RT + rt][g + 8 * y];
+                    f[k] = ml.x == top ? 1.f : ex2(ml.x - top);
+                    sum = fmaf(ml.y, f[k], sum);
+                }
+                if (row >= rows) continue;
+                const int tok = row / a.group, head = h * a.group + row - tok * a.group;
+                const long long pr = ((long long)blockIdx.x * 2 + (w.opens ? 0 : 1)) * R + 16 * rt + g + 8 * y;
+                const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                float *out = whole ? static_cast<float *>(a.out) + w.b * a.os[0] + tok * a.os[1] + (long long)head * a.os[2] : part_o + pr * D;
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col = 32 * x + 16 * e + 4 * t;
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = o[x][i][2 * y + e] * f0;
+#pragma unroll
+                        for (int k = 1; k < KG; ++k) {
+                            const float4 z = *reinterpret_cast<const float4 *>(join + ((((k - 1) * RT + rt) * 16 + g + 8 * y) * D + col) * 4);
+                            v[0] = fmaf(z.x, f[k], v[0]);
+                            v[1] = fmaf(z.y, f[k], v[1]);
+                            v[2] = fmaf(z.z, f[k], v[2]);
+                            v[3] = fmaf(z.w, f[k], v[3]);
+                        }
+                        for (unsigned long long rest = s_bad & sees[y]; rest; rest &= rest - 1) {
+                            const float *bad = static_cast<const float *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)(w.len + __ffsll(rest) - 1) * a.vs[2] + col;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (!isfinite(bad[i])) v[i] += bad[i];
+                        }
+                        *reinterpret_cast<float4 *>(out + col) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    }
+                if (t == 0) {
+                    if (!whole) part_ml[pr] = make_float2(top, sum);
+                    else if (a.lse) a.lse[((long long)w.b * a.tokens + tok) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                }
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 0) s_bad = 0;  // the next segment's first barrier comes before its first use
+        w.advance();
+    }
+}
+
+// The masses of a 32-bit cache: a warp has eight slots of a tile, split once, and goes through the query rows 16 at a
+// time; a lane's two slots are summed over its rows, and over the eight lanes that share them at the end.
+template <int D>
+struct F32Mass {
+    static constexpr int kRows = 256;
+    static constexpr int kStage = kTile32 * D * 4;
+    static constexpr int kStages = 3;
+    static constexpr int kSmem = 1024 + kRows * D * 4 + kStages * kStage;
+};
+template <int D>
+__global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
+    using S_ = F32Mass<D>;
+    constexpr int NST = S_::kStages;
+    extern __shared__ char dyn[];
+    char *ring = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *sq = ring + NST * S_::kStage;
+    __shared__ uint64_t b_full[NST], b_empty[NST];
+    __shared__ int s_gave_up;
+    __shared__ Share s_share;
+    __shared__ float s_nl[S_::kRows];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const Waits wait{&s_gave_up};
+    const Cut cut{1 << 30, kTile32};
+    if (warp == 0) {
+        const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
+        if (lane == 0) s_share = s;
+    } else if (tid == 256) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(b_empty + i, 8);
+        }
+        s_gave_up = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    Walk w(a, cut, s_share);
+    if (warp == 8) {
+        uint32_t n = 0;
+        while (w.next()) {
+            for (int t = w.ta; t < w.tb; ++t, ++n) {
+                const int st = n % NST;
+                wait(b_empty + st, (n / NST & 1) ^ 1);
+                if (lane == 0) {
+                    mbar_expect_tx(b_full + st, S_::kStage);
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x) tma_load(ring + st * S_::kStage + x * 8192, &mk, 32 * x, t * kTile32, w.u, w.b, b_full + st);
+                }
+            }
+            w.advance();
+        }
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        return;
+    }
+    const int g = lane / 4, t = lane % 4;
+    const float c = a.scale * 1.4426950408889634f;
+    uint32_t n = 0;
+    while (w.next()) {
+        const int rows = w.n * a.gc, h = w.u, padded = (rows + 15) / 16 * 16;
+        for (int i = tid; i < padded * (D / 4); i += 256) {
+            const int col4 = i % (D / 4), row = i / (D / 4);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float nl = -INFINITY;
+            if (row < rows) {
+                const int k = row / a.gc, head = h * a.group + a.g0 + row - k * a.gc;
+                const int src = a.rows ? a.rows[(long long)w.b * a.tokens + k] : k;
+                if (src < 0 || src >= a.tokens) {
+                    if (col4 == 0) atomicOr(&g_cache_error, kErrRange);
+                } else {
+                    const float lse = a.lse_in[((long long)w.b * a.tokens + src) * a.heads + head];
+                    if (lse != -INFINITY) {
+                        nl = lse * -1.4426950408889634f;
+                        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + w.b * a.qs[0] + src * a.qs[1] + (long long)head * a.qs[2] + 4 * col4);
+                        v.x *= c; v.y *= c; v.z *= c; v.w *= c;
+                    }
+                }
+            }
+            *query32<D>(sq, row, col4) = v;
+            if (col4 == 0) s_nl[row] = nl;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float *min_ = a.mass + w.b * a.ms[0] + h * a.ms[1];
+        float *mout = a.mass_out + w.b * a.mos[0] + h * a.mos[1];
+        for (int tile = w.ta; tile < w.tb; ++tile) {
+            const int key0 = tile * kTile32 + 8 * warp;
+            const int st = n % NST;
+            wait(b_full + st, n / NST & 1);
+            ++n;
+            float4 k[D / 16];
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) k[d] = stage32(ring + st * S_::kStage, 8 * warp + (g >> 1) + ((g & 1) << 2), 4 * d + t);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_empty + st);
+            if (key0 >= w.len + w.n) continue;
+            float sum[2] = {0.f, 0.f};
+            int from[2];  // the first row that sees the slot
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int late = key0 + t + 4 * e - w.len;
+                from[e] = late <= 0 ? 0 : late < w.n ? late * a.gc : rows;
+            }
+            for (int r0 = 0; r0 < padded; r0 += 16) {
+                float s[4] = {};
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const float4 q0 = *query32<D>(sq, r0 + g, 4 * d + t), q1 = *query32<D>(sq, r0 + g + 8, 4 * d + t);
+                    mma_split(s, Frag(q0.x, q1.x, q0.y, q1.y), k[d].x, k[d].y);
+                    mma_split(s, Frag(q0.z, q1.z, q0.w, q1.w), k[d].z, k[d].w);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = r0 + g + 8 * (e >> 1);
+                    const float p = ex2(s[e] + s_nl[row]);
+                    if (row >= from[e & 1] && row < rows) sum[e & 1] += p;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], x);
+                const int key = key0 + t + 4 * e;
+                if (g == 0 && key < w.len + w.n) mout[key] = (key < w.len ? min_[key] : a.more ? mout[key] : 0.f) + sum[e];
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the query rows are done with
+        w.advance();
+    }
+}
+
 // ----------------------------------------------------------------------------------------------------------------
 // host side
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -974,16 +1300,17 @@ EncodeTiled encode_tiled() {  // from the driver, so that the library does not l
     }();
     return fn;
 }
-// 64 columns x 128 slots of one head, in the 128-byte swizzle; slots behind the last read as zero
+// 128 bytes of columns x a tile of slots of one head, in the 128-byte swizzle; slots behind the last read as zero
 bool cache_map(CUtensorMap *m, const p8_kv *c, const void *base, const int64_t *st) {
     const EncodeTiled f = encode_tiled();
     if (!f) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)c->width, (cuuint64_t)c->slots, (cuuint64_t)c->heads, (cuuint64_t)c->batch};
     // the stride of a dimension of one is never used, but has to be a valid one
-    const cuuint64_t row = (cuuint64_t)c->width * 2;
-    const cuuint64_t strides[3] = {c->slots > 1 ? (cuuint64_t)st[3] * 2 : row, c->heads > 1 ? (cuuint64_t)st[2] * 2 : row, c->batch > 1 ? (cuuint64_t)st[1] * 2 : row};
-    const cuuint32_t box[4] = {64, kTile, 1, 1}, one[4] = {1, 1, 1, 1};
-    return f(m, c->type == P8_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one,
+    const bool wide = c->type == P8_KV_F32;
+    const cuuint64_t es = wide ? 4 : 2, row = (cuuint64_t)c->width * es;
+    const cuuint64_t strides[3] = {c->slots > 1 ? (cuuint64_t)st[3] * es : row, c->heads > 1 ? (cuuint64_t)st[2] * es : row, c->batch > 1 ? (cuuint64_t)st[1] * es : row};
+    const cuuint32_t box[4] = {wide ? 32u : 64u, (cuuint32_t)(wide ? kTile32 : kTile), 1, 1}, one[4] = {1, 1, 1, 1};
+    return f(m, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : c->type == P8_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -998,6 +1325,14 @@ void allow() {
     cudaFuncSetAttribute(k_attn_mass_tc<T, D, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 256>::kSmem);
     cudaFuncSetAttribute(k_attn_mass_tc<T, D, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 512>::kSmem);
 }
+template <int D>
+void allow32() {
+    cudaFuncSetAttribute(k_tree_attn_f32<D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 1>::kSmem);
+    cudaFuncSetAttribute(k_tree_attn_f32<D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 2>::kSmem);
+    cudaFuncSetAttribute(k_tree_attn_f32<D, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 4>::kSmem);
+    cudaFuncSetAttribute(k_tree_attn_f32<D, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 8>::kSmem);
+    cudaFuncSetAttribute(k_attn_mass_f32<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Mass<D>::kSmem);
+}
 // SM count of the current device; the first call on a device raises the kernels' shared-memory limits there
 int sm_count() {
     static std::atomic<int> n[64];
@@ -1010,35 +1345,40 @@ int sm_count() {
         allow<__half, 128>();
         allow<__nv_bfloat16, 64>();
         allow<__nv_bfloat16, 128>();
+        allow32<64>();
+        allow32<128>();
         n[dev].store(v, std::memory_order_release);
     }
     return v;
 }
 
-bool two_tiles(int64_t rows) { return rows > 128; }
+// Query rows of a unit: as few as hold them all, so that K and V are read once; the largest block has to be enough for
+// the rest (the last SM-sized part of a longer row list reads its tiles from L2).
+Cut attn_cut(const p8_kv *c, int64_t rows) {
+    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile};
+    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32};
+}
 // CTAs of a call: no more than there can be tiles
-int tc_ctas(const p8_kv *c, int64_t rows, int rblock) {
-    const int64_t tiles = c->batch * c->heads * ((rows + rblock - 1) / rblock) * ((c->slots + kTile - 1) / kTile);
+int attn_ctas(const p8_kv *c, int64_t rows, Cut cut) {
+    const int64_t tiles = c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile);
     return (int)std::min<int64_t>(sm_count(), tiles);
 }
 
-size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {
-    if (c->type == P8_KV_F32) return 0;
-    // two parts a CTA, each with the rows' two statistics
+size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {  // two parts a CTA, each with the rows' two statistics
     const int64_t rows = tokens * (heads / c->heads);
-    const int R = two_tiles(rows) ? 256 : 128;
-    return (size_t)2 * tc_ctas(c, rows, R) * R * ((size_t)c->width * 4 + 8);
+    const Cut cut = attn_cut(c, rows);
+    return (size_t)2 * attn_ctas(c, rows, cut) * cut.rblock * ((size_t)c->width * 4 + 8);
 }
 
-template <typename T, int D, bool TWO>
-p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
-    constexpr int R = TcShape<D, TWO>::kRows;
+template <typename T, int D, typename K>
+p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     CUtensorMap mk, mv;
     if (!cache_map(&mk, c, c->k, c->k_stride) || !cache_map(&mv, c, c->v, c->v_stride)) return P8_ERR_CUDA;
-    const int ctas = tc_ctas(c, (int64_t)a.tokens * a.group, R);
+    const Cut cut = attn_cut(c, (int64_t)a.tokens * a.group);
+    const int ctas = attn_ctas(c, (int64_t)a.tokens * a.group, cut);
     float *po = static_cast<float *>(ws);
-    float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * R * D);
-    k_tree_attn_tc<T, D, TWO><<<ctas, 320, TcShape<D, TWO>::kSmem, st>>>(a, mk, mv, po, ml);
+    float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * cut.rblock * D);
+    kernel<<<ctas, threads, smem, st>>>(a, mk, mv, po, ml);
     if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at;
@@ -1049,48 +1389,60 @@ p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_attn_join<T, D>, a, R, ctas, Half16<T>::kLift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, k_attn_join<T, D>, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 template <typename T, int D>
 p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
-    return two_tiles((int64_t)a.tokens * a.group) ? run_tc<T, D, true>(c, a, ws, st) : run_tc<T, D, false>(c, a, ws, st);
+    constexpr float lift = Half16<T>::kLift;
+    if (a.tokens * a.group > 128) return run_attn<T, D>(k_tree_attn_tc<T, D, true>, 320, TcShape<D, true>::kSmem, lift, c, a, ws, st);
+    return run_attn<T, D>(k_tree_attn_tc<T, D, false>, 320, TcShape<D, false>::kSmem, lift, c, a, ws, st);
 }
-template <typename T, int D>
-p8_status run_mass_tc(const p8_kv *c, AttnArgs a, cudaStream_t st) {
-    CUtensorMap mk;
-    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
-    const int ctas = tc_ctas(c, 1, 1 << 30), most = 512 / a.tokens;
-    for (a.g0 = 0; a.g0 < a.group; a.g0 += a.gc) {  // at most 512 rows a launch; the later ones add to the first one's sums
-        a.gc = std::min(most, a.group - a.g0);
+template <int D>
+p8_status run_f32(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
+    switch (attn_cut(c, (int64_t)a.tokens * a.group).rblock) {
+        case 16: return run_attn<float, D>(k_tree_attn_f32<D, 1>, 288, F32Shape<D, 1>::kSmem, 0.f, c, a, ws, st);
+        case 32: return run_attn<float, D>(k_tree_attn_f32<D, 2>, 288, F32Shape<D, 2>::kSmem, 0.f, c, a, ws, st);
+        case 64: return run_attn<float, D>(k_tree_attn_f32<D, 4>, 288, F32Shape<D, 4>::kSmem, 0.f, c, a, ws, st);
+        default: return run_attn<float, D>(k_tree_attn_f32<D, 8>, 288, F32Shape<D, 8>::kSmem, 0.f, c, a, ws, st);
+    }
+}
+// At most `most` rows a launch (what its shared memory holds); the later launches add to the first one's sums.
+template <typename F>
+p8_status mass_launches(AttnArgs a, int most, F launch) {
+    for (a.g0 = 0; a.g0 < a.group; a.g0 += a.gc) {
+        a.gc = std::min(most / a.tokens, a.group - a.g0);
         a.more = a.g0 > 0;
         if (a.more) {
             a.mass = a.mass_out;
             for (int i = 0; i < 2; ++i) a.ms[i] = a.mos[i];
         }
-        if (a.tokens * a.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(a, mk);
-        else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(a, mk);
+        launch(a);
         if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
     }
     return P8_OK;
 }
-template <typename T>
-p8_status run16(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cudaStream_t st) {
-    if (c->width == 128) return mass ? run_mass_tc<T, 128>(c, a, st) : run_tc<T, 128>(c, a, ws, st);
-    return mass ? run_mass_tc<T, 64>(c, a, st) : run_tc<T, 64>(c, a, ws, st);
+template <typename T, int D>
+p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
+    CUtensorMap mk;
+    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile});
+    return mass_launches(a, 512, [&](const AttnArgs &x) {
+        if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(x, mk);
+        else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(x, mk);
+    });
 }
-
-template <typename T>
-void run_attn(const p8_kv *c, const AttnArgs &a, bool mass, cudaStream_t st) {
-    const int blocks = (a.tokens * a.group + 7) / 8;
-    if (mass) {
-        const dim3 g(512, a.kvh, a.batch);
-        if (c->width == 128) k_attn_mass_plain<T, 128><<<g, 128, 0, st>>>(a);
-        else k_attn_mass_plain<T, 64><<<g, 128, 0, st>>>(a);
-    } else {
-        const dim3 g(blocks, a.kvh, a.batch);
-        if (c->width == 128) k_tree_attn_plain<T, 128><<<g, 128, 0, st>>>(a);
-        else k_tree_attn_plain<T, 64><<<g, 128, 0, st>>>(a);
-    }
+template <int D>
+p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
+    CUtensorMap mk;
+    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile32});
+    return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, 288, F32Mass<D>::kSmem, st>>>(x, mk); });
+}
+template <int D>
+p8_status run_width(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cudaStream_t st) {
+    if (c->type == P8_KV_F32) return mass ? run_mass_f32<D>(c, a, st) : run_f32<D>(c, a, ws, st);
+    if (c->type == P8_KV_F16) return mass ? run_mass_tc<__half, D>(c, a, st) : run_tc<__half, D>(c, a, ws, st);
+    return mass ? run_mass_tc<__nv_bfloat16, D>(c, a, st) : run_tc<__nv_bfloat16, D>(c, a, ws, st);
 }
 
 void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, int64_t tokens, int64_t heads) {
@@ -1102,10 +1454,7 @@ void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, in
 }
 
 p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
-    if (c->type == P8_KV_F16) return run16<__half>(c, x, mass, ws, st);
-    if (c->type == P8_KV_BF16) return run16<__nv_bfloat16>(c, x, mass, ws, st);
-    run_attn<float>(c, x, mass, st);
-    return cudaGetLastError() == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+    return c->width == 128 ? run_width<128>(c, x, mass, ws, st) : run_width<64>(c, x, mass, ws, st);
 }
 
 p8_status launch_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *ws, cudaStream_t st) {
