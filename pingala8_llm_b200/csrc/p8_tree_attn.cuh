@@ -262,6 +262,31 @@ __device__ __forceinline__ void load_q(char *sq, const AttnArgs &a, int b, int h
     }
 }
 
+// Which of 32 columns a row sees, where `off` of them are the sequence's and the drafted tokens follow.
+__device__ __forceinline__ uint32_t seen32(bool live, unsigned long long sees, int off) {
+    uint32_t see = off >= 32 ? ~0u : off > 0 ? (1u << off) - 1 : 0u;
+    if (off < 32 && off > -64) see |= off >= 0 ? (uint32_t)sees << off : (uint32_t)(sees >> -off);
+    return live ? see : 0u;
+}
+__device__ __forceinline__ void hide(uint32_t (&x)[32], uint32_t see) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+        if (!(see >> k & 1)) x[k] = 0xFF800000u;  // -infinity
+}
+
+// A drafted token's infinities and NaN (those of the tokens in `bad`) onto the values that a row has written: x plus
+// each of them, in columns [x0, x1).
+template <typename T, typename O>
+__device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsigned long long bad, int x0, int x1) {
+    for (; bad; bad &= bad - 1) {
+        const T *y = v + (__ffsll(bad) - 1) * stride;
+        for (int k = x0; k < x1; ++k) {
+            const float z = to_f(y[k]);
+            if (!isfinite(z)) out[k] = from_f<O>(to_f(out[k]) + z);
+        }
+    }
+}
+
 // The tree attention kernel. Ten warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
 // brings tiles of K and V into a ring by TMA, one that issues the MMAs. Two streams of work alternate, one per softmax
 // group, so that the tensor cores compute one stream's scores while the other's are exponentiated:
@@ -434,30 +459,24 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 wait(b_s + s, c_s++ & 1);
                 tc_fence_after();
                 if (warp_live) {
-                    uint32_t x[4][32];
+                    // Two passes over the scores in chunks of 32, read from TMEM twice: half the registers, and a loop
+                    // body that is fetched once instead of straight code for 128 columns (few tiles pass through a CTA
+                    // of a short sequence, and fetching code would take it longer than running it).
+                    const int off = w.len - key0;  // the tile's columns before it are the sequence's
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[32];
+                        tmem_ld32(tS + 32 * j, x);
+                        tmem_wait_ld(x);
+                        if (tail) hide(x, seen32(live, sees, off - 32 * j));
+                        float t4[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) tmem_ld32(tS + 32 * j, x[j]);
-                    tmem_wait_ld(x[0]);
+                        for (int k = 0; k < 4; ++k) t4[k] = __uint_as_float(x[k]);
 #pragma unroll
-                    for (int j = 1; j < 4; ++j) tmem_waited(x[j]);
-                    if (tail) {
-                        const int off = w.len - key0;  // the tile's columns before it are the sequence's
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int o = off - 32 * j;  // bit k of `see`: column 32 j + k
-                            uint32_t see = o >= 32 ? ~0u : o > 0 ? (1u << o) - 1 : 0u;
-                            if (o < 32 && o > -64) see |= o >= 0 ? (uint32_t)sees << o : (uint32_t)(sees >> -o);
-                            if (!live) see = 0;
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!(see >> k & 1)) x[j][k] = 0xFF800000u;
-                        }
+                        for (int k = 4; k < 32; ++k) t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(x[k]));
+                        top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
                     }
-                    float top = __uint_as_float(x[0][0]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(x[j][k]));
                     top = top == -INFINITY ? m : fmaxf(m, top * c);
                     if (m == -INFINITY) m = top;  // nothing summed so far
                     const bool raise = top > m + H::kSlack;
@@ -465,7 +484,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                         const float f = raise ? ex2(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
-#pragma unroll
+#pragma unroll 1
                         for (int j = 0; j < D / 32; ++j) {
                             uint32_t o[32];
                             tmem_ld32(tO + 32 * j, o);
@@ -477,18 +496,20 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                     }
                     const float sub = m == -INFINITY ? 0.f : H::kLift - m;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[32], p[16];
+                        tmem_ld32(tS + 32 * j, x);
+                        tmem_wait_ld(x);
+                        if (tail) hide(x, seen32(live, sees, off - 32 * j));
 #pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        uint32_t p[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const float p0 = ex2(fmaf(__uint_as_float(x[j + k / 16][2 * (k % 16)]), c, sub));
-                            const float p1 = ex2(fmaf(__uint_as_float(x[j + k / 16][2 * (k % 16) + 1]), c, sub));
+                        for (int k = 0; k < 16; ++k) {
+                            const float p0 = ex2(fmaf(__uint_as_float(x[2 * k]), c, sub)), p1 = ex2(fmaf(__uint_as_float(x[2 * k + 1]), c, sub));
                             l4[k & 1] += p0;
                             l4[2 + (k & 1)] += p1;
                             p[k] = H::pack(p0, p1);
                         }
-                        tmem_st32(tS + 16 * j, p);
+                        tmem_st16(tS + 16 * j, p);  // over scores that have been read: 16 j + 15 < 32 (j + 1)
                     }
                     l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     tmem_wait_st();
@@ -548,9 +569,9 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 both = ns > 1;
                 const float top = fmaxf(m0, m1);
                 f0 = m0 == top ? 1.f : ex2(m0 - top);
-                f1 = !both ? 0.f : m1 == top ? 1.f : ex2(m1 - top);
+                f1 = m1 == top ? 1.f : ex2(m1 - top);
                 m = top;
-                l = l0 * f0 + (both ? l1 * f1 : 0.f);
+                l = both ? l0 * f0 + l1 * f1 : l0;
                 x0 = s * (D / 2);
                 x1 = x0 + D / 2;
             }
@@ -561,48 +582,38 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 T *out = static_cast<T *>(a.out) + w.b * a.os[0] + t * a.os[1] + (long long)head * a.os[2];
                 float *po = part_o + pr * D;
-                const uint32_t t0 = tmem + 256 + lanes + (TWO ? 128 * s : 0);
-#pragma unroll
-                for (int j = 0; j < (TWO ? D : D / 2) / 32; ++j) {
+                const uint32_t t0 = tmem + 256 + lanes + (TWO ? 128 * s : 0) + x0;
+#pragma unroll 1
+                for (int j = 0; j < x1 - x0; j += 32) {
                     uint32_t o[32];
-                    tmem_ld32(t0 + x0 + 32 * j, o);
+                    tmem_ld32(t0 + j, o);
                     tmem_wait_ld(o);
                     if (!TWO) {
-                        uint32_t o1[32];
                         if (both) {
-                            tmem_ld32(t0 + 128 + x0 + 32 * j, o1);
+                            uint32_t o1[32];
+                            tmem_ld32(t0 + 128 + j, o1);
                             tmem_wait_ld(o1);
-                        }
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            float y = __uint_as_float(o[k]) * f0;
-                            if (both) y = fmaf(__uint_as_float(o1[k]), f1, y);
-                            o[k] = __float_as_uint(y);
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o[k]) * f0));
                         }
                     }
-                    if (live) {
-                        for (unsigned long long rest = bad; rest; rest &= rest - 1) {
-                            const T *v = static_cast<const T *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)(w.len + __ffsll(rest) - 1) * a.vs[2] + x0 + 32 * j;
+                    if (live && whole) {
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                const float y = to_f(v[k]);
-                                if (!isfinite(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
-                            }
+                        for (int k = 0; k < 32; k += 8) {
+                            uint32_t q[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) q[e] = H::pack(__uint_as_float(o[k + 2 * e]) * inv, __uint_as_float(o[k + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(out + x0 + j + k) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
-                        if (whole) {
+                    } else if (live) {
 #pragma unroll
-                            for (int k = 0; k < 32; k += 8) {
-                                uint32_t q[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    q[e] = H::pack(__uint_as_float(o[k + 2 * e]) * inv, __uint_as_float(o[k + 2 * e + 1]) * inv);
-                                *reinterpret_cast<uint4 *>(out + x0 + 32 * j + k) = make_uint4(q[0], q[1], q[2], q[3]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(po + x0 + 32 * j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                        }
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(po + x0 + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
+                }
+                if (live && bad) {
+                    const T *v = static_cast<const T *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)w.len * a.vs[2];
+                    if (whole) add_bad(out, v, a.vs[2], bad, x0, x1);
+                    else add_bad(po, v, a.vs[2], bad, x0, x1);
                 }
                 if (live && x0 == 0) {
                     if (!whole) part_ml[pr] = make_float2(m, l);
@@ -991,7 +1002,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
             if (warp_live) {
                 const char *st = ring + sk * S_::kStage;
                 const int slot = kg * NK * 8 + (g >> 1) + ((g & 1) << 2);
-#pragma unroll
+#pragma unroll 1
                 for (int d = 0; d < D / 16; ++d) {
                     const float4 q0 = *query32<D>(sq, 16 * rt + g, 4 * d + t), q1 = *query32<D>(sq, 16 * rt + g + 8, 4 * d + t);
                     const Frag fa(q0.x, q1.x, q0.y, q1.y), fb(q0.z, q1.z, q0.w, q1.w);
@@ -1052,28 +1063,34 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
             wait(b_full + sv, n / NST & 1);
             ++n;
             if (warp_live) {
-                const char *st = ring + sv * S_::kStage;
+                char *st = ring + sv * S_::kStage;
+                if (tail) {
+                    // A weight of 0 times an infinity is not 0: the warp's slots that no row sees become zero, and so do a
+                    // drafted token's infinities and NaN (they reach the rows that see it at the segment's end). Warps
+                    // with other rows of the same slots write the same zeros.
+#pragma unroll 1
+                    for (int i = lane; i < NK * 8 * (D / 4); i += 32) {
+                        const int slot = kg * NK * 8 + i / (D / 4), col4 = i % (D / 4), at = tile * kTile32 + slot - w.len;
+                        if (at < 0) continue;
+                        float4 *v = reinterpret_cast<float4 *>(st + (col4 / 8) * 8192 + slot * 128 + ((col4 % 8) ^ (slot % 8)) * 16);
+                        const float4 x = *v;
+                        if (at < w.n && isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w)) continue;
+                        if (at < w.n) atomicOr(&s_bad, 1ull << at);
+                        const bool real = at < w.n;
+                        *v = make_float4(real && isfinite(x.x) ? x.x : 0.f, real && isfinite(x.y) ? x.y : 0.f, real && isfinite(x.z) ? x.z : 0.f,
+                                         real && isfinite(x.w) ? x.w : 0.f);
+                    }
+                    fence_proxy_async();  // the stage is the TMA's again after this tile
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     const Frag p(s[j][0], s[j][2], s[j][1], s[j][3]);
-                    const int slot = kg * NK * 8 + 8 * j + t, at = key0 + 8 * j + t - w.len;
+                    const int slot = kg * NK * 8 + 8 * j + t;
 #pragma unroll
                     for (int x = 0; x < D / 32; ++x) {
                         const int col4 = 8 * x + (g >> 1) + ((g & 1) << 2);
-                        float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
-                        if (tail) {  // a weight of 0 times an infinity is not 0: what no row sees, and a drafted token's infinities and NaN, leave here
-                            float *both[2] = {&u.x, &v.x};
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const int k = at + 4 * y;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (k >= 0 && (k >= w.n || !isfinite(both[y][i]))) {
-                                        if (k < w.n) atomicOr(&s_bad, 1ull << k);
-                                        both[y][i] = 0.f;
-                                    }
-                            }
-                        }
+                        const float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
                         mma_split(o[x][0], p, u.x, v.x);
                         mma_split(o[x][1], p, u.y, v.y);
                         mma_split(o[x][2], p, u.z, v.z);
@@ -1140,14 +1157,13 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                             v[2] = fmaf(z.z, f[k], v[2]);
                             v[3] = fmaf(z.w, f[k], v[3]);
                         }
-                        for (unsigned long long rest = s_bad & sees[y]; rest; rest &= rest - 1) {
-                            const float *bad = static_cast<const float *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)(w.len + __ffsll(rest) - 1) * a.vs[2] + col;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (!isfinite(bad[i])) v[i] += bad[i];
-                        }
                         *reinterpret_cast<float4 *>(out + col) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                     }
+                const unsigned long long bad = s_bad & sees[y];
+                if (bad) {
+                    const float *v = static_cast<const float *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)w.len * a.vs[2];
+                    for (int col = 4 * t; col < D; col += 16) add_bad(out, v, a.vs[2], bad, col, col + 4);  // the thread's own columns
+                }
                 if (t == 0) {
                     if (!whole) part_ml[pr] = make_float2(top, sum);
                     else if (a.lse) a.lse[((long long)w.b * a.tokens + tok) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
