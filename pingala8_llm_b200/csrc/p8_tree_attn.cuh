@@ -23,41 +23,40 @@ struct AttnArgs {
 // together whatever the lengths are, and one long sequence still fills them. A unit that lies in one share is finished
 // there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
 constexpr int kTile = 128;  // of a 16-bit cache; 64 of a 32-bit one (as many bytes)
-struct Cut {                // how a kernel cuts its work: query rows of a unit, slots of a tile
-    int rblock, tile;
+struct Cut {                // how a kernel cuts its work
+    int rblock, tile;       // query rows of a unit, slots of a tile
+    int least;              // tiles of a share, at least
 };
 
 struct Share {
-    long long pos, end;  // the CTA's tiles
-    long long off;       // of pos, within sequence b
-    int b;
+    int pos, end;           // the CTA's tiles
+    int b, off, len, n;     // the sequence that pos lies in, and where in it
 };
 
-struct Walk {            // a CTA's way through its share, one segment (the tiles of one unit) at a time
+struct Walk {               // a CTA's way through its share, one segment (the tiles of one unit) at a time
     const AttnArgs &a;
     const Cut cut;
-    long long pos, end, off;
-    int b, len, n, nt, units, u, ta, tb;
-    bool opens;          // the segment is the share's first
-    __device__ Walk(const AttnArgs &a_, Cut c, const Share &s) : a(a_), cut(c), pos(s.pos), end(s.end), off(s.off), b(s.b) {
-        opens = true;
-        if (pos < end) load();
+    int pos, end, off, b, len, n, nt, units, u, ta, tb;
+    bool opens;             // the segment is the share's first
+    __device__ Walk(const AttnArgs &a_, Cut c, const Share &s)
+        : a(a_), cut(c), pos(s.pos), end(s.end), off(s.off), b(s.b), len(s.len), n(s.n), opens(true) {
+        count();
     }
-    __device__ void load() {
-        if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
+    __device__ void count() {
         nt = n ? (len + n + cut.tile - 1) / cut.tile : 0;
         units = n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) : 0;
     }
     __device__ bool next() {
         if (pos >= end) return false;
-        while (off >= (long long)units * nt) {
-            off -= (long long)units * nt;
+        while (off >= units * nt) {
+            off -= units * nt;
             ++b;
-            load();
+            if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
+            count();
         }
-        u = (int)(off / nt);
-        ta = (int)(off - (long long)u * nt);
-        tb = (int)min((long long)nt, ta + (end - pos));
+        u = off / nt;
+        ta = off - u * nt;
+        tb = min(nt, ta + (end - pos));
         return true;
     }
     __device__ void advance() {
@@ -71,53 +70,46 @@ struct Walk {            // a CTA's way through its share, one segment (the tile
     __device__ bool whole() const { return ta == 0 && tb == nt; }
 };
 
-__device__ __forceinline__ long long seq_tiles(const AttnArgs &a, Cut cut, int b, bool *bad) {
-    int len, n;
+// (the host refuses what would not fit 31 bits)
+__device__ __forceinline__ int seq_tiles(const AttnArgs &a, Cut cut, int b, int &len, int &n, bool *bad) {
     if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
         *bad = true;
-        return 0;
+        n = 0;
     }
-    return n ? (long long)a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) * ((len + n + cut.tile - 1) / cut.tile) : 0;
+    return n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) * ((len + n + cut.tile - 1) / cut.tile) : 0;
 }
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-__device__ __forceinline__ long long warp_scan(long long v, int lane) {  // inclusive
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += x;
     }
     return v;
 }
-// tiles of all sequences (whole warp)
-__device__ __forceinline__ long long all_tiles(const AttnArgs &a, Cut cut, int lane, bool *bad) {
-    long long total = 0;
-    for (int b = lane; b < a.batch; b += 32) total += seq_tiles(a, cut, b, bad);
-    return warp_sum(total);
-}
+// tiles of a share, of a list of that many
+__device__ __forceinline__ int share_of(int total, Cut cut, int ctas) { return max(cut.least, (int)(((unsigned)total + ctas - 1) / (unsigned)ctas)); }
 // the share of one CTA (whole warp)
 __device__ __forceinline__ Share find_share(const AttnArgs &a, Cut cut, int lane, int cta, int ctas) {
     bool bad = false;
-    const long long total = all_tiles(a, cut, lane, &bad);
+    int len = 0, n = 0, mine = 0, total = 0;
+    for (int b = lane; b < a.batch; b += 32) total += mine = seq_tiles(a, cut, b, len, n, &bad);
+    total = __reduce_add_sync(0xffffffffu, total);
     if (bad && cta == 0) atomicOr(&g_cache_error, kErrRange);
-    const long long each = (total + ctas - 1) / ctas;
-    Share s;
-    s.pos = min(total, cta * each);
-    s.end = min(total, s.pos + each);
-    s.b = 0;
-    s.off = 0;
-    long long run = 0;
+    const int each = share_of(total, cut, ctas);
+    Share s = {};
+    s.pos = (int)min((long long)total, (long long)cta * each);
+    s.end = (int)min((long long)total, (long long)s.pos + each);
+    int run = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const long long mine = b0 + lane < a.batch ? seq_tiles(a, cut, b0 + lane, &bad) : 0;
-        const long long incl = run + warp_scan(mine, lane);
+        if (a.batch > 32) mine = b0 + lane < a.batch ? seq_tiles(a, cut, b0 + lane, len, n, &bad) : 0;
+        const int incl = run + warp_scan(mine, lane);
         const unsigned int hit = __ballot_sync(0xffffffffu, incl > s.pos);
         if (hit) {
             const int l = __ffs(hit) - 1;
             s.b = b0 + l;
             s.off = s.pos - __shfl_sync(0xffffffffu, incl - mine, l);
+            s.len = __shfl_sync(0xffffffffu, len, l);
+            s.n = __shfl_sync(0xffffffffu, n, l);
             break;
         }
         run = __shfl_sync(0xffffffffu, incl, 31);
@@ -151,6 +143,7 @@ __device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int 
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void map_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // Shared-memory operand of 128-byte rows in the 128-byte swizzle (what the tensor map's loads leave; a stage is `rows`
 // rows per 64 columns). Rows as the outer extent (Q, K): groups of 8 rows 1024 bytes apart. Rows as the summed one (V):
 // the same bytes read the other way, the next 64 columns a whole stage part (16 KB) on.
@@ -304,6 +297,7 @@ struct TcShape {
     static constexpr int kQ = (TWO ? 2 : 1) * 128 * D * 2;
     static constexpr int kStages = D == 64 ? 10 : TWO ? 5 : 6;
     static constexpr int kRows = TWO ? 256 : 128;
+    static constexpr int kLeast = TWO ? 1 : 2;  // one tile for each stream
     static constexpr int kSmem = 1024 + kQ + kStages * kStage;
 };
 
@@ -323,11 +317,13 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, Cut{S_::kRows, kTile}, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, Cut{S_::kRows, kTile, S_::kLeast}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
     } else if (tid == 256) {
+        map_prefetch(&mk);
+        map_prefetch(&mv);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
@@ -348,7 +344,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    Walk w(a, Cut{S_::kRows, kTile}, s_share);
+    Walk w(a, Cut{S_::kRows, kTile, S_::kLeast}, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
@@ -415,9 +411,11 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 tc_fence_after();
                 if (lane == 0) {
                     const uint32_t va = smem_u32(ring + st * S_::kStage);
+                    // slots behind the drafted tokens are not multiplied, but for the rest of a step of 16
+                    const int real = w.len + w.n - (w.ta + (TWO ? i / 2 : i)) * kTile, steps = min(kTile / 16, (real + 15) / 16);
 #pragma unroll
                     for (int kk = 0; kk < kTile / 16; ++kk)
-                        mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, desc_cols(va + kk * 2048), id_o, i >= 2 || kk != 0);
+                        if (kk < steps) mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, desc_cols(va + kk * 2048), id_o, i >= 2 || kk != 0);
                     if (!TWO || s == 1) umma_commit(b_empty + st);
                     umma_commit(b_pv + s);
                 }
@@ -463,9 +461,10 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                     // body that is fetched once instead of straight code for 128 columns (few tiles pass through a CTA
                     // of a short sequence, and fetching code would take it longer than running it).
                     const int off = w.len - key0;  // the tile's columns before it are the sequence's
+                    const int chunks = min(4, (off + w.n + 31) / 32);
                     float top = -INFINITY;
 #pragma unroll 1
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < chunks; ++j) {
                         uint32_t x[32];
                         tmem_ld32(tS + 32 * j, x);
                         tmem_wait_ld(x);
@@ -497,7 +496,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                     const float sub = m == -INFINITY ? 0.f : H::kLift - m;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < chunks; ++j) {
                         uint32_t x[32], p[16];
                         tmem_ld32(tS + 32 * j, x);
                         tmem_wait_ld(x);
@@ -516,12 +515,12 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 }
                 if (tail && (!TWO || s == 0)) {
                     // Weights are 0 where a row does not see a slot, but 0 times an infinity is not: rows of V behind the
-                    // drafted tokens become zero, and so do a drafted token's infinities and NaN, which reach the rows
+                    // drafted tokens (up to the next 16) become zero, and so do a drafted token's infinities and NaN, which reach the rows
                     // that do see it at the segment's end.
                     const uint32_t at = base + (TWO ? 2 * (i / 2) + 1 : i + min(i + 2, ns)), st = at % NST;
                     wait(b_full + st, at / NST & 1);
                     const int first = max(0, w.len - key0), real = w.len + w.n - key0;
-                    for (int k = r; k < (kTile - first) * (D / 8); k += 128) {
+                    for (int k = r; k < (min(kTile, (real + 15) / 16 * 16) - first) * (D / 8); k += 128) {
                         const int y = first + k / (D / 8), ch = k % (D / 8);
                         uint4 *v = reinterpret_cast<uint4 *>(ring + st * S_::kStage + (ch / 8) * 16384 + y * 128 + ((ch % 8) ^ (y % 8)) * 16);
                         if (y >= real) {
@@ -636,7 +635,6 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
 // the parts in their order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x % 32;
     const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     if (id >= (long long)a.batch * a.tokens * a.heads) return;
@@ -644,20 +642,22 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
     int len, n;
     if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n) || t >= n) return;
     bool bad = false;
-    long long total = 0, before = 0;
+    int total = 0, before = 0, l_, n_;
     for (int x = lane; x < a.batch; x += 32) {
-        const long long k = seq_tiles(a, cut, x, &bad);
+        const int k = seq_tiles(a, cut, x, l_, n_, &bad);
         total += k;
         before += x < b ? k : 0;
     }
-    total = warp_sum(total);
-    before = warp_sum(before);
-    const long long each = (total + ctas - 1) / ctas;
+    total = __reduce_add_sync(0xffffffffu, total);
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int each = share_of(total, cut, ctas);
     const int blocks = (n * a.group + cut.rblock - 1) / cut.rblock, nt = (len + n + cut.tile - 1) / cut.tile;
     const int h = head / a.group, row = t * a.group + head % a.group;
-    const long long u0 = before + (long long)(h * blocks + row / cut.rblock) * nt, u1 = u0 + nt;
-    const int c0 = (int)(u0 / each), c1 = (int)((u1 - 1) / each);
+    const int u0 = before + (h * blocks + row / cut.rblock) * nt, u1 = u0 + nt;
+    const int c0 = u0 / each, c1 = (u1 - 1) / each;
     if (c0 == c1) return;  // finished by that CTA
+    // Everything so far came from the call's inputs, while the attention kernel ran; the parts are its outputs.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each != u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
     float m = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[at(c)].x);
@@ -706,11 +706,12 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, Cut{1 << 30, kTile}, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, Cut{1 << 30, kTile, 1}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
     } else if (tid == 256) {
+        map_prefetch(&mk);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    Walk w(a, Cut{1 << 30, kTile}, s_share);
+    Walk w(a, Cut{1 << 30, kTile, 1}, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
@@ -928,11 +929,13 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
     __shared__ unsigned long long s_bad;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{R, kTile32};
+    const Cut cut{R, kTile32, 1};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (tid == 256) {
+        map_prefetch(&mk);
+        map_prefetch(&mv);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 8);
@@ -1197,11 +1200,12 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
     __shared__ float s_nl[S_::kRows];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{1 << 30, kTile32};
+    const Cut cut{1 << 30, kTile32, 1};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (tid == 256) {
+        map_prefetch(&mk);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 8);
@@ -1371,14 +1375,14 @@ int sm_count() {
 // Query rows of a unit: as few as hold them all, so that K and V are read once; the largest block has to be enough for
 // the rest (the last SM-sized part of a longer row list reads its tiles from L2).
 Cut attn_cut(const p8_kv *c, int64_t rows) {
-    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile};
-    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32};
+    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2};
+    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32, 1};
+}
+int64_t attn_tiles(const p8_kv *c, int64_t rows, Cut cut) {
+    return c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile);
 }
 // CTAs of a call: no more than there can be tiles
-int attn_ctas(const p8_kv *c, int64_t rows, Cut cut) {
-    const int64_t tiles = c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile);
-    return (int)std::min<int64_t>(sm_count(), tiles);
-}
+int attn_ctas(const p8_kv *c, int64_t rows, Cut cut) { return (int)std::min<int64_t>(sm_count(), attn_tiles(c, rows, cut)); }
 
 size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {  // two parts a CTA, each with the rows' two statistics
     const int64_t rows = tokens * (heads / c->heads);
@@ -1441,7 +1445,7 @@ template <typename T, int D>
 p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
-    const int ctas = attn_ctas(c, 1, Cut{1, kTile});
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1});
     return mass_launches(a, 512, [&](const AttnArgs &x) {
         if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(x, mk);
         else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(x, mk);
@@ -1451,7 +1455,7 @@ template <int D>
 p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
-    const int ctas = attn_ctas(c, 1, Cut{1, kTile32});
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1});
     return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, 288, F32Mass<D>::kSmem, st>>>(x, mk); });
 }
 template <int D>
@@ -1470,6 +1474,8 @@ void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, in
 }
 
 p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
+    const int64_t rows = mass ? 1 : (int64_t)x.tokens * x.group;
+    if (attn_tiles(c, rows, attn_cut(c, rows)) > INT32_MAX / 2) return P8_ERR_UNSUPPORTED;
     return c->width == 128 ? run_width<128>(c, x, mass, ws, st) : run_width<64>(c, x, mass, ws, st);
 }
 
