@@ -267,6 +267,12 @@ __device__ __forceinline__ void hide(uint32_t (&x)[32], uint32_t see) {
         if (!(see >> k & 1)) x[k] = 0xFF800000u;  // -infinity
 }
 
+// Groups of 16 slots that a step multiplies: those that hold something, and at least one.
+__device__ __forceinline__ int live_groups(const Walk &w, int tile, int half) {
+    const int real = w.len + w.n - tile * kTile - 64 * half;
+    return max(1, min(4, (real + 15) / 16));
+}
+
 // A drafted token's infinities and NaN (those of the tokens in `bad`) onto the values that a row has written: x plus
 // each of them, in columns [x0, x1).
 template <typename T, typename O>
@@ -280,36 +286,41 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
     }
 }
 
-// The tree attention kernel. Ten warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
-// brings tiles of K and V into a ring by TMA, one that issues the MMAs. Two streams of work alternate, one per softmax
-// group, so that the tensor cores compute one stream's scores while the other's are exponentiated:
-//   TWO = false (at most 128 query rows): both streams have the same rows, and the tiles alternate between them; their
-//                accumulators are joined at the segment's end.
-//   TWO = true: stream s has rows 128 s .. of a block of 256, both take every tile (one copy of K and V for 256 rows).
-// Step i of a segment is stream i % 2 on tile i (TWO: i / 2):  S = Q K^T (128 x 128, TMEM) -> softmax group: mask,
-// running maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). The next S of a
-// stream is issued once its P V is done.
-// Bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.7 k cycles, the MMAs 1 k per
-// stream's step, the exponentials (128 x 128 at 16 a cycle) another 1 k.
+// The tree attention kernel. Eleven warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
+// brings tiles of K and V into a ring by TMA, and one for each of two streams that issues its MMAs. A stream is a
+// softmax group with its scores and its accumulator in TMEM; a step is 64 slots:
+//   TWO = false (at most 128 query rows): both streams have the same rows, stream s takes the slots 64 s .. of every
+//                tile; the accumulators are joined at the segment's end.
+//   TWO = true: stream s has rows 128 s .. of a block of 256 and takes every tile's halves one after the other (K and V
+//               come once for 256 rows).
+// Step k of a stream: S = Q K^T (128 x 64, into one of the stream's two score buffers) -> softmax group: mask, running
+// maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). With two buffers the next
+// scores are computed while this step's are exponentiated, and the softmax groups never wait for the tensor cores in the
+// steady state (steps of 128 slots with one buffer a stream, whose chain scores - softmax - products was serial, took
+// 204 us where this takes TIME_LONG, 131,064 slots x 8 heads x 256 rows of bf16).
+// Bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.8 k cycles; TWO: the MMAs
+// 2.6 k (N = 64 reads Q more often than the tensor cores would like) and the exponentials (256 x 128 at 16 a cycle) 2 k.
 template <int D, bool TWO>
 struct TcShape {
     static constexpr int kStage = kTile * D * 2;
     static constexpr int kQ = (TWO ? 2 : 1) * 128 * D * 2;
     static constexpr int kStages = D == 64 ? 10 : TWO ? 5 : 6;
     static constexpr int kRows = TWO ? 256 : 128;
-    static constexpr int kLeast = TWO ? 1 : 2;  // one tile for each stream
+    static constexpr int kLeast = TWO ? 1 : 2;
+    static constexpr int kThreads = 352;
     static constexpr int kSmem = 1024 + kQ + kStages * kStage;
 };
 
 template <typename T, int D, bool TWO>
-__global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                                                         float *part_o, float2 *part_ml) {
+__global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk,
+                                                                              const __grid_constant__ CUtensorMap mv, float *part_o, float2 *part_ml) {
     using S_ = TcShape<D, TWO>;
     using H = Half16<T>;
-    constexpr int NST = S_::kStages, kBoxes = D / 64;
+    constexpr int NST = S_::kStages, kBoxes = D / 64, kStep = 64, PER = TWO ? 2 : 1;  // PER: a stream's steps of a tile
+    constexpr Cut cut{S_::kRows, kTile, S_::kLeast};
     extern __shared__ char dyn[];
     char *sq = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = sq + S_::kQ;
-    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2], b_p[2], b_pv[2], b_q, b_seg;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2][2], b_p[2][2], b_pv[2][2], b_q, b_seg, b_tail;  // [stream][score buffer]
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, Cut{S_::kRows, kTile, S_::kLeast}, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
@@ -326,16 +337,17 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
         map_prefetch(&mv);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
-            mbar_init(b_empty + i, 1);
+            mbar_init(b_empty + i, 2);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(b_s + i, 1);
-            mbar_init(b_p + i, 128);
-            mbar_init(b_pv + i, 1);
-            s_bad[i] = 0;
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&b_s[0][0] + i, 1);
+            mbar_init(&b_p[0][0] + i, 128);
+            mbar_init(&b_pv[0][0] + i, 1);
         }
         mbar_init(&b_q, 256);
         mbar_init(&b_seg, 256);
+        mbar_init(&b_tail, 256);
+        s_bad[0] = s_bad[1] = 0;
         s_gave_up = 0;
         fence_mbar_init();
     }
@@ -344,100 +356,88 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    Walk w(a, Cut{S_::kRows, kTile, S_::kLeast}, s_share);
+    Walk w(a, cut, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
-        auto load = [&](const CUtensorMap *m, int tile) {
-            const int st = n % NST;
-            wait(b_empty + st, (n / NST & 1) ^ 1);
-            if (lane == 0) {
-                mbar_expect_tx(b_full + st, S_::kStage);
-#pragma unroll
-                for (int x = 0; x < kBoxes; ++x) tma_load(ring + st * S_::kStage + x * 16384, m, 64 * x, tile * kTile, w.head(), w.b, b_full + st);
-            }
-            ++n;
-        };
         while (w.next()) {
-            const int nt = w.tb - w.ta;
-            if (TWO) {
-                for (int t = 0; t < nt; ++t) {
-                    load(&mk, w.ta + t);
-                    load(&mv, w.ta + t);
+            for (int t = w.ta; t < w.tb; ++t)
+                for (int z = 0; z < 2; ++z, ++n) {
+                    const int st = n % NST;
+                    wait(b_empty + st, (n / NST & 1) ^ 1);
+                    if (lane == 0) {
+                        mbar_expect_tx(b_full + st, S_::kStage);
+#pragma unroll
+                        for (int x = 0; x < kBoxes; ++x)
+                            tma_load(ring + st * S_::kStage + x * 16384, z ? &mv : &mk, 64 * x, t * kTile, w.head(), w.b, b_full + st);
+                    }
                 }
-            } else {  // in the order of use: K0 K1 V0 K2 V1 ...
-                load(&mk, w.ta);
-                if (nt > 1) load(&mk, w.ta + 1);
-                for (int t = 0; t < nt; ++t) {
-                    load(&mv, w.ta + t);
-                    if (t + 2 < nt) load(&mk, w.ta + t + 2);
-                }
-            }
             w.advance();
         }
         // nothing may be in flight into this CTA's shared memory when it ends
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
-    } else if (warp == 9) {  // ----------------------------------------------------------- MMAs
-        uint32_t base = 0, seg = 0, c_p[2] = {0, 0}, c_pv[2] = {0, 0};
-        constexpr uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(D, true);
+    } else if (warp > 8) {  // ----------------------------------------------------------- MMAs of stream s
+        const int s = warp - 9;
+        constexpr uint32_t id_s = idesc_of<T>(kStep, false), id_o = idesc_of<T>(D, true);
+        const uint32_t qa = smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0);
+        uint32_t base = 0, seg = 0, step = 0;  // ring position and the stream's step count at the segment's start
         while (w.next()) {
-            const int ns = (w.tb - w.ta) * (TWO ? 2 : 1);
+            const int ns = (w.tb - w.ta) * PER;
             wait(&b_q, seg & 1);
             tc_fence_after();
-            auto scores = [&](int i) {
-                const int s = i & 1;
-                const uint32_t at = base + (TWO ? 2 * (i / 2) : i < 2 ? i : 2 * i - 1), st = at % NST;
+            auto scores = [&](int k) {
+                const uint32_t at = base + 2 * (k / PER), st = at % NST, buf = (step + k) & 1;
                 wait(b_full + st, at / NST & 1);
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t qa = smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0), ka = smem_u32(ring + st * S_::kStage);
+                    const uint32_t ka = smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128);
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t o = (kk / 4) * 16384 + (kk % 4) * 32;
-                        mma_ss(tmem + 128 * s, desc_rows(qa + o), desc_rows(ka + o), id_s, kk != 0);
+                        mma_ss(tmem + 128 * s + 64 * buf, desc_rows(qa + o), desc_rows(ka + o), id_s, kk != 0);
                     }
-                    if (!TWO || s == 1) umma_commit(b_empty + st);
-                    umma_commit(b_s + s);
+                    if (k % PER == PER - 1) umma_commit(b_empty + st);
+                    umma_commit(&b_s[s][buf]);
                 }
                 __syncwarp();
             };
             scores(0);
             if (ns > 1) scores(1);
-            for (int i = 0; i < ns; ++i) {
-                const int s = i & 1;
-                const uint32_t at = base + (TWO ? 2 * (i / 2) + 1 : i + min(i + 2, ns)), st = at % NST;
-                wait(b_p + s, c_p[s]++ & 1);
+            for (int k = 0; k < ns; ++k) {
+                const uint32_t at = base + 2 * (k / PER) + 1, st = at % NST, buf = (step + k) & 1, use = (step + k) / 2 & 1;
+                wait(&b_p[s][buf], use);
                 wait(b_full + st, at / NST & 1);
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t va = smem_u32(ring + st * S_::kStage);
-                    // slots behind the drafted tokens are not multiplied, but for the rest of a step of 16
-                    const int real = w.len + w.n - (w.ta + (TWO ? i / 2 : i)) * kTile, steps = min(kTile / 16, (real + 15) / 16);
+                    const int half = TWO ? k & 1 : s;
+                    const uint32_t va = smem_u32(ring + st * S_::kStage) + half * (kStep * 128);
+                    // slots behind the drafted tokens are not multiplied, but for the rest of a group of 16
+                    const int groups = live_groups(w, w.ta + k / PER, half);
 #pragma unroll
-                    for (int kk = 0; kk < kTile / 16; ++kk)
-                        if (kk < steps) mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, desc_cols(va + kk * 2048), id_o, i >= 2 || kk != 0);
-                    if (!TWO || s == 1) umma_commit(b_empty + st);
-                    umma_commit(b_pv + s);
+                    for (int kk = 0; kk < kStep / 16; ++kk)
+                        if (kk < groups) mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 64 * buf + 8 * kk, desc_cols(va + kk * 2048), id_o, (k | kk) != 0);
+                    if (k % PER == PER - 1) umma_commit(b_empty + st);
+                    umma_commit(&b_pv[s][buf]);
                 }
                 __syncwarp();
-                if (i + 2 < ns) {
-                    wait(b_pv + s, c_pv[s] & 1);  // P is read: its columns may hold the next scores
-                    scores(i + 2);
+                if (k + 2 < ns) {
+                    wait(&b_pv[s][buf], use);  // P is read: its columns may hold new scores
+                    scores(k + 2);
                 }
-                ++c_pv[s];
             }
             base += 2 * (w.tb - w.ta);
+            step += ns;
             ++seg;
             w.advance();
         }
     } else {  // -------------------------------------------------------------------------- softmax
         const int s = warp / 4, r = tid & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, tS = tmem + 128 * s + lanes, tO = tmem + 256 + 128 * s + lanes;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, tO = tmem + 256 + 128 * s + lanes;
         const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // scores in base 2; 0 as a number that vanishes beside them
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-        uint32_t base = 0, seg = 0, c_s = 0, c_pv = 0;
+        uint32_t base = 0, seg = 0, step = 0, tails = 0;
         while (w.next()) {
-            const int ns = (w.tb - w.ta) * (TWO ? 2 : 1), h = w.head(), row0 = w.row0(), rows = w.n * a.group;
+            const int ns = (w.tb - w.ta) * PER, h = w.head(), row0 = w.row0(), rows = w.n * a.group;
             const int row = row0 + (TWO ? 128 * s : 0) + r;
             const bool live = row < rows;
             const bool warp_live = row0 + (TWO ? 128 * s : 0) + (warp & 3) * 32 < rows;
@@ -451,78 +451,73 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 if (w.n < 64) sees &= (1ull << w.n) - 1;
             }
             float m = -INFINITY, l = 0.f;
-            for (int i = s; i < ns; i += 2) {
-                const int tile = w.ta + (TWO ? i / 2 : i), key0 = tile * kTile;
-                const bool tail = key0 + kTile > w.len;
-                wait(b_s + s, c_s++ & 1);
+#pragma unroll 1
+            for (int k = 0; k < ns; ++k) {
+                const int half = TWO ? k & 1 : s, key0 = (w.ta + k / PER) * kTile + half * kStep;
+                const bool tail = key0 + kStep > w.len;
+                const uint32_t buf = (step + k) & 1, use = (step + k) / 2 & 1, tS = tmem + 128 * s + 64 * buf + lanes;
+                wait(&b_s[s][buf], use);
                 tc_fence_after();
                 if (warp_live) {
-                    // Two passes over the scores in chunks of 32, read from TMEM twice: half the registers, and a loop
-                    // body that is fetched once instead of straight code for 128 columns (few tiles pass through a CTA
-                    // of a short sequence, and fetching code would take it longer than running it).
-                    const int off = w.len - key0;  // the tile's columns before it are the sequence's
-                    const int chunks = min(4, (off + w.n + 31) / 32);
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int j = 0; j < chunks; ++j) {
-                        uint32_t x[32];
-                        tmem_ld32(tS + 32 * j, x);
-                        tmem_wait_ld(x);
-                        if (tail) hide(x, seen32(live, sees, off - 32 * j));
-                        float t4[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) t4[k] = __uint_as_float(x[k]);
-#pragma unroll
-                        for (int k = 4; k < 32; ++k) t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(x[k]));
-                        top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+                    uint32_t x[2][32], p[32];
+                    tmem_ld32(tS, x[0]);
+                    tmem_ld32(tS + 32, x[1]);
+                    tmem_wait_ld(x[0]);
+                    tmem_waited(x[1]);
+                    if (tail) {
+                        const int off = w.len - key0;  // the step's columns before it are the sequence's
+                        hide(x[0], seen32(live, sees, off));
+                        hide(x[1], seen32(live, sees, off - 32));
                     }
+                    float t4[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(__uint_as_float(x[0][j]), __uint_as_float(x[1][j]));
+#pragma unroll
+                    for (int j = 4; j < 32; ++j) t4[j & 3] = fmaxf(t4[j & 3], fmaxf(__uint_as_float(x[0][j]), __uint_as_float(x[1][j])));
+                    float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                     top = top == -INFINITY ? m : fmaxf(m, top * c);
                     if (m == -INFINITY) m = top;  // nothing summed so far
                     const bool raise = top > m + H::kSlack;
                     if (__any_sync(0xffffffffu, raise)) {
+                        wait(&b_pv[s][buf ^ 1], (step + k - 1) / 2 & 1);  // the step before has added its products (a first step never raises)
+                        tc_fence_after();
                         const float f = raise ? ex2(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
 #pragma unroll 1
                         for (int j = 0; j < D / 32; ++j) {
-                            uint32_t o[32];
-                            tmem_ld32(tO + 32 * j, o);
-                            tmem_wait_ld(o);
+                            tmem_ld32(tO + 32 * j, p);
+                            tmem_wait_ld(p);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tmem_st32(tO + 32 * j, o);
+                            for (int i = 0; i < 32; ++i) p[i] = __float_as_uint(__uint_as_float(p[i]) * f);
+                            tmem_st32(tO + 32 * j, p);
                         }
                     }
                     const float sub = m == -INFINITY ? 0.f : H::kLift - m;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-                    for (int j = 0; j < chunks; ++j) {
-                        uint32_t x[32], p[16];
-                        tmem_ld32(tS + 32 * j, x);
-                        tmem_wait_ld(x);
-                        if (tail) hide(x, seen32(live, sees, off - 32 * j));
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float p0 = ex2(fmaf(__uint_as_float(x[2 * k]), c, sub)), p1 = ex2(fmaf(__uint_as_float(x[2 * k + 1]), c, sub));
-                            l4[k & 1] += p0;
-                            l4[2 + (k & 1)] += p1;
-                            p[k] = H::pack(p0, p1);
-                        }
-                        tmem_st16(tS + 16 * j, p);  // over scores that have been read: 16 j + 15 < 32 (j + 1)
+                    for (int j = 0; j < 32; ++j) {
+                        const float p0 = ex2(fmaf(__uint_as_float(x[j / 16][2 * (j % 16)]), c, sub));
+                        const float p1 = ex2(fmaf(__uint_as_float(x[j / 16][2 * (j % 16) + 1]), c, sub));
+                        l4[j & 1] += p0;
+                        l4[2 + (j & 1)] += p1;
+                        p[j] = H::pack(p0, p1);
                     }
+                    tmem_st32(tS, p);  // over the scores
                     l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     tmem_wait_st();
                 }
-                if (tail && (!TWO || s == 0)) {
+                if (tail) {
                     // Weights are 0 where a row does not see a slot, but 0 times an infinity is not: rows of V behind the
-                    // drafted tokens (up to the next 16) become zero, and so do a drafted token's infinities and NaN, which reach the rows
-                    // that do see it at the segment's end.
-                    const uint32_t at = base + (TWO ? 2 * (i / 2) + 1 : i + min(i + 2, ns)), st = at % NST;
+                    // drafted tokens (up to the next 16) become zero, and so do a drafted token's infinities and NaN, which
+                    // reach the rows that do see it at the segment's end. TWO: both groups use these rows, and clean every
+                    // other one.
+                    const uint32_t at = base + 2 * (k / PER) + 1, st = at % NST;
                     wait(b_full + st, at / NST & 1);
-                    const int first = max(0, w.len - key0), real = w.len + w.n - key0;
-                    for (int k = r; k < (min(kTile, (real + 15) / 16 * 16) - first) * (D / 8); k += 128) {
-                        const int y = first + k / (D / 8), ch = k % (D / 8);
-                        uint4 *v = reinterpret_cast<uint4 *>(ring + st * S_::kStage + (ch / 8) * 16384 + y * 128 + ((ch % 8) ^ (y % 8)) * 16);
+                    const int first = max(0, w.len - key0), real = w.len + w.n - key0, last = 16 * live_groups(w, w.ta + k / PER, half);
+                    for (int i = TWO ? 2 * r + s : r; i < (last - first) * (D / 8); i += TWO ? 256 : 128) {
+                        const int y = first + i / (D / 8), ch = i % (D / 8);
+                        uint4 *v = reinterpret_cast<uint4 *>(ring + st * S_::kStage + (ch / 8) * 16384 + (half * kStep + y) * 128 + ((ch % 8) ^ (y % 8)) * 16);
                         if (y >= real) {
                             *v = make_uint4(0, 0, 0, 0);
                         } else {
@@ -540,16 +535,19 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                         }
                     }
                     fence_proxy_async();
+                    if (TWO) {
+                        mbar_arrive(&b_tail);
+                        wait(&b_tail, tails++ & 1);
+                    }
                 }
                 tc_fence_before();
-                mbar_arrive(b_p + s);
-                ++c_pv;
+                mbar_arrive(&b_p[s][buf]);
             }
-            const int mine = (ns - s + 1) / 2;
-            if (mine > 0) wait(b_pv + s, (c_pv - 1) & 1);
+            const uint32_t last = step + ns - 1;
+            wait(&b_pv[s][last & 1], last / 2 & 1);
             tc_fence_after();
             if (!TWO) {  // the stream's statistics for the other group, over its scores, which are done with
-                tmem_st2(tS, m, l);
+                tmem_st2(tmem + 128 * s + lanes, m, l);
                 tmem_wait_st();
                 tc_fence_before();
             }
@@ -558,21 +556,17 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
             tc_fence_after();
             if (tid == 0) s_bad[(seg + 1) & 1] = 0;
             const unsigned long long bad = s_bad[seg & 1] & sees;
-            // out = sum over this thread's streams of f O, in columns [x0, x1)
+            // out = sum over this thread's streams of f O, in columns [x0, x0 + width)
             float f0 = 1.f, f1 = 0.f;
-            int x0 = 0, x1 = D;
-            bool both = false;
+            constexpr int width = TWO ? D : D / 2;
+            const int x0 = TWO ? 0 : s * width;
             if (!TWO) {
                 const float2 o = tmem_ld2(tmem + 128 * (s ^ 1) + lanes);
                 const float m0 = s ? o.x : m, m1 = s ? m : o.x, l0 = s ? o.y : l, l1 = s ? l : o.y;
-                both = ns > 1;
-                const float top = fmaxf(m0, m1);
-                f0 = m0 == top ? 1.f : ex2(m0 - top);
-                f1 = m1 == top ? 1.f : ex2(m1 - top);
-                m = top;
-                l = both ? l0 * f0 + l1 * f1 : l0;
-                x0 = s * (D / 2);
-                x1 = x0 + D / 2;
+                m = fmaxf(m0, m1);
+                f0 = m0 == m ? 1.f : ex2(m0 - m);
+                f1 = m1 == m ? 1.f : ex2(m1 - m);
+                l = l0 * f0 + l1 * f1;
             }
             if (warp_live) {
                 const bool whole = w.whole();
@@ -583,36 +577,34 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
                 float *po = part_o + pr * D;
                 const uint32_t t0 = tmem + 256 + lanes + (TWO ? 128 * s : 0) + x0;
 #pragma unroll 1
-                for (int j = 0; j < x1 - x0; j += 32) {
+                for (int j = 0; j < width; j += 32) {
                     uint32_t o[32];
                     tmem_ld32(t0 + j, o);
                     tmem_wait_ld(o);
                     if (!TWO) {
-                        if (both) {
-                            uint32_t o1[32];
-                            tmem_ld32(t0 + 128 + j, o1);
-                            tmem_wait_ld(o1);
+                        uint32_t o1[32];
+                        tmem_ld32(t0 + 128 + j, o1);
+                        tmem_wait_ld(o1);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o[k]) * f0));
-                        }
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o1[i]), f1, __uint_as_float(o[i]) * f0));
                     }
                     if (live && whole) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
+                        for (int i = 0; i < 32; i += 8) {
                             uint32_t q[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) q[e] = H::pack(__uint_as_float(o[k + 2 * e]) * inv, __uint_as_float(o[k + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4 *>(out + x0 + j + k) = make_uint4(q[0], q[1], q[2], q[3]);
+                            for (int e = 0; e < 4; ++e) q[e] = H::pack(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(out + x0 + j + i) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
                     } else if (live) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(po + x0 + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4 *>(po + x0 + j + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
                 if (live && bad) {
                     const T *v = static_cast<const T *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)w.len * a.vs[2];
-                    if (whole) add_bad(out, v, a.vs[2], bad, x0, x1);
-                    else add_bad(po, v, a.vs[2], bad, x0, x1);
+                    if (whole) add_bad(out, v, a.vs[2], bad, x0, x0 + width);
+                    else add_bad(po, v, a.vs[2], bad, x0, x0 + width);
                 }
                 if (live && x0 == 0) {
                     if (!whole) part_ml[pr] = make_float2(m, l);
@@ -621,6 +613,7 @@ __global__ void __launch_bounds__(320, 1) k_tree_attn_tc(const AttnArgs a, const
             }
             tc_fence_before();
             base += 2 * (w.tb - w.ta);
+            step += ns;
             ++seg;
             w.advance();
         }
@@ -1414,8 +1407,8 @@ p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, 
 template <typename T, int D>
 p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     constexpr float lift = Half16<T>::kLift;
-    if (a.tokens * a.group > 128) return run_attn<T, D>(k_tree_attn_tc<T, D, true>, 320, TcShape<D, true>::kSmem, lift, c, a, ws, st);
-    return run_attn<T, D>(k_tree_attn_tc<T, D, false>, 320, TcShape<D, false>::kSmem, lift, c, a, ws, st);
+    if (a.tokens * a.group > 128) return run_attn<T, D>(k_tree_attn_tc<T, D, true>, TcShape<D, true>::kThreads, TcShape<D, true>::kSmem, lift, c, a, ws, st);
+    return run_attn<T, D>(k_tree_attn_tc<T, D, false>, TcShape<D, false>::kThreads, TcShape<D, false>::kSmem, lift, c, a, ws, st);
 }
 template <int D>
 p8_status run_f32(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
