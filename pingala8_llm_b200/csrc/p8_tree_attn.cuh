@@ -181,6 +181,14 @@ __host__ __device__ constexpr uint32_t idesc_of(int n, bool b_cols) {  // f32 ac
     const uint32_t f = Half16<T>::bf16 ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | ((b_cols ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
+// One thread of the warp, chosen so that the compiler knows the branch to be the warp's: the MMAs' operands then stay in
+// uniform registers (under `lane == 0`, with a descriptor put together for each, an MMA took 91 cycles to issue, where a
+// 128 x 128 x 16 one runs for 64).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred P;\n elect.sync _|P, 0xffffffff;\n selp.b32 %0, 1, 0, P;\n}\n" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(da), "l"(db),
                  "r"(idesc), "r"(acc)
@@ -377,9 +385,9 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         // nothing may be in flight into this CTA's shared memory when it ends
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
     } else if (warp > 8) {  // ----------------------------------------------------------- MMAs of stream s
-        const int s = warp - 9;
+        const int s = __shfl_sync(0xffffffffu, warp, 0) - 9;
         constexpr uint32_t id_s = idesc_of<T>(kStep, false), id_o = idesc_of<T>(D, true);
-        const uint32_t qa = smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0);
+        const uint64_t dq = desc_rows(smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0));
         uint32_t base = 0, seg = 0, step = 0;  // ring position and the stream's step count at the segment's start
         while (w.next()) {
             const int ns = (w.tb - w.ta) * PER;
@@ -389,12 +397,14 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                 const uint32_t at = base + 2 * (k / PER), st = at % NST, buf = (step + k) & 1;
                 wait(b_full + st, at / NST & 1);
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t ka = smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128);
+                const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128));
+                const uint32_t to = tmem + 128 * s + 64 * buf;
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t o = (kk / 4) * 16384 + (kk % 4) * 32;
-                        mma_ss(tmem + 128 * s + 64 * buf, desc_rows(qa + o), desc_rows(ka + o), id_s, kk != 0);
+                        constexpr uint32_t kUnit = 16;  // of a descriptor's address
+                        const uint32_t o = ((kk / 4) * 16384 + (kk % 4) * 32) / kUnit;
+                        mma_ss(to, dq + o, dk + o, id_s, kk != 0);
                     }
                     if (k % PER == PER - 1) umma_commit(b_empty + st);
                     umma_commit(&b_s[s][buf]);
@@ -408,14 +418,18 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                 wait(&b_p[s][buf], use);
                 wait(b_full + st, at / NST & 1);
                 tc_fence_after();
-                if (lane == 0) {
-                    const int half = TWO ? k & 1 : s;
-                    const uint32_t va = smem_u32(ring + st * S_::kStage) + half * (kStep * 128);
-                    // slots behind the drafted tokens are not multiplied, but for the rest of a group of 16
-                    const int groups = live_groups(w, w.ta + k / PER, half);
+                const int half = TWO ? k & 1 : s;
+                const uint64_t dv = desc_cols(smem_u32(ring + st * S_::kStage) + half * (kStep * 128));
+                const uint32_t to = tmem + 256 + 128 * s, from = tmem + 128 * s + 64 * buf;
+                // slots behind the drafted tokens are not multiplied, but for the rest of a group of 16
+                const int groups = live_groups(w, w.ta + k / PER, half);
+                if (elect_one()) {
+                    if (groups == kStep / 16) {
 #pragma unroll
-                    for (int kk = 0; kk < kStep / 16; ++kk)
-                        if (kk < groups) mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 64 * buf + 8 * kk, desc_cols(va + kk * 2048), id_o, (k | kk) != 0);
+                        for (int kk = 0; kk < kStep / 16; ++kk) mma_ts(to, from + 8 * kk, dv + kk * 128, id_o, (k | kk) != 0);
+                    } else {
+                        for (int kk = 0; kk < groups; ++kk) mma_ts(to, from + 8 * kk, dv + kk * 128, id_o, (k | kk) != 0);
+                    }
                     if (k % PER == PER - 1) umma_commit(b_empty + st);
                     umma_commit(&b_pv[s][buf]);
                 }
@@ -751,12 +765,12 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
                 for (int r0 = 0; r0 < rows; r0 += 256) {
                     wait(b_free + s, (c_free[s]++ & 1) ^ 1);
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t ka = smem_u32(ring + st * S_::kStage), qa = smem_u32(sq) + r0 * 128;
-                        const uint32_t id = idesc_of<T>((min(rows - r0, 256) + 15) / 16 * 16, false);
+                    const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage)), dq = desc_rows(smem_u32(sq) + r0 * 128);
+                    const uint32_t id = idesc_of<T>((min(rows - r0, 256) + 15) / 16 * 16, false), to = tmem + 256 * s;
+                    if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            mma_ss(tmem + 256 * s, desc_rows(ka + (kk / 4) * 16384 + (kk % 4) * 32), desc_rows(qa + (kk / 4) * kAtom + (kk % 4) * 32), id, kk != 0);
+                            mma_ss(to, dk + ((kk / 4) * 16384 + (kk % 4) * 32) / 16, dq + ((kk / 4) * kAtom + (kk % 4) * 32) / 16, id, kk != 0);
                         if (r0 + 256 >= rows) umma_commit(b_empty + st);
                         umma_commit(b_s + s);
                     }
