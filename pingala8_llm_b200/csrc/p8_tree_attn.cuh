@@ -19,13 +19,16 @@ struct AttnArgs {
 };
 
 // A unit is (sequence, cache head, block of query rows); its slots are cut into tiles. All tiles of all units
-// form one list, sequence by sequence, and every CTA takes an equal contiguous share of it, so that the SMs finish
-// together whatever the lengths are, and one long sequence still fills them. A unit that lies in one share is finished
+// form one list, sequence by sequence, with a few places more for the beginning of each unit, and every CTA takes an
+// equal contiguous share of it, so that the SMs finish together whatever the lengths are, and one long sequence still
+// fills them. A unit that lies in one share is finished
 // there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
+constexpr int kStart = 1;    // of a 16-bit attention segment
 constexpr int kTile = 128;  // of a 16-bit cache; 64 of a 32-bit one (as many bytes)
 struct Cut {                // how a kernel cuts its work
     int rblock, tile;       // query rows of a unit, slots of a tile
     int least;              // tiles of a share, at least
+    int start;              // what it costs to begin a segment, in tiles
 };
 
 struct Share {
@@ -36,7 +39,7 @@ struct Share {
 struct Walk {               // a CTA's way through its share, one segment (the tiles of one unit) at a time
     const AttnArgs &a;
     const Cut cut;
-    int pos, end, off, b, len, n, nt, units, u, ta, tb;
+    int pos, end, off, b, len, n, nt, units, u, ta, tb, step;
     bool opens;             // the segment is the share's first
     __device__ Walk(const AttnArgs &a_, Cut c, const Share &s)
         : a(a_), cut(c), pos(s.pos), end(s.end), off(s.off), b(s.b), len(s.len), n(s.n), opens(true) {
@@ -47,21 +50,29 @@ struct Walk {               // a CTA's way through its share, one segment (the t
         units = n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) : 0;
     }
     __device__ bool next() {
-        if (pos >= end) return false;
-        while (off >= units * nt) {
-            off -= units * nt;
-            ++b;
-            if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
-            count();
+        while (pos < end) {
+            const int cost = nt + cut.start;
+            if (off >= units * cost) {
+                off -= units * cost;
+                ++b;
+                if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) n = 0;
+                count();
+                continue;
+            }
+            u = off / cost;
+            const int in = off - u * cost;  // the unit's first `start` places stand for its beginning
+            ta = max(0, in - cut.start);
+            step = min(cost - in, end - pos);
+            tb = in + step - cut.start;
+            if (tb > ta) return true;
+            pos += step;
+            off += step;
         }
-        u = off / nt;
-        ta = off - u * nt;
-        tb = min(nt, ta + (end - pos));
-        return true;
+        return false;
     }
     __device__ void advance() {
-        pos += tb - ta;
-        off += tb - ta;
+        pos += step;
+        off += step;
         opens = false;
     }
     __device__ int blocks() const { return units / a.kvh; }
@@ -76,7 +87,7 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs &a, Cut cut, int b, int 
         *bad = true;
         n = 0;
     }
-    return n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) * ((len + n + cut.tile - 1) / cut.tile) : 0;
+    return n ? a.kvh * ((n * a.group + cut.rblock - 1) / cut.rblock) * ((len + n + cut.tile - 1) / cut.tile + cut.start) : 0;
 }
 __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
@@ -230,37 +241,32 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
         : "memory");
 }
 #undef P8_R16
-__device__ __forceinline__ void tmem_st2(uint32_t at, float x, float y) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
-}
-__device__ __forceinline__ float2 tmem_ld2(uint32_t at) {
-    float2 v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];\n tcgen05.wait::ld.sync.aligned;" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
-// Q rows [row0, row0 + tiles * 128) of a unit into swizzled shared memory, 16 bytes a thread and step; rows behind the
-// last are zero. flip: the sign bits (a negative scale is taken as its magnitude and -q).
+// Rows [row0, row0 + 128 tiles) of a unit's queries into swizzled shared memory, by one warp. Places behind the last row
+// keep what they had: a row of the products depends on no other. flip: the sign bits (a negative scale is taken as its
+// magnitude and -q).
 template <typename T, int D>
-__device__ __forceinline__ void load_q(char *sq, const AttnArgs &a, int b, int h, int row0, int rows, int tiles, uint32_t flip, int tid, int threads) {
-    constexpr int C = D / 8;
-    const T *q = static_cast<const T *>(a.q) + b * a.qs[0];
-    for (int i = tid; i < tiles * 128 * C; i += threads) {
-        const int c = i % C, r = i / C, row = row0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < rows) {
-            const int t = row / a.group, g = row - t * a.group;
-            v = *reinterpret_cast<const uint4 *>(q + t * a.qs[1] + (long long)(h * a.group + g) * a.qs[2] + c * 8);
-            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-        }
-        char *at = sq + (r / 128) * (128 * D * 2) + (c / 8) * 16384 + (r % 128) * 128 + (((c % 8) ^ (r % 8)) * 16);
-        *reinterpret_cast<uint4 *>(at) = v;
+__device__ __forceinline__ void load_q(char *sq, const AttnArgs &a, int b, int h, int row0, int rows, int tiles, uint32_t flip, int lane) {
+    constexpr int C = D / 8, STEP = 32 / C;
+    const int c = lane % C, n = min(tiles * 128, rows - row0);
+    const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + c * 8;
+    int t = (row0 + lane / C) / a.group, g = row0 + lane / C - t * a.group;
+    auto place = [&](int r) { return sq + (r / 128) * (128 * D * 2) + (c / 8) * 16384 + (r % 128) * 128 + (((c % 8) ^ (r % 8)) * 16); };
+    for (int r = lane / C; r < n; r += STEP) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(r))), "l"(q + t * a.qs[1] + (long long)(h * a.group + g) * a.qs[2]) : "memory");
+        for (g += STEP; g >= a.group; g -= a.group) ++t;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (flip)
+        for (int r = lane / C; r < n; r += STEP) {
+            uint4 *v = reinterpret_cast<uint4 *>(place(r));
+            *v = make_uint4(v->x ^ flip, v->y ^ flip, v->z ^ flip, v->w ^ flip);
+        }
 }
 
 // Which of 32 columns a row sees, where `off` of them are the sequence's and the drafted tokens follow.
@@ -294,8 +300,9 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
     }
 }
 
-// The tree attention kernel. Eleven warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
-// brings tiles of K and V into a ring by TMA, and one for each of two streams that issues its MMAs. A stream is a
+// The tree attention kernel. Twelve warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
+// brings tiles of K and V into a ring by TMA, one that brings queries, and one for each of two streams that issues its
+// MMAs. A stream is a
 // softmax group with its scores and its accumulator in TMEM; a step is 64 slots:
 //   TWO = false (at most 128 query rows): both streams have the same rows, stream s takes the slots 64 s .. of every
 //                tile; the accumulators are joined at the segment's end.
@@ -311,12 +318,13 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
 template <int D, bool TWO>
 struct TcShape {
     static constexpr int kStage = kTile * D * 2;
-    static constexpr int kQ = (TWO ? 2 : 1) * 128 * D * 2;
-    static constexpr int kStages = D == 64 ? 10 : TWO ? 5 : 6;
+    static constexpr int kQBufs = TWO ? 1 : 2;
+    static constexpr int kQ = 2 * 128 * D * 2;  // of 256 rows, or of 128 for this segment and the next
+    static constexpr int kStages = D == 64 ? 10 : 5;
     static constexpr int kRows = TWO ? 256 : 128;
     static constexpr int kLeast = TWO ? 1 : 2;
-    static constexpr int kThreads = 352;
-    static constexpr int kSmem = 1024 + kQ + kStages * kStage;
+    static constexpr int kThreads = 384;
+    static constexpr int kSmem = kQ + kStages * kStage;
 };
 
 template <typename T, int D, bool TWO>
@@ -324,15 +332,16 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                                                                               const __grid_constant__ CUtensorMap mv, float *part_o, float2 *part_ml) {
     using S_ = TcShape<D, TWO>;
     using H = Half16<T>;
-    constexpr int NST = S_::kStages, kBoxes = D / 64, kStep = 64, PER = TWO ? 2 : 1;  // PER: a stream's steps of a tile
-    constexpr Cut cut{S_::kRows, kTile, S_::kLeast};
-    extern __shared__ char dyn[];
-    char *sq = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = sq + S_::kQ;
-    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2][2], b_p[2][2], b_pv[2][2], b_q, b_seg, b_tail;  // [stream][score buffer]
+    constexpr int NST = S_::kStages, NQ = S_::kQBufs, kBoxes = D / 64, kStep = 64, PER = TWO ? 2 : 1;  // PER: a stream's steps of a tile
+    constexpr Cut cut{S_::kRows, kTile, S_::kLeast, kStart};
+    extern __shared__ __align__(1024) char dyn[];  // the swizzle goes by address bits
+    char *sq = dyn, *ring = sq + S_::kQ;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_q[2], b_qfree[2], b_s[2][2], b_p[2][2], b_pv[2][2], b_seg, b_read, b_tail;  // [stream][score buffer]
+    __shared__ float2 s_ml[2][TWO ? 1 : 128];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
-    __shared__ unsigned long long s_bad[2];
+    __shared__ unsigned long long s_bad[3];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
@@ -352,10 +361,14 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
             mbar_init(&b_p[0][0] + i, 128);
             mbar_init(&b_pv[0][0] + i, 1);
         }
-        mbar_init(&b_q, 256);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_q + i, 32);
+            mbar_init(b_qfree + i, 2);
+        }
         mbar_init(&b_seg, 256);
+        mbar_init(&b_read, 256);
         mbar_init(&b_tail, 256);
-        s_bad[0] = s_bad[1] = 0;
+        s_bad[0] = s_bad[1] = s_bad[2] = 0;
         s_gave_up = 0;
         fence_mbar_init();
     }
@@ -384,17 +397,28 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         }
         // nothing may be in flight into this CTA's shared memory when it ends
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+    } else if (warp == 11) {  // ---------------------------------------------------------- queries, a segment ahead where there is room
+        uint32_t seg = 0;
+        while (w.next()) {
+            const int qb = seg % NQ;
+            wait(b_qfree + qb, (seg / NQ & 1) ^ 1);
+            load_q<T, D>(sq + qb * (128 * D * 2), a, w.b, w.head(), w.row0(), w.n * a.group, TWO ? 2 : 1, a.scale < 0.f ? 0x80008000u : 0u, lane);
+            fence_proxy_async();
+            mbar_arrive(b_q + qb);
+            ++seg;
+            w.advance();
+        }
     } else if (warp > 8) {  // ----------------------------------------------------------- MMAs of stream s
         const int s = __shfl_sync(0xffffffffu, warp, 0) - 9;
         constexpr uint32_t id_s = idesc_of<T>(kStep, false), id_o = idesc_of<T>(D, true);
-        const uint64_t dq = desc_rows(smem_u32(sq) + (TWO ? s * (128 * D * 2) : 0));
         uint32_t base = 0, seg = 0, step = 0;  // ring position and the stream's step count at the segment's start
         while (w.next()) {
-            const int ns = (w.tb - w.ta) * PER;
-            wait(&b_q, seg & 1);
-            tc_fence_after();
+            const int ns = (w.tb - w.ta) * PER, qb = seg % NQ;
+            const uint64_t dq = desc_rows(smem_u32(sq) + (TWO ? s : qb) * (128 * D * 2));
+            wait(b_q + qb, seg / NQ & 1);
             auto scores = [&](int k) {
-                const uint32_t at = base + 2 * (k / PER), st = at % NST, buf = (step + k) & 1;
+                const uint32_t at = base + 2 * (k / PER), st = at % NST, g = step + k, buf = g & 1;
+                if (g >= 2) wait(&b_pv[s][buf], ((g - 2) / 2) & 1);  // the P that the buffer held is read
                 wait(b_full + st, at / NST & 1);
                 tc_fence_after();
                 const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128));
@@ -407,6 +431,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                         mma_ss(to, dq + o, dk + o, id_s, kk != 0);
                     }
                     if (k % PER == PER - 1) umma_commit(b_empty + st);
+                    if (k == ns - 1) umma_commit(b_qfree + qb);
                     umma_commit(&b_s[s][buf]);
                 }
                 __syncwarp();
@@ -434,10 +459,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     umma_commit(&b_pv[s][buf]);
                 }
                 __syncwarp();
-                if (k + 2 < ns) {
-                    wait(&b_pv[s][buf], use);  // P is read: its columns may hold new scores
-                    scores(k + 2);
-                }
+                if (k + 2 < ns) scores(k + 2);
             }
             base += 2 * (w.tb - w.ta);
             step += ns;
@@ -448,16 +470,13 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         const int s = warp / 4, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, tO = tmem + 256 + 128 * s + lanes;
         const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // scores in base 2; 0 as a number that vanishes beside them
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
         uint32_t base = 0, seg = 0, step = 0, tails = 0;
         while (w.next()) {
             const int ns = (w.tb - w.ta) * PER, h = w.head(), row0 = w.row0(), rows = w.n * a.group;
             const int row = row0 + (TWO ? 128 * s : 0) + r;
             const bool live = row < rows;
             const bool warp_live = row0 + (TWO ? 128 * s : 0) + (warp & 3) * 32 < rows;
-            load_q<T, D>(sq, a, w.b, h, row0, rows, TWO ? 2 : 1, flip, tid, 256);
-            fence_proxy_async();
-            mbar_arrive(&b_q);
+            if (tid == 0) s_bad[(seg + 1) % 3] = 0;  // last read two segments ago, next written after this one's b_seg
             unsigned long long sees = 0;
             if (live) {
                 const int t = row / a.group;
@@ -544,7 +563,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                             }
                             if (bad) {
                                 *v = make_uint4(q[0], q[1], q[2], q[3]);
-                                atomicOr(&s_bad[seg & 1], 1ull << (key0 + y - w.len));
+                                atomicOr(&s_bad[seg % 3], 1ull << (key0 + y - w.len));
                             }
                         }
                     }
@@ -555,27 +574,23 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     }
                 }
                 tc_fence_before();
+                if (!TWO && k == 0 && seg > 0) wait(&b_read, (seg - 1) & 1);  // both groups have read both accumulators
                 mbar_arrive(&b_p[s][buf]);
             }
             const uint32_t last = step + ns - 1;
             wait(&b_pv[s][last & 1], last / 2 & 1);
             tc_fence_after();
-            if (!TWO) {  // the stream's statistics for the other group, over its scores, which are done with
-                tmem_st2(tmem + 128 * s + lanes, m, l);
-                tmem_wait_st();
-                tc_fence_before();
-            }
+            if (!TWO) s_ml[s][r] = make_float2(m, l);
             mbar_arrive(&b_seg);
             wait(&b_seg, seg & 1);
             tc_fence_after();
-            if (tid == 0) s_bad[(seg + 1) & 1] = 0;
-            const unsigned long long bad = s_bad[seg & 1] & sees;
+            const unsigned long long bad = s_bad[seg % 3] & sees;
             // out = sum over this thread's streams of f O, in columns [x0, x0 + width)
             float f0 = 1.f, f1 = 0.f;
             constexpr int width = TWO ? D : D / 2;
             const int x0 = TWO ? 0 : s * width;
             if (!TWO) {
-                const float2 o = tmem_ld2(tmem + 128 * (s ^ 1) + lanes);
+                const float2 o = s_ml[s ^ 1][r];
                 const float m0 = s ? o.x : m, m1 = s ? m : o.x, l0 = s ? o.y : l, l1 = s ? l : o.y;
                 m = fmaxf(m0, m1);
                 f0 = m0 == m ? 1.f : ex2(m0 - m);
@@ -626,6 +641,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                 }
             }
             tc_fence_before();
+            if (!TWO) mbar_arrive(&b_read);
             base += 2 * (w.tb - w.ta);
             step += ns;
             ++seg;
@@ -660,12 +676,12 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
     const int each = share_of(total, cut, ctas);
     const int blocks = (n * a.group + cut.rblock - 1) / cut.rblock, nt = (len + n + cut.tile - 1) / cut.tile;
     const int h = head / a.group, row = t * a.group + head % a.group;
-    const int u0 = before + (h * blocks + row / cut.rblock) * nt, u1 = u0 + nt;
-    const int c0 = u0 / each, c1 = (u1 - 1) / each;
+    const int u0 = before + (h * blocks + row / cut.rblock) * (nt + cut.start), u1 = u0 + cut.start + nt;
+    const int c0 = (u0 + cut.start) / each, c1 = (u1 - 1) / each;
     if (c0 == c1) return;  // finished by that CTA
     // Everything so far came from the call's inputs, while the attention kernel ran; the parts are its outputs.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each != u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
+    auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
     float m = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[at(c)].x);
 #pragma unroll
@@ -713,7 +729,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
-        const Share s = find_share(a, Cut{1 << 30, kTile, 1}, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, Cut{1 << 30, kTile, 1, 0}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
         tmem_alloc(&s_tmem, 512);
@@ -736,7 +752,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    Walk w(a, Cut{1 << 30, kTile, 1}, s_share);
+    Walk w(a, Cut{1 << 30, kTile, 1, 0}, s_share);
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
@@ -936,7 +952,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
     __shared__ unsigned long long s_bad;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{R, kTile32, 1};
+    const Cut cut{R, kTile32, 1, 0};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
@@ -1207,7 +1223,7 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
     __shared__ float s_nl[S_::kRows];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{1 << 30, kTile32, 1};
+    const Cut cut{1 << 30, kTile32, 1, 0};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
@@ -1382,11 +1398,11 @@ int sm_count() {
 // Query rows of a unit: as few as hold them all, so that K and V are read once; the largest block has to be enough for
 // the rest (the last SM-sized part of a longer row list reads its tiles from L2).
 Cut attn_cut(const p8_kv *c, int64_t rows) {
-    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2};
-    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32, 1};
+    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2, kStart};
+    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32, 1, 0};
 }
 int64_t attn_tiles(const p8_kv *c, int64_t rows, Cut cut) {
-    return c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile);
+    return c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile + cut.start);
 }
 // CTAs of a call: no more than there can be tiles
 int attn_ctas(const p8_kv *c, int64_t rows, Cut cut) { return (int)std::min<int64_t>(sm_count(), attn_tiles(c, rows, cut)); }
@@ -1452,7 +1468,7 @@ template <typename T, int D>
 p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
-    const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1});
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1, 0});
     return mass_launches(a, 512, [&](const AttnArgs &x) {
         if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(x, mk);
         else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(x, mk);
@@ -1462,7 +1478,7 @@ template <int D>
 p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
-    const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1});
+    const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1, 0});
     return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, 288, F32Mass<D>::kSmem, st>>>(x, mk); });
 }
 template <int D>
