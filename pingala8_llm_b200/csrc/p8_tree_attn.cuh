@@ -322,7 +322,7 @@ struct TcShape {
     static constexpr int kQ = 2 * 128 * D * 2;  // of 256 rows, or of 128 for this segment and the next
     static constexpr int kStages = D == 64 ? 10 : 5;
     static constexpr int kRows = TWO ? 256 : 128;
-    static constexpr int kLeast = TWO ? 1 : 2;
+    static constexpr int kLeast = TWO ? 1 : 2 + kStart;
     static constexpr int kThreads = 384;
     static constexpr int kSmem = kQ + kStages * kStage;
 };
@@ -1398,7 +1398,7 @@ int sm_count() {
 // Query rows of a unit: as few as hold them all, so that K and V are read once; the largest block has to be enough for
 // the rest (the last SM-sized part of a longer row list reads its tiles from L2).
 Cut attn_cut(const p8_kv *c, int64_t rows) {
-    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2, kStart};
+    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2 + kStart, kStart};
     return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32, 1, 0};
 }
 int64_t attn_tiles(const p8_kv *c, int64_t rows, Cut cut) {
