@@ -654,8 +654,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
     if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// Adds up a unit's parts: one warp per query row; lanes find the largest maximum, then every lane sums its columns over
-// the parts in their order.
+// Adds up a unit's parts, one warp per query row, in the parts' order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
     const int lane = threadIdx.x % 32;
@@ -682,19 +681,41 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
     // Everything so far came from the call's inputs, while the attention kernel ran; the parts are its outputs.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
-    float m = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[at(c)].x);
+    // lane i has the statistics of parts c0 + i, c0 + i + 32, ..; the columns' loads do not wait for them
+    constexpr int W = D / 32, AHEAD = 8;
+    float m = -INFINITY, l = 0.f, acc[W] = {};
+    for (int c = c0; c <= c1; c += 32) {
+        const int cnt = min(32, c1 - c + 1);
+        const float2 ml = lane < cnt ? part_ml[at(c + lane)] : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, acc[D / 32] = {};
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-        const float2 ml = part_ml[at(c)];
-        const float f = ml.x == m ? 1.f : ex2(ml.x - m);
-        l = fmaf(ml.y, f, l);
-        const float *p = part_o + at(c) * D + lane * (D / 32);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, m);
+        const float f = ml.x == top ? 1.f : ex2(ml.x - top), old = m == top ? 1.f : ex2(m - top);
+        m = top;
+        float sum = ml.y * f;
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) acc[k] = fmaf(p[k], f, acc[k]);
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = fmaf(l, old, sum);
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k] *= old;
+        for (int i0 = 0; i0 < cnt; i0 += AHEAD) {
+            float v[AHEAD][W];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (i0 + i < cnt) {
+                    const float *p = part_o + at(c + i0 + i) * D + lane * W;
+                    if (W == 4) *reinterpret_cast<float4 *>(v[i]) = *reinterpret_cast<const float4 *>(p);
+                    else *reinterpret_cast<float2 *>(v[i]) = *reinterpret_cast<const float2 *>(p);
+                }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+                if (i0 + i < cnt)
+#pragma unroll
+                    for (int k = 0; k < W; ++k) acc[k] = fmaf(v[i][k], fi, acc[k]);
+            }
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *out = static_cast<T *>(a.out) + b * a.os[0] + t * a.os[1] + (long long)head * a.os[2] + lane * (D / 32);
@@ -887,31 +908,46 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
 // x = hi + lo, both TF32 (8 + 11 bits): x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y|, three mma.sync products with
 // fp32 sums. (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
 // more shared-memory traffic than the products take. From registers the split costs three integer or fp32 operations.)
-__device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
-    hi = __float_as_uint(x) & 0xFFFFE000u;
-    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
+// The products run through independent sums first (N of them, then the next piece): each waits for the one before on
+// the same sum.
+struct Split {
+    uint32_t hi, lo;  // the tensor cores leave out the last 13 bits
+};
+__device__ __forceinline__ Split split(float x) {
+    Split s;
+    s.hi = __float_as_uint(x) & 0xFFFFE000u;
+    s.lo = __float_as_uint(x - __uint_as_float(s.hi));
+    return s;
 }
 __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-struct Frag {  // a 16 x 8 left operand in two pieces
-    uint32_t hi[4], lo[4];
+struct Frag {  // a 16 x 8 left operand
+    Split x[4];
     __device__ __forceinline__ Frag(float x0, float x1, float x2, float x3) {
-        split(x0, hi[0], lo[0]);
-        split(x1, hi[1], lo[1]);
-        split(x2, hi[2], lo[2]);
-        split(x3, hi[3], lo[3]);
+        x[0] = split(x0);
+        x[1] = split(x1);
+        x[2] = split(x2);
+        x[3] = split(x3);
     }
 };
-__device__ __forceinline__ void mma_split(float (&c)[4], const Frag &a, float b0, float b1) {
-    uint32_t h0, l0, h1, l1;
-    split(b0, h0, l0);
-    split(b1, h1, l1);
-    mma8(c, a.hi[0], a.hi[1], a.hi[2], a.hi[3], l0, l1);
-    mma8(c, a.lo[0], a.lo[1], a.lo[2], a.lo[3], h0, h1);
-    mma8(c, a.hi[0], a.hi[1], a.hi[2], a.hi[3], h0, h1);
+// c[i] += a (b0[i], b1[i]) for N sums
+template <int N>
+__device__ __forceinline__ void mma_split(float (&c)[N][4], const Frag &a, const float (&b0)[N], const float (&b1)[N]) {
+    Split u[N], v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u[i] = split(b0[i]);
+        v[i] = split(b1[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u[i].lo, v[i].lo);
+#pragma unroll
+    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].lo, a.x[1].lo, a.x[2].lo, a.x[3].lo, u[i].hi, v[i].hi);
+#pragma unroll
+    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u[i].hi, v[i].hi);
 }
 constexpr int kTile32 = 64;
 // A stage holds 64 slots in parts of 32 columns as the tensor map's loads leave them: 128-byte rows, the 16-byte pieces
@@ -925,7 +961,7 @@ __device__ __forceinline__ float4 *query32(char *sq, int row, int col4) {
     return reinterpret_cast<float4 *>(sq + row * (D * 4) + (col4 ^ ((row & 1) << 2)) * 16);
 }
 
-// RT row tiles of 16 x 8 / RT groups of slots: warp w has row tile w % RT and the slots of group w / RT in every tile,
+// RT row tiles of 16 x KG = 8 / RT groups of slots: warp w has row tile w / KG and the slots of group w % KG in every tile,
 // with its own running maximum, sum and accumulator; the groups are joined at the segment's end. No barrier but the
 // ring's in between. Within the products the columns of K (and the slots in S and P) are taken in the order in which a
 // lane finds them in 16 consecutive bytes: the sums do not depend on it.
@@ -989,7 +1025,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
         return;
     }
-    const int rt = warp % RT, kg = warp / RT, g = lane / 4, t = lane % 4;
+    const int rt = warp / KG, kg = warp % KG, g = lane / 4, t = lane % 4;  // (so that the four schedulers share the row tiles that are there)
     const float c = a.scale * 1.4426950408889634f;
     uint32_t n = 0;
     while (w.next()) {
@@ -1032,12 +1068,14 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                 for (int d = 0; d < D / 16; ++d) {
                     const float4 q0 = *query32<D>(sq, 16 * rt + g, 4 * d + t), q1 = *query32<D>(sq, 16 * rt + g + 8, 4 * d + t);
                     const Frag fa(q0.x, q1.x, q0.y, q1.y), fb(q0.z, q1.z, q0.w, q1.w);
+                    float b[4][NK];
 #pragma unroll
                     for (int j = 0; j < NK; ++j) {
                         const float4 k = stage32(st, slot + 8 * j, 4 * d + t);
-                        mma_split(s[j], fa, k.x, k.y);
-                        mma_split(s[j], fb, k.z, k.w);
+                        b[0][j] = k.x; b[1][j] = k.y; b[2][j] = k.z; b[3][j] = k.w;
                     }
+                    mma_split(s, fa, b[0], b[1]);
+                    mma_split(s, fb, b[2], b[3]);
                 }
             }
             __syncwarp();
@@ -1117,10 +1155,8 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                     for (int x = 0; x < D / 32; ++x) {
                         const int col4 = 8 * x + (g >> 1) + ((g & 1) << 2);
                         const float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
-                        mma_split(o[x][0], p, u.x, v.x);
-                        mma_split(o[x][1], p, u.y, v.y);
-                        mma_split(o[x][2], p, u.z, v.z);
-                        mma_split(o[x][3], p, u.w, v.w);
+                        const float b0[4] = {u.x, u.y, u.z, u.w}, b1[4] = {v.x, v.y, v.z, v.w};
+                        mma_split(o[x], p, b0, b1);
                     }
                 }
             }
@@ -1141,7 +1177,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                 for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float4 *>(join + (((warp - RT) * 16 + g + 8 * y) * D + 32 * x + 16 * e + 4 * t) * 4) =
+                        *reinterpret_cast<float4 *>(join + ((((kg - 1) * RT + rt) * 16 + g + 8 * y) * D + 32 * x + 16 * e + 4 * t) * 4) =
                             make_float4(o[x][0][2 * y + e], o[x][1][2 * y + e], o[x][2][2 * y + e], o[x][3][2 * y + e]);
             }
         }
@@ -1153,12 +1189,12 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                 const int row = row0 + 16 * rt + g + 8 * y;
                 float top = m[y];
 #pragma unroll
-                for (int k = 1; k < KG; ++k) top = fmaxf(top, s_ml[k * RT + rt][g + 8 * y].x);
+                for (int k = 1; k < KG; ++k) top = fmaxf(top, s_ml[rt * KG + k][g + 8 * y].x);
                 const float f0 = m[y] == top ? 1.f : ex2(m[y] - top);
                 float f[KG], sum = l[y] * f0;
 #pragma unroll
                 for (int k = 1; k < KG; ++k) {
-                    const float2 ml = s_ml[k * RT + rt][g + 8 * y];
+                    const float2 ml = s_ml[rt * KG + k][g + 8 * y];
                     f[k] = ml.x == top ? 1.f : ex2(ml.x - top);
                     sum = fmaf(ml.y, f[k], sum);
                 }
@@ -1303,17 +1339,17 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
                 from[e] = late <= 0 ? 0 : late < w.n ? late * a.gc : rows;
             }
             for (int r0 = 0; r0 < padded; r0 += 16) {
-                float s[4] = {};
+                float s0[1][4] = {}, s1[1][4] = {};  // two sums, so that their products need not wait for one another
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
                     const float4 q0 = *query32<D>(sq, r0 + g, 4 * d + t), q1 = *query32<D>(sq, r0 + g + 8, 4 * d + t);
-                    mma_split(s, Frag(q0.x, q1.x, q0.y, q1.y), k[d].x, k[d].y);
-                    mma_split(s, Frag(q0.z, q1.z, q0.w, q1.w), k[d].z, k[d].w);
+                    mma_split<1>(s0, Frag(q0.x, q1.x, q0.y, q1.y), {k[d].x}, {k[d].y});
+                    mma_split<1>(s1, Frag(q0.z, q1.z, q0.w, q1.w), {k[d].z}, {k[d].w});
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = r0 + g + 8 * (e >> 1);
-                    const float p = ex2(s[e] + s_nl[row]);
+                    const float p = ex2(s0[0][e] + s1[0][e] + s_nl[row]);
                     if (row >= from[e & 1] && row < rows) sum[e & 1] += p;
                 }
             }
