@@ -681,12 +681,19 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
     // Everything so far came from the call's inputs, while the attention kernel ran; the parts are its outputs.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
-    // lane i has the statistics of parts c0 + i, c0 + i + 32, ..; the columns' loads do not wait for them
-    constexpr int W = D / 32, AHEAD = 8;
+    constexpr int W = D / 32, AHEAD = 16;
     float m = -INFINITY, l = 0.f, acc[W] = {};
-    for (int c = c0; c <= c1; c += 32) {
-        const int cnt = min(32, c1 - c + 1);
+    for (int c = c0; c <= c1; c += AHEAD) {  // all loads of 16 parts at once; lane i has the statistics of part c + i
+        const int cnt = min(AHEAD, c1 - c + 1);
         const float2 ml = lane < cnt ? part_ml[at(c + lane)] : make_float2(-INFINITY, 0.f);
+        float v[AHEAD][W];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (i < cnt) {
+                const float *p = part_o + at(c + i) * D + lane * W;
+                if (W == 4) *reinterpret_cast<float4 *>(v[i]) = *reinterpret_cast<const float4 *>(p);
+                else *reinterpret_cast<float2 *>(v[i]) = *reinterpret_cast<const float2 *>(p);
+            }
         float top = ml.x;
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -699,22 +706,12 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
         l = fmaf(l, old, sum);
 #pragma unroll
         for (int k = 0; k < W; ++k) acc[k] *= old;
-        for (int i0 = 0; i0 < cnt; i0 += AHEAD) {
-            float v[AHEAD][W];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                if (i0 + i < cnt) {
-                    const float *p = part_o + at(c + i0 + i) * D + lane * W;
-                    if (W == 4) *reinterpret_cast<float4 *>(v[i]) = *reinterpret_cast<const float4 *>(p);
-                    else *reinterpret_cast<float2 *>(v[i]) = *reinterpret_cast<const float2 *>(p);
-                }
+        for (int i = 0; i < AHEAD; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            if (i < cnt)
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
-                if (i0 + i < cnt)
-#pragma unroll
-                    for (int k = 0; k < W; ++k) acc[k] = fmaf(v[i][k], fi, acc[k]);
-            }
+                for (int k = 0; k < W; ++k) acc[k] = fmaf(v[i][k], fi, acc[k]);
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1031,15 +1028,18 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
     while (w.next()) {
         const int h = w.head(), row0 = w.row0(), rows = w.n * a.group;
         const float *q = static_cast<const float *>(a.q) + w.b * a.qs[0];
-        for (int i = tid; i < R * (D / 4); i += 256) {
-            const int col4 = i % (D / 4), r = i / (D / 4), row = row0 + r;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < rows) {
-                const int tok = row / a.group;
-                v = *reinterpret_cast<const float4 *>(q + tok * a.qs[1] + (long long)(h * a.group + row - tok * a.group) * a.qs[2] + 4 * col4);
-                v.x *= c; v.y *= c; v.z *= c; v.w *= c;  // scores in base 2
-            }
-            *query32<D>(sq, r, col4) = v;
+        constexpr int C = D / 4, QN = R * C / 256;  // a thread's pieces of the query rows, all in flight at once
+        float4 qv[QN];
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int row = row0 + tid / C + i * (256 / C), tok = row / a.group;
+            qv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < rows) qv[i] = *reinterpret_cast<const float4 *>(q + tok * a.qs[1] + (long long)(h * a.group + row - tok * a.group) * a.qs[2] + 4 * (tid % C));
+        }
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const float4 v = qv[i];
+            *query32<D>(sq, tid / C + i * (256 / C), tid % C) = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);  // scores in base 2
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const bool warp_live = row0 + 16 * rt < rows;
@@ -1128,14 +1128,14 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
             ++n;
             if (warp_live) {
                 char *st = ring + sv * S_::kStage;
+                const int groups = (w.len + w.n - key0 + 7) / 8;  // of eight slots that hold something; the others are not multiplied
                 if (tail) {
-                    // A weight of 0 times an infinity is not 0: the warp's slots that no row sees become zero, and so do a
+                    // A weight of 0 times an infinity is not 0: the warp's slots that no row sees become zero (as far as they are multiplied), and so do a
                     // drafted token's infinities and NaN (they reach the rows that see it at the segment's end). Warps
                     // with other rows of the same slots write the same zeros.
 #pragma unroll 1
-                    for (int i = lane; i < NK * 8 * (D / 4); i += 32) {
+                    for (int i = max(0, w.len - key0) * (D / 4) + lane; i < min(NK, groups) * 8 * (D / 4); i += 32) {
                         const int slot = kg * NK * 8 + i / (D / 4), col4 = i % (D / 4), at = tile * kTile32 + slot - w.len;
-                        if (at < 0) continue;
                         float4 *v = reinterpret_cast<float4 *>(st + (col4 / 8) * 8192 + slot * 128 + ((col4 % 8) ^ (slot % 8)) * 16);
                         const float4 x = *v;
                         if (at < w.n && isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w)) continue;
@@ -1149,6 +1149,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                 }
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
+                    if (j >= groups) break;
                     const Frag p(s[j][0], s[j][2], s[j][1], s[j][3]);
                     const int slot = kg * NK * 8 + 8 * j + t;
 #pragma unroll
