@@ -130,8 +130,10 @@ __global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a) {
 
 // ----------------------------------------------------------------------------------------------------------------
 // eviction, step 1: the kept slots of one (layer, sequence, head). Radix select on an order-preserving 32-bit key in
-// three digits of 11, 11 and 10 bits finds the smallest kept key; then every warp walks a contiguous part of the
-// slots, so that the kept ones come out in order and, among equal keys, the lowest slots win.
+// three digits of 11, 11 and 10 bits finds the smallest kept key; then ballots and one scan over their counts give every
+// kept slot its place, so that they come out in order and, among equal keys, the lowest slots win. A thread holds 16
+// keys, loaded at once; a middle of more than 16 x 1024 slots is read in such pieces, once per digit and twice at the end.
+// Bound by its few dependent steps (a load, three histograms and scans), not by the 4 bytes a slot.
 struct EvictArgs {
     const float *mass;
     float *mass_out;
@@ -152,12 +154,16 @@ __device__ __forceinline__ uint32_t mass_key(float m) {  // larger mass, larger 
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+constexpr int kSelKeys = 16, kSelPiece = 1024 * kSelKeys;
+
 __global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
     __shared__ int hist[2048];
-    __shared__ int wsum[32], weq[32];
-    __shared__ int s_digit, s_above;
+    __shared__ int wsum[32];
+    __shared__ int cnt_gt[kSelKeys * 32], cnt_eq[kSelKeys * 32];
+    __shared__ int s_digit, s_above, s_gt, s_eq;
     const int row = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int len = a.lens[b];
     if (len < 0 || len > a.slots) {
         if (tid == 0) atomicOr(&g_cache_error, kErrRange);
@@ -169,25 +175,48 @@ __global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
         for (int i = tid; i < a.budget; i += 1024) kept[i] = i < len ? i : -1;
         return;
     }
-    const float *m = a.mass + layer * a.ms[0] + b * a.ms[1] + h * a.ms[2];
     const int need = a.budget - a.sinks - a.recent, lo = a.sinks, hi = len - a.recent, n = hi - lo;
+    const float *m = a.mass + layer * a.ms[0] + b * a.ms[1] + h * a.ms[2] + lo;
     for (int i = tid; i < a.sinks; i += 1024) kept[i] = i;
     for (int i = tid; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
     if (need == 0) return;
+    uint32_t key[kSelKeys];  // of slots lo + piece + 1024 j + tid
+    auto load = [&](int piece) {
+        float v[kSelKeys];
+#pragma unroll
+        for (int j = 0; j < kSelKeys; ++j)
+            if (piece + 1024 * j + tid < n) v[j] = m[piece + 1024 * j + tid];
+#pragma unroll
+        for (int j = 0; j < kSelKeys; ++j) key[j] = mass_key(v[j]);
+    };
+    const bool one = n <= kSelPiece;
+    if (one) load(0);
     uint32_t prefix = 0, fixed = 0;  // the threshold key's known bits, and which they are
     int left = need;                 // kept among the keys that share them
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
         hist[tid] = 0;
         hist[tid + 1024] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += 1024) {
-            const uint32_t k = mass_key(m[lo + i]);
-            if ((k & fixed) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+        for (int piece = 0; piece < n; piece += kSelPiece) {
+            if (!one) load(piece);
+#pragma unroll
+            for (int j = 0; j < kSelKeys; ++j) {
+                if (piece + 1024 * j + warp * 32 >= n) break;  // (the whole warp)
+                const bool in = piece + 1024 * j + tid < n && (key[j] & fixed) == prefix;
+                const unsigned int who = __ballot_sync(0xffffffffu, in);
+                if (!in) continue;
+                const int bin = (key[j] >> shift) & (bins - 1), first = __shfl_sync(who, bin, __ffs(who) - 1);
+                if (__all_sync(who, bin == first)) {  // alike, as digits of masses often are: one addition
+                    if (lane == __ffs(who) - 1) atomicAdd(&hist[bin], __popc(who));
+                } else {
+                    atomicAdd(&hist[bin], 1);
+                }
+            }
         }
         __syncthreads();
-        // thread t holds bins 2t' and 2t'+1 counted from the top; a scan over them finds the digit where `left` falls
+        // thread t holds two bins, counted from the top; a scan over them finds the digit where `left` falls
         const int hi_bin = bins - 1 - 2 * tid, lo_bin = hi_bin - 1;
         const int c0 = hi_bin > 0 ? hist[hi_bin] : 0, c1 = hi_bin > 0 ? hist[lo_bin] : 0;
         int sum = c0 + c1;
@@ -198,42 +227,61 @@ __global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
         }
         if (lane == 31) wsum[warp] = sum;
         __syncthreads();
-        int base = 0;
-        for (int w = 0; w < warp; ++w) base += wsum[w];
-        const int before = base + sum - c0 - c1;
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0) + sum - c0 - c1;
         if (before < left && left <= before + c0) { s_digit = hi_bin; s_above = before; }
         if (before + c0 < left && left <= before + c0 + c1) { s_digit = lo_bin; s_above = before + c0; }
         __syncthreads();
         prefix |= (uint32_t)s_digit << shift;
         fixed |= (uint32_t)(bins - 1) << shift;
         left -= s_above;
-        __syncthreads();
     }
     // keys above `prefix` are kept, and the first `left` of those equal to it
-    const int seg = ((n + 31) / 32 + 31) / 32 * 32, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
-    int gt = 0, eq = 0;
-    for (int i = s0 + lane; i < s1; i += 32) {
-        const uint32_t k = mass_key(m[lo + i]);
-        gt += k > prefix;
-        eq += k == prefix;
-    }
-    gt = __reduce_add_sync(0xffffffffu, gt);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    if (lane == 0) { wsum[warp] = gt; weq[warp] = eq; }
-    __syncthreads();
-    int gt0 = 0, eq0 = 0;
-    for (int w = 0; w < warp; ++w) { gt0 += wsum[w]; eq0 += weq[w]; }
-    int at = a.sinks + gt0 + min(eq0, left);
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t k = i < s1 ? mass_key(m[lo + i]) : 0u;
-        const bool e = i < s1 && k == prefix;
-        const unsigned int em = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1u;
-        const bool keep = i < s1 && (k > prefix || (e && eq0 + __popc(em & below) < left));
-        const unsigned int km = __ballot_sync(0xffffffffu, keep);
-        if (keep) kept[at + __popc(km & below)] = lo + i;
-        at += __popc(km);
-        eq0 += __popc(em);
+    int gt0 = 0, eq0 = 0;  // in the pieces before
+    for (int piece = 0; piece < n; piece += kSelPiece) {
+        if (!one) load(piece);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSelKeys; ++j) {
+            const bool in = piece + 1024 * j + tid < n;
+            const unsigned int g = __ballot_sync(0xffffffffu, in && key[j] > prefix), e = __ballot_sync(0xffffffffu, in && key[j] == prefix);
+            if (lane == 0) {
+                cnt_gt[32 * j + warp] = __popc(g);
+                cnt_eq[32 * j + warp] = __popc(e);
+            }
+        }
+        __syncthreads();
+        if (tid < 64) {  // two warps: exclusive scans over the 512 counts of each kind
+            int *c = tid < 32 ? cnt_gt : cnt_eq, v[kSelKeys], sum = 0;
+#pragma unroll
+            for (int i = 0; i < kSelKeys; ++i) {
+                v[i] = c[lane * kSelKeys + i];
+                sum += v[i];
+            }
+            int at = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += u;
+            }
+            if (lane == 31) *(tid < 32 ? &s_gt : &s_eq) = at;
+            at -= sum;
+#pragma unroll
+            for (int i = 0; i < kSelKeys; ++i) {
+                c[lane * kSelKeys + i] = at;
+                at += v[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSelKeys; ++j) {
+            const int i = piece + 1024 * j + tid;
+            const bool g = i < n && key[j] > prefix, e = i < n && key[j] == prefix;
+            const unsigned int gm = __ballot_sync(0xffffffffu, g), em = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1u;
+            const int eqs = eq0 + cnt_eq[32 * j + warp] + __popc(em & below);  // equal keys before this slot
+            if (g || (e && eqs < left)) kept[a.sinks + gt0 + cnt_gt[32 * j + warp] + __popc(gm & below) + min(eqs, left)] = lo + i;
+        }
+        gt0 += s_gt;
+        eq0 += s_eq;
     }
 }
 
@@ -242,6 +290,7 @@ __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
     const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     const int len = a.lens[b];
     if (len < 0 || len > a.slots) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for `kept`
     const int keep = min(len, a.budget), per = a.row_bytes / 16, rows = 256 / per;
     const int *kept = a.kept + (long long)row * a.budget;
     const char *s0 = a.src[0] + layer * a.ss[0][0] + b * a.ss[0][1] + h * a.ss[0][2], *s1 = a.src[1] + layer * a.ss[1][0] + b * a.ss[1][1] + h * a.ss[1][2];
@@ -309,6 +358,7 @@ __global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
     const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     const int len = a.lens[b];
     if (len <= a.budget || len > a.slots) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for `kept`
     const int *kept = a.kept + (long long)row * a.budget;
     const int z = blockIdx.z;
     if (z == 2) {
@@ -402,6 +452,22 @@ __global__ void __launch_bounds__(256) k_tree_accept(const AcceptArgs a) {
         for (int j = 0; j < 4; ++j)
             if (to[j]) *reinterpret_cast<uint4 *>(to[j]) = v[j];
     }
+}
+
+// A launch whose blocks may start while the launch before it in the stream still runs; they wait for its results
+// themselves (griddepcontrol.wait).
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 #include "p8_tree_attn.cuh"
@@ -564,13 +630,10 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     if (rows > 65535) return P8_ERR_UNSUPPORTED;
     cudaStream_t st = (cudaStream_t)stream;
     k_evict_select<<<(unsigned int)rows, 1024, 0, st>>>(k);
-    if (same) {
-        k_evict_slide<<<dim3((unsigned int)(k.row_bytes / 64), (unsigned int)rows, 3), 256, 0, st>>>(k);
-    } else {
-        const int chunk = 4 * (256 / (k.row_bytes / 16));
-        k_evict_copy<<<dim3((unsigned int)((a->budget + chunk - 1) / chunk), (unsigned int)rows), 256, 0, st>>>(k);
-    }
-    return launched();
+    if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
+    const int chunk = 4 * (256 / (k.row_bytes / 16));
+    const dim3 grid = same ? dim3((unsigned int)(k.row_bytes / 64), (unsigned int)rows, 3) : dim3((unsigned int)((a->budget + chunk - 1) / chunk), (unsigned int)rows);
+    return launch_after(same ? k_evict_slide : k_evict_copy, grid, dim3(256), st, k) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 
 p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream) {

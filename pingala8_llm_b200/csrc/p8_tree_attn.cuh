@@ -722,36 +722,38 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
 }
 
 // The mass kernel: S^T = K Q^T, a tile's 128 slots as the TMEM lanes and the query rows as its columns, so that a thread
-// holds one slot and its sum over rows needs no other thread. Two softmax groups take tiles in turn. Keys come through
-// a TMA ring, the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows
+// holds one slot and sums it over rows. Tiles go to two score buffers in turn, each with two groups of four warps that
+// take half of the rows each (four warps a scheduler hide the exponentials' latency: MASS_NOTE). Keys come through a TMA
+// ring, the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows
 // (32 KB a tile: 1.4 k cycles at 1/148 of the bandwidth), by the exponentials (8 cycles a row and tile) beyond.
 template <int D, int ROWS>
 struct MassShape {
     static constexpr int kStage = kTile * D * 2;
     static constexpr int kQ = ROWS * D * 2;
-    static constexpr int kStages = D == 64 ? 6 : ROWS == 256 ? 5 : 2;
-    static constexpr int kSmem = 1024 + kQ + kStages * kStage;
+    static constexpr int kStages = D == 64 ? 6 : ROWS == 256 ? 4 : 2;
+    static constexpr int kSmem = kQ + kStages * kStage;
 };
 
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
+__global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
     using S_ = MassShape<D, ROWS>;
     constexpr int NST = S_::kStages, kBoxes = D / 64, C = D / 8, kAtom = ROWS * 128;
-    extern __shared__ char dyn[];
-    char *sq = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = sq + S_::kQ;
+    extern __shared__ __align__(1024) char dyn[];
+    char *sq = dyn, *ring = sq + S_::kQ;
     __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2], b_free[2], b_q, b_seg;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
     __shared__ alignas(16) float s_nl[ROWS];
+    __shared__ float s_sum[2][2][128];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
         const Share s = find_share(a, Cut{1 << 30, kTile, 1, 0}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         tmem_alloc(&s_tmem, 512);
-    } else if (tid == 256) {
+    } else if (tid == 512) {
         map_prefetch(&mk);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
@@ -759,10 +761,10 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(b_s + i, 1);
-            mbar_init(b_free + i, 128);
+            mbar_init(b_free + i, 256);
         }
-        mbar_init(&b_q, 256);
-        mbar_init(&b_seg, 256);
+        mbar_init(&b_q, 512);
+        mbar_init(&b_seg, 512);
         s_gave_up = 0;
         fence_mbar_init();
     }
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     const uint32_t tmem = s_tmem;
     Walk w(a, Cut{1 << 30, kTile, 1, 0}, s_share);
 
-    if (warp == 8) {  // ---------------------------------------------------------------- loads
+    if (warp == 16) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
         while (w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
@@ -787,7 +789,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
             w.advance();
         }
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
-    } else if (warp == 9) {  // ----------------------------------------------------------- MMAs
+    } else if (warp == 17) {  // ----------------------------------------------------------- MMAs
         uint32_t n = 0, seg = 0, c_free[2] = {0, 0};
         while (w.next()) {
             const int rows = w.n * a.gc;
@@ -815,13 +817,13 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
             w.advance();
         }
     } else {  // -------------------------------------------------------------------------- sums
-        const int s = warp / 4, r = tid & 127;
+        const int s = warp / 4 & 1, half = warp / 8, r = tid & 127;
         const uint32_t tS = tmem + 256 * s + ((uint32_t)(warp & 3) << 21);
         const float c = a.scale * 1.4426950408889634f;
-        uint32_t seg = 0, c_s = 0;
+        uint32_t seg = 0, c_s = 0, it = 0;
         while (w.next()) {
             const int rows = w.n * a.gc, h = w.u;
-            for (int i = tid; i < (rows + 15) / 16 * 16 * C; i += 256) {
+            for (int i = tid; i < (rows + 15) / 16 * 16 * C; i += 512) {
                 const int ch = i % C, row = i / C;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 float nl = -INFINITY;
@@ -850,16 +852,18 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
                 const int key = t * kTile + r, late = key - w.len;
                 const bool tail = t * kTile + kTile > w.len;
                 float before = 0.f;
-                if (late < 0) before = min_[key];
-                else if (a.more && late < w.n) before = mout[key];
+                if (half == 0) {
+                    if (late < 0) before = min_[key];
+                    else if (a.more && late < w.n) before = mout[key];
+                }
                 const int from = late > 0 ? (late < w.n ? late * a.gc : rows) : 0;  // the first row that sees the slot
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int r0 = 0; r0 < rows; r0 += 256) {
                     wait(b_s + s, c_s++ & 1);
                     tc_fence_after();
-                    const int cnt = min(rows - r0, 256);
+                    const int all = min(rows - r0, 256), mid = (all + 63) / 64 * 32, cnt = half ? all : min(mid, all);
 #pragma unroll 1
-                    for (int j = 0; j < cnt; j += 32) {
+                    for (int j = half ? mid : 0; j < cnt; j += 32) {
                         uint32_t x[32];
                         tmem_ld32(tS + j, x);
                         tmem_wait_ld(x);
@@ -885,9 +889,16 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
                     tc_fence_before();
                     mbar_arrive(b_free + s);
                 }
-                if (late < w.n) mout[key] = before + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                float sums = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (rows > 32) {  // the other half's; two places by turns, so that one barrier a tile is enough
+                    float *other = &s_sum[s][it++ & 1][r];
+                    if (half) *other = sums;
+                    asm volatile("bar.sync %0, 256;" ::"r"(1 + s) : "memory");
+                    if (!half) sums += *other;
+                }
+                if (!half && late < w.n) mout[key] = before + sums;
             }
-            mbar_arrive(&b_seg);  // both groups have seen all of the segment's scores: its query rows are done with
+            mbar_arrive(&b_seg);  // all groups have seen all of the segment's scores: its query rows are done with
             wait(&b_seg, seg & 1);
             ++seg;
             w.advance();
@@ -896,7 +907,7 @@ __global__ void __launch_bounds__(320, 1) k_attn_mass_tc(const AttnArgs a, const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (warp == 17) tmem_dealloc(tmem, 512);
 }
 
 // ================================================================================================================
@@ -1460,16 +1471,8 @@ p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, 
     float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * cut.rblock * D);
     kernel<<<ctas, threads, smem, st>>>(a, mk, mv, po, ml);
     if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned int)(((long long)a.batch * a.tokens * a.heads + 7) / 8));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_attn_join<T, D>, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+    const dim3 grid((unsigned int)(((long long)a.batch * a.tokens * a.heads + 7) / 8));
+    return launch_after(k_attn_join<T, D>, grid, dim3(256), st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 template <typename T, int D>
 p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
@@ -1507,8 +1510,8 @@ p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1, 0});
     return mass_launches(a, 512, [&](const AttnArgs &x) {
-        if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 320, MassShape<D, 256>::kSmem, st>>>(x, mk);
-        else k_attn_mass_tc<T, D, 512><<<ctas, 320, MassShape<D, 512>::kSmem, st>>>(x, mk);
+        if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 576, MassShape<D, 256>::kSmem, st>>>(x, mk);
+        else k_attn_mass_tc<T, D, 512><<<ctas, 576, MassShape<D, 512>::kSmem, st>>>(x, mk);
     });
 }
 template <int D>
