@@ -129,11 +129,12 @@ __global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a) {
 }
 
 // ----------------------------------------------------------------------------------------------------------------
-// eviction, step 1: the kept slots of one (layer, sequence, head). Radix select on an order-preserving 32-bit key in
-// three digits of 11, 11 and 10 bits finds the smallest kept key; then ballots and one scan over their counts give every
-// kept slot its place, so that they come out in order and, among equal keys, the lowest slots win. A thread holds 16
-// keys, loaded at once; a middle of more than 16 x 1024 slots is read in such pieces, once per digit and twice at the end.
-// Bound by its few dependent steps (a load, three histograms and scans), not by the 4 bytes a slot.
+// eviction, step 1: the kept slots of one (layer, sequence, head). A radix select on an order-preserving 32-bit key, in
+// digits of 11, 11 and 10 bits, finds the smallest kept key; as soon as at most 1024 keys share its digits (after the
+// first one, for most masses) only they are looked at. Then ballots and one scan over their counts give every kept slot
+// its place, so that they come out in order and, among equal keys, the lowest slots win. Keys of up to 16384 slots stay in
+// shared memory (two blocks an SM), longer middles are read again for each step. Bound by its dependent steps, and with
+// many rows by the histogram's additions (two copies, for even and odd lanes, meet less often), not by the 4 bytes a slot.
 struct EvictArgs {
     const float *mass;
     float *mass_out;
@@ -154,16 +155,18 @@ __device__ __forceinline__ uint32_t mass_key(float m) {  // larger mass, larger 
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelKeys = 16, kSelPiece = 1024 * kSelKeys;
+constexpr int kSelPiece = 16384, kSelFew = 1024, kSelBins = 2048, kSelCopy = kSelBins + 16;
 
-__global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
-    __shared__ int hist[2048];
+__global__ void __launch_bounds__(1024, 2) k_evict_select(const EvictArgs a) {
+    extern __shared__ uint32_t s_key[];  // kSelPiece
+    __shared__ int hist[2 * kSelCopy];   // in the last step: ballots and counts
+    __shared__ uint32_t few[kSelFew];
     __shared__ int wsum[32];
-    __shared__ int cnt_gt[kSelKeys * 32], cnt_eq[kSelKeys * 32];
-    __shared__ int s_digit, s_above, s_gt, s_eq;
+    __shared__ int s_digit, s_above, s_share, s_few, s_all;
     const int row = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) s_few = 0;
     const int len = a.lens[b];
     if (len < 0 || len > a.slots) {
         if (tid == 0) atomicOr(&g_cache_error, kErrRange);
@@ -180,45 +183,37 @@ __global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
     for (int i = tid; i < a.sinks; i += 1024) kept[i] = i;
     for (int i = tid; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
     if (need == 0) return;
-    uint32_t key[kSelKeys];  // of slots lo + piece + 1024 j + tid
-    auto load = [&](int piece) {
-        float v[kSelKeys];
-#pragma unroll
-        for (int j = 0; j < kSelKeys; ++j)
-            if (piece + 1024 * j + tid < n) v[j] = m[piece + 1024 * j + tid];
-#pragma unroll
-        for (int j = 0; j < kSelKeys; ++j) key[j] = mass_key(v[j]);
-    };
-    const bool one = n <= kSelPiece;
-    if (one) load(0);
+    const bool held = n <= kSelPiece;
+    if (held) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += 1024) s_key[i] = mass_key(m[i]);
+    }
     uint32_t prefix = 0, fixed = 0;  // the threshold key's known bits, and which they are
     int left = need;                 // kept among the keys that share them
+    bool in_few = false;             // those keys are in `few`
+    int share = n;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        hist[tid] = 0;
-        hist[tid + 1024] = 0;
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : kSelBins;
+        for (int i = tid; i < 2 * kSelCopy; i += 1024) hist[i] = 0;
         __syncthreads();
-        for (int piece = 0; piece < n; piece += kSelPiece) {
-            if (!one) load(piece);
-#pragma unroll
-            for (int j = 0; j < kSelKeys; ++j) {
-                if (piece + 1024 * j + warp * 32 >= n) break;  // (the whole warp)
-                const bool in = piece + 1024 * j + tid < n && (key[j] & fixed) == prefix;
-                const unsigned int who = __ballot_sync(0xffffffffu, in);
-                if (!in) continue;
-                const int bin = (key[j] >> shift) & (bins - 1), first = __shfl_sync(who, bin, __ffs(who) - 1);
-                if (__all_sync(who, bin == first)) {  // alike, as digits of masses often are: one addition
-                    if (lane == __ffs(who) - 1) atomicAdd(&hist[bin], __popc(who));
-                } else {
-                    atomicAdd(&hist[bin], 1);
-                }
-            }
+        int *mine = hist + (lane & 1) * kSelCopy;
+        auto add = [&](uint32_t k) {
+            if ((k & fixed) == prefix) atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
+        };
+        if (in_few) {
+            if (tid < share) add(few[tid]);
+        } else if (held) {
+#pragma unroll 4
+            for (int i = tid; i < n; i += 1024) add(s_key[i]);
+        } else {
+#pragma unroll 8
+            for (int i = tid; i < n; i += 1024) add(mass_key(m[i]));
         }
         __syncthreads();
         // thread t holds two bins, counted from the top; a scan over them finds the digit where `left` falls
         const int hi_bin = bins - 1 - 2 * tid, lo_bin = hi_bin - 1;
-        const int c0 = hi_bin > 0 ? hist[hi_bin] : 0, c1 = hi_bin > 0 ? hist[lo_bin] : 0;
+        const int c0 = hi_bin > 0 ? hist[hi_bin] + hist[kSelCopy + hi_bin] : 0, c1 = hi_bin > 0 ? hist[lo_bin] + hist[kSelCopy + lo_bin] : 0;
         int sum = c0 + c1;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -228,60 +223,68 @@ __global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs a) {
         if (lane == 31) wsum[warp] = sum;
         __syncthreads();
         const int before = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0) + sum - c0 - c1;
-        if (before < left && left <= before + c0) { s_digit = hi_bin; s_above = before; }
-        if (before + c0 < left && left <= before + c0 + c1) { s_digit = lo_bin; s_above = before + c0; }
+        if (before < left && left <= before + c0) { s_digit = hi_bin; s_above = before; s_share = c0; }
+        if (before + c0 < left && left <= before + c0 + c1) { s_digit = lo_bin; s_above = before + c0; s_share = c1; }
         __syncthreads();
         prefix |= (uint32_t)s_digit << shift;
         fixed |= (uint32_t)(bins - 1) << shift;
         left -= s_above;
+        if (!in_few) {
+            share = s_share;
+            if (pass < 2 && share <= kSelFew) {  // (in any order: only their values count from here on)
+#pragma unroll 4
+                for (int i = tid; i < n; i += 1024) {
+                    const uint32_t k = held ? s_key[i] : mass_key(m[i]);
+                    if ((k & fixed) == prefix) few[atomicAdd(&s_few, 1)] = k;
+                }
+                in_few = true;
+            }
+        }
     }
     // keys above `prefix` are kept, and the first `left` of those equal to it
-    int gt0 = 0, eq0 = 0;  // in the pieces before
+    uint32_t *above = reinterpret_cast<uint32_t *>(hist), *equal = above + 512;  // ballots of 32 slots each
+    int *count = hist + 1024;                                                    // their bits, above + 65536 equal; then the sums before them
+    int gt0 = 0, eq0 = 0;                                                        // in the pieces before
     for (int piece = 0; piece < n; piece += kSelPiece) {
-        if (!one) load(piece);
+        const int groups = min(512, (n - piece + 31) / 32);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kSelKeys; ++j) {
-            const bool in = piece + 1024 * j + tid < n;
-            const unsigned int g = __ballot_sync(0xffffffffu, in && key[j] > prefix), e = __ballot_sync(0xffffffffu, in && key[j] == prefix);
+#pragma unroll 4
+        for (int w = warp; w < groups; w += 32) {
+            const int i = piece + 32 * w + lane;
+            const uint32_t k = i < n ? (held ? s_key[i] : mass_key(m[i])) : 0u;
+            const unsigned int g = __ballot_sync(0xffffffffu, i < n && k > prefix), e = __ballot_sync(0xffffffffu, i < n && k == prefix);
             if (lane == 0) {
-                cnt_gt[32 * j + warp] = __popc(g);
-                cnt_eq[32 * j + warp] = __popc(e);
+                above[w] = g;
+                equal[w] = e;
+                count[w] = __popc(g) | __popc(e) << 16;  // (at most 16384 each)
             }
         }
         __syncthreads();
-        if (tid < 64) {  // two warps: exclusive scans over the 512 counts of each kind
-            int *c = tid < 32 ? cnt_gt : cnt_eq, v[kSelKeys], sum = 0;
-#pragma unroll
-            for (int i = 0; i < kSelKeys; ++i) {
-                v[i] = c[lane * kSelKeys + i];
-                sum += v[i];
-            }
-            int at = sum;
+        int own = 0, upto = 0;
+        if (tid < 512) {
+            own = upto = tid < groups ? count[tid] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, at, o);
-                if (lane >= o) at += u;
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
             }
-            if (lane == 31) *(tid < 32 ? &s_gt : &s_eq) = at;
-            at -= sum;
-#pragma unroll
-            for (int i = 0; i < kSelKeys; ++i) {
-                c[lane * kSelKeys + i] = at;
-                at += v[i];
-            }
+            if (lane == 31) wsum[warp] = upto;
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kSelKeys; ++j) {
-            const int i = piece + 1024 * j + tid;
-            const bool g = i < n && key[j] > prefix, e = i < n && key[j] == prefix;
-            const unsigned int gm = __ballot_sync(0xffffffffu, g), em = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1u;
-            const int eqs = eq0 + cnt_eq[32 * j + warp] + __popc(em & below);  // equal keys before this slot
-            if (g || (e && eqs < left)) kept[a.sinks + gt0 + cnt_gt[32 * j + warp] + __popc(gm & below) + min(eqs, left)] = lo + i;
+        if (tid < 512) {
+            upto += __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0);
+            count[tid] = upto - own;
+            if (tid == 511) s_all = upto;
         }
-        gt0 += s_gt;
-        eq0 += s_eq;
+        __syncthreads();
+#pragma unroll 4
+        for (int w = warp; w < groups; w += 32) {
+            const uint32_t g = above[w], e = equal[w], below = (1u << lane) - 1u;
+            const int c = count[w], eqs = eq0 + (c >> 16) + __popc(e & below);  // equal keys before this slot
+            if ((g >> lane & 1) || ((e >> lane & 1) && eqs < left)) kept[a.sinks + gt0 + (c & 0xFFFF) + __popc(g & below) + min(eqs, left)] = lo + piece + 32 * w + lane;
+        }
+        gt0 += s_all & 0xFFFF;
+        eq0 += s_all >> 16;
     }
 }
 
@@ -629,7 +632,11 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     const int64_t rows = s->layers * s->batch * s->heads;
     if (rows > 65535) return P8_ERR_UNSUPPORTED;
     cudaStream_t st = (cudaStream_t)stream;
-    k_evict_select<<<(unsigned int)rows, 1024, 0, st>>>(k);
+    // Keys go to shared memory where a middle can be that short; the limit is raised on every call, it is a call's device's.
+    const int64_t most = s->slots - a->sinks - a->recent;
+    const int smem = (int)std::min<int64_t>(std::max<int64_t>(most, 0), kSelPiece) * 4;
+    if (smem > 36 * 1024 && cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelPiece * 4) != cudaSuccess) return P8_ERR_CUDA;
+    k_evict_select<<<(unsigned int)rows, 1024, smem, st>>>(k);
     if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
     const int chunk = 4 * (256 / (k.row_bytes / 16));
     const dim3 grid = same ? dim3((unsigned int)(k.row_bytes / 64), (unsigned int)rows, 3) : dim3((unsigned int)((a->budget + chunk - 1) / chunk), (unsigned int)rows);
