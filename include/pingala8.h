@@ -304,7 +304,7 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
  * Sequence b is as long as the device array lens[b] says, and every call reads the lengths on the device, so that a
  * captured graph stays valid while sequences grow. A call adds n_b tokens to sequence b: n_b = counts[b] where `counts`
  * is given (0 <= counts[b] <= tokens), else `tokens`; token t of the call has slot lens[b] + t. Rows of tokens t >= n_b
- * are neither read nor written. A sequence with lens[b] < 0, n_b out of its range or lens[b] + n_b > slots is left
+ * have no effect and are not written. A sequence with lens[b] < 0, n_b out of its range or lens[b] + n_b > slots is left
  * alone, outputs included (p8_tree_accept: reported as nothing accepted), and p8_device_error reports bit 6 (64).
  *
  * Layouts: element (layer, b, h, slot, d) of the keys is k[layer * k_stride[0] + b * k_stride[1] + h * k_stride[2] +

@@ -5,7 +5,7 @@ leading layer dimension for the two operators that serve all layers at once (kv_
 rows start on 16 bytes and have unit stride inside; the keys and the values may lie apart. Sequence b is as long as
 the int32 device tensor lens[b] says and the device alone reads it, so calls can be captured in a CUDA graph and replayed
 while sequences grow. A call's tokens have the slots behind the sequence's end; `counts` (int32 [batch]) says how many
-of them are real where a batch is padded, and what belongs to the others is neither read nor written.
+of them are real where a batch is padded, and what belongs to the others has no effect and is not written.
 
 One step of speculative decoding with a bounded cache:
 

@@ -74,29 +74,29 @@ struct AppendArgs {
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a) {
     constexpr int L = D / 8, RPB = 256 / L;
-    const int rows = a.heads + 2 * a.kvh;
-    const long long id = (long long)blockIdx.x * RPB + threadIdx.x / L;
+    const unsigned int rows = a.heads + 2 * a.kvh, id = blockIdx.x * RPB + threadIdx.x / L;
     const int l = threadIdx.x % L;
-    const long long tok = id / rows;
-    if (tok >= (long long)a.batch * a.tokens) return;  // a whole group of lanes leaves
-    const int r = (int)(id - tok * rows), b = (int)(tok / a.tokens), t = (int)(tok - (long long)b * a.tokens);
+    const unsigned int tok = id / rows;
+    if (tok >= (unsigned int)a.batch * a.tokens) return;  // a whole group of lanes leaves
+    const int r = (int)(id - tok * rows), b = (int)(tok / (unsigned int)a.tokens), t = (int)(tok - (unsigned int)b * a.tokens);
+    const int which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2;
+    const int h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
+    // the row, the length and the position are asked for together: one round of latency before the table's
+    const float *x = a.x[which] + b * a.xs[which][0] + t * a.xs[which][1] + h * a.xs[which][2] + 4 * l;
+    float u[4], w[4];
+    *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(x);
+    *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(x + D / 2);
+    const int p = a.pos[tok];
     int len, n;
     if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n)) {
         if (t == 0 && r == 0 && l == 0) atomicOr(&g_cache_error, kErrRange);
         return;
     }
     if (t >= n) return;
-    const int p = a.pos[tok];
     if (p < 0 || p >= a.positions) {
         if (r == 0 && l == 0) atomicOr(&g_cache_error, kErrRange);
         return;
     }
-    const int which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2;
-    const int h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
-    const float *x = a.x[which] + b * a.xs[which][0] + t * a.xs[which][1] + h * a.xs[which][2] + 4 * l;
-    float u[4], w[4];
-    *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(x);
-    *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(x + D / 2);
     if (which < 2) {
         float c[4], s[4];
         *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(a.cos + (long long)p * (D / 2) + 4 * l);
@@ -399,15 +399,19 @@ __global__ void __launch_bounds__(256) k_tree_accept(const AcceptArgs a) {
         const long long at = (long long)b * a.T;
         int par[2];
         bool fits[2];
+        long long tok[2], tgt[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // the whole tree at once; a parent's target comes from its lane
+            const int c = tid + 32 * k;
+            par[k] = c < a.T ? a.parents[at + c] : -1;
+            tok[k] = c < a.T ? a.tokens[at + c] : 0;
+            tgt[k] = c < a.T ? a.target[at + c] : 0;
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int c = tid + 32 * k;
-            par[k] = -1;
-            fits[k] = false;
-            if (ok && c > 0 && c < n) {
-                par[k] = a.parents[at + c];
-                fits[k] = par[k] >= 0 && par[k] < c && a.tokens[at + c] == a.target[at + par[k]];
-            }
+            const long long t0 = __shfl_sync(0xffffffffu, tgt[0], par[k] & 31), t1 = __shfl_sync(0xffffffffu, tgt[1], par[k] & 31);
+            fits[k] = ok && c < n && par[k] >= 0 && par[k] < c && tok[k] == (par[k] < 32 ? t0 : t1);
         }
         int cur = 0, cnt = ok && n > 0 ? 1 : 0;
         if (tid == 0) path[0] = 0;
@@ -533,7 +537,7 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
     if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
     if (!a->q || !a->k || !a->v || !a->q_out || !a->lens || !a->pos || !a->cos || !a->sin || a->tokens < 0 || a->positions < 1) return P8_ERR_ARG;
     if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->q_out) || !al16(a->cos) || !al16(a->sin) || !(a->eps >= 0.0)) return P8_ERR_ARG;
-    if (a->tokens > c->slots || c->batch * a->tokens * (a->heads + 2 * c->heads) > (int64_t(1) << 34)) return P8_ERR_ARG;
+    if (a->tokens > c->slots || c->batch * a->tokens * (a->heads + 2 * c->heads) > (int64_t(1) << 31) - 64) return P8_ERR_ARG;
     const int es = elem_size(c->type);
     const int64_t dq[3] = {c->batch, a->tokens, a->heads}, dk[3] = {c->batch, a->tokens, c->heads};
     if (!strides_ok(a->q_stride, dq, 3, 4) || !strides_ok(a->k_stride, dk, 3, 4) || !strides_ok(a->v_stride, dk, 3, 4) ||

@@ -23,7 +23,7 @@ struct AttnArgs {
 // equal contiguous share of it, so that the SMs finish together whatever the lengths are, and one long sequence still
 // fills them. A unit that lies in one share is finished
 // there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
-constexpr int kStart = 1;    // of a 16-bit attention segment
+__host__ __device__ constexpr int start_of(int rblock) { return rblock > 128 ? 4 : 1; }  // of a 16-bit attention segment, as measured
 constexpr int kTile = 128;  // of a 16-bit cache; 64 of a 32-bit one (as many bytes)
 struct Cut {                // how a kernel cuts its work
     int rblock, tile;       // query rows of a unit, slots of a tile
@@ -322,7 +322,7 @@ struct TcShape {
     static constexpr int kQ = 2 * 128 * D * 2;  // of 256 rows, or of 128 for this segment and the next
     static constexpr int kStages = D == 64 ? 10 : 5;
     static constexpr int kRows = TWO ? 256 : 128;
-    static constexpr int kLeast = TWO ? 1 : 2 + kStart;
+    static constexpr int kLeast = (TWO ? 1 : 2) + start_of(kRows);  // one tile at least, or one for each stream at once
     static constexpr int kThreads = 384;
     static constexpr int kSmem = kQ + kStages * kStage;
 };
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
     using S_ = TcShape<D, TWO>;
     using H = Half16<T>;
     constexpr int NST = S_::kStages, NQ = S_::kQBufs, kBoxes = D / 64, kStep = 64, PER = TWO ? 2 : 1;  // PER: a stream's steps of a tile
-    constexpr Cut cut{S_::kRows, kTile, S_::kLeast, kStart};
+    constexpr Cut cut{S_::kRows, kTile, S_::kLeast, start_of(S_::kRows)};
     extern __shared__ __align__(1024) char dyn[];  // the swizzle goes by address bits
     char *sq = dyn, *ring = sq + S_::kQ;
     __shared__ uint64_t b_full[NST], b_empty[NST], b_q[2], b_qfree[2], b_s[2][2], b_p[2][2], b_pv[2][2], b_seg, b_read, b_tail;  // [stream][score buffer]
@@ -627,7 +627,10 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                         }
                     } else if (live) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4 *>(po + x0 + j + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 8)  // a whole sector a thread: half as many requests to L2 as with 16 bytes
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(po + x0 + j + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]),
+                                         "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
+                                         : "memory");
                     }
                 }
                 if (live && bad) {
@@ -1421,7 +1424,6 @@ void allow32() {
     cudaFuncSetAttribute(k_tree_attn_f32<D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 1>::kSmem);
     cudaFuncSetAttribute(k_tree_attn_f32<D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 2>::kSmem);
     cudaFuncSetAttribute(k_tree_attn_f32<D, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 4>::kSmem);
-    cudaFuncSetAttribute(k_tree_attn_f32<D, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Shape<D, 8>::kSmem);
     cudaFuncSetAttribute(k_attn_mass_f32<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Mass<D>::kSmem);
 }
 // SM count of the current device; the first call on a device raises the kernels' shared-memory limits there
@@ -1443,11 +1445,12 @@ int sm_count() {
     return v;
 }
 
-// Query rows of a unit: as few as hold them all, so that K and V are read once; the largest block has to be enough for
-// the rest (the last SM-sized part of a longer row list reads its tiles from L2).
+// Query rows of a unit. 16-bit: one block for up to 256, so that K and V are read once. 32-bit: the products bound it, so
+// blocks whose 16-row tiles fill the four schedulers (three tiles: 32 + 16 rows take 576 products a scheduler and tile,
+// a block of 64 takes 768); more blocks read K and V from L2 again, at less than half of its rate.
 Cut attn_cut(const p8_kv *c, int64_t rows) {
-    if (c->type != P8_KV_F32) return {rows > 128 ? 256 : 128, kTile, rows > 128 ? 1 : 2 + kStart, kStart};
-    return {rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, kTile32, 1, 0};
+    if (c->type != P8_KV_F32) return rows > 128 ? Cut{256, kTile, TcShape<64, true>::kLeast, start_of(256)} : Cut{128, kTile, TcShape<64, false>::kLeast, start_of(128)};
+    return {rows <= 16 ? 16 : rows <= 48 ? 32 : 64, kTile32, 1, 0};
 }
 int64_t attn_tiles(const p8_kv *c, int64_t rows, Cut cut) {
     return c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile + cut.start);
@@ -1485,8 +1488,7 @@ p8_status run_f32(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) 
     switch (attn_cut(c, (int64_t)a.tokens * a.group).rblock) {
         case 16: return run_attn<float, D>(k_tree_attn_f32<D, 1>, 288, F32Shape<D, 1>::kSmem, 0.f, c, a, ws, st);
         case 32: return run_attn<float, D>(k_tree_attn_f32<D, 2>, 288, F32Shape<D, 2>::kSmem, 0.f, c, a, ws, st);
-        case 64: return run_attn<float, D>(k_tree_attn_f32<D, 4>, 288, F32Shape<D, 4>::kSmem, 0.f, c, a, ws, st);
-        default: return run_attn<float, D>(k_tree_attn_f32<D, 8>, 288, F32Shape<D, 8>::kSmem, 0.f, c, a, ws, st);
+        default: return run_attn<float, D>(k_tree_attn_f32<D, 4>, 288, F32Shape<D, 4>::kSmem, 0.f, c, a, ws, st);
     }
 }
 // At most `most` rows a launch (what its shared memory holds); the later launches add to the first one's sums.
