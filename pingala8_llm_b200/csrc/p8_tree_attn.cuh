@@ -919,8 +919,8 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 // x = hi + lo, both TF32 (8 + 11 bits): x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y|, three mma.sync products with
 // fp32 sums. (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
 // more shared-memory traffic than the products take. From registers the split costs three integer or fp32 operations.)
-// The products run through independent sums first (N of them, then the next piece): each waits for the one before on
-// the same sum.
+// A product waits for the one before it on the same sum (four of them take that long to issue), so the order is by piece,
+// through as many sums as there are, and scores have two sums each.
 struct Split {
     uint32_t hi, lo;  // the tensor cores leave out the last 13 bits
 };
@@ -944,21 +944,38 @@ struct Frag {  // a 16 x 8 left operand
         x[3] = split(x3);
     }
 };
-// c[i] += a (b0[i], b1[i]) for N sums
-template <int N>
-__device__ __forceinline__ void mma_split(float (&c)[N][4], const Frag &a, const float (&b0)[N], const float (&b1)[N]) {
-    Split u[N], v[N];
+__device__ __forceinline__ void mma_part(float (&c)[4], const Frag &a, int part, const Split &u, const Split &v) {  // the small pieces first
+    if (part == 0) mma8(c, a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u.lo, v.lo);
+    else if (part == 1) mma8(c, a.x[0].lo, a.x[1].lo, a.x[2].lo, a.x[3].lo, u.hi, v.hi);
+    else mma8(c, a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u.hi, v.hi);
+}
+// c[i] += a (b0[i], b1[i]) for four sums
+__device__ __forceinline__ void mma_four(float (&c)[4][4], const Frag &a, const float4 &b0, const float4 &b1) {
+    const Split u[4] = {split(b0.x), split(b0.y), split(b0.z), split(b0.w)}, v[4] = {split(b1.x), split(b1.y), split(b1.z), split(b1.w)};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        u[i] = split(b0[i]);
-        v[i] = split(b1[i]);
+    for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma_part(c[i], a, part, u[i], v[i]);
+}
+// 16 columns of scores: c[0] and c[1] each take half of the columns, for N groups of slots (k[j]: a lane's four columns)
+template <int N>
+__device__ __forceinline__ void mma_scores(float (&c)[2][N][4], const float4 &q0, const float4 &q1, const float4 (&k)[N]) {
+    const Frag a(q0.x, q1.x, q0.y, q1.y), b(q0.z, q1.z, q0.w, q1.w);
+    Split s[N][4];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        s[j][0] = split(k[j].x);
+        s[j][1] = split(k[j].y);
+        s[j][2] = split(k[j].z);
+        s[j][3] = split(k[j].w);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u[i].lo, v[i].lo);
+    for (int part = 0; part < 3; ++part)
 #pragma unroll
-    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].lo, a.x[1].lo, a.x[2].lo, a.x[3].lo, u[i].hi, v[i].hi);
-#pragma unroll
-    for (int i = 0; i < N; ++i) mma8(c[i], a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u[i].hi, v[i].hi);
+        for (int j = 0; j < N; ++j) {
+            mma_part(c[0][j], a, part, s[j][0], s[j][1]);
+            mma_part(c[1][j], b, part, s[j][2], s[j][3]);
+        }
 }
 constexpr int kTile32 = 64;
 // A stage holds 64 slots in parts of 32 columns as the tensor map's loads leave them: 128-byte rows, the 16-byte pieces
@@ -1071,26 +1088,24 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
         for (int tile = w.ta; tile < w.tb; ++tile) {
             const int key0 = tile * kTile32 + kg * NK * 8;  // the warp's first slot
             const bool tail = key0 + NK * 8 > w.len;
-            float s[NK][4] = {};
+            float s[NK][4] = {}, s2[2][NK][4] = {};
             const int sk = n % NST;
             wait(b_full + sk, n / NST & 1);
             ++n;
             if (warp_live) {
                 const char *st = ring + sk * S_::kStage;
                 const int slot = kg * NK * 8 + (g >> 1) + ((g & 1) << 2);
-#pragma unroll 1
+#pragma unroll 2
                 for (int d = 0; d < D / 16; ++d) {
-                    const float4 q0 = *query32<D>(sq, 16 * rt + g, 4 * d + t), q1 = *query32<D>(sq, 16 * rt + g + 8, 4 * d + t);
-                    const Frag fa(q0.x, q1.x, q0.y, q1.y), fb(q0.z, q1.z, q0.w, q1.w);
-                    float b[4][NK];
+                    float4 k[NK];
 #pragma unroll
-                    for (int j = 0; j < NK; ++j) {
-                        const float4 k = stage32(st, slot + 8 * j, 4 * d + t);
-                        b[0][j] = k.x; b[1][j] = k.y; b[2][j] = k.z; b[3][j] = k.w;
-                    }
-                    mma_split(s, fa, b[0], b[1]);
-                    mma_split(s, fb, b[2], b[3]);
+                    for (int j = 0; j < NK; ++j) k[j] = stage32(st, slot + 8 * j, 4 * d + t);
+                    mma_scores(s2, *query32<D>(sq, 16 * rt + g, 4 * d + t), *query32<D>(sq, 16 * rt + g + 8, 4 * d + t), k);
                 }
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] = s2[0][j][e] + s2[1][j][e];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(b_empty + sk);
@@ -1170,8 +1185,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                     for (int x = 0; x < D / 32; ++x) {
                         const int col4 = 8 * x + (g >> 1) + ((g & 1) << 2);
                         const float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
-                        const float b0[4] = {u.x, u.y, u.z, u.w}, b1[4] = {v.x, v.y, v.z, v.w};
-                        mma_split(o[x], p, b0, b1);
+                        mma_four(o[x], p, u, v);
                     }
                 }
             }
@@ -1354,17 +1368,16 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
                 from[e] = late <= 0 ? 0 : late < w.n ? late * a.gc : rows;
             }
             for (int r0 = 0; r0 < padded; r0 += 16) {
-                float s0[1][4] = {}, s1[1][4] = {};  // two sums, so that their products need not wait for one another
+                float s2[2][1][4] = {};
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    const float4 q0 = *query32<D>(sq, r0 + g, 4 * d + t), q1 = *query32<D>(sq, r0 + g + 8, 4 * d + t);
-                    mma_split<1>(s0, Frag(q0.x, q1.x, q0.y, q1.y), {k[d].x}, {k[d].y});
-                    mma_split<1>(s1, Frag(q0.z, q1.z, q0.w, q1.w), {k[d].z}, {k[d].w});
+                    const float4 kd[1] = {k[d]};
+                    mma_scores(s2, *query32<D>(sq, r0 + g, 4 * d + t), *query32<D>(sq, r0 + g + 8, 4 * d + t), kd);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = r0 + g + 8 * (e >> 1);
-                    const float p = ex2(s0[0][e] + s1[0][e] + s_nl[row]);
+                    const float p = ex2(s2[0][0][e] + s2[1][0][e] + s_nl[row]);
                     if (row >= from[e & 1] && row < rows) sum[e & 1] += p;
                 }
             }
