@@ -1,7 +1,8 @@
 """pingala8_llm_b200 -- B200-native (sm_100a) Pingala-8 quantized-weight matmul path.
 
 Drop-in for the reference's ggml Pingala-8 hooks (Genrius-AI/pingala8-llm): batch-1 table GEMV, batched product,
-get_rows / f32 dequant, and a tensor-parallel split. The compute lives in libpingala8_b200.so (C ABI:
+get_rows / f32 dequant, a tensor-parallel split, and (pingala8_llm_b200.cache) the key/value cache operators of a decode
+step. The compute lives in libpingala8_b200.so (C ABI:
 include/pingala8.h); this package is the thin host mirror over it.
 """
 from ._lib import LIB_PATH, P8Error, P8_STATUS, header_functions, lib  # noqa: F401
@@ -16,4 +17,8 @@ def __getattr__(name):
         import importlib
 
         return getattr(importlib.import_module(".ops", __name__), name)
+    if name in ("cache", "decode"):
+        import importlib
+
+        return importlib.import_module("." + name, __name__)
     raise AttributeError(name)

@@ -6,7 +6,8 @@ norm weight before q/k/v and gate/up, SwiGLU before down). The rest is ordinary 
 in Q8_0 (blocks of 32 int8 with one fp16 scale, as the reference's model files keep them; the head multiplies the
 Q8_0 values as fp16), RoPE, the optional per-head q/k RMSNorm of Qwen3, attention with torch SDPA over a static KV
 cache, residual adds, greedy sampling. A decode step reads its position from the device and writes into fixed
-buffers, so it is captured once as a CUDA graph and replayed per token.
+buffers, so it is captured once as a CUDA graph and replayed per token. TreeDecoder runs the same layers over drafted
+trees of tokens and a cache that can be bounded, with the package's own cache operators in place of the torch ones.
 
 The reference runs this model in llama.cpp (MUL_MAT nodes dispatched to ggml_cuda_f44_mul_mat_vec / _mul_mat_q8,
 CU:1330-1342); its runtime is not available here, so this module restates the same architecture as a plain
@@ -18,7 +19,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import synth
+from . import cache, synth
 from .ops import P8Tensor, group_workspace_size, mul_mat_group, mul_mat_vec_group
 
 
@@ -240,6 +241,127 @@ class Model:
             hid.append(self.xl.clone())
             self.pos += 1
         return torch.cat(out), logits, hid
+
+
+class TreeDecoder:
+    """Greedy decoding of a Model with drafted trees of tokens and, if wanted, a bounded cache.
+
+    Each pass takes 1 to 64 tokens at once: the projections through the batched product (which reads the packed weights
+    once for all of them), norms, rotation and cache writes through cache.kv_append, attention through
+    cache.tree_attention, so a pass over a tree costs little more than one token's. step() then walks the tree along the
+    model's own choices (cache.tree_accept) and keeps what it confirms: the tokens are those that greedy decoding gives one
+    by one. dtype is the cache's type (float32, float16 or bfloat16).
+
+    With a budget, the attention weight that every slot draws is added up (cache.attention_mass), and a sequence that has
+    grown `slack` slots over the budget is cut back to it (cache.kv_evict): the first `sinks` slots, the last `recent` ones
+    and the heaviest of the others stay, per layer and head. Tokens keep the positions they had."""
+
+    def __init__(self, model, max_len, dtype=torch.float16, budget=None, sinks=4, recent=64, slack=128):
+        c, dev = model.c, model.device
+        self.m, self.budget, self.sinks, self.recent, self.slack = model, budget, sinks, recent, slack
+        slots = max_len if budget is None else min(max_len, budget + slack + cache.TREE_MAX)
+        self.k, self.v = (torch.zeros(model.nl, 1, c.kv_heads, slots, c.head_dim, dtype=dtype, device=dev) for _ in range(2))
+        self.mass = None if budget is None else torch.zeros(model.nl, 1, c.kv_heads, slots, device=dev)
+        self.cos, self.sin = rope_tables(c, max_len, dev)
+        self.max_len = max_len
+        self.reset()
+
+    def reset(self):
+        self.lens = torch.zeros(1, dtype=torch.int32, device=self.m.device)  # slots in use
+        self.used = self.position = 0  # the same on the host, and how many tokens the sequence has
+
+    def forward(self, tokens, mask, depth):
+        """tokens int64 [T], their ancestor bits int64 [T] and depths int32 [T] (cache.tree_plan) -> logits [T, vocab]; the
+        keys and values of all T are in the slots behind the sequence, which is as long as before"""
+        m, c, T = self.m, self.m.c, tokens.numel()
+        if self.position + T > self.max_len:
+            raise ValueError(f"{self.position} + {T} tokens are more than max_len {self.max_len}")
+        pos = (depth + self.position)[None]
+        x = m.embed.dequant(tokens)
+        self.seen = []
+        for L, layer in enumerate(m.layers):
+            t = layer["t"]
+            q, k, v = mul_mat_group([t["q"], t["k"], t["v"]], x, norm_weight=layer["attn_norm"], eps=c.eps)
+            qn, kn = layer["qk_norm"] if c.qk_norm else (None, None)
+            q = cache.kv_append(q.view(1, T, c.heads, c.head_dim), k.view(1, T, c.kv_heads, c.head_dim), v.view(1, T, c.kv_heads, c.head_dim),
+                                self.k[L], self.v[L], self.lens, pos, self.cos, self.sin, q_norm=qn, k_norm=kn, eps=c.eps)
+            a, lse = cache.tree_attention(q, self.k[L], self.v[L], self.lens, mask=mask)
+            self.seen.append((q, lse))
+            h = x + t["o"].mul_mat(a.view(T, -1).float())
+            g, u = mul_mat_group([t["gate"], t["up"]], h, norm_weight=layer["ffn_norm"], eps=c.eps)
+            x = h + t["down"].mul_mat(g, up=u)
+        self.hidden = rms(x, m.final_norm, c.eps)
+        return (self.hidden.half() @ m.head_w.T).float()
+
+    def _grow(self, new_lens, n, rows=None, counts=None):
+        """n tokens of the last forward() belong to the sequence now"""
+        if self.budget is not None:
+            for L, (q, lse) in enumerate(self.seen):
+                cache.attention_mass(q, lse, self.k[L], self.lens, self.mass[L], rows=rows, counts=counts)
+        self.lens = new_lens
+        self.used += n
+        self.position += n
+        if self.budget is not None and self.used > self.budget + self.slack:
+            self.lens, _ = cache.kv_evict(self.k, self.v, self.mass, self.lens, self.budget, self.sinks, self.recent)
+            self.used = self.budget
+
+    def prefill(self, tokens):
+        """a prompt, int64 [n], in passes of up to 64 tokens; returns the last token's logits"""
+        for i in range(0, tokens.numel(), cache.TREE_MAX):
+            part = tokens[i:i + cache.TREE_MAX]
+            n = part.numel()
+            mask, depth = cache.tree_plan(torch.arange(-1, n - 1, device=tokens.device))
+            logits = self.forward(part, mask, depth)
+            self._grow(self.lens + n, n)
+        return logits[-1]
+
+    def step(self, tokens, parents):
+        """One pass over a drafted tree: tokens int64 [T] (token 0 the last known one, not yet in the cache), parents int32
+        [T]. Returns the confirmed tokens and the model's next one, int64 [1..T]; the last of them is the next tree's root."""
+        mask, depth = cache.tree_plan(parents)
+        self.logits = self.forward(tokens, mask, depth)
+        target = torch.argmax(self.logits, dim=-1)
+        acc = cache.tree_accept(tokens[None].contiguous(), parents[None].contiguous(), target[None], self.k, self.v, self.lens)
+        n = int(acc.accepted[0])
+        path = acc.path[0, :n].long()
+        self.path = path
+        self._grow(acc.new_lens, n, rows=acc.path, counts=acc.accepted)
+        return torch.cat([tokens[path[1:]], acc.next_token])
+
+    def generate(self, prompt, n_new, draft=None):
+        """greedy: prompt int64 [n], then n_new tokens; draft(history) -> (tokens, parents) of the tree to try, whose token 0 is
+        the last of `history` (a list of ints); None: lookup_draft. Returns (tokens [n_new], passes)."""
+        draft = draft or lookup_draft
+        self.reset()
+        history = prompt.tolist()
+        history.append(int(torch.argmax(self.prefill(prompt))))
+        out, passes = [history[-1]], 0
+        while len(out) < n_new:
+            tokens, parents = draft(history)
+            room = min(len(tokens), n_new - len(out), self.max_len - self.position)
+            tokens, parents = tokens[:room], parents[:room]  # a child comes after its parent: the rest is still a tree
+            got = self.step(torch.tensor(tokens, device=prompt.device), torch.tensor(parents, dtype=torch.int32, device=prompt.device)).tolist()
+            out += got
+            history += got
+            passes += 1
+        return torch.tensor(out[:n_new], device=prompt.device), passes
+
+
+def lookup_draft(history, width=4, depth=7):
+    """A tree out of the text itself: what followed the last token at its latest `width` earlier places, `depth` tokens of
+    each, with common beginnings shared. Returns (tokens, parents); token 0 is the last of `history`."""
+    last = history[-1]
+    tokens, parents, child = [last], [-1], {}
+    places = [i for i in range(len(history) - 2, -1, -1) if history[i] == last][:width]
+    for i in places:
+        at = 0
+        for tok in history[i + 1:i + 1 + depth]:
+            if (at, tok) not in child:
+                child[(at, tok)] = len(tokens)
+                tokens.append(tok)
+                parents.append(at)
+            at = child[(at, tok)]
+    return tokens, parents
 
 
 def reference_forward(c, weights, norms, embed, head, final_norm, seq):
