@@ -309,7 +309,8 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
  *
  * Layouts: element (layer, b, h, slot, d) of the keys is k[layer * k_stride[0] + b * k_stride[1] + h * k_stride[2] +
  * slot * k_stride[3] + d], of the values alike. width is 64 or 128; every base address and every stride that is used
- * (its dimension is above 1) is a multiple of 16 bytes. Query heads: `heads` is a multiple of the cache's heads, query
+ * (its dimension is above 1) is positive and a multiple of 16 bytes; keys and values share no memory. The current device
+ * is the buffers'. Calls that share a workspace or an output must not overlap on the GPU. Query heads: `heads` is a multiple of the cache's heads, query
  * head i reads cache head i / (heads / kv heads). Strides are in elements. */
 typedef enum p8_kv_type { P8_KV_F32 = 0, P8_KV_F16 = 1, P8_KV_BF16 = 2 } p8_kv_type;
 #define P8_TREE_MAX 64   /* tokens of one sequence in a tree attention, mass or accept call */
@@ -326,7 +327,8 @@ typedef struct p8_kv {
  * q_norm / k_norm [width] is given), then the halves rotate by the token's position p = pos[b * tokens + t]:
  *     y[i] = x'[i] cos[p][i] - x'[i + width/2] sin[p][i],  y[i + width/2] = x'[i + width/2] cos[p][i] + x'[i] sin[p][i]
  * with cos / sin f32 [positions][width / 2]. Rotated keys and plain values are rounded once to the cache's type and
- * written to the tokens' slots, rotated queries to q_out (the cache's type). Any number of tokens. A token whose
+ * written to the tokens' slots, rotated queries to q_out (the cache's type; it may be q itself where that is f32, but
+ * must not overlap it otherwise). Any number of tokens. A token whose
  * position is outside [0, positions) is left out and sets bit 6. */
 typedef struct p8_kv_append_args {
     const float *q, *k, *v;
@@ -347,8 +349,8 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
  * mask[b * mask_stride + t] is set (mask NULL: j <= t, a chain). out = softmax(scale q k^T) v over what it sees, in q's
  * type (the cache's); lse [batch][tokens][heads] f32 (or NULL) the natural log of the sum of exponentials. A token that
  * sees nothing gets 0 and -infinity. What a token does not see does not reach it, whatever its bits (infinities and NaN
- * included). Products and sums in fp32 (16-bit types: the weights are rounded to the type before they multiply v).
- * Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
+ * included). Products and sums in fp32 (16-bit types: the weights are rounded to the type before they multiply v; f32:
+ * products of two TF32 pieces each, 2^-21). out must not overlap q, k or v. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
 typedef struct p8_tree_attn_args {
     const void *q;
     int64_t q_stride[3];                  /* sequence, token, head */

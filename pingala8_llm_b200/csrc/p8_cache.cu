@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(1024, 2) k_evict_select(const EvictArgs a) {
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
     const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     const int len = a.lens[b];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for `kept` (every block: what follows in the stream waits for this launch alone)
     if (len < 0 || len > a.slots) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for `kept`
     const int keep = min(len, a.budget), per = a.row_bytes / 16, rows = 256 / per;
     const int *kept = a.kept + (long long)row * a.budget;
     const char *s0 = a.src[0] + layer * a.ss[0][0] + b * a.ss[0][1] + h * a.ss[0][2], *s1 = a.src[1] + layer * a.ss[1][0] + b * a.ss[1][1] + h * a.ss[1][2];
@@ -360,8 +360,8 @@ __device__ __forceinline__ void evict_slide(const char *base, long long stride, 
 __global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
     const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     const int len = a.lens[b];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // as above
     if (len <= a.budget || len > a.slots) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for `kept`
     const int *kept = a.kept + (long long)row * a.budget;
     const int z = blockIdx.z;
     if (z == 2) {
@@ -544,6 +544,9 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
         !strides_ok(a->q_out_stride, dq, 3, es))
         return P8_ERR_ARG;
     if (a->tokens == 0) return P8_OK;
+    bool same = c->type == P8_KV_F32 && (const void *)a->q == a->q_out;  // in place: every lane writes what it has read
+    for (int i = 0; i < 3; ++i) same = same && a->q_stride[i] == a->q_out_stride[i];
+    if (!same && overlap(a->q, a->q_stride, dq, 4, c->width, a->q_out, a->q_out_stride, dq, es, c->width)) return P8_ERR_ARG;
     AppendArgs k;
     const float *x[3] = {a->q, a->k, a->v};
     const int64_t *xs[3] = {a->q_stride, a->k_stride, a->v_stride};
@@ -636,10 +639,11 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     const int64_t rows = s->layers * s->batch * s->heads;
     if (rows > 65535) return P8_ERR_UNSUPPORTED;
     cudaStream_t st = (cudaStream_t)stream;
-    // Keys go to shared memory where a middle can be that short; the limit is raised on every call, it is a call's device's.
+    // Keys go to shared memory as far as a middle can be long. Beside the kernel's own 22 KB, more than 24 KB needs the limit
+    // raised; on every call, since it is the device's.
     const int64_t most = s->slots - a->sinks - a->recent;
     const int smem = (int)std::min<int64_t>(std::max<int64_t>(most, 0), kSelPiece) * 4;
-    if (smem > 36 * 1024 && cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelPiece * 4) != cudaSuccess) return P8_ERR_CUDA;
+    if (smem > 24 * 1024 && cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelPiece * 4) != cudaSuccess) return P8_ERR_CUDA;
     k_evict_select<<<(unsigned int)rows, 1024, smem, st>>>(k);
     if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
     const int chunk = 4 * (256 / (k.row_bytes / 16));

@@ -660,29 +660,33 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
 // Adds up a unit's parts, one warp per query row, in the parts' order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
+    // Everything up to the wait comes from the call's inputs, while the attention kernel runs; the parts are its outputs.
+    // Every warp waits, with or without something to add: what follows in the stream waits for this launch alone.
     const int lane = threadIdx.x % 32;
     const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-    if (id >= (long long)a.batch * a.tokens * a.heads) return;
-    const int head = (int)(id % a.heads), t = (int)(id / a.heads % a.tokens), b = (int)(id / a.heads / a.tokens);
-    int len, n;
-    if (!seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n) || t >= n) return;
-    bool bad = false;
-    int total = 0, before = 0, l_, n_;
-    for (int x = lane; x < a.batch; x += 32) {
-        const int k = seq_tiles(a, cut, x, l_, n_, &bad);
-        total += k;
-        before += x < b ? k : 0;
-    }
-    total = __reduce_add_sync(0xffffffffu, total);
-    before = __reduce_add_sync(0xffffffffu, before);
-    const int each = share_of(total, cut, ctas);
-    const int blocks = (n * a.group + cut.rblock - 1) / cut.rblock, nt = (len + n + cut.tile - 1) / cut.tile;
+    const bool is = id < (long long)a.batch * a.tokens * a.heads;
+    const int head = is ? (int)(id % a.heads) : 0, t = is ? (int)(id / a.heads % a.tokens) : 0, b = is ? (int)(id / a.heads / a.tokens) : 0;
+    int len, n, u0 = 0, each = 1, c0 = 0, c1 = 0;
+    const bool ok = seq_range(a.lens, a.counts, b, a.tokens, a.slots, len, n) && t < n && is;
     const int h = head / a.group, row = t * a.group + head % a.group;
-    const int u0 = before + (h * blocks + row / cut.rblock) * (nt + cut.start), u1 = u0 + cut.start + nt;
-    const int c0 = (u0 + cut.start) / each, c1 = (u1 - 1) / each;
-    if (c0 == c1) return;  // finished by that CTA
-    // Everything so far came from the call's inputs, while the attention kernel ran; the parts are its outputs.
+    if (ok) {
+        bool bad = false;
+        int total = 0, before = 0, l_, n_;
+        for (int x = lane; x < a.batch; x += 32) {
+            const int k = seq_tiles(a, cut, x, l_, n_, &bad);
+            total += k;
+            before += x < b ? k : 0;
+        }
+        total = __reduce_add_sync(0xffffffffu, total);
+        before = __reduce_add_sync(0xffffffffu, before);
+        each = share_of(total, cut, ctas);
+        const int blocks = (n * a.group + cut.rblock - 1) / cut.rblock, nt = (len + n + cut.tile - 1) / cut.tile;
+        u0 = before + (h * blocks + row / cut.rblock) * (nt + cut.start);
+        c0 = (u0 + cut.start) / each;
+        c1 = (u0 + cut.start + nt - 1) / each;
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (c0 == c1) return;  // finished by that CTA, or not there
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
     constexpr int W = D / 32, AHEAD = 16;
     float m = -INFINITY, l = 0.f, acc[W] = {};
@@ -1410,7 +1414,6 @@ EncodeTiled encode_tiled() {  // from the driver, so that the library does not l
 // 128 bytes of columns x a tile of slots of one head, in the 128-byte swizzle; slots behind the last read as zero
 bool cache_map(CUtensorMap *m, const p8_kv *c, const void *base, const int64_t *st) {
     const EncodeTiled f = encode_tiled();
-    if (!f) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)c->width, (cuuint64_t)c->slots, (cuuint64_t)c->heads, (cuuint64_t)c->batch};
     // the stride of a dimension of one is never used, but has to be a valid one
     const bool wide = c->type == P8_KV_F32;
@@ -1480,7 +1483,8 @@ size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {  // 
 template <typename T, int D, typename K>
 p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     CUtensorMap mk, mv;
-    if (!cache_map(&mk, c, c->k, c->k_stride) || !cache_map(&mv, c, c->v, c->v_stride)) return P8_ERR_CUDA;
+    if (!encode_tiled()) return P8_ERR_CUDA;
+    if (!cache_map(&mk, c, c->k, c->k_stride) || !cache_map(&mv, c, c->v, c->v_stride)) return P8_ERR_UNSUPPORTED;
     const Cut cut = attn_cut(c, (int64_t)a.tokens * a.group);
     const int ctas = attn_ctas(c, (int64_t)a.tokens * a.group, cut);
     float *po = static_cast<float *>(ws);
@@ -1522,7 +1526,8 @@ p8_status mass_launches(AttnArgs a, int most, F launch) {
 template <typename T, int D>
 p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
-    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
+    if (!encode_tiled()) return P8_ERR_CUDA;
+    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1, 0});
     return mass_launches(a, 512, [&](const AttnArgs &x) {
         if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 576, MassShape<D, 256>::kSmem, st>>>(x, mk);
@@ -1532,7 +1537,8 @@ p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
 template <int D>
 p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
-    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_CUDA;
+    if (!encode_tiled()) return P8_ERR_CUDA;
+    if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1, 0});
     return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, 288, F32Mass<D>::kSmem, st>>>(x, mk); });
 }
@@ -1553,7 +1559,7 @@ void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, in
 
 p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
     const int64_t rows = mass ? 1 : (int64_t)x.tokens * x.group;
-    if (attn_tiles(c, rows, attn_cut(c, rows)) > INT32_MAX / 2) return P8_ERR_UNSUPPORTED;
+    if (attn_tiles(c, rows, attn_cut(c, rows)) > INT32_MAX / 2 || c->batch * x.tokens * x.heads > INT32_MAX) return P8_ERR_UNSUPPORTED;
     return c->width == 128 ? run_width<128>(c, x, mass, ws, st) : run_width<64>(c, x, mass, ws, st);
 }
 

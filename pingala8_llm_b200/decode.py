@@ -286,7 +286,8 @@ class TreeDecoder:
             q = cache.kv_append(q.view(1, T, c.heads, c.head_dim), k.view(1, T, c.kv_heads, c.head_dim), v.view(1, T, c.kv_heads, c.head_dim),
                                 self.k[L], self.v[L], self.lens, pos, self.cos, self.sin, q_norm=qn, k_norm=kn, eps=c.eps)
             a, lse = cache.tree_attention(q, self.k[L], self.v[L], self.lens, mask=mask)
-            self.seen.append((q, lse))
+            if self.budget is not None:
+                self.seen.append((q, lse))
             h = x + t["o"].mul_mat(a.view(T, -1).float())
             g, u = mul_mat_group([t["gate"], t["up"]], h, norm_weight=layer["ffn_norm"], eps=c.eps)
             x = h + t["down"].mul_mat(g, up=u)
@@ -332,13 +333,15 @@ class TreeDecoder:
         """greedy: prompt int64 [n], then n_new tokens; draft(history) -> (tokens, parents) of the tree to try, whose token 0 is
         the last of `history` (a list of ints); None: lookup_draft. Returns (tokens [n_new], passes)."""
         draft = draft or lookup_draft
+        if prompt.numel() < 1 or prompt.numel() + n_new > self.max_len:
+            raise ValueError(f"{prompt.numel()} + {n_new} tokens do not fit max_len {self.max_len}")
         self.reset()
         history = prompt.tolist()
         history.append(int(torch.argmax(self.prefill(prompt))))
         out, passes = [history[-1]], 0
         while len(out) < n_new:
             tokens, parents = draft(history)
-            room = min(len(tokens), n_new - len(out), self.max_len - self.position)
+            room = min(len(tokens), cache.TREE_MAX, n_new - len(out))
             tokens, parents = tokens[:room], parents[:room]  # a child comes after its parent: the rest is still a tree
             got = self.step(torch.tensor(tokens, device=prompt.device), torch.tensor(parents, dtype=torch.int32, device=prompt.device)).tolist()
             out += got

@@ -314,5 +314,6 @@ def active(slot):
 
 
 def device_error():
-    """1 if a kernel gave up on a bounded device wait since the last call (synchronises)."""
+    """Non-zero if a kernel gave up on a bounded device wait, or a cache operator left out something out of range, since the
+    last call (the bits of p8_device_error; synchronises)."""
     return int(lib().p8_device_error())

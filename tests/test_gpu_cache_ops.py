@@ -376,7 +376,7 @@ def masses(g, kind, *shape):
 @pytest.mark.parametrize("dt,layers,B,hk,D,lens,cap,budget,sinks,recent", [
     ("bf16", None, 1, 2, 64, [40], 40, 8, 0, 0), ("fp32", 2, 3, 2, 128, [0, 90, 33], 97, 33, 4, 8), ("fp16", 3, 2, 1, 128, [2500, 2049], 2600, 2048, 4, 64),
     ("bf16", 1, 2, 3, 128, [5000, 4000], 5001, 1, 0, 0), ("fp32", None, 2, 1, 64, [300, 300], 300, 64, 32, 32), ("fp16", None, 1, 2, 64, [70000], 70001, 9999, 3, 100),
-    ("bf16", None, 1, 1, 64, [20000], 20000, 1500, 0, 1500)])
+    ("bf16", None, 1, 1, 64, [20000], 20000, 1500, 0, 1500), ("fp16", None, 1, 1, 64, [7100], 7100, 700, 1, 1), ("fp32", None, 1, 1, 64, [6200], 12000, 100, 0, 9)])
 def test_evict(kind, dt, layers, B, hk, D, lens, cap, budget, sinks, recent):
     g, dtype = gen(budget + D), TYPES[dt]
     lead = (B, hk) if layers is None else (layers, B, hk)
@@ -555,6 +555,95 @@ def test_graphs_that_share_a_workspace_and_sequences_that_grow(dt):
         for i in range(2):
             assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
         assert torch.equal(mass, total)
+
+
+def test_a_whole_step_in_a_graph():
+    """append, attention, acceptance, masses and eviction of two layers captured together and replayed on other inputs give
+    what eager calls give, bit for bit"""
+    g = gen(16)
+    N, B, T, H, hk, D, cap, P = 2, 3, 6, 8, 2, 64, 200, 400
+    cos, sin = torch.rand(P, D // 2, device="cuda", generator=g), torch.rand(P, D // 2, device="cuda", generator=g)
+    par = torch.tensor([[-1, 0, 0, 1, 2, 3]] * B, dtype=torch.int32, device="cuda")
+    mask, depth = cache.tree_plan(par)
+
+    def inputs(seed):
+        g = gen(seed)
+        s = {"k": randn(g, N, B, hk, cap, D, dtype=torch.bfloat16), "v": randn(g, N, B, hk, cap, D, dtype=torch.bfloat16),
+             "q": randn(g, N, B, T, H, D), "xk": randn(g, N, B, T, hk, D), "xv": randn(g, N, B, T, hk, D), "mass": torch.rand(N, B, hk, cap, device="cuda", generator=g)}
+        s["lens"] = torch.randint(0, cap - T, (B,), device="cuda", generator=g).int()
+        s["tokens"], s["target"] = (torch.randint(0, 2, (B, T), device="cuda", generator=g) for _ in range(2))
+        return s
+
+    def step(s):
+        pos = s["lens"][:, None] + depth
+        outs = []
+        for i in range(N):
+            q = cache.kv_append(s["q"][i], s["xk"][i], s["xv"][i], s["k"][i], s["v"][i], s["lens"], pos, cos, sin)
+            outs.append((q, *cache.tree_attention(q, s["k"][i], s["v"][i], s["lens"], mask=mask)))
+        acc = cache.tree_accept(s["tokens"], par, s["target"], s["k"], s["v"], s["lens"])
+        for i in range(N):
+            cache.attention_mass(outs[i][0], outs[i][2], s["k"][i], s["lens"], s["mass"][i], rows=acc.path, counts=acc.accepted)
+        new, kept = cache.kv_evict(s["k"], s["v"], s["mass"], acc.new_lens, 64, 4, 16)
+        return [x for o in outs for x in o] + list(acc) + [new, kept]
+
+    fixed = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step({k: v.clone() for k, v in fixed.items()})
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(fixed)
+    for seed in (1, 2, 3):
+        new = inputs(seed)
+        for k in fixed:
+            fixed[k].copy_(new[k])
+        graph.replay()
+        want = step(new)
+        ended()
+        for i, (x, y) in enumerate(zip(got, want)):
+            assert torch.equal(x, y), i
+        for k in ("k", "v", "mass"):
+            assert torch.equal(fixed[k], new[k]), k
+
+
+def test_calls_run_in_order():
+    """what reads a call's results right behind it sees them, also where the joining launch has nothing to do (sequences
+    short enough for one CTA each) and where an eviction leaves every sequence as it is"""
+    g = gen(17)
+    k, v = randn(g, 8, 8, 300, 128, dtype=torch.float16), randn(g, 8, 8, 300, 128, dtype=torch.float16)
+    q = [randn(g, 8, 4, 32, 128, dtype=torch.float16) for _ in range(20)]
+    m = torch.rand(8, 8, 300, device="cuda", generator=g)
+    lens = ints(*[290] * 8)
+    want = [cache.tree_attention(x, k, v, lens)[0].float().sum() for x in q]
+    torch.cuda.synchronize()
+    out, lse = torch.empty_like(q[0]), torch.empty(8, 4, 32, device="cuda")
+    got = []
+    for x in q:
+        cache.tree_attention(x, k, v, lens, out=out, lse=lse)
+        got.append(out.float().sum())
+        out.zero_()
+        new, kept = cache.kv_evict(k, v, m, lens, 300)
+        got[-1] = got[-1] + 0 * (kept.sum() + new.sum())
+        assert torch.equal(new, lens) and bool((kept[:, :, 290:] == -1).all()) and torch.equal(kept[0, 0, :290].long(), torch.arange(290, device="cuda"))
+    ended()
+    assert torch.equal(torch.stack(got), torch.stack(want))
+
+
+def test_append_in_place_and_overlapping():
+    g = gen(18)
+    x, c = randn(g, 2, 5, 4, 64), torch.rand(9, 32, device="cuda", generator=g)
+    kc, vc = torch.zeros(2, 2, 12, 64, device="cuda"), torch.zeros(2, 2, 12, 64, device="cuda")
+    kv = randn(g, 2, 5, 2, 64)
+    pos = torch.arange(5, dtype=torch.int32, device="cuda").repeat(2, 1)
+    want = cache.kv_append(x, kv, kv, kc, vc, ints(0, 3), pos, c, c)
+    y = x.clone()
+    assert cache.kv_append(y, kv, kv, kc, vc, ints(0, 3), pos, c, c, q_out=y) is y and torch.equal(y, want)
+    big = torch.zeros(2, 6, 4, 64, device="cuda")
+    with pytest.raises(p8.P8Error):
+        cache.kv_append(big[:, :5], kv, kv, kc, vc, ints(0, 3), pos, c, c, q_out=big[:, 1:])
+    ended()
 
 
 def test_another_stream_and_two_calls_at_once():
