@@ -993,43 +993,51 @@ __device__ __forceinline__ float4 *query32(char *sq, int row, int col4) {
     return reinterpret_cast<float4 *>(sq + row * (D * 4) + (col4 ^ ((row & 1) << 2)) * 16);
 }
 
-// RT row tiles of 16 x KG = 8 / RT groups of slots: warp w has row tile w / KG and the slots of group w % KG in every tile,
-// with its own running maximum, sum and accumulator; the groups are joined at the segment's end. No barrier but the
-// ring's in between. Within the products the columns of K (and the slots in S and P) are taken in the order in which a
-// lane finds them in 16 consecutive bytes: the sums do not depend on it.
+// A group of four warps has 16 query rows. In a tile of 64 slots warp w of it computes the scores of slots 16 w .., the
+// group agrees on the running maximum, the weights go through shared memory, and warp w adds up the columns 32 w .. (of 64
+// columns: of half of the slots) of all weights and values. So every group keeps all four schedulers busy whatever the
+// number of row tiles, and a warp holds 16 accumulators a thread, not 64 (eight warps with all columns of their own slots
+// took 28 us where this takes F32_NOTE, 12 tokens x 32 heads over 2,047 slots). RT row tiles share every tile of K and V;
+// with fewer than four, two such sets of groups take the tiles in turn (NS) and are joined at the segment's end.
+// Within the products the columns of K (and the slots in S and P) are taken in the order in which a lane finds them in 16
+// consecutive bytes: the sums do not depend on it.
 // Bound by K and V from HBM for up to 16 rows, by the products beyond.
 template <int D, int RT>
 struct F32Shape {
+    static constexpr int NS = RT == 4 ? 1 : 2, kGroups = RT * NS, kWarps = 4 * kGroups, kThreads = kWarps * 32 + 32;
+    static constexpr int kSlices = D / 32, kParts = 4 / kSlices;  // of the columns; of the slots for each
     static constexpr int kStage = kTile32 * D * 4;
     static constexpr int kStages = D == 64 ? 8 : 5;
-    static constexpr int kQ = RT * 16 * D * 4, kJoin = (8 - RT) * 16 * D * 4;
-    static constexpr int kSmem = 1024 + kQ + kJoin + kStages * kStage;
+    static constexpr int kP = 68;  // a row of weights, so that rows start four banks apart
+    static constexpr int kQ = RT * 16 * D * 4, kWeights = kGroups * 16 * kP * 4, kJoin = (NS * kParts - 1) * RT * 16 * D * 4;
+    static constexpr int kSmem = kStages * kStage + kQ + kWeights + kJoin;
 };
 
 template <int D, int RT>
-__global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                                                          float *part_o, float2 *part_ml) {
+__global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk,
+                                                                               const __grid_constant__ CUtensorMap mv, float *part_o, float2 *part_ml) {
     using S_ = F32Shape<D, RT>;
-    constexpr int NST = S_::kStages, KG = 8 / RT, NK = kTile32 / 8 / KG, R = RT * 16;  // NK: groups of eight slots of a warp
-    extern __shared__ char dyn[];
-    char *ring = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *sq = ring + NST * S_::kStage, *join = sq + S_::kQ;
+    constexpr int NST = S_::kStages, NS = S_::NS, PARTS = S_::kParts, R = RT * 16, P = S_::kP, ALL = S_::kWarps * 32;
+    constexpr Cut cut{R, kTile32, 1, 0};
+    extern __shared__ __align__(1024) char dyn[];
+    char *ring = dyn, *sq = ring + NST * S_::kStage;
+    float *weights = reinterpret_cast<float *>(sq + S_::kQ), *join = weights + S_::kWeights / 4;
     __shared__ uint64_t b_full[NST], b_empty[NST];
     __shared__ int s_gave_up;
     __shared__ Share s_share;
-    __shared__ float2 s_ml[8][16];
+    __shared__ float s_max[S_::kGroups][4][16], s_sum[S_::kGroups][4][16], s_m[S_::kGroups][16];
     __shared__ unsigned long long s_bad;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{R, kTile32, 1, 0};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
-    } else if (tid == 256) {
+    } else if (tid == ALL) {
         map_prefetch(&mk);
         map_prefetch(&mv);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
-            mbar_init(b_empty + i, 8);
+            mbar_init(b_empty + i, 4 * RT);
         }
         s_gave_up = 0;
         s_bad = 0;
@@ -1038,7 +1046,7 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Walk w(a, cut, s_share);
-    if (warp == 8) {  // loads
+    if (tid >= ALL) {  // loads
         uint32_t n = 0;
         while (w.next()) {
             for (int t = w.ta; t < w.tb; ++t)
@@ -1057,29 +1065,34 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
         return;
     }
-    const int rt = warp / KG, kg = warp % KG, g = lane / 4, t = lane % 4;  // (so that the four schedulers share the row tiles that are there)
+    const int group = warp / 4, rt = group % RT, ns = group / RT, wq = warp % 4, g = lane / 4, t = lane % 4;
+    const int slice = wq % S_::kSlices, part = wq / S_::kSlices, contrib = ns * PARTS + part;
+    auto sync_group = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
+    auto sync_all = [&] { asm volatile("bar.sync 8, %0;" ::"n"(ALL) : "memory"); };
+    float *pw = weights + group * 16 * P;
     const float c = a.scale * 1.4426950408889634f;
-    uint32_t n = 0;
+    uint32_t base = 0;
     while (w.next()) {
         const int h = w.head(), row0 = w.row0(), rows = w.n * a.group;
         const float *q = static_cast<const float *>(a.q) + w.b * a.qs[0];
-        constexpr int C = D / 4, QN = R * C / 256;  // a thread's pieces of the query rows, all in flight at once
+        constexpr int C = D / 4, QN = (R * C + ALL - 1) / ALL;  // a thread's pieces of the query rows, all in flight at once
         float4 qv[QN];
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
-            const int row = row0 + tid / C + i * (256 / C), tok = row / a.group;
+            const int r = tid / C + i * (ALL / C), row = row0 + r, tok = row / a.group;
             qv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < rows) qv[i] = *reinterpret_cast<const float4 *>(q + tok * a.qs[1] + (long long)(h * a.group + row - tok * a.group) * a.qs[2] + 4 * (tid % C));
+            if (r < R && row < rows) qv[i] = *reinterpret_cast<const float4 *>(q + tok * a.qs[1] + (long long)(h * a.group + row - tok * a.group) * a.qs[2] + 4 * (tid % C));
         }
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
             const float4 v = qv[i];
-            *query32<D>(sq, tid / C + i * (256 / C), tid % C) = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);  // scores in base 2
+            const int r = tid / C + i * (ALL / C);
+            if (r < R) *query32<D>(sq, r, tid % C) = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);  // scores in base 2
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const bool warp_live = row0 + 16 * rt < rows;
+        sync_all();
+        const bool live = row0 + 16 * rt < rows;  // the group has rows
         unsigned long long sees[2] = {0, 0};
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 32][4][4] = {};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4] = {};
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             const int row = row0 + 16 * rt + g + 8 * y;
@@ -1089,86 +1102,88 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                 if (w.n < 64) sees[y] &= (1ull << w.n) - 1;
             }
         }
-        for (int tile = w.ta; tile < w.tb; ++tile) {
-            const int key0 = tile * kTile32 + kg * NK * 8;  // the warp's first slot
-            const bool tail = key0 + NK * 8 > w.len;
-            float s[NK][4] = {}, s2[2][NK][4] = {};
-            const int sk = n % NST;
-            wait(b_full + sk, n / NST & 1);
-            ++n;
-            if (warp_live) {
-                const char *st = ring + sk * S_::kStage;
-                const int slot = kg * NK * 8 + (g >> 1) + ((g & 1) << 2);
+#pragma unroll 1
+        for (int tile = w.ta + ns; tile < w.tb; tile += NS) {
+            const uint32_t nk = base + 2 * (tile - w.ta), nv = nk + 1;
+            const int stk = nk % NST, stv = nv % NST;
+            const int key0 = tile * kTile32, off = key0 + 16 * wq;  // off: the first slot of the warp's scores
+            const bool tail = key0 + kTile32 > w.len;
+            float s[2][4];
+            wait(b_full + stk, nk / NST & 1);
+            if (live) {
+                const char *st = ring + stk * S_::kStage;
+                const int slot = 16 * wq + (g >> 1) + ((g & 1) << 2);
+                float s2[2][2][4] = {};
 #pragma unroll 2
                 for (int d = 0; d < D / 16; ++d) {
-                    float4 k[NK];
-#pragma unroll
-                    for (int j = 0; j < NK; ++j) k[j] = stage32(st, slot + 8 * j, 4 * d + t);
+                    const float4 k[2] = {stage32(st, slot, 4 * d + t), stage32(st, slot + 8, 4 * d + t)};
                     mma_scores(s2, *query32<D>(sq, 16 * rt + g, 4 * d + t), *query32<D>(sq, 16 * rt + g + 8, 4 * d + t), k);
                 }
 #pragma unroll
-                for (int j = 0; j < NK; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[j][e] = s2[0][j][e] + s2[1][j][e];
+                    for (int e = 0; e < 4; ++e) s[j][e] = s2[0][j][e] + s2[1][j][e];  // row g + 8 (e / 2), slot off + 8 j + t + 4 (e % 2)
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(b_empty + sk);
-            if (warp_live) {  // s[j][2 y + e]: row g + 8 y, slot key0 + 8 j + t + 4 e
+            if (lane == 0) mbar_arrive(b_empty + stk);
+            if (live) {
                 if (tail) {
 #pragma unroll
-                    for (int j = 0; j < NK; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int at = key0 + 8 * j + t + 4 * (e & 1) - w.len, row = row0 + 16 * rt + g + 8 * (e >> 1);
+                            const int at = off + 8 * j + t + 4 * (e & 1) - w.len, row = row0 + 16 * rt + g + 8 * (e >> 1);
                             if (row >= rows || (at >= 0 && (at >= w.n || !(sees[e >> 1] >> at & 1)))) s[j][e] = -INFINITY;
                         }
                 }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float top = fmaxf(fmaxf(s[0][2 * y], s[0][2 * y + 1]), fmaxf(s[1][2 * y], s[1][2 * y + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (t == 0) s_max[group][wq][g + 8 * y] = top;
+                }
+                sync_group();
                 float f[2];
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    float top = s[0][2 * y];
-#pragma unroll
-                    for (int j = 0; j < NK; ++j) top = fmaxf(top, fmaxf(s[j][2 * y], s[j][2 * y + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    top = fmaxf(top, m[y]);
+                    const int r = g + 8 * y;
+                    const float top = fmaxf(fmaxf(fmaxf(s_max[group][0][r], s_max[group][1][r]), fmaxf(s_max[group][2][r], s_max[group][3][r])), m[y]);
                     f[y] = top == m[y] ? 1.f : ex2(m[y] - top);
                     m[y] = top;
                     const float sub = top == -INFINITY ? 0.f : top;
                     float sum = 0.f;
 #pragma unroll
-                    for (int j = 0; j < NK; ++j) {
-                        s[j][2 * y] = ex2(s[j][2 * y] - sub);
-                        s[j][2 * y + 1] = ex2(s[j][2 * y + 1] - sub);
-                        sum += s[j][2 * y] + s[j][2 * y + 1];
-                    }
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float p = ex2(s[j][2 * y + e] - sub);
+                            sum += p;
+                            pw[r * P + 16 * wq + 8 * j + t + 4 * e] = p;
+                        }
                     l[y] = l[y] * f[y] + sum;
                 }
                 if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-                    for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[x][i][0] *= f[0];
-                            o[x][i][1] *= f[0];
-                            o[x][i][2] *= f[1];
-                            o[x][i][3] *= f[1];
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        o[i][0] *= f[0];
+                        o[i][1] *= f[0];
+                        o[i][2] *= f[1];
+                        o[i][3] *= f[1];
+                    }
                 }
             }
-            const int sv = n % NST;
-            wait(b_full + sv, n / NST & 1);
-            ++n;
-            if (warp_live) {
-                char *st = ring + sv * S_::kStage;
-                const int groups = (w.len + w.n - key0 + 7) / 8;  // of eight slots that hold something; the others are not multiplied
+            wait(b_full + stv, nv / NST & 1);
+            if (live) {
+                char *st = ring + stv * S_::kStage;
+                const int eights = (w.len + w.n - key0 + 7) / 8;  // of the tile's slots that hold something; the others are not multiplied
                 if (tail) {
-                    // A weight of 0 times an infinity is not 0: the warp's slots that no row sees become zero (as far as they are multiplied), and so do a
-                    // drafted token's infinities and NaN (they reach the rows that see it at the segment's end). Warps
-                    // with other rows of the same slots write the same zeros.
+                    // A weight of 0 times an infinity is not 0: slots that no row sees become zero (as far as they are multiplied),
+                    // and so do a drafted token's infinities and NaN (they reach the rows that see it at the segment's end).
+                    // Groups with other rows of the same slots write the same zeros.
 #pragma unroll 1
-                    for (int i = max(0, w.len - key0) * (D / 4) + lane; i < min(NK, groups) * 8 * (D / 4); i += 32) {
-                        const int slot = kg * NK * 8 + i / (D / 4), col4 = i % (D / 4), at = tile * kTile32 + slot - w.len;
+                    for (int i = max(0, w.len - key0) * (D / 4) + wq * 32 + lane; i < min(8, eights) * 8 * (D / 4); i += 128) {
+                        const int slot = i / (D / 4), col4 = i % (D / 4), at = key0 + slot - w.len;
                         float4 *v = reinterpret_cast<float4 *>(st + (col4 / 8) * 8192 + slot * 128 + ((col4 % 8) ^ (slot % 8)) * 16);
                         const float4 x = *v;
                         if (at < w.n && isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w)) continue;
@@ -1178,95 +1193,86 @@ __global__ void __launch_bounds__(288, 1) k_tree_attn_f32(const AttnArgs a, cons
                                          real && isfinite(x.w) ? x.w : 0.f);
                     }
                     fence_proxy_async();  // the stage is the TMA's again after this tile
-                    __syncwarp();
                 }
-#pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    if (j >= groups) break;
-                    const Frag p(s[j][0], s[j][2], s[j][1], s[j][3]);
-                    const int slot = kg * NK * 8 + 8 * j + t;
-#pragma unroll
-                    for (int x = 0; x < D / 32; ++x) {
-                        const int col4 = 8 * x + (g >> 1) + ((g & 1) << 2);
-                        const float4 u = stage32(st, slot, col4), v = stage32(st, slot + 4, col4);
-                        mma_four(o[x], p, u, v);
-                    }
+                sync_group();  // the weights are there
+                const int j1 = min((part + 1) * (8 / PARTS), eights), col4 = 8 * slice + (g >> 1) + ((g & 1) << 2);
+#pragma unroll 2
+                for (int j = part * (8 / PARTS); j < j1; ++j) {
+                    const float *x = pw + g * P + 8 * j + t;
+                    mma_four(o, Frag(x[0], x[8 * P], x[4], x[8 * P + 4]), stage32(st, 8 * j + t, col4), stage32(st, 8 * j + t + 4, col4));
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(b_empty + sv);
+            if (lane == 0) mbar_arrive(b_empty + stv);
         }
-        // o[x][i][2 y + e]: row g + 8 y, column 32 x + 16 e + 4 t + i
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
-            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
-        }
-        if (KG > 1 && kg > 0 && warp_live) {
+        // o[i][2 y + e]: row g + 8 y, column 32 slice + 16 e + 4 t + i
+        if (live) {
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                if (t == 0) s_ml[warp][g + 8 * y] = make_float2(m[y], l[y]);
+                l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+                l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+                if (t == 0) {
+                    s_sum[group][wq][g + 8 * y] = l[y];
+                    if (wq == 0) s_m[group][g + 8 * y] = m[y];
+                }
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float4 *>(join + ((((kg - 1) * RT + rt) * 16 + g + 8 * y) * D + 32 * x + 16 * e + 4 * t) * 4) =
-                            make_float4(o[x][0][2 * y + e], o[x][1][2 * y + e], o[x][2][2 * y + e], o[x][3][2 * y + e]);
+                for (int e = 0; e < 2; ++e)
+                    if (contrib > 0)
+                        *reinterpret_cast<float4 *>(join + (((contrib - 1) * RT + rt) * 16 + g + 8 * y) * D + 32 * slice + 16 * e + 4 * t) =
+                            make_float4(o[0][2 * y + e], o[1][2 * y + e], o[2][2 * y + e], o[3][2 * y + e]);
             }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (kg == 0 && warp_live) {
+        sync_all();
+        if (contrib == 0 && live) {
             const bool whole = w.whole();
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const int row = row0 + 16 * rt + g + 8 * y;
-                float top = m[y];
+                const int r = g + 8 * y, row = row0 + 16 * rt + r;
+                float top = m[y], f[NS], sum = 0.f;
 #pragma unroll
-                for (int k = 1; k < KG; ++k) top = fmaxf(top, s_ml[rt * KG + k][g + 8 * y].x);
-                const float f0 = m[y] == top ? 1.f : ex2(m[y] - top);
-                float f[KG], sum = l[y] * f0;
+                for (int x = 0; x < NS; ++x) top = fmaxf(top, s_m[x * RT + rt][r]);
 #pragma unroll
-                for (int k = 1; k < KG; ++k) {
-                    const float2 ml = s_ml[rt * KG + k][g + 8 * y];
-                    f[k] = ml.x == top ? 1.f : ex2(ml.x - top);
-                    sum = fmaf(ml.y, f[k], sum);
+                for (int x = 0; x < NS; ++x) {
+                    const float mx = s_m[x * RT + rt][r];
+                    f[x] = mx == top ? 1.f : ex2(mx - top);
+                    sum += f[x] * ((s_sum[x * RT + rt][0][r] + s_sum[x * RT + rt][1][r]) + (s_sum[x * RT + rt][2][r] + s_sum[x * RT + rt][3][r]));
                 }
                 if (row >= rows) continue;
                 const int tok = row / a.group, head = h * a.group + row - tok * a.group;
-                const long long pr = ((long long)blockIdx.x * 2 + (w.opens ? 0 : 1)) * R + 16 * rt + g + 8 * y;
+                const long long pr = ((long long)blockIdx.x * 2 + (w.opens ? 0 : 1)) * R + 16 * rt + r;
                 const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                 float *out = whole ? static_cast<float *>(a.out) + w.b * a.os[0] + tok * a.os[1] + (long long)head * a.os[2] : part_o + pr * D;
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x)
+                for (int e = 0; e < 2; ++e) {
+                    const int col = 32 * slice + 16 * e + 4 * t;
+                    float v[4];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int col = 32 * x + 16 * e + 4 * t;
-                        float v[4];
+                    for (int i = 0; i < 4; ++i) v[i] = o[i][2 * y + e] * f[0];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = o[x][i][2 * y + e] * f0;
-#pragma unroll
-                        for (int k = 1; k < KG; ++k) {
-                            const float4 z = *reinterpret_cast<const float4 *>(join + ((((k - 1) * RT + rt) * 16 + g + 8 * y) * D + col) * 4);
-                            v[0] = fmaf(z.x, f[k], v[0]);
-                            v[1] = fmaf(z.y, f[k], v[1]);
-                            v[2] = fmaf(z.z, f[k], v[2]);
-                            v[3] = fmaf(z.w, f[k], v[3]);
-                        }
-                        *reinterpret_cast<float4 *>(out + col) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    for (int x = 1; x < NS * PARTS; ++x) {
+                        const float4 z = *reinterpret_cast<const float4 *>(join + (((x - 1) * RT + rt) * 16 + r) * D + col);
+                        const float fx = f[x / PARTS];
+                        v[0] = fmaf(z.x, fx, v[0]);
+                        v[1] = fmaf(z.y, fx, v[1]);
+                        v[2] = fmaf(z.z, fx, v[2]);
+                        v[3] = fmaf(z.w, fx, v[3]);
                     }
-                const unsigned long long bad = s_bad & sees[y];
-                if (bad) {
-                    const float *v = static_cast<const float *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)w.len * a.vs[2];
-                    for (int col = 4 * t; col < D; col += 16) add_bad(out, v, a.vs[2], bad, col, col + 4);  // the thread's own columns
+                    *reinterpret_cast<float4 *>(out + col) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                 }
-                if (t == 0) {
+                const unsigned long long bad = s_bad & sees[y];
+                if (bad) {  // the thread's own columns
+                    const float *v = static_cast<const float *>(a.v) + w.b * a.vs[0] + h * a.vs[1] + (long long)w.len * a.vs[2];
+                    for (int e = 0; e < 2; ++e) add_bad(out, v, a.vs[2], bad, 32 * slice + 16 * e + 4 * t, 32 * slice + 16 * e + 4 * t + 4);
+                }
+                if (t == 0 && wq == 0) {
                     if (!whole) part_ml[pr] = make_float2(top, sum);
                     else if (a.lse) a.lse[((long long)w.b * a.tokens + tok) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
                 }
             }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        sync_all();
         if (tid == 0) s_bad = 0;  // the next segment's first barrier comes before its first use
+        base += 2 * (w.tb - w.ta);
         w.advance();
     }
 }
@@ -1461,12 +1467,11 @@ int sm_count() {
     return v;
 }
 
-// Query rows of a unit. 16-bit: one block for up to 256, so that K and V are read once. 32-bit: the products bound it, so
-// blocks whose 16-row tiles fill the four schedulers (three tiles: 32 + 16 rows take 576 products a scheduler and tile,
-// a block of 64 takes 768); more blocks read K and V from L2 again, at less than half of its rate.
+// Query rows of a unit. 16-bit: one block for up to 256, so that K and V are read once. 32-bit: up to 64, since the
+// products bound more rows anyway; further blocks read K and V from L2 again, at less than half of its rate.
 Cut attn_cut(const p8_kv *c, int64_t rows) {
     if (c->type != P8_KV_F32) return rows > 128 ? Cut{256, kTile, TcShape<64, true>::kLeast, start_of(256)} : Cut{128, kTile, TcShape<64, false>::kLeast, start_of(128)};
-    return {rows <= 16 ? 16 : rows <= 48 ? 32 : 64, kTile32, 1, 0};
+    return {rows <= 16 ? 16 : rows <= 32 ? 32 : 64, kTile32, 1, 0};
 }
 int64_t attn_tiles(const p8_kv *c, int64_t rows, Cut cut) {
     return c->batch * c->heads * ((rows + cut.rblock - 1) / cut.rblock) * ((c->slots + cut.tile - 1) / cut.tile + cut.start);
@@ -1503,9 +1508,9 @@ p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
 template <int D>
 p8_status run_f32(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     switch (attn_cut(c, (int64_t)a.tokens * a.group).rblock) {
-        case 16: return run_attn<float, D>(k_tree_attn_f32<D, 1>, 288, F32Shape<D, 1>::kSmem, 0.f, c, a, ws, st);
-        case 32: return run_attn<float, D>(k_tree_attn_f32<D, 2>, 288, F32Shape<D, 2>::kSmem, 0.f, c, a, ws, st);
-        default: return run_attn<float, D>(k_tree_attn_f32<D, 4>, 288, F32Shape<D, 4>::kSmem, 0.f, c, a, ws, st);
+        case 16: return run_attn<float, D>(k_tree_attn_f32<D, 1>, F32Shape<D, 1>::kThreads, F32Shape<D, 1>::kSmem, 0.f, c, a, ws, st);
+        case 32: return run_attn<float, D>(k_tree_attn_f32<D, 2>, F32Shape<D, 2>::kThreads, F32Shape<D, 2>::kSmem, 0.f, c, a, ws, st);
+        default: return run_attn<float, D>(k_tree_attn_f32<D, 4>, F32Shape<D, 4>::kThreads, F32Shape<D, 4>::kSmem, 0.f, c, a, ws, st);
     }
 }
 // At most `most` rows a launch (what its shared memory holds); the later launches add to the first one's sums.
