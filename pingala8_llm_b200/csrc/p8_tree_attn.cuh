@@ -1277,43 +1277,44 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
     }
 }
 
-// The masses of a 32-bit cache: a warp has eight slots of a tile, split once, and goes through the query rows 16 at a
-// time; a lane's two slots are summed over its rows, and over the eight lanes that share them at the end.
+// The masses of a 32-bit cache. Four groups of four warps take the tiles in turn; a warp has 16 of the 64 slots and goes
+// through the query rows 16 at a time. A lane's four slots are summed over its rows, and over the eight lanes that share
+// them at the end. (Eight warps with eight slots of every tile each: OLD_MASS.)
 template <int D>
 struct F32Mass {
-    static constexpr int kRows = 256;
+    static constexpr int kRows = 128, kGroups = 4, kThreads = 4 * kGroups * 32 + 32;
     static constexpr int kStage = kTile32 * D * 4;
-    static constexpr int kStages = 3;
-    static constexpr int kSmem = 1024 + kRows * D * 4 + kStages * kStage;
+    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kSmem = kStages * kStage + kRows * D * 4;
 };
 template <int D>
-__global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
+__global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
     using S_ = F32Mass<D>;
-    constexpr int NST = S_::kStages;
-    extern __shared__ char dyn[];
-    char *ring = (char *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *sq = ring + NST * S_::kStage;
+    constexpr int NST = S_::kStages, NG = S_::kGroups, ALL = NG * 128;
+    constexpr Cut cut{1 << 30, kTile32, 1, 0};
+    extern __shared__ __align__(1024) char dyn[];
+    char *ring = dyn, *sq = ring + NST * S_::kStage;
     __shared__ uint64_t b_full[NST], b_empty[NST];
     __shared__ int s_gave_up;
     __shared__ Share s_share;
     __shared__ float s_nl[S_::kRows];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
-    const Cut cut{1 << 30, kTile32, 1, 0};
     if (warp == 0) {
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
-    } else if (tid == 256) {
+    } else if (tid == ALL) {
         map_prefetch(&mk);
         for (int i = 0; i < NST; ++i) {
             mbar_init(b_full + i, 1);
-            mbar_init(b_empty + i, 8);
+            mbar_init(b_empty + i, 4);
         }
         s_gave_up = 0;
         fence_mbar_init();
     }
     __syncthreads();
     Walk w(a, cut, s_share);
-    if (warp == 8) {
+    if (tid >= ALL) {
         uint32_t n = 0;
         while (w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
@@ -1330,12 +1331,13 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
         return;
     }
-    const int g = lane / 4, t = lane % 4;
+    auto sync_all = [&] { asm volatile("bar.sync 1, %0;" ::"n"(ALL) : "memory"); };
+    const int group = warp / 4, wq = warp % 4, g = lane / 4, t = lane % 4;
     const float c = a.scale * 1.4426950408889634f;
-    uint32_t n = 0;
+    uint32_t base = 0;
     while (w.next()) {
         const int rows = w.n * a.gc, h = w.u, padded = (rows + 15) / 16 * 16;
-        for (int i = tid; i < padded * (D / 4); i += 256) {
+        for (int i = tid; i < padded * (D / 4); i += ALL) {
             const int col4 = i % (D / 4), row = i / (D / 4);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float nl = -INFINITY;
@@ -1356,50 +1358,63 @@ __global__ void __launch_bounds__(288, 1) k_attn_mass_f32(const AttnArgs a, cons
             *query32<D>(sq, row, col4) = v;
             if (col4 == 0) s_nl[row] = nl;
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        sync_all();
         const float *min_ = a.mass + w.b * a.ms[0] + h * a.ms[1];
         float *mout = a.mass_out + w.b * a.mos[0] + h * a.mos[1];
-        for (int tile = w.ta; tile < w.tb; ++tile) {
-            const int key0 = tile * kTile32 + 8 * warp;
-            const int st = n % NST;
-            wait(b_full + st, n / NST & 1);
-            ++n;
-            float4 k[D / 16];
+#pragma unroll 1
+        for (int tile = w.ta + group; tile < w.tb; tile += NG) {
+            const uint32_t n = base + tile - w.ta;
+            const char *st = ring + n % NST * S_::kStage;
+            const int key0 = tile * kTile32 + 16 * wq, end = w.len + w.n, slot = 16 * wq + (g >> 1) + ((g & 1) << 2);
+            float before = 0.f;  // of slot key0 + lane
+            if (lane < 16 && key0 + lane < end) before = key0 + lane < w.len ? min_[key0 + lane] : a.more ? mout[key0 + lane] : 0.f;
+            wait(b_full + n % NST, n / NST & 1);
+            float sum[2][2] = {};
+            if (key0 < end) {
+                int from[2][2];  // the first row that sees the slot
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) k[d] = stage32(ring + st * S_::kStage, 8 * warp + (g >> 1) + ((g & 1) << 2), 4 * d + t);
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int late = key0 + 8 * j + t + 4 * e - w.len;
+                        from[j][e] = late <= 0 ? 0 : late < w.n ? late * a.gc : rows;
+                    }
+#pragma unroll 1
+                for (int r0 = 0; r0 < padded; r0 += 16) {
+                    float s2[2][2][4] = {};
+#pragma unroll 2
+                    for (int d = 0; d < D / 16; ++d) {
+                        const float4 k[2] = {stage32(st, slot, 4 * d + t), stage32(st, slot + 8, 4 * d + t)};
+                        mma_scores(s2, *query32<D>(sq, r0 + g, 4 * d + t), *query32<D>(sq, r0 + g + 8, 4 * d + t), k);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = r0 + g + 8 * (e >> 1);
+                        const float nl = s_nl[row];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float p = ex2(s2[0][j][e] + s2[1][j][e] + nl);
+                            if (row >= from[j][e & 1] && row < rows) sum[j][e & 1] += p;
+                        }
+                    }
+                }
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(b_empty + st);
-            if (key0 >= w.len + w.n) continue;
-            float sum[2] = {0.f, 0.f};
-            int from[2];  // the first row that sees the slot
+            if (lane == 0) mbar_arrive(b_empty + n % NST);
+            // lane i < 16 writes slot key0 + i: the sum that lanes t = i % 4 hold as (j, e) = (i / 8, i / 4 % 2)
+            float mine = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int late = key0 + t + 4 * e - w.len;
-                from[e] = late <= 0 ? 0 : late < w.n ? late * a.gc : rows;
-            }
-            for (int r0 = 0; r0 < padded; r0 += 16) {
-                float s2[2][1][4] = {};
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                    const float4 kd[1] = {k[d]};
-                    mma_scores(s2, *query32<D>(sq, r0 + g, 4 * d + t), *query32<D>(sq, r0 + g + 8, 4 * d + t), kd);
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) sum[j][e] += __shfl_xor_sync(0xffffffffu, sum[j][e], x);
+                    if (lane / 4 == 2 * j + e) mine = sum[j][e];
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = r0 + g + 8 * (e >> 1);
-                    const float p = ex2(s2[0][0][e] + s2[1][0][e] + s_nl[row]);
-                    if (row >= from[e & 1] && row < rows) sum[e & 1] += p;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], x);
-                const int key = key0 + t + 4 * e;
-                if (g == 0 && key < w.len + w.n) mout[key] = (key < w.len ? min_[key] : a.more ? mout[key] : 0.f) + sum[e];
-            }
+            if (lane < 16 && key0 + lane < end) mout[key0 + lane] = before + mine;
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the query rows are done with
+        sync_all();  // the query rows are done with
+        base += w.tb - w.ta;
         w.advance();
     }
 }
@@ -1545,7 +1560,7 @@ p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     if (!encode_tiled()) return P8_ERR_CUDA;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1, 0});
-    return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, 288, F32Mass<D>::kSmem, st>>>(x, mk); });
+    return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, F32Mass<D>::kThreads, F32Mass<D>::kSmem, st>>>(x, mk); });
 }
 template <int D>
 p8_status run_width(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cudaStream_t st) {
