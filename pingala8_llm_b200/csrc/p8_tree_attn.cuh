@@ -920,17 +920,20 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 // ================================================================================================================
 // 32-bit caches: products of 32-bit values on the tensor cores
 // ================================================================================================================
-// x = hi + lo, both TF32 (8 + 11 bits): x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y|, three mma.sync products with
-// fp32 sums. (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
+// x = hi + lo, both TF32 (8 + 11 bits; hi rounded, so that lo has either sign): x y = hi hi' + hi lo' + lo hi' up to
+// 2^-21 |x y|, three mma.sync products with fp32 sums. The tensor cores cut what they add off, they do not round it: so
+// products with a small piece have sums of their own, a tile's products of weights and values are added to the
+// accumulator by fp32 additions, and scores have two sums (all in one, and hi cut off: 2.8e-6 off 64 bits instead of 0.6e-6, where
+// a plain fp32 product is 1.2e-6 off; it costs 27.7 us instead of 24.9 at 12 tokens x 32 heads over 2,047 slots). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
 // more shared-memory traffic than the products take. From registers the split costs three integer or fp32 operations.)
 // A product waits for the one before it on the same sum (four of them take that long to issue), so the order is by piece,
-// through as many sums as there are, and scores have two sums each.
+// through as many sums as there are.
 struct Split {
     uint32_t hi, lo;  // the tensor cores leave out the last 13 bits
 };
 __device__ __forceinline__ Split split(float x) {
     Split s;
-    s.hi = __float_as_uint(x) & 0xFFFFE000u;
+    s.hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
     s.lo = __float_as_uint(x - __uint_as_float(s.hi));
     return s;
 }
@@ -953,33 +956,32 @@ __device__ __forceinline__ void mma_part(float (&c)[4], const Frag &a, int part,
     else if (part == 1) mma8(c, a.x[0].lo, a.x[1].lo, a.x[2].lo, a.x[3].lo, u.hi, v.hi);
     else mma8(c, a.x[0].hi, a.x[1].hi, a.x[2].hi, a.x[3].hi, u.hi, v.hi);
 }
-// c[i] += a (b0[i], b1[i]) for four sums
-__device__ __forceinline__ void mma_four(float (&c)[4][4], const Frag &a, const float4 &b0, const float4 &b1) {
+// c[i] += a (b0[i], b1[i]) for four sums of the large pieces' products, x[i] for those with a small one
+__device__ __forceinline__ void mma_four(float (&c)[4][4], float (&x)[4][4], const Frag &a, const float4 &b0, const float4 &b1) {
     const Split u[4] = {split(b0.x), split(b0.y), split(b0.z), split(b0.w)}, v[4] = {split(b1.x), split(b1.y), split(b1.z), split(b1.w)};
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mma_part(c[i], a, part, u[i], v[i]);
+        for (int i = 0; i < 4; ++i) mma_part(part < 2 ? x[i] : c[i], a, part, u[i], v[i]);
 }
-// 16 columns of scores: c[0] and c[1] each take half of the columns, for N groups of slots (k[j]: a lane's four columns)
+// 16 columns of scores: c[0] and c[1] each take half of the columns' large pieces, c[2] the products with a small one, for N
+// groups of slots (k[j]: a lane's four columns)
 template <int N>
-__device__ __forceinline__ void mma_scores(float (&c)[2][N][4], const float4 &q0, const float4 &q1, const float4 (&k)[N]) {
-    const Frag a(q0.x, q1.x, q0.y, q1.y), b(q0.z, q1.z, q0.w, q1.w);
-    Split s[N][4];
+__device__ __forceinline__ void mma_scores(float (&c)[3][N][4], const float4 &q0, const float4 &q1, const float4 (&k)[N]) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        s[j][0] = split(k[j].x);
-        s[j][1] = split(k[j].y);
-        s[j][2] = split(k[j].z);
-        s[j][3] = split(k[j].w);
-    }
-#pragma unroll
-    for (int part = 0; part < 3; ++part)
+    for (int half = 0; half < 2; ++half) {
+        const Frag a = half ? Frag(q0.z, q1.z, q0.w, q1.w) : Frag(q0.x, q1.x, q0.y, q1.y);
+        Split s[N][2];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            mma_part(c[0][j], a, part, s[j][0], s[j][1]);
-            mma_part(c[1][j], b, part, s[j][2], s[j][3]);
+            s[j][0] = split(half ? k[j].z : k[j].x);
+            s[j][1] = split(half ? k[j].w : k[j].y);
         }
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int j = 0; j < N; ++j) mma_part(c[part < 2 ? 2 : half][j], a, part, s[j][0], s[j][1]);
+    }
 }
 constexpr int kTile32 = 64;
 // A stage holds 64 slots in parts of 32 columns as the tensor map's loads leave them: 128-byte rows, the 16-byte pieces
@@ -1113,8 +1115,8 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
             if (live) {
                 const char *st = ring + stk * S_::kStage;
                 const int slot = 16 * wq + (g >> 1) + ((g & 1) << 2);
-                float s2[2][2][4] = {};
-#pragma unroll 2
+                float s2[3][2][4] = {};
+#pragma unroll 1
                 for (int d = 0; d < D / 16; ++d) {
                     const float4 k[2] = {stage32(st, slot, 4 * d + t), stage32(st, slot + 8, 4 * d + t)};
                     mma_scores(s2, *query32<D>(sq, 16 * rt + g, 4 * d + t), *query32<D>(sq, 16 * rt + g + 8, 4 * d + t), k);
@@ -1122,7 +1124,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[j][e] = s2[0][j][e] + s2[1][j][e];  // row g + 8 (e / 2), slot off + 8 j + t + 4 (e % 2)
+                    for (int e = 0; e < 4; ++e) s[j][e] = (s2[0][j][e] + s2[1][j][e]) + s2[2][j][e];  // row g + 8 (e / 2), slot off + 8 j + t + 4 (e % 2)
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(b_empty + stk);
@@ -1196,11 +1198,16 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
                 }
                 sync_group();  // the weights are there
                 const int j1 = min((part + 1) * (8 / PARTS), eights), col4 = 8 * slice + (g >> 1) + ((g & 1) << 2);
-#pragma unroll 2
+                float large[4][4] = {}, small[4][4] = {};
+#pragma unroll 1
                 for (int j = part * (8 / PARTS); j < j1; ++j) {
                     const float *x = pw + g * P + 8 * j + t;
-                    mma_four(o, Frag(x[0], x[8 * P], x[4], x[8 * P + 4]), stage32(st, 8 * j + t, col4), stage32(st, 8 * j + t + 4, col4));
+                    mma_four(large, small, Frag(x[0], x[8 * P], x[4], x[8 * P + 4]), stage32(st, 8 * j + t, col4), stage32(st, 8 * j + t + 4, col4));
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] += large[i][e] + small[i][e];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(b_empty + stv);
@@ -1381,7 +1388,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
                     }
 #pragma unroll 1
                 for (int r0 = 0; r0 < padded; r0 += 16) {
-                    float s2[2][2][4] = {};
+                    float s2[3][2][4] = {};
 #pragma unroll 2
                     for (int d = 0; d < D / 16; ++d) {
                         const float4 k[2] = {stage32(st, slot, 4 * d + t), stage32(st, slot + 8, 4 * d + t)};
@@ -1393,7 +1400,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
                         const float nl = s_nl[row];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float p = ex2(s2[0][j][e] + s2[1][j][e] + nl);
+                            const float p = ex2((s2[0][j][e] + s2[1][j][e]) + (s2[2][j][e] + nl));
                             if (row >= from[j][e & 1] && row < rows) sum[j][e & 1] += p;
                         }
                     }
