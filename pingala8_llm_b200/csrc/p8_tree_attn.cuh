@@ -21,10 +21,13 @@ struct AttnArgs {
 // A unit is (sequence, cache head, block of query rows); its slots are cut into tiles. All tiles of all units
 // form one list, sequence by sequence, with a few places more for the beginning of each unit, and every CTA takes an
 // equal contiguous share of it, so that the SMs finish together whatever the lengths are, and one long sequence still
-// fills them. A unit that lies in one share is finished
-// there; the parts of the others go to the workspace as (sum of p v, maximum, sum of p) and k_attn_join adds them up.
-__host__ __device__ constexpr int start_of(int rblock) { return rblock > 128 ? 4 : 1; }  // of a 16-bit attention segment, as measured
+// fills them. A unit that lies in one share is finished there; the parts of the others go to the workspace as (sum of p v,
+// maximum, sum of p) and k_attn_join adds them up.
 constexpr int kTile = 128;  // of a 16-bit cache; 64 of a 32-bit one (as many bytes)
+// What a 16-bit attention segment costs beside its tiles, in tiles: filling and draining its pipeline and, for 256 rows,
+// writing 128 KB of sums takes about 9 us where a tile takes 2.3 (24 sequences of 501 to 8,192 slots: 105 us without, 79
+// with the queries brought ahead as well; 131,000 slots x 256 rows: 161 us with 1, 155 with 4).
+__host__ __device__ constexpr int start_of(int rblock) { return rblock > 128 ? 4 : 1; }
 struct Cut {                // how a kernel cuts its work
     int rblock, tile;       // query rows of a unit, slots of a tile
     int least;              // tiles of a share, at least
@@ -302,19 +305,21 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
 
 // The tree attention kernel. Twelve warps: two groups of four for the softmax (thread = query row = TMEM lane), one that
 // brings tiles of K and V into a ring by TMA, one that brings queries, and one for each of two streams that issues its
-// MMAs. A stream is a
-// softmax group with its scores and its accumulator in TMEM; a step is 64 slots:
+// MMAs. A stream is a softmax group with its scores and its accumulator in TMEM; a step is 64 slots:
 //   TWO = false (at most 128 query rows): both streams have the same rows, stream s takes the slots 64 s .. of every
 //                tile; the accumulators are joined at the segment's end.
 //   TWO = true: stream s has rows 128 s .. of a block of 256 and takes every tile's halves one after the other (K and V
 //               come once for 256 rows).
 // Step k of a stream: S = Q K^T (128 x 64, into one of the stream's two score buffers) -> softmax group: mask, running
 // maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). With two buffers the next
-// scores are computed while this step's are exponentiated, and the softmax groups never wait for the tensor cores in the
-// steady state (steps of 128 slots with one buffer a stream, whose chain scores - softmax - products was serial, took
-// 204 us where this takes TIME_LONG, 131,064 slots x 8 heads x 256 rows of bf16).
-// Bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.8 k cycles; TWO: the MMAs
-// 2.6 k (N = 64 reads Q more often than the tensor cores would like) and the exponentials (256 x 128 at 16 a cycle) 2 k.
+// scores are computed while this step's are exponentiated.
+// TWO = false is bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.8 k cycles, a
+// stream's step 2 k (24 sequences x 7 tokens x 32 heads, fp16: 82 us, 5.2 TB/s). TWO = true is bound by the tensor cores
+// and the shared memory that feeds them: a 128 x 64 x 16 product takes 60 cycles there, not 32, for its 4 KB of Q, so a
+// tile takes 2.9 k at best and 3.9 k in fact (131,000 slots x 8 heads x 256 rows, bf16: 153 us, 0.9 PFLOP/s). Measured
+// there and not kept: 128-slot steps with one buffer a stream (twice the columns a product, but scores, softmax and
+// products one after the other) 184 us; weights by the old maximum while the new one is found 159 us; with no
+// exponentials at all it would still be 147 us.
 template <int D, bool TWO>
 struct TcShape {
     static constexpr int kStage = kTile * D * 2;
@@ -730,7 +735,8 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
 
 // The mass kernel: S^T = K Q^T, a tile's 128 slots as the TMEM lanes and the query rows as its columns, so that a thread
 // holds one slot and sums it over rows. Tiles go to two score buffers in turn, each with two groups of four warps that
-// take half of the rows each (four warps a scheduler hide the exponentials' latency: MASS_NOTE). Keys come through a TMA
+// take half of the rows each (four warps a scheduler hide the exponentials'
+// latency: 66 us, with two of them 84, for 64 tokens x 32 heads over 2 x 32 k slots). Keys come through a TMA
 // ring, the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows
 // (32 KB a tile: 1.4 k cycles at 1/148 of the bandwidth), by the exponentials (8 cycles a row and tile) beyond.
 template <int D, int ROWS>
@@ -923,9 +929,10 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 // x = hi + lo, both TF32 (8 + 11 bits; hi rounded, so that lo has either sign): x y = hi hi' + hi lo' + lo hi' up to
 // 2^-21 |x y|, three mma.sync products with fp32 sums. The tensor cores cut what they add off, they do not round it: so
 // products with a small piece have sums of their own, a tile's products of weights and values are added to the
-// accumulator by fp32 additions, and scores have two sums (all in one, and hi cut off: 2.8e-6 off 64 bits instead of 0.6e-6, where
-// a plain fp32 product is 1.2e-6 off; it costs 27.7 us instead of 24.9 at 12 tokens x 32 heads over 2,047 slots). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back:
-// more shared-memory traffic than the products take. From registers the split costs three integer or fp32 operations.)
+// accumulator by fp32 additions, and scores have two sums (all in one, and hi cut off: 2.8e-6 off 64 bits instead of
+// 0.6e-6, where a plain fp32 product is 1.2e-6 off; it costs 27.7 us instead of 24.9 at 12 tokens x 32 heads over 2,047
+// slots). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back: more
+// shared-memory traffic than the products take. From registers the split costs four integer or fp32 operations.)
 // A product waits for the one before it on the same sum (four of them take that long to issue), so the order is by piece,
 // through as many sums as there are.
 struct Split {
@@ -1286,7 +1293,8 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
 
 // The masses of a 32-bit cache. Four groups of four warps take the tiles in turn; a warp has 16 of the 64 slots and goes
 // through the query rows 16 at a time. A lane's four slots are summed over its rows, and over the eight lanes that share
-// them at the end. (Eight warps with eight slots of every tile each: OLD_MASS.)
+// them at the end. 12 tokens x 32 heads over 65,536 slots take 141 us, one token 57 us, 4.7 TB/s (eight warps with eight
+// slots of every tile each: 200 and 110 us). Bound by K from HBM for up to 16 rows, by the products beyond.
 template <int D>
 struct F32Mass {
     static constexpr int kRows = 128, kGroups = 4, kThreads = 4 * kGroups * 32 + 32;
