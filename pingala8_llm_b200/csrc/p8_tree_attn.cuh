@@ -662,11 +662,13 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
     if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// Adds up a unit's parts, one warp per query row, in the parts' order.
-template <typename T, int D>
+// Adds up a unit's parts in their order, one warp per query row, AHEAD parts a round of loads. Bound by its rounds where
+// rows are few, by how many blocks fit an SM where they are many (fewer loads ahead, fewer registers).
+template <typename T, int D, int AHEAD>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
     // Everything up to the wait comes from the call's inputs, while the attention kernel runs; the parts are its outputs.
     // Every warp waits, with or without something to add: what follows in the stream waits for this launch alone.
+    constexpr int W = D / 32;
     const int lane = threadIdx.x % 32;
     const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     const bool is = id < (long long)a.batch * a.tokens * a.heads;
@@ -693,9 +695,8 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;  // finished by that CTA, or not there
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
-    constexpr int W = D / 32, AHEAD = 16;
     float m = -INFINITY, l = 0.f, acc[W] = {};
-    for (int c = c0; c <= c1; c += AHEAD) {  // all loads of 16 parts at once; lane i has the statistics of part c + i
+    for (int c = c0; c <= c1; c += AHEAD) {  // all loads of AHEAD parts at once; lane i has the statistics of part c + i
         const int cnt = min(AHEAD, c1 - c + 1);
         const float2 ml = lane < cnt ? part_ml[at(c + lane)] : make_float2(-INFINITY, 0.f);
         float v[AHEAD][W];
@@ -727,9 +728,9 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T *out = static_cast<T *>(a.out) + b * a.os[0] + t * a.os[1] + (long long)head * a.os[2] + lane * (D / 32);
+    T *out = static_cast<T *>(a.out) + b * a.os[0] + t * a.os[1] + (long long)head * a.os[2] + lane * W;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) out[k] = from_f<T>(acc[k] * inv);
+    for (int k = 0; k < W; ++k) out[k] = from_f<T>(acc[k] * inv);
     if (a.lse && lane == 0) a.lse[((long long)b * a.tokens + t) * a.heads + head] = l == 0.f ? -INFINITY : (m - lift + log2f(l)) * 0.6931471805599453f;
 }
 
@@ -1515,6 +1516,9 @@ size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {  // 
     return (size_t)2 * attn_ctas(c, rows, cut) * cut.rblock * ((size_t)c->width * 4 + 8);
 }
 
+// Rows up to which k_attn_join loads 16 parts at once, not 8: 2,048 rows of 131,000 slots take 154 us with 16 and 161 with
+// 8 (the whole call), 5,376 rows of 24 sequences 82 with 16 and 79 with 8.
+constexpr long long kFewRows = 2048;
 template <typename T, int D, typename K>
 p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     CUtensorMap mk, mv;
@@ -1526,8 +1530,11 @@ p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, 
     float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * cut.rblock * D);
     kernel<<<ctas, threads, smem, st>>>(a, mk, mv, po, ml);
     if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
-    const dim3 grid((unsigned int)(((long long)a.batch * a.tokens * a.heads + 7) / 8));
-    return launch_after(k_attn_join<T, D>, grid, dim3(256), st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+    const long long rows = (long long)a.batch * a.tokens * a.heads;
+    const bool few = rows <= kFewRows;
+    const dim3 grid((unsigned int)((rows + 7) / 8));
+    const auto join = few ? k_attn_join<T, D, 16> : k_attn_join<T, D, 8>;
+    return launch_after(join, grid, dim3(256), st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 template <typename T, int D>
 p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
