@@ -298,8 +298,8 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
 
 /* What a decoder runs between its projections, on a cache of keys and values that holds `batch` sequences in `slots`
  * slots each: write new tokens behind a sequence, let a tree of drafted tokens attend, take the accepted ones into the
- * sequence, add up how much attention each slot drew, and keep the slots that drew most. (ggml builds the first two
- * from RMS_NORM, MUL, ROPE, SET_ROWS and FLASH_ATTN_EXT nodes; it has no op for the others.)
+ * sequence, add up how much attention each slot drew, and keep the slots that drew most. (A llama.cpp graph
+ * has several nodes for each of the first two, and none for the others.)
  *
  * Sequence b is as long as the device array lens[b] says, and every call reads the lengths on the device, so that a
  * captured graph stays valid while sequences grow. A call adds n_b tokens to sequence b: n_b = counts[b] where `counts`
