@@ -315,6 +315,7 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
 typedef enum p8_kv_type { P8_KV_F32 = 0, P8_KV_F16 = 1, P8_KV_BF16 = 2 } p8_kv_type;
 #define P8_TREE_MAX 64   /* tokens of one sequence in a tree attention, mass or accept call */
 #define P8_BATCH_MAX 4096
+#define P8_SLOTS_MAX (1 << 30)
 typedef struct p8_kv {
     void *k, *v;
     int64_t type;                      /* p8_kv_type of k and v */
@@ -349,8 +350,9 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
  * mask[b * mask_stride + t] is set (mask NULL: j <= t, a chain). out = softmax(scale q k^T) v over what it sees, in q's
  * type (the cache's); lse [batch][tokens][heads] f32 (or NULL) the natural log of the sum of exponentials. A token that
  * sees nothing gets 0 and -infinity. What a token does not see does not reach it, whatever its bits (infinities and NaN
- * included). Products and sums in fp32 (16-bit types: the weights are rounded to the type before they multiply v; f32:
- * products of two TF32 pieces each, 2^-21). out must not overlap q, k or v. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
+ * included; f32: an infinity that it does see, before the call's tokens, comes out as NaN). Products and sums in fp32
+ * (16-bit types: the weights are rounded to the type before they multiply v; f32: products of two TF32 pieces each,
+ * 2^-21). out must not overlap q, k or v. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
 typedef struct p8_tree_attn_args {
     const void *q;
     int64_t q_stride[3];                  /* sequence, token, head */

@@ -497,7 +497,7 @@ bool kv_ok(const p8_kv *c, bool values = true) {
     if (!c || !c->k || (values && !c->v) || !al16(c->k) || !al16(c->v)) return false;
     if (c->type != P8_KV_F32 && c->type != P8_KV_F16 && c->type != P8_KV_BF16) return false;
     if (c->width != 64 && c->width != 128) return false;
-    if (c->layers < 1 || c->batch < 1 || c->batch > P8_BATCH_MAX || c->heads < 1 || c->slots < 1 || c->slots > INT32_MAX - 4096) return false;
+    if (c->layers < 1 || c->batch < 1 || c->batch > P8_BATCH_MAX || c->heads < 1 || c->slots < 1 || c->slots > P8_SLOTS_MAX) return false;
     if (c->heads > 65535 || c->layers > 65535 || c->layers * c->batch * c->heads > (int64_t(1) << 30)) return false;
     const int64_t dims[4] = {c->layers, c->batch, c->heads, c->slots};
     const int es = elem_size(c->type);

@@ -121,6 +121,8 @@ SHAPES = [
     (1, 64, 24, 3, 64, [64], "shared"),
     (2, 64, 5, 1, 128, [3, 2000], "tree"),
     (5, 3, 4, 4, 128, [0, 1, 127, 129, 700], "shared"),
+    (1, 64, 20, 1, 64, [500], "tree"),  # 1280 query rows of one cache head
+    (70, 2, 4, 2, 64, [(37 * b) % 333 for b in range(70)], "chain"),  # more sequences than a warp has lanes
 ]
 
 
@@ -286,7 +288,8 @@ def test_offsets_beyond_32_bits():
 @pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("B,T,H,hk,D,lens,path", [
     (1, 1, 1, 1, 64, [0], False), (1, 1, 14, 2, 64, [1000], False), (2, 6, 32, 8, 128, [127, 129], True), (1, 64, 8, 2, 128, [900], False),
-    (3, 33, 9, 3, 64, [0, 300, 128], True), (1, 64, 40, 5, 128, [77], True), (2, 64, 5, 1, 64, [4000, 5], False)])
+    (3, 33, 9, 3, 64, [0, 300, 128], True), (1, 64, 40, 5, 128, [77], True), (2, 64, 5, 1, 64, [4000, 5], False),
+    (1, 64, 20, 1, 64, [500], True), (70, 2, 4, 2, 64, [(37 * b) % 333 for b in range(70)], False)])
 def test_attention_mass(dt, B, T, H, hk, D, lens, path):
     g, dtype = gen(T * 7 + B), TYPES[dt]
     cap, G, scale = max(lens) + T + 9, H // hk, D ** -0.5
