@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
+        after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 9) {
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         s_gave_up = 0;
         fence_mbar_init();
     }
+    after_prior();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -692,7 +694,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
         c0 = (u0 + cut.start) / each;
         c1 = (u0 + cut.start + nt - 1) / each;
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_prior();
     if (c0 == c1) return;  // finished by that CTA, or not there
     auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && c0 * each < u0 ? 1 : 0)) * cut.rblock + row % cut.rblock; };
     float m = -INFINITY, l = 0.f, acc[W] = {};
@@ -763,6 +765,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
+        after_prior();
         const Share s = find_share(a, Cut{1 << 30, kTile, 1, 0}, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 17) {
@@ -782,6 +785,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
         s_gave_up = 0;
         fence_mbar_init();
     }
+    after_prior();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1040,6 +1044,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
+        after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (tid == ALL) {
@@ -1053,6 +1058,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
         s_bad = 0;
         fence_mbar_init();
     }
+    after_prior();
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Walk w(a, cut, s_share);
@@ -1317,6 +1323,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
+        after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (tid == ALL) {
@@ -1328,6 +1335,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
         s_gave_up = 0;
         fence_mbar_init();
     }
+    after_prior();
     __syncthreads();
     Walk w(a, cut, s_share);
     if (tid >= ALL) {
@@ -1528,13 +1536,12 @@ p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, 
     const int ctas = attn_ctas(c, (int64_t)a.tokens * a.group, cut);
     float *po = static_cast<float *>(ws);
     float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * cut.rblock * D);
-    kernel<<<ctas, threads, smem, st>>>(a, mk, mv, po, ml);
-    if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
+    if (launch_after(kernel, dim3(ctas), dim3(threads), (size_t)smem, st, a, mk, mv, po, ml) != cudaSuccess) return P8_ERR_CUDA;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
     const bool few = rows <= kFewRows;
     const dim3 grid((unsigned int)((rows + 7) / 8));
     const auto join = few ? k_attn_join<T, D, 16> : k_attn_join<T, D, 8>;
-    return launch_after(join, grid, dim3(256), st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
+    return launch_after(join, grid, dim3(256), 0, st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 template <typename T, int D>
 p8_status run_tc(const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
@@ -1560,8 +1567,7 @@ p8_status mass_launches(AttnArgs a, int most, F launch) {
             a.mass = a.mass_out;
             for (int i = 0; i < 2; ++i) a.ms[i] = a.mos[i];
         }
-        launch(a);
-        if (cudaGetLastError() != cudaSuccess) return P8_ERR_CUDA;
+        if (launch(a) != cudaSuccess) return P8_ERR_CUDA;
     }
     return P8_OK;
 }
@@ -1572,8 +1578,9 @@ p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1, 0});
     return mass_launches(a, 512, [&](const AttnArgs &x) {
-        if (x.tokens * x.gc <= 256) k_attn_mass_tc<T, D, 256><<<ctas, 576, MassShape<D, 256>::kSmem, st>>>(x, mk);
-        else k_attn_mass_tc<T, D, 512><<<ctas, 576, MassShape<D, 512>::kSmem, st>>>(x, mk);
+        const bool one = x.tokens * x.gc <= 256;
+        return launch_after(one ? k_attn_mass_tc<T, D, 256> : k_attn_mass_tc<T, D, 512>, dim3(ctas), dim3(576),
+                            (size_t)(one ? MassShape<D, 256>::kSmem : MassShape<D, 512>::kSmem), st, x, mk);
     });
 }
 template <int D>
@@ -1582,7 +1589,7 @@ p8_status run_mass_f32(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     if (!encode_tiled()) return P8_ERR_CUDA;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
     const int ctas = attn_ctas(c, 1, Cut{1, kTile32, 1, 0});
-    return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { k_attn_mass_f32<D><<<ctas, F32Mass<D>::kThreads, F32Mass<D>::kSmem, st>>>(x, mk); });
+    return mass_launches(a, F32Mass<D>::kRows, [&](const AttnArgs &x) { return launch_after(k_attn_mass_f32<D>, dim3(ctas), dim3(F32Mass<D>::kThreads), (size_t)F32Mass<D>::kSmem, st, x, mk); });
 }
 template <int D>
 p8_status run_width(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cudaStream_t st) {
