@@ -314,7 +314,7 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
 // maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). With two buffers the next
 // scores are computed while this step's are exponentiated.
 // TWO = false is bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.8 k cycles, a
-// stream's step 2 k (24 sequences x 7 tokens x 32 heads, fp16: 82 us, 5.2 TB/s). TWO = true is bound by the tensor cores
+// stream's step 2 k (24 sequences x 7 tokens x 32 heads, fp16: 78 us, 5.5 TB/s). TWO = true is bound by the tensor cores
 // and the shared memory that feeds them: a 128 x 64 x 16 product takes 60 cycles there, not 32, for its 4 KB of Q, so a
 // tile takes 2.9 k at best and 3.9 k in fact (131,000 slots x 8 heads x 256 rows, bf16: 153 us, 0.9 PFLOP/s). Measured
 // there and not kept: 128-slot steps with one buffer a stream (twice the columns a product, but scores, softmax and
@@ -762,6 +762,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     __shared__ Share s_share;
     __shared__ alignas(16) float s_nl[ROWS];
     __shared__ float s_sum[2][2][128];
+    __shared__ int s_skips;  // 1 + the last segment with a row that counts for nothing
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
     if (warp == 0) {
@@ -783,6 +784,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
         mbar_init(&b_q, 512);
         mbar_init(&b_seg, 512);
         s_gave_up = 0;
+        s_skips = 0;
         fence_mbar_init();
     }
     after_prior();
@@ -859,11 +861,15 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
                     }
                 }
                 *reinterpret_cast<uint4 *>(sq + (ch / 8) * kAtom + row * 128 + (((ch % 8) ^ (row % 8)) * 16)) = v;
-                if (ch == 0) s_nl[row] = nl;
+                if (ch == 0) {
+                    s_nl[row] = nl;
+                    if (nl == -INFINITY && row < rows) s_skips = seg + 1;
+                }
             }
             fence_proxy_async();
             mbar_arrive(&b_q);
             wait(&b_q, seg & 1);  // s_nl is there
+            const bool skips = s_skips == seg + 1;  // (then no infinity of the keys may reach the sums through its zeros)
             const float *min_ = a.mass + w.b * a.ms[0] + h * a.ms[1];
             float *mout = a.mass_out + w.b * a.mos[0] + h * a.mos[1];
             for (int t = w.ta + s; t < w.tb; t += 2) {
@@ -886,12 +892,12 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
                         tmem_ld32(tS + j, x);
                         tmem_wait_ld(x);
                         const float4 *nl = reinterpret_cast<const float4 *>(s_nl + r0 + j);
-                        if (tail || j + 32 > cnt) {
+                        if (tail || skips || j + 32 > cnt) {
                             const int lo = from - r0 - j, hi = cnt - j;
 #pragma unroll
                             for (int k = 0; k < 32; ++k) {
-                                const float p = ex2(fmaf(__uint_as_float(x[k]), c, k < hi ? s_nl[r0 + j + k] : 0.f));
-                                sum[k & 3] += k >= lo && k < hi ? p : 0.f;
+                                const float n1 = k < hi ? s_nl[r0 + j + k] : -INFINITY, p = ex2(fmaf(__uint_as_float(x[k]), c, n1));
+                                sum[k & 3] += k >= lo && n1 != -INFINITY ? p : 0.f;
                             }
                         } else {
 #pragma unroll
@@ -935,7 +941,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 // 2^-21 |x y|, three mma.sync products with fp32 sums. The tensor cores cut what they add off, they do not round it: so
 // products with a small piece have sums of their own, a tile's products of weights and values are added to the
 // accumulator by fp32 additions, and scores have two sums (all in one, and hi cut off: 2.8e-6 off 64 bits instead of
-// 0.6e-6, where a plain fp32 product is 1.2e-6 off; it costs 27.7 us instead of 24.9 at 12 tokens x 32 heads over 2,047
+// 0.6e-6, where a plain fp32 product is 1.2e-6 off; it costs 27.2 us instead of 24.7 at 12 tokens x 32 heads over 2,047
 // slots). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back: more
 // shared-memory traffic than the products take. From registers the split costs four integer or fp32 operations.)
 // A product waits for the one before it on the same sum (four of them take that long to issue), so the order is by piece,
@@ -1011,7 +1017,7 @@ __device__ __forceinline__ float4 *query32(char *sq, int row, int col4) {
 // group agrees on the running maximum, the weights go through shared memory, and warp w adds up the columns 32 w .. (of 64
 // columns: of half of the slots) of all weights and values. So every group keeps all four schedulers busy whatever the
 // number of row tiles, and a warp holds 16 accumulators a thread, not 64 (eight warps with all columns of their own slots
-// took 28 us where this takes F32_NOTE, 12 tokens x 32 heads over 2,047 slots). RT row tiles share every tile of K and V;
+// took 28.1 us where this took 24.7, 12 tokens x 32 heads over 2,047 slots). RT row tiles share every tile of K and V;
 // with fewer than four, two such sets of groups take the tiles in turn (NS) and are joined at the segment's end.
 // Within the products the columns of K (and the slots in S and P) are taken in the order in which a lane finds them in 16
 // consecutive bytes: the sums do not depend on it.
@@ -1418,7 +1424,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const float p = ex2((s2[0][j][e] + s2[1][j][e]) + (s2[2][j][e] + nl));
-                            if (row >= from[j][e & 1] && row < rows) sum[j][e & 1] += p;
+                            if (row >= from[j][e & 1] && nl != -INFINITY) sum[j][e & 1] += p;  // (nor of rows behind the last)
                         }
                     }
                 }

@@ -338,6 +338,35 @@ def test_mass_of_an_attention_call_adds_up_to_its_rows():
     assert float((mass.sum(-1) - T * H / hk).abs().max()) < T * H / hk * ((D + 16) * E * 288 + 720 * E)
 
 
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dt", list(TYPES))
+def test_mass_rows_that_count_for_nothing(dt, D, T):
+    """lse = -infinity: not even where the keys are not finite (0 times infinity is no weight)"""
+    g = gen(T + D)
+    n, k, q = 200, randn(g, 1, 2, 320, D, dtype=TYPES[dt]), randn(g, 1, T, 8, D, dtype=TYPES[dt])
+    mass, lse = torch.rand(1, 2, 320, device="cuda", generator=g), torch.full((1, T, 8), -INF, device="cuda")
+    k[0, :, 5], k[0, :, 131, 3], k[0, :, n + T - 1, D - 1] = INF, NAN, -INF
+    q[0, -1, 2, 7] = NAN
+    want = mass.clone()
+    want[0, :, n : n + T] = 0
+    assert torch.equal(cache.attention_mass(q, lse, k, ints(n), mass, out=mass.clone()), want)
+    # one head's last token counts: its score for slot 5 is -infinity, the others' as if it were alone
+    if dt != "fp32":
+        k[0, :, 5], k[0, :, 131, 3], k[0, :, n + T - 1, D - 1], k[0, :, 5, 0] = 0.5, 0.5, 0.5, INF
+        q[0, -1, 6, 0] = -1.0
+        lse[0, -1, 6] = 6.0
+        got = cache.attention_mass(q, lse, k, ints(n), mass, out=mass.clone())
+        alone = torch.full_like(lse, 6.0)
+        want[0, 1, : n + T] = cache.attention_mass(q[:, -1:, 6:7], alone[:, -1:, 6:7].contiguous(), k[:, 1:], ints(n + T - 1), mass[:, 1:], out=mass[:, 1:].clone())[0, 0, : n + T]
+        want[0, 1, n : n + T - 1] -= mass[0, 1, n : n + T - 1]
+        # the two calls' scores may differ in the order of their sums; a rounding of a mass below 2 is at most E / 2
+        ds = 2 * (D + 16) * E * float((k[0, 1].float().nan_to_num(posinf=0.0).abs() @ q[0, -1, 6].float().abs()).max()) / math.sqrt(D)
+        most = float((want - mass)[0, 1].max().clamp_min(float(want[0, 1, n : n + T].max())))
+        assert float((got - want).abs().max()) <= ds * most + 2 * E and bool(got[0, 1, 5] == mass[0, 1, 5])
+    ended()
+
+
 def test_mass_rows_out_of_range():
     g = gen(13)
     k, q = randn(g, 1, 1, 40, 64), randn(g, 1, 3, 2, 64)
