@@ -78,7 +78,7 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
 // append: y = rotate(norm(x)) per head of a token. A group of D / 8 lanes holds one head's row, lane l the values
 // 4l..4l+3 of both halves, so a rotation pair is in one lane, the sum of squares is a butterfly over the group, and
 // every access is 8 or 16 bytes wide. Bound by memory on a prompt (4,099 tokens x 48 heads of 128, 153 MB: 31 us, 4.9
-// TB/s; 34.5 with the rows asked for only after the lengths and positions), by its one launch on a token (2.2 us).
+// TB/s; 34.5 with the rows asked for only after the lengths and positions), by its one launch on a token (1.8 us).
 struct AppendArgs {
     const float *x[3];          // q, k, v
     long long xs[3][3];
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(1024, 2) k_evict_select(const EvictArgs a) {
 }
 
 // step 2, into other buffers: every row moves on its own, 16 bytes a thread. Bound by HBM (288 rows x 2,048 kept of 16,384
-// slots, 604 MB: 105 us of the call's 135, 5.7 TB/s).
+// slots, 604 MB: 105 to 110 us of the call's 135, 5.6 TB/s).
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
     const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     after_prior();  // every block: what follows in the stream waits for this launch alone
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
 // acceptance: one block per (layer, sequence, keys or values). Each finds the path on its own (the first warp, two
 // nodes a lane, one ballot per step: cheaper than a launch between the walk and the moves), then moves the rows of all
 // heads in chunks, reading a chunk before writing it: path[i] >= i and the chunks go up, so no source is lost. Bound by two
-// rounds of latency and the launch: 2.6 us for 36 layers and 8 drafted tokens, 7.1 us for 32 layers x 16 sequences.
+// rounds of latency and the launch: 2.3 us for 36 layers and 8 drafted tokens, 6.6 us for 32 layers x 16 sequences.
 struct AcceptArgs {
     const long long *tokens, *target;
     const int *parents, *lens, *counts;
