@@ -737,26 +737,34 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
 }
 
 // The mass kernel: S^T = K Q^T, a tile's 128 slots as the TMEM lanes and the query rows as its columns, so that a thread
-// holds one slot and sums it over rows. Tiles go to two score buffers in turn, each with two groups of four warps that
-// take half of the rows each (four warps a scheduler hide the exponentials'
-// latency: 66 us, with two of them 84, for 64 tokens x 32 heads over 2 x 32 k slots). Keys come through a TMA
-// ring, the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows
-// (32 KB a tile: 1.4 k cycles at 1/148 of the bandwidth), by the exponentials (8 cycles a row and tile) beyond.
+// holds one slot and sums it over rows. Four score buffers of 128 columns, each with four warps of its own: with more than
+// 32 rows two of them take the halves of a tile's rows, so that two tiles are under way, with fewer rows four tiles are. A
+// buffer is given back once its last columns are in registers, before their exponentials. Keys come through a TMA ring,
+// the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows (32 KB a tile: 1.4 k
+// cycles at 1/148 of the bandwidth; 7 tokens x 32 heads over 24 x 8 k slots: 68 us, 6.1 TB/s), by the exponentials (8 cycles
+// a row and tile) beyond: 64 tokens x 32 heads over 2 x 32 k slots 50 us, of which the exponentials are 29. That case took
+// 84 us with one group a buffer, 66 with two that shared one and with the query rows loaded one piece after the other, 55
+// without what mass_cut counts. With few rows it costs up to 4 us in 28 to have more than four stages.
 template <int D, int ROWS>
 struct MassShape {
     static constexpr int kStage = kTile * D * 2;
     static constexpr int kQ = ROWS * D * 2;
-    static constexpr int kStages = D == 64 ? 6 : ROWS == 256 ? 4 : 2;
+    static constexpr int kStages = D == 64 ? 6 : ROWS == 512 ? 2 : 4;
     static constexpr int kSmem = kQ + kStages * kStage;
 };
+
+// With many rows it takes as long as four tiles to load them behind the first tiles of K and to fill and drain the buffers.
+__host__ __device__ constexpr Cut mass_cut(int rows) { return {1 << 30, kTile, 1, rows > 128 ? 4 : 0}; }
 
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const __grid_constant__ CUtensorMap mk) {
     using S_ = MassShape<D, ROWS>;
     constexpr int NST = S_::kStages, kBoxes = D / 64, C = D / 8, kAtom = ROWS * 128;
+    constexpr bool SPLIT = ROWS > 32;          // halves of the rows, or every group has tiles of its own
+    constexpr int kTurns = SPLIT ? 2 : 4;
     extern __shared__ __align__(1024) char dyn[];
     char *sq = dyn, *ring = sq + S_::kQ;
-    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[2], b_free[2], b_q, b_seg;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[4], b_free[4], b_q, b_seg;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
@@ -765,9 +773,10 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     __shared__ int s_skips;  // 1 + the last segment with a row that counts for nothing
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const Waits wait{&s_gave_up};
+    const Cut cut = mass_cut(a.tokens * a.gc);
     if (warp == 0) {
         after_prior();
-        const Share s = find_share(a, Cut{1 << 30, kTile, 1, 0}, lane, blockIdx.x, gridDim.x);
+        const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
         if (lane == 0) s_share = s;
     } else if (warp == 17) {
         tmem_alloc(&s_tmem, 512);
@@ -777,9 +786,9 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(b_s + i, 1);
-            mbar_init(b_free + i, 256);
+            mbar_init(b_free + i, 128);
         }
         mbar_init(&b_q, 512);
         mbar_init(&b_seg, 512);
@@ -792,13 +801,14 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    Walk w(a, Cut{1 << 30, kTile, 1, 0}, s_share);
+    Walk w(a, cut, s_share);
 
     if (warp == 16) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
         while (w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST;
+                if (n == 2 && w.opens && w.n * a.gc > 64) wait(&b_q, 0);  // the first query rows before the rest of the ring: 0.7 us
                 wait(b_empty + st, (n / NST & 1) ^ 1);
                 if (lane == 0) {
                     mbar_expect_tx(b_full + st, S_::kStage);
@@ -810,69 +820,85 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
         }
         for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
     } else if (warp == 17) {  // ----------------------------------------------------------- MMAs
-        uint32_t n = 0, seg = 0, c_free[2] = {0, 0};
+        uint32_t n = 0, seg = 0, held = 0;  // (bit: the phase of b_free)
         while (w.next()) {
             const int rows = w.n * a.gc;
             wait(&b_q, seg & 1);
             tc_fence_after();
             for (int t = w.ta; t < w.tb; ++t, ++n) {
-                const int st = n % NST, s = (t - w.ta) & 1;
+                const int st = n % NST, s = (t - w.ta) % kTurns;
                 wait(b_full + st, n / NST & 1);
                 for (int r0 = 0; r0 < rows; r0 += 256) {
-                    wait(b_free + s, (c_free[s]++ & 1) ^ 1);
-                    tc_fence_after();
-                    const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage)), dq = desc_rows(smem_u32(sq) + r0 * 128);
-                    const uint32_t id = idesc_of<T>((min(rows - r0, 256) + 15) / 16 * 16, false), to = tmem + 256 * s;
-                    if (elect_one()) {
+                    const int all = min(rows - r0, 256), mid = min((all + 63) / 64 * 32, all);
+                    for (int half = 0; half < 2; ++half) {
+                        const int from = half ? mid : 0, cols = ((half ? all : mid) - from + 15) / 16 * 16, g = SPLIT ? 2 * s + half : s;
+                        if (!cols) break;
+                        wait(b_free + g, (held >> g & 1) ^ 1);
+                        held ^= 1u << g;
+                        tc_fence_after();
+                        const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage)), dq = desc_rows(smem_u32(sq) + (r0 + from) * 128);
+                        const uint32_t id = idesc_of<T>(cols, false), to = tmem + 128 * g;
+                        if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            mma_ss(to, dk + ((kk / 4) * 16384 + (kk % 4) * 32) / 16, dq + ((kk / 4) * kAtom + (kk % 4) * 32) / 16, id, kk != 0);
-                        if (r0 + 256 >= rows) umma_commit(b_empty + st);
-                        umma_commit(b_s + s);
+                            for (int kk = 0; kk < D / 16; ++kk)
+                                mma_ss(to, dk + ((kk / 4) * 16384 + (kk % 4) * 32) / 16, dq + ((kk / 4) * kAtom + (kk % 4) * 32) / 16, id, kk != 0);
+                            if (r0 + 256 >= rows && (half || mid == all)) umma_commit(b_empty + st);
+                            umma_commit(b_s + g);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             ++seg;
             w.advance();
         }
     } else {  // -------------------------------------------------------------------------- sums
-        const int s = warp / 4 & 1, half = warp / 8, r = tid & 127;
-        const uint32_t tS = tmem + 256 * s + ((uint32_t)(warp & 3) << 21);
+        const int s = warp / 4 % kTurns, half = SPLIT ? warp / 8 : 0, g = SPLIT ? 2 * s + half : s, r = tid & 127;
+        const uint32_t tS = tmem + 128 * g + ((uint32_t)(warp & 3) << 21);
         const float c = a.scale * 1.4426950408889634f;
         uint32_t seg = 0, c_s = 0, it = 0;
         while (w.next()) {
             const int rows = w.n * a.gc, h = w.u;
-            for (int i = tid; i < (rows + 15) / 16 * 16 * C; i += 512) {
-                const int ch = i % C, row = i / C;
-                uint4 v = make_uint4(0, 0, 0, 0);
+            // Query rows warp, warp + 16, ..: lane i finds where the i-th lies and its lse, then 16 bytes a lane, eight loads
+            // under way. (Rows that count for nothing are kept out of the sums; what their queries are does not matter.)
+            long long at = -1;
+            if (const int row = warp + 16 * lane; row < rows) {
+                const int k = row / a.gc, head = h * a.group + a.g0 + row - k * a.gc;
+                const int src = a.rows ? a.rows[(long long)w.b * a.tokens + k] : k;
                 float nl = -INFINITY;
-                if (row < rows) {
-                    const int k = row / a.gc, head = h * a.group + a.g0 + row - k * a.gc;
-                    const int src = a.rows ? a.rows[(long long)w.b * a.tokens + k] : k;
-                    if (src < 0 || src >= a.tokens) {
-                        if (ch == 0) atomicOr(&g_cache_error, kErrRange);
-                    } else {
-                        const float lse = a.lse_in[((long long)w.b * a.tokens + src) * a.heads + head];
-                        if (lse != -INFINITY) {
-                            nl = lse * -1.4426950408889634f;
-                            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + w.b * a.qs[0] + src * a.qs[1] + (long long)head * a.qs[2] + ch * 8);
-                        }
-                    }
+                if (src < 0 || src >= a.tokens) {
+                    atomicOr(&g_cache_error, kErrRange);
+                } else {
+                    at = w.b * a.qs[0] + src * a.qs[1] + (long long)head * a.qs[2];
+                    const float lse = a.lse_in[((long long)w.b * a.tokens + src) * a.heads + head];
+                    if (lse != -INFINITY) nl = lse * -1.4426950408889634f;
                 }
-                *reinterpret_cast<uint4 *>(sq + (ch / 8) * kAtom + row * 128 + (((ch % 8) ^ (row % 8)) * 16)) = v;
-                if (ch == 0) {
-                    s_nl[row] = nl;
-                    if (nl == -INFINITY && row < rows) s_skips = seg + 1;
+                s_nl[row] = nl;
+                if (nl == -INFINITY) s_skips = seg + 1;
+            }
+            constexpr int kPer = 32 / C, kAhead = SPLIT ? 8 : 1;  // rows of a load, loads (32 rows: one)
+            const int ch = lane % C;
+            for (int i0 = 0; warp + 16 * i0 < rows; i0 += kPer * kAhead) {
+                uint4 v[kAhead];
+#pragma unroll
+                for (int x = 0; x < kAhead; ++x) {
+                    const int i = i0 + kPer * x + lane / C;
+                    const long long from = __shfl_sync(0xffffffffu, at, i & 31);
+                    v[x] = make_uint4(0, 0, 0, 0);
+                    if (warp + 16 * i < rows && from >= 0) v[x] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + from + ch * 8);
                 }
+#pragma unroll
+                for (int x = 0; x < kAhead; ++x)
+                    if (const int row = warp + 16 * (i0 + kPer * x + lane / C); row < rows)
+                        *reinterpret_cast<uint4 *>(sq + (ch / 8) * kAtom + row * 128 + ((ch ^ row) & 7) * 16) = v[x];
             }
             fence_proxy_async();
             mbar_arrive(&b_q);
             wait(&b_q, seg & 1);  // s_nl is there
-            const bool skips = s_skips == seg + 1;  // (then no infinity of the keys may reach the sums through its zeros)
+            const bool skips = s_skips == seg + 1;  // (then the sums leave them out)
             const float *min_ = a.mass + w.b * a.ms[0] + h * a.ms[1];
             float *mout = a.mass_out + w.b * a.mos[0] + h * a.mos[1];
-            for (int t = w.ta + s; t < w.tb; t += 2) {
+            for (int t = w.ta + s; t < w.tb; t += kTurns) {
                 const int key = t * kTile + r, late = key - w.len;
                 const bool tail = t * kTile + kTile > w.len;
                 float before = 0.f;
@@ -883,14 +909,19 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
                 const int from = late > 0 ? (late < w.n ? late * a.gc : rows) : 0;  // the first row that sees the slot
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int r0 = 0; r0 < rows; r0 += 256) {
-                    wait(b_s + s, c_s++ & 1);
+                    const int all = min(rows - r0, 256), mid = min((all + 63) / 64 * 32, all), cnt = half ? all : mid;
+                    if (half && mid == all) break;
+                    wait(b_s + g, c_s++ & 1);
                     tc_fence_after();
-                    const int all = min(rows - r0, 256), mid = (all + 63) / 64 * 32, cnt = half ? all : min(mid, all);
 #pragma unroll 1
                     for (int j = half ? mid : 0; j < cnt; j += 32) {
                         uint32_t x[32];
-                        tmem_ld32(tS + j, x);
+                        tmem_ld32(half ? tS + j - mid : tS + j, x);
                         tmem_wait_ld(x);
+                        if (j + 32 >= cnt) {  // all read: the next scores may come
+                            tc_fence_before();
+                            mbar_arrive(b_free + g);
+                        }
                         const float4 *nl = reinterpret_cast<const float4 *>(s_nl + r0 + j);
                         if (tail || skips || j + 32 > cnt) {
                             const int lo = from - r0 - j, hi = cnt - j;
@@ -910,11 +941,9 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
                             }
                         }
                     }
-                    tc_fence_before();
-                    mbar_arrive(b_free + s);
                 }
                 float sums = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (rows > 32) {  // the other half's; two places by turns, so that one barrier a tile is enough
+                if (SPLIT && rows > 32) {  // the other half's; two places by turns, so that one barrier a tile is enough
                     float *other = &s_sum[s][it++ & 1][r];
                     if (half) *other = sums;
                     asm volatile("bar.sync %0, 256;" ::"r"(1 + s) : "memory");
@@ -1483,6 +1512,7 @@ template <typename T, int D>
 void allow() {
     allow_attn<T, D, false>();
     allow_attn<T, D, true>();
+    cudaFuncSetAttribute(k_attn_mass_tc<T, D, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 32>::kSmem);
     cudaFuncSetAttribute(k_attn_mass_tc<T, D, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 256>::kSmem);
     cudaFuncSetAttribute(k_attn_mass_tc<T, D, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassShape<D, 512>::kSmem);
 }
@@ -1582,11 +1612,12 @@ p8_status run_mass_tc(const p8_kv *c, const AttnArgs &a, cudaStream_t st) {
     CUtensorMap mk;
     if (!encode_tiled()) return P8_ERR_CUDA;
     if (!cache_map(&mk, c, c->k, c->k_stride)) return P8_ERR_UNSUPPORTED;
-    const int ctas = attn_ctas(c, 1, Cut{1, kTile, 1, 0});
+    const int ctas = attn_ctas(c, 1, mass_cut(std::min(512 / a.tokens, a.group) * a.tokens));
     return mass_launches(a, 512, [&](const AttnArgs &x) {
-        const bool one = x.tokens * x.gc <= 256;
-        return launch_after(one ? k_attn_mass_tc<T, D, 256> : k_attn_mass_tc<T, D, 512>, dim3(ctas), dim3(576),
-                            (size_t)(one ? MassShape<D, 256>::kSmem : MassShape<D, 512>::kSmem), st, x, mk);
+        const int rows = x.tokens * x.gc;
+        if (rows <= 32) return launch_after(k_attn_mass_tc<T, D, 32>, dim3(ctas), dim3(576), (size_t)MassShape<D, 32>::kSmem, st, x, mk);
+        return launch_after(rows <= 256 ? k_attn_mass_tc<T, D, 256> : k_attn_mass_tc<T, D, 512>, dim3(ctas), dim3(576),
+                            (size_t)(rows <= 256 ? MassShape<D, 256>::kSmem : MassShape<D, 512>::kSmem), st, x, mk);
     });
 }
 template <int D>
@@ -1614,7 +1645,7 @@ void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, in
 
 p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
     const int64_t rows = mass ? 1 : (int64_t)x.tokens * x.group;
-    if (attn_tiles(c, rows, attn_cut(c, rows)) > INT32_MAX / 2 || c->batch * x.tokens * x.heads > INT32_MAX) return P8_ERR_UNSUPPORTED;
+    if (attn_tiles(c, rows, mass && c->type != P8_KV_F32 ? mass_cut(512) : attn_cut(c, rows)) > INT32_MAX / 2 || c->batch * x.tokens * x.heads > INT32_MAX) return P8_ERR_UNSUPPORTED;
     return c->width == 128 ? run_width<128>(c, x, mass, ws, st) : run_width<64>(c, x, mass, ws, st);
 }
 
