@@ -325,6 +325,12 @@ def test_attention_mass(dt, B, T, H, hk, D, lens, path):
             close(out[b, h, :end], want, tol)
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("T,H", [(31, 1), (32, 1), (33, 1), (16, 4), (17, 4), (32, 4), (33, 4), (64, 4), (52, 5), (64, 8), (64, 9)])
+def test_attention_mass_around_the_row_counts_of_its_variants(dt, T, H):
+    test_attention_mass(dt, 2, T, H, 1, 128, [1030, 515], True)
+
+
 def test_mass_of_an_attention_call_adds_up_to_its_rows():
     """over all slots, the weights of a token's heads sum to one each"""
     g = gen(12)
