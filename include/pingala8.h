@@ -389,6 +389,13 @@ typedef struct p8_attn_mass_args {
 } p8_attn_mass_args;
 p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream);
 
+/* The tree attention and mass kernels are pipelines of warps that wait for one another. A wait that is not over after `ns`
+ * nanoseconds gives up: the call ends, once the copies and products that it has started are done, its results are invalid,
+ * and p8_device_error reports bit 7 (128). Two seconds unless set here, for the calls made (or captured) from then on by this
+ * process; at most 2^32 - 1. 0: every wait that is not over at its first look gives up, which is how a program's way of dealing with
+ * the error can be tried out. */
+p8_status p8_cache_wait_limit(int64_t ns);
+
 /* Shorten every sequence with more than `budget` slots to `budget`, per layer and head: the first `sinks` slots, the
  * last `recent` slots and, of those between, the ones with the largest mass (ties: the lowest slot; NaN counts as
  * -infinity), in their order. Keys, values and mass [layer][b][h] of the kept slots are written to the first slots of

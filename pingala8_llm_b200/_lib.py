@@ -105,6 +105,7 @@ _SIGS = {
     "p8_attn_mass": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
     "p8_kv_evict": (C.c_int, [C.c_char_p, C.c_char_p, C.c_char_p, _vp]),
     "p8_tree_accept": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
+    "p8_cache_wait_limit": (C.c_int, [_i64]),
     "p8_device_error": (C.c_int, []),
     "p8_status_str": (C.c_char_p, [C.c_int]),
     "p8_build_info": (C.c_char_p, []),

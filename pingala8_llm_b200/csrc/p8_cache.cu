@@ -541,6 +541,12 @@ using namespace p8;
 
 extern "C" {
 
+p8_status p8_cache_wait_limit(int64_t ns) {
+    if (ns < 0 || ns > UINT32_MAX) return P8_ERR_ARG;
+    g_wait_ns.store((unsigned int)ns, std::memory_order_relaxed);
+    return P8_OK;
+}
+
 p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream) {
     if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
     if (!a->q || !a->k || !a->v || !a->q_out || !a->lens || !a->pos || !a->cos || !a->sin || a->tokens < 0 || a->positions < 1) return P8_ERR_ARG;

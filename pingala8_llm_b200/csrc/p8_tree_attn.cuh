@@ -2,6 +2,8 @@
 // p8_cache.cu).
 #pragma once
 
+constexpr unsigned int kWaitNs = 2000000000u;  // what waits are bounded by, unless the host says otherwise
+
 struct AttnArgs {
     const void *q, *k, *v;
     long long qs[3], ks[3], vs[3], os[3];  // q, out: sequence, token, head; k, v: sequence, head, slot
@@ -16,6 +18,7 @@ struct AttnArgs {
     int batch, tokens, heads, kvh, group;
     int g0, gc, more;  // mass: the query heads g0 .. g0 + gc - 1 of each group; more: added to what `out` has
     float scale;
+    unsigned int wait_ns;  // bound of one wait
 };
 
 // A unit is (sequence, cache head, block of query rows); its slots are cut into tiles. All tiles of all units
@@ -131,23 +134,44 @@ __device__ __forceinline__ Share find_share(const AttnArgs &a, Cut cut, int lane
     return s;
 }
 
-// Waits give up after two seconds (the kernel's results are then invalid and bit 128 is set); from then on every wait
-// of the CTA returns at once, so that all roles run through to the end and meet there.
+// Waits give up after `ns` (the kernel's results are then invalid and bit 128 is set); from then on every wait of the CTA that
+// is not over at its first look returns false at once. What follows from that goes by the role. Warps that start something
+// asynchronous (TMA loads, cp.async, MMAs) start nothing more and leave their loops: a stage that was not handed over may
+// still be written or read, and its barrier may be inside a phase. Before they go to the CTA's end they wait for all that they
+// did start (settle, which does not ask whether something gave up). The others run through to the end and meet there.
 struct Waits {
     volatile int *gave_up;
-    __device__ void operator()(uint64_t *bar, uint32_t parity) const {
-        if (mbar_try_wait(bar, parity) || *gave_up) return;
-        unsigned long long t0, t;
-        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
-        for (uint32_t i = 1;; ++i) {
-            if (mbar_try_wait(bar, parity)) return;
-            if ((i & 63) == 0) {
-                asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-                if (*gave_up || t - t0 > 2000000000ull) break;
-            }
-        }
+    unsigned int ns;
+    // whether the barrier's phase is over
+    __device__ bool operator()(uint64_t *bar, uint32_t parity) const {
+        if (mbar_test_wait(bar, parity)) return true;
+        if (*gave_up) return false;
+        if (ns && poll(bar, parity, ns, gave_up)) return true;
         *gave_up = 1;
         atomicOr(&g_cache_error, kErrWait);
+        return false;
+    }
+    // For a whole warp that starts something behind it: true for all lanes or for none. `arrivals`: the phase ends by
+    // those of roles that go on arriving after something gave up.
+    __device__ bool warp(uint64_t *bar, uint32_t parity, bool arrivals = false) const {
+        bool ok = (*this)(bar, parity);
+        if (arrivals) ok = ok && !*gave_up;
+        return __all_sync(0xffffffffu, ok);
+    }
+    // for what this role has started and what ends by itself
+    __device__ void settle(uint64_t *bar, uint32_t parity) const {
+        if (mbar_try_wait(bar, parity) || poll(bar, parity, kWaitNs, nullptr)) return;
+        *gave_up = 1;
+        atomicOr(&g_cache_error, kErrWait);
+    }
+    static __device__ bool poll(uint64_t *bar, uint32_t parity, unsigned int ns, volatile int *stop) {
+        unsigned long long t0, t;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+        do {
+            if (mbar_try_wait(bar, parity)) return true;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        } while (t - t0 <= ns && !(stop && *stop));
+        return false;
     }
 };
 
@@ -341,14 +365,14 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
     constexpr Cut cut{S_::kRows, kTile, S_::kLeast, start_of(S_::kRows)};
     extern __shared__ __align__(1024) char dyn[];  // the swizzle goes by address bits
     char *sq = dyn, *ring = sq + S_::kQ;
-    __shared__ uint64_t b_full[NST], b_empty[NST], b_q[2], b_qfree[2], b_s[2][2], b_p[2][2], b_pv[2][2], b_seg, b_read, b_tail;  // [stream][score buffer]
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_q[2], b_qfree[2], b_s[2][2], b_p[2][2], b_pv[2][2], b_end[2], b_seg, b_read, b_tail;  // [stream][score buffer]
     __shared__ float2 s_ml[2][TWO ? 1 : 128];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
     __shared__ unsigned long long s_bad[3];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const Waits wait{&s_gave_up};
+    const Waits wait{&s_gave_up, a.wait_ns};
     if (warp == 0) {
         after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
@@ -370,6 +394,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         for (int i = 0; i < 2; ++i) {
             mbar_init(b_q + i, 32);
             mbar_init(b_qfree + i, 2);
+            mbar_init(b_end + i, 1);
         }
         mbar_init(&b_seg, 256);
         mbar_init(&b_read, 256);
@@ -388,11 +413,12 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
 
     if (warp == 8) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
-        while (w.next()) {
-            for (int t = w.ta; t < w.tb; ++t)
+        bool on = true;
+        while (on && w.next()) {
+            for (int t = w.ta; on && t < w.tb; ++t)
                 for (int z = 0; z < 2; ++z, ++n) {
                     const int st = n % NST;
-                    wait(b_empty + st, (n / NST & 1) ^ 1);
+                    if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1))) break;
                     if (lane == 0) {
                         mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -403,12 +429,12 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
             w.advance();
         }
         // nothing may be in flight into this CTA's shared memory when it ends
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
     } else if (warp == 11) {  // ---------------------------------------------------------- queries, a segment ahead where there is room
         uint32_t seg = 0;
         while (w.next()) {
             const int qb = seg % NQ;
-            wait(b_qfree + qb, (seg / NQ & 1) ^ 1);
+            if (!wait.warp(b_qfree + qb, (seg / NQ & 1) ^ 1)) break;
             load_q<T, D>(sq + qb * (128 * D * 2), a, w.b, w.head(), w.row0(), w.n * a.group, TWO ? 2 : 1, a.scale < 0.f ? 0x80008000u : 0u, lane);
             fence_proxy_async();
             mbar_arrive(b_q + qb);
@@ -419,14 +445,16 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         const int s = __shfl_sync(0xffffffffu, warp, 0) - 9;
         constexpr uint32_t id_s = idesc_of<T>(kStep, false), id_o = idesc_of<T>(D, true);
         uint32_t base = 0, seg = 0, step = 0;  // ring position and the stream's step count at the segment's start
-        while (w.next()) {
+        bool on = true;
+        while (on && w.next()) {
             const int ns = (w.tb - w.ta) * PER, qb = seg % NQ;
             const uint64_t dq = desc_rows(smem_u32(sq) + (TWO ? s : qb) * (128 * D * 2));
-            wait(b_q + qb, seg / NQ & 1);
+            on = wait.warp(b_q + qb, seg / NQ & 1);
             auto scores = [&](int k) {
                 const uint32_t at = base + 2 * (k / PER), st = at % NST, g = step + k, buf = g & 1;
-                if (g >= 2) wait(&b_pv[s][buf], ((g - 2) / 2) & 1);  // the P that the buffer held is read
-                wait(b_full + st, at / NST & 1);
+                bool ok = g < 2 || wait(&b_pv[s][buf], ((g - 2) / 2) & 1);  // the P that the buffer held is read
+                ok = wait(b_full + st, at / NST & 1) && ok;
+                if (!__all_sync(0xffffffffu, ok)) return false;
                 tc_fence_after();
                 const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128));
                 const uint32_t to = tmem + 128 * s + 64 * buf;
@@ -442,13 +470,14 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     umma_commit(&b_s[s][buf]);
                 }
                 __syncwarp();
+                return true;
             };
-            scores(0);
-            if (ns > 1) scores(1);
-            for (int k = 0; k < ns; ++k) {
+            on = on && scores(0) && (ns < 2 || scores(1));
+            for (int k = 0; on && k < ns; ++k) {
                 const uint32_t at = base + 2 * (k / PER) + 1, st = at % NST, buf = (step + k) & 1, use = (step + k) / 2 & 1;
-                wait(&b_p[s][buf], use);
-                wait(b_full + st, at / NST & 1);
+                on = wait(&b_p[s][buf], use);
+                on = wait(b_full + st, at / NST & 1) && on;
+                if (!(on = __all_sync(0xffffffffu, on))) break;
                 tc_fence_after();
                 const int half = TWO ? k & 1 : s;
                 const uint64_t dv = desc_cols(smem_u32(ring + st * S_::kStage) + half * (kStep * 128));
@@ -466,13 +495,17 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     umma_commit(&b_pv[s][buf]);
                 }
                 __syncwarp();
-                if (k + 2 < ns) scores(k + 2);
+                if (k + 2 < ns) on = scores(k + 2);
             }
             base += 2 * (w.tb - w.ta);
             step += ns;
             ++seg;
             w.advance();
         }
+        // nor may a product be on its way when TMEM is given back
+        if (elect_one()) umma_commit(b_end + s);
+        __syncwarp();
+        wait.settle(b_end + s, 0);
     } else {  // -------------------------------------------------------------------------- softmax
         const int s = warp / 4, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, tO = tmem + 256 + 128 * s + lanes;
@@ -764,7 +797,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     constexpr int kTurns = SPLIT ? 2 : 4;
     extern __shared__ __align__(1024) char dyn[];
     char *sq = dyn, *ring = sq + S_::kQ;
-    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[4], b_free[4], b_q, b_seg;
+    __shared__ uint64_t b_full[NST], b_empty[NST], b_s[4], b_free[4], b_q, b_seg, b_end;
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ Share s_share;
@@ -772,7 +805,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
     __shared__ float s_sum[2][2][128];
     __shared__ int s_skips;  // 1 + the last segment with a row that counts for nothing
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const Waits wait{&s_gave_up};
+    const Waits wait{&s_gave_up, a.wait_ns};
     const Cut cut = mass_cut(a.tokens * a.gc);
     if (warp == 0) {
         after_prior();
@@ -792,6 +825,7 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
         }
         mbar_init(&b_q, 512);
         mbar_init(&b_seg, 512);
+        mbar_init(&b_end, 1);
         s_gave_up = 0;
         s_skips = 0;
         fence_mbar_init();
@@ -805,11 +839,12 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 
     if (warp == 16) {  // ---------------------------------------------------------------- loads
         uint32_t n = 0;
-        while (w.next()) {
+        bool on = true;
+        while (on && w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST;
-                if (n == 2 && w.opens && w.n * a.gc > 64) wait(&b_q, 0);  // the first query rows before the rest of the ring: 0.7 us
-                wait(b_empty + st, (n / NST & 1) ^ 1);
+                if (n == 2 && w.opens && w.n * a.gc > 64) on = wait.warp(&b_q, 0);  // the first query rows before the rest of the ring: 0.7 us
+                if (!(on = on && wait.warp(b_empty + st, (n / NST & 1) ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -818,22 +853,23 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
             }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
     } else if (warp == 17) {  // ----------------------------------------------------------- MMAs
         uint32_t n = 0, seg = 0, held = 0;  // (bit: the phase of b_free)
-        while (w.next()) {
+        bool on = true;
+        while (on && w.next()) {
             const int rows = w.n * a.gc;
-            wait(&b_q, seg & 1);
+            on = wait.warp(&b_q, seg & 1);
             tc_fence_after();
-            for (int t = w.ta; t < w.tb; ++t, ++n) {
+            for (int t = w.ta; on && t < w.tb; ++t, ++n) {
                 const int st = n % NST, s = (t - w.ta) % kTurns;
-                wait(b_full + st, n / NST & 1);
-                for (int r0 = 0; r0 < rows; r0 += 256) {
+                on = wait.warp(b_full + st, n / NST & 1);
+                for (int r0 = 0; on && r0 < rows; r0 += 256) {
                     const int all = min(rows - r0, 256), mid = min((all + 63) / 64 * 32, all);
                     for (int half = 0; half < 2; ++half) {
                         const int from = half ? mid : 0, cols = ((half ? all : mid) - from + 15) / 16 * 16, g = SPLIT ? 2 * s + half : s;
                         if (!cols) break;
-                        wait(b_free + g, (held >> g & 1) ^ 1);
+                        if (!(on = wait.warp(b_free + g, (held >> g & 1) ^ 1))) break;
                         held ^= 1u << g;
                         tc_fence_after();
                         const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage)), dq = desc_rows(smem_u32(sq) + (r0 + from) * 128);
@@ -852,6 +888,9 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
             ++seg;
             w.advance();
         }
+        if (elect_one()) umma_commit(&b_end);  // nothing may be on its way when TMEM is given back
+        __syncwarp();
+        wait.settle(&b_end, 0);
     } else {  // -------------------------------------------------------------------------- sums
         const int s = warp / 4 % kTurns, half = SPLIT ? warp / 8 : 0, g = SPLIT ? 2 * s + half : s, r = tid & 127;
         const uint32_t tS = tmem + 128 * g + ((uint32_t)(warp & 3) << 21);
@@ -1077,7 +1116,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
     __shared__ float s_max[S_::kGroups][4][16], s_sum[S_::kGroups][4][16], s_m[S_::kGroups][16];
     __shared__ unsigned long long s_bad;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const Waits wait{&s_gave_up};
+    const Waits wait{&s_gave_up, a.wait_ns};
     if (warp == 0) {
         after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
@@ -1099,11 +1138,12 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
     Walk w(a, cut, s_share);
     if (tid >= ALL) {  // loads
         uint32_t n = 0;
-        while (w.next()) {
-            for (int t = w.ta; t < w.tb; ++t)
+        bool on = true;
+        while (on && w.next()) {
+            for (int t = w.ta; on && t < w.tb; ++t)
                 for (int z = 0; z < 2; ++z, ++n) {
                     const int st = n % NST;
-                    wait(b_empty + st, (n / NST & 1) ^ 1);
+                    if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1, true))) break;
                     if (lane == 0) {
                         mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -1113,7 +1153,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
                 }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
         return;
     }
     const int group = warp / 4, rt = group % RT, ns = group / RT, wq = warp % 4, g = lane / 4, t = lane % 4;
@@ -1356,7 +1396,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
     __shared__ Share s_share;
     __shared__ float s_nl[S_::kRows];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const Waits wait{&s_gave_up};
+    const Waits wait{&s_gave_up, a.wait_ns};
     if (warp == 0) {
         after_prior();
         const Share s = find_share(a, cut, lane, blockIdx.x, gridDim.x);
@@ -1375,10 +1415,11 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
     Walk w(a, cut, s_share);
     if (tid >= ALL) {
         uint32_t n = 0;
-        while (w.next()) {
+        bool on = true;
+        while (on && w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST;
-                wait(b_empty + st, (n / NST & 1) ^ 1);
+                if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1, true))) break;
                 if (lane == 0) {
                     mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -1387,7 +1428,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
             }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
         return;
     }
     auto sync_all = [&] { asm volatile("bar.sync 1, %0;" ::"n"(ALL) : "memory"); };
@@ -1635,12 +1676,14 @@ p8_status run_width(const p8_kv *c, const AttnArgs &a, bool mass, void *ws, cuda
     return mass ? run_mass_tc<__nv_bfloat16, D>(c, a, st) : run_tc<__nv_bfloat16, D>(c, a, ws, st);
 }
 
+std::atomic<unsigned int> g_wait_ns{kWaitNs};
 void base_args(AttnArgs &x, const p8_kv *c, const void *q, const int64_t *qs, int64_t tokens, int64_t heads) {
     memset(&x, 0, sizeof(x));
     x.q = q; x.k = c->k; x.v = c->v;
     for (int i = 0; i < 3; ++i) { x.qs[i] = qs[i]; x.ks[i] = c->k_stride[1 + i]; x.vs[i] = c->v_stride[1 + i]; }
     x.slots = c->slots; x.batch = (int)c->batch; x.tokens = (int)tokens; x.heads = (int)heads; x.kvh = (int)c->heads;
     x.group = (int)(heads / c->heads);
+    x.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
 }
 
 p8_status launch_attn(const p8_kv *c, const AttnArgs &x, bool mass, void *ws, cudaStream_t st) {
