@@ -454,7 +454,7 @@ p8_status p8_gguf_load_linear(p8_gguf *g, int64_t i, uint8_t *out, size_t out_ca
 /* Non-zero if a kernel since the last call gave up (that launch's results are invalid), then clears the word. Bits:
  * 4 GEMM pipeline wait timed out, 8 row-parallel exchange wait timed out, 16 exchange entry with a foreign tag, 64 a
  * cache operator met a length, count, position or row out of range and left it out, 128 a tree attention or mass
- * pipeline wait timed out (1, 2 and 32 are unused). Synchronises the device. */
+ * pipeline wait timed out (1, 2 and 32 are unused). Waits for all streams of the current device. */
 int p8_device_error(void);
 
 const char *p8_status_str(p8_status s);

@@ -366,8 +366,12 @@ p8_status p8_chain_trace(p8_chain *c, uint64_t *dev_buf, size_t words) {
     return chain_trace(c, reinterpret_cast<unsigned long long *>(dev_buf), words);
 }
 
-/* 1 if a kernel since the last call gave up on a bounded wait (results of that launch are invalid). Synchronous. */
-int p8_device_error(void) { return (int)(read_and_clear_device_error() | read_and_clear_cache_error()); }
+/* The error words of the current device, then cleared. The copies alone would wait for the default stream, and not for streams
+ * that do not block it (torch's others). */
+int p8_device_error(void) {
+    cudaDeviceSynchronize();
+    return (int)(read_and_clear_device_error() | read_and_clear_cache_error());
+}
 
 const char *p8_build_info(void) { return "pingala8_b200 sm_100a (tcgen05/TMA), C ABI v1"; }
 
