@@ -520,19 +520,71 @@ cudaError_t run_append(const p8_kv *c, const AppendArgs &a, cudaStream_t st) {
     return launch_after(c->width == 128 ? k_kv_append<T, 128> : k_kv_append<T, 64>, grid, dim3(256), 0, st, a);
 }
 
-// whether two strided views (three outer dimensions, `last` elements inside) can share bytes
-void span(const void *base, const int64_t *st, const int64_t *dims, int n, int es, int64_t last, uintptr_t &lo, uintptr_t &hi) {
-    int64_t neg = 0, pos = last;
-    for (int i = 0; i < n; ++i) (st[i] < 0 ? neg : pos) += st[i] * (dims[i] - 1);
-    lo = (uintptr_t)base + (uintptr_t)(neg * es);
-    hi = (uintptr_t)base + (uintptr_t)(pos * es);
+// A buffer as a call uses it: rows of `last` bytes at at + sum of i_k st[k], 0 <= i_k < dims[k].
+struct View {
+    uintptr_t at;
+    int n;
+    int64_t dims[4], st[4], last;
+    View(const void *p, const int64_t *strides, const int64_t *counts, int dimensions, int es, int64_t elements)
+        : at((uintptr_t)p), n(dimensions), last(elements * es) {
+        for (int i = 0; i < n; ++i) { dims[i] = counts[i]; st[i] = strides[i] * es; }
+    }
+    void span(uintptr_t &lo, uintptr_t &hi) const {
+        lo = hi = at;
+        for (int i = 0; i < n; ++i) (st[i] < 0 ? lo : hi) += (uintptr_t)(st[i] * (dims[i] - 1));
+        hi += (uintptr_t)last;
+    }
+};
+// Terms c s with lo <= c <= hi, of which one sum between `least` and `most` is looked for, the largest strides first. Views
+// cut from one buffer have strides that nest, which leaves one or two values for each; where there are more than `looks` in all the answer is yes.
+struct Term { int64_t s, lo, hi; };
+bool reaches(const Term *t, int n, int64_t least, int64_t most, int &looks) {
+    if (n == 0) return least <= 0 && 0 <= most;
+    int64_t lo = 0, hi = 0;  // what the others can come to
+    for (int i = 1; i < n; ++i) { lo += t[i].lo * t[i].s; hi += t[i].hi * t[i].s; }
+    const int64_t s = t->s;
+    const auto down = [s](int64_t a) { return a / s - (a % s < 0); };
+    const int64_t from = std::max(t->lo, -down(hi - least)), to = std::min(t->hi, down(most - lo));
+    for (int64_t c = from; c <= to; ++c) {
+        if (--looks < 0 || reaches(t + 1, n - 1, least - c * s, most - c * s, looks)) return true;
+    }
+    return false;
+}
+// whether two views share bytes; what lies between the rows of one may belong to the other
+bool overlap(const View &x, const View &y) {
+    uintptr_t x0, x1, y0, y1;
+    x.span(x0, x1);
+    y.span(y0, y1);
+    if (x0 >= y1 || y0 >= x1) return false;
+    Term t[8] = {};  // by strides, the largest first
+    int n = 0;
+    const auto add = [&](int64_t st, int64_t most, int sign) {
+        if (st == 0 || most == 0) return;
+        const int64_t s = st < 0 ? -st : st;
+        if (st < 0) sign = -sign;
+        int i = 0;
+        while (i < n && t[i].s > s) ++i;
+        if (i == n || t[i].s != s) {
+            for (int j = n++; j > i; --j) t[j] = t[j - 1];
+            t[i] = {s, 0, 0};
+        }
+        (sign > 0 ? t[i].hi : t[i].lo) += sign * most;
+    };
+    for (int i = 0; i < x.n; ++i) add(x.st[i], x.dims[i] - 1, 1);
+    for (int i = 0; i < y.n; ++i) add(y.st[i], y.dims[i] - 1, -1);
+    const int64_t off = (int64_t)(y.at - x.at);  // a row of x and one of y share bytes where the rows' difference is within (off - x.last, off + y.last)
+    int looks = 1000;
+    return reaches(t, n, off - x.last + 1, off + y.last - 1, looks);
 }
 bool overlap(const void *x, const int64_t *xs, const int64_t *xd, int xe, int64_t xl, const void *y, const int64_t *ys, const int64_t *yd, int ye,
              int64_t yl, int n = 3) {
-    uintptr_t x0, x1, y0, y1;
-    span(x, xs, xd, n, xe, xl, x0, x1);
-    span(y, ys, yd, n, ye, yl, y0, y1);
-    return x0 < y1 && y0 < x1;
+    return overlap(View(x, xs, xd, n, xe, xl), View(y, ys, yd, n, ye, yl));
+}
+// whether two views of the same sizes are one: a dimension of one has no stride to speak of
+bool same_strides(const int64_t *a, const int64_t *b, const int64_t *dims, int n) {
+    for (int i = 0; i < n; ++i)
+        if (dims[i] > 1 && a[i] != b[i]) return false;
+    return true;
 }
 }  // namespace
 }  // namespace p8
@@ -558,8 +610,8 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
         !strides_ok(a->q_out_stride, dq, 3, es))
         return P8_ERR_ARG;
     if (a->tokens == 0) return P8_OK;
-    bool same = c->type == P8_KV_F32 && (const void *)a->q == a->q_out;  // in place: every lane writes what it has read
-    for (int i = 0; i < 3; ++i) same = same && a->q_stride[i] == a->q_out_stride[i];
+    // in place: every lane writes what it has read
+    const bool same = c->type == P8_KV_F32 && (const void *)a->q == a->q_out && same_strides(a->q_stride, a->q_out_stride, dq, 3);
     if (!same && overlap(a->q, a->q_stride, dq, 4, c->width, a->q_out, a->q_out_stride, dq, es, c->width)) return P8_ERR_ARG;
     AppendArgs k;
     const float *x[3] = {a->q, a->k, a->v};
@@ -609,9 +661,9 @@ p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream)
     if (!isfinite(a->scale)) return P8_ERR_ARG;
     const int64_t dq[3] = {c->batch, a->tokens, a->heads};
     if (!strides_ok(a->q_stride, dq, 3, elem_size(c->type))) return P8_ERR_ARG;
-    const int64_t dm[3] = {c->batch, c->heads, c->slots}, m3[3] = {a->mass_stride[0], a->mass_stride[1], 1}, o3[3] = {a->out_stride[0], a->out_stride[1], 1};
-    const bool same = a->mass == a->out && m3[0] == o3[0] && m3[1] == o3[1];
-    if (!same && overlap(a->mass, m3, dm, 4, 1, a->out, o3, dm, 4, 1)) return P8_ERR_ARG;
+    const int64_t dm[3] = {c->batch, c->heads, c->slots}, m3[2] = {a->mass_stride[0], a->mass_stride[1]}, o3[2] = {a->out_stride[0], a->out_stride[1]};
+    const bool same = a->mass == a->out && same_strides(m3, o3, dm, 2);
+    if (!same && overlap(a->mass, m3, dm, 4, c->slots, a->out, o3, dm, 4, c->slots, 2)) return P8_ERR_ARG;
     return launch_attn_mass(c, a, (cudaStream_t)stream);
 }
 
@@ -624,17 +676,14 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     const int es = elem_size(s->type);
     const int64_t dims[4] = {s->layers, s->batch, s->heads, s->slots}, ddims[4] = {s->layers, s->batch, s->heads, a->budget};
     // in place: all three buffers and their strides the same; else no overlap at all
-    bool same = s->k == d->k && s->v == d->v && a->mass == a->mass_out;
-    for (int i = 0; i < 4; ++i) same = same && s->k_stride[i] == d->k_stride[i] && s->v_stride[i] == d->v_stride[i];
-    for (int i = 0; i < 3; ++i) same = same && a->mass_stride[i] == a->mass_out_stride[i];
+    const bool same = s->k == d->k && s->v == d->v && a->mass == a->mass_out && same_strides(s->k_stride, d->k_stride, dims, 4) &&
+                      same_strides(s->v_stride, d->v_stride, dims, 4) && same_strides(a->mass_stride, a->mass_out_stride, dims, 3);
     if (!same) {
-        const int64_t m4[4] = {a->mass_stride[0], a->mass_stride[1], a->mass_stride[2], 1}, o4[4] = {a->mass_out_stride[0], a->mass_out_stride[1], a->mass_out_stride[2], 1};
-        const void *from[3] = {s->k, s->v, a->mass}, *to[3] = {d->k, d->v, a->mass_out};
-        const int64_t *fs[3] = {s->k_stride, s->v_stride, m4}, *ts[3] = {d->k_stride, d->v_stride, o4};
-        for (int i = 0; i < 3; ++i)
-            for (int j = 0; j < 3; ++j)
-                if (overlap(from[i], fs[i], dims, i < 2 ? es : 4, i < 2 ? s->width : 1, to[j], ts[j], ddims, j < 2 ? es : 4, j < 2 ? s->width : 1, 4))
-                    return P8_ERR_ARG;
+        const View from[3] = {View(s->k, s->k_stride, dims, 4, es, s->width), View(s->v, s->v_stride, dims, 4, es, s->width), View(a->mass, a->mass_stride, dims, 3, 4, s->slots)};
+        const View to[3] = {View(d->k, d->k_stride, ddims, 4, es, s->width), View(d->v, d->v_stride, ddims, 4, es, s->width), View(a->mass_out, a->mass_out_stride, dims, 3, 4, a->budget)};
+        for (const View &x : from)
+            for (const View &y : to)
+                if (overlap(x, y)) return P8_ERR_ARG;
     }
     EvictArgs k;
     k.mass = a->mass; k.mass_out = a->mass_out;

@@ -1,16 +1,73 @@
-"""What the key/value cache operators refuse, without a GPU (the C entries get addresses that nothing reads: every call below
-ends before it touches a device)."""
+"""What the key/value cache operators refuse before they touch a device, and what they do not. The C entries get addresses that
+nothing may read: without a GPU a call that is not refused ends at its launch, with another status than P8_ERR_ARG."""
 import os
+import random
 import sys
 
 import pytest
+import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 import pingala8_llm_b200 as p8  # noqa: E402
-from test_cache_ops import ARG  # noqa: E402
+from test_cache_ops import ARG, PTR, accept_args, append_args, attn_args, evict_args, kv, mass_args  # noqa: E402
+
+if torch.cuda.is_available():
+    pytest.skip("addresses that nothing may read: not where a launch would reach a GPU", allow_module_level=True)
+
+MB = 1 << 20
 
 
 @pytest.mark.parametrize("ns", [-1, 1 << 32, -(1 << 62)])
 def test_a_wait_limit_out_of_range(ns):
     assert p8.lib().p8_cache_wait_limit(ns) == ARG
+
+
+def places(at, dims, strides, last):
+    """the addresses of 4-byte values"""
+    rows = [at]
+    for d, s in zip(dims, strides):
+        rows = [r + 4 * s * i for r in rows for i in range(d)]
+    return {r + 4 * j for r in rows for j in range(last)}
+
+
+def test_buffers_that_share_memory_are_refused_and_those_that_lie_between_one_another_are_not():
+    """masses and their sums, small strided views of one buffer, against all their addresses"""
+    rng = random.Random(1)
+    refused = taken = between = 0
+    for _ in range(3000):
+        b, h, n = rng.randint(1, 4), rng.randint(1, 4), rng.randint(1, 6)
+        inner = n + rng.choice([0, 0, 1, rng.randint(0, 12)])
+        if rng.random() < 0.5:
+            os_ = (inner * h + rng.randint(0, 9), inner)
+        else:
+            os_ = (inner, inner * b + rng.randint(0, 9))
+        ms = os_ if rng.random() < 0.5 else (rng.randint(1, 60), rng.randint(1, 60))
+        base = 50 * MB
+        off = rng.randint(-80, 80)
+        x, y = places(base, (b, h), os_, n), places(base + 4 * off, (b, h), ms, n)
+        one = off == 0 and (b == 1 or ms[0] == os_[0]) and (h == 1 or ms[1] == os_[1])
+        st = p8.lib().p8_attn_mass(kv(batch=b, heads=h, slots=n), mass_args(heads=2 * h, qs=(2 * h * 2 * 64, 2 * h * 64, 64), q=4 * MB, out=base, os=os_, mass=base + 4 * off, ms=ms,
+                                                                         lens=100 * MB, lse=101 * MB), None)
+        assert st != 0
+        assert (st == ARG) == (bool(x & y) and not one), (b, h, n, os_, ms, off)
+        refused += st == ARG
+        taken += st != ARG
+        between += st != ARG and not one and min(x) < max(y) and min(y) < max(x)
+    assert min(refused, taken, between) > 200
+
+
+def test_interleaved_buffers_are_taken():
+    """queries and outputs side by side in one buffer; a cache's two halves in turn, layer by layer"""
+    L, c = p8.lib(), kv()
+    side = dict(qs=(1024, 512, 128), os=(1024, 512, 128))
+    assert L.p8_tree_attn(c, attn_args(out=4 * PTR + 128, lens=100 * MB, **side), 200 * MB, 1 << 40, None) != ARG
+    assert L.p8_tree_attn(c, attn_args(out=4 * PTR + 64, lens=100 * MB, **side), 200 * MB, 1 << 40, None) == ARG
+    assert L.p8_tree_attn(c, attn_args(out=4 * PTR - 112, lens=100 * MB, **side), 200 * MB, 1 << 40, None) == ARG
+    heads = 2 * 64 * 64  # 2 heads x 64 slots x 64, as many bytes as 2 sequences' 16-bit halves
+    st = (4 * heads, 2 * heads, 64 * 64, 64)
+    src, dst = kv(k=16 * MB, v=32 * MB, layers=2, ks=(8 * heads, *st[1:]), vs=(8 * heads, *st[1:])), kv(k=16 * MB + 4 * heads * 2, v=32 * MB + 4 * heads * 2, layers=2, ks=(8 * heads, *st[1:]), vs=(8 * heads, *st[1:]))
+    args = dict(mass=48 * MB, ms=(512, 128, 64), out=48 * MB + 4 * 256, os=(512, 128, 64), lens=100 * MB, new=101 * MB, kept=102 * MB)
+    assert L.p8_kv_evict(src, dst, evict_args(**args), None) != ARG
+    assert L.p8_kv_evict(src, dst, evict_args(**{**args, "out": 48 * MB + 4 * 255}), None) == ARG
+    assert L.p8_kv_evict(src, kv(k=16 * MB + 2 * (2 * heads + 64 * 64), v=32 * MB + 4 * heads * 2, layers=2, ks=(8 * heads, *st[1:]), vs=(8 * heads, *st[1:])), evict_args(**args), None) == ARG

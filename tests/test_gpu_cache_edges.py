@@ -43,3 +43,37 @@ def test_an_error_on_another_stream_is_there_when_it_is_asked_for():
     cache.tree_attention(q, k, v, lens, stream=side)
     ended(64)
     ended()
+
+
+def test_buffers_that_lie_between_one_another():
+    """outputs in the gaps of inputs: what is documented is that they share no memory, not that they lie apart"""
+    g = gen(2)
+    B, T, H, hk, D, cap = 2, 5, 4, 2, 64, 90
+    k, v, lens = randn(g, B, hk, cap, D, dtype=torch.float16), randn(g, B, hk, cap, D, dtype=torch.float16), ints(70, 31)
+    both = randn(g, B, T, 2, H, D, dtype=torch.float16)  # a token's queries, then its outputs
+    q = both[:, :, 0].clone()
+    want, lse = cache.tree_attention(q, k, v, lens)
+    got, _ = cache.tree_attention(both[:, :, 0], k, v, lens, out=both[:, :, 1])
+    assert torch.equal(got, want) and torch.equal(both[:, :, 0], q)
+    mass = torch.rand(B, 2, hk, cap, device="cuda", generator=g)
+    plain = cache.attention_mass(q, lse, k, lens, mass[:, 0].contiguous(), out=mass[:, 1].contiguous())
+    old = mass[:, 0].clone()
+    assert torch.equal(cache.attention_mass(q, lse, k, lens, mass[:, 0], out=mass[:, 1]), plain) and torch.equal(mass[:, 0], old)
+    kv = randn(g, 3, 2, B, hk, cap, D, dtype=torch.float16)  # of each layer the cache, then room for what is kept of it
+    vv, m = randn(g, 3, 2, B, hk, cap, D, dtype=torch.float16), torch.rand(3, 2, B, hk, cap, device="cuda", generator=g)
+    args = [x[:, 0].clone() for x in (kv, vv, m)]
+    new, kept = cache.kv_evict(*args, lens, 40, 2, 8)
+    new2, kept2 = cache.kv_evict(kv[:, 0], vv[:, 0], m[:, 0], lens, 40, 2, 8, k_out=kv[:, 1], v_out=vv[:, 1], mass_out=m[:, 1])
+    assert torch.equal(new, new2) and torch.equal(kept, kept2)
+    for b, n in enumerate(new.tolist()):
+        for x, y in zip(args, (kv, vv, m)):
+            assert torch.equal(y[:, 1, b, :, :n], x[:, b, :, :n])
+    # one sequence, whose stride says nothing: in place all the same
+    x = randn(g, 1, T, 3, D).as_strided((1, T, 3, D), (4 * D, 3 * D, D, 1))
+    xk, c, pos = randn(g, 1, T, 1, D), torch.rand(9, D // 2, device="cuda", generator=g), ints(0, 1, 2, 3, 4)[None]
+    kc, vc = randn(g, 1, 1, 20, D), randn(g, 1, 1, 20, D)
+    want = cache.kv_append(x, xk, xk, kc, vc, ints(3), pos, c, c)
+    y = x.clone()
+    z = y.as_strided((1, T, 3, D), (8 * D, 3 * D, D, 1))
+    assert torch.equal(cache.kv_append(y, xk, xk, kc, vc, ints(3), pos, c, c, q_out=z), want)
+    ended()
