@@ -420,7 +420,8 @@ p8_status p8_kv_evict(const p8_kv *src, const p8_kv *dst, const p8_kv_evict_args
  * goes on to the lowest child whose token is the target's at the node it has reached. The path's keys and values are
  * moved, in all layers, from slots lens[b] + path[i] to lens[b] + i. path [batch][tokens] (-1 behind the path),
  * accepted[b] its length, next_token[b] the target at its end, new_lens[b] = lens[b] + accepted[b]; n_b = 0: nothing
- * accepted, next_token -1. new_lens must not be lens. */
+ * accepted, next_token -1. What is written (path, accepted, new_lens, next_token, the keys, the values) overlaps neither one
+ * another nor what is read. */
 typedef struct p8_tree_accept_args {
     const int64_t *tokens, *target;       /* [batch][ntokens] */
     const int32_t *parents;

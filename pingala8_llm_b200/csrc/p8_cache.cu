@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 #include "p8_device.cuh"
 #include "p8_internal.h"
@@ -521,18 +522,19 @@ cudaError_t run_append(const p8_kv *c, const AppendArgs &a, cudaStream_t st) {
 }
 
 // A buffer as a call uses it: rows of `last` bytes at at + sum of i_k st[k], 0 <= i_k < dims[k].
+// One whose address is NULL is not there.
 struct View {
-    uintptr_t at;
+    uintptr_t at, lo, hi;  // [lo, hi): from the first of its bytes to the last
     int n;
     int64_t dims[4], st[4], last;
-    View(const void *p, const int64_t *strides, const int64_t *counts, int dimensions, int es, int64_t elements)
-        : at((uintptr_t)p), n(dimensions), last(elements * es) {
-        for (int i = 0; i < n; ++i) { dims[i] = counts[i]; st[i] = strides[i] * es; }
-    }
-    void span(uintptr_t &lo, uintptr_t &hi) const {
-        lo = hi = at;
-        for (int i = 0; i < n; ++i) (st[i] < 0 ? lo : hi) += (uintptr_t)(st[i] * (dims[i] - 1));
-        hi += (uintptr_t)last;
+    View(const void *p, int64_t bytes) : at((uintptr_t)p), lo(at), hi(at + (uintptr_t)(p ? bytes : 0)), n(0), last(bytes) {}
+    View(const void *p, const int64_t *strides, const int64_t *counts, int dimensions, int es, int64_t elements) : View(p, elements * es) {
+        n = dimensions;
+        for (int i = 0; i < n; ++i) {
+            dims[i] = counts[i];
+            st[i] = strides[i] * es;
+            if (p) (st[i] < 0 ? lo : hi) += (uintptr_t)(st[i] * (dims[i] - 1));
+        }
     }
 };
 // Terms c s with lo <= c <= hi, of which one sum between `least` and `most` is looked for, the largest strides first. Views
@@ -552,10 +554,7 @@ bool reaches(const Term *t, int n, int64_t least, int64_t most, int &looks) {
 }
 // whether two views share bytes; what lies between the rows of one may belong to the other
 bool overlap(const View &x, const View &y) {
-    uintptr_t x0, x1, y0, y1;
-    x.span(x0, x1);
-    y.span(y0, y1);
-    if (x0 >= y1 || y0 >= x1) return false;
+    if (x.lo >= y.hi || y.lo >= x.hi) return false;
     Term t[8] = {};  // by strides, the largest first
     int n = 0;
     const auto add = [&](int64_t st, int64_t most, int sign) {
@@ -579,6 +578,16 @@ bool overlap(const View &x, const View &y) {
 bool overlap(const void *x, const int64_t *xs, const int64_t *xd, int xe, int64_t xl, const void *y, const int64_t *ys, const int64_t *yd, int ye,
              int64_t yl, int n = 3) {
     return overlap(View(x, xs, xd, n, xe, xl), View(y, ys, yd, n, ye, yl));
+}
+// whether a call would write to what it reads or to one place twice
+bool clash(std::initializer_list<View> out, std::initializer_list<View> in) {
+    for (const View *x = out.begin(); x != out.end(); ++x) {
+        for (const View *y = x + 1; y != out.end(); ++y)
+            if (overlap(*x, *y)) return true;
+        for (const View &y : in)
+            if (overlap(*x, y)) return true;
+    }
+    return false;
 }
 // whether two views of the same sizes are one: a dimension of one has no stride to speak of
 bool same_strides(const int64_t *a, const int64_t *b, const int64_t *dims, int n) {
@@ -713,8 +722,14 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
 p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream) {
     if (!kv_ok(c) || !a || !a->tokens || !a->target || !a->parents || !a->lens || !a->path || !a->accepted || !a->new_lens || !a->next_token)
         return P8_ERR_ARG;
-    if (a->ntokens < 1 || a->ntokens > P8_TREE_MAX || a->new_lens == a->lens) return P8_ERR_ARG;
+    if (a->ntokens < 1 || a->ntokens > P8_TREE_MAX) return P8_ERR_ARG;
     const int es = elem_size(c->type);
+    // every block reads the tree, and one writes the results: no order is between them
+    const int64_t dims[4] = {c->layers, c->batch, c->heads, c->slots}, B = c->batch, BT = B * a->ntokens;
+    if (clash({View(a->path, 4 * BT), View(a->accepted, 4 * B), View(a->new_lens, 4 * B), View(a->next_token, 8 * B), View(c->k, c->k_stride, dims, 4, es, c->width),
+               View(c->v, c->v_stride, dims, 4, es, c->width)},
+              {View(a->tokens, 8 * BT), View(a->target, 8 * BT), View(a->parents, 4 * BT), View(a->lens, 4 * B), View(a->counts, 4 * B)}))
+        return P8_ERR_ARG;
     AcceptArgs k;
     k.tokens = (const long long *)a->tokens; k.target = (const long long *)a->target; k.next = (long long *)a->next_token;
     k.parents = a->parents; k.lens = a->lens; k.counts = a->counts;

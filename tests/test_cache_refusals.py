@@ -71,3 +71,21 @@ def test_interleaved_buffers_are_taken():
     assert L.p8_kv_evict(src, dst, evict_args(**args), None) != ARG
     assert L.p8_kv_evict(src, dst, evict_args(**{**args, "out": 48 * MB + 4 * 255}), None) == ARG
     assert L.p8_kv_evict(src, kv(k=16 * MB + 2 * (2 * heads + 64 * 64), v=32 * MB + 4 * heads * 2, layers=2, ks=(8 * heads, *st[1:]), vs=(8 * heads, *st[1:])), evict_args(**args), None) == ARG
+
+
+def accept(cache=None, **o):
+    at = dict(tokens=50 * MB, target=51 * MB, parents=52 * MB, lens=53 * MB, counts=54 * MB, path=55 * MB, accepted=56 * MB, new=57 * MB, next=58 * MB) | o
+    return p8.lib().p8_tree_accept(cache or kv(), accept_args(**at), None)
+
+
+def test_accept_refuses_results_over_its_inputs():
+    """two sequences, four tokens: the tree is 64 bytes of tokens and of targets and 32 of parents, lengths are 8 bytes"""
+    assert accept() != ARG and accept(counts=0) != ARG
+    assert accept(accepted=54 * MB + 8, path=52 * MB + 32, new=53 * MB + 8, next=51 * MB + 64) != ARG  # right behind one another
+    for bad in (dict(accepted=54 * MB), dict(accepted=54 * MB + 4), dict(accepted=53 * MB), dict(path=52 * MB), dict(path=52 * MB + 28), dict(path=50 * MB + 60), dict(new=53 * MB),
+                dict(new=53 * MB + 4), dict(new=53 * MB - 4), dict(new=54 * MB), dict(next=51 * MB + 56), dict(next=50 * MB), dict(next=58 * MB, new=58 * MB + 12),
+                dict(accepted=57 * MB), dict(path=56 * MB - 28), dict(path=PTR), dict(next=2 * PTR + 2 * 2 * 64 * 64 * 2 - 8), dict(lens=PTR + 4096)):
+        assert accept(**bad) == ARG, bad
+    assert accept(kv(k=PTR, v=PTR)) == ARG and accept(kv(k=PTR, v=PTR + 4096)) == ARG  # keys and values over one another
+    turns = (2 * 2 * 64 * 64 * 2, 2 * 64 * 64 * 2, 64 * 64 * 2, 64 * 2)
+    assert accept(kv(k=PTR, v=PTR + 128, ks=turns, vs=turns)) != ARG  # and side by side in every slot

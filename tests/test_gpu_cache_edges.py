@@ -77,3 +77,20 @@ def test_buffers_that_lie_between_one_another():
     z = y.as_strided((1, T, 3, D), (8 * D, 3 * D, D, 1))
     assert torch.equal(cache.kv_append(y, xk, xk, kc, vc, ints(3), pos, c, c, q_out=z), want)
     ended()
+
+
+def refused(call):
+    with pytest.raises(p8.P8Error) as e:
+        call()
+    assert e.value.status == -1
+
+
+def test_accept_in_place_of_its_inputs_is_refused():
+    g = gen(3)
+    k, v, lens, counts = randn(g, 2, 3, 2, 40, 64), randn(g, 2, 3, 2, 40, 64), ints(3, 0, 20), ints(4, 4, 2)
+    tok, par = torch.zeros(3, 4, dtype=torch.int64, device="cuda"), ints(-1, 0, 1, 2).repeat(3, 1)
+    for o in (dict(accepted=counts), dict(accepted=lens), dict(path=par), dict(new_lens=counts), dict(new_lens=lens)):
+        refused(lambda: cache.tree_accept(tok, par, tok, k, v, lens, counts=counts, **o))
+    refused(lambda: cache.tree_accept(tok, par, tok, k, k, lens))
+    assert cache.tree_accept(tok, par, tok, k, v, lens, counts=counts).accepted.tolist() == [4, 4, 2]
+    ended()
