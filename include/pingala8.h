@@ -401,8 +401,8 @@ p8_status p8_cache_wait_limit(int64_t ns);
  * -infinity), in their order. Keys, values and mass [layer][b][h] of the kept slots are written to the first slots of
  * dst and mass_out, which are either the same buffers as src and mass (in place) or do not overlap them; a shorter
  * sequence is kept whole. new_lens[b] = min(lens[b], budget), kept [layers][batch][heads][budget] the kept slots (-1
- * behind new_lens[b]). sinks + recent <= budget <= the slots of dst and of src; new_lens must not be lens. Mass
- * strides: layer, sequence, head. A sequence with lens[b] outside [0, slots] is left alone, its new_lens and kept too,
+ * behind new_lens[b]). sinks + recent <= budget <= the slots of dst and of src. new_lens and kept overlap
+ * neither each other nor anything else, nor do what is written of keys, of values and of masses. Mass strides: layer, sequence, head. A sequence with lens[b] outside [0, slots] is left alone, its new_lens and kept too,
  * and sets bit 6. */
 typedef struct p8_kv_evict_args {
     const float *mass;

@@ -677,7 +677,7 @@ p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream)
 }
 
 p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a, void *stream) {
-    if (!kv_ok(s) || !kv_ok(d) || !a || !a->mass || !a->mass_out || !a->lens || !a->new_lens || !a->kept || a->new_lens == a->lens) return P8_ERR_ARG;
+    if (!kv_ok(s) || !kv_ok(d) || !a || !a->mass || !a->mass_out || !a->lens || !a->new_lens || !a->kept) return P8_ERR_ARG;
     if (s->type != d->type || s->width != d->width || s->layers != d->layers || s->batch != d->batch || s->heads != d->heads) return P8_ERR_ARG;
     if (a->budget < 1 || a->sinks < 0 || a->recent < 0 || a->sinks > a->budget || a->recent > a->budget - a->sinks || a->budget > d->slots ||
         a->budget > s->slots)
@@ -687,13 +687,11 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     // in place: all three buffers and their strides the same; else no overlap at all
     const bool same = s->k == d->k && s->v == d->v && a->mass == a->mass_out && same_strides(s->k_stride, d->k_stride, dims, 4) &&
                       same_strides(s->v_stride, d->v_stride, dims, 4) && same_strides(a->mass_stride, a->mass_out_stride, dims, 3);
-    if (!same) {
-        const View from[3] = {View(s->k, s->k_stride, dims, 4, es, s->width), View(s->v, s->v_stride, dims, 4, es, s->width), View(a->mass, a->mass_stride, dims, 3, 4, s->slots)};
-        const View to[3] = {View(d->k, d->k_stride, ddims, 4, es, s->width), View(d->v, d->v_stride, ddims, 4, es, s->width), View(a->mass_out, a->mass_out_stride, dims, 3, 4, a->budget)};
-        for (const View &x : from)
-            for (const View &y : to)
-                if (overlap(x, y)) return P8_ERR_ARG;
-    }
+    const int64_t B = s->batch;
+    const View sk(s->k, s->k_stride, dims, 4, es, s->width), sv(s->v, s->v_stride, dims, 4, es, s->width), sm(a->mass, a->mass_stride, dims, 3, 4, s->slots);
+    const View dk(d->k, d->k_stride, ddims, 4, es, s->width), dv(d->v, d->v_stride, ddims, 4, es, s->width), dm(a->mass_out, a->mass_out_stride, dims, 3, 4, a->budget);
+    const View lens(a->lens, 4 * B), new_lens(a->new_lens, 4 * B), kept(a->kept, 4 * s->layers * B * s->heads * a->budget);
+    if (same ? clash({new_lens, kept, sk, sv, sm}, {lens}) : clash({new_lens, kept, dk, dv, dm}, {lens, sk, sv, sm})) return P8_ERR_ARG;
     EvictArgs k;
     k.mass = a->mass; k.mass_out = a->mass_out;
     for (int i = 0; i < 3; ++i) { k.ms[i] = a->mass_stride[i]; k.mos[i] = a->mass_out_stride[i]; }

@@ -89,3 +89,27 @@ def test_accept_refuses_results_over_its_inputs():
     assert accept(kv(k=PTR, v=PTR)) == ARG and accept(kv(k=PTR, v=PTR + 4096)) == ARG  # keys and values over one another
     turns = (2 * 2 * 64 * 64 * 2, 2 * 64 * 64 * 2, 64 * 64 * 2, 64 * 2)
     assert accept(kv(k=PTR, v=PTR + 128, ks=turns, vs=turns)) != ARG  # and side by side in every slot
+
+
+def evict(src=None, dst=None, **o):
+    at = dict(mass=48 * MB, out=48 * MB, lens=53 * MB, new=54 * MB, kept=55 * MB) | o
+    src = src or kv(k=16 * MB, v=32 * MB)
+    return p8.lib().p8_kv_evict(src, dst or src, evict_args(**at), None)
+
+
+def test_evict_refuses_results_over_its_inputs():
+    """two sequences of two heads, 64 slots cut to 8: lengths are 8 bytes, kept slots 128, masses 1,024 (in rows of 256)"""
+    other = kv(k=64 * MB, v=80 * MB)
+    assert evict() != ARG and evict(dst=other, out=49 * MB) != ARG
+    assert evict(new=53 * MB + 8, kept=53 * MB - 128) != ARG
+    for bad in (dict(new=53 * MB), dict(new=53 * MB + 4), dict(new=53 * MB - 4), dict(kept=53 * MB), dict(kept=53 * MB - 124), dict(kept=54 * MB + 4), dict(new=55 * MB + 124),
+                dict(kept=48 * MB + 1020), dict(new=48 * MB), dict(kept=16 * MB), dict(new=32 * MB), dict(lens=48 * MB), dict(lens=16 * MB + 4)):
+        assert evict(**bad) == ARG, bad
+        if not {48 * MB, 16 * MB, 32 * MB} & {x // 4096 * 4096 for x in bad.values()}:
+            assert evict(dst=other, out=49 * MB, **bad) == ARG, bad
+    one = kv(k=16 * MB, v=16 * MB)
+    assert evict(one) == ARG  # keys and values in one place, cut in place
+    assert evict(one, other, out=49 * MB) != ARG  # read from one place
+    assert evict(dst=kv(k=64 * MB, v=64 * MB), out=49 * MB) == ARG  # written to one place
+    assert evict(dst=other, out=64 * MB) == ARG and evict(dst=other, out=16 * MB) == ARG
+    assert evict(dst=kv(k=32 * MB, v=80 * MB), out=49 * MB) == ARG

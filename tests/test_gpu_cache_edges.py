@@ -94,3 +94,17 @@ def test_accept_in_place_of_its_inputs_is_refused():
     refused(lambda: cache.tree_accept(tok, par, tok, k, k, lens))
     assert cache.tree_accept(tok, par, tok, k, v, lens, counts=counts).accepted.tolist() == [4, 4, 2]
     ended()
+
+
+def test_evict_over_its_inputs_is_refused():
+    g = gen(4)
+    k, v, m = randn(g, 2, 2, 40, 64), randn(g, 2, 2, 40, 64), torch.rand(2, 2, 40, device="cuda", generator=g)
+    lens = ints(30, 20, 10)
+    refused(lambda: cache.kv_evict(k, v, m, lens[:2], 8, new_lens=lens[:2]))
+    refused(lambda: cache.kv_evict(k, v, m, lens[:2], 8, new_lens=lens[1:]))
+    refused(lambda: cache.kv_evict(k, k, m, lens[:2], 8))
+    x = k.clone()
+    refused(lambda: cache.kv_evict(k, v, m, lens[:2], 8, k_out=x, v_out=x, mass_out=m.clone()))
+    refused(lambda: cache.kv_evict(k, v, m, lens[:2], 8, kept=m.view(torch.int32).view(-1)[:32].view(2, 2, 8)))
+    assert cache.kv_evict(k, v, m, lens[:2], 8)[0].tolist() == [8, 8]
+    ended()
