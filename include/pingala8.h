@@ -328,8 +328,8 @@ typedef struct p8_kv {
  * q_norm / k_norm [width] is given), then the halves rotate by the token's position p = pos[b * tokens + t]:
  *     y[i] = x'[i] cos[p][i] - x'[i + width/2] sin[p][i],  y[i + width/2] = x'[i + width/2] cos[p][i] + x'[i] sin[p][i]
  * with cos / sin f32 [positions][width / 2]. Rotated keys and plain values are rounded once to the cache's type and
- * written to the tokens' slots, rotated queries to q_out (the cache's type; it may be q itself where that is f32, but
- * must not overlap it otherwise). Any number of tokens. A token whose
+ * written to the tokens' slots, rotated queries to q_out (the cache's type; it may be q itself where that is f32). Otherwise
+ * q_out, the keys and the values overlap neither one another nor anything that is read. Any number of tokens. A token whose
  * position is outside [0, positions) is left out and sets bit 6. */
 typedef struct p8_kv_append_args {
     const float *q, *k, *v;

@@ -621,7 +621,12 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
     if (a->tokens == 0) return P8_OK;
     // in place: every lane writes what it has read
     const bool same = c->type == P8_KV_F32 && (const void *)a->q == a->q_out && same_strides(a->q_stride, a->q_out_stride, dq, 3);
-    if (!same && overlap(a->q, a->q_stride, dq, 4, c->width, a->q_out, a->q_out_stride, dq, es, c->width)) return P8_ERR_ARG;
+    const int64_t dkv[3] = {c->batch, c->heads, c->slots}, B = c->batch, table = a->positions * (c->width / 2) * 4;
+    const View q(same ? nullptr : a->q, a->q_stride, dq, 3, 4, c->width);
+    if (clash({View(a->q_out, a->q_out_stride, dq, 3, es, c->width), View(c->k, c->k_stride + 1, dkv, 3, es, c->width), View(c->v, c->v_stride + 1, dkv, 3, es, c->width)},
+              {q, View(a->k, a->k_stride, dk, 3, 4, c->width), View(a->v, a->v_stride, dk, 3, 4, c->width), View(a->lens, 4 * B), View(a->counts, 4 * B),
+               View(a->pos, 4 * B * a->tokens), View(a->cos, table), View(a->sin, table), View(a->q_norm, 4 * c->width), View(a->k_norm, 4 * c->width)}))
+        return P8_ERR_ARG;
     AppendArgs k;
     const float *x[3] = {a->q, a->k, a->v};
     const int64_t *xs[3] = {a->q_stride, a->k_stride, a->v_stride};

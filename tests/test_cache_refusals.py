@@ -113,3 +113,27 @@ def test_evict_refuses_results_over_its_inputs():
     assert evict(dst=kv(k=64 * MB, v=64 * MB), out=49 * MB) == ARG  # written to one place
     assert evict(dst=other, out=64 * MB) == ARG and evict(dst=other, out=16 * MB) == ARG
     assert evict(dst=kv(k=32 * MB, v=80 * MB), out=49 * MB) == ARG
+
+
+def append(cache=None, **o):
+    at = dict(q=50 * MB, k=51 * MB, v=52 * MB, lens=53 * MB, counts=54 * MB, pos=55 * MB, cos=56 * MB, sin=57 * MB, qn=58 * MB, kn=59 * MB, out=60 * MB) | o
+    return p8.lib().p8_kv_append(cache or kv(), append_args(**at), None)
+
+
+def test_append_refuses_results_over_its_inputs():
+    """two sequences of two tokens: q is 4,096 bytes and its 16-bit result 2,048, k and v are 2,048 each, tables 10 x 128"""
+    assert append() != ARG and append(qn=0, kn=0, counts=0) != ARG
+    for bad in (dict(out=51 * MB), dict(out=51 * MB + 2032), dict(out=52 * MB), dict(out=50 * MB), dict(out=53 * MB), dict(out=54 * MB - 2032), dict(out=55 * MB), dict(out=56 * MB + 1264),
+                dict(out=57 * MB), dict(out=58 * MB), dict(out=59 * MB + 240), dict(out=PTR), dict(out=2 * PTR + 32752), dict(k=PTR), dict(v=PTR + 128), dict(q=2 * PTR), dict(lens=PTR),
+                dict(cos=2 * PTR), dict(qn=PTR + 256)):
+        assert append(**bad) == ARG, bad
+    assert append(out=51 * MB + 2048, qn=59 * MB + 256) != ARG
+    assert append(kv(k=PTR, v=PTR)) == ARG and append(kv(k=PTR, v=PTR + 64)) == ARG
+    wide = kv(type=0)
+    assert append(wide, out=50 * MB) != ARG  # in place
+    for bad in (dict(k=50 * MB), dict(v=50 * MB + 2048), dict(cos=50 * MB), dict(out=50 * MB + 16), dict(os=(512, 256, 128))):
+        assert append(wide, **{"out": 50 * MB, **bad}) == ARG, bad
+    # queries, keys and values as one product leaves them, the queries in place
+    packed = dict(q=50 * MB, k=50 * MB + 1024, v=50 * MB + 1536, qs=(1024, 512, 64), ks=(1024, 512, 64), vs=(1024, 512, 64))
+    assert append(wide, out=50 * MB, os=(1024, 512, 64), **packed) != ARG
+    assert append(wide, out=50 * MB, os=(1024, 512, 64), **{**packed, "k": 50 * MB + 1008}) == ARG

@@ -108,3 +108,20 @@ def test_evict_over_its_inputs_is_refused():
     refused(lambda: cache.kv_evict(k, v, m, lens[:2], 8, kept=m.view(torch.int32).view(-1)[:32].view(2, 2, 8)))
     assert cache.kv_evict(k, v, m, lens[:2], 8)[0].tolist() == [8, 8]
     ended()
+
+
+def test_append_over_its_inputs_is_refused():
+    g = gen(5)
+    x = randn(g, 2, 5, 6, 64)
+    q, xk, xv = x[:, :, :2], x[:, :, 2:4], x[:, :, 4:]
+    k, v, c, pos = randn(g, 2, 2, 20, 64), randn(g, 2, 2, 20, 64), torch.rand(9, 32, device="cuda", generator=g), torch.arange(5, device="cuda").int().repeat(2, 1)
+    lens = ints(3, 11)
+    k0, v0 = k.clone(), v.clone()
+    want = cache.kv_append(q, xk, xv, k0, v0, lens, pos, c, c)
+    refused(lambda: cache.kv_append(q, xk, xv, k, v, lens, pos, c, c, q_out=xk))
+    refused(lambda: cache.kv_append(q, xk, xv, k, v, lens, pos, c, c, q_out=k.transpose(1, 2)[:, :5]))
+    refused(lambda: cache.kv_append(q, xk, xv, k, k, lens, pos, c, c))
+    refused(lambda: cache.kv_append(q, k.transpose(1, 2)[:, 3:8], xv, k, v, lens, pos, c, c))
+    assert torch.equal(cache.kv_append(q, xk, xv, k, v, lens, pos, c, c, q_out=q), want)  # in the product's own place
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    ended()
