@@ -352,7 +352,7 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
  * sees nothing gets 0 and -infinity. What a token does not see does not reach it, whatever its bits (infinities and NaN
  * included; f32: an infinity that it does see, before the call's tokens, comes out as NaN). Products and sums in fp32
  * (16-bit types: the weights are rounded to the type before they multiply v; f32: products of two TF32 pieces each,
- * 2^-21). out must not overlap q, k or v. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
+ * 2^-21). out, lse and the workspace overlap neither one another nor anything that is read. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
 typedef struct p8_tree_attn_args {
     const void *q;
     int64_t q_stride[3];                  /* sequence, token, head */
@@ -373,7 +373,7 @@ p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspa
  * p8_tree_accept has moved into place): token i sees slots <= lens[b] + i, and its query and lse rows are those of row
  * r = rows[b * tokens + i] (rows NULL: r = i) of a p8_tree_attn call. With w the sum of exp(scale q . k - lse):
  *     out[b][h][j] = mass[b][h][j] + w for j < lens[b],  = w for the slots of the n_b tokens, untouched behind them.
- * Strides of mass and out: sequence, head; out may be mass (in place). A row that is out of [0, tokens) counts for
+ * Strides of mass and out: sequence, head; out may be mass (in place), and overlaps nothing else that is read. A row that is out of [0, tokens) counts for
  * nothing and sets bit 6; a row with lse = -infinity counts for nothing. Deterministic. */
 typedef struct p8_attn_mass_args {
     const void *q;

@@ -575,10 +575,6 @@ bool overlap(const View &x, const View &y) {
     int looks = 1000;
     return reaches(t, n, off - x.last + 1, off + y.last - 1, looks);
 }
-bool overlap(const void *x, const int64_t *xs, const int64_t *xd, int xe, int64_t xl, const void *y, const int64_t *ys, const int64_t *yd, int ye,
-             int64_t yl, int n = 3) {
-    return overlap(View(x, xs, xd, n, xe, xl), View(y, ys, yd, n, ye, yl));
-}
 // whether a call would write to what it reads or to one place twice
 bool clash(std::initializer_list<View> out, std::initializer_list<View> in) {
     for (const View *x = out.begin(); x != out.end(); ++x) {
@@ -660,11 +656,12 @@ p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspa
     const int64_t dq[3] = {c->batch, a->tokens, a->heads};
     if (!strides_ok(a->q_stride, dq, 3, es) || !strides_ok(a->out_stride, dq, 3, es)) return P8_ERR_ARG;
     const int64_t dkv[3] = {c->batch, c->heads, c->slots};
-    if (overlap(a->out, a->out_stride, dq, es, c->width, a->q, a->q_stride, dq, es, c->width) ||
-        overlap(a->out, a->out_stride, dq, es, c->width, c->k, c->k_stride + 1, dkv, es, c->width) ||
-        overlap(a->out, a->out_stride, dq, es, c->width, c->v, c->v_stride + 1, dkv, es, c->width))
-        return P8_ERR_ARG;
     const size_t need = tree_attn_workspace(c, a->tokens, a->heads);
+    const int64_t B = c->batch, T = a->tokens;
+    if (clash({View(a->out, a->out_stride, dq, 3, es, c->width), View(a->lse, 4 * B * T * a->heads), View(need && workspace_bytes >= need ? workspace : nullptr, (int64_t)need)},
+              {View(a->q, a->q_stride, dq, 3, es, c->width), View(c->k, c->k_stride + 1, dkv, 3, es, c->width), View(c->v, c->v_stride + 1, dkv, 3, es, c->width),
+               View(a->lens, 4 * B), View(a->counts, 4 * B), View(a->mask, 8 * T * (a->mask_stride ? B : 1))}))
+        return P8_ERR_ARG;
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return P8_ERR_WORKSPACE;
     return launch_tree_attn(c, a, workspace, (cudaStream_t)stream);
 }
@@ -677,7 +674,11 @@ p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream)
     if (!strides_ok(a->q_stride, dq, 3, elem_size(c->type))) return P8_ERR_ARG;
     const int64_t dm[3] = {c->batch, c->heads, c->slots}, m3[2] = {a->mass_stride[0], a->mass_stride[1]}, o3[2] = {a->out_stride[0], a->out_stride[1]};
     const bool same = a->mass == a->out && same_strides(m3, o3, dm, 2);
-    if (!same && overlap(a->mass, m3, dm, 4, c->slots, a->out, o3, dm, 4, c->slots, 2)) return P8_ERR_ARG;
+    const int64_t B = c->batch, T = a->tokens;
+    if (clash({View(a->out, o3, dm, 2, 4, c->slots)},
+              {View(same ? nullptr : a->mass, m3, dm, 2, 4, c->slots), View(a->q, a->q_stride, dq, 3, elem_size(c->type), c->width), View(a->lse, 4 * B * T * a->heads),
+               View(c->k, c->k_stride + 1, dm, 3, elem_size(c->type), c->width), View(a->lens, 4 * B), View(a->counts, 4 * B), View(a->rows, 4 * B * T)}))
+        return P8_ERR_ARG;
     return launch_attn_mass(c, a, (cudaStream_t)stream);
 }
 

@@ -137,3 +137,32 @@ def test_append_refuses_results_over_its_inputs():
     packed = dict(q=50 * MB, k=50 * MB + 1024, v=50 * MB + 1536, qs=(1024, 512, 64), ks=(1024, 512, 64), vs=(1024, 512, 64))
     assert append(wide, out=50 * MB, os=(1024, 512, 64), **packed) != ARG
     assert append(wide, out=50 * MB, os=(1024, 512, 64), **{**packed, "k": 50 * MB + 1008}) == ARG
+
+
+def attend(cache=None, ws=70 * MB, **o):
+    at = dict(q=50 * MB, lens=53 * MB, counts=54 * MB, mask=55 * MB, ms=2, out=60 * MB, lse=61 * MB) | o
+    return p8.lib().p8_tree_attn(cache or kv(), attn_args(**at), ws, 8 * MB, None)
+
+
+def test_attention_refuses_results_over_its_inputs():
+    """two sequences of two tokens and four heads of 64: q and out are 2,048 bytes, lse 64, masks 32"""
+    assert attend() != ARG and attend(mask=0, counts=0, lse=0) != ARG and attend(kv(k=PTR, v=PTR)) != ARG
+    for bad in (dict(out=50 * MB), dict(out=50 * MB + 2032), dict(out=53 * MB), dict(out=54 * MB - 2032), dict(out=55 * MB + 16), dict(out=61 * MB + 48), dict(lse=60 * MB + 2044), dict(lse=50 * MB),
+                dict(lse=PTR), dict(lse=2 * PTR + 4), dict(lse=53 * MB + 4), dict(lse=55 * MB - 60), dict(ws=50 * MB), dict(ws=60 * MB), dict(ws=61 * MB), dict(ws=PTR), dict(ws=53 * MB),
+                dict(ws=54 * MB), dict(ws=55 * MB)):
+        assert attend(**bad) == ARG, bad
+    assert attend(out=50 * MB + 2048, lse=55 * MB + 32) != ARG and attend(ms=0, lse=55 * MB + 16) != ARG
+
+
+def weigh(cache=None, **o):
+    at = dict(q=50 * MB, lse=52 * MB, lens=53 * MB, counts=54 * MB, rows=55 * MB, mass=60 * MB, out=60 * MB) | o
+    return p8.lib().p8_attn_mass(cache or kv(), mass_args(**at), None)
+
+
+def test_mass_refuses_results_over_its_inputs():
+    """masses are 1,024 bytes, the two tokens' rows of two sequences 16"""
+    assert weigh() != ARG and weigh(out=61 * MB) != ARG and weigh(counts=0, rows=0) != ARG
+    for bad in (dict(q=60 * MB), dict(lse=60 * MB + 1020), dict(lse=60 * MB - 60), dict(lens=60 * MB), dict(counts=60 * MB + 512), dict(rows=60 * MB - 12), dict(out=52 * MB + 60), dict(out=PTR),
+                dict(out=PTR + 2 * 2 * 64 * 64 * 2 - 4), dict(out=55 * MB + 12)):
+        assert weigh(**bad) == ARG, bad
+    assert weigh(out=52 * MB + 64) != ARG and weigh(out=55 * MB + 16) != ARG
