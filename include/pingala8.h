@@ -309,9 +309,11 @@ p8_status p8_encode_slice(const float *X, int64_t ldx, const float *Hb, int64_t 
  *
  * Layouts: element (layer, b, h, slot, d) of the keys is k[layer * k_stride[0] + b * k_stride[1] + h * k_stride[2] +
  * slot * k_stride[3] + d], of the values alike. width is 64 or 128; every base address and every stride that is used
- * (its dimension is above 1) is positive and a multiple of 16 bytes; keys and values share no memory. The current device
- * is the buffers'. Where buffers must not overlap, what lies between the rows of one may still belong to another. Calls that share a workspace or an output must not overlap on the GPU. Query heads: `heads` is a multiple of the cache's heads, query
- * head i reads cache head i / (heads / kv heads). Strides are in elements. */
+ * (its dimension is above 1) is positive and a multiple of 16 bytes. Keys and values share no memory in a call that writes
+ * them. Rows that are written share none with one another: each stride of an output, the masses among them, steps over all
+ * that the smaller ones reach. Where buffers must not overlap, what lies between the rows of one may still belong to another.
+ * The current device is the buffers'. Calls that share a workspace or an output must not overlap on the GPU. Query heads:
+ * `heads` is a multiple of the cache's heads, query head i reads cache head i / (heads / kv heads). Strides are in elements. */
 typedef enum p8_kv_type { P8_KV_F32 = 0, P8_KV_F16 = 1, P8_KV_BF16 = 2 } p8_kv_type;
 #define P8_TREE_MAX 64   /* tokens of one sequence in a tree attention, mass or accept call */
 #define P8_BATCH_MAX 4096

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -536,6 +537,22 @@ struct View {
             if (p) (st[i] < 0 ? lo : hi) += (uintptr_t)(st[i] * (dims[i] - 1));
         }
     }
+    // Whether its rows may share bytes: each used stride has to step over all that the smaller ones reach, as the strides of every
+    // slice and every order of a dense array's dimensions do.
+    bool folds() const {
+        int64_t reach = last;
+        bool seen[4] = {};
+        for (int k = 0; k < n; ++k) {
+            int least = -1;
+            for (int i = 0; i < n; ++i)
+                if (!seen[i] && dims[i] > 1 && (least < 0 || std::abs(st[i]) < std::abs(st[least]))) least = i;
+            if (least < 0) break;
+            if (std::abs(st[least]) < reach) return true;
+            seen[least] = true;
+            reach += std::abs(st[least]) * (dims[least] - 1);
+        }
+        return false;
+    }
 };
 // Terms c s with lo <= c <= hi, of which one sum between `least` and `most` is looked for, the largest strides first. Views
 // cut from one buffer have strides that nest, which leaves one or two values for each; where there are more than `looks` in all the answer is yes.
@@ -578,6 +595,7 @@ bool overlap(const View &x, const View &y) {
 // whether a call would write to what it reads or to one place twice
 bool clash(std::initializer_list<View> out, std::initializer_list<View> in) {
     for (const View *x = out.begin(); x != out.end(); ++x) {
+        if (x->at && x->folds()) return true;
         for (const View *y = x + 1; y != out.end(); ++y)
             if (overlap(*x, *y)) return true;
         for (const View &y : in)

@@ -166,3 +166,20 @@ def test_mass_refuses_results_over_its_inputs():
                 dict(out=PTR + 2 * 2 * 64 * 64 * 2 - 4), dict(out=55 * MB + 12)):
         assert weigh(**bad) == ARG, bad
     assert weigh(out=52 * MB + 64) != ARG and weigh(out=55 * MB + 16) != ARG
+
+
+def test_outputs_whose_rows_share_memory_are_refused():
+    """a stride of nothing (a tensor expanded over its sequences), or one that does not step over the rows between"""
+    for st in ((0, 64), (128, 0), (0, 0), (64, 64), (32, 64), (100, 64), (64, 100)):
+        assert weigh(os=st, out=61 * MB) == ARG and weigh(ms=st, os=st) == ARG, st
+        assert weigh(ms=st, out=61 * MB) != ARG, st  # read alone
+    assert weigh(os=(64, 128), out=61 * MB) != ARG and weigh(os=(67, 200), out=61 * MB) != ARG
+    heads = 64 * 64
+    for ks in ((0, 2 * heads, 64, 64), (0, heads, heads, 64), (0, 2 * heads, heads, 32), (0, 128, 64, 64)):
+        c = kv(ks=ks)
+        assert append(c) == ARG and accept(c) == ARG and evict(kv(k=16 * MB, v=32 * MB, ks=ks)) == ARG, ks
+        assert evict(kv(k=16 * MB, v=32 * MB, ks=ks), kv(k=64 * MB, v=80 * MB), out=49 * MB) != ARG, ks  # read alone
+        assert attend(c) != ARG, ks
+    assert append(kv(ks=(0, 64, 128, 256))) != ARG  # slots before heads before sequences
+    assert append(os=(512, 64, 64)) == ARG and attend(os=(256, 256, 64)) == ARG and attend(os=(64, 128, 256)) != ARG
+    assert evict(ms=(256, 128, 0), os=(256, 128, 0)) == ARG and evict(ms=(256, 0, 64), os=(256, 0, 64)) == ARG and evict(ms=(0, 128, 64), os=(0, 128, 64)) != ARG

@@ -125,3 +125,16 @@ def test_append_over_its_inputs_is_refused():
     assert torch.equal(cache.kv_append(q, xk, xv, k, v, lens, pos, c, c, q_out=q), want)  # in the product's own place
     assert torch.equal(k, k0) and torch.equal(v, v0)
     ended()
+
+
+def test_masses_expanded_over_sequences_are_read_and_not_written():
+    g = gen(6)
+    k, q, lens = randn(g, 3, 2, 40, 64), randn(g, 3, 1, 4, 64), ints(30, 20, 10)
+    lse = randn(g, 3, 1, 4) + 4
+    one = torch.rand(1, 2, 40, device="cuda", generator=g)
+    refused(lambda: cache.attention_mass(q, lse, k, lens, one.expand(3, 2, 40)))
+    out = cache.attention_mass(q, lse, k, lens, one.expand(3, 2, 40), out=torch.zeros(3, 2, 40, device="cuda"))
+    assert torch.equal(out, cache.attention_mass(q, lse, k, lens, one.repeat(3, 1, 1), out=torch.zeros(3, 2, 40, device="cuda")))
+    refused(lambda: cache.tree_accept(torch.zeros(3, 1, dtype=torch.int64, device="cuda"), ints(-1, -1, -1)[:, None], torch.zeros(3, 1, dtype=torch.int64, device="cuda"),
+                                      k[:1].expand(3, 2, 40, 64), k.clone(), lens))
+    ended()
