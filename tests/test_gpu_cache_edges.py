@@ -138,3 +138,50 @@ def test_masses_expanded_over_sequences_are_read_and_not_written():
     refused(lambda: cache.tree_accept(torch.zeros(3, 1, dtype=torch.int64, device="cuda"), ints(-1, -1, -1)[:, None], torch.zeros(3, 1, dtype=torch.int64, device="cuda"),
                                       k[:1].expand(3, 2, 40, 64), k.clone(), lens))
     ended()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_values_next_to_the_end_of_the_type(dtype, D):
+    """the largest finite numbers are numbers: in a drafted token that others do not see, in a key that draws no weight, in a value
+    that is seen"""
+    g = gen(7 + D)
+    B, T, H, hk, n, big = 1, 5, 8, 2, 130, torch.finfo(dtype).max
+    k, v = randn(g, B, hk, 150, D, dtype=dtype), randn(g, B, hk, 150, D, dtype=dtype)
+    q, lens = randn(g, B, T, H, D, dtype=dtype), ints(n)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    mask = torch.tensor([1, 3, 5, 1 | 8, 1 | 16], device="cuda")
+    want, lse = cache.tree_attention(q, k, v, lens, mask=mask)
+    k2, v2 = k.clone(), v.clone()
+    for sign, col in ((1, 3), (-1, 9)):
+        k2[:, :, n + 3, col], v2[:, :, n + 3, col] = sign * big, sign * big  # token 3, which 0, 1, 2 and 4 do not see
+    got = cache.tree_attention(q, k2, v2, lens, mask=mask)
+    others = [0, 1, 2, 4]
+    assert torch.equal(got[0][:, others], want[:, others]) and torch.equal(got[1][:, others], lse[:, others])
+    # slot 17's key is the lowest number in one column: its score is far below all others, and the rest as without the slot
+    k2, rest = k.clone(), [x for x in range(n + T) if x != 17]
+    k2[:, :, 17] = 0
+    k2[:, :, 17, 0] = -big
+    out, l2 = cache.tree_attention(q, k2, v, lens, mask=mask)
+    less, l3 = cache.tree_attention(q, k[:, :, rest].contiguous(), v[:, :, rest].contiguous(), ints(n - 1), mask=mask)
+    # two orders of the same sums: twice the bound that one has against 64 bits, (2 ds + (68 + 8 sqrt(n)) e) sum p |v| + the weights' and the result's roundings
+    e, u = 2.0 ** -23, torch.finfo(dtype).eps / 2
+    ds = (D + 16) * e * float((q.float().abs().amax(dim=(1, 2)) * k.float().abs().amax(dim=(0, 1, 2))).sum()) / D ** 0.5
+    most = float(v.float().abs().max())
+    tol = 2 * (2 * ds + (68 + 8 * 12) * e + (u if dtype != torch.float32 else 0)) * most + 2 * u * most
+    assert float((out.float() - less.float()).abs().max()) <= tol and float((l2 - l3).abs().max()) <= 2 * (ds + (68 + 8 * 12) * e) + 2 * e * float(l3.abs().max())
+    mass = cache.attention_mass(q, lse, k2, lens, torch.zeros(B, hk, 150, device="cuda"))
+    assert bool((mass[..., 17] == 0).all()) and bool(mass.isfinite().all())
+    # a value that is seen: weight times value, in 64 bits
+    v2 = v.clone()
+    v2[:, :, 40, 5] = big
+    out, _ = cache.tree_attention(q, k, v2, lens, mask=mask)
+    see = torch.cat([torch.ones(T, n, dtype=torch.bool, device="cuda"), (mask[:, None] >> torch.arange(T, device="cuda") & 1).bool()], dim=1)
+    z = torch.einsum("thd,hsd->ths", q[0].double(), k[0, :, : n + T].double().repeat_interleave(H // hk, 0)) / D ** 0.5
+    p = torch.softmax(z.masked_fill(~see[:, None], -float("inf")), -1)
+    y = v2[0, :, : n + T, 5].double().repeat_interleave(H // hk, 0)
+    exact, size = torch.einsum("ths,hs->th", p, y), torch.einsum("ths,hs->th", p, y.abs())
+    assert bool(out[0, :, :, 5].isfinite().all())
+    over = (out[0, :, :, 5].double() - exact).abs() - ((2 * ds + (68 + 8 * 12) * e + (u if dtype != torch.float32 else 0)) * size + u * exact.abs())
+    assert float(over.max()) <= 0
+    ended()
