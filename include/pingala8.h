@@ -354,7 +354,8 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
  * sees nothing gets 0 and -infinity. What a token does not see does not reach it, whatever its bits (infinities and NaN
  * included; f32: an infinity that it does see, before the call's tokens, comes out as itself or as NaN). Products and sums in fp32
  * (16-bit types: the weights are rounded to the type before they multiply v; f32: products of two TF32 pieces each,
- * 2^-21). out, lse and the workspace overlap neither one another nor anything that is read. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
+ * 2^-21). scale and scale / ln 2 are finite in 32 bits (here and in p8_attn_mass). out, lse and the workspace overlap neither
+ * one another nor anything that is read. Workspace: p8_tree_attn_workspace bytes, 256-byte aligned. Deterministic. */
 typedef struct p8_tree_attn_args {
     const void *q;
     int64_t q_stride[3];                  /* sequence, token, head */

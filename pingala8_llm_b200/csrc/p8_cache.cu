@@ -513,6 +513,8 @@ bool kv_ok(const p8_kv *c, bool values = true) {
 }
 bool heads_ok(const p8_kv *c, int64_t heads) { return heads >= c->heads && heads % c->heads == 0 && heads <= 65535; }
 
+bool scale_ok(double scale) { return isfinite((float)scale * 1.4426950408889634f); }  // in base 2, in the kernels' 32 bits
+
 p8_status done(cudaError_t e) { return e == cudaSuccess ? P8_OK : P8_ERR_CUDA; }
 
 template <typename T>
@@ -669,7 +671,7 @@ size_t p8_tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {
 p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspace, size_t workspace_bytes, void *stream) {
     if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
     if (!a->q || !a->out || !a->lens || a->tokens < 1 || a->tokens > P8_TREE_MAX || !al16(a->q) || !al16(a->out)) return P8_ERR_ARG;
-    if (!isfinite(a->scale) || (a->mask && a->mask_stride != 0 && a->mask_stride != a->tokens)) return P8_ERR_ARG;
+    if (!scale_ok(a->scale) || (a->mask && a->mask_stride != 0 && a->mask_stride != a->tokens)) return P8_ERR_ARG;
     const int es = elem_size(c->type);
     const int64_t dq[3] = {c->batch, a->tokens, a->heads};
     if (!strides_ok(a->q_stride, dq, 3, es) || !strides_ok(a->out_stride, dq, 3, es)) return P8_ERR_ARG;
@@ -687,7 +689,7 @@ p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspa
 p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream) {
     if (!kv_ok(c, false) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
     if (!a->q || !a->lse || !a->lens || !a->mass || !a->out || a->tokens < 1 || a->tokens > P8_TREE_MAX || !al16(a->q)) return P8_ERR_ARG;
-    if (!isfinite(a->scale)) return P8_ERR_ARG;
+    if (!scale_ok(a->scale)) return P8_ERR_ARG;
     const int64_t dq[3] = {c->batch, a->tokens, a->heads};
     if (!strides_ok(a->q_stride, dq, 3, elem_size(c->type))) return P8_ERR_ARG;
     const int64_t dm[3] = {c->batch, c->heads, c->slots}, m3[2] = {a->mass_stride[0], a->mass_stride[1]}, o3[2] = {a->out_stride[0], a->out_stride[1]};

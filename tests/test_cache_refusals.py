@@ -183,3 +183,10 @@ def test_outputs_whose_rows_share_memory_are_refused():
     assert append(kv(ks=(0, 64, 128, 256))) != ARG  # slots before heads before sequences
     assert append(os=(512, 64, 64)) == ARG and attend(os=(256, 256, 64)) == ARG and attend(os=(64, 128, 256)) != ARG
     assert evict(ms=(256, 128, 0), os=(256, 128, 0)) == ARG and evict(ms=(256, 0, 64), os=(256, 0, 64)) == ARG and evict(ms=(0, 128, 64), os=(0, 128, 64)) != ARG
+
+
+def test_scales_that_32_bits_do_not_hold_are_refused():
+    for scale in (1e39, -1e300, 3e38, -2.4e38, float("inf"), float("nan")):
+        assert attend(scale=scale) == ARG and weigh(scale=scale) == ARG, scale
+    for scale in (2.3e38, -2.3e38, 0.0, 1e-300, -0.5):
+        assert attend(scale=scale) != ARG and weigh(scale=scale) != ARG, scale
