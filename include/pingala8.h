@@ -331,7 +331,8 @@ typedef struct p8_kv {
  *     y[i] = x'[i] cos[p][i] - x'[i + width/2] sin[p][i],  y[i + width/2] = x'[i + width/2] cos[p][i] + x'[i] sin[p][i]
  * with cos / sin f32 [positions][width / 2]. Rotated keys and plain values are rounded once to the cache's type and
  * written to the tokens' slots, rotated queries to q_out (the cache's type; it may be q itself where that is f32). Otherwise
- * q_out, the keys and the values overlap neither one another nor anything that is read. Any number of tokens. A token whose
+ * q_out, the keys and the values overlap neither one another nor anything that is read. Any number of tokens (none: nothing is
+ * looked at but the cache and the heads). A token whose
  * position is outside [0, positions) is left out and sets bit 6. */
 typedef struct p8_kv_append_args {
     const float *q, *k, *v;

@@ -626,7 +626,9 @@ p8_status p8_cache_wait_limit(int64_t ns) {
 
 p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream) {
     if (!kv_ok(c) || !a || c->layers != 1 || !heads_ok(c, a->heads)) return P8_ERR_ARG;
-    if (!a->q || !a->k || !a->v || !a->q_out || !a->lens || !a->pos || !a->cos || !a->sin || a->tokens < 0 || a->positions < 1) return P8_ERR_ARG;
+    if (a->tokens < 0) return P8_ERR_ARG;
+    if (a->tokens == 0) return P8_OK;  // buffers of nothing may have no address
+    if (!a->q || !a->k || !a->v || !a->q_out || !a->lens || !a->pos || !a->cos || !a->sin || a->positions < 1) return P8_ERR_ARG;
     if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->q_out) || !al16(a->cos) || !al16(a->sin) || !(a->eps >= 0.0)) return P8_ERR_ARG;
     if (a->tokens > c->slots || c->batch * a->tokens * (a->heads + 2 * c->heads) > (int64_t(1) << 31) - 64) return P8_ERR_ARG;
     const int es = elem_size(c->type);
@@ -634,7 +636,6 @@ p8_status p8_kv_append(const p8_kv *c, const p8_kv_append_args *a, void *stream)
     if (!strides_ok(a->q_stride, dq, 3, 4) || !strides_ok(a->k_stride, dk, 3, 4) || !strides_ok(a->v_stride, dk, 3, 4) ||
         !strides_ok(a->q_out_stride, dq, 3, es))
         return P8_ERR_ARG;
-    if (a->tokens == 0) return P8_OK;
     // in place: every lane writes what it has read
     const bool same = c->type == P8_KV_F32 && (const void *)a->q == a->q_out && same_strides(a->q_stride, a->q_out_stride, dq, 3);
     const int64_t dkv[3] = {c->batch, c->heads, c->slots}, B = c->batch, table = a->positions * (c->width / 2) * 4;

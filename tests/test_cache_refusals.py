@@ -190,3 +190,9 @@ def test_scales_that_32_bits_do_not_hold_are_refused():
         assert attend(scale=scale) == ARG and weigh(scale=scale) == ARG, scale
     for scale in (2.3e38, -2.3e38, 0.0, 1e-300, -0.5):
         assert attend(scale=scale) != ARG and weigh(scale=scale) != ARG, scale
+
+
+def test_append_of_no_tokens_is_a_call_that_does_nothing():
+    nothing = dict(tokens=0, q=0, k=0, v=0, out=0, pos=0)
+    assert append(**nothing) == 0 and append(**nothing, lens=0, cos=0, sin=0) == 0
+    assert append(kv(width=96), **nothing) == ARG and append(**nothing, heads=3) == ARG and append(**{**nothing, "tokens": -1}) == ARG

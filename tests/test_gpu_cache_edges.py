@@ -185,3 +185,12 @@ def test_values_next_to_the_end_of_the_type(dtype, D):
     over = (out[0, :, :, 5].double() - exact).abs() - ((2 * ds + (68 + 8 * 12) * e + (u if dtype != torch.float32 else 0)) * size + u * exact.abs())
     assert float(over.max()) <= 0
     ended()
+
+
+def test_append_of_no_tokens():
+    k, v = torch.ones(2, 2, 20, 64, device="cuda"), torch.ones(2, 2, 20, 64, device="cuda")
+    c = torch.rand(9, 32, device="cuda")
+    x = torch.empty(2, 0, 4, 64, device="cuda")
+    out = cache.kv_append(x, x[:, :, :2], x[:, :, 2:], k, v, ints(3, 11), torch.empty(2, 0, dtype=torch.int32, device="cuda"), c, c)
+    ended()
+    assert out.shape == (2, 0, 4, 64) and bool((k == 1).all()) and bool((v == 1).all())
