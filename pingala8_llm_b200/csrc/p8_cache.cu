@@ -169,6 +169,7 @@ struct EvictArgs {
     long long ss[2][4], ds[2][4];  // bytes: layer, sequence, head, slot
     long long slots;
     int batch, heads, budget, sinks, recent, row_bytes;
+    int per_row;  // step 2: blocks of a row (all rows' blocks in one dimension of the grid: there may be more than 65,535 rows)
 };
 
 __device__ __forceinline__ uint32_t mass_key(float m) {  // larger mass, larger key; NaN as -infinity, -0 as +0
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(1024, 2) k_evict_select(const EvictArgs a) {
 // step 2, into other buffers: every row moves on its own, 16 bytes a thread. Bound by HBM (288 rows x 2,048 kept of 16,384
 // slots, 604 MB: 105 to 110 us of the call's 135, 5.6 TB/s).
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
-    const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    const int row = blockIdx.x / a.per_row, block = blockIdx.x - row * a.per_row, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     after_prior();  // every block: what follows in the stream waits for this launch alone
     const int len = a.lens[b];
     if (len < 0 || len > a.slots) return;
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
     const char *s0 = a.src[0] + layer * a.ss[0][0] + b * a.ss[0][1] + h * a.ss[0][2], *s1 = a.src[1] + layer * a.ss[1][0] + b * a.ss[1][1] + h * a.ss[1][2];
     char *d0 = a.dst[0] + layer * a.ds[0][0] + b * a.ds[0][1] + h * a.ds[0][2], *d1 = a.dst[1] + layer * a.ds[1][0] + b * a.ds[1][1] + h * a.ds[1][2];
     const int unit = 16 * (threadIdx.x % per);
-    const int first = blockIdx.x * rows * 4 + threadIdx.x / per;
+    const int first = block * rows * 4 + threadIdx.x / per;
     uint4 x[4], y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -343,13 +344,13 @@ __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
             *reinterpret_cast<uint4 *>(d1 + i * a.ds[1][3] + unit) = y[j];
         }
     }
-    for (int i = blockIdx.x * rows * 4 + threadIdx.x; i < min(keep, (int)(blockIdx.x + 1) * rows * 4); i += 256)
+    for (int i = block * rows * 4 + threadIdx.x; i < min(keep, (block + 1) * rows * 4); i += 256)
         a.mass_out[layer * a.mos[0] + b * a.mos[1] + h * a.mos[2] + i] = a.mass[layer * a.ms[0] + b * a.ms[1] + h * a.ms[2] + kept[i]];
 }
 
 // step 2 in place: kept[i] >= i, so a block that goes up through a range of the row's bytes (64 of them: its columns
 // belong to no other block), reads a chunk of sources before it writes their destinations, and reads the next chunk
-// (sources at or behind every destination written so far) meanwhile, loses nothing. blockIdx.z 0 / 1: keys / values,
+// (sources at or behind every destination written so far) meanwhile, loses nothing. blockIdx.y 0 / 1: keys / values,
 // 2: the masses.
 template <typename U>
 __device__ __forceinline__ void evict_slide(const char *base, long long stride, int per, int keep, const int *kept) {
@@ -383,18 +384,18 @@ __device__ __forceinline__ void evict_slide(const char *base, long long stride, 
 }
 
 __global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
-    const int row = blockIdx.y, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
+    const int row = blockIdx.x / a.per_row, block = blockIdx.x - row * a.per_row, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     after_prior();
     const int len = a.lens[b];
     if (len <= a.budget || len > a.slots) return;
     const int *kept = a.kept + (long long)row * a.budget;
-    const int z = blockIdx.z;
+    const int z = blockIdx.y;
     if (z == 2) {
-        if (blockIdx.x == 0)
+        if (block == 0)
             evict_slide<float>(reinterpret_cast<const char *>(a.mass + layer * a.ms[0] + b * a.ms[1] + h * a.ms[2]), 4, 1, a.budget, kept);
         return;
     }
-    evict_slide<uint4>(a.src[z] + layer * a.ss[z][0] + b * a.ss[z][1] + h * a.ss[z][2] + 64 * blockIdx.x, a.ss[z][3], 4, a.budget, kept);
+    evict_slide<uint4>(a.src[z] + layer * a.ss[z][0] + b * a.ss[z][1] + h * a.ss[z][2] + 64 * block, a.ss[z][3], 4, a.budget, kept);
 }
 
 // ----------------------------------------------------------------------------------------------------------------
@@ -731,7 +732,9 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     k.slots = s->slots; k.batch = (int)s->batch; k.heads = (int)s->heads;
     k.budget = (int)a->budget; k.sinks = (int)a->sinks; k.recent = (int)a->recent; k.row_bytes = (int)s->width * es;
     const int64_t rows = s->layers * s->batch * s->heads;
-    if (rows > 65535) return P8_ERR_UNSUPPORTED;
+    const int chunk = 4 * (256 / (k.row_bytes / 16));
+    k.per_row = same ? k.row_bytes / 64 : (int)((a->budget + chunk - 1) / chunk);
+    if (rows * k.per_row > INT32_MAX) return P8_ERR_UNSUPPORTED;
     cudaStream_t st = (cudaStream_t)stream;
     // Keys go to shared memory as far as a middle can be long. Beside the kernel's own 22 KB, more than 24 KB needs the limit
     // raised; on every call, since it is the device's.
@@ -739,9 +742,7 @@ p8_status p8_kv_evict(const p8_kv *s, const p8_kv *d, const p8_kv_evict_args *a,
     const int smem = (int)std::min<int64_t>(std::max<int64_t>(most, 0), kSelPiece) * 4;
     if (smem > 24 * 1024 && cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelPiece * 4) != cudaSuccess) return P8_ERR_CUDA;
     if (launch_after(k_evict_select, dim3((unsigned int)rows), dim3(1024), (size_t)smem, st, k) != cudaSuccess) return P8_ERR_CUDA;
-    const int chunk = 4 * (256 / (k.row_bytes / 16));
-    const dim3 grid = same ? dim3((unsigned int)(k.row_bytes / 64), (unsigned int)rows, 3) : dim3((unsigned int)((a->budget + chunk - 1) / chunk), (unsigned int)rows);
-    return done(launch_after(same ? k_evict_slide : k_evict_copy, grid, dim3(256), 0, st, k));
+    return done(launch_after(same ? k_evict_slide : k_evict_copy, dim3((unsigned int)(rows * k.per_row), same ? 3 : 1), dim3(256), 0, st, k));
 }
 
 p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream) {

@@ -10,7 +10,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 import pingala8_llm_b200 as p8  # noqa: E402
-from test_cache_ops import ARG, PTR, accept_args, append_args, attn_args, evict_args, kv, mass_args  # noqa: E402
+from test_cache_ops import ARG, PTR, UNSUPPORTED, accept_args, append_args, attn_args, evict_args, kv, mass_args  # noqa: E402
 
 if torch.cuda.is_available():
     pytest.skip("addresses that nothing may read: not where a launch would reach a GPU", allow_module_level=True)
@@ -196,3 +196,17 @@ def test_append_of_no_tokens_is_a_call_that_does_nothing():
     nothing = dict(tokens=0, q=0, k=0, v=0, out=0, pos=0)
     assert append(**nothing) == 0 and append(**nothing, lens=0, cos=0, sin=0) == 0
     assert append(kv(width=96), **nothing) == ARG and append(**nothing, heads=3) == ARG and append(**{**nothing, "tokens": -1}) == ARG
+
+
+def test_evict_takes_more_rows_than_a_grid_is_high():
+    many = dict(layers=80, batch=128, heads=8, slots=8)
+    st = tuple(64 * x for x in (128 * 8 * 8, 8 * 8, 8, 1))
+    src, dst = kv(k=1 << 32, v=2 << 32, ks=st, vs=st, **many), kv(k=3 << 32, v=4 << 32, ks=st, vs=st, **many)
+    far = dict(mass=5 << 32, ms=(128 * 64, 64, 8), os=(128 * 64, 64, 8), kept=6 << 32, sinks=1, recent=1, budget=4)
+    assert evict(src, **far, out=5 << 32) not in (ARG, UNSUPPORTED) and evict(src, dst, **far, out=7 << 32) not in (ARG, UNSUPPORTED)
+    # 2^30 rows of 64 blocks are more than a grid has at all
+    huge = dict(layers=1024, batch=4096, heads=256, slots=2048)
+    st = tuple(64 * x for x in (4096 * 256 * 2048, 256 * 2048, 2048, 1))
+    src, dst = kv(k=1 << 48, v=1 << 52, ks=st, vs=st, **huge), kv(k=1 << 53, v=1 << 54, ks=st, vs=st, **huge)
+    far = dict(mass=1 << 55, ms=(4096 * 256 * 2048, 256 * 2048, 2048), os=(4096 * 256 * 2048, 256 * 2048, 2048), kept=1 << 56, budget=2048)
+    assert evict(src, dst, **far, out=1 << 57) == UNSUPPORTED

@@ -194,3 +194,33 @@ def test_append_of_no_tokens():
     out = cache.kv_append(x, x[:, :, :2], x[:, :, 2:], k, v, ints(3, 11), torch.empty(2, 0, dtype=torch.int32, device="cuda"), c, c)
     ended()
     assert out.shape == (2, 0, 4, 64) and bool((k == 1).all()) and bool((v == 1).all())
+
+
+@pytest.mark.parametrize("place", ["in place", "other buffers"])
+def test_evict_of_very_many_rows(place):
+    """80 layers x 128 sequences x 8 heads: the heaviest of the middle slots beside the first and the last"""
+    g = gen(8)
+    N, B, hk, cap, D, budget = 80, 128, 8, 6, 64, 3
+    k, v = randn(g, N, B, hk, cap, D, dtype=torch.bfloat16), randn(g, N, B, hk, cap, D, dtype=torch.bfloat16)
+    m = torch.rand(N, B, hk, cap, device="cuda", generator=g)
+    lens = torch.randint(0, cap + 1, (B,), device="cuda", generator=g).int()
+    at = torch.arange(cap, device="cuda")
+    mid = (at >= 1) & (at < lens[:, None] - 1)
+    best = torch.where(mid[None, :, None], m, -1.0).argmax(-1)
+    n = lens[None, :, None].expand(N, B, hk)
+    kept = torch.stack([torch.zeros_like(best), torch.where(n > budget, best, 1), torch.where(n > budget, n - 1, 2)], -1)
+    kept = torch.where(torch.arange(budget, device="cuda") < n.clamp(max=budget)[..., None], kept, -1)
+    x = [k.clone(), v.clone(), m.clone()]
+    out = {} if place == "in place" else dict(k_out=torch.full_like(k[..., :budget, :], 3.0).contiguous(), v_out=torch.full_like(v[..., :budget, :], 3.0).contiguous(),
+                                              mass_out=torch.full_like(m[..., :budget], 3.0).contiguous())
+    new, got = cache.kv_evict(*x, lens, budget, 1, 1, **out)
+    ended()
+    assert torch.equal(new, lens.clamp(max=budget)) and torch.equal(got.long(), kept)
+    y = list(out.values()) or x
+    live, take = kept >= 0, kept.clamp(min=0)
+    for a, b in ((k, y[0]), (v, y[1])):
+        want = a.gather(3, take[..., None].expand(*take.shape, D))
+        rest = torch.full_like(want, 3.0) if out else a[..., :budget, :]
+        assert torch.equal(b[..., :budget, :], torch.where(live[..., None], want, rest))
+        assert out or torch.equal(b[..., budget:, :], a[..., budget:, :])
+    assert torch.equal(y[2][..., :budget], torch.where(live, m.gather(3, take), torch.full_like(m[..., :budget], 3.0) if out else m[..., :budget]))
