@@ -257,6 +257,8 @@ class TreeDecoder:
     and the heaviest of the others stay, per layer and head. Tokens keep the positions they had."""
 
     def __init__(self, model, max_len, dtype=torch.float16, budget=None, sinks=4, recent=64, slack=128):
+        if budget is not None and (budget < 1 or min(sinks, recent, slack) < 0 or sinks + recent > budget):
+            raise ValueError(f"a budget of {budget} slots with {sinks} first, {recent} last ones and a slack of {slack}: budget >= sinks + recent, none negative, budget >= 1")
         c, dev = model.c, model.device
         self.m, self.budget, self.sinks, self.recent, self.slack = model, budget, sinks, recent, slack
         slots = max_len if budget is None else min(max_len, budget + slack + cache.TREE_MAX)

@@ -210,3 +210,17 @@ def test_evict_takes_more_rows_than_a_grid_is_high():
     src, dst = kv(k=1 << 48, v=1 << 52, ks=st, vs=st, **huge), kv(k=1 << 53, v=1 << 54, ks=st, vs=st, **huge)
     far = dict(mass=1 << 55, ms=(4096 * 256 * 2048, 256 * 2048, 2048), os=(4096 * 256 * 2048, 256 * 2048, 2048), kept=1 << 56, budget=2048)
     assert evict(src, dst, **far, out=1 << 57) == UNSUPPORTED
+
+
+def test_a_decoder_refuses_a_budget_that_its_first_eviction_could_not_keep():
+    from types import SimpleNamespace
+
+    from pingala8_llm_b200 import decode
+
+    model = SimpleNamespace(c=decode.ModelConfig("small", 2, 64, 128, 2, 1, 64, 100, 1e4, False), device=torch.device("cpu"), nl=2)
+    for bad in (dict(budget=64), dict(budget=0, sinks=0, recent=0), dict(budget=-1, sinks=0, recent=0), dict(budget=100, sinks=-1), dict(budget=100, recent=-1), dict(budget=100, slack=-1),
+                dict(budget=100, sinks=50, recent=51)):
+        with pytest.raises(ValueError, match="budget"):
+            decode.TreeDecoder(model, 500, **bad)
+    assert decode.TreeDecoder(model, 500, budget=68, sinks=4, recent=64, slack=0).k.shape == (2, 1, 1, 132, 64)
+    assert decode.TreeDecoder(model, 500).mass is None
