@@ -19,7 +19,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import cache, synth
+from . import synth
 from .ops import P8Tensor, group_workspace_size, mul_mat_group, mul_mat_vec_group
 
 
@@ -259,9 +259,12 @@ class TreeDecoder:
     def __init__(self, model, max_len, dtype=torch.float16, budget=None, sinks=4, recent=64, slack=128):
         if budget is not None and (budget < 1 or min(sinks, recent, slack) < 0 or sinks + recent > budget):
             raise ValueError(f"a budget of {budget} slots with {sinks} first, {recent} last ones and a slack of {slack}: budget >= sinks + recent, none negative, budget >= 1")
+        from . import cache  # its calls are a module built against torch's headers, which Model does without
+
+        self._cache = cache
         c, dev = model.c, model.device
         self.m, self.budget, self.sinks, self.recent, self.slack = model, budget, sinks, recent, slack
-        slots = max_len if budget is None else min(max_len, budget + slack + cache.TREE_MAX)
+        slots = max_len if budget is None else min(max_len, budget + slack + self._cache.TREE_MAX)
         self.k, self.v = (torch.zeros(model.nl, 1, c.kv_heads, slots, c.head_dim, dtype=dtype, device=dev) for _ in range(2))
         self.mass = None if budget is None else torch.zeros(model.nl, 1, c.kv_heads, slots, device=dev)
         self.cos, self.sin = rope_tables(c, max_len, dev)
@@ -285,9 +288,9 @@ class TreeDecoder:
             t = layer["t"]
             q, k, v = mul_mat_group([t["q"], t["k"], t["v"]], x, norm_weight=layer["attn_norm"], eps=c.eps)
             qn, kn = layer["qk_norm"] if c.qk_norm else (None, None)
-            q = cache.kv_append(q.view(1, T, c.heads, c.head_dim), k.view(1, T, c.kv_heads, c.head_dim), v.view(1, T, c.kv_heads, c.head_dim),
-                                self.k[L], self.v[L], self.lens, pos, self.cos, self.sin, q_norm=qn, k_norm=kn, eps=c.eps)
-            a, lse = cache.tree_attention(q, self.k[L], self.v[L], self.lens, mask=mask)
+            q = self._cache.kv_append(q.view(1, T, c.heads, c.head_dim), k.view(1, T, c.kv_heads, c.head_dim), v.view(1, T, c.kv_heads, c.head_dim),
+                                      self.k[L], self.v[L], self.lens, pos, self.cos, self.sin, q_norm=qn, k_norm=kn, eps=c.eps)
+            a, lse = self._cache.tree_attention(q, self.k[L], self.v[L], self.lens, mask=mask)
             if self.budget is not None:
                 self.seen.append((q, lse))
             h = x + t["o"].mul_mat(a.view(T, -1).float())
@@ -300,20 +303,20 @@ class TreeDecoder:
         """n tokens of the last forward() belong to the sequence now"""
         if self.budget is not None:
             for L, (q, lse) in enumerate(self.seen):
-                cache.attention_mass(q, lse, self.k[L], self.lens, self.mass[L], rows=rows, counts=counts)
+                self._cache.attention_mass(q, lse, self.k[L], self.lens, self.mass[L], rows=rows, counts=counts)
         self.lens = new_lens
         self.used += n
         self.position += n
         if self.budget is not None and self.used > self.budget + self.slack:
-            self.lens, _ = cache.kv_evict(self.k, self.v, self.mass, self.lens, self.budget, self.sinks, self.recent)
+            self.lens, _ = self._cache.kv_evict(self.k, self.v, self.mass, self.lens, self.budget, self.sinks, self.recent)
             self.used = self.budget
 
     def prefill(self, tokens):
         """a prompt, int64 [n], in passes of up to 64 tokens; returns the last token's logits"""
-        for i in range(0, tokens.numel(), cache.TREE_MAX):
-            part = tokens[i:i + cache.TREE_MAX]
+        for i in range(0, tokens.numel(), self._cache.TREE_MAX):
+            part = tokens[i:i + self._cache.TREE_MAX]
             n = part.numel()
-            mask, depth = cache.tree_plan(torch.arange(-1, n - 1, device=tokens.device))
+            mask, depth = self._cache.tree_plan(torch.arange(-1, n - 1, device=tokens.device))
             logits = self.forward(part, mask, depth)
             self._grow(self.lens + n, n)
         return logits[-1]
@@ -321,10 +324,10 @@ class TreeDecoder:
     def step(self, tokens, parents):
         """One pass over a drafted tree: tokens int64 [T] (token 0 the last known one, not yet in the cache), parents int32
         [T]. Returns the confirmed tokens and the model's next one, int64 [1..T]; the last of them is the next tree's root."""
-        mask, depth = cache.tree_plan(parents)
+        mask, depth = self._cache.tree_plan(parents)
         self.logits = self.forward(tokens, mask, depth)
         target = torch.argmax(self.logits, dim=-1)
-        acc = cache.tree_accept(tokens[None].contiguous(), parents[None].contiguous(), target[None], self.k, self.v, self.lens)
+        acc = self._cache.tree_accept(tokens[None].contiguous(), parents[None].contiguous(), target[None], self.k, self.v, self.lens)
         n = int(acc.accepted[0])
         path = acc.path[0, :n].long()
         self.path = path
@@ -343,7 +346,7 @@ class TreeDecoder:
         out, passes = [history[-1]], 0
         while len(out) < n_new:
             tokens, parents = draft(history)
-            room = min(len(tokens), cache.TREE_MAX, n_new - len(out))
+            room = min(len(tokens), self._cache.TREE_MAX, n_new - len(out))
             tokens, parents = tokens[:room], parents[:room]  # a child comes after its parent: the rest is still a tree
             got = self.step(torch.tensor(tokens, device=prompt.device), torch.tensor(parents, dtype=torch.int32, device=prompt.device)).tolist()
             out += got

@@ -224,3 +224,22 @@ def test_a_decoder_refuses_a_budget_that_its_first_eviction_could_not_keep():
             decode.TreeDecoder(model, 500, **bad)
     assert decode.TreeDecoder(model, 500, budget=68, sinks=4, recent=64, slack=0).k.shape == (2, 1, 1, 132, 64)
     assert decode.TreeDecoder(model, 500).mass is None
+
+
+def test_the_decoder_without_the_cache_operators_module():
+    """decode and its Model import where _cache_calls was not built; TreeDecoder says what is missing"""
+    import subprocess
+
+    code = """
+import sys
+sys.modules["pingala8_llm_b200._cache_calls"] = None
+from pingala8_llm_b200 import decode
+assert decode.Model and decode.lookup_draft([1, 2, 3]) == ([3], [-1])
+try:
+    decode.TreeDecoder(None, 10)
+except ImportError as e:
+    assert "pingala8_llm_b200.build" in str(e)
+    print("named")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    assert subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, check=True).stdout == "named\n"
