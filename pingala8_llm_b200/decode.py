@@ -338,7 +338,7 @@ class TreeDecoder:
         """greedy: prompt int64 [n], then n_new tokens; draft(history) -> (tokens, parents) of the tree to try, whose token 0 is
         the last of `history` (a list of ints); None: lookup_draft. Returns (tokens [n_new], passes)."""
         draft = draft or lookup_draft
-        if prompt.numel() < 1 or prompt.numel() + n_new > self.max_len:
+        if prompt.numel() < 1 or n_new < 0 or prompt.numel() + n_new > self.max_len:
             raise ValueError(f"{prompt.numel()} + {n_new} tokens do not fit max_len {self.max_len}")
         self.reset()
         history = prompt.tolist()
@@ -352,7 +352,7 @@ class TreeDecoder:
             out += got
             history += got
             passes += 1
-        return torch.tensor(out[:n_new], device=prompt.device), passes
+        return torch.tensor(out[:n_new], dtype=torch.int64, device=prompt.device), passes
 
 
 def lookup_draft(history, width=4, depth=7):

@@ -147,3 +147,12 @@ def test_right_wrong_and_no_drafts(model):
     toks, passes = d.generate(prompt, 6, draft=bad)
     assert toks.tolist() == plain[:6].tolist() and passes == 5
     assert device_error() == 0
+
+
+def test_generate_nothing(model):
+    d = decode.TreeDecoder(model, 60, dtype=torch.float16)
+    toks, passes = d.generate(prompt_of(20, 5), 0)
+    assert toks.shape == (0,) and toks.dtype == torch.int64 and passes == 0
+    for n in (-1, 41):
+        with pytest.raises(ValueError, match="max_len"):
+            d.generate(prompt_of(20, 5), n)
