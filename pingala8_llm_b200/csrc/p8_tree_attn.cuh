@@ -1617,9 +1617,13 @@ size_t tree_attn_workspace(const p8_kv *c, int64_t tokens, int64_t heads) {  // 
     return (size_t)2 * attn_ctas(c, rows, cut) * cut.rblock * ((size_t)c->width * 4 + 8);
 }
 
-// Rows up to which k_attn_join loads 16 parts at once, not 8: 2,048 rows of 131,000 slots take 154 us with 16 and 161 with
-// 8 (the whole call), 5,376 rows of 24 sequences 82 with 16 and 79 with 8.
-constexpr long long kFewRows = 2048;
+// k_attn_join with 16 parts a round has 107 (64 columns: 72) registers a thread, so 2 (3) blocks of eight rows fit an SM; with
+// 8 parts, 64 (48). Sixteen are used as long as all blocks run at once, 2,368 (3,552) rows of 148 SMs; beyond, the blocks behind the
+// first wave cost more than the loads save. Times of a call, 16 against 8 parts, 16 bit, 128 columns: 256 rows of 65,000 slots
+// 55.3 : 57.9 us, 2,304 rows of them 117.4 : 119.6; 2,560 rows of 3,000 slots 32.9 : 29.9, 16,384 rows of 2,000 slots 76.1 :
+// 66.3. 64 columns: 2,560 rows of 3,000 slots 24.1 : 25.0, 3,584 rows of 4,000 slots 44.4 : 43.0.
+template <int D>
+constexpr int kJoinBlocks = D == 128 ? 2 : 3;
 template <typename T, int D, typename K>
 p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, const AttnArgs &a, void *ws, cudaStream_t st) {
     CUtensorMap mk, mv;
@@ -1631,9 +1635,8 @@ p8_status run_attn(K kernel, int threads, int smem, float lift, const p8_kv *c, 
     float2 *ml = reinterpret_cast<float2 *>(po + (size_t)2 * ctas * cut.rblock * D);
     if (launch_after(kernel, dim3(ctas), dim3(threads), (size_t)smem, st, a, mk, mv, po, ml) != cudaSuccess) return P8_ERR_CUDA;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
-    const bool few = rows <= kFewRows;
     const dim3 grid((unsigned int)((rows + 7) / 8));
-    const auto join = few ? k_attn_join<T, D, 16> : k_attn_join<T, D, 8>;
+    const auto join = rows <= 8ll * kJoinBlocks<D> * sm_count() ? k_attn_join<T, D, 16> : k_attn_join<T, D, 8>;
     return launch_after(join, grid, dim3(256), 0, st, a, cut, ctas, lift, (const float *)po, (const float2 *)ml) == cudaSuccess ? P8_OK : P8_ERR_CUDA;
 }
 template <typename T, int D>

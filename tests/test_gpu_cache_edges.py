@@ -224,3 +224,26 @@ def test_evict_of_very_many_rows(place):
         assert torch.equal(b[..., :budget, :], torch.where(live[..., None], want, rest))
         assert out or torch.equal(b[..., budget:, :], a[..., budget:, :])
     assert torch.equal(y[2][..., :budget], torch.where(live, m.gather(3, take), torch.full_like(m[..., :budget], 3.0) if out else m[..., :budget]))
+
+
+@pytest.mark.parametrize("D,B", [(128, 37), (128, 38), (64, 55), (64, 56)])
+def test_split_sequences_on_either_side_of_the_joins_row_counts(D, B):
+    """64 rows a sequence: 2,368 rows are the last that 148 SMs add up at once with 128 columns, 3,520 of 3,552 with 64"""
+    g = gen(B)
+    T, H, hk, n = 16, 4, 1, 900
+    k, v = randn(g, B, hk, n + T, D, dtype=torch.float16), randn(g, B, hk, n + T, D, dtype=torch.float16)
+    q = randn(g, B, T, H, D, dtype=torch.float16)
+    lens = (n - 7 * torch.arange(B, device="cuda")).int()
+    out, lse = cache.tree_attention(q, k, v, lens)
+    ended()
+    z = torch.einsum("bthd,bsd->bths", q.double(), k[:, 0].double()) / D ** 0.5
+    at = torch.arange(n + T, device="cuda") - lens[:, None, None]
+    z = z.masked_fill((at > torch.arange(T, device="cuda")[None, :, None])[:, :, None], -float("inf"))
+    p, want = torch.softmax(z, -1), torch.logsumexp(z, -1)
+    exact, size = p @ v[:, :1].double(), p @ v[:, :1].double().abs()
+    # per value: the weights' rounding to fp16, two errors of a score, the sum's; then the result's rounding
+    e, u = 2.0 ** -23, 2.0 ** -11
+    ds = (D + 16) * e * float((q.float().norm(dim=-1).max() * k.float().norm(dim=-1).max())) / D ** 0.5
+    acc = (68 + 8 * 31) * e
+    assert float(((out.double() - exact).abs() - ((u + 2 * ds + acc) * size + u * exact.abs())).max()) <= 0
+    assert float((lse.double() - want).abs().max()) <= ds + acc + e * float(want.abs().max())
