@@ -295,6 +295,7 @@ PyObject *workspace_(PyObject *const *a, Py_ssize_t n) {
     if (n != 3) refuse("attention_workspace takes 3 arguments");
     const Tensor &k = tensor(a[0], "k_cache");
     const Cache c = cache(k, &k, false);
+    const On on(c);  // the size goes by the device's SMs
     return PyLong_FromSize_t(g_p8.attn_workspace(&c.c, integer(a[1]), integer(a[2])));
 }
 PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) {
