@@ -135,29 +135,26 @@ __device__ __forceinline__ Share find_share(const AttnArgs &a, Cut cut, int lane
 }
 
 // Waits give up after `ns` (the kernel's results are then invalid and bit 128 is set); from then on every wait of the CTA that
-// is not over at its first look returns false at once. What follows from that goes by the role. Warps that start something
-// asynchronous (TMA loads, cp.async, MMAs) start nothing more and leave their loops: a stage that was not handed over may
-// still be written or read, and its barrier may be inside a phase. Before they go to the CTA's end they wait for all that they
-// did start (settle, which does not ask whether something gave up). The others run through to the end and meet there.
+// is not over within one look returns false. What follows from that goes by the role. A thread that starts something
+// asynchronous (TMA loads, cp.async, MMAs) starts nothing more: a stage that was not handed over may still be written or read,
+// and its barrier may be inside a phase. Before it goes to the CTA's end it waits for all that it did start (settle, which does
+// not ask whether something gave up). The others run through to the end and meet there. Each thread goes by its own waits, also in a
+// warp of which one issues: votes between them cost 2 % of the attention.
 struct Waits {
     volatile int *gave_up;
     unsigned int ns;
     // whether the barrier's phase is over
     __device__ bool operator()(uint64_t *bar, uint32_t parity) const {
         if (mbar_test_wait(bar, parity)) return true;
+        if (ns && mbar_try_wait(bar, parity)) return true;  // stays for up to about 4 us
         if (*gave_up) return false;
         if (ns && poll(bar, parity, ns, gave_up)) return true;
         *gave_up = 1;
         atomicOr(&g_cache_error, kErrWait);
         return false;
     }
-    // For a whole warp that starts something behind it: true for all lanes or for none. `arrivals`: the phase ends by
-    // those of roles that go on arriving after something gave up.
-    __device__ bool warp(uint64_t *bar, uint32_t parity, bool arrivals = false) const {
-        bool ok = (*this)(bar, parity);
-        if (arrivals) ok = ok && !*gave_up;
-        return __all_sync(0xffffffffu, ok);
-    }
+    // the same, where the phase is ended by roles that go on arriving after something gave up
+    __device__ bool arrivals(uint64_t *bar, uint32_t parity) const { return (*this)(bar, parity) && !*gave_up; }
     // for what this role has started and what ends by itself
     __device__ void settle(uint64_t *bar, uint32_t parity) const {
         if (mbar_try_wait(bar, parity) || poll(bar, parity, kWaitNs, nullptr)) return;
@@ -420,7 +417,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
             for (int t = w.ta; on && t < w.tb; ++t)
                 for (int z = 0; z < 2; ++z, ++n) {
                     const int st = n % NST;
-                    if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1))) break;
+                    if (!(on = wait(b_empty + st, (n / NST & 1) ^ 1))) break;
                     if (lane == 0) {
                         mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -431,12 +428,12 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
             w.advance();
         }
         // nothing may be in flight into this CTA's shared memory when it ends
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; lane == 0 && i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
     } else if (warp == 11) {  // ---------------------------------------------------------- queries, a segment ahead where there is room
         uint32_t seg = 0;
         while (w.next()) {
             const int qb = seg % NQ;
-            if (!wait.warp(b_qfree + qb, (seg / NQ & 1) ^ 1)) break;
+            if (!__all_sync(0xffffffffu, wait(b_qfree + qb, (seg / NQ & 1) ^ 1))) break;
             load_q<T, D>(sq + qb * (128 * D * 2), a, w.b, w.head(), w.row0(), w.n * a.group, TWO ? 2 : 1, a.scale < 0.f ? 0x80008000u : 0u, lane);
             fence_proxy_async();
             mbar_arrive(b_q + qb);
@@ -447,20 +444,20 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
         const int s = __shfl_sync(0xffffffffu, warp, 0) - 9;
         constexpr uint32_t id_s = idesc_of<T>(kStep, false), id_o = idesc_of<T>(D, true);
         uint32_t base = 0, seg = 0, step = 0;  // ring position and the stream's step count at the segment's start
-        bool on = true;
-        while (on && w.next()) {
+        bool on = true;  // (what the thread waited for has come)
+        while (w.next()) {
             const int ns = (w.tb - w.ta) * PER, qb = seg % NQ;
             const uint64_t dq = desc_rows(smem_u32(sq) + (TWO ? s : qb) * (128 * D * 2));
-            on = wait.warp(b_q + qb, seg / NQ & 1);
+            on = wait(b_q + qb, seg / NQ & 1) && on;
             auto scores = [&](int k) {
                 const uint32_t at = base + 2 * (k / PER), st = at % NST, g = step + k, buf = g & 1;
                 bool ok = g < 2 || wait(&b_pv[s][buf], ((g - 2) / 2) & 1);  // the P that the buffer held is read
                 ok = wait(b_full + st, at / NST & 1) && ok;
-                if (!__all_sync(0xffffffffu, ok)) return false;
+                on = on && ok;
                 tc_fence_after();
                 const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage) + (TWO ? k & 1 : s) * (kStep * 128));
                 const uint32_t to = tmem + 128 * s + 64 * buf;
-                if (elect_one()) {
+                if (elect_one() && on) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         constexpr uint32_t kUnit = 16;  // of a descriptor's address
@@ -472,21 +469,20 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     umma_commit(&b_s[s][buf]);
                 }
                 __syncwarp();
-                return true;
             };
-            on = on && scores(0) && (ns < 2 || scores(1));
-            for (int k = 0; on && k < ns; ++k) {
+            scores(0);
+            if (ns > 1) scores(1);
+            for (int k = 0; k < ns; ++k) {
                 const uint32_t at = base + 2 * (k / PER) + 1, st = at % NST, buf = (step + k) & 1, use = (step + k) / 2 & 1;
-                on = wait(&b_p[s][buf], use);
+                on = wait(&b_p[s][buf], use) && on;
                 on = wait(b_full + st, at / NST & 1) && on;
-                if (!(on = __all_sync(0xffffffffu, on))) break;
                 tc_fence_after();
                 const int half = TWO ? k & 1 : s;
                 const uint64_t dv = desc_cols(smem_u32(ring + st * S_::kStage) + half * (kStep * 128));
                 const uint32_t to = tmem + 256 + 128 * s, from = tmem + 128 * s + 64 * buf;
                 // slots behind the drafted tokens are not multiplied, but for the rest of a group of 16
                 const int groups = live_groups(w, w.ta + k / PER, half);
-                if (elect_one()) {
+                if (elect_one() && on) {
                     if (groups == kStep / 16) {
 #pragma unroll
                         for (int kk = 0; kk < kStep / 16; ++kk) mma_ts(to, from + 8 * kk, dv + kk * 128, id_o, (k | kk) != 0);
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
                     umma_commit(&b_pv[s][buf]);
                 }
                 __syncwarp();
-                if (k + 2 < ns) on = scores(k + 2);
+                if (k + 2 < ns) scores(k + 2);
             }
             base += 2 * (w.tb - w.ta);
             step += ns;
@@ -845,8 +841,8 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
         while (on && w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST;
-                if (n == 2 && w.opens && w.n * a.gc > 64) on = wait.warp(&b_q, 0);  // the first query rows before the rest of the ring: 0.7 us
-                if (!(on = on && wait.warp(b_empty + st, (n / NST & 1) ^ 1))) break;
+                if (n == 2 && w.opens && w.n * a.gc > 64) on = wait(&b_q, 0);  // the first query rows before the rest of the ring: 0.7 us
+                if (!(on = on && wait(b_empty + st, (n / NST & 1) ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -855,28 +851,28 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
             }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; lane == 0 && i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
     } else if (warp == 17) {  // ----------------------------------------------------------- MMAs
         uint32_t n = 0, seg = 0, held = 0;  // (bit: the phase of b_free)
         bool on = true;
-        while (on && w.next()) {
+        while (w.next()) {
             const int rows = w.n * a.gc;
-            on = wait.warp(&b_q, seg & 1);
+            on = wait(&b_q, seg & 1) && on;
             tc_fence_after();
-            for (int t = w.ta; on && t < w.tb; ++t, ++n) {
+            for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST, s = (t - w.ta) % kTurns;
-                on = wait.warp(b_full + st, n / NST & 1);
-                for (int r0 = 0; on && r0 < rows; r0 += 256) {
+                on = wait(b_full + st, n / NST & 1) && on;
+                for (int r0 = 0; r0 < rows; r0 += 256) {
                     const int all = min(rows - r0, 256), mid = min((all + 63) / 64 * 32, all);
                     for (int half = 0; half < 2; ++half) {
                         const int from = half ? mid : 0, cols = ((half ? all : mid) - from + 15) / 16 * 16, g = SPLIT ? 2 * s + half : s;
                         if (!cols) break;
-                        if (!(on = wait.warp(b_free + g, (held >> g & 1) ^ 1))) break;
+                        on = wait(b_free + g, (held >> g & 1) ^ 1) && on;
                         held ^= 1u << g;
                         tc_fence_after();
                         const uint64_t dk = desc_rows(smem_u32(ring + st * S_::kStage)), dq = desc_rows(smem_u32(sq) + (r0 + from) * 128);
                         const uint32_t id = idesc_of<T>(cols, false), to = tmem + 128 * g;
-                        if (elect_one()) {
+                        if (elect_one() && on) {
 #pragma unroll
                             for (int kk = 0; kk < D / 16; ++kk)
                                 mma_ss(to, dk + ((kk / 4) * 16384 + (kk % 4) * 32) / 16, dq + ((kk / 4) * kAtom + (kk % 4) * 32) / 16, id, kk != 0);
@@ -1159,7 +1155,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
             for (int t = w.ta; on && t < w.tb; ++t)
                 for (int z = 0; z < 2; ++z, ++n) {
                     const int st = n % NST;
-                    if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1, true))) break;
+                    if (!(on = wait.arrivals(b_empty + st, (n / NST & 1) ^ 1))) break;
                     if (lane == 0) {
                         mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -1169,7 +1165,7 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
                 }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; lane == 0 && i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
         return;
     }
     const int group = warp / 4, rt = group % RT, ns = group / RT, wq = warp % 4, g = lane / 4, t = lane % 4;
@@ -1435,7 +1431,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
         while (on && w.next()) {
             for (int t = w.ta; t < w.tb; ++t, ++n) {
                 const int st = n % NST;
-                if (!(on = wait.warp(b_empty + st, (n / NST & 1) ^ 1, true))) break;
+                if (!(on = wait.arrivals(b_empty + st, (n / NST & 1) ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(b_full + st, S_::kStage);
 #pragma unroll
@@ -1444,7 +1440,7 @@ __global__ void __launch_bounds__(F32Mass<D>::kThreads, 1) k_attn_mass_f32(const
             }
             w.advance();
         }
-        for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
+        for (uint32_t i = n > NST ? n - NST : 0; lane == 0 && i < n; ++i) wait.settle(b_full + i % NST, i / NST & 1);
         return;
     }
     auto sync_all = [&] { asm volatile("bar.sync 1, %0;" ::"n"(ALL) : "memory"); };
