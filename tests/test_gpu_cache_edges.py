@@ -247,3 +247,37 @@ def test_split_sequences_on_either_side_of_the_joins_row_counts(D, B):
     acc = (68 + 8 * 31) * e
     assert float(((out.double() - exact).abs() - ((u + 2 * ds + acc) * size + u * exact.abs())).max()) <= 0
     assert float((lse.double() - want).abs().max()) <= ds + acc + e * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dtype,T,H,hk,D,cap", [(torch.bfloat16, 3, 4, 2, 64, 60), (torch.float32, 2, 8, 1, 64, 90), (torch.float16, 40, 4, 1, 64, 75)])
+def test_as_many_sequences_as_there_may_be(dtype, T, H, hk, D, cap):
+    """4,096 sequences, padded: attention and masses of all against 64 bits"""
+    g = gen(T)
+    B, G = 4096, H // hk
+    k, v = randn(g, B, hk, cap, D, dtype=dtype), randn(g, B, hk, cap, D, dtype=dtype)
+    q = randn(g, B, T, H, D, dtype=dtype)
+    lens = torch.randint(0, cap - T + 1, (B,), device="cuda", generator=g).int()
+    counts = torch.randint(0, T + 1, (B,), device="cuda", generator=g).int()
+    out, lse = cache.tree_attention(q, k, v, lens, counts=counts)
+    mass = cache.attention_mass(q, lse, k, lens, torch.zeros(B, hk, cap, device="cuda"), counts=counts)
+    ended()
+    e, u = 2.0 ** -23, torch.finfo(dtype).eps / 2
+    acc = (68 + 8 * cap ** 0.5) * e
+    for b in torch.arange(B, device="cuda").split(512):
+        n, c = lens[b], counts[b]
+        z = torch.einsum("bthd,bhsd->bths", q[b].double(), k[b].double().repeat_interleave(G, 1)) / D ** 0.5
+        ds = (D + 16) * e * float(q[b].float().norm(dim=-1).max() * k[b].float().norm(dim=-1).max()) / D ** 0.5
+        at = torch.arange(cap, device="cuda") - n[:, None, None]
+        t = torch.arange(T, device="cuda")[None, :, None]
+        z = z.masked_fill(((at > t) | (at >= c[:, None, None]))[:, :, None], -float("inf"))
+        real = torch.arange(T, device="cuda") < c[:, None]
+        want = torch.logsumexp(z, -1)[real]
+        p = torch.softmax(z, -1)
+        vv = v[b].double().repeat_interleave(G, 1)
+        exact, size = torch.einsum("bths,bhsd->bthd", p, vv)[real], torch.einsum("bths,bhsd->bthd", p, vv.abs())[real]
+        assert float(((out[b][real].double() - exact).abs() - (((u if dtype != torch.float32 else 0) + 2 * ds + acc) * size + u * exact.abs())).max()) <= 0
+        assert float(((lse[b][real].double() - want).abs() - (ds + acc + e * want.abs())).max()) <= 0
+        assert bool((out[b][~real] == 0).all()) and bool((lse[b][~real] == 0).all())
+        # a weight is off by its score's and lse's errors and a few steps, a sum of T * G of them by a step each
+        w = torch.exp(z - lse[b].double()[..., None]).masked_fill(~real[:, :, None, None], 0).sum(1).unflatten(1, (hk, G)).sum(2)
+        assert float(((mass[b].double() - w).abs() - (2 * ds + 8 * e + (T * G + 2) * e) * w).max()) <= 1e-30
