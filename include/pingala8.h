@@ -377,8 +377,8 @@ p8_status p8_tree_attn(const p8_kv *c, const p8_tree_attn_args *a, void *workspa
  * p8_tree_accept has moved into place): token i sees slots <= lens[b] + i, and its query and lse rows are those of row
  * r = rows[b * tokens + i] (rows NULL: r = i) of a p8_tree_attn call. With w the sum of exp(scale q . k - lse):
  *     out[b][h][j] = mass[b][h][j] + w for j < lens[b],  = w for the slots of the n_b tokens, untouched behind them.
- * Strides of mass and out: sequence, head; out may be mass (in place), and overlaps nothing else that is read. A row that is out of [0, tokens) counts for
- * nothing and sets bit 6; a row with lse = -infinity counts for nothing. Deterministic. */
+ * Strides of mass and out: sequence, head; out may be mass (in place), and overlaps nothing else that is read. A row that is
+ * out of [0, tokens) counts for nothing and sets bit 6; a row with lse = -infinity counts for nothing. Deterministic. */
 typedef struct p8_attn_mass_args {
     const void *q;
     int64_t q_stride[3];
@@ -395,9 +395,9 @@ p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream)
 
 /* The tree attention and mass kernels are pipelines of warps that wait for one another. A wait that is not over after `ns`
  * nanoseconds gives up: the call ends, once the copies and products that it has started are done, its results are invalid,
- * and p8_device_error reports bit 7 (128). Two seconds unless set here, for the calls made (or captured) from then on by this
- * process; at most 2^32 - 1. 0: every wait that is not over at its first look gives up, which is how a program's way of dealing with
- * the error can be tried out. */
+ * and p8_device_error reports bit 7 (128). Two seconds unless set here, for the calls made (or captured) from then on by
+ * this process; at most 2^32 - 1. 0: every wait that is not over at its first look gives up, which is how a program's way of
+ * dealing with the error can be tried out. */
 p8_status p8_cache_wait_limit(int64_t ns);
 
 /* Shorten every sequence with more than `budget` slots to `budget`, per layer and head: the first `sinks` slots, the
@@ -405,9 +405,9 @@ p8_status p8_cache_wait_limit(int64_t ns);
  * -infinity), in their order. Keys, values and mass [layer][b][h] of the kept slots are written to the first slots of
  * dst and mass_out, which are either the same buffers as src and mass (in place) or do not overlap them; a shorter
  * sequence is kept whole. new_lens[b] = min(lens[b], budget), kept [layers][batch][heads][budget] the kept slots (-1
- * behind new_lens[b]). sinks + recent <= budget <= the slots of dst and of src. new_lens and kept overlap
- * neither each other nor anything else, nor do what is written of keys, of values and of masses. Mass strides: layer, sequence, head. A sequence with lens[b] outside [0, slots] is left alone, its new_lens and kept too,
- * and sets bit 6. */
+ * behind new_lens[b]). sinks + recent <= budget <= the slots of dst and of src. new_lens and kept overlap neither each other
+ * nor anything else, nor does what is written of keys, of values and of masses. Mass strides: layer, sequence, head. A sequence
+ * with lens[b] outside [0, slots] is left alone, its new_lens and kept too, and sets bit 6. */
 typedef struct p8_kv_evict_args {
     const float *mass;
     int64_t mass_stride[3];

@@ -18,7 +18,8 @@ One step of speculative decoding with a bounded cache:
 
 Every call goes through the C ABI of libpingala8_b200.so on the tensors' device, on its current stream or the one
 given; there is no CPU path and no gradient. Lengths, counts, positions and rows that are out of range leave their
-sequence or token out and set bit 64 of device_error().
+sequence or token out and set bit 64 of device_error(). Outputs overlap neither one another nor what a call reads, but where
+"in place" is said; a tensor expanded over a dimension (stride 0) is no output. Buffers may lie between one another's rows.
 """
 import ctypes as C
 from collections import namedtuple
@@ -81,7 +82,8 @@ def kv_append(q, k, v, k_cache, v_cache, lens, pos, cos, sin, q_norm=None, k_nor
     the tokens' slots.
 
     pos int32 [batch, tokens]: each token's row of cos / sin float32 [positions, width / 2] (rotate-half form). q_norm,
-    k_norm float32 [width]: RMSNorm per head before the rotation. Any number of tokens up to the cache's slots."""
+    k_norm float32 [width]: RMSNorm per head before the rotation. Any number of tokens up to the cache's slots, none too.
+    q_out may be q (in place) where the cache is float32."""
     if stream is not None:
         return _on(stream, k_cache, kv_append, q, k, v, k_cache, v_cache, lens, pos, cos, sin, q_norm, k_norm, eps, counts, q_out)
     if q_out is None:

@@ -80,7 +80,7 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
 // append: y = rotate(norm(x)) per head of a token. A group of D / 8 lanes holds one head's row, lane l the values
 // 4l..4l+3 of both halves, so a rotation pair is in one lane, the sum of squares is a butterfly over the group, and
 // every access is 8 or 16 bytes wide. Bound by memory on a prompt (4,099 tokens x 48 heads of 128, 153 MB: 31 us, 4.9
-// TB/s; 34.5 with the rows asked for only after the lengths and positions), by its one launch on a token (1.8 us).
+// TB/s; 34.5 with the rows asked for only after the lengths and positions), by its one launch on a token (2.0 us).
 struct AppendArgs {
     const float *x[3];          // q, k, v
     long long xs[3][3];
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(1024, 2) k_evict_select(const EvictArgs a) {
 }
 
 // step 2, into other buffers: every row moves on its own, 16 bytes a thread. Bound by HBM (288 rows x 2,048 kept of 16,384
-// slots, 604 MB: 105 to 110 us of the call's 135, 5.6 TB/s).
+// slots, 604 MB: 105 to 110 us of the call's 136, 5.6 TB/s).
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
     const int row = blockIdx.x / a.per_row, block = blockIdx.x - row * a.per_row, h = row % a.heads, b = row / a.heads % a.batch, layer = row / a.heads / a.batch;
     after_prior();  // every block: what follows in the stream waits for this launch alone
@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a) {
 // step 2 in place: kept[i] >= i, so a block that goes up through a range of the row's bytes (64 of them: its columns
 // belong to no other block), reads a chunk of sources before it writes their destinations, and reads the next chunk
 // (sources at or behind every destination written so far) meanwhile, loses nothing. blockIdx.y 0 / 1: keys / values,
-// 2: the masses.
+// 2: the masses. Bound by its rounds of latency, eight for 2,048 kept rows of 256 bytes: one layer of 2,112 slots x 8 heads takes 17
+// us, 36 layers of 16,384 slots 151, with the select before it.
 template <typename U>
 __device__ __forceinline__ void evict_slide(const char *base, long long stride, int per, int keep, const int *kept) {
     constexpr int kRows = 4;
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(256) k_evict_slide(const EvictArgs a) {
 // acceptance: one block per (layer, sequence, keys or values). Each finds the path on its own (the first warp, two
 // nodes a lane, one ballot per step: cheaper than a launch between the walk and the moves), then moves the rows of all
 // heads in chunks, reading a chunk before writing it: path[i] >= i and the chunks go up, so no source is lost. Bound by two
-// rounds of latency and the launch: 2.3 us for 36 layers and 8 drafted tokens, 6.6 us for 32 layers x 16 sequences.
+// rounds of latency and the launch: 2.4 us for 36 layers and 8 drafted tokens, 6.8 us for 32 layers x 16 sequences.
 struct AcceptArgs {
     const long long *tokens, *target;
     const int *parents, *lens, *counts;

@@ -1,5 +1,9 @@
 // p8_tree_attn.cuh -- attention of a tree of drafted tokens over a cache, and the attention mass per slot (included by
 // p8_cache.cu).
+//
+// Times here are a call's in a CUDA graph at full clocks (1,965 MHz). Calls that follow one another for seconds draw the
+// 1,000 W that the GPU may, at 1.6 GHz in the attention: 24 sequences x 7 tokens then take 91 us, not 79, 64 tokens over
+// 131,000 slots 182, not 154. A form that was not kept is given with the kept one's time of the same day.
 #pragma once
 
 constexpr unsigned int kWaitNs = 2000000000u;  // what waits are bounded by, unless the host says otherwise
@@ -337,10 +341,10 @@ __device__ __noinline__ void add_bad(O *out, const T *v, long long stride, unsig
 // maximum and sum in base 2, P rounded to the type over S's columns -> O += P V (P from TMEM). With two buffers the next
 // scores are computed while this step's are exponentiated.
 // TWO = false is bound by K and V from HBM: 64 KB a tile of 128 columns at 1/148 of the bandwidth takes 2.8 k cycles, a
-// stream's step 2 k (24 sequences x 7 tokens x 32 heads, fp16: 78 us, 5.5 TB/s). TWO = true is bound by the tensor cores
+// stream's step 2 k (24 sequences x 7 tokens x 32 heads, fp16: 79 us, 5.4 TB/s). TWO = true is bound by the tensor cores
 // and the shared memory that feeds them: a 128 x 64 x 16 product takes 60 cycles there, not 32, for its 4 KB of Q, so a
-// tile takes 2.9 k at best and 3.9 k in fact (131,000 slots x 8 heads x 256 rows, bf16: 153 us, 0.9 PFLOP/s). Measured
-// there and not kept: 128-slot steps with one buffer a stream (twice the columns a product, but scores, softmax and
+// tile takes 2.9 k at best and 3.9 k in fact (131,000 slots x 8 heads x 256 rows, bf16: 154 us, 0.9 PFLOP/s). Measured
+// there (153 us then) and not kept: 128-slot steps with one buffer a stream (twice the columns a product, but scores, softmax and
 // products one after the other) 184 us; weights by the old maximum while the new one is found 159 us; with no
 // exponentials at all it would still be 147 us.
 template <int D, bool TWO>
@@ -699,8 +703,10 @@ __global__ void __launch_bounds__(TcShape<D, TWO>::kThreads, 1) k_tree_attn_tc(c
 // rows are few, by how many blocks fit an SM where they are many (fewer loads ahead, fewer registers).
 template <typename T, int D, int AHEAD>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, int ctas, float lift, const float *part_o, const float2 *part_ml) {
-    // Everything up to the wait comes from the call's inputs, while the attention kernel runs; the parts are its outputs.
-    // Every warp waits, with or without something to add: what follows in the stream waits for this launch alone.
+    // Everything up to the wait comes from the call's inputs; the parts are the attention kernel's outputs. The blocks start
+    // early where an SM has room: on one without an attention CTA, or whose CTA has ended. Beside a CTA their registers fit only with
+    // 32-bit caches and one row tile (a 16-bit one leaves 7 K of 65,536, a block wants 12 K to 27 K). Every warp waits, with or without
+    // something to add: what follows in the stream waits for this launch alone.
     constexpr int W = D / 32;
     const int lane = threadIdx.x % 32;
     const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
@@ -772,10 +778,10 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a, Cut cut, in
 // 32 rows two of them take the halves of a tile's rows, so that two tiles are under way, with fewer rows four tiles are. A
 // buffer is given back once its last columns are in registers, before their exponentials. Keys come through a TMA ring,
 // the unit's query rows and their -lse stay in shared memory. Bound by K from HBM up to about 170 rows (32 KB a tile: 1.4 k
-// cycles at 1/148 of the bandwidth; 7 tokens x 32 heads over 24 x 8 k slots: 68 us, 6.1 TB/s), by the exponentials (8 cycles
-// a row and tile) beyond: 64 tokens x 32 heads over 2 x 32 k slots 50 us, of which the exponentials are 29. That case took
-// 84 us with one group a buffer, 66 with two that shared one and with the query rows loaded one piece after the other, 55
-// without what mass_cut counts. With few rows it costs up to 4 us in 28 to have more than four stages.
+// cycles at 1/148 of the bandwidth; 7 tokens x 32 heads over 24 x 8 k slots: 69 us, 6.0 TB/s), by the exponentials (8 cycles
+// a row and tile) beyond: 64 tokens x 32 heads over 2 x 32 k slots 54 us (50 of keys that are partly in
+// L2), of which the exponentials are 29. That case, of such keys, took 84 us with one group a buffer, 66 with two that shared one
+// and with the query rows loaded one piece after the other, 55 without what mass_cut counts. With few rows it costs up to 4 us in 28 to have more than four stages.
 template <int D, int ROWS>
 struct MassShape {
     static constexpr int kStage = kTile * D * 2;
@@ -1007,9 +1013,9 @@ __global__ void __launch_bounds__(576, 1) k_attn_mass_tc(const AttnArgs a, const
 // 2^-21 |x y|, three mma.sync products with fp32 sums. The tensor cores cut what they add off, they do not round it: so
 // products with a small piece have sums of their own, a tile's products of weights and values are added to the
 // accumulator by fp32 additions, and scores have two sums (all in one, and hi cut off: 2.8e-6 off 64 bits instead of
-// 0.6e-6, where a plain fp32 product is 1.2e-6 off; it costs 27.2 us instead of 24.7 at 12 tokens x 32 heads over 2,047
-// slots). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back: more
-// shared-memory traffic than the products take. From registers the split costs four integer or fp32 operations.)
+// 0.6e-6, where a plain fp32 product is 1.2e-6 off; at 12 tokens x 32 heads over 2,047 slots it
+// cost 2.5 us of 27). (tcgen05 takes its operands from shared memory, where the split of K and V would have to be written back: more
+// shared-memory traffic than the products take. From registers a split costs three integer or fp32 operations.)
 // A product waits for the one before it on the same sum (four of them take that long to issue), so the order is by piece,
 // through as many sums as there are.
 struct Split {
@@ -1017,8 +1023,8 @@ struct Split {
 };
 // kAny: x may be anything. Rounding carries the last 2^12 numbers below infinity over to it, so hi comes from a magnitude
 // below them (lo then has up to 13 bits); an infinity stays one, in lo. It is the fourth operation of a split: 12 tokens x 32
-// heads over 2,047 slots take 27.9 us, not 27.4, 64 tokens over 8,192 slots 210, not 201, masses of 12 tokens over 32,768 slots
-// 77.9, not 74.3. Weights are never that large, and queries are kept below it when they are staged.
+// heads over 2,047 slots take 28.7 us, not 27.8, 64 tokens over 8,192 slots 217, not 207, masses of 12 tokens over 32,768 slots
+// 81, not 78. Weights are never that large, and queries are kept below it when they are staged.
 constexpr uint32_t kRounds = 0x7F7FEFFFu;  // the largest number that is rounded to a finite one
 template <bool kAny>
 __device__ __forceinline__ Split split(float x) {
@@ -1387,8 +1393,8 @@ __global__ void __launch_bounds__(F32Shape<D, RT>::kThreads, 1) k_tree_attn_f32(
 
 // The masses of a 32-bit cache. Four groups of four warps take the tiles in turn; a warp has 16 of the 64 slots and goes
 // through the query rows 16 at a time. A lane's four slots are summed over its rows, and over the eight lanes that share
-// them at the end. 12 tokens x 32 heads over 65,536 slots take 141 us, one token 57 us, 4.7 TB/s (eight warps with eight
-// slots of every tile each: 200 and 110 us). Bound by K from HBM for up to 16 rows, by the products beyond.
+// them at the end. 12 tokens x 32 heads over 65,536 slots take 147 us, one token 59 us, 4.6 TB/s (eight warps with eight
+// slots of every tile each took 200 and 110 us where this took 141 and 57). Bound by K from HBM for up to 16 rows, by the products beyond.
 template <int D>
 struct F32Mass {
     static constexpr int kRows = 128, kGroups = 4, kThreads = 4 * kGroups * 32 + 32;

@@ -248,13 +248,17 @@ class TreeDecoder:
 
     Each pass takes 1 to 64 tokens at once: the projections through the batched product (which reads the packed weights
     once for all of them), norms, rotation and cache writes through cache.kv_append, attention through
-    cache.tree_attention, so a pass over a tree costs little more than one token's. step() then walks the tree along the
-    model's own choices (cache.tree_accept) and keeps what it confirms: the tokens are those that greedy decoding gives one
-    by one. dtype is the cache's type (float32, float16 or bfloat16).
+    cache.tree_attention. A pass over 8 tokens takes 2.3 times as long on the GPU as one over a single token, over 64 tokens 2.8
+    times (Qwen3-4B behind 500 tokens: 2.4, 5.5 and 6.7 ms); step() is not captured, waits for the accepted count on the
+    host and takes 7.8 to 8.7 ms there. It walks the tree along the model's own choices (cache.tree_accept) and keeps what it
+    confirms: without a budget the tokens are those that greedy decoding gives one by one, up to ties within the rounding of
+    products of other widths. dtype is the cache's type (float32, float16 or bfloat16).
 
     With a budget, the attention weight that every slot draws is added up (cache.attention_mass), and a sequence that has
     grown `slack` slots over the budget is cut back to it (cache.kv_evict): the first `sinks` slots, the last `recent` ones
-    and the heaviest of the others stay, per layer and head. Tokens keep the positions they had."""
+    and the heaviest of the others stay, per layer and head. Tokens keep the positions they had. Cuts come between passes, so
+    what a token sees, and with it the text, also depends on how many drafted tokens the passes took. budget is at least
+    sinks + recent and 1."""
 
     def __init__(self, model, max_len, dtype=torch.float16, budget=None, sinks=4, recent=64, slack=128):
         if budget is not None and (budget < 1 or min(sinks, recent, slack) < 0 or sinks + recent > budget):
