@@ -100,7 +100,8 @@ def tree_attention(q, k_cache, v_cache, lens, mask=None, counts=None, scale=None
     q [batch, tokens, heads, width] in the cache's type. Token t sees the whole sequence before the call's tokens and the
     tokens whose bits mask[t] has (int64 [tokens] or [batch, tokens], as tree_plan makes it; None: a chain). Returns
     (out like q, lse float32 [batch, tokens, heads]): the softmax average of the values and the natural log of the sum
-    of exponentials; 0 and -inf for a token that sees nothing. scale: 1 / sqrt(width) unless given."""
+    of exponentials; 0 and -inf for a token that sees nothing. scale: 1 / sqrt(width) unless given. With a 16-bit cache the
+    weights are rounded to its type: out is off by up to 1.4 times as much as one of 32-bit weights, rounded once."""
     if stream is not None:
         return _on(stream, k_cache, tree_attention, q, k_cache, v_cache, lens, mask, counts, scale, out, lse, workspace)
     if out is None:
