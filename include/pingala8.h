@@ -436,6 +436,102 @@ typedef struct p8_tree_accept_args {
 } p8_tree_accept_args;
 p8_status p8_tree_accept(const p8_kv *c, const p8_tree_accept_args *a, void *stream);
 
+/* ---------------------------------------------------------------- paged key/value cache, beam search ------------- */
+
+/* The same decode step for a server: keys and values in pages of `page` slots each that sequences share out, and may share.
+ * Slot s of sequence (row) b is slot s % page of page tables[b * table_stride + s / page]. Element (layer, page, head, slot,
+ * d) of the keys is k[layer * k_stride[0] + page * k_stride[1] + head * k_stride[2] + slot * k_stride[3] + d], of the
+ * values alike; types, widths, alignment, what may overlap, query heads, lens and errors are as for the cache above. Any page size
+ * from 1; columns * page <= P8_SLOTS_MAX. Table entries are only looked at where a call has a slot; one that is outside
+ * [0, pages) there sets bit 6 (64). table_stride may be 0 (all rows read one table) where the tables are only read. */
+#define P8_PAGE_MAX (1 << 20)
+#define P8_BEAMS_MAX 64      /* beams of a group */
+#define P8_CANDIDATES_MAX 64
+typedef struct p8_paged {
+    void *k, *v;
+    int64_t type;                      /* p8_kv_type of k and v */
+    int64_t layers, pages, heads, page, width;
+    int64_t k_stride[4], v_stride[4];  /* layer, page, head, slot */
+    int32_t *tables;                   /* [rows][columns] */
+    int64_t rows, columns, table_stride;
+} p8_paged;
+
+/* New tokens into one layer's pages (layers = 1), 1 row a sequence: as p8_kv_append, but only the first `rotary` elements of
+ * a head turn (a multiple of 8, at most width; cos / sin are f32 [positions][rotary / 2]), as pairs (i, i + rotary / 2), or
+ * (2i, 2i + 1) where `interleaved` is not 0; the others go through (normed, where there is a norm). A token whose slot's page
+ * is out of range is not written to the cache (its query is written to q_out). Sequences of one call may share pages
+ * that they do not write to; a slot that two of them write holds one of the two. */
+typedef struct p8_paged_append_args {
+    const float *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];  /* sequence, token, head */
+    int64_t tokens, heads;
+    const int32_t *lens, *counts, *pos;   /* [rows], [rows] or NULL, [rows][tokens] */
+    const float *cos, *sin;
+    int64_t positions, rotary, interleaved;
+    const float *q_norm, *k_norm;         /* [width] or NULL */
+    double eps;
+    void *q_out;
+    int64_t q_out_stride[3];
+} p8_paged_append_args;
+p8_status p8_paged_append(const p8_paged *c, const p8_paged_append_args *a, void *stream);
+
+/* Attention of one new token per sequence over one layer's pages (layers = 1), its own key and value already in slot lens[b]:
+ * out = softmax(scale q k^T) v over the slots 0..lens[b], in q's type (the cache's); lse [rows][heads] f32 (or NULL) the
+ * natural log of the sum of exponentials. counts[b] (0 or 1; NULL: 1) = 0: the row has no token, nothing of it is read or
+ * written. Slots in pages out of range count as not there; a sequence of which nothing is left gets 0 and -infinity. What lies behind slot
+ * lens[b] is not read. Products and sums in fp32; 16-bit types: the weights as two pieces of the type each (2^-14). Workspace:
+ * p8_paged_attn_workspace bytes, 256-byte aligned. Deterministic. */
+typedef struct p8_paged_attn_args {
+    const void *q;
+    int64_t q_stride[2];                  /* sequence, head */
+    int64_t heads;
+    const int32_t *lens, *counts;
+    double scale;
+    void *out;
+    int64_t out_stride[2];
+    float *lse;
+} p8_paged_attn_args;
+size_t p8_paged_attn_workspace(const p8_paged *c, int64_t heads);
+p8_status p8_paged_attn(const p8_paged *c, const p8_paged_attn_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One step of beam search for `batch` groups of `beams` beams: of all continuations (beam w, token t) of a group, with
+ *     total = scores[b][w] + logits[b][w][t] - log sum over t' of exp(logits[b][w][t'])
+ * the `candidates` largest in their order: out_scores (the total, rounded to f32), parents (w), tokens (t). Continuations
+ * of one beam are in the order of their logits (ties: the lowest token), those of several beams in the order of their totals, which are
+ * held in 64 bits (ties: the lowest beam). A beam with done[b][w] not 0 has ended: it has one continuation, itself, with its score
+ * and the token `end`. What is no continuation: all of a beam whose score is not finite, or one of whose logits is +infinity, or all -infinity
+ * (an ended beam: whose score is not finite); NaN logits, which count as -infinity, and logits of -infinity. Where there are fewer
+ * continuations than candidates, the others have score -infinity, parent -1 and token -1. out_done [b][i] (or NULL) is 1 where the
+ * parent had ended or the token is `end` (end < 0: there is none, and done must be NULL), 0 for candidates that are not there.
+ *
+ * Logits of p8_kv_type `type`, element (b, w, t) at b * stride[0] + w * stride[1] + t, strides >= 0 (0: the
+ * same for all; 1 <= vocab < 2^31); scores and results are contiguous. Logits of beams that have ended or whose score is not finite are not read.
+ * Results overlap neither one another, nor the workspace, nor what is read. Workspace: p8_beam_select_workspace bytes, 256-byte
+ * aligned. Deterministic. */
+typedef struct p8_beam_select_args {
+    const void *logits;
+    int64_t type, batch, beams, vocab, stride[2];
+    const float *scores;                  /* [batch][beams] */
+    const uint8_t *done;                  /* [batch][beams] or NULL */
+    int64_t end, candidates;
+    float *out_scores;                    /* [batch][candidates], as all that follow */
+    int32_t *parents;
+    int64_t *tokens;
+    uint8_t *out_done;
+} p8_beam_select_args;
+size_t p8_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t candidates);
+p8_status p8_beam_select(const p8_beam_select_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The beams go on from their parents: row b * beams + i of the tables becomes that of beam parents[b][i] of the same group (-1:
+ * its own), in place, for all layers. With n = lens[b * beams + i], which is the same for all beams of a group: columns before n / page
+ * are the parent's (its pages are shared from now on). Where n % page != 0, column n / page names a page that was begun and will be
+ * written to, one for each beam: the lowest child takes its parent's; every further child takes one of those of the beams
+ * without children, the lowest first, and the first n % page slots of its parent's page are copied there. Columns behind stay, so that
+ * each beam keeps the pages that were laid out for it; the begun pages of a group are different ones. A group with a parent outside
+ * [-1, beams), with several lengths or with one outside [0, columns * page] is left alone and sets bit 6, as does a page that is
+ * out of range, which is not copied. batch * beams = rows of the tables. */
+p8_status p8_beam_reorder(const p8_paged *c, const int32_t *parents, const int32_t *lens, int64_t batch, int64_t beams, void *stream);
+
 /* ---------------------------------------------------------------- model files (GGUF) ---------------------------- */
 
 /* A GGUF file holding a Pingala-8 ("VR native") model, opened and checked as llama_model_loader::vr_native_init does
@@ -458,7 +554,7 @@ p8_status p8_gguf_load_linear(p8_gguf *g, int64_t i, uint8_t *out, size_t out_ca
 
 /* Non-zero if a kernel since the last call gave up (that launch's results are invalid), then clears the word. Bits:
  * 4 GEMM pipeline wait timed out, 8 row-parallel exchange wait timed out, 16 exchange entry with a foreign tag, 64 a
- * cache operator met a length, count, position or row out of range and left it out, 128 a tree attention or mass
+ * cache operator met a length, count, position, row, page or parent out of range and left it out, 128 a tree attention or mass
  * pipeline wait timed out (1, 2 and 32 are unused). Waits for all streams of the current device. */
 int p8_device_error(void);
 

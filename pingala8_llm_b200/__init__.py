@@ -1,8 +1,8 @@
 """pingala8_llm_b200 -- B200-native (sm_100a) Pingala-8 quantized-weight matmul path.
 
 Drop-in for the reference's ggml Pingala-8 hooks (Genrius-AI/pingala8-llm): batch-1 table GEMV, batched product,
-get_rows / f32 dequant, a tensor-parallel split, and (pingala8_llm_b200.cache) the key/value cache operators of a decode
-step. The compute lives in libpingala8_b200.so (C ABI:
+get_rows / f32 dequant, a tensor-parallel split, (pingala8_llm_b200.cache) the key/value cache operators of a decode
+step and (pingala8_llm_b200.paged) those of serving from a paged cache with beam search. The compute lives in libpingala8_b200.so (C ABI:
 include/pingala8.h); this package is the thin host mirror over it.
 """
 from ._lib import LIB_PATH, P8Error, P8_STATUS, header_functions, lib  # noqa: F401
@@ -17,7 +17,7 @@ def __getattr__(name):
         import importlib
 
         return getattr(importlib.import_module(".ops", __name__), name)
-    if name in ("cache", "decode"):
+    if name in ("cache", "decode", "paged"):
         import importlib
 
         return importlib.import_module("." + name, __name__)

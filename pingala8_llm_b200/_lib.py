@@ -105,6 +105,12 @@ _SIGS = {
     "p8_attn_mass": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
     "p8_kv_evict": (C.c_int, [C.c_char_p, C.c_char_p, C.c_char_p, _vp]),
     "p8_tree_accept": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
+    "p8_paged_append": (C.c_int, [C.c_char_p, C.c_char_p, _vp]),
+    "p8_paged_attn_workspace": (_sz, [C.c_char_p, _i64]),
+    "p8_paged_attn": (C.c_int, [C.c_char_p, C.c_char_p, _vp, _sz, _vp]),
+    "p8_beam_select_workspace": (_sz, [_i64, _i64, _i64, _i64]),
+    "p8_beam_select": (C.c_int, [C.c_char_p, _vp, _sz, _vp]),
+    "p8_beam_reorder": (C.c_int, [C.c_char_p, _vp, _vp, _i64, _i64, _vp]),
     "p8_cache_wait_limit": (C.c_int, [_i64]),
     "p8_device_error": (C.c_int, []),
     "p8_status_str": (C.c_char_p, [C.c_int]),

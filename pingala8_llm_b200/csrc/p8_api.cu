@@ -14,6 +14,7 @@ using namespace p8;
 namespace p8 {
 unsigned int read_and_clear_device_error();
 unsigned int read_and_clear_cache_error();
+unsigned int read_and_clear_paged_error();
 }
 
 namespace {
@@ -370,7 +371,7 @@ p8_status p8_chain_trace(p8_chain *c, uint64_t *dev_buf, size_t words) {
  * that do not block it (torch's others). */
 int p8_device_error(void) {
     cudaDeviceSynchronize();
-    return (int)(read_and_clear_device_error() | read_and_clear_cache_error());
+    return (int)(read_and_clear_device_error() | read_and_clear_cache_error() | read_and_clear_paged_error());
 }
 
 const char *p8_build_info(void) { return "pingala8_b200 sm_100a (tcgen05/TMA), C ABI v1"; }

@@ -4,22 +4,9 @@
 //
 // The module does not link against the library: bind() is given the entry points' addresses by the package, which has
 // the library loaded. Every function returns the p8_status; what is refused before the call raises ValueError.
-#include <Python.h>
-
-#include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <optional>
-#include <string>
-
-#include "pingala8.h"
+#include "p8_py.h"
 
 namespace {
-
-using at::Tensor;
 
 struct Entries {
     decltype(&p8_kv_append) append;
@@ -29,23 +16,6 @@ struct Entries {
     decltype(&p8_kv_evict) evict;
     decltype(&p8_tree_accept) accept;
 } g_p8;
-
-struct Refused {
-    std::string what;
-};
-[[noreturn]] void refuse(std::string what) { throw Refused{std::move(what)}; }
-
-const Tensor &tensor(PyObject *o, const char *name) {
-    if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
-    return THPVariable_Unpack(o);
-}
-
-const char *type_name(at::ScalarType t) { return t == at::kInt ? "int32" : t == at::kLong ? "int64" : t == at::kFloat ? "float32" : "the cache's type"; }
-std::string shape_name(at::IntArrayRef s) {
-    std::string r = "[";
-    for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
-    return r + "]";
-}
 
 // a cache [batch, kv heads, slots, width], with a leading layer dimension where `layers`; v may be absent
 struct Cache {
@@ -82,24 +52,6 @@ Cache cache(const Tensor &k, const Tensor *v, bool layers) {
     return r;
 }
 
-// a contiguous tensor of exactly this shape, or NULL for None
-template <typename T>
-T *flat(PyObject *o, const char *name, at::ScalarType type, at::IntArrayRef shape, const Cache &c, bool optional = false) {
-    if (optional && o == Py_None) return nullptr;
-    const Tensor &t = tensor(o, name);
-    if (t.scalar_type() != type || t.sizes() != shape || !t.is_cuda() || t.get_device() != c.dev || !t.is_contiguous())
-        refuse(std::string(name) + " must be contiguous " + type_name(type) + " " + shape_name(shape) + " on the cache's device");
-    return static_cast<T *>(t.data_ptr());
-}
-// [batch, tokens, heads, width]: address and outer strides
-template <typename T>
-T *rows(PyObject *o, const char *name, at::ScalarType type, at::IntArrayRef shape, const Cache &c, int64_t (&st)[3]) {
-    const Tensor &t = tensor(o, name);
-    if (t.scalar_type() != type || t.sizes() != shape || !t.is_cuda() || t.get_device() != c.dev || t.stride(3) != 1)
-        refuse(std::string(name) + " must be " + type_name(type) + " " + shape_name(shape) + " with unit stride in its last dimension, on the cache's device");
-    for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
-    return static_cast<T *>(t.data_ptr());
-}
 struct Query {
     int64_t tokens, heads;
 };
@@ -123,43 +75,6 @@ float *masses(PyObject *o, const char *name, const Cache &c, int64_t dims, int64
     st[2] = t.stride(four + 1);
     return static_cast<float *>(t.data_ptr());
 }
-
-double number(PyObject *o) {
-    const double x = PyFloat_AsDouble(o);
-    if (x == -1.0 && PyErr_Occurred()) throw nullptr;
-    return x;
-}
-int64_t integer(PyObject *o) {
-    const long long x = PyLong_AsLongLong(o);
-    if (x == -1 && PyErr_Occurred()) throw nullptr;
-    return x;
-}
-
-// The tensors' device current for the launch, and its current stream.
-struct On {
-    std::optional<c10::DeviceGuard> guard;
-    void *stream;
-    explicit On(const Cache &c) {
-        const c10::Device d(c10::kCUDA, (c10::DeviceIndex)c.dev);
-        guard.emplace(d);
-        stream = c10::cuda::getCurrentCUDAStream(d.index()).stream();
-    }
-};
-
-#define ENTRY(name, count)                                                                  \
-    PyObject *name(PyObject *, PyObject *const *a, Py_ssize_t n) {                          \
-        try {                                                                               \
-            if (n != (count)) refuse(#name " takes " #count " arguments");                  \
-            if (!g_p8.append) refuse("bind() comes first");                                 \
-            return PyLong_FromLong(name##_(a));                                             \
-        } catch (const Refused &r) {                                                        \
-            PyErr_SetString(PyExc_ValueError, r.what.c_str());                              \
-        } catch (const std::exception &e) {                                                 \
-            PyErr_SetString(PyExc_RuntimeError, e.what());                                  \
-        } catch (std::nullptr_t) { /* the Python error is set */                            \
-        }                                                                                   \
-        return nullptr;                                                                     \
-    }
 
 // q k v k_cache v_cache lens pos cos sin q_norm k_norm eps counts q_out
 p8_status kv_append_(PyObject *const *a) {
@@ -300,7 +215,7 @@ PyObject *workspace_(PyObject *const *a, Py_ssize_t n) {
 }
 PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) {
     try {
-        if (!g_p8.append) refuse("bind() comes first");
+        if (!g_bound) refuse("bind() comes first");
         return workspace_(a, n);
     } catch (const Refused &r) {
         PyErr_SetString(PyExc_ValueError, r.what.c_str());
@@ -327,6 +242,7 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     g_p8 = {(decltype(&p8_kv_append))p[0], (decltype(&p8_tree_attn_workspace))p[1], (decltype(&p8_tree_attn))p[2],
             (decltype(&p8_attn_mass))p[3], (decltype(&p8_kv_evict))p[4], (decltype(&p8_tree_accept))p[5]};
+    g_bound = true;
     Py_RETURN_NONE;
 }
 

@@ -1,0 +1,788 @@
+// p8_paged_attn.cuh -- attention of one new token per sequence over a paged cache; included by p8_paged.cu.
+//
+// o = softmax(scale q K^T) V for the query heads of one cache head, which share its keys and values: every byte of the cache
+// is read once, 4 to 16 operations are done on it, so the memory bounds it (and latency, where there is little to read). The tiles of all
+// sequences and heads form one list, of which every CTA gets an equal contiguous share and every warp of it an equal part:
+// the warps finish together whatever the lengths are. A warp works on its own: keys and values go from the pages straight
+// into its registers, in the layout in which the matrix instruction takes them, with no shared memory and no
+// barrier in its way. Each warp keeps the running maximum m, the sum l of 2^(s - m) and the sum of 2^(s - m) v. Where a sequence's
+// head is spread over several warps, their sums meet in shared memory at the end of the CTA, and those of several
+// CTAs in a second launch.
+
+struct PagedAttnArgs {
+    const char *q;
+    long long qs[2];     // bytes: sequence, head
+    const char *kv[2];
+    long long st[2][3];  // bytes: page, head, slot
+    const int *tables, *lens, *counts;
+    long long ts;
+    char *out;
+    long long os[2];     // bytes: sequence, head
+    float *lse, *part;
+    long long slots;
+    PageDiv div;
+    int batch, heads, kvh, group, blocks, pages, ctas;  // group: query heads of a cache head; blocks: of these, rows of a warp's tile
+    float scale2;                                       // scale / ln 2: the kernel's exponentials are powers of two
+};
+
+constexpr int kAttnWarps = 4;
+constexpr int kSpan = 128;  // slots that a share of the list has at least: two tiles of 16 for each warp of a CTA
+
+// Tiles of a sequence; none where it has no token in this call or is out of range.
+template <int kTile>
+__device__ __forceinline__ int row_tiles(const PagedAttnArgs &a, int b, bool &bad) {
+    const int len = a.lens[b], n = a.counts ? a.counts[b] : 1;
+    bad = len < 0 || n < 0 || n > 1 || (long long)len + n > a.slots;
+    return bad || n == 0 ? 0 : len / kTile + 1;
+}
+
+// The list of tiles, as a warp sees it: lane l has the sequences [l per, (l + 1) per).
+template <int kTile>
+struct TileList {
+    static constexpr int kLeast = kSpan / kTile;
+    const PagedAttnArgs &a;
+    int per, units;
+    long long upto, total, share;  // places of the lanes up to this one; of all; of a CTA
+
+    __device__ __forceinline__ TileList(const PagedAttnArgs &a_, int lane, bool report) : a(a_), per((a_.batch + 31) / 32), units(a_.kvh * a_.blocks) {
+        long long mine = 0;
+        bool any_bad = false;
+        for (int i = 0; i < per; ++i) {
+            const int b = lane * per + i;
+            if (b >= a.batch) break;
+            bool bad;
+            mine += unit_places(row_tiles<kTile>(a, b, bad), kLeast);
+            any_bad |= bad;
+        }
+        if (report && any_bad) out_of_range();
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        upto *= units;
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        share = cta_share(total, a.ctas, kLeast);
+    }
+    // the sequence that has place p < total, and its first place
+    __device__ __forceinline__ int find(long long p, int lane, long long &begin) const {
+        const unsigned int m = __ballot_sync(0xffffffffu, upto > p);
+        const int l = __ffs(m) - 1;
+        const long long before = __shfl_sync(0xffffffffu, upto, l > 0 ? l - 1 : 0);
+        begin = l > 0 ? before : 0;
+        if (per == 1) return l;
+        for (int i0 = 0;; i0 += 32) {  // (the place is in one of these sequences)
+            const int b = l * per + i0 + lane;
+            bool bad;
+            long long c = i0 + lane < per && b < a.batch ? unit_places(row_tiles<kTile>(a, b, bad), kLeast) * units : 0, u = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, u, o);
+                if (lane >= o) u += v;
+            }
+            const unsigned int w = __ballot_sync(0xffffffffu, begin + u > p);
+            if (w || i0 + 32 >= per) {
+                const int k = w ? __ffs(w) - 1 : 31;
+                begin += __shfl_sync(0xffffffffu, u - c, k);
+                return l * per + i0 + k;
+            }
+            begin += __shfl_sync(0xffffffffu, u, 31);
+        }
+    }
+};
+
+// 16 bytes of the cache, which no one reads again
+__device__ __forceinline__ uint4 ld_once(const char *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of 16-bit values, two neighbours of a row in each lane, the other way round
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// two values cut (not rounded) to the type
+template <typename T> __device__ __forceinline__ uint32_t cut2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t cut2<__half>(float lo, float hi) { uint32_t v; asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo)); return v; }
+template <> __device__ __forceinline__ uint32_t cut2<__nv_bfloat16>(float lo, float hi) { uint32_t v; asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo)); return v; }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+
+// A tile's pages: lane l looks up slot l % kTile.
+template <int kTile>
+struct Lookup {
+    int id;           // the page; -1 behind the sequence's end
+    unsigned int in;  // the slot's place in it
+    __device__ __forceinline__ void ask(const PagedAttnArgs &a, const int *table, int tile, int n, int lane) {
+        const int slot = tile * kTile + lane % kTile;
+        const unsigned int page = page_of(a.div, (unsigned int)slot);
+        in = (unsigned int)slot - page * a.div.size;
+        id = -1;
+        if (slot < n) {
+            id = table[page];
+            if (id < 0) id = INT_MIN;  // out of range, as any number of pages or above
+        }
+    }
+    // byte offsets of the slot's key and value; a bit for each slot that is there
+    __device__ __forceinline__ unsigned int resolve(const PagedAttnArgs &a, long long &ko, long long &vo) const {
+        const bool there = (unsigned int)id < (unsigned int)a.pages;
+        if (!there && id != -1) out_of_range();
+        ko = vo = 0;
+        if (there) {
+            ko = id * a.st[0][0] + in * a.st[0][2];
+            vo = id * a.st[1][0] + in * a.st[1][2];
+        }
+        return __ballot_sync(0xffffffffu, there);
+    }
+};
+
+// ----------------------------------------------------------------------------------------------------------------
+// 16-bit types: S^T = K Q^T and O^T += V^T P^T by m16n8k16, the query heads (8 kN of them) as columns. The order of the elements
+// within a product's sum is free, so lane (g, t) of a key's operand takes 16 consecutive bytes of key g (and g + 8) for two
+// products; of the values it takes 16 bytes of slots 2t, 2t + 1, 2t + 8 and 2t + 9, and interleaves them in pairs. S^T comes out
+// with slots as rows and P^T goes in with slots along the sum: movmatrix turns it. The weights go in as two pieces of the
+// type, so that their rounding (2^-14 bf16, 2^-20 fp16) is nothing to that of the result; fp16 has them lifted by 2^7, so
+// that those 2^-31 of the largest still count. The pieces are cut, not rounded, and the second one's last bit is set: neither is negative
+// or nothing, so that an infinite value that is seen comes out as itself. The maximum only moves where a score is 2^8 above it: one vote a tile in place of
+// a reduction and a rescaling.
+template <typename T, int D, int kN>
+struct Core16 {
+    static constexpr int kTile = 16, kRows = 8 * kN;
+    static constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = 8.f;
+    uint32_t q[kN][D / 32][4];
+    float o[kN][D / 16][4], m[kN][2], l[kN][2];
+    uint4 k[2][D / 32], v[4][D / 64];
+
+    __device__ __forceinline__ Core16(float *) {}
+    __device__ __forceinline__ void begin(const char *qrow, long long qs, int nq, float, int lane) {
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (8 * i + g < nq) x = *reinterpret_cast<const uint4 *>(qrow + (8 * i + g) * qs + 64 * j + 16 * t);
+                q[i][j][0] = x.x; q[i][j][1] = x.y; q[i][j][2] = x.z; q[i][j][3] = x.w;
+            }
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+            m[i][0] = m[i][1] = -INFINITY;
+            l[i][0] = l[i][1] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void load_k(const char *base, long long off, unsigned int mask, int lane) {
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const long long at = __shfl_sync(0xffffffffu, off, g + 8 * r);
+            const bool there = mask >> (g + 8 * r) & 1;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                k[r][j] = make_uint4(0, 0, 0, 0);
+                if (there) k[r][j] = ld_once(base + at + 64 * j + 16 * t);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const char *base, long long off, unsigned int mask, int lane) {
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int slot = 2 * t + (r & 1) + 8 * (r >> 1);
+            const long long at = __shfl_sync(0xffffffffu, off, slot);
+            const bool there = mask >> slot & 1;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                v[r][c] = make_uint4(0, 0, 0, 0);
+                if (there) v[r][c] = ld_once(base + at + 128 * c + 16 * g);
+            }
+        }
+    }
+    __device__ __forceinline__ void scores(float (&s)[kN][4]) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                mma16816<T>(s[i], k[0][j].x, k[1][j].x, k[0][j].y, k[1][j].y, q[i][j][0], q[i][j][1]);
+                mma16816<T>(s[i], k[0][j].z, k[1][j].z, k[0][j].w, k[1][j].w, q[i][j][2], q[i][j][3]);
+            }
+        }
+    }
+    // scores to weights; their pieces as operands
+    __device__ __forceinline__ void weights(float (&s)[kN][4], unsigned int mask, float scale2, int lane, uint32_t (&hi)[kN][2], uint32_t (&lo)[kN][2]) {
+        const int g = lane / 4;
+        const bool there0 = mask >> g & 1, there1 = mask >> (g + 8) & 1;
+        bool rise = false;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            s[i][0] = there0 ? s[i][0] * scale2 : -INFINITY;
+            s[i][1] = there0 ? s[i][1] * scale2 : -INFINITY;
+            s[i][2] = there1 ? s[i][2] * scale2 : -INFINITY;
+            s[i][3] = there1 ? s[i][3] * scale2 : -INFINITY;
+            rise |= fmaxf(s[i][0], s[i][2]) > m[i][0] + (kLift + kSlack) || fmaxf(s[i][1], s[i][3]) > m[i][1] + (kLift + kSlack);
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(s[i][e], s[i][e + 2]);
+#pragma unroll
+                    for (int o_ = 4; o_ < 32; o_ <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o_));
+                    const float now = fmaxf(m[i][e], x - kLift), f = m[i][e] == now ? 1.f : ex2(m[i][e] - now);
+                    m[i][e] = now;
+                    l[i][e] *= f;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        o[i][j][e] *= f;
+                        o[i][j][e + 2] *= f;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float m0 = m[i][0] == -INFINITY ? 0.f : m[i][0], m1 = m[i][1] == -INFINITY ? 0.f : m[i][1];
+            const float p0 = ex2(s[i][0] - m0), p1 = ex2(s[i][1] - m1), p2 = ex2(s[i][2] - m0), p3 = ex2(s[i][3] - m1);
+            l[i][0] += p0 + p2;
+            l[i][1] += p1 + p3;
+            const uint32_t h0 = cut2<T>(p0, p1), h1 = cut2<T>(p2, p3);
+            const float2 r0 = unpack2<T>(h0), r1 = unpack2<T>(h1);
+            hi[i][0] = transpose8(h0);
+            hi[i][1] = transpose8(h1);
+            lo[i][0] = transpose8(cut2<T>(p0 - r0.x, p1 - r0.y) | 0x00010001u);
+            lo[i][1] = transpose8(cut2<T>(p2 - r1.x, p3 - r1.y) | 0x00010001u);
+        }
+    }
+    __device__ __forceinline__ void add(const uint32_t (&hi)[kN][2], const uint32_t (&lo)[kN][2]) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            const uint32_t *x0 = reinterpret_cast<const uint32_t *>(&v[0][c]), *x1 = reinterpret_cast<const uint32_t *>(&v[1][c]);
+            const uint32_t *x2 = reinterpret_cast<const uint32_t *>(&v[2][c]), *x3 = reinterpret_cast<const uint32_t *>(&v[3][c]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t a0 = __byte_perm(x0[e], x1[e], 0x5410), a1 = __byte_perm(x0[e], x1[e], 0x7632);
+                const uint32_t a2 = __byte_perm(x2[e], x3[e], 0x5410), a3 = __byte_perm(x2[e], x3[e], 0x7632);
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, hi[i][0], hi[i][1]);
+                    mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, lo[i][0], lo[i][1]);
+                }
+            }
+        }
+    }
+    // tiles [t0, t1) of a sequence of n slots
+    __device__ __forceinline__ void run(const PagedAttnArgs &a, const int *table, const char *kb, const char *vb, int t0, int t1, int n, int lane) {
+        Lookup<kTile> look;
+        long long ko, vo;
+        look.ask(a, table, t0, n, lane);
+        unsigned int mask = look.resolve(a, ko, vo);
+        load_k(kb, ko, mask, lane);
+        load_v(vb, vo, mask, lane);
+        if (t0 + 1 < t1) look.ask(a, table, t0 + 1, n, lane);
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+            float s[kN][4];
+            uint32_t hi[kN][2], lo[kN][2];
+            scores(s);
+            const unsigned int now = mask;
+            const bool more = t + 1 < t1;
+            if (more) {
+                mask = look.resolve(a, ko, vo);
+                load_k(kb, ko, mask, lane);
+                if (t + 2 < t1) look.ask(a, table, t + 2, n, lane);
+            }
+            weights(s, now, a.scale2, lane, hi, lo);
+            add(hi, lo);
+            if (more) load_v(vb, vo, mask, lane);
+        }
+    }
+    // the sums of 2^(s - m) over all lanes
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int o_ = 4; o_ < 32; o_ <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], o_);
+    }
+    // f(row, d, eight values from d on), and h(row, m, l) once a row
+    template <typename F, typename H>
+    __device__ __forceinline__ void each(int lane, F f, H h) const {
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * i + 2 * t + e;
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[2 * j] = o[i][4 * c + j][e];
+                        x[2 * j + 1] = o[i][4 * c + j][e + 2];
+                    }
+                    f(r, 64 * c + 8 * g, x, m[i][e], l[i][e]);
+                }
+                if (g == 0) h(r, m[i][e], l[i][e]);
+            }
+    }
+};
+
+// ----------------------------------------------------------------------------------------------------------------
+// 32-bit type: plain multiplications and additions, which the CUDA cores do fast enough for up to eight query heads on each byte
+// (one instruction for a key's element and head), with the rounding, infinities and NaN of 32 bits. Tiles of 8 slots. Scores: eight
+// lanes a key, 16 bytes of it each at a time; their sums for all heads are added up and spread over the eight lanes in one pass
+// (lane j of them ends up with head j). Values: a lane has four columns of all slots; the weights come from shared memory.
+template <int D, int kN>
+struct Core32 {
+    static constexpr int kTile = 8, kRows = kN;
+    static constexpr int kR = kN == 8 ? 2 : 1;  // scores of a lane
+    static constexpr int kV = D == 128 ? 8 : 4;  // values' rows of a lane
+    static constexpr float kSlack = 8.f;
+    float *sq, *sp;  // this warp's queries [kN][D] and weights [8][kN]
+    float o[kN][4], m, l;
+    float4 k[2][D / 32], v[kV];
+
+    __device__ __forceinline__ Core32(float *shared) : sq(shared), sp(shared + kN * D) {}
+    __device__ __forceinline__ void begin(const char *qrow, long long qs, int nq, float scale2, int lane) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kN * D / 128; ++i) {
+            const int e = 4 * (i * 32 + lane), r = e / D, d = e % D;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < nq) x = *reinterpret_cast<const float4 *>(qrow + r * qs + 4 * d);
+            *reinterpret_cast<float4 *>(sq + e) = x;
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+        __syncwarp();
+    }
+    static __device__ __forceinline__ float4 ld4(const char *p) {
+        const uint4 x = ld_once(p);
+        return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+    }
+    __device__ __forceinline__ void load_k(const char *base, long long off, unsigned int mask, int lane) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int slot = lane / 8 + 4 * r;
+            const long long at = __shfl_sync(0xffffffffu, off, slot);
+            const bool there = mask >> slot & 1;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                k[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (there) k[r][c] = ld4(base + at + 128 * c + 16 * (lane % 8));
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const char *base, long long off, unsigned int mask, int lane) {
+#pragma unroll
+        for (int r = 0; r < kV; ++r) {
+            const int slot = D == 128 ? r : 2 * r + lane / 16;
+            const long long at = __shfl_sync(0xffffffffu, off, slot);
+            v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mask >> slot & 1) v[r] = ld4(base + at + 16 * (lane % (D / 4)));
+        }
+    }
+    __device__ __forceinline__ void scores(float (&x)[kR], int lane) const {
+        const int j = lane % 8;
+        float s[2][kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) s[0][i] = s[1][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float4 y = *reinterpret_cast<const float4 *>(sq + i * D + 32 * c + 4 * j);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    s[r][i] = fmaf(k[r][c].x, y.x, s[r][i]);
+                    s[r][i] = fmaf(k[r][c].y, y.y, s[r][i]);
+                    s[r][i] = fmaf(k[r][c].z, y.z, s[r][i]);
+                    s[r][i] = fmaf(k[r][c].w, y.w, s[r][i]);
+                }
+            }
+        // halves of what is left go to the lane that keeps them
+        float w[2 * kN];
+#pragma unroll
+        for (int i = 0; i < 2 * kN; ++i) w[i] = kN == 8 ? s[i % 2][i / 2] : s[i / kN][i % kN];  // 8: heads outermost; 4: rows
+        int left = 2 * kN;
+#pragma unroll
+        for (int b = 4; b >= 1; b >>= 1) {
+            left /= 2;
+            const bool up = j & b;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                if (i >= left) break;
+                const float keep = up ? w[i + left] : w[i], send = up ? w[i] : w[i + left];
+                w[i] = keep + __shfl_xor_sync(0xffffffffu, send, b);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kR; ++r) x[r] = w[r];
+    }
+    __device__ __forceinline__ int slot_of(int r, int lane) const { return kN == 8 ? lane / 8 + 4 * r : lane / 8 + 4 * (lane % 8 / 4); }
+    __device__ __forceinline__ int head_of(int lane) const { return lane % kN; }
+    __device__ __forceinline__ void weights(float (&x)[kR], unsigned int mask, float scale2, int lane) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            x[r] = mask >> slot_of(r, lane) & 1 ? x[r] * scale2 : -INFINITY;
+            top = fmaxf(top, x[r]);
+        }
+        if (__any_sync(0xffffffffu, top > m + kSlack)) {
+#pragma unroll
+            for (int b = kN; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+            const float now = fmaxf(m, top), f = m == now ? 1.f : ex2(m - now);
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float g = __shfl_sync(0xffffffffu, f, i);
+                o[i][0] *= g; o[i][1] *= g; o[i][2] *= g; o[i][3] *= g;
+            }
+        }
+        const float m0 = m == -INFINITY ? 0.f : m;
+        __syncwarp();  // the last tile's weights have been read
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            const float p = ex2(x[r] - m0);
+            l += p;
+            sp[slot_of(r, lane) * kN + head_of(lane)] = p;
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void add(int lane) {
+#pragma unroll
+        for (int r = 0; r < kV; ++r) {
+            const int slot = D == 128 ? r : 2 * r + lane / 16;
+#pragma unroll
+            for (int i = 0; i < kN; i += 4) {
+                const float4 p = *reinterpret_cast<const float4 *>(sp + slot * kN + i);
+                const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[i + e][0] = fmaf(w[e], v[r].x, o[i + e][0]);
+                    o[i + e][1] = fmaf(w[e], v[r].y, o[i + e][1]);
+                    o[i + e][2] = fmaf(w[e], v[r].z, o[i + e][2]);
+                    o[i + e][3] = fmaf(w[e], v[r].w, o[i + e][3]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void run(const PagedAttnArgs &a, const int *table, const char *kb, const char *vb, int t0, int t1, int n, int lane) {
+        Lookup<kTile> look;
+        long long ko, vo;
+        look.ask(a, table, t0, n, lane);
+        unsigned int mask = look.resolve(a, ko, vo);
+        load_k(kb, ko, mask, lane);
+        load_v(vb, vo, mask, lane);
+        if (t0 + 1 < t1) look.ask(a, table, t0 + 1, n, lane);
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+            float x[kR];
+            scores(x, lane);
+            const unsigned int now = mask;
+            const bool more = t + 1 < t1;
+            if (more) {
+                mask = look.resolve(a, ko, vo);
+                load_k(kb, ko, mask, lane);
+                if (t + 2 < t1) look.ask(a, table, t + 2, n, lane);
+            }
+            weights(x, now, a.scale2, lane);
+            add(lane);
+            if (more) load_v(vb, vo, mask, lane);
+        }
+    }
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int b = kN; b < 32; b <<= 1) l += __shfl_xor_sync(0xffffffffu, l, b);
+        if (D == 64) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] += __shfl_xor_sync(0xffffffffu, o[i][e], 16);
+        }
+    }
+    template <typename F, typename H>
+    __device__ __forceinline__ void each(int lane, F f, H h) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float mi = __shfl_sync(0xffffffffu, m, i), li = __shfl_sync(0xffffffffu, l, i);
+            if (D == 128 || lane < 16) f(i, 4 * (lane % (D / 4)), o[i], mi, li);
+            if (lane == 0) h(i, mi, li);
+        }
+    }
+};
+
+// ----------------------------------------------------------------------------------------------------------------
+template <typename T, int N>
+__device__ __forceinline__ void store_row(char *p, const float (&x)[N], float f) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float y[4] = {x[i] * f, x[i + 1] * f, x[i + 2] * f, x[i + 3] * f};
+        store4(reinterpret_cast<T *>(p) + i, y);
+    }
+}
+__device__ __forceinline__ float over(float l) { return l == 0.f ? 0.f : 1.f / l; }  // a row that sees nothing gets 0
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f; }
+
+// A part of a sequence's head: [kRows][D] sums, then the maxima, then the sums of the weights.
+template <typename Core, int D> constexpr int kPartFloats = Core::kRows * (D + 2);
+
+template <typename T, int D, typename Core, int kPerSm>
+__global__ void __launch_bounds__(32 * kAttnWarps, kPerSm) k_paged_attn(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kSlots = 2 * kAttnWarps;
+    constexpr bool k32 = std::is_same<T, float>::value;
+    extern __shared__ __align__(16) float s_part[];  // kSlots parts; 32 bits: the warps' queries and weights behind them
+    struct Piece { int b, unit; long long first; int left, right; };  // left, right: whether the unit begins and ends in this piece
+    __shared__ Piece s_piece[kSlots];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    after_prior();
+    if (lane < 2) s_piece[2 * warp + lane].b = -1;
+    __syncwarp();
+    const TileList<kTile> list(a, lane, blockIdx.x == 0 && warp == 0);
+    const long long base = list.share * blockIdx.x;
+    long long p = base + warp_first(list.share, warp, kAttnWarps);
+    const long long end = min(base + warp_first(list.share, warp + 1, kAttnWarps), list.total);
+    Core core(k32 ? s_part + kSlots * kPart + warp * (Core::kRows * D + 8 * Core::kRows) : nullptr);
+    const int per_block = (a.group + a.blocks - 1) / a.blocks;
+    if (p < end) {
+        long long begin;
+        int b = list.find(p, lane, begin);
+        bool bad;
+        int tiles = row_tiles<kTile>(a, b, bad), places = (int)unit_places(tiles, list.kLeast);
+        int unit = (p - begin) >> 32 ? (int)((p - begin) / places) : (int)((uint32_t)(p - begin) / (uint32_t)places);
+        int off = (int)(p - begin - (long long)unit * places);
+        while (true) {
+            const int upto = (int)min((long long)places, off + (end - p)), real = min(upto, tiles);
+            if (off < real) {
+                const int h = unit / a.blocks, r0 = (unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
+                const int *table = a.tables + b * a.ts;
+                core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane);
+                core.run(a, table, a.kv[0] + h * a.st[0][1], a.kv[1] + h * a.st[1][1], off, real, a.lens[b] + 1, lane);
+                core.finish();
+                if (off == 0 && real == tiles) {
+                    char *out = a.out + b * a.os[0] + head * a.os[1];
+                    float *lse = a.lse ? a.lse + (long long)b * a.heads + head : nullptr;
+                    core.each(lane, [&](int r, int d, const auto &x, float, float l) { if (r < nq) store_row<T>(out + r * a.os[1] + d * (int)sizeof(T), x, over(l)); },
+                              [&](int r, float m, float l) { if (r < nq && lse) lse[r] = log_sum(m, l); });
+                } else {
+                    const int slot = 2 * warp + (off == 0);
+                    float *to = s_part + slot * kPart;
+                    core.each(lane, [&](int r, int d, const auto &x, float, float) {
+#pragma unroll
+                        for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); i += 4) *reinterpret_cast<float4 *>(to + r * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    }, [&](int r, float m, float l) { to[Core::kRows * D + r] = m; to[Core::kRows * (D + 1) + r] = l; });
+                    if (lane == 0) s_piece[slot] = {b, unit, 0, off == 0, real == tiles};
+                }
+            }
+            p += upto - off;
+            if (p >= end) break;
+            off = 0;
+            if (++unit == list.units) {
+                unit = 0;
+                do ++b; while ((tiles = row_tiles<kTile>(a, b, bad)) == 0);  // there is one: p < total
+                places = (int)unit_places(tiles, list.kLeast);
+            }
+        }
+    }
+    __syncthreads();
+    // join the pieces that the warps left, in their order; what is not a whole unit goes to the workspace
+    for (int s = 0; s < kSlots;) {
+        const Piece first = s_piece[s];
+        int e = s + 1;
+        if (first.b < 0) { s = e; continue; }
+        bool right = first.right;
+        for (; e < kSlots; ++e) {
+            const Piece x = s_piece[e];
+            if (x.b < 0) continue;
+            if (x.b != first.b || x.unit != first.unit) break;
+            right = x.right;
+        }
+        const int h = first.unit / a.blocks, r0 = (first.unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
+        const bool whole = first.left && right;
+        float *to = a.part + (2ll * blockIdx.x + first.left) * kPart;
+        for (int i = threadIdx.x; i < nq * (D / 4); i += 32 * kAttnWarps) {
+            const int r = i / (D / 4), d = 4 * (i % (D / 4));
+            float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int j = s; j < e; ++j)
+                if (s_piece[j].b >= 0) top = fmaxf(top, s_part[j * kPart + Core::kRows * D + r]);
+            for (int j = s; j < e; ++j) {
+                if (s_piece[j].b < 0) continue;
+                const float *from = s_part + j * kPart, m = from[Core::kRows * D + r], f = m == top ? 1.f : ex2(m - top);
+                const float4 y = *reinterpret_cast<const float4 *>(from + r * D + d);
+                l += f * from[Core::kRows * (D + 1) + r];
+                x[0] += f * y.x; x[1] += f * y.y; x[2] += f * y.z; x[3] += f * y.w;
+            }
+            if (whole) {
+                store_row<T>(a.out + first.b * a.os[0] + (head + r) * a.os[1] + d * (int)sizeof(T), x, over(l));
+                if (d == 0 && a.lse) a.lse[(long long)first.b * a.heads + head + r] = log_sum(top, l);
+            } else {
+                *reinterpret_cast<float4 *>(to + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d == 0) {
+                    to[Core::kRows * D + r] = top;
+                    to[Core::kRows * (D + 1) + r] = l;
+                }
+            }
+        }
+        s = e;
+    }
+}
+
+// The second launch: kWarps warps for each query head of a sequence look where its tiles were; where that is more than one CTA,
+// they add the parts up (a warp every kWarps-th of them), in one order.
+template <typename T, int D, typename Core, int kWarps>
+__global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kE = D / 32;
+    __shared__ float s_x[8][D], s_m[8], s_l[8];
+    after_prior();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % kWarps;
+    const long long row = (long long)blockIdx.x * (8 / kWarps) + warp / kWarps;
+    const bool there = row < (long long)a.batch * a.heads;
+    const int b = there ? (int)(row / a.heads) : 0, head = there ? (int)(row - (long long)b * a.heads) : 0, h = head / a.group, per_block = (a.group + a.blocks - 1) / a.blocks;
+    const int blk = (head - h * a.group) / per_block, r = head - h * a.group - blk * per_block;
+    const TileList<kTile> list(a, lane, false);
+    bool bad;
+    const int tiles = row_tiles<kTile>(a, b, bad);
+    // the places before this sequence
+    long long before = 0;
+    const int l0 = b / list.per;
+    for (int i = l0 * list.per + lane; i < b; i += 32) {
+        bool x;
+        before += unit_places(row_tiles<kTile>(a, i, x), list.kLeast);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const long long upto = __shfl_sync(0xffffffffu, list.upto, l0 > 0 ? l0 - 1 : 0);
+    const long long begin = before * list.units + (l0 > 0 ? upto : 0) + (long long)(h * a.blocks + blk) * unit_places(tiles, list.kLeast);
+    const int c0 = (int)(begin / list.share), c1 = tiles ? (int)((begin + tiles - 1) / list.share) : c0;
+    float x[kE], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) x[i] = 0.f;
+    const bool split = there && c1 > c0;
+    if (split) {
+#pragma unroll 4
+        for (int c = c0 + mine; c <= c1; c += kWarps) {
+            const float *from = a.part + (2ll * c + (c == c0)) * kPart;
+            const float pm = from[Core::kRows * D + r], pl = from[Core::kRows * (D + 1) + r], now = fmaxf(m, pm);
+            const float f = m == now ? 1.f : ex2(m - now), g = pm == now ? 1.f : ex2(pm - now);
+            m = now;
+            l = l * f + pl * g;
+#pragma unroll
+            for (int i = 0; i < kE; ++i) x[i] = x[i] * f + from[r * D + kE * lane + i] * g;
+        }
+    }
+    if (kWarps > 1) {
+        if (split) {
+#pragma unroll
+            for (int i = 0; i < kE; ++i) s_x[warp][kE * lane + i] = x[i];
+            if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+        }
+        __syncthreads();
+        if (mine) return;
+        if (split) {
+            for (int w = warp + 1; w < warp + kWarps; ++w) {
+                const float pm = s_m[w], now = fmaxf(m, pm), f = m == now ? 1.f : ex2(m - now), g = pm == now ? 1.f : ex2(pm - now);
+                m = now;
+                l = l * f + s_l[w] * g;
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[i] = x[i] * f + s_x[w][kE * lane + i] * g;
+            }
+        }
+    }
+    if (split) {
+        T *out = reinterpret_cast<T *>(a.out + b * a.os[0] + head * a.os[1]) + kE * lane;
+        const float f = over(l);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) out[i] = from_f<T>(x[i] * f);
+        if (lane == 0 && a.lse) a.lse[(long long)b * a.heads + head] = log_sum(m, l);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// rows of a warp's tile: the query heads of a cache head in equal blocks of at most 16 (16 bits) or 8 (32 bits)
+int attn_blocks(const p8_paged *c, int64_t heads) {
+    const int64_t group = heads / c->heads, most = c->type == P8_KV_F32 ? 8 : 16;
+    return (int)((group + most - 1) / most);
+}
+bool attn_wide(const p8_paged *c, int64_t heads) {  // the larger of the two tiles
+    const int64_t group = heads / c->heads, blocks = attn_blocks(c, heads), rows = (group + blocks - 1) / blocks;
+    return c->type == P8_KV_F32 ? rows > 4 : rows > 8;
+}
+int attn_per_sm(const p8_paged *c, int64_t heads) { return c->type != P8_KV_F32 && attn_wide(c, heads) ? 2 : 3; }
+int attn_rows(const p8_paged *c, int64_t heads) { return (c->type == P8_KV_F32 ? 4 : 8) * (attn_wide(c, heads) ? 2 : 1); }
+// Whether a unit can be cut at all: not where each has a CTA's least share to itself and no sequence can be longer.
+bool attn_cuts(const p8_paged *c, int64_t heads) {
+    const int64_t units = c->rows * c->heads * attn_blocks(c, heads), ctas = (int64_t)sm_count() * attn_per_sm(c, heads);
+    return c->columns * c->page > kSpan || units > ctas;
+}
+size_t paged_attn_workspace(const p8_paged *c, int64_t heads) {
+    if (!attn_cuts(c, heads)) return 0;
+    return (size_t)sm_count() * attn_per_sm(c, heads) * 2 * attn_rows(c, heads) * (c->width + 2) * 4;
+}
+
+template <typename T, int D, typename Core, int kPerSm>
+p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
+    constexpr bool k32 = std::is_same<T, float>::value;
+    constexpr int smem = 4 * (2 * kAttnWarps * kPartFloats<Core, D> + (k32 ? kAttnWarps * Core::kRows * (D + 8) : 0));
+    const auto kernel = k_paged_attn<T, D, Core, kPerSm>;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return P8_ERR_CUDA;
+    const bool cuts = attn_cuts(c, a.heads);
+    const int64_t units = c->rows * c->heads * a.blocks;
+    const int64_t most = units * ((c->columns * c->page + kSpan - 1) / kSpan);  // shares that there can be
+    if (launch_after(kernel, dim3((unsigned int)std::min<int64_t>(a.ctas, most)), dim3(32 * kAttnWarps), (size_t)smem, st, a) != cudaSuccess) return P8_ERR_CUDA;
+    if (!cuts) return P8_OK;
+    const int64_t rows = c->rows * a.heads;
+    if (a.ctas >= 4 * units) return done(launch_after(k_paged_join<T, D, Core, 8>, dim3((unsigned int)rows), dim3(256), 0, st, a));
+    return done(launch_after(k_paged_join<T, D, Core, 1>, dim3((unsigned int)((rows + 7) / 8)), dim3(256), 0, st, a));
+}
+template <int D>
+p8_status run_paged_attn_d(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
+    const bool wide = attn_wide(c, a.heads);
+    if (c->type == P8_KV_F32) return wide ? run_paged_attn<float, D, Core32<D, 8>, 3>(c, a, st) : run_paged_attn<float, D, Core32<D, 4>, 3>(c, a, st);
+    if (c->type == P8_KV_F16) return wide ? run_paged_attn<__half, D, Core16<__half, D, 2>, 2>(c, a, st) : run_paged_attn<__half, D, Core16<__half, D, 1>, 3>(c, a, st);
+    return wide ? run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 2>, 2>(c, a, st) : run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 1>, 3>(c, a, st);
+}
+
+p8_status launch_paged_attn(const p8_paged *c, const p8_paged_attn_args *x, void *workspace, cudaStream_t st) {
+    const int es = elem_size(c->type);
+    PagedAttnArgs a;
+    a.q = (const char *)x->q; a.out = (char *)x->out;
+    for (int i = 0; i < 2; ++i) { a.qs[i] = x->q_stride[i] * es; a.os[i] = x->out_stride[i] * es; }
+    a.kv[0] = (const char *)c->k; a.kv[1] = (const char *)c->v;
+    for (int i = 0; i < 3; ++i) { a.st[0][i] = c->k_stride[1 + i] * es; a.st[1][i] = c->v_stride[1 + i] * es; }
+    a.tables = c->tables; a.ts = c->table_stride; a.lens = x->lens; a.counts = x->counts;
+    a.lse = x->lse; a.part = (float *)workspace;
+    a.slots = c->columns * c->page; a.div = page_div((uint32_t)c->page);
+    a.batch = (int)c->rows; a.heads = (int)x->heads; a.kvh = (int)c->heads; a.group = (int)(x->heads / c->heads); a.blocks = attn_blocks(c, x->heads);
+    a.pages = (int)c->pages; a.ctas = sm_count() * attn_per_sm(c, x->heads);
+    a.scale2 = (float)x->scale * 1.4426950408889634f;
+    return c->width == 128 ? run_paged_attn_d<128>(c, a, st) : run_paged_attn_d<64>(c, a, st);
+}

@@ -1,0 +1,60 @@
+// p8_paged_index.h -- index arithmetic of the paged cache and beam search operators; plain C++, so that it is also tested on the host.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define P8_HD __host__ __device__ __forceinline__
+#else
+#define P8_HD inline
+#endif
+
+namespace p8 {
+
+// slot / page for 0 <= slot < 2^31, 1 <= page <= 2^20, by a multiplication: with l = ceil(log2 page), mul = ceil(2^(31 + l) /
+// page) < 2^32 is off by e < page <= 2^l, so slot mul / 2^(31 + l) is above slot / page by slot e / (page 2^(31 + l)) < 1 / page.
+struct PageDiv {
+    uint32_t size, mul, shift;
+};
+P8_HD PageDiv page_div(uint32_t page) {
+    uint32_t l = 0;
+    while ((uint64_t(1) << l) < page) ++l;
+    return {page, (uint32_t)(((uint64_t(1) << (31 + l)) + page - 1) / page), 31 + l};
+}
+P8_HD uint32_t page_of(const PageDiv &d, uint32_t slot) { return (uint32_t)(((uint64_t)slot * d.mul) >> d.shift); }
+
+// Places of a sequence's head in the attention's list of tiles: one for each of its tiles, `least` at least (a place costs
+// nothing where there is no tile; short sequences then begin where a CTA's share does and stay in one piece).
+P8_HD int64_t unit_places(int64_t tiles, int64_t least) { return tiles == 0 ? 0 : tiles < least ? least : tiles; }
+// Each CTA's share of `total` places.
+P8_HD int64_t cta_share(int64_t total, int64_t ctas, int64_t least) {
+    const int64_t s = total >> 32 ? (total + ctas - 1) / ctas : (int64_t)(((uint32_t)total + (uint32_t)ctas - 1) / (uint32_t)ctas);
+    return s < least ? least : s;
+}
+// Warp w's part of a share, from its first place.
+P8_HD int64_t warp_first(int64_t share, int w, int warps) { return (share * w) / warps; }
+
+// The position of the k-th set bit (k = 0: the lowest) of a word that has more than k.
+P8_HD int nth_bit(uint64_t m, int k) {
+    for (; k > 0; --k) m &= m - 1;
+#ifdef __CUDA_ARCH__
+    return __ffsll((long long)m) - 1;
+#else
+    return __builtin_ctzll(m);
+#endif
+}
+
+// A float's bits (not those of -0) as an integer of the same order, and back.
+P8_HD uint32_t order_key(uint32_t bits) { return bits & 0x80000000u ? ~bits : bits | 0x80000000u; }
+P8_HD uint32_t order_bits(uint32_t key) { return key & 0x80000000u ? key & 0x7fffffffu : ~key; }
+
+// Blocks of one row of logits: enough for four on every SM, none with less than `least` logits, so few for many beams that
+// the `lists` of a group stay within 256.
+P8_HD int64_t select_splits(int64_t rows, int64_t beams, int64_t vocab, int64_t sms, int64_t least) {
+    int64_t s = (4 * sms + rows - 1) / rows;
+    const int64_t most = 256 / beams, fit = (vocab + least - 1) / least;
+    if (s > most) s = most;
+    if (s > fit) s = fit;
+    return s < 1 ? 1 : s;
+}
+
+}  // namespace p8

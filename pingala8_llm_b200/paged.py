@@ -1,0 +1,180 @@
+"""Serving operators: a key/value cache in pages that sequences share, and beam search on it.
+
+Keys and values are a pair of tensors [pages, kv heads, page slots, width] (float32, float16 or bfloat16; width 64 or 128; any
+number of slots in a page), or with a leading layer dimension for beam_reorder. Any strides whose rows start on 16
+bytes and have unit stride inside. Slot s of sequence b is slot s % page of page tables[b, s // page]; tables int32
+[batch, columns] is one for all layers, and entries that no sequence has come to yet may hold anything. Sequence b is as long as the int32
+device tensor lens[b] says and the device alone reads it, so calls can be captured in a CUDA graph and replayed while
+sequences grow. Several sequences may read a page (a prompt's pages under all of its beams); only one writes to it at a time.
+
+One step of beam search, `lens` [batch * beams]:
+
+    q = paged_append(q, k, v, k_pages, v_pages, tables, lens, lens[:, None], cos, sin)      # per layer
+    out, lse = paged_attention(q[:, 0], k_pages, v_pages, tables, lens)                     # per layer
+    best = beam_select(logits, scores, done=done, end=end)
+    lens += 1
+    beam_reorder(best.parents, all_k, all_v, tables, lens)
+
+Every call goes through the C ABI of libpingala8_b200.so on the tensors' device, on its current stream or the one
+given; there is no CPU path and no gradient. Lengths, counts, positions, pages and parents that are out of range leave their
+sequence, token or group out and set bit 64 of device_error(). Outputs overlap neither one another nor what a call reads, but where
+"in place" is said; a tensor expanded over a dimension (stride 0) is no output.
+"""
+import ctypes as C
+import math
+from collections import namedtuple
+
+import torch
+
+from ._lib import check, lib
+
+try:
+    from . import _paged_calls as _c
+except ImportError as e:
+    raise ImportError(f"{e}: build it with `python -m pingala8_llm_b200.build` (no fallback)") from e
+
+_c.bind(*(C.cast(getattr(lib(), n), C.c_void_p).value
+          for n in ("p8_paged_append", "p8_paged_attn_workspace", "p8_paged_attn", "p8_beam_select_workspace", "p8_beam_select", "p8_beam_reorder")))
+
+BEAMS_MAX = 64
+CANDIDATES_MAX = 64
+
+Best = namedtuple("Best", "scores parents tokens done")
+
+
+def _refuse(what):
+    raise ValueError(what)
+
+
+def _on(stream, like, call, *args, **kw):
+    """the call with the caller's stream current, for the launch and for what it allocates"""
+    if stream.device != like.device:
+        _refuse("the stream must belong to the tensors' device")
+    with torch.cuda.stream(stream):
+        return call(*args, **kw)
+
+
+def rotary_tables(positions, width, theta=10000.0, kind=None, factor=1.0, original=None, low=1.0, high=4.0, device=None):
+    """cos and sin float32 [positions, width / 2] of the angles position * theta^(-2 i / width) (computed in 64 bits), for
+    heads of which `width` elements turn; positions: how many, from 0 on. For contexts `factor` times as long as the
+    model was trained on, kind says how the angles are slowed down:
+
+      "linear"  all by 1 / factor
+      "theta"   by a larger theta, theta * factor^(width / (width - 2)): the slowest by 1 / factor, the fastest not at all
+      "bands"   those that turn less than `low` times within the `original` context by 1 / factor, those that turn more than
+                `high` times not at all, in between in proportion to the turns
+      "ramp"    those that turn less than `low` times by 1 / factor, more than `high` times not at all, in between linearly in i;
+                cos and sin times 0.1 ln(factor) + 1 (low 1, high 32 is usual)
+    """
+    if width < 2 or width % 2 or positions < 1 or not theta > 0:
+        _refuse("an even width, one position or more, theta above 0")
+    if kind not in (None, "linear", "theta", "bands", "ramp") or not factor >= 1:
+        _refuse("kind must be None, 'linear', 'theta', 'bands' or 'ramp', and factor 1 or more")
+    if kind in ("bands", "ramp") and (original is None or not original >= 1 or not 0 < low < high):
+        _refuse(f"'{kind}' needs the original context and 0 < low < high")
+    if kind == "theta" and width < 4:
+        _refuse("'theta' needs a width of 4 or more")
+    if kind == "theta":
+        theta = theta * factor ** (width / (width - 2))
+    i = torch.arange(width // 2, dtype=torch.float64, device=device)
+    inv = theta ** (-2 * i / width)
+    gain = 1.0
+    if kind == "linear":
+        inv = inv / factor
+    elif kind == "bands":
+        keep = ((original * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        inv = inv * (keep + (1 - keep) / factor)
+    elif kind == "ramp":
+        at = lambda turns: width * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta))  # noqa: E731  the i that turns so often
+        first, last = max(math.floor(at(high)), 0), min(math.ceil(at(low)), width - 1)
+        keep = 1 - ((i - first) / max(last - first, 1e-3)).clamp(0, 1)
+        inv = inv * (keep + (1 - keep) / factor)
+        gain = 0.1 * math.log(factor) + 1
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
+    return (torch.cos(angle) * gain).float(), (torch.sin(angle) * gain).float()
+
+
+def paged_append(q, k, v, k_pages, v_pages, tables, lens, pos, cos, sin, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, counts=None, q_out=None, stream=None):
+    """New tokens into the pages: q float32 [batch, tokens, heads, width], k and v float32 [batch, tokens, kv heads,
+    width] (views of the projections' outputs) -> rotated queries in the cache's type; rotated keys and plain values in
+    slots lens[b], lens[b] + 1, ... of the pages that tables [batch, columns] names.
+
+    pos int32 [batch, tokens]: each token's row of cos / sin float32 [positions, R / 2] (rotary_tables). The first R elements of a head
+    turn (a multiple of 8), as pairs (i, i + R / 2) or, interleaved, (2 i, 2 i + 1); the others stay. q_norm, k_norm float32
+    [width]: RMSNorm per head before the rotation. counts int32 [batch]: how many of the tokens are real; what belongs to the
+    others is not written. q_out may be q (in place) where the cache is float32."""
+    if stream is not None:
+        return _on(stream, k_pages, paged_append, q, k, v, k_pages, v_pages, tables, lens, pos, cos, sin, interleaved, q_norm, k_norm, eps, counts, q_out)
+    if q_out is None:
+        q_out = (torch.empty if counts is None else torch.zeros)(q.shape, dtype=k_pages.dtype, device=k_pages.device)
+    st = _c.paged_append(q, k, v, k_pages, v_pages, tables, lens, pos, cos, sin, interleaved, q_norm, k_norm, eps, counts, q_out)
+    if st:
+        check(st, "p8_paged_append")
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, tables, lens, counts=None, scale=None, out=None, lse=None, workspace=None, stream=None):
+    """Attention of one new token per sequence, q [batch, heads, width] in the cache's type, over slots 0 .. lens[b] (its own key
+    and value already in slot lens[b]: paged_append with the same lens). Returns (out like q, lse float32 [batch, heads]):
+    the softmax average of the values and the natural log of the sum of exponentials. counts int32 [batch], 0 or 1: sequences with 0
+    have no token; their rows are not written. scale: 1 / sqrt(width) unless given. Slots whose page is out of range count as not there;
+    a token that sees nothing gets 0 and -inf."""
+    if stream is not None:
+        return _on(stream, k_pages, paged_attention, q, k_pages, v_pages, tables, lens, counts, scale, out, lse, workspace)
+    if out is None:
+        out = (torch.empty if counts is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = (torch.empty if counts is None else torch.zeros)(q.shape[:2], dtype=torch.float32, device=q.device)
+    st = _c.paged_attention(q, k_pages, v_pages, tables, lens, counts, scale, out, lse, workspace)
+    if st:
+        check(st, "p8_paged_attn")
+    return out, lse
+
+
+def attention_workspace_size(k_pages, v_pages, tables, heads):
+    """workspace bytes of paged_attention, for callers that keep their own"""
+    return _c.attention_workspace(k_pages, v_pages, tables, heads)
+
+
+def beam_select(logits, scores, done=None, end=None, candidates=None, out_scores=None, parents=None, tokens=None, out_done=None, workspace=None, stream=None):
+    """The best continuations of each group of beams: logits [batch, beams, vocabulary] (float32, float16 or bfloat16, any strides
+    with unit stride inside; one beam's may be expanded over the others), scores float32 [batch, beams]: each beam's sum of log
+    probabilities so far (-inf: no such beam). done bool [batch, beams]: beams that have ended with the token `end` go on as
+    they are, as one candidate.
+
+    Returns Best(scores float32, parents int32, tokens int64, done bool), all [batch, candidates] (as many as beams unless given; 1 to
+    64), the best first; of equal logits of a beam the lowest token, of equal totals the lowest beam. Where there are fewer
+    continuations: score -inf, parent -1, token -1. Logits of -inf or NaN are no continuations."""
+    if stream is not None:
+        return _on(stream, logits, beam_select, logits, scores, done, end, candidates, out_scores, parents, tokens, out_done, workspace)
+    n = logits.shape[1] if candidates is None and logits.dim() == 3 else candidates
+    if out_scores is None or parents is None or tokens is None or out_done is None:
+        if isinstance(n, bool) or not isinstance(n, int) or not 1 <= n <= CANDIDATES_MAX:
+            _refuse(f"1 to {CANDIDATES_MAX} candidates")
+        new = lambda given, dtype: torch.empty(logits.shape[0], n, dtype=dtype, device=logits.device) if given is None else given  # noqa: E731
+        out_scores, parents, tokens, out_done = new(out_scores, torch.float32), new(parents, torch.int32), new(tokens, torch.int64), new(out_done, torch.bool)
+    st = _c.beam_select(logits, scores, done, end, n, out_scores, parents, tokens, out_done, workspace)
+    if st:
+        check(st, "p8_beam_select")
+    return Best(out_scores, parents, tokens, out_done)
+
+
+def select_workspace_size(logits, candidates):
+    """workspace bytes of beam_select, for callers that keep their own"""
+    return _c.select_workspace(logits, candidates)
+
+
+def beam_reorder(parents, k_pages, v_pages, tables, lens, stream=None):
+    """The beams go on from their parents: parents int32 [batch, beams], tables int32 [batch * beams, columns] and lens int32
+    [batch * beams] (one length for all beams of a group), pages [layers, pages, kv heads, page slots, width] or without layers. In place.
+
+    Full pages of a beam are its parent's from now on. The page that a group's beams are in the middle of goes from the parent to its
+    lowest child; every further child takes the one of a beam that has no child, with a copy of what is in the parent's. Columns
+    behind it stay, so that a beam can be given the pages of all its future slots beforehand; the begun and future pages of the
+    beams must be different ones. parents -1: the beam goes on as it is. Returns tables."""
+    if stream is not None:
+        return _on(stream, k_pages, beam_reorder, parents, k_pages, v_pages, tables, lens)
+    st = _c.beam_reorder(parents, k_pages, v_pages, tables, lens)
+    if st:
+        check(st, "p8_beam_reorder")
+    return tables
