@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -38,6 +39,18 @@ int sm_count() {
         n[dev].store(v, std::memory_order_relaxed);
     }
     return v;
+}
+
+// Raises a kernel's limit of dynamic shared memory, once on each device; `slot` says which kernel it is.
+template <typename K>
+bool allow_shared(K *kernel, int64_t slot, int bytes) {
+    static std::atomic<unsigned long long> done_on[64];
+    int dev = 0;
+    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && slot < 64;
+    if (known && (done_on[dev].load(std::memory_order_acquire) >> slot & 1)) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    if (known) done_on[dev].fetch_or(1ull << slot, std::memory_order_release);
+    return true;
 }
 
 // ----------------------------------------------------------------------------------------------------------------

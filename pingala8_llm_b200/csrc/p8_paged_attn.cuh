@@ -98,9 +98,9 @@ __device__ __forceinline__ uint4 ld_once(const char *p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-__device__ __forceinline__ float ex2(float x) {
+__device__ __forceinline__ float ex2(float x) {  // 0 below 2^-126, which is nothing beside the sums here: the largest term of each is 1 or more
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

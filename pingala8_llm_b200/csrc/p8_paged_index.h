@@ -47,14 +47,20 @@ P8_HD int nth_bit(uint64_t m, int k) {
 P8_HD uint32_t order_key(uint32_t bits) { return bits & 0x80000000u ? ~bits : bits | 0x80000000u; }
 P8_HD uint32_t order_bits(uint32_t key) { return key & 0x80000000u ? key & 0x7fffffffu : ~key; }
 
-// Blocks of one row of logits: enough for four on every SM, none with less than `least` logits, so few for many beams that
-// the `lists` of a group stay within 256.
-P8_HD int64_t select_splits(int64_t rows, int64_t beams, int64_t vocab, int64_t sms, int64_t least) {
-    int64_t s = (4 * sms + rows - 1) / rows;
+// Blocks of one row of logits, none with less than `least` of them, and so few for many beams that the pieces of a group stay within
+// 256. With `slots` blocks at a time the rows take as long as the blocks of one slot, one after the other: their logits, and for each
+// block what it takes beside them (`extra`, in logits). The number that makes this least.
+P8_HD int64_t select_splits(int64_t rows, int64_t beams, int64_t vocab, int64_t slots, int64_t least, int64_t extra) {
     const int64_t most = 256 / beams, fit = (vocab + least - 1) / least;
-    if (s > most) s = most;
-    if (s > fit) s = fit;
-    return s < 1 ? 1 : s;
+    int64_t best = 1, best_cost = INT64_MAX;
+    for (int64_t s = 1; s <= most && s <= fit; ++s) {
+        const int64_t cost = (rows * s + slots - 1) / slots * ((vocab + s - 1) / s + extra);
+        if (cost < best_cost) {
+            best = s;
+            best_cost = cost;
+        }
+    }
+    return best;
 }
 
 }  // namespace p8

@@ -526,8 +526,9 @@ def test_select_strides_first_step_and_far_scores():
     assert best.parents.eq(0).all()
     turned = randn(g, 4, 3, V).transpose(0, 1)  # beams before groups
     check_select(paged.beam_select(turned, torch.zeros(3, 4, device="cuda"), candidates=4), select_ref(turned, torch.zeros(3, 4), None, None, 4), V)
-    big = randn(g, 1, 2, V, scale=1e37)
-    check_select(paged.beam_select(big, torch.zeros(1, 2, device="cuda")), select_ref(big, torch.zeros(1, 2), None, None, 2), V)
+    for scale in (1e-30, 1e-3, 1e4, 1e7, 2e8, 4e8, 1e10, 1e37):
+        big = randn(g, 1, 2, V, scale=scale)
+        check_select(paged.beam_select(big, torch.zeros(1, 2, device="cuda")), select_ref(big, torch.zeros(1, 2), None, None, 2), V)
     ended()
 
 

@@ -26,7 +26,7 @@ int64_t warp_first(int64_t s, int w, int n) { return p8::warp_first(s, w, n); }
 int nth_bit(uint64_t m, int k) { return p8::nth_bit(m, k); }
 uint32_t order_key(uint32_t b) { return p8::order_key(b); }
 uint32_t order_bits(uint32_t k) { return p8::order_bits(k); }
-int64_t select_splits(int64_t r, int64_t b, int64_t v, int64_t s, int64_t l) { return p8::select_splits(r, b, v, s, l); }
+int64_t select_splits(int64_t r, int64_t b, int64_t v, int64_t s, int64_t l, int64_t x) { return p8::select_splits(r, b, v, s, l, x); }
 }
 """
 
@@ -39,7 +39,7 @@ def ix(tmp_path_factory):
     L = C.CDLL(str(d / "x.so"))
     i64, u32, u64 = C.c_int64, C.c_uint32, C.c_uint64
     for name, res, args in (("page_of_", u32, [u32, u32]), ("wrong", i64, [u32, u32]), ("unit_places", i64, [i64, i64]), ("cta_share", i64, [i64, i64, i64]), ("warp_first", i64, [i64, C.c_int, C.c_int]),
-                            ("nth_bit", C.c_int, [u64, C.c_int]), ("order_key", u32, [u32]), ("order_bits", u32, [u32]), ("select_splits", i64, [i64] * 5)):
+                            ("nth_bit", C.c_int, [u64, C.c_int]), ("order_key", u32, [u32]), ("order_bits", u32, [u32]), ("select_splits", i64, [i64] * 6)):
         getattr(L, name).restype, getattr(L, name).argtypes = res, args
     return L
 
@@ -137,6 +137,6 @@ def test_shares_cover_every_tile_once_and_the_join_finds_all_parts(ix, seed):
 def test_rows_of_logits_are_split_within_the_lists(ix):
     for rows, beams in ((1, 1), (4, 4), (12, 4), (256, 8), (64, 64), (4096 * 64, 64), (3, 3), (7, 1)):
         for vocab in (1, 15, 4096, 4097, 50001, 151936, 2 ** 31 - 65537):
-            s = ix.select_splits(rows, beams, vocab, 148, 4096)
-            chunk = (-(-vocab // s) + 15) // 16 * 16
+            s = ix.select_splits(rows, beams, vocab, 444, 4096, 100000)
+            chunk = (-(-vocab // s) + 127) // 128 * 128
             assert 1 <= s and s * beams <= 256 and chunk * s >= vocab and chunk * s < 2 ** 31
