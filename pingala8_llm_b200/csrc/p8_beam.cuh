@@ -672,7 +672,7 @@ struct ReorderArgs {
     const int *parents, *lens;
     long long ts, slots, columns;
     PageDiv div;
-    int batch, beams, heads, pages, row_bytes, chunks, alone;  // chunks: blocks of a page; alone: there is no first launch
+    int batch, beams, heads, pages, row_bytes, segments, alone;  // segments: layers x keys and values x heads; alone: there is no first launch
 };
 struct BeamPlan {
     bool ok;
@@ -717,39 +717,45 @@ __device__ __forceinline__ int page_from(const BeamPlan &r, int i) {
     return nth_bit(r.childless, __popcll(r.further & ((1ull << i) - 1)));
 }
 
-constexpr int kMoveUnits = 8;  // 16 bytes each, of a thread
+constexpr int kMoveUnits = 8;  // 16 bytes each, of a lane in flight
 
+// Block (k, part) copies a part of the begun page of a group's k-th further child: a warp takes the slots of one layer's keys or values
+// and head at a time, which lie side by side.
 __global__ void __launch_bounds__(256) k_beam_move(const __grid_constant__ ReorderArgs a) {
     after_prior();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, b = row / a.beams, i = row - b * a.beams, lane = threadIdx.x % 32;
-    const int layer = blockIdx.y / 2, z = blockIdx.y % 2;
+    const int most = a.beams - 1, b = blockIdx.x / most, k = blockIdx.x - b * most, lane = threadIdx.x % 32;
     const BeamPlan r = beam_plan(a, b, lane);
-    if (!r.ok || !(r.further >> i & 1)) return;
-    const int full = (int)page_of(a.div, (unsigned int)r.len), rest = r.len - full * (int)a.div.size, per = a.row_bytes / 16;
-    const int items = rest * a.heads * per, first = chunk * 256 * kMoveUnits;
-    if (first >= items) return;
-    const int src = a.tables[((long long)b * a.beams + r.parent(i)) * a.ts + full], dst = a.tables[((long long)b * a.beams + page_from(r, i)) * a.ts + full];
+    if (!r.ok || k >= __popcll(r.further)) return;
+    const int full = (int)page_of(a.div, (unsigned int)r.len), rest = r.len - full * (int)a.div.size;
+    if (rest == 0) return;
+    const int i = nth_bit(r.further, k);
+    const int *table = a.tables + (long long)b * a.beams * a.ts + full;
+    const int src = table[r.parent(i) * a.ts], dst = table[nth_bit(r.childless, k) * a.ts];
     if ((unsigned int)src >= (unsigned int)a.pages || (unsigned int)dst >= (unsigned int)a.pages) {
         if (threadIdx.x == 0) out_of_range();
         return;
     }
-    const char *from = a.kv[z] + layer * a.st[z][0] + src * a.st[z][1];
-    char *to = a.kv[z] + layer * a.st[z][0] + dst * a.st[z][1];
-    uint4 v[kMoveUnits];
-    long long at[kMoveUnits];
+    const int shift = 31 - __clz(a.row_bytes / 16), units = rest << shift;  // a row is 8, 16 or 32 units
+    for (int seg = blockIdx.y * 8 + threadIdx.x / 32; seg < a.segments; seg += gridDim.y * 8) {
+        const int lz = seg / a.heads, h = seg - lz * a.heads, z = lz & 1;
+        const char *base = a.kv[z] + (lz >> 1) * a.st[z][0] + h * a.st[z][2];
+        const char *from = base + src * a.st[z][1];
+        char *to = const_cast<char *>(base) + dst * a.st[z][1];
+        for (int u0 = lane; u0 < units; u0 += 32 * kMoveUnits) {
+            uint4 v[kMoveUnits];
 #pragma unroll
-    for (int j = 0; j < kMoveUnits; ++j) {
-        const int k = first + 256 * j + threadIdx.x;
-        if (k < items) {
-            const int unit = k % per, hs = k / per, h = hs / rest, s = hs - h * rest;
-            at[j] = h * a.st[z][2] + s * a.st[z][3] + 16 * unit;
-            v[j] = *reinterpret_cast<const uint4 *>(from + at[j]);
+            for (int j = 0; j < kMoveUnits; ++j) {
+                const int u = u0 + 32 * j;
+                if (u < units) v[j] = *reinterpret_cast<const uint4 *>(from + (u >> shift) * a.st[z][3] + 16 * (u & ((1 << shift) - 1)));
+            }
+#pragma unroll
+            for (int j = 0; j < kMoveUnits; ++j) {
+                const int u = u0 + 32 * j;
+                if (u < units) *reinterpret_cast<uint4 *>(to + (u >> shift) * a.st[z][3] + 16 * (u & ((1 << shift) - 1))) = v[j];
+            }
         }
     }
-#pragma unroll
-    for (int j = 0; j < kMoveUnits; ++j)
-        if (first + 256 * j + (int)threadIdx.x < items) *reinterpret_cast<uint4 *>(to + at[j]) = v[j];
 }
 
 constexpr int kColumns = 64;
@@ -804,11 +810,12 @@ p8_status launch_beam_reorder(const p8_paged *c, const int32_t *parents, const i
     a.tables = c->tables; a.parents = parents; a.lens = lens; a.ts = c->table_stride; a.slots = c->columns * c->page; a.columns = c->columns;
     a.div = page_div((uint32_t)c->page);
     a.batch = (int)batch; a.beams = (int)beams; a.heads = (int)c->heads; a.pages = (int)c->pages; a.row_bytes = (int)c->width * es;
-    const int64_t units = (c->page - 1) * c->heads * (a.row_bytes / 16), chunks = (units + 256 * kMoveUnits - 1) / (256 * kMoveUnits);
-    if (units > INT32_MAX || chunks * c->rows > INT32_MAX) return P8_ERR_UNSUPPORTED;
-    a.chunks = (int)chunks;
-    a.alone = chunks == 0 || beams == 1;
-    if (!a.alone && launch_after(k_beam_move, dim3((unsigned int)(chunks * c->rows), (unsigned int)(2 * c->layers)), dim3(256), 0, st, a) != cudaSuccess) return P8_ERR_CUDA;
+    if (2 * c->layers * c->heads > INT32_MAX / 2) return P8_ERR_UNSUPPORTED;
+    a.segments = (int)(2 * c->layers * c->heads);
+    a.alone = c->page == 1 || beams == 1;
+    // so many blocks for each child that there are some twelve on every SM if all are there; a segment a warp at least
+    const int64_t children = batch * (beams - 1), parts = children ? std::max<int64_t>(1, std::min<int64_t>((a.segments + 7) / 8, 12 * sm_count() / children)) : 1;
+    if (!a.alone && launch_after(k_beam_move, dim3((unsigned int)children, (unsigned int)parts), dim3(256), 0, st, a) != cudaSuccess) return P8_ERR_CUDA;
     const int64_t across = std::max<int64_t>(1, std::min<int64_t>((c->columns + kColumns - 1) / kColumns, (2 * sm_count() + batch - 1) / batch));
     return done(launch_after(k_beam_tables, dim3((unsigned int)across, (unsigned int)batch), dim3(256), 0, st, a));
 }
