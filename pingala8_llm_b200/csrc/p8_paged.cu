@@ -74,82 +74,107 @@ struct PagedAppendArgs {
     float eps;
 };
 
-template <typename T, int D, bool kPairs>
-__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ PagedAppendArgs a) {
-    constexpr int L = D / 8, RPB = 256 / L;
+// four values, rounded to the type, that make room in the L2 for others first
+__device__ __forceinline__ void stream4(float *p, const float (&v)[4]) { __stcs(reinterpret_cast<float4 *>(p), make_float4(v[0], v[1], v[2], v[3])); }
+template <typename T>
+__device__ __forceinline__ void stream4(T *p, const float (&v)[4]) {
+    union { T t[4]; uint2 u; } r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.t[i] = from_f<T>(v[i]);
+    __stcs(reinterpret_cast<uint2 *>(p), r.u);
+}
+
+template <typename T, int D, bool kPairs, int kRows>
+__global__ void __launch_bounds__(128) k_paged_append(const __grid_constant__ PagedAppendArgs a) {
+    constexpr int L = D / 8, RPB = 128 / L;
     after_prior();
-    const unsigned int rows = a.heads + 2 * a.kvh, id = blockIdx.x * RPB + threadIdx.x / L;
+    const unsigned int rows = a.heads + 2 * a.kvh, per = (rows + kRows - 1) / kRows, id = blockIdx.x * RPB + threadIdx.x / L;
     const int l = threadIdx.x % L;
-    const unsigned int tok = id / rows;
+    const unsigned int tok = id / per;
     if (tok >= (unsigned int)a.batch * a.tokens) return;  // a whole group of lanes leaves
-    const int r = (int)(id - tok * rows), b = (int)(tok / (unsigned int)a.tokens), t = (int)(tok - (unsigned int)b * a.tokens);
-    const int which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2;
-    const int h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
+    const int r0 = (int)(id - tok * per) * kRows, b = (int)(tok / (unsigned int)a.tokens), t = (int)(tok - (unsigned int)b * a.tokens);
     const int turned = a.half / 4, past = l - turned;  // lanes that turn; this lane among the others
     const int e0 = kPairs ? 8 * l : past < 0 ? 4 * l : 2 * a.half + 4 * past, e1 = kPairs ? 8 * l + 4 : past < 0 ? a.half + 4 * l : a.half + D / 2 + 4 * past;
-    const float *x = a.x[which] + b * a.xs[which][0] + t * a.xs[which][1] + h * a.xs[which][2];
-    float u[4], w[4];
-    *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(x + e0);
-    *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(x + e1);
+    float u[kRows][4], w[kRows][4];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + i, which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2, h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
+        if (r >= (int)rows) break;
+        const float *x = a.x[which] + b * a.xs[which][0] + t * a.xs[which][1] + h * a.xs[which][2];
+        *reinterpret_cast<float4 *>(u[i]) = __ldcs(reinterpret_cast<const float4 *>(x + e0));
+        *reinterpret_cast<float4 *>(w[i]) = __ldcs(reinterpret_cast<const float4 *>(x + e1));
+    }
     const int p = a.pos[tok], len = a.lens[b], n = a.counts ? a.counts[b] : a.tokens;
     if (len < 0 || n < 0 || n > a.tokens || (long long)len + n > a.slots) {
-        if (t == 0 && r == 0 && l == 0) out_of_range();
+        if (t == 0 && r0 == 0 && l == 0) out_of_range();
         return;
     }
     if (t >= n) return;
     if (p < 0 || p >= a.positions) {
-        if (r == 0 && l == 0) out_of_range();
+        if (r0 == 0 && l == 0) out_of_range();
         return;
     }
-    unsigned int page = 0, in = 0;
+    unsigned int in = 0;
     int at = 0;
-    if (which > 0) {
-        page = page_of(a.div, len + t);
+    if (r0 + kRows > a.heads) {  // keys or values among the rows
+        const unsigned int page = page_of(a.div, len + t);
         in = len + t - page * a.div.size;
         at = a.tables[b * a.ts + page];
     }
-    if (which < 2) {
-        const float *g = which == 0 ? a.qn : a.kn;
-        if (g) {
-            float ss = 0.f;
+    float c[4], s[4];
+    if (past < 0 && r0 < a.heads + a.kvh) {
+        *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(a.cos + (long long)p * a.half + 4 * l);
+        *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(a.sin + (long long)p * a.half + 4 * l);
+    }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss += u[i] * u[i] + w[i] * w[i];
-            const unsigned int group = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << (threadIdx.x % 32 / L * L);
+    for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + i, which = r < a.heads ? 0 : r < a.heads + a.kvh ? 1 : 2, h = which == 0 ? r : which == 1 ? r - a.heads : r - a.heads - a.kvh;
+        if (r >= (int)rows) break;
+        if (which < 2) {
+            const float *g = which == 0 ? a.qn : a.kn;
+            if (g) {
+                float ss = 0.f;
 #pragma unroll
-            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(group, ss, m);
-            const float rs = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+                for (int j = 0; j < 4; ++j) ss += u[i][j] * u[i][j] + w[i][j] * w[i][j];
+                const unsigned int group = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << (threadIdx.x % 32 / L * L);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                u[i] = u[i] * rs * g[e0 + i];
-                w[i] = w[i] * rs * g[e1 + i];
+                for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(group, ss, m);
+                const float rs = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u[i][j] = u[i][j] * rs * g[e0 + j];
+                    w[i][j] = w[i][j] * rs * g[e1 + j];
+                }
+            }
+            if (past < 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float &x0 = kPairs ? (j < 2 ? u[i][2 * j] : w[i][2 * j - 4]) : u[i][j], &x1 = kPairs ? (j < 2 ? u[i][2 * j + 1] : w[i][2 * j - 3]) : w[i][j];
+                    const float y0 = x0 * c[j] - x1 * s[j], y1 = x1 * c[j] + x0 * s[j];
+                    x0 = y0;
+                    x1 = y1;
+                }
             }
         }
-        if (past < 0) {
-            float c[4], s[4];
-            *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(a.cos + (long long)p * a.half + 4 * l);
-            *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(a.sin + (long long)p * a.half + 4 * l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float &x0 = kPairs ? (i < 2 ? u[2 * i] : w[2 * i - 4]) : u[i], &x1 = kPairs ? (i < 2 ? u[2 * i + 1] : w[2 * i - 3]) : w[i];
-                const float y0 = x0 * c[i] - x1 * s[i], y1 = x1 * c[i] + x0 * s[i];
-                x0 = y0;
-                x1 = y1;
+        T *y;
+        if (which == 0) {
+            y = static_cast<T *>(a.q_out) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
+        } else {
+            if ((unsigned int)at >= (unsigned int)a.pages) {
+                if (h == 0 && l == 0) out_of_range();
+                continue;
             }
+            const int z = which - 1;
+            y = static_cast<T *>(a.kv[z]) + at * a.ps[z][0] + h * a.ps[z][1] + in * a.ps[z][2];
+        }
+        if (kRows > 1) {
+            stream4(y + e0, u[i]);
+            stream4(y + e1, w[i]);
+        } else {
+            store4(y + e0, u[i]);
+            store4(y + e1, w[i]);
         }
     }
-    T *y;
-    if (which == 0) {
-        y = static_cast<T *>(a.q_out) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
-    } else {
-        if ((unsigned int)at >= (unsigned int)a.pages) {
-            if (h == 0 && l == 0) out_of_range();
-            return;
-        }
-        const int z = which - 1;
-        y = static_cast<T *>(a.kv[z]) + at * a.ps[z][0] + h * a.ps[z][1] + in * a.ps[z][2];
-    }
-    store4(y + e0, u);
-    store4(y + e1, w);
 }
 
 #include "p8_paged_attn.cuh"
@@ -175,11 +200,18 @@ View pages_view(const p8_paged *c, bool values) {
 }
 View tables_view(const p8_paged *c) { return View(c->tables, &c->table_stride, &c->rows, 1, 4, c->columns); }
 
+template <typename T, int D, bool kPairs>
+cudaError_t run_paged_append(const PagedAppendArgs &a, cudaStream_t st) {
+    const long long rows = a.heads + 2 * a.kvh, tokens = (long long)a.batch * a.tokens, per = 128 / (D / 8);
+    const auto blocks = [&](int n) { return (tokens * ((rows + n - 1) / n) + per - 1) / per; };
+    // Two rows a lane, asked for together, and what is written not kept for long (prompt of 4,099 tokens 27.1 us; 33.3 with one row and blocks of 256), where there is work for the whole GPU all the same; else one, which is done sooner.
+    const int n = blocks(2) >= 8 * sm_count() ? 2 : 1;
+    return launch_after(n == 2 ? k_paged_append<T, D, kPairs, 2> : k_paged_append<T, D, kPairs, 1>, dim3((unsigned int)blocks(n)), dim3(128), 0, st, a);
+}
 template <typename T>
 cudaError_t run_paged_append(const p8_paged *c, const PagedAppendArgs &a, bool pairs, cudaStream_t st) {
-    const long long rows = (long long)a.batch * a.tokens * (a.heads + 2 * a.kvh), per = 256 / (c->width / 8);
-    const auto kernel = c->width == 128 ? (pairs ? k_paged_append<T, 128, true> : k_paged_append<T, 128, false>) : (pairs ? k_paged_append<T, 64, true> : k_paged_append<T, 64, false>);
-    return launch_after(kernel, dim3((unsigned int)((rows + per - 1) / per)), dim3(256), 0, st, a);
+    if (c->width == 128) return pairs ? run_paged_append<T, 128, true>(a, st) : run_paged_append<T, 128, false>(a, st);
+    return pairs ? run_paged_append<T, 64, true>(a, st) : run_paged_append<T, 64, false>(a, st);
 }
 
 }  // namespace
