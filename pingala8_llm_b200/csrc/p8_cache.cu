@@ -480,6 +480,8 @@ cudaError_t run_append(const p8_kv *c, const AppendArgs &a, cudaStream_t st) {
 }
 
 }  // namespace
+
+unsigned int cache_wait_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
 }  // namespace p8
 
 using namespace p8;

@@ -11,12 +11,15 @@
 #include <atomic>
 
 #include "p8_cache_common.cuh"
+#include "p8_device.cuh"
 #include "p8_internal.h"
 #include "p8_paged_index.h"
 
 namespace p8 {
 
-__device__ unsigned int g_paged_error = 0;  // bit 64 of p8_device_error
+unsigned int cache_wait_ns();  // p8_cache_wait_limit
+
+__device__ unsigned int g_paged_error = 0;  // bits 64 and 128 of p8_device_error
 
 unsigned int read_and_clear_paged_error() {
     unsigned int v = 0, z = 0;

@@ -2,12 +2,12 @@
 //
 // o = softmax(scale q K^T) V for the query heads of one cache head, which share its keys and values: every byte of the cache
 // is read once, 4 to 16 operations are done on it, so the memory bounds it (and latency, where there is little to read). The tiles of all
-// sequences and heads form one list, of which every CTA gets an equal contiguous share and every warp of it an equal part:
-// the warps finish together whatever the lengths are. A warp works on its own: keys and values go from the pages straight
-// into its registers, in the layout in which the matrix instruction takes them, with no shared memory and no
-// barrier in its way. Each warp keeps the running maximum m, the sum l of 2^(s - m) and the sum of 2^(s - m) v. Where a sequence's
-// head is spread over several warps, their sums meet in shared memory at the end of the CTA, and those of several
-// CTAs in a second launch.
+// sequences and heads form one list, of which every CTA (one an SM) gets an equal contiguous share and every warp of it an equal part:
+// the warps finish together whatever the lengths are. A warp works on its own, with tiles of its own on their way into shared memory:
+// each lane starts the bulk copy of one row, a key or a value, from wherever its page is, and a barrier in shared memory counts
+// the tile's bytes. So 190 KB are in flight on every SM, at one instruction a tile. Each warp keeps the running maximum m, the sum l of 2^(s - m) and
+// the sum of 2^(s - m) v. Where a sequence's head is spread over several warps, their sums meet in shared memory at the end of
+// the CTA, and those of several CTAs in a second launch.
 
 struct PagedAttnArgs {
     const char *q;
@@ -18,15 +18,46 @@ struct PagedAttnArgs {
     long long ts;
     char *out;
     long long os[2];     // bytes: sequence, head
-    float *lse, *part;
+    float *lse, *part;   // part: two parts a CTA, then one for each warp that goes on to another unit
+    int2 *cut;           // [rows][units]: the first and last CTA of a unit, the same where there is nothing to join; NULL: no unit can be cut
     long long slots;
     PageDiv div;
+    unsigned int wait_ns;
     int batch, heads, kvh, group, blocks, pages, ctas;  // group: query heads of a cache head; blocks: of these, rows of a warp's tile
     float scale2;                                       // scale / ln 2: the kernel's exponentials are powers of two
 };
 
-constexpr int kAttnWarps = 4;
-constexpr int kSpan = 128;  // slots that a share of the list has at least: two tiles of 16 for each warp of a CTA
+constexpr int kSpan = 192;     // slots that a share of the list has at least: a tile of 16 for each warp of a CTA
+constexpr unsigned int kSettleNs = 2000000000u;
+
+// A warp's wait for one of its tiles. One that is not over after `ns` gives up for good: bit 128 is set and the results are invalid; the warp
+// asks for no more tiles and waits for those on their way before it goes on to the CTA's end.
+struct TileWaits {
+    unsigned int ns;
+    bool gave_up;
+    __device__ bool operator()(uint64_t *bar, uint32_t parity) {
+        bool over = mbar_test_wait(bar, parity);
+        if (!over && ns && !gave_up) over = mbar_try_wait(bar, parity) || poll(bar, parity, ns);  // a look stays for up to about 4 us
+        if (__all_sync(0xffffffffu, over)) return true;
+        if (threadIdx.x % 32 == 0) atomicOr(&g_paged_error, kErrWait);
+        gave_up = true;
+        return false;
+    }
+    static __device__ void settle(uint64_t *bar, uint32_t parity) {
+        if (!mbar_try_wait(bar, parity)) poll(bar, parity, kSettleNs);
+        __syncwarp();
+    }
+    // Beside the time there is a least number of looks: the clock goes on while the GPU runs something else in this kernel's place.
+    static __device__ bool poll(uint64_t *bar, uint32_t parity, unsigned int ns) {
+        unsigned long long t0, t;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+        for (unsigned int i = 0;; ++i) {
+            if (mbar_try_wait(bar, parity)) return true;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+            if (i >= ns >> 14 && t - t0 > ns) return false;
+        }
+    }
+};
 
 // Tiles of a sequence; none where it has no token in this call or is out of range.
 template <int kTile>
@@ -130,12 +161,14 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
-// A tile's pages: lane l looks up slot l % kTile.
-template <int kTile>
-struct Lookup {
+// A tile's rows, one a lane: the keys of its slots in the first kTile lanes, the values in the next. The rows lie kKeyStride and
+// kValueStride bytes apart in shared memory.
+template <int kTile, int kRowBytes, int kKeyStride, int kValueStride>
+struct Tiles {
+    static constexpr int kBytes = kTile * (kKeyStride + kValueStride);
     int id;           // the page; -1 behind the sequence's end
     unsigned int in;  // the slot's place in it
-    __device__ __forceinline__ void ask(const PagedAttnArgs &a, const int *table, int tile, int n, int lane) {
+    __device__ __forceinline__ void look(const PagedAttnArgs &a, const int *table, int tile, int n, int lane) {
         const int slot = tile * kTile + lane % kTile;
         const unsigned int page = page_of(a.div, (unsigned int)slot);
         in = (unsigned int)slot - page * a.div.size;
@@ -145,16 +178,28 @@ struct Lookup {
             if (id < 0) id = INT_MIN;  // out of range, as any number of pages or above
         }
     }
-    // byte offsets of the slot's key and value; a bit for each slot that is there
-    __device__ __forceinline__ unsigned int resolve(const PagedAttnArgs &a, long long &ko, long long &vo) const {
+    // Asks for the rows that have been looked up. Returns a bit for each slot that is there; of one that is not, the value becomes zeros
+    // (its key is whatever was there, and its score is not looked at).
+    __device__ __forceinline__ unsigned int ask(const PagedAttnArgs &a, char *to, uint64_t *bar, int h, int lane) const {
         const bool there = (unsigned int)id < (unsigned int)a.pages;
         if (!there && id != -1) out_of_range();
-        ko = vo = 0;
-        if (there) {
-            ko = id * a.st[0][0] + in * a.st[0][2];
-            vo = id * a.st[1][0] + in * a.st[1][2];
+        const unsigned int mask = __ballot_sync(0xffffffffu, there) & ((1u << kTile) - 1);
+        const int z = lane / kTile;
+        if (lane == 0) mbar_expect_tx(bar, __popc(mask) * 2 * kRowBytes);
+        char *row = to + (z ? kTile * kKeyStride + lane % kTile * kValueStride : lane * kKeyStride);
+        if (z == 1 && !there) {
+#pragma unroll 1
+            for (int i = 0; i < kRowBytes; i += 16) *reinterpret_cast<uint4 *>(row + i) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();  // before the next tile's copies
         }
-        return __ballot_sync(0xffffffffu, there);
+        __syncwarp();
+        if (z < 2 && there) {
+            const char *from = a.kv[z] + h * a.st[z][1] + id * a.st[z][0] + in * a.st[z][2];
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"((unsigned int)__cvta_generic_to_shared(row)), "l"(from), "r"(kRowBytes),
+                         "r"((unsigned int)__cvta_generic_to_shared(bar))
+                         : "memory");
+        }
+        return mask;
     }
 };
 
@@ -169,13 +214,14 @@ struct Lookup {
 // a reduction and a rescaling.
 template <typename T, int D, int kN>
 struct Core16 {
-    static constexpr int kTile = 16, kRows = 8 * kN;
+    static constexpr int kTile = 16, kRows = 8 * kN, kKeys = 2 * D + 64, kValues = 2 * D + 16;  // rows so far apart that eight lanes' 16 bytes are in different banks
+    using Tile = Tiles<kTile, 2 * D, kKeys, kValues>;
+    static constexpr int kDepth = D == 64 || kN == 2 ? 3 : 2, kWarps = kN == 1 ? 12 : 8, kShared = kDepth * Tile::kBytes;  // of a warp
     static constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = 8.f;
     uint32_t q[kN][D / 32][4];
     float o[kN][D / 16][4], m[kN][2], l[kN][2];
-    uint4 k[2][D / 32], v[4][D / 64];
 
-    __device__ __forceinline__ Core16(float *) {}
+    __device__ __forceinline__ Core16(char *) {}
     __device__ __forceinline__ void begin(const char *qrow, long long qs, int nq, float, int lane) {
         const int g = lane / 4, t = lane % 4;
 #pragma unroll
@@ -192,46 +238,27 @@ struct Core16 {
             l[i][0] = l[i][1] = 0.f;
         }
     }
-    __device__ __forceinline__ void load_k(const char *base, long long off, unsigned int mask, int lane) {
-        const int g = lane / 4, t = lane % 4;
+    struct Scores { float x[kN][4]; };
+    __device__ __forceinline__ void scores(Scores &y, const char *tile, int lane) const {
+        float (&s)[kN][4] = y.x;
+        const char *key = tile + lane / 4 * kKeys + 16 * (lane % 4);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const long long at = __shfl_sync(0xffffffffu, off, g + 8 * r);
-            const bool there = mask >> (g + 8 * r) & 1;
+        for (int i = 0; i < kN; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                k[r][j] = make_uint4(0, 0, 0, 0);
-                if (there) k[r][j] = ld_once(base + at + 64 * j + 16 * t);
-            }
-        }
-    }
-    __device__ __forceinline__ void load_v(const char *base, long long off, unsigned int mask, int lane) {
-        const int g = lane / 4, t = lane % 4;
+        for (int j = 0; j < D / 32; ++j) {
+            const uint4 k0 = *reinterpret_cast<const uint4 *>(key + 64 * j), k1 = *reinterpret_cast<const uint4 *>(key + 8 * kKeys + 64 * j);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int slot = 2 * t + (r & 1) + 8 * (r >> 1);
-            const long long at = __shfl_sync(0xffffffffu, off, slot);
-            const bool there = mask >> slot & 1;
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                v[r][c] = make_uint4(0, 0, 0, 0);
-                if (there) v[r][c] = ld_once(base + at + 128 * c + 16 * g);
-            }
-        }
-    }
-    __device__ __forceinline__ void scores(float (&s)[kN][4]) const {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                mma16816<T>(s[i], k[0][j].x, k[1][j].x, k[0][j].y, k[1][j].y, q[i][j][0], q[i][j][1]);
-                mma16816<T>(s[i], k[0][j].z, k[1][j].z, k[0][j].w, k[1][j].w, q[i][j][2], q[i][j][3]);
+            for (int i = 0; i < kN; ++i) {
+                mma16816<T>(s[i], k0.x, k1.x, k0.y, k1.y, q[i][j][0], q[i][j][1]);
+                mma16816<T>(s[i], k0.z, k1.z, k0.w, k1.w, q[i][j][2], q[i][j][3]);
             }
         }
     }
     // scores to weights; their pieces as operands
-    __device__ __forceinline__ void weights(float (&s)[kN][4], unsigned int mask, float scale2, int lane, uint32_t (&hi)[kN][2], uint32_t (&lo)[kN][2]) {
+    // .. and to what is added: the weights' pieces times the values
+    __device__ __forceinline__ void weigh_and_add(Scores &y, const char *tile, unsigned int mask, float scale2, int lane) {
+        float (&s)[kN][4] = y.x;
+        uint32_t hi[kN][2], lo[kN][2];
         const int g = lane / 4;
         const bool there0 = mask >> g & 1, there1 = mask >> (g + 8) & 1;
         bool rise = false;
@@ -275,48 +302,25 @@ struct Core16 {
             lo[i][0] = transpose8(cut2<T>(p0 - r0.x, p1 - r0.y) | 0x00010001u);
             lo[i][1] = transpose8(cut2<T>(p2 - r1.x, p3 - r1.y) | 0x00010001u);
         }
-    }
-    __device__ __forceinline__ void add(const uint32_t (&hi)[kN][2], const uint32_t (&lo)[kN][2]) {
+        const char *value = tile + kTile * kKeys + 2 * (lane % 4) * kValues + 16 * g;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
-            const uint32_t *x0 = reinterpret_cast<const uint32_t *>(&v[0][c]), *x1 = reinterpret_cast<const uint32_t *>(&v[1][c]);
-            const uint32_t *x2 = reinterpret_cast<const uint32_t *>(&v[2][c]), *x3 = reinterpret_cast<const uint32_t *>(&v[3][c]);
+            uint32_t x[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(value + ((r & 1) + 8 * (r >> 1)) * kValues + 128 * c);
+                x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t a0 = __byte_perm(x0[e], x1[e], 0x5410), a1 = __byte_perm(x0[e], x1[e], 0x7632);
-                const uint32_t a2 = __byte_perm(x2[e], x3[e], 0x5410), a3 = __byte_perm(x2[e], x3[e], 0x7632);
+                const uint32_t a0 = __byte_perm(x[0][e], x[1][e], 0x5410), a1 = __byte_perm(x[0][e], x[1][e], 0x7632);
+                const uint32_t a2 = __byte_perm(x[2][e], x[3][e], 0x5410), a3 = __byte_perm(x[2][e], x[3][e], 0x7632);
 #pragma unroll
                 for (int i = 0; i < kN; ++i) {
                     mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, hi[i][0], hi[i][1]);
                     mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, lo[i][0], lo[i][1]);
                 }
             }
-        }
-    }
-    // tiles [t0, t1) of a sequence of n slots
-    __device__ __forceinline__ void run(const PagedAttnArgs &a, const int *table, const char *kb, const char *vb, int t0, int t1, int n, int lane) {
-        Lookup<kTile> look;
-        long long ko, vo;
-        look.ask(a, table, t0, n, lane);
-        unsigned int mask = look.resolve(a, ko, vo);
-        load_k(kb, ko, mask, lane);
-        load_v(vb, vo, mask, lane);
-        if (t0 + 1 < t1) look.ask(a, table, t0 + 1, n, lane);
-#pragma unroll 1
-        for (int t = t0; t < t1; ++t) {
-            float s[kN][4];
-            uint32_t hi[kN][2], lo[kN][2];
-            scores(s);
-            const unsigned int now = mask;
-            const bool more = t + 1 < t1;
-            if (more) {
-                mask = look.resolve(a, ko, vo);
-                load_k(kb, ko, mask, lane);
-                if (t + 2 < t1) look.ask(a, table, t + 2, n, lane);
-            }
-            weights(s, now, a.scale2, lane, hi, lo);
-            add(hi, lo);
-            if (more) load_v(vb, vo, mask, lane);
         }
     }
     // the sums of 2^(s - m) over all lanes
@@ -362,12 +366,13 @@ struct Core32 {
     static constexpr int kTile = 8, kRows = kN;
     static constexpr int kR = kN == 8 ? 2 : 1;  // scores of a lane
     static constexpr int kV = D == 128 ? 8 : 4;  // values' rows of a lane
+    using Tile = Tiles<kTile, 4 * D, 4 * D, 4 * D>;
+    static constexpr int kDepth = D == 64 ? 4 : 2, kWarps = kN == 8 ? 10 : 12, kShared = kDepth * Tile::kBytes + 4 * kN * (D + 8);
     static constexpr float kSlack = 8.f;
     float *sq, *sp;  // this warp's queries [kN][D] and weights [8][kN]
     float o[kN][4], m, l;
-    float4 k[2][D / 32], v[kV];
 
-    __device__ __forceinline__ Core32(float *shared) : sq(shared), sp(shared + kN * D) {}
+    __device__ __forceinline__ Core32(char *shared) : sq(reinterpret_cast<float *>(shared + kDepth * Tile::kBytes)), sp(sq + kN * D) {}
     __device__ __forceinline__ void begin(const char *qrow, long long qs, int nq, float scale2, int lane) {
         __syncwarp();
 #pragma unroll
@@ -383,50 +388,29 @@ struct Core32 {
         l = 0.f;
         __syncwarp();
     }
-    static __device__ __forceinline__ float4 ld4(const char *p) {
-        const uint4 x = ld_once(p);
-        return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
-    }
-    __device__ __forceinline__ void load_k(const char *base, long long off, unsigned int mask, int lane) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int slot = lane / 8 + 4 * r;
-            const long long at = __shfl_sync(0xffffffffu, off, slot);
-            const bool there = mask >> slot & 1;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                k[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (there) k[r][c] = ld4(base + at + 128 * c + 16 * (lane % 8));
-            }
-        }
-    }
-    __device__ __forceinline__ void load_v(const char *base, long long off, unsigned int mask, int lane) {
-#pragma unroll
-        for (int r = 0; r < kV; ++r) {
-            const int slot = D == 128 ? r : 2 * r + lane / 16;
-            const long long at = __shfl_sync(0xffffffffu, off, slot);
-            v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (mask >> slot & 1) v[r] = ld4(base + at + 16 * (lane % (D / 4)));
-        }
-    }
-    __device__ __forceinline__ void scores(float (&x)[kR], int lane) const {
+    struct Scores { float x[kR]; };
+    __device__ __forceinline__ void scores(Scores &out, const char *tile, int lane) const {
         const int j = lane % 8;
         float s[2][kN];
 #pragma unroll
         for (int i = 0; i < kN; ++i) s[0][i] = s[1][i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
+        for (int c = 0; c < D / 32; ++c) {
+            float4 k[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) k[r] = *reinterpret_cast<const float4 *>(tile + (lane / 8 + 4 * r) * (4 * D) + 128 * c + 16 * j);
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 const float4 y = *reinterpret_cast<const float4 *>(sq + i * D + 32 * c + 4 * j);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    s[r][i] = fmaf(k[r][c].x, y.x, s[r][i]);
-                    s[r][i] = fmaf(k[r][c].y, y.y, s[r][i]);
-                    s[r][i] = fmaf(k[r][c].z, y.z, s[r][i]);
-                    s[r][i] = fmaf(k[r][c].w, y.w, s[r][i]);
+                    s[r][i] = fmaf(k[r].x, y.x, s[r][i]);
+                    s[r][i] = fmaf(k[r].y, y.y, s[r][i]);
+                    s[r][i] = fmaf(k[r].z, y.z, s[r][i]);
+                    s[r][i] = fmaf(k[r].w, y.w, s[r][i]);
                 }
             }
+        }
         // halves of what is left go to the lane that keeps them
         float w[2 * kN];
 #pragma unroll
@@ -444,11 +428,12 @@ struct Core32 {
             }
         }
 #pragma unroll
-        for (int r = 0; r < kR; ++r) x[r] = w[r];
+        for (int r = 0; r < kR; ++r) out.x[r] = w[r];
     }
     __device__ __forceinline__ int slot_of(int r, int lane) const { return kN == 8 ? lane / 8 + 4 * r : lane / 8 + 4 * (lane % 8 / 4); }
     __device__ __forceinline__ int head_of(int lane) const { return lane % kN; }
-    __device__ __forceinline__ void weights(float (&x)[kR], unsigned int mask, float scale2, int lane) {
+    __device__ __forceinline__ void weigh_and_add(Scores &y, const char *tile, unsigned int mask, float scale2, int lane) {
+        float (&x)[kR] = y.x;
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
@@ -476,47 +461,22 @@ struct Core32 {
             sp[slot_of(r, lane) * kN + head_of(lane)] = p;
         }
         __syncwarp();
-    }
-    __device__ __forceinline__ void add(int lane) {
 #pragma unroll
         for (int r = 0; r < kV; ++r) {
             const int slot = D == 128 ? r : 2 * r + lane / 16;
+            const float4 v = *reinterpret_cast<const float4 *>(tile + (kTile + slot) * (4 * D) + 16 * (lane % (D / 4)));
 #pragma unroll
             for (int i = 0; i < kN; i += 4) {
                 const float4 p = *reinterpret_cast<const float4 *>(sp + slot * kN + i);
                 const float w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[i + e][0] = fmaf(w[e], v[r].x, o[i + e][0]);
-                    o[i + e][1] = fmaf(w[e], v[r].y, o[i + e][1]);
-                    o[i + e][2] = fmaf(w[e], v[r].z, o[i + e][2]);
-                    o[i + e][3] = fmaf(w[e], v[r].w, o[i + e][3]);
+                    o[i + e][0] = fmaf(w[e], v.x, o[i + e][0]);
+                    o[i + e][1] = fmaf(w[e], v.y, o[i + e][1]);
+                    o[i + e][2] = fmaf(w[e], v.z, o[i + e][2]);
+                    o[i + e][3] = fmaf(w[e], v.w, o[i + e][3]);
                 }
             }
-        }
-    }
-    __device__ __forceinline__ void run(const PagedAttnArgs &a, const int *table, const char *kb, const char *vb, int t0, int t1, int n, int lane) {
-        Lookup<kTile> look;
-        long long ko, vo;
-        look.ask(a, table, t0, n, lane);
-        unsigned int mask = look.resolve(a, ko, vo);
-        load_k(kb, ko, mask, lane);
-        load_v(vb, vo, mask, lane);
-        if (t0 + 1 < t1) look.ask(a, table, t0 + 1, n, lane);
-#pragma unroll 1
-        for (int t = t0; t < t1; ++t) {
-            float x[kR];
-            scores(x, lane);
-            const unsigned int now = mask;
-            const bool more = t + 1 < t1;
-            if (more) {
-                mask = look.resolve(a, ko, vo);
-                load_k(kb, ko, mask, lane);
-                if (t + 2 < t1) look.ask(a, table, t + 2, n, lane);
-            }
-            weights(x, now, a.scale2, lane);
-            add(lane);
-            if (more) load_v(vb, vo, mask, lane);
         }
     }
     __device__ __forceinline__ void finish() {
@@ -555,23 +515,71 @@ __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -
 // A part of a sequence's head: [kRows][D] sums, then the maxima, then the sums of the weights.
 template <typename Core, int D> constexpr int kPartFloats = Core::kRows * (D + 2);
 
-template <typename T, int D, typename Core, int kPerSm>
-__global__ void __launch_bounds__(32 * kAttnWarps, kPerSm) k_paged_attn(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kSlots = 2 * kAttnWarps;
-    constexpr bool k32 = std::is_same<T, float>::value;
-    extern __shared__ __align__(16) float s_part[];  // kSlots parts; 32 bits: the warps' queries and weights behind them
-    struct Piece { int b, unit; long long first; int left, right; };  // left, right: whether the unit begins and ends in this piece
-    __shared__ Piece s_piece[kSlots];
+// Tiles [t0, t1) of a sequence of n slots. Their pages are looked up one tile before they are asked for. phase: a bit for
+// each stage of the warp's ring.
+template <typename Core>
+__device__ __forceinline__ void run_tiles(Core &core, const PagedAttnArgs &a, TileWaits &wait, char *ring, uint64_t *bars, uint32_t &phase, const int *table, int h, int t0, int t1, int n, int lane) {
+    constexpr int kDepth = Core::kDepth;
+    typename Core::Tile next, first[kDepth];
+    unsigned int mask[kDepth];
+    if (wait.gave_up) return;
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+        if (t0 + i < t1) first[i].look(a, table, t0 + i, n, lane);
+    if (t0 + kDepth < t1) next.look(a, table, t0 + kDepth, n, lane);
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) mask[i] = t0 + i < t1 ? first[i].ask(a, ring + i * Core::Tile::kBytes, bars + i, h, lane) : 0;
+    int stage = 0;
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+        char *tile = ring + stage * Core::Tile::kBytes;
+        if (!wait(bars + stage, phase >> stage & 1)) {
+            for (int i = 0; i < kDepth && t + i < t1; ++i) {
+                TileWaits::settle(bars + stage, phase >> stage & 1);
+                phase ^= 1u << stage;
+                stage = stage + 1 == kDepth ? 0 : stage + 1;
+            }
+            return;
+        }
+        phase ^= 1u << stage;
+        typename Core::Scores s;
+        core.scores(s, tile, lane);
+        core.weigh_and_add(s, tile, mask[0], a.scale2, lane);
+#pragma unroll
+        for (int i = 0; i + 1 < kDepth; ++i) mask[i] = mask[i + 1];
+        __syncwarp();  // all have read the tile
+        if (t + kDepth < t1) {
+            mask[kDepth - 1] = next.ask(a, tile, bars + stage, h, lane);
+            if (t + kDepth + 1 < t1) next.look(a, table, t + kDepth + 1, n, lane);
+        }
+        stage = stage + 1 == kDepth ? 0 : stage + 1;
+    }
+}
+
+template <typename T, int D, typename Core>
+__global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kWarps = Core::kWarps, kSlots = 2 * kWarps;
+    static_assert(4 * kPart <= Core::kDepth * Core::Tile::kBytes, "a part takes the place of a warp's tiles");
+    extern __shared__ __align__(16) char s_warps[];  // kShared bytes for each warp
+    struct Piece { int b, unit, left, right, last; };  // left, right: whether the unit begins and ends in this piece; last (of one that begins): the CTA of its end
+    __shared__ uint64_t s_bars[kWarps][Core::kDepth];
+    __shared__ Piece s_piece[kSlots];            // of each warp: what it left before it went on to another unit, and at its end
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     after_prior();
     if (lane < 2) s_piece[2 * warp + lane].b = -1;
+    if (lane < Core::kDepth) mbar_init(&s_bars[warp][lane], 1);
+    fence_mbar_init();
+    fence_proxy_async();
     __syncwarp();
+    TileWaits wait{a.wait_ns, false};
+    uint32_t phase = 0;
     const TileList<kTile> list(a, lane, blockIdx.x == 0 && warp == 0);
     const long long base = list.share * blockIdx.x;
-    long long p = base + warp_first(list.share, warp, kAttnWarps);
-    const long long end = min(base + warp_first(list.share, warp + 1, kAttnWarps), list.total);
-    Core core(k32 ? s_part + kSlots * kPart + warp * (Core::kRows * D + 8 * Core::kRows) : nullptr);
+    long long p = base + warp_first(list.share, warp, kWarps);
+    const long long end = min(base + warp_first(list.share, warp + 1, kWarps), list.total);
+    Core core(s_warps + warp * Core::kShared);
+    float *const early = a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + warp) * kPart, *const late = reinterpret_cast<float *>(s_warps + warp * Core::kShared);
     const int per_block = (a.group + a.blocks - 1) / a.blocks;
     if (p < end) {
         long long begin;
@@ -586,21 +594,25 @@ __global__ void __launch_bounds__(32 * kAttnWarps, kPerSm) k_paged_attn(const __
                 const int h = unit / a.blocks, r0 = (unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
                 const int *table = a.tables + b * a.ts;
                 core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane);
-                core.run(a, table, a.kv[0] + h * a.st[0][1], a.kv[1] + h * a.st[1][1], off, real, a.lens[b] + 1, lane);
+                run_tiles(core, a, wait, s_warps + warp * Core::kShared, s_bars[warp], phase, table, h, off, real, a.lens[b] + 1, lane);
                 core.finish();
                 if (off == 0 && real == tiles) {
                     char *out = a.out + b * a.os[0] + head * a.os[1];
                     float *lse = a.lse ? a.lse + (long long)b * a.heads + head : nullptr;
                     core.each(lane, [&](int r, int d, const auto &x, float, float l) { if (r < nq) store_row<T>(out + r * a.os[1] + d * (int)sizeof(T), x, over(l)); },
                               [&](int r, float m, float l) { if (r < nq && lse) lse[r] = log_sum(m, l); });
+                    if (lane == 0 && a.cut) a.cut[(long long)b * list.units + unit] = make_int2(0, 0);
                 } else {
-                    const int slot = 2 * warp + (off == 0);
-                    float *to = s_part + slot * kPart;
+                    const bool last = p + (upto - off) >= end;  // the ring is free then
+                    float *to = last ? late : early;
+                    __syncwarp();
                     core.each(lane, [&](int r, int d, const auto &x, float, float) {
 #pragma unroll
                         for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); i += 4) *reinterpret_cast<float4 *>(to + r * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                     }, [&](int r, float m, float l) { to[Core::kRows * D + r] = m; to[Core::kRows * (D + 1) + r] = l; });
-                    if (lane == 0) s_piece[slot] = {b, unit, 0, off == 0, real == tiles};
+                    const long long past = p - off - base + tiles - 1;  // its last tile's place, from this CTA's first
+                    const int further = past < list.share ? 0 : past >> 32 ? (int)(past / list.share) : (int)((uint32_t)past / (uint32_t)list.share);
+                    if (lane == 0) s_piece[2 * warp + last] = {b, unit, off == 0, real == tiles, (int)blockIdx.x + further};
                 }
             }
             p += upto - off;
@@ -615,28 +627,29 @@ __global__ void __launch_bounds__(32 * kAttnWarps, kPerSm) k_paged_attn(const __
     }
     __syncthreads();
     // join the pieces that the warps left, in their order; what is not a whole unit goes to the workspace
+    const auto piece_at = [&](int j) { return j & 1 ? reinterpret_cast<const float *>(s_warps + j / 2 * Core::kShared) : a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + j / 2) * kPart; };
     for (int s = 0; s < kSlots;) {
         const Piece first = s_piece[s];
         int e = s + 1;
         if (first.b < 0) { s = e; continue; }
+        unsigned int among = 1u << s;  // the slots of this unit's pieces
         bool right = first.right;
         for (; e < kSlots; ++e) {
             const Piece x = s_piece[e];
             if (x.b < 0) continue;
             if (x.b != first.b || x.unit != first.unit) break;
+            among |= 1u << e;
             right = x.right;
         }
         const int h = first.unit / a.blocks, r0 = (first.unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
         const bool whole = first.left && right;
         float *to = a.part + (2ll * blockIdx.x + first.left) * kPart;
-        for (int i = threadIdx.x; i < nq * (D / 4); i += 32 * kAttnWarps) {
+        for (int i = threadIdx.x; i < nq * (D / 4); i += 32 * kWarps) {
             const int r = i / (D / 4), d = 4 * (i % (D / 4));
             float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int j = s; j < e; ++j)
-                if (s_piece[j].b >= 0) top = fmaxf(top, s_part[j * kPart + Core::kRows * D + r]);
-            for (int j = s; j < e; ++j) {
-                if (s_piece[j].b < 0) continue;
-                const float *from = s_part + j * kPart, m = from[Core::kRows * D + r], f = m == top ? 1.f : ex2(m - top);
+            for (unsigned int j = among; j; j &= j - 1) top = fmaxf(top, piece_at(__ffs(j) - 1)[Core::kRows * D + r]);
+            for (unsigned int j = among; j; j &= j - 1) {
+                const float *from = piece_at(__ffs(j) - 1), m = from[Core::kRows * D + r], f = m == top ? 1.f : ex2(m - top);
                 const float4 y = *reinterpret_cast<const float4 *>(from + r * D + d);
                 l += f * from[Core::kRows * (D + 1) + r];
                 x[0] += f * y.x; x[1] += f * y.y; x[2] += f * y.z; x[3] += f * y.w;
@@ -652,15 +665,16 @@ __global__ void __launch_bounds__(32 * kAttnWarps, kPerSm) k_paged_attn(const __
                 }
             }
         }
+        if (first.left && threadIdx.x == 0 && a.cut) a.cut[(long long)first.b * list.units + first.unit] = make_int2((int)blockIdx.x, first.last);
         s = e;
     }
 }
 
-// The second launch: kWarps warps for each query head of a sequence look where its tiles were; where that is more than one CTA,
+// The second launch: kWarps warps for each query head of a sequence look whether its tiles were more than one CTA's; if so,
 // they add the parts up (a warp every kWarps-th of them), in one order.
 template <typename T, int D, typename Core, int kWarps>
 __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kE = D / 32;
+    constexpr int kPart = kPartFloats<Core, D>, kE = D / 32;
     __shared__ float s_x[8][D], s_m[8], s_l[8];
     after_prior();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % kWarps;
@@ -668,29 +682,16 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
     const bool there = row < (long long)a.batch * a.heads;
     const int b = there ? (int)(row / a.heads) : 0, head = there ? (int)(row - (long long)b * a.heads) : 0, h = head / a.group, per_block = (a.group + a.blocks - 1) / a.blocks;
     const int blk = (head - h * a.group) / per_block, r = head - h * a.group - blk * per_block;
-    const TileList<kTile> list(a, lane, false);
+    const int2 cut = a.cut[(long long)b * a.kvh * a.blocks + h * a.blocks + blk];
     bool bad;
-    const int tiles = row_tiles<kTile>(a, b, bad);
-    // the places before this sequence
-    long long before = 0;
-    const int l0 = b / list.per;
-    for (int i = l0 * list.per + lane; i < b; i += 32) {
-        bool x;
-        before += unit_places(row_tiles<kTile>(a, i, x), list.kLeast);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    const long long upto = __shfl_sync(0xffffffffu, list.upto, l0 > 0 ? l0 - 1 : 0);
-    const long long begin = before * list.units + (l0 > 0 ? upto : 0) + (long long)(h * a.blocks + blk) * unit_places(tiles, list.kLeast);
-    const int c0 = (int)(begin / list.share), c1 = tiles ? (int)((begin + tiles - 1) / list.share) : c0;
+    const bool split = there && row_tiles<Core::kTile>(a, b, bad) && cut.x < cut.y;  // (of a row without a token no one has written the cut)
     float x[kE], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < kE; ++i) x[i] = 0.f;
-    const bool split = there && c1 > c0;
     if (split) {
 #pragma unroll 4
-        for (int c = c0 + mine; c <= c1; c += kWarps) {
-            const float *from = a.part + (2ll * c + (c == c0)) * kPart;
+        for (int c = cut.x + mine; c <= cut.y; c += kWarps) {
+            const float *from = a.part + (2ll * c + (c == cut.x)) * kPart;
             const float pm = from[Core::kRows * D + r], pl = from[Core::kRows * (D + 1) + r], now = fmaxf(m, pm);
             const float f = m == now ? 1.f : ex2(m - now), g = pm == now ? 1.f : ex2(pm - now);
             m = now;
@@ -708,7 +709,9 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
         __syncthreads();
         if (mine) return;
         if (split) {
-            for (int w = warp + 1; w < warp + kWarps; ++w) {
+#pragma unroll
+            for (int k = 1; k < kWarps; ++k) {
+                const int w = warp + k;
                 const float pm = s_m[w], now = fmaxf(m, pm), f = m == now ? 1.f : ex2(m - now), g = pm == now ? 1.f : ex2(pm - now);
                 m = now;
                 l = l * f + s_l[w] * g;
@@ -736,29 +739,27 @@ bool attn_wide(const p8_paged *c, int64_t heads) {  // the larger of the two til
     const int64_t group = heads / c->heads, blocks = attn_blocks(c, heads), rows = (group + blocks - 1) / blocks;
     return c->type == P8_KV_F32 ? rows > 4 : rows > 8;
 }
-int attn_per_sm(const p8_paged *c, int64_t heads) { return c->type != P8_KV_F32 && attn_wide(c, heads) ? 2 : 3; }
 int attn_rows(const p8_paged *c, int64_t heads) { return (c->type == P8_KV_F32 ? 4 : 8) * (attn_wide(c, heads) ? 2 : 1); }
+int attn_warps(const p8_paged *c, int64_t heads) {
+    if (c->type == P8_KV_F32) return attn_wide(c, heads) ? Core32<128, 8>::kWarps : Core32<128, 4>::kWarps;
+    return attn_wide(c, heads) ? Core16<__half, 128, 2>::kWarps : Core16<__half, 128, 1>::kWarps;
+}
+int64_t attn_units(const p8_paged *c, int64_t heads) { return c->rows * c->heads * attn_blocks(c, heads); }
 // Whether a unit can be cut at all: not where each has a CTA's least share to itself and no sequence can be longer.
-bool attn_cuts(const p8_paged *c, int64_t heads) {
-    const int64_t units = c->rows * c->heads * attn_blocks(c, heads), ctas = (int64_t)sm_count() * attn_per_sm(c, heads);
-    return c->columns * c->page > kSpan || units > ctas;
+bool attn_cuts(const p8_paged *c, int64_t heads) { return c->columns * c->page > kSpan || attn_units(c, heads) > sm_count(); }
+size_t attn_part_bytes(const p8_paged *c, int64_t heads) {
+    return (size_t)sm_count() * (2 + attn_warps(c, heads)) * attn_rows(c, heads) * (c->width + 2) * 4;
 }
-size_t paged_attn_workspace(const p8_paged *c, int64_t heads) {
-    if (!attn_cuts(c, heads)) return 0;
-    return (size_t)sm_count() * attn_per_sm(c, heads) * 2 * attn_rows(c, heads) * (c->width + 2) * 4;
-}
+size_t paged_attn_workspace(const p8_paged *c, int64_t heads) { return attn_cuts(c, heads) ? attn_part_bytes(c, heads) + (size_t)attn_units(c, heads) * sizeof(int2) : 0; }
 
-template <typename T, int D, typename Core, int kPerSm>
-p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
-    constexpr bool k32 = std::is_same<T, float>::value;
-    constexpr int smem = 4 * (2 * kAttnWarps * kPartFloats<Core, D> + (k32 ? kAttnWarps * Core::kRows * (D + 8) : 0));
-    const auto kernel = k_paged_attn<T, D, Core, kPerSm>;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return P8_ERR_CUDA;
-    const bool cuts = attn_cuts(c, a.heads);
-    const int64_t units = c->rows * c->heads * a.blocks;
-    const int64_t most = units * ((c->columns * c->page + kSpan - 1) / kSpan);  // shares that there can be
-    if (launch_after(kernel, dim3((unsigned int)std::min<int64_t>(a.ctas, most)), dim3(32 * kAttnWarps), (size_t)smem, st, a) != cudaSuccess) return P8_ERR_CUDA;
-    if (!cuts) return P8_OK;
+template <typename T, int D, typename Core>
+p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStream_t st) {
+    const auto kernel = k_paged_attn<T, D, Core>;
+    constexpr int smem = Core::kWarps * Core::kShared;
+    if (!allow_shared(kernel, which, smem)) return P8_ERR_CUDA;
+    const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);  // shares that there can be
+    if (launch_after(kernel, dim3((unsigned int)std::min<int64_t>(a.ctas, most)), dim3(32 * Core::kWarps), (size_t)smem, st, a) != cudaSuccess) return P8_ERR_CUDA;
+    if (!a.cut) return P8_OK;
     const int64_t rows = c->rows * a.heads;
     if (a.ctas >= 4 * units) return done(launch_after(k_paged_join<T, D, Core, 8>, dim3((unsigned int)rows), dim3(256), 0, st, a));
     return done(launch_after(k_paged_join<T, D, Core, 1>, dim3((unsigned int)((rows + 7) / 8)), dim3(256), 0, st, a));
@@ -766,9 +767,10 @@ p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
 template <int D>
 p8_status run_paged_attn_d(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
     const bool wide = attn_wide(c, a.heads);
-    if (c->type == P8_KV_F32) return wide ? run_paged_attn<float, D, Core32<D, 8>, 3>(c, a, st) : run_paged_attn<float, D, Core32<D, 4>, 3>(c, a, st);
-    if (c->type == P8_KV_F16) return wide ? run_paged_attn<__half, D, Core16<__half, D, 2>, 2>(c, a, st) : run_paged_attn<__half, D, Core16<__half, D, 1>, 3>(c, a, st);
-    return wide ? run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 2>, 2>(c, a, st) : run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 1>, 3>(c, a, st);
+    const int which = 4 * (int)c->type + 2 * wide + (D == 128);
+    if (c->type == P8_KV_F32) return wide ? run_paged_attn<float, D, Core32<D, 8>>(c, a, which, st) : run_paged_attn<float, D, Core32<D, 4>>(c, a, which, st);
+    if (c->type == P8_KV_F16) return wide ? run_paged_attn<__half, D, Core16<__half, D, 2>>(c, a, which, st) : run_paged_attn<__half, D, Core16<__half, D, 1>>(c, a, which, st);
+    return wide ? run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 2>>(c, a, which, st) : run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 1>>(c, a, which, st);
 }
 
 p8_status launch_paged_attn(const p8_paged *c, const p8_paged_attn_args *x, void *workspace, cudaStream_t st) {
@@ -779,10 +781,12 @@ p8_status launch_paged_attn(const p8_paged *c, const p8_paged_attn_args *x, void
     a.kv[0] = (const char *)c->k; a.kv[1] = (const char *)c->v;
     for (int i = 0; i < 3; ++i) { a.st[0][i] = c->k_stride[1 + i] * es; a.st[1][i] = c->v_stride[1 + i] * es; }
     a.tables = c->tables; a.ts = c->table_stride; a.lens = x->lens; a.counts = x->counts;
-    a.lse = x->lse; a.part = (float *)workspace;
-    a.slots = c->columns * c->page; a.div = page_div((uint32_t)c->page);
+    const bool cuts = attn_cuts(c, x->heads);
+    a.lse = x->lse; a.part = cuts ? (float *)workspace : nullptr;
+    a.cut = cuts ? reinterpret_cast<int2 *>((char *)workspace + attn_part_bytes(c, x->heads)) : nullptr;
+    a.slots = c->columns * c->page; a.div = page_div((uint32_t)c->page); a.wait_ns = cache_wait_ns();
     a.batch = (int)c->rows; a.heads = (int)x->heads; a.kvh = (int)c->heads; a.group = (int)(x->heads / c->heads); a.blocks = attn_blocks(c, x->heads);
-    a.pages = (int)c->pages; a.ctas = sm_count() * attn_per_sm(c, x->heads);
+    a.pages = (int)c->pages; a.ctas = sm_count();
     a.scale2 = (float)x->scale * 1.4426950408889634f;
     return c->width == 128 ? run_paged_attn_d<128>(c, a, st) : run_paged_attn_d<64>(c, a, st);
 }

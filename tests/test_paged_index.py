@@ -66,7 +66,7 @@ def test_bits_and_orders(ix):
 
 
 def walk(ix, units, tiles, ctas, least, warps):
-    """What the kernel's CTAs leave: {unit: pieces}, in which parts of the workspace, for `tiles` [sequences]"""
+    """What the kernel's CTAs leave for `tiles` [sequences]: {unit: its tiles in pieces}, {part of the workspace: unit}, {unit: who notes its cut}"""
     places = [ix.unit_places(t, least) for t in tiles]
     total = units * sum(places)
     share = ix.cta_share(total, ctas, least)
@@ -76,7 +76,7 @@ def walk(ix, units, tiles, ctas, least, warps):
             start[b, u] = at
             at += c
     order = sorted(((s, k) for k, s in start.items() if places[k[0]]), key=lambda x: x[0])
-    covered, parts = {}, {}
+    covered, parts, cuts = {}, {}, {}
     for cta in range(ctas):
         pieces = []
         for w in range(warps):
@@ -92,8 +92,9 @@ def walk(ix, units, tiles, ctas, least, warps):
                     continue
                 covered.setdefault((b, u), []).append((t0, t1))
                 if t0 == 0 and t1 == tiles[b]:
+                    cuts.setdefault((b, u), []).append((0, 0))
                     continue
-                slot = 1 if t0 == 0 else 0
+                slot = 1 if hi == end else 0  # at the warp's end in place of its tiles, before that in the workspace
                 assert slot not in slots, "two pieces of a warp in one place"
                 slots.add(slot)
                 pieces.append((w, slot, (b, u), t0 == 0, t1 == tiles[b]))
@@ -104,21 +105,26 @@ def walk(ix, units, tiles, ctas, least, warps):
             while j < len(pieces) and pieces[j][2] == pieces[i][2]:
                 j += 1
             left, right = pieces[i][3], pieces[j - 1][4]
+            if left:
+                b, u = pieces[i][2]
+                further = (start[b, u] - cta * share + tiles[b] - 1) // share
+                cuts.setdefault((b, u), []).append((cta, cta + further))
+                assert right == (further == 0)
             if not (left and right):
                 key = (cta, 1 if left else 0)
                 assert key not in parts, "two parts of a CTA in one place"
                 parts[key] = pieces[i][2]
             i = j
-    return start, share, total, covered, parts
+    return start, share, total, covered, parts, cuts
 
 
 @pytest.mark.parametrize("seed", range(60))
 def test_shares_cover_every_tile_once_and_the_join_finds_all_parts(ix, seed):
     rng = random.Random(seed)
-    ctas, least, warps = rng.choice([3, 7, 20, 44]), rng.choice([1, 2, 8, 16]), 4
+    ctas, least, warps = rng.choice([3, 7, 20, 44]), rng.choice([1, 2, 8, 12, 24]), rng.choice([4, 8, 10, 12])
     units, B = rng.choice([1, 2, 8]), rng.choice([1, 2, 5, 40])
     tiles = [rng.choice([0, 1, 2, rng.randint(0, 30), rng.randint(0, 400)]) for _ in range(B)]
-    start, share, total, covered, parts = walk(ix, units, tiles, ctas, least, warps)
+    start, share, total, covered, parts, cuts = walk(ix, units, tiles, ctas, least, warps)
     assert share * ctas >= total
     used = -(-total // share) if total else 0
     assert used <= units * sum(1 for _ in tiles) * max(1, -(-max(tiles) // least))  # the grid's bound
@@ -129,6 +135,9 @@ def test_shares_cover_every_tile_once_and_the_join_finds_all_parts(ix, seed):
             assert [x for x, _ in got] == [0] * (t > 0) + [y for _, y in got[:-1]] and (not t or got[-1][1] == t)
             s = start[b, u]
             c0, c1 = s // share, (s + t - 1) // share if t else s // share
+            if t:
+                (cut,) = cuts[b, u]
+                assert cut == ((c0, c1) if c1 > c0 else cut) and (c1 > c0) == (cut[1] > cut[0])
             for c in range(c0, c1 + 1) if c1 > c0 else ():
                 assert left.pop((c, 1 if c == c0 else 0)) == (b, u)
     assert not left  # and nothing lies in the workspace that no one joins
