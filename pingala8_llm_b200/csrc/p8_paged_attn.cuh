@@ -23,7 +23,7 @@ struct PagedAttnArgs {
     long long slots;
     PageDiv div;
     unsigned int wait_ns;
-    int batch, heads, kvh, group, blocks, pages, ctas;  // group: query heads of a cache head; blocks: of these, rows of a warp's tile
+    int batch, heads, kvh, group, blocks, per_block, pages, ctas;  // group: query heads of a cache head, in so many blocks of at most per_block
     float scale2;                                       // scale / ln 2: the kernel's exponentials are powers of two
 };
 
@@ -73,7 +73,8 @@ struct TileList {
     static constexpr int kLeast = kSpan / kTile;
     const PagedAttnArgs &a;
     int per, units;
-    long long upto, total, share;  // places of the lanes up to this one; of all; of a CTA
+    long long upto, total;  // places of the lanes up to this one; of all
+    int share;              // of a CTA
 
     __device__ __forceinline__ TileList(const PagedAttnArgs &a_, int lane, bool report) : a(a_), per((a_.batch + 31) / 32), units(a_.kvh * a_.blocks) {
         long long mine = 0;
@@ -94,7 +95,7 @@ struct TileList {
         }
         upto *= units;
         total = __shfl_sync(0xffffffffu, upto, 31);
-        share = cta_share(total, a.ctas, kLeast);
+        share = (int)cta_share(total, a.ctas, kLeast);
     }
     // the sequence that has place p < total, and its first place
     __device__ __forceinline__ int find(long long p, int lane, long long &begin) const {
@@ -517,18 +518,22 @@ template <typename Core, int D> constexpr int kPartFloats = Core::kRows * (D + 2
 
 // Tiles [t0, t1) of a sequence of n slots. Their pages are looked up one tile before they are asked for. phase: a bit for
 // each stage of the warp's ring.
-template <typename Core>
-__device__ __forceinline__ void run_tiles(Core &core, const PagedAttnArgs &a, TileWaits &wait, char *ring, uint64_t *bars, uint32_t &phase, const int *table, int h, int t0, int t1, int n, int lane) {
+template <typename Core, typename Begin>
+__device__ __forceinline__ void run_tiles(Core &core, const Begin &begin, const PagedAttnArgs &a, TileWaits &wait, char *ring, uint64_t *bars, uint32_t &phase, const int *table, int h, int t0, int t1, int n, int lane) {
     constexpr int kDepth = Core::kDepth;
     typename Core::Tile next, first[kDepth];
     unsigned int mask[kDepth];
-    if (wait.gave_up) return;
+    if (wait.gave_up) {
+        begin();
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i)
         if (t0 + i < t1) first[i].look(a, table, t0 + i, n, lane);
     if (t0 + kDepth < t1) next.look(a, table, t0 + kDepth, n, lane);
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) mask[i] = t0 + i < t1 ? first[i].ask(a, ring + i * Core::Tile::kBytes, bars + i, h, lane) : 0;
+    begin();  // the queries, while the first tiles are on their way
     int stage = 0;
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
@@ -561,12 +566,11 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
     constexpr int kTile = Core::kTile, kPart = kPartFloats<Core, D>, kWarps = Core::kWarps, kSlots = 2 * kWarps;
     static_assert(4 * kPart <= Core::kDepth * Core::Tile::kBytes, "a part takes the place of a warp's tiles");
     extern __shared__ __align__(16) char s_warps[];  // kShared bytes for each warp
-    struct Piece { int b, unit, left, right, last; };  // left, right: whether the unit begins and ends in this piece; last (of one that begins): the CTA of its end
+    struct __align__(16) Piece { int b, unit, ends, last; };  // ends: 1 where the unit begins in this piece, 2 where it ends; last (where it begins): the CTA of its end
     __shared__ uint64_t s_bars[kWarps][Core::kDepth];
     __shared__ Piece s_piece[kSlots];            // of each warp: what it left before it went on to another unit, and at its end
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    after_prior();
     if (lane < 2) s_piece[2 * warp + lane].b = -1;
     if (lane < Core::kDepth) mbar_init(&s_bars[warp][lane], 1);
     fence_mbar_init();
@@ -574,99 +578,143 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
     __syncwarp();
     TileWaits wait{a.wait_ns, false};
     uint32_t phase = 0;
-    const TileList<kTile> list(a, lane, blockIdx.x == 0 && warp == 0);
-    const long long base = list.share * blockIdx.x;
-    long long p = base + warp_first(list.share, warp, kWarps);
-    const long long end = min(base + warp_first(list.share, warp + 1, kWarps), list.total);
     Core core(s_warps + warp * Core::kShared);
     float *const early = a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + warp) * kPart, *const late = reinterpret_cast<float *>(s_warps + warp * Core::kShared);
-    const int per_block = (a.group + a.blocks - 1) / a.blocks;
-    if (p < end) {
-        long long begin;
-        int b = list.find(p, lane, begin);
-        bool bad;
-        int tiles = row_tiles<kTile>(a, b, bad), places = (int)unit_places(tiles, list.kLeast);
-        int unit = (p - begin) >> 32 ? (int)((p - begin) / places) : (int)((uint32_t)(p - begin) / (uint32_t)places);
-        int off = (int)(p - begin - (long long)unit * places);
-        while (true) {
-            const int upto = (int)min((long long)places, off + (end - p)), real = min(upto, tiles);
+    after_prior();
+    // Places from here on are counted from the CTA's first.
+    const int units = a.kvh * a.blocks;
+    int share = TileList<kTile>::kLeast, there = share, b = 0, unit = 0, off = 0, tiles = 0, places = share;
+    int p = warp_first(share, warp, kWarps), end = warp_first(share, warp + 1, kWarps);
+    bool bad = false;
+    if (!a.cut) {  // a unit a CTA
+        b = (int)blockIdx.x / units;
+        unit = (int)blockIdx.x - b * units;
+        tiles = row_tiles<kTile>(a, b, bad);
+        if (bad && unit == 0 && threadIdx.x == 0) out_of_range();
+        off = p;
+    } else {
+        const TileList<kTile> list(a, lane, blockIdx.x == 0 && warp == 0);
+        share = list.share;
+        const long long base = (long long)share * blockIdx.x;
+        there = (int)max(0ll, min((long long)share, list.total - base));
+        p = warp_first(share, warp, kWarps);
+        end = min(warp_first(share, warp + 1, kWarps), there);
+        if (p < end) {
+            long long begin;
+            b = list.find(base + p, lane, begin);
+            tiles = row_tiles<kTile>(a, b, bad);
+            places = unit_places(tiles, list.kLeast);
+            begin = base + p - begin;
+            unit = begin >> 31 ? (int)(begin / places) : (int)((uint32_t)begin / (uint32_t)places);
+            off = (int)(begin - (long long)unit * places);
+        }
+    }
+    if (tiles) {
+        while (p < end) {
+            const int upto = (int)min((long long)places, off + ((long long)end - p)), real = min(upto, tiles);
             if (off < real) {
-                const int h = unit / a.blocks, r0 = (unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
-                const int *table = a.tables + b * a.ts;
-                core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane);
-                run_tiles(core, a, wait, s_warps + warp * Core::kShared, s_bars[warp], phase, table, h, off, real, a.lens[b] + 1, lane);
+                const int h = a.blocks == 1 ? unit : unit / a.blocks, r0 = (unit - h * a.blocks) * a.per_block, nq = min(a.per_block, a.group - r0), head = h * a.group + r0;
+                run_tiles(core, [&] { core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane); }, a, wait, s_warps + warp * Core::kShared, s_bars[warp], phase, a.tables + b * a.ts, h, off, real,
+                          a.lens[b] + 1, lane);
                 core.finish();
                 if (off == 0 && real == tiles) {
                     char *out = a.out + b * a.os[0] + head * a.os[1];
                     float *lse = a.lse ? a.lse + (long long)b * a.heads + head : nullptr;
                     core.each(lane, [&](int r, int d, const auto &x, float, float l) { if (r < nq) store_row<T>(out + r * a.os[1] + d * (int)sizeof(T), x, over(l)); },
                               [&](int r, float m, float l) { if (r < nq && lse) lse[r] = log_sum(m, l); });
-                    if (lane == 0 && a.cut) a.cut[(long long)b * list.units + unit] = make_int2(0, 0);
+                    if (lane == 0 && a.cut) a.cut[(long long)b * units + unit] = make_int2(0, 0);
                 } else {
                     const bool last = p + (upto - off) >= end;  // the ring is free then
                     float *to = last ? late : early;
                     __syncwarp();
                     core.each(lane, [&](int r, int d, const auto &x, float, float) {
+                        if (r >= nq) return;
 #pragma unroll
                         for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); i += 4) *reinterpret_cast<float4 *>(to + r * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                     }, [&](int r, float m, float l) { to[Core::kRows * D + r] = m; to[Core::kRows * (D + 1) + r] = l; });
-                    const long long past = p - off - base + tiles - 1;  // its last tile's place, from this CTA's first
-                    const int further = past < list.share ? 0 : past >> 32 ? (int)(past / list.share) : (int)((uint32_t)past / (uint32_t)list.share);
-                    if (lane == 0) s_piece[2 * warp + last] = {b, unit, off == 0, real == tiles, (int)blockIdx.x + further};
+                    const unsigned int past = (unsigned int)(p - off + tiles - 1);  // its last tile's place, where it begins in this CTA
+                    if (lane == 0) s_piece[2 * warp + last] = {b, unit, (off == 0) | (real == tiles) << 1, (int)blockIdx.x + (off == 0 && past >= (unsigned int)share ? (int)(past / (unsigned int)share) : 0)};
                 }
             }
             p += upto - off;
             if (p >= end) break;
             off = 0;
-            if (++unit == list.units) {
+            if (++unit == units) {
                 unit = 0;
-                do ++b; while ((tiles = row_tiles<kTile>(a, b, bad)) == 0);  // there is one: p < total
-                places = (int)unit_places(tiles, list.kLeast);
+                do ++b; while ((tiles = row_tiles<kTile>(a, b, bad)) == 0);  // there is one before the end
+                places = unit_places(tiles, TileList<kTile>::kLeast);
             }
         }
     }
     __syncthreads();
-    // join the pieces that the warps left, in their order; what is not a whole unit goes to the workspace
-    const auto piece_at = [&](int j) { return j & 1 ? reinterpret_cast<const float *>(s_warps + j / 2 * Core::kShared) : a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + j / 2) * kPart; };
-    for (int s = 0; s < kSlots;) {
-        const Piece first = s_piece[s];
-        int e = s + 1;
-        if (first.b < 0) { s = e; continue; }
-        unsigned int among = 1u << s;  // the slots of this unit's pieces
-        bool right = first.right;
-        for (; e < kSlots; ++e) {
-            const Piece x = s_piece[e];
-            if (x.b < 0) continue;
-            if (x.b != first.b || x.unit != first.unit) break;
-            among |= 1u << e;
-            right = x.right;
-        }
-        const int h = first.unit / a.blocks, r0 = (first.unit - h * a.blocks) * per_block, nq = min(per_block, a.group - r0), head = h * a.group + r0;
-        const bool whole = first.left && right;
-        float *to = a.part + (2ll * blockIdx.x + first.left) * kPart;
-        for (int i = threadIdx.x; i < nq * (D / 4); i += 32 * kWarps) {
-            const int r = i / (D / 4), d = 4 * (i % (D / 4));
-            float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-            for (unsigned int j = among; j; j &= j - 1) top = fmaxf(top, piece_at(__ffs(j) - 1)[Core::kRows * D + r]);
-            for (unsigned int j = among; j; j &= j - 1) {
-                const float *from = piece_at(__ffs(j) - 1), m = from[Core::kRows * D + r], f = m == top ? 1.f : ex2(m - top);
-                const float4 y = *reinterpret_cast<const float4 *>(from + r * D + d);
-                l += f * from[Core::kRows * (D + 1) + r];
-                x[0] += f * y.x; x[1] += f * y.y; x[2] += f * y.z; x[3] += f * y.w;
+    // Join the pieces that the warps left; what is not a whole unit goes to the workspace. Lane j of every warp has the j-th piece, and a
+    // warp one row of the unit at a time: a piece's factor is worked out in its lane, then all lanes go through the pieces.
+    static_assert(kSlots <= 32, "");
+    Piece mine = {-1, 0, 0, 0};
+    if (lane < kSlots) mine = s_piece[lane];
+    const unsigned int valid = __ballot_sync(0xffffffffu, mine.b >= 0), below = valid & ((1u << lane) - 1);
+    const int before = below ? 31 - __clz(below) : lane;  // the piece before this one
+    const int b0 = __shfl_sync(0xffffffffu, mine.b, before), unit0 = __shfl_sync(0xffffffffu, mine.unit, before);
+    const unsigned int firsts = __ballot_sync(0xffffffffu, mine.b >= 0 && (!below || b0 != mine.b || unit0 != mine.unit));
+    const float *const from = lane & 1 ? reinterpret_cast<const float *>(s_warps + lane / 2 * Core::kShared) : a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + lane / 2) * kPart;
+    constexpr int kE = D / 32;
+    for (unsigned int left_over = firsts; left_over; left_over &= left_over - 1) {
+        const int s0 = __ffs(left_over) - 1;
+        const unsigned int later = firsts & ~((2u << s0) - 1), pieces = valid & ~((1u << s0) - 1) & (later ? (1u << (__ffs(later) - 1)) - 1 : ~0u);
+        const int b = __shfl_sync(0xffffffffu, mine.b, s0), unit = __shfl_sync(0xffffffffu, mine.unit, s0), last = __shfl_sync(0xffffffffu, mine.last, s0);
+        const int left = __shfl_sync(0xffffffffu, mine.ends, s0) & 1;
+        const bool whole = left && (__shfl_sync(0xffffffffu, mine.ends, 31 - __clz(pieces)) & 2);
+        const int h = a.blocks == 1 ? unit : unit / a.blocks, r0 = (unit - h * a.blocks) * a.per_block, nq = min(a.per_block, a.group - r0), head = h * a.group + r0;
+        float *to = a.part + (2ll * blockIdx.x + left) * kPart;
+        for (int r = warp; r < nq; r += kWarps) {
+            float m = -INFINITY, l = 0.f, x[kE];
+            if (pieces >> lane & 1) { m = from[Core::kRows * D + r]; l = from[Core::kRows * (D + 1) + r]; }
+            float top = m;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float f = m == top ? 1.f : ex2(m - top);
+            l *= f;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+            for (int i = 0; i < kE; ++i) x[i] = 0.f;
+            for (unsigned int p4 = pieces; p4;) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // (a piece that is not there: the first one, times nothing)
+                    const int j = p4 ? __ffs(p4) - 1 : s0;
+                    const float g = p4 ? __shfl_sync(0xffffffffu, f, j) : 0.f;
+                    const float *part = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)from, j)) + r * D + kE * lane;
+                    float y[kE];
+                    if constexpr (kE == 4) *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(part);
+                    else *reinterpret_cast<float2 *>(y) = *reinterpret_cast<const float2 *>(part);
+                    if (p4) {
+#pragma unroll
+                        for (int i = 0; i < kE; ++i) x[i] += g * y[i];
+                    }
+                    p4 &= p4 - 1;
+                }
             }
             if (whole) {
-                store_row<T>(a.out + first.b * a.os[0] + (head + r) * a.os[1] + d * (int)sizeof(T), x, over(l));
-                if (d == 0 && a.lse) a.lse[(long long)first.b * a.heads + head + r] = log_sum(top, l);
+                T *out = reinterpret_cast<T *>(a.out + b * a.os[0] + (head + r) * a.os[1]) + kE * lane;
+                const float g = over(l);
+                if constexpr (kE == 4) {
+                    const float y[4] = {x[0] * g, x[1] * g, x[2] * g, x[3] * g};
+                    store4(out, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kE; ++i) out[i] = from_f<T>(x[i] * g);
+                }
+                if (lane == 0 && a.lse) a.lse[(long long)b * a.heads + head + r] = log_sum(top, l);
             } else {
-                *reinterpret_cast<float4 *>(to + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-                if (d == 0) {
+                if constexpr (kE == 4) *reinterpret_cast<float4 *>(to + r * D + kE * lane) = make_float4(x[0], x[1], x[2], x[3]);
+                else *reinterpret_cast<float2 *>(to + r * D + kE * lane) = make_float2(x[0], x[1]);
+                if (lane == 0) {
                     to[Core::kRows * D + r] = top;
                     to[Core::kRows * (D + 1) + r] = l;
                 }
             }
         }
-        if (first.left && threadIdx.x == 0 && a.cut) a.cut[(long long)first.b * list.units + first.unit] = make_int2((int)blockIdx.x, first.last);
-        s = e;
+        if (left && threadIdx.x == 0 && a.cut) a.cut[(long long)b * units + unit] = make_int2((int)blockIdx.x, last);
     }
 }
 
@@ -678,13 +726,13 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Page
     __shared__ float s_x[8][D], s_m[8], s_l[8];
     after_prior();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % kWarps;
-    const long long row = (long long)blockIdx.x * (8 / kWarps) + warp / kWarps;
-    const bool there = row < (long long)a.batch * a.heads;
-    const int b = there ? (int)(row / a.heads) : 0, head = there ? (int)(row - (long long)b * a.heads) : 0, h = head / a.group, per_block = (a.group + a.blocks - 1) / a.blocks;
-    const int blk = (head - h * a.group) / per_block, r = head - h * a.group - blk * per_block;
+    const int row = (int)blockIdx.x * (8 / kWarps) + warp / kWarps;
+    const bool there = row < a.batch * a.heads;
+    const int b = there ? row / a.heads : 0, head = there ? row - b * a.heads : 0, h = head / a.group;
+    const int blk = a.blocks == 1 ? 0 : (head - h * a.group) / a.per_block, r = head - h * a.group - blk * a.per_block;
     const int2 cut = a.cut[(long long)b * a.kvh * a.blocks + h * a.blocks + blk];
     bool bad;
-    const bool split = there && row_tiles<Core::kTile>(a, b, bad) && cut.x < cut.y;  // (of a row without a token no one has written the cut)
+    const bool split = there && row_tiles<Core::kTile>(a, b, bad) && cut.x >= 0 && cut.x < cut.y && cut.y < a.ctas;  // (of a row without a token no one has written the cut)
     float x[kE], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < kE; ++i) x[i] = 0.f;
@@ -757,7 +805,9 @@ p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStr
     const auto kernel = k_paged_attn<T, D, Core>;
     constexpr int smem = Core::kWarps * Core::kShared;
     if (!allow_shared(kernel, which, smem)) return P8_ERR_CUDA;
-    const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);  // shares that there can be
+    // shares that there can be; in a CTA's share, and in the workspace, places and rows are counted in 32 bits
+    const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);
+    if (most / a.ctas >= INT32_MAX / 32 || c->rows * a.heads >= INT32_MAX - 256) return P8_ERR_UNSUPPORTED;
     if (launch_after(kernel, dim3((unsigned int)std::min<int64_t>(a.ctas, most)), dim3(32 * Core::kWarps), (size_t)smem, st, a) != cudaSuccess) return P8_ERR_CUDA;
     if (!a.cut) return P8_OK;
     const int64_t rows = c->rows * a.heads;
@@ -785,7 +835,7 @@ p8_status launch_paged_attn(const p8_paged *c, const p8_paged_attn_args *x, void
     a.lse = x->lse; a.part = cuts ? (float *)workspace : nullptr;
     a.cut = cuts ? reinterpret_cast<int2 *>((char *)workspace + attn_part_bytes(c, x->heads)) : nullptr;
     a.slots = c->columns * c->page; a.div = page_div((uint32_t)c->page); a.wait_ns = cache_wait_ns();
-    a.batch = (int)c->rows; a.heads = (int)x->heads; a.kvh = (int)c->heads; a.group = (int)(x->heads / c->heads); a.blocks = attn_blocks(c, x->heads);
+    a.batch = (int)c->rows; a.heads = (int)x->heads; a.kvh = (int)c->heads; a.group = (int)(x->heads / c->heads); a.blocks = attn_blocks(c, x->heads); a.per_block = (a.group + a.blocks - 1) / a.blocks;
     a.pages = (int)c->pages; a.ctas = sm_count();
     a.scale2 = (float)x->scale * 1.4426950408889634f;
     return c->width == 128 ? run_paged_attn_d<128>(c, a, st) : run_paged_attn_d<64>(c, a, st);

@@ -24,14 +24,14 @@ P8_HD uint32_t page_of(const PageDiv &d, uint32_t slot) { return (uint32_t)(((ui
 
 // Places of a sequence's head in the attention's list of tiles: one for each of its tiles, `least` at least (a place costs
 // nothing where there is no tile; short sequences then begin where a CTA's share does and stay in one piece).
-P8_HD int64_t unit_places(int64_t tiles, int64_t least) { return tiles == 0 ? 0 : tiles < least ? least : tiles; }
+P8_HD int unit_places(int tiles, int least) { return tiles == 0 ? 0 : tiles < least ? least : tiles; }
 // Each CTA's share of `total` places.
 P8_HD int64_t cta_share(int64_t total, int64_t ctas, int64_t least) {
     const int64_t s = total >> 32 ? (total + ctas - 1) / ctas : (int64_t)(((uint32_t)total + (uint32_t)ctas - 1) / (uint32_t)ctas);
     return s < least ? least : s;
 }
 // Warp w's part of a share, from its first place.
-P8_HD int64_t warp_first(int64_t share, int w, int warps) { return (share * w) / warps; }
+P8_HD int warp_first(int share, int w, int warps) { return share / warps * w + share % warps * w / warps; }
 
 // The position of the k-th set bit (k = 0: the lowest) of a word that has more than k.
 P8_HD int nth_bit(uint64_t m, int k) {

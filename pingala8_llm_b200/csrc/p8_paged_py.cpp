@@ -3,6 +3,8 @@
 // points' addresses by the package. Every call returns the p8_status; what is refused before it raises ValueError.
 #include "p8_py.h"
 
+#include <c10/cuda/CUDACachingAllocator.h>
+
 namespace {
 
 struct Entries {
@@ -86,12 +88,24 @@ p8_status paged_append_(PyObject *const *a) {
 }
 ENTRY(paged_append, 16)
 
-Tensor scratch(PyObject *o, size_t need, const Tensor &like, int64_t dev) {
-    if (o == Py_None) return at::empty({(int64_t)need}, like.options().dtype(at::kByte));
-    const Tensor &ws = tensor(o, "workspace");
-    if (!ws.is_cuda() || ws.get_device() != dev || !ws.is_contiguous()) refuse("workspace must be contiguous on the call's device");
-    return ws;
-}
+// the caller's workspace, or one of torch's allocator for this call (which goes back in the stream's order)
+struct Scratch {
+    c10::DataPtr own;
+    void *at = nullptr;
+    size_t bytes = 0;
+    Scratch(PyObject *o, size_t need, int64_t dev) {
+        if (o != Py_None) {
+            const Tensor &ws = tensor(o, "workspace");
+            if (!ws.is_cuda() || ws.get_device() != dev || !ws.is_contiguous()) refuse("workspace must be contiguous on the call's device");
+            at = ws.data_ptr();
+            bytes = ws.nbytes();
+        } else if (need) {
+            own = c10::cuda::CUDACachingAllocator::get()->allocate(need);
+            at = own.get();
+            bytes = need;
+        }
+    }
+};
 
 // q k_pages v_pages tables lens counts scale out lse workspace
 p8_status paged_attention_(PyObject *const *a) {
@@ -108,8 +122,8 @@ p8_status paged_attention_(PyObject *const *a) {
     x.out = rows<void>(a[7], "out", c.type, {B, H, D}, c, x.out_stride);
     x.lse = flat<float>(a[8], "lse", at::kFloat, {B, H}, c);
     const On on(c);
-    const Tensor ws = scratch(a[9], a[9] == Py_None ? g_p8.attn_workspace(&c.c, H) : 0, k, c.dev);
-    return g_p8.attn(&c.c, &x, ws.data_ptr(), ws.nbytes(), on.stream);
+    const Scratch ws(a[9], a[9] == Py_None ? g_p8.attn_workspace(&c.c, H) : 0, c.dev);
+    return g_p8.attn(&c.c, &x, ws.at, ws.bytes, on.stream);
 }
 ENTRY(paged_attention, 10)
 
@@ -141,8 +155,8 @@ p8_status beam_select_(PyObject *const *a) {
     x.tokens = flat<int64_t>(a[7], "tokens", at::kLong, {B, n}, c);
     x.out_done = flat<uint8_t>(a[8], "out_done", at::kBool, {B, n}, c);
     const On on(c);
-    const Tensor ws = scratch(a[9], a[9] == Py_None ? g_p8.select_workspace(B, W, x.vocab, n) : 0, l, c.dev);
-    return g_p8.select(&x, ws.data_ptr(), ws.nbytes(), on.stream);
+    const Scratch ws(a[9], a[9] == Py_None ? g_p8.select_workspace(B, W, x.vocab, n) : 0, c.dev);
+    return g_p8.select(&x, ws.at, ws.bytes, on.stream);
 }
 ENTRY(beam_select, 10)
 

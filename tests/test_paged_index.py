@@ -20,9 +20,9 @@ int64_t wrong(uint32_t page, uint32_t slots) {
             if (s >= 0 && s <= slots && p8::page_of(d, (uint32_t)s) != s / page) return s;
     return -1;
 }
-int64_t unit_places(int64_t t, int64_t least) { return p8::unit_places(t, least); }
+int unit_places(int t, int least) { return p8::unit_places(t, least); }
 int64_t cta_share(int64_t t, int64_t c, int64_t least) { return p8::cta_share(t, c, least); }
-int64_t warp_first(int64_t s, int w, int n) { return p8::warp_first(s, w, n); }
+int warp_first(int s, int w, int n) { return p8::warp_first(s, w, n); }
 int nth_bit(uint64_t m, int k) { return p8::nth_bit(m, k); }
 uint32_t order_key(uint32_t b) { return p8::order_key(b); }
 uint32_t order_bits(uint32_t k) { return p8::order_bits(k); }
@@ -38,7 +38,7 @@ def ix(tmp_path_factory):
     subprocess.run(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-I", os.path.join(ROOT, "pingala8_llm_b200", "csrc"), str(d / "x.cpp"), "-o", str(d / "x.so")], check=True)
     L = C.CDLL(str(d / "x.so"))
     i64, u32, u64 = C.c_int64, C.c_uint32, C.c_uint64
-    for name, res, args in (("page_of_", u32, [u32, u32]), ("wrong", i64, [u32, u32]), ("unit_places", i64, [i64, i64]), ("cta_share", i64, [i64, i64, i64]), ("warp_first", i64, [i64, C.c_int, C.c_int]),
+    for name, res, args in (("page_of_", u32, [u32, u32]), ("wrong", i64, [u32, u32]), ("unit_places", C.c_int, [C.c_int, C.c_int]), ("cta_share", i64, [i64, i64, i64]), ("warp_first", C.c_int, [C.c_int, C.c_int, C.c_int]),
                             ("nth_bit", C.c_int, [u64, C.c_int]), ("order_key", u32, [u32]), ("order_bits", u32, [u32]), ("select_splits", i64, [i64] * 6)):
         getattr(L, name).restype, getattr(L, name).argtypes = res, args
     return L
