@@ -80,7 +80,7 @@ __device__ __forceinline__ void sort128(unsigned long long (&x)[4], int lane) {
 }
 
 // keeps the n best of a warp's list, in order, and fills what is behind them with 0; returns the n-th
-__device__ __forceinline__ unsigned long long prune(unsigned long long *list, int count, int n, int lane) {
+__device__ __noinline__ unsigned long long prune(unsigned long long *list, int count, int n, int lane) {
     unsigned long long x[4];
     __syncwarp();
 #pragma unroll
@@ -624,10 +624,10 @@ bool select_sizes_ok(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
 // a block has 16 KB of logits or more
 int64_t splits_of(int64_t rows, int64_t beams, int64_t vocab, int es) { return select_splits(rows, beams, vocab, (int64_t)sm_count() * kScanBlocks, 16384 / es, 100000); }
 size_t select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
-    int64_t most = 1;
-    for (int es = 2; es <= 4; es += 2)
-        for (int64_t rows : {batch, batch * beams}) most = std::max(most, splits_of(rows, beams, vocab, es));
-    return (size_t)(batch * beams * most * (n + 1) * 8);
+    // of either type of logits, for all beams or for one of each group
+    const int64_t slots = (int64_t)sm_count() * kScanBlocks, least = 16384 / 4;
+    const int64_t pieces = std::max(batch * beams * select_limit(batch * beams, beams, vocab, slots, least), batch * select_limit(batch, beams, vocab, slots, least));
+    return (size_t)(pieces * (n + 1) * 8);
 }
 
 p8_status launch_beam_select(const p8_beam_select_args *x, void *workspace, cudaStream_t st) {

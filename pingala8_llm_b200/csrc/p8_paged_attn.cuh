@@ -333,7 +333,7 @@ struct Core16 {
 #pragma unroll
                 for (int o_ = 4; o_ < 32; o_ <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], o_);
     }
-    // f(row, d, eight values from d on), and h(row, m, l) once a row
+    // f(row, d, some values from d on), and h(row, m, l) once a row
     template <typename F, typename H>
     __device__ __forceinline__ void each(int lane, F f, H h) const {
         const int g = lane / 4, t = lane % 4;
@@ -350,7 +350,7 @@ struct Core16 {
                         x[2 * j] = o[i][4 * c + j][e];
                         x[2 * j + 1] = o[i][4 * c + j][e + 2];
                     }
-                    f(r, 64 * c + 8 * g, x, m[i][e], l[i][e]);
+                    f(r, 64 * c + 8 * g, x);
                 }
                 if (g == 0) h(r, m[i][e], l[i][e]);
             }
@@ -495,69 +495,119 @@ struct Core32 {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const float mi = __shfl_sync(0xffffffffu, m, i), li = __shfl_sync(0xffffffffu, l, i);
-            if (D == 128 || lane < 16) f(i, 4 * (lane % (D / 4)), o[i], mi, li);
+            if (D == 128 || lane < 16) f(i, 4 * (lane % (D / 4)), o[i]);
             if (lane == 0) h(i, mi, li);
         }
     }
 };
 
 // ----------------------------------------------------------------------------------------------------------------
-template <typename T, int N>
-__device__ __forceinline__ void store_row(char *p, const float (&x)[N], float f) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const float y[4] = {x[i] * f, x[i + 1] * f, x[i + 2] * f, x[i + 3] * f};
-        store4(reinterpret_cast<T *>(p) + i, y);
-    }
-}
 __device__ __forceinline__ float over(float l) { return l == 0.f ? 0.f : 1.f / l; }  // a row that sees nothing gets 0
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f; }
 
 // A part of a sequence's head: [kRows][D] sums, then the maxima, then the sums of the weights.
 template <typename Core, int D> constexpr int kPartFloats = Core::kRows * (D + 2);
 
-// Tiles [t0, t1) of a sequence of n slots. Their pages are looked up one tile before they are asked for. phase: a bit for
-// each stage of the warp's ring.
+// Tiles [t0, t1) of a sequence of n slots. Their pages are looked up one tile before they are asked for, and they are asked for
+// kDepth tiles before they are wanted: the loop begins that much earlier. (Written once, not as a beginning and a loop: code that a launch comes to for the
+// first time is slow.) phase: a bit for each stage of the warp's ring.
 template <typename Core, typename Begin>
 __device__ __forceinline__ void run_tiles(Core &core, const Begin &begin, const PagedAttnArgs &a, TileWaits &wait, char *ring, uint64_t *bars, uint32_t &phase, const int *table, int h, int t0, int t1, int n, int lane) {
     constexpr int kDepth = Core::kDepth;
-    typename Core::Tile next, first[kDepth];
-    unsigned int mask[kDepth];
-    if (wait.gave_up) {
-        begin();
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i)
-        if (t0 + i < t1) first[i].look(a, table, t0 + i, n, lane);
-    if (t0 + kDepth < t1) next.look(a, table, t0 + kDepth, n, lane);
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i) mask[i] = t0 + i < t1 ? first[i].ask(a, ring + i * Core::Tile::kBytes, bars + i, h, lane) : 0;
-    begin();  // the queries, while the first tiles are on their way
+    typename Core::Tile next;
+    unsigned int mask[kDepth] = {};
     int stage = 0;
+    next.look(a, table, t0, n, lane);
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
+    for (int t = t0 - kDepth; t < t1; ++t) {
         char *tile = ring + stage * Core::Tile::kBytes;
-        if (!wait(bars + stage, phase >> stage & 1)) {
-            for (int i = 0; i < kDepth && t + i < t1; ++i) {
-                TileWaits::settle(bars + stage, phase >> stage & 1);
-                phase ^= 1u << stage;
-                stage = stage + 1 == kDepth ? 0 : stage + 1;
+        if (t >= t0) {
+            if (!wait.gave_up && !wait(bars + stage, phase >> stage & 1)) {
+                for (int i = 0, at = stage; i < kDepth && t + i < t1; ++i) {
+                    TileWaits::settle(bars + at, phase >> at & 1);
+                    phase ^= 1u << at;
+                    at = at + 1 == kDepth ? 0 : at + 1;
+                }
             }
-            return;
+            if (wait.gave_up) return;
+            phase ^= 1u << stage;
+            typename Core::Scores s;
+            core.scores(s, tile, lane);
+            core.weigh_and_add(s, tile, mask[0], a.scale2, lane);
+            __syncwarp();  // all have read the tile
         }
-        phase ^= 1u << stage;
-        typename Core::Scores s;
-        core.scores(s, tile, lane);
-        core.weigh_and_add(s, tile, mask[0], a.scale2, lane);
 #pragma unroll
         for (int i = 0; i + 1 < kDepth; ++i) mask[i] = mask[i + 1];
-        __syncwarp();  // all have read the tile
-        if (t + kDepth < t1) {
+        if (t + kDepth < t1 && !wait.gave_up) {
             mask[kDepth - 1] = next.ask(a, tile, bars + stage, h, lane);
             if (t + kDepth + 1 < t1) next.look(a, table, t + kDepth + 1, n, lane);
         }
+        if (t == t0 - 1) begin();  // the queries, while the first tiles are on their way
         stage = stage + 1 == kDepth ? 0 : stage + 1;
+    }
+}
+
+// Adds the parts of a unit's rows up: lane j has the address of the j-th (of `pieces`, those that there are; the lowest is piece
+// s0). A part's factor for a row is worked out in its lane, then all lanes go through the parts. The rows are r0, r0 + step, .. of nq, of query heads head, ..;
+// to: where the sum goes as a part; NULL: it is all, and goes to the outputs.
+template <typename T, int D, int kRows>
+__device__ __noinline__ void join_parts(const PagedAttnArgs &a, const float *from, unsigned int pieces, int s0, int r0, int step, int nq, int b, int head, float *to) {
+    constexpr int kE = D / 32;
+    const int lane = threadIdx.x % 32;
+#pragma unroll 1
+    for (int r = r0; r < nq; r += step) {
+        float m = -INFINITY, l = 0.f, x[kE];
+        if (pieces >> lane & 1) { m = from[kRows * D + r]; l = from[kRows * (D + 1) + r]; }
+        float top = m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float f = m == top ? 1.f : ex2(m - top);
+        l *= f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) x[i] = 0.f;
+#pragma unroll 1
+        for (unsigned int left = pieces; left;) {
+            float y[4][kE], g[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // (a part that is not there: the first one, times nothing)
+                const int j = left ? __ffs(left) - 1 : s0;
+                g[k] = __shfl_sync(0xffffffffu, f, j);
+                if (!left) g[k] = 0.f;
+                const float *part = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)from, j)) + r * D + kE * lane;
+                if constexpr (kE == 4) *reinterpret_cast<float4 *>(y[k]) = *reinterpret_cast<const float4 *>(part);
+                else *reinterpret_cast<float2 *>(y[k]) = *reinterpret_cast<const float2 *>(part);
+                if (!left) {
+#pragma unroll
+                    for (int i = 0; i < kE; ++i) y[k][i] = 0.f;
+                }
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[i] += g[k] * y[k][i];
+        }
+        if (!to) {
+            T *out = reinterpret_cast<T *>(a.out + b * a.os[0] + (head + r) * a.os[1]) + kE * lane;
+            const float inv = over(l);
+            if constexpr (kE == 4) {
+                const float z[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+                store4(out, z);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kE; ++i) out[i] = from_f<T>(x[i] * inv);
+            }
+            if (lane == 0 && a.lse) a.lse[(long long)b * a.heads + head + r] = log_sum(top, l);
+        } else {
+            if constexpr (kE == 4) *reinterpret_cast<float4 *>(to + r * D + kE * lane) = make_float4(x[0], x[1], x[2], x[3]);
+            else *reinterpret_cast<float2 *>(to + r * D + kE * lane) = make_float2(x[0], x[1]);
+            if (lane == 0) {
+                to[kRows * D + r] = top;
+                to[kRows * (D + 1) + r] = l;
+            }
+        }
     }
 }
 
@@ -617,21 +667,21 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
                 run_tiles(core, [&] { core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane); }, a, wait, s_warps + warp * Core::kShared, s_bars[warp], phase, a.tables + b * a.ts, h, off, real,
                           a.lens[b] + 1, lane);
                 core.finish();
-                if (off == 0 && real == tiles) {
-                    char *out = a.out + b * a.os[0] + head * a.os[1];
-                    float *lse = a.lse ? a.lse + (long long)b * a.heads + head : nullptr;
-                    core.each(lane, [&](int r, int d, const auto &x, float, float l) { if (r < nq) store_row<T>(out + r * a.os[1] + d * (int)sizeof(T), x, over(l)); },
-                              [&](int r, float m, float l) { if (r < nq && lse) lse[r] = log_sum(m, l); });
-                    if (lane == 0 && a.cut) a.cut[(long long)b * units + unit] = make_int2(0, 0);
-                } else {
-                    const bool last = p + (upto - off) >= end;  // the ring is free then
-                    float *to = last ? late : early;
-                    __syncwarp();
-                    core.each(lane, [&](int r, int d, const auto &x, float, float) {
-                        if (r >= nq) return;
+                const bool all = off == 0 && real == tiles, last = p + (upto - off) >= end;  // the ring is free at the warp's end, and for as long as a whole unit is written
+                float *to = all || last ? late : early;
+                __syncwarp();
+                core.each(lane, [&](int r, int d, const auto &x) {
+                    if (r >= nq) return;
 #pragma unroll
-                        for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); i += 4) *reinterpret_cast<float4 *>(to + r * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-                    }, [&](int r, float m, float l) { to[Core::kRows * D + r] = m; to[Core::kRows * (D + 1) + r] = l; });
+                    for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); i += 4) *reinterpret_cast<float4 *>(to + r * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                }, [&](int r, float m, float l) { to[Core::kRows * D + r] = m; to[Core::kRows * (D + 1) + r] = l; });
+                if (all) {
+                    __syncwarp();
+                    join_parts<T, D, Core::kRows>(a, to, 1u, 0, 0, 1, nq, b, head, nullptr);
+                    if (lane == 0 && a.cut) a.cut[(long long)b * units + unit] = make_int2(0, 0);
+                    __syncwarp();
+                    fence_proxy_async();  // before the next unit's tiles
+                } else {
                     const unsigned int past = (unsigned int)(p - off + tiles - 1);  // its last tile's place, where it begins in this CTA
                     if (lane == 0) s_piece[2 * warp + last] = {b, unit, (off == 0) | (real == tiles) << 1, (int)blockIdx.x + (off == 0 && past >= (unsigned int)share ? (int)(past / (unsigned int)share) : 0)};
                 }
@@ -647,8 +697,7 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
         }
     }
     __syncthreads();
-    // Join the pieces that the warps left; what is not a whole unit goes to the workspace. Lane j of every warp has the j-th piece, and a
-    // warp one row of the unit at a time: a piece's factor is worked out in its lane, then all lanes go through the pieces.
+    // Join the pieces that the warps left; what is not a whole unit goes to the workspace. Lane j of every warp has the j-th piece.
     static_assert(kSlots <= 32, "");
     Piece mine = {-1, 0, 0, 0};
     if (lane < kSlots) mine = s_piece[lane];
@@ -657,7 +706,7 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
     const int b0 = __shfl_sync(0xffffffffu, mine.b, before), unit0 = __shfl_sync(0xffffffffu, mine.unit, before);
     const unsigned int firsts = __ballot_sync(0xffffffffu, mine.b >= 0 && (!below || b0 != mine.b || unit0 != mine.unit));
     const float *const from = lane & 1 ? reinterpret_cast<const float *>(s_warps + lane / 2 * Core::kShared) : a.part + (2ll * gridDim.x + (long long)blockIdx.x * kWarps + lane / 2) * kPart;
-    constexpr int kE = D / 32;
+#pragma unroll 1
     for (unsigned int left_over = firsts; left_over; left_over &= left_over - 1) {
         const int s0 = __ffs(left_over) - 1;
         const unsigned int later = firsts & ~((2u << s0) - 1), pieces = valid & ~((1u << s0) - 1) & (later ? (1u << (__ffs(later) - 1)) - 1 : ~0u);
@@ -665,55 +714,7 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
         const int left = __shfl_sync(0xffffffffu, mine.ends, s0) & 1;
         const bool whole = left && (__shfl_sync(0xffffffffu, mine.ends, 31 - __clz(pieces)) & 2);
         const int h = a.blocks == 1 ? unit : unit / a.blocks, r0 = (unit - h * a.blocks) * a.per_block, nq = min(a.per_block, a.group - r0), head = h * a.group + r0;
-        float *to = a.part + (2ll * blockIdx.x + left) * kPart;
-        for (int r = warp; r < nq; r += kWarps) {
-            float m = -INFINITY, l = 0.f, x[kE];
-            if (pieces >> lane & 1) { m = from[Core::kRows * D + r]; l = from[Core::kRows * (D + 1) + r]; }
-            float top = m;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float f = m == top ? 1.f : ex2(m - top);
-            l *= f;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-#pragma unroll
-            for (int i = 0; i < kE; ++i) x[i] = 0.f;
-            for (unsigned int p4 = pieces; p4;) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {  // (a piece that is not there: the first one, times nothing)
-                    const int j = p4 ? __ffs(p4) - 1 : s0;
-                    const float g = p4 ? __shfl_sync(0xffffffffu, f, j) : 0.f;
-                    const float *part = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)from, j)) + r * D + kE * lane;
-                    float y[kE];
-                    if constexpr (kE == 4) *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(part);
-                    else *reinterpret_cast<float2 *>(y) = *reinterpret_cast<const float2 *>(part);
-                    if (p4) {
-#pragma unroll
-                        for (int i = 0; i < kE; ++i) x[i] += g * y[i];
-                    }
-                    p4 &= p4 - 1;
-                }
-            }
-            if (whole) {
-                T *out = reinterpret_cast<T *>(a.out + b * a.os[0] + (head + r) * a.os[1]) + kE * lane;
-                const float g = over(l);
-                if constexpr (kE == 4) {
-                    const float y[4] = {x[0] * g, x[1] * g, x[2] * g, x[3] * g};
-                    store4(out, y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kE; ++i) out[i] = from_f<T>(x[i] * g);
-                }
-                if (lane == 0 && a.lse) a.lse[(long long)b * a.heads + head + r] = log_sum(top, l);
-            } else {
-                if constexpr (kE == 4) *reinterpret_cast<float4 *>(to + r * D + kE * lane) = make_float4(x[0], x[1], x[2], x[3]);
-                else *reinterpret_cast<float2 *>(to + r * D + kE * lane) = make_float2(x[0], x[1]);
-                if (lane == 0) {
-                    to[Core::kRows * D + r] = top;
-                    to[Core::kRows * (D + 1) + r] = l;
-                }
-            }
-        }
+        join_parts<T, D, Core::kRows>(a, from, pieces, s0, warp, kWarps, nq, b, head, whole ? nullptr : a.part + (2ll * blockIdx.x + left) * kPart);
         if (left && threadIdx.x == 0 && a.cut) a.cut[(long long)b * units + unit] = make_int2((int)blockIdx.x, last);
     }
 }

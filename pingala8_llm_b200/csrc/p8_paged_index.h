@@ -50,10 +50,18 @@ P8_HD uint32_t order_bits(uint32_t key) { return key & 0x80000000u ? key & 0x7ff
 // Blocks of one row of logits, none with less than `least` of them, and so few for many beams that the pieces of a group stay within
 // 256. With `slots` blocks at a time the rows take as long as the blocks of one slot, one after the other: their logits, and for each
 // block what it takes beside them (`extra`, in logits). The number that makes this least.
+P8_HD int64_t select_limit(int64_t rows, int64_t beams, int64_t vocab, int64_t slots, int64_t least) {
+    int64_t s = 256 / beams;
+    const int64_t fit = (vocab + least - 1) / least, waves = 2 * slots / rows + 2;  // (beyond two rounds of blocks the extra outweighs any evenness)
+    if (s > fit) s = fit;
+    if (s > waves) s = waves;
+    return s < 1 ? 1 : s;
+}
 P8_HD int64_t select_splits(int64_t rows, int64_t beams, int64_t vocab, int64_t slots, int64_t least, int64_t extra) {
-    const int64_t most = 256 / beams, fit = (vocab + least - 1) / least;
-    int64_t best = 1, best_cost = INT64_MAX;
-    for (int64_t s = 1; s <= most && s <= fit; ++s) {
+    const int64_t most = select_limit(rows, beams, vocab, slots, least);
+    const int64_t first = rows <= slots ? slots / rows < most ? slots / rows : most : 1;  // as many as run at once
+    int64_t best = first, best_cost = INT64_MAX;
+    for (int64_t s = first; s <= most && s <= first + 8; ++s) {
         const int64_t cost = (rows * s + slots - 1) / slots * ((vocab + s - 1) / s + extra);
         if (cost < best_cost) {
             best = s;
