@@ -7,7 +7,8 @@ in Q8_0 (blocks of 32 int8 with one fp16 scale, as the reference's model files k
 Q8_0 values as fp16), RoPE, the optional per-head q/k RMSNorm of Qwen3, attention with torch SDPA over a static KV
 cache, residual adds, greedy sampling. A decode step reads its position from the device and writes into fixed
 buffers, so it is captured once as a CUDA graph and replayed per token. TreeDecoder runs the same layers over drafted
-trees of tokens and a cache that can be bounded, with the package's own cache operators in place of the torch ones.
+trees of tokens and a cache that can be bounded, with the package's own cache operators in place of the torch ones; BeamDecoder
+runs them for a batch of prompts with several beams each over a paged cache.
 
 The reference runs this model in llama.cpp (MUL_MAT nodes dispatched to ggml_cuda_f44_mul_mat_vec / _mul_mat_q8,
 CU:1330-1342); its runtime is not available here, so this module restates the same architecture as a plain
@@ -357,6 +358,163 @@ class TreeDecoder:
             history += got
             passes += 1
         return torch.tensor(out[:n_new], dtype=torch.int64, device=prompt.device), passes
+
+
+class BeamDecoder:
+    """Beam search of a Model for a batch of prompts, over a paged cache: the beams of a prompt share its full pages, and share what
+    they write for as long as they go the same way.
+
+    A step takes one token of every beam at once: the projections through the batched product, norms, rotation and
+    cache writes through paged.paged_append, attention through paged.paged_attention, the choice through paged.beam_select, the
+    cache's change of beams through paged.beam_reorder. All pages that a beam can come to are laid out beforehand, so the device
+    decides everything and a step is captured once as a CUDA graph. batch, beams: how many prompts and beams of each; max_prompt,
+    max_new: how long prompts and continuations can be; dtype: the cache's type; page: its slots; end: the token that ends a
+    sequence, whose beam then stays as it is; rotary: how far positions are stretched (arguments of paged.rotary_tables)."""
+
+    def __init__(self, model, batch, beams, max_prompt, max_new, dtype=torch.float16, page=16, end=None, rotary=None):
+        if min(batch, beams, max_prompt, max_new, page) < 1 or (end is not None and not 0 <= end < model.c.vocab):
+            raise ValueError(f"{batch} prompts of up to {max_prompt} tokens, {beams} beams, {max_new} new tokens, pages of {page}, end {end}: one of each or more, a token that there is")
+        from . import paged  # its calls are a module built against torch's headers, which Model does without
+
+        if beams > paged.BEAMS_MAX:
+            raise ValueError(f"{beams} beams: {paged.BEAMS_MAX} at most")
+        self._paged = paged
+        c, dev = model.c, model.device
+        self.m, self.batch, self.beams, self.max_prompt, self.max_new, self.page, self.end = model, batch, beams, max_prompt, max_new, page, end
+        shared, rows = max_prompt // page, batch * beams
+        self.columns = (max_prompt + max_new + page - 1) // page
+        own = max_new // page + 2  # columns of a beam that begin behind the prompt's full pages
+        pages = batch * shared + rows * own
+        self.k, self.v = (torch.zeros(model.nl, pages, c.kv_heads, page, c.head_dim, dtype=dtype, device=dev) for _ in range(2))
+        self._shared, self._own = shared, own
+        self.cos, self.sin = rope_tables(c, max_prompt + max_new, dev) if rotary is None else paged.rotary_tables(max_prompt + max_new, c.head_dim, c.rope_theta, device=dev, **rotary)
+        self.tables = torch.zeros(rows, self.columns, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
+        self.scores = torch.zeros(batch, beams, device=dev)
+        self.done = None if end is None else torch.zeros(batch, beams, dtype=torch.bool, device=dev)
+        self.tokens = torch.zeros(batch, beams, dtype=torch.int64, device=dev)
+        self.said, self.came_from = (torch.zeros(max_new, batch, beams, dtype=torch.int64, device=dev) for _ in range(2))
+        self.at = torch.zeros(1, dtype=torch.int64, device=dev)  # how many tokens every beam has
+
+    def _layers(self, x, attend):
+        """the layers over x [n, hidden]; attend(layer index, q, k, v) -> [n, heads * head_dim]"""
+        c = self.m.c
+        for L, layer in enumerate(self.m.layers):
+            t = layer["t"]
+            q, k, v = mul_mat_group([t["q"], t["k"], t["v"]], x, norm_weight=layer["attn_norm"], eps=c.eps)
+            h = x + t["o"].mul_mat(attend(L, q, k, v).float())
+            g, u = mul_mat_group([t["gate"], t["up"]], h, norm_weight=layer["ffn_norm"], eps=c.eps)
+            x = h + t["down"].mul_mat(g, up=u)
+        return x
+
+    def _append(self, L, q, k, v, B, T, tables, lens, pos):
+        c = self.m.c
+        qn, kn = self.m.layers[L]["qk_norm"] if c.qk_norm else (None, None)
+        return self._paged.paged_append(q.view(B, T, c.heads, c.head_dim), k.view(B, T, c.kv_heads, c.head_dim), v.view(B, T, c.kv_heads, c.head_dim), self.k[L], self.v[L], tables, lens, pos,
+                                        self.cos, self.sin, q_norm=qn, k_norm=kn, eps=c.eps)
+
+    def _choose(self, logits):
+        """logits [batch, beams, vocab] -> the beams' next tokens, their parents noted, the cache theirs"""
+        best = self._paged.beam_select(logits, self.scores, done=self.done, end=self.end)
+        self.scores.copy_(best.scores)
+        if self.done is not None:
+            self.done.copy_(best.done)
+        self.tokens.copy_(best.tokens)
+        self.said.index_copy_(0, self.at, best.tokens[None])
+        self.came_from.index_copy_(0, self.at, best.parents[None].long())
+        self.at += 1
+        self._paged.beam_reorder(best.parents, self.k, self.v, self.tables, self.lens)
+
+    def prefill(self, prompts):
+        """a list of `batch` prompts, int64 [n] each: their keys and values into the first beam's pages, the first tokens chosen"""
+        c, P, W = self.m.c, self.page, self.beams
+        if len(prompts) != self.batch or any(not 1 <= p.numel() <= self.max_prompt for p in prompts):
+            raise ValueError(f"{self.batch} prompts of 1 to {self.max_prompt} tokens")
+        lens = [p.numel() for p in prompts]
+        first = self.batch * self._shared  # pages from here on belong to one beam each
+        tables = torch.zeros(self.batch * W, self.columns, dtype=torch.int32)
+        for b, n in enumerate(lens):
+            full = n // P
+            tables[b * W:(b + 1) * W, :full] = torch.arange(b * self._shared, b * self._shared + full, dtype=torch.int32)
+            behind = self.columns - full if self.columns - full < self._own else self._own
+            tables[b * W:(b + 1) * W, full:full + behind] = first + torch.arange(b * W, (b + 1) * W, dtype=torch.int32)[:, None] * self._own + torch.arange(behind, dtype=torch.int32)
+        self.tables.copy_(tables)
+        self.at.zero_()
+        self.scores.fill_(-math.inf)
+        self.scores[:, 0] = 0
+        if self.done is not None:
+            self.done.zero_()
+        zero, last = torch.zeros(1, dtype=torch.int32, device=self.m.device), []
+        for b, p in enumerate(prompts):
+            n, row = lens[b], self.tables[b * W:b * W + 1]
+            pos = torch.arange(n, dtype=torch.int32, device=self.m.device)[None]
+            used = row[0, :(n + P - 1) // P].long()
+
+            def attend(L, q, k, v):
+                q = self._append(L, q, k, v, 1, n, row, zero, pos)[0].transpose(0, 1)
+                kk, vv = (x[L][used].transpose(0, 1).reshape(c.kv_heads, -1, c.head_dim)[:, :n] for x in (self.k, self.v))
+                o = torch.nn.functional.scaled_dot_product_attention(q[None], kk[None], vv[None], is_causal=True, enable_gqa=True)
+                return o[0].transpose(0, 1).reshape(n, -1)
+
+            last.append(self._layers(self.m.embed.dequant(p), attend)[-1])
+        self.lens.copy_(torch.tensor(lens, dtype=torch.int32).repeat_interleave(W))
+        self.hidden = rms(torch.stack(last), self.m.final_norm, c.eps)
+        self.logits = (self.hidden.half() @ self.m.head_w.T)[:, None].expand(-1, W, -1)
+        self._choose(self.logits)
+
+    def step(self):
+        """one token for every beam; graph-capturable"""
+        rows = self.batch * self.beams
+        pos = self.lens[:, None].contiguous()
+        tokens = self.tokens.view(-1).clamp(min=0)  # (-1: a beam that is not there)
+
+        def attend(L, q, k, v):
+            q = self._append(L, q, k, v, rows, 1, self.tables, self.lens, pos)
+            return self._paged.paged_attention(q[:, 0], self.k[L], self.v[L], self.tables, self.lens)[0].reshape(rows, -1)
+
+        self.hidden = rms(self._layers(self.m.embed.dequant(tokens), attend), self.m.final_norm, self.m.c.eps)
+        self.lens += 1
+        self.logits = (self.hidden.half() @ self.m.head_w.T).view(self.batch, self.beams, -1)
+        self._choose(self.logits)
+
+    def capture(self):
+        """step() as a CUDA graph; the state (cache, tables, lengths, scores) is as it was afterwards only if prefill() follows"""
+        st = torch.cuda.Stream(device=self.m.device)
+        st.wait_stream(torch.cuda.current_stream(self.m.device))
+        with torch.cuda.stream(st):
+            self.step()  # warm-up outside capture
+        torch.cuda.synchronize(self.m.device)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=st):
+            self.step()
+        return self.graph
+
+    def history(self, n):
+        """the beams' tokens so far, int64 [batch, beams, n], the best beam first; -1 where a beam is not there"""
+        beam = torch.arange(self.beams, device=self.said.device).expand(self.batch, -1)
+        out = []
+        for i in range(n - 1, -1, -1):
+            out.append(self.said[i].gather(1, beam))
+            parent = self.came_from[i].gather(1, beam)
+            beam = torch.where(parent < 0, beam, parent)
+        return torch.stack(out[::-1], dim=-1)
+
+    def generate(self, prompts, n_new, graph=True):
+        """prompts: `batch` tensors int64 [n]; returns (tokens int64 [batch, beams, n_new], scores float32 [batch, beams]): the best
+        continuations that the search found, the best first, with the sums of their log probabilities (the token `end` goes on to the end of
+        a sequence that has ended, for nothing)."""
+        if not 1 <= n_new <= self.max_new:
+            raise ValueError(f"1 to {self.max_new} new tokens")
+        if graph and n_new > 1 and not hasattr(self, "graph"):
+            self.prefill(prompts)
+            self.capture()
+        self.prefill(prompts)
+        for _ in range(n_new - 1):
+            if graph:
+                self.graph.replay()
+            else:
+                self.step()
+        return self.history(n_new), self.scores.clone()
 
 
 def lookup_draft(history, width=4, depth=7):
