@@ -23,7 +23,7 @@ struct PagedAttnArgs {
     long long slots;
     PageDiv div;
     unsigned int wait_ns;
-    int batch, heads, kvh, group, blocks, per_block, pages, ctas;  // group: query heads of a cache head, in so many blocks of at most per_block
+    int batch, heads, kvh, group, blocks, per_block, pages, ctas, pad;  // group: query heads of a cache head, in so many blocks of at most per_block
     float scale2;                                       // scale / ln 2: the kernel's exponentials are powers of two
 };
 
@@ -83,7 +83,7 @@ struct TileList {
             const int b = lane * per + i;
             if (b >= a.batch) break;
             bool bad;
-            mine += unit_places(row_tiles<kTile>(a, b, bad), kLeast);
+            mine += unit_places(row_tiles<kTile>(a, b, bad), a.pad);
             any_bad |= bad;
         }
         if (report && any_bad) out_of_range();
@@ -107,7 +107,7 @@ struct TileList {
         for (int i0 = 0;; i0 += 32) {  // (the place is in one of these sequences)
             const int b = l * per + i0 + lane;
             bool bad;
-            long long c = i0 + lane < per && b < a.batch ? unit_places(row_tiles<kTile>(a, b, bad), kLeast) * units : 0, u = c;
+            long long c = i0 + lane < per && b < a.batch ? unit_places(row_tiles<kTile>(a, b, bad), a.pad) * units : 0, u = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long v = __shfl_up_sync(0xffffffffu, u, o);
@@ -117,7 +117,7 @@ struct TileList {
             if (w || i0 + 32 >= per) {
                 const int k = w ? __ffs(w) - 1 : 31;
                 begin += __shfl_sync(0xffffffffu, u - c, k);
-                return l * per + i0 + k;
+                return min(l * per + i0 + k, a.batch - 1);
             }
             begin += __shfl_sync(0xffffffffu, u, 31);
         }
@@ -162,7 +162,7 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
-// A tile's rows, one a lane: the keys of its slots in the first kTile lanes, the values in the next. The rows lie kKeyStride and
+// A tile's rows, one a lane: the keys of its slots in the first kTile lanes, the values in the next (of 32 slots: both in one). The rows lie kKeyStride and
 // kValueStride bytes apart in shared memory.
 template <int kTile, int kRowBytes, int kKeyStride, int kValueStride>
 struct Tiles {
@@ -184,21 +184,25 @@ struct Tiles {
     __device__ __forceinline__ unsigned int ask(const PagedAttnArgs &a, char *to, uint64_t *bar, int h, int lane) const {
         const bool there = (unsigned int)id < (unsigned int)a.pages;
         if (!there && id != -1) out_of_range();
-        const unsigned int mask = __ballot_sync(0xffffffffu, there) & ((1u << kTile) - 1);
-        const int z = lane / kTile;
+        const unsigned int mask = __ballot_sync(0xffffffffu, there) & (~0u >> (32 - kTile));
         if (lane == 0) mbar_expect_tx(bar, __popc(mask) * 2 * kRowBytes);
-        char *row = to + (z ? kTile * kKeyStride + lane % kTile * kValueStride : lane * kKeyStride);
-        if (z == 1 && !there) {
+        constexpr int kBoth = kTile == 32 ? 2 : 1;  // rows of a lane
+#pragma unroll
+        for (int i = 0; i < kBoth; ++i) {
+            const int z = kBoth == 2 ? i : lane / kTile;
+            char *row = to + (z ? kTile * kKeyStride + lane % kTile * kValueStride : lane * kKeyStride);
+            if (z == 1 && !there) {
 #pragma unroll 1
-            for (int i = 0; i < kRowBytes; i += 16) *reinterpret_cast<uint4 *>(row + i) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async();  // before the next tile's copies
-        }
-        __syncwarp();
-        if (z < 2 && there) {
-            const char *from = a.kv[z] + h * a.st[z][1] + id * a.st[z][0] + in * a.st[z][2];
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"((unsigned int)__cvta_generic_to_shared(row)), "l"(from), "r"(kRowBytes),
-                         "r"((unsigned int)__cvta_generic_to_shared(bar))
-                         : "memory");
+                for (int j = 0; j < kRowBytes; j += 16) *reinterpret_cast<uint4 *>(row + j) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();  // before the next tile's copies
+            }
+            if (i == 0) __syncwarp();
+            if (z < 2 && there) {
+                const char *from = a.kv[z] + h * a.st[z][1] + id * a.st[z][0] + in * a.st[z][2];
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"((unsigned int)__cvta_generic_to_shared(row)), "l"(from), "r"(kRowBytes),
+                             "r"((unsigned int)__cvta_generic_to_shared(bar))
+                             : "memory");
+            }
         }
         return mask;
     }
@@ -215,9 +219,10 @@ struct Tiles {
 // a reduction and a rescaling.
 template <typename T, int D, int kN>
 struct Core16 {
-    static constexpr int kTile = 16, kRows = 8 * kN, kKeys = 2 * D + 64, kValues = 2 * D + 16;  // rows so far apart that eight lanes' 16 bytes are in different banks
+    static constexpr int kSub = D == 64 ? 2 : 1, kTile = 16 * kSub, kRows = 8 * kN;  // sixteen slots make a product; shorter rows come in tiles of as many bytes
+    static constexpr int kKeys = D == 64 ? 128 : 2 * D + 64, kValues = 2 * D + 16;  // rows so far apart that eight lanes' 16 bytes are in different banks (keys of 64: two in each)
     using Tile = Tiles<kTile, 2 * D, kKeys, kValues>;
-    static constexpr int kDepth = D == 64 || kN == 2 ? 3 : 2, kWarps = kN == 1 ? 12 : 8, kShared = kDepth * Tile::kBytes;  // of a warp
+    static constexpr int kDepth = kN == 2 ? 3 : 2, kWarps = kN == 1 ? 12 : 8, kShared = kDepth * Tile::kBytes;  // of a warp
     static constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = 8.f;
     uint32_t q[kN][D / 32][4];
     float o[kN][D / 16][4], m[kN][2], l[kN][2];
@@ -239,44 +244,49 @@ struct Core16 {
             l[i][0] = l[i][1] = 0.f;
         }
     }
-    struct Scores { float x[kN][4]; };
+    struct Scores { float x[kSub][kN][4]; };
     __device__ __forceinline__ void scores(Scores &y, const char *tile, int lane) const {
-        float (&s)[kN][4] = y.x;
-        const char *key = tile + lane / 4 * kKeys + 16 * (lane % 4);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int u = 0; u < kSub; ++u) {
+            const char *key = tile + (16 * u + lane / 4) * kKeys + 16 * (lane % 4);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            const uint4 k0 = *reinterpret_cast<const uint4 *>(key + 64 * j), k1 = *reinterpret_cast<const uint4 *>(key + 8 * kKeys + 64 * j);
+            for (int i = 0; i < kN; ++i) y.x[u][i][0] = y.x[u][i][1] = y.x[u][i][2] = y.x[u][i][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                mma16816<T>(s[i], k0.x, k1.x, k0.y, k1.y, q[i][j][0], q[i][j][1]);
-                mma16816<T>(s[i], k0.z, k1.z, k0.w, k1.w, q[i][j][2], q[i][j][3]);
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 k0 = *reinterpret_cast<const uint4 *>(key + 64 * j), k1 = *reinterpret_cast<const uint4 *>(key + 8 * kKeys + 64 * j);
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    mma16816<T>(y.x[u][i], k0.x, k1.x, k0.y, k1.y, q[i][j][0], q[i][j][1]);
+                    mma16816<T>(y.x[u][i], k0.z, k1.z, k0.w, k1.w, q[i][j][2], q[i][j][3]);
+                }
             }
         }
     }
     // scores to weights; their pieces as operands
     // .. and to what is added: the weights' pieces times the values
     __device__ __forceinline__ void weigh_and_add(Scores &y, const char *tile, unsigned int mask, float scale2, int lane) {
-        float (&s)[kN][4] = y.x;
-        uint32_t hi[kN][2], lo[kN][2];
         const int g = lane / 4;
-        const bool there0 = mask >> g & 1, there1 = mask >> (g + 8) & 1;
         bool rise = false;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            s[i][0] = there0 ? s[i][0] * scale2 : -INFINITY;
-            s[i][1] = there0 ? s[i][1] * scale2 : -INFINITY;
-            s[i][2] = there1 ? s[i][2] * scale2 : -INFINITY;
-            s[i][3] = there1 ? s[i][3] * scale2 : -INFINITY;
-            rise |= fmaxf(s[i][0], s[i][2]) > m[i][0] + (kLift + kSlack) || fmaxf(s[i][1], s[i][3]) > m[i][1] + (kLift + kSlack);
+        for (int u = 0; u < kSub; ++u) {
+            const bool there0 = mask >> (16 * u + g) & 1, there1 = mask >> (16 * u + g + 8) & 1;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                float (&s)[4] = y.x[u][i];
+                s[0] = there0 ? s[0] * scale2 : -INFINITY;
+                s[1] = there0 ? s[1] * scale2 : -INFINITY;
+                s[2] = there1 ? s[2] * scale2 : -INFINITY;
+                s[3] = there1 ? s[3] * scale2 : -INFINITY;
+                rise |= fmaxf(s[0], s[2]) > m[i][0] + (kLift + kSlack) || fmaxf(s[1], s[3]) > m[i][1] + (kLift + kSlack);
+            }
         }
         if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(s[i][e], s[i][e + 2]);
+                    float x = fmaxf(y.x[0][i][e], y.x[0][i][e + 2]);
+                    if (kSub == 2) x = fmaxf(x, fmaxf(y.x[kSub - 1][i][e], y.x[kSub - 1][i][e + 2]));
 #pragma unroll
                     for (int o_ = 4; o_ < 32; o_ <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o_));
                     const float now = fmaxf(m[i][e], x - kLift), f = m[i][e] == now ? 1.f : ex2(m[i][e] - now);
@@ -291,35 +301,40 @@ struct Core16 {
             }
         }
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const float m0 = m[i][0] == -INFINITY ? 0.f : m[i][0], m1 = m[i][1] == -INFINITY ? 0.f : m[i][1];
-            const float p0 = ex2(s[i][0] - m0), p1 = ex2(s[i][1] - m1), p2 = ex2(s[i][2] - m0), p3 = ex2(s[i][3] - m1);
-            l[i][0] += p0 + p2;
-            l[i][1] += p1 + p3;
-            const uint32_t h0 = cut2<T>(p0, p1), h1 = cut2<T>(p2, p3);
-            const float2 r0 = unpack2<T>(h0), r1 = unpack2<T>(h1);
-            hi[i][0] = transpose8(h0);
-            hi[i][1] = transpose8(h1);
-            lo[i][0] = transpose8(cut2<T>(p0 - r0.x, p1 - r0.y) | 0x00010001u);
-            lo[i][1] = transpose8(cut2<T>(p2 - r1.x, p3 - r1.y) | 0x00010001u);
-        }
-        const char *value = tile + kTile * kKeys + 2 * (lane % 4) * kValues + 16 * g;
+        for (int u = 0; u < kSub; ++u) {
+            uint32_t hi[kN][2], lo[kN][2];
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            uint32_t x[4][4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(value + ((r & 1) + 8 * (r >> 1)) * kValues + 128 * c);
-                x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
+            for (int i = 0; i < kN; ++i) {
+                const float (&s)[4] = y.x[u][i];
+                const float m0 = m[i][0] == -INFINITY ? 0.f : m[i][0], m1 = m[i][1] == -INFINITY ? 0.f : m[i][1];
+                const float p0 = ex2(s[0] - m0), p1 = ex2(s[1] - m1), p2 = ex2(s[2] - m0), p3 = ex2(s[3] - m1);
+                l[i][0] += p0 + p2;
+                l[i][1] += p1 + p3;
+                const uint32_t h0 = cut2<T>(p0, p1), h1 = cut2<T>(p2, p3);
+                const float2 r0 = unpack2<T>(h0), r1 = unpack2<T>(h1);
+                hi[i][0] = transpose8(h0);
+                hi[i][1] = transpose8(h1);
+                lo[i][0] = transpose8(cut2<T>(p0 - r0.x, p1 - r0.y) | 0x00010001u);
+                lo[i][1] = transpose8(cut2<T>(p2 - r1.x, p3 - r1.y) | 0x00010001u);
             }
+            const char *value = tile + kTile * kKeys + (16 * u + 2 * (lane % 4)) * kValues + 16 * g;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t a0 = __byte_perm(x[0][e], x[1][e], 0x5410), a1 = __byte_perm(x[0][e], x[1][e], 0x7632);
-                const uint32_t a2 = __byte_perm(x[2][e], x[3][e], 0x5410), a3 = __byte_perm(x[2][e], x[3][e], 0x7632);
+            for (int c = 0; c < D / 64; ++c) {
+                uint32_t x[4][4];
 #pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, hi[i][0], hi[i][1]);
-                    mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, lo[i][0], lo[i][1]);
+                for (int r = 0; r < 4; ++r) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(value + ((r & 1) + 8 * (r >> 1)) * kValues + 128 * c);
+                    x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t a0 = __byte_perm(x[0][e], x[1][e], 0x5410), a1 = __byte_perm(x[0][e], x[1][e], 0x7632);
+                    const uint32_t a2 = __byte_perm(x[2][e], x[3][e], 0x5410), a3 = __byte_perm(x[2][e], x[3][e], 0x7632);
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) {
+                        mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, hi[i][0], hi[i][1]);
+                        mma16816<T>(o[i][4 * c + e], a0, a1, a2, a3, lo[i][0], lo[i][1]);
+                    }
                 }
             }
         }
@@ -531,6 +546,7 @@ __device__ __forceinline__ void run_tiles(Core &core, const Begin &begin, const 
             }
             if (wait.gave_up) return;
             phase ^= 1u << stage;
+            __syncwarp();  // zeros that other lanes have put in place of rows that are not there
             typename Core::Scores s;
             core.scores(s, tile, lane);
             core.weigh_and_add(s, tile, mask[0], a.scale2, lane);
@@ -653,10 +669,11 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
             long long begin;
             b = list.find(base + p, lane, begin);
             tiles = row_tiles<kTile>(a, b, bad);
-            places = unit_places(tiles, list.kLeast);
+            places = unit_places(tiles, a.pad);
             begin = base + p - begin;
-            unit = begin >> 31 ? (int)(begin / places) : (int)((uint32_t)begin / (uint32_t)places);
+            unit = places == 0 ? 0 : begin >> 31 ? (int)(begin / places) : (int)((uint32_t)begin / (uint32_t)places);
             off = (int)(begin - (long long)unit * places);
+            if ((unsigned int)unit >= (unsigned int)units || off < 0) tiles = 0;  // lengths that were changed meanwhile: nothing out of range is touched
         }
     }
     if (tiles) {
@@ -665,7 +682,7 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
             if (off < real) {
                 const int h = a.blocks == 1 ? unit : unit / a.blocks, r0 = (unit - h * a.blocks) * a.per_block, nq = min(a.per_block, a.group - r0), head = h * a.group + r0;
                 run_tiles(core, [&] { core.begin(a.q + b * a.qs[0] + head * a.qs[1], a.qs[1], nq, a.scale2, lane); }, a, wait, s_warps + warp * Core::kShared, s_bars[warp], phase, a.tables + b * a.ts, h, off, real,
-                          a.lens[b] + 1, lane);
+                          min(a.lens[b], (int)a.slots - 1) + 1, lane);
                 core.finish();
                 const bool all = off == 0 && real == tiles, last = p + (upto - off) >= end;  // the ring is free at the warp's end, and for as long as a whole unit is written
                 float *to = all || last ? late : early;
@@ -691,8 +708,9 @@ __global__ void __launch_bounds__(32 * Core::kWarps, 1) k_paged_attn(const __gri
             off = 0;
             if (++unit == units) {
                 unit = 0;
-                do ++b; while ((tiles = row_tiles<kTile>(a, b, bad)) == 0);  // there is one before the end
-                places = unit_places(tiles, TileList<kTile>::kLeast);
+                do tiles = ++b < a.batch ? row_tiles<kTile>(a, b, bad) : 0; while (tiles == 0 && b < a.batch);
+                if (tiles == 0) break;
+                places = unit_places(tiles, a.pad);
             }
         }
     }
@@ -806,6 +824,7 @@ p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStr
     const auto kernel = k_paged_attn<T, D, Core>;
     constexpr int smem = Core::kWarps * Core::kShared;
     if (!allow_shared(kernel, which, smem)) return P8_ERR_CUDA;
+    a.pad = attn_units(c, a.heads) <= a.ctas ? kSpan / Core::kTile : 1;  // where every unit can have a CTA, a short one does
     // shares that there can be; in a CTA's share, and in the workspace, places and rows are counted in 32 bits
     const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);
     if (most / a.ctas >= INT32_MAX / 32 || c->rows * a.heads >= INT32_MAX - 256) return P8_ERR_UNSUPPORTED;

@@ -65,9 +65,9 @@ def test_bits_and_orders(ix):
     assert keys == sorted(keys) and [ix.order_bits(k) for k in keys] == bits
 
 
-def walk(ix, units, tiles, ctas, least, warps):
+def walk(ix, units, tiles, ctas, least, warps, pad):
     """What the kernel's CTAs leave for `tiles` [sequences]: {unit: its tiles in pieces}, {part of the workspace: unit}, {unit: who notes its cut}"""
-    places = [ix.unit_places(t, least) for t in tiles]
+    places = [ix.unit_places(t, pad) for t in tiles]
     total = units * sum(places)
     share = ix.cta_share(total, ctas, least)
     start, at = {}, 0
@@ -124,7 +124,7 @@ def test_shares_cover_every_tile_once_and_the_join_finds_all_parts(ix, seed):
     ctas, least, warps = rng.choice([3, 7, 20, 44]), rng.choice([1, 2, 8, 12, 24]), rng.choice([4, 8, 10, 12])
     units, B = rng.choice([1, 2, 8]), rng.choice([1, 2, 5, 40])
     tiles = [rng.choice([0, 1, 2, rng.randint(0, 30), rng.randint(0, 400)]) for _ in range(B)]
-    start, share, total, covered, parts, cuts = walk(ix, units, tiles, ctas, least, warps)
+    start, share, total, covered, parts, cuts = walk(ix, units, tiles, ctas, least, warps, least if units * B <= ctas else 1)
     assert share * ctas >= total
     used = -(-total // share) if total else 0
     assert used <= units * sum(1 for _ in tiles) * max(1, -(-max(tiles) // least))  # the grid's bound
