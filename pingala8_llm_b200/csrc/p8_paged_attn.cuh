@@ -23,6 +23,7 @@ struct PagedAttnArgs {
     long long slots;
     PageDiv div;
     unsigned int wait_ns;
+    int side[2];  // whether rows that a copy can take at once lie side by side: of keys, of values
     int batch, heads, kvh, group, blocks, per_block, pages, ctas, pad;  // group: query heads of a cache head, in so many blocks of at most per_block
     float scale2;                                       // scale / ln 2: the kernel's exponentials are powers of two
 };
@@ -162,11 +163,15 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
-// A tile's rows, one a lane: the keys of its slots in the first kTile lanes, the values in the next (of 32 slots: both in one). The rows lie kKeyStride and
-// kValueStride bytes apart in shared memory.
-template <int kTile, int kRowBytes, int kKeyStride, int kValueStride>
+// A tile's rows, one a lane: the keys of its slots in the first kTile lanes, the values in the next (of 32 slots: both in one). In shared
+// memory there is a gap of kKeyGap bytes behind every kKeyRows keys, and likewise for the values; so many rows come in one copy where they lie side by side in one
+// page (single rows take a copy engine some 11 cycles each: 128-byte ones 3.2 TB/s of the whole GPU, 256-byte ones 5.7).
+template <int kTile, int kRowBytes, int kKeyRows, int kKeyGap, int kValueRows, int kValueGap>
 struct Tiles {
-    static constexpr int kBytes = kTile * (kKeyStride + kValueStride);
+    static constexpr int kValueBase = kTile * kRowBytes + kTile / kKeyRows * kKeyGap, kBytes = kValueBase + kTile * kRowBytes + kTile / kValueRows * kValueGap;
+    static constexpr int kRowsOf[2] = {kKeyRows, kValueRows};
+    static __device__ __forceinline__ int key_at(int slot) { return slot * kRowBytes + slot / kKeyRows * kKeyGap; }
+    static __device__ __forceinline__ int value_at(int slot) { return kValueBase + slot * kRowBytes + slot / kValueRows * kValueGap; }
     int id;           // the page; -1 behind the sequence's end
     unsigned int in;  // the slot's place in it
     __device__ __forceinline__ void look(const PagedAttnArgs &a, const int *table, int tile, int n, int lane) {
@@ -189,8 +194,8 @@ struct Tiles {
         constexpr int kBoth = kTile == 32 ? 2 : 1;  // rows of a lane
 #pragma unroll
         for (int i = 0; i < kBoth; ++i) {
-            const int z = kBoth == 2 ? i : lane / kTile;
-            char *row = to + (z ? kTile * kKeyStride + lane % kTile * kValueStride : lane * kKeyStride);
+            const int z = kBoth == 2 ? i : lane / kTile, r = lane % kTile;
+            char *row = to + (z ? value_at(r) : key_at(r));
             if (z == 1 && !there) {
 #pragma unroll 1
                 for (int j = 0; j < kRowBytes; j += 16) *reinterpret_cast<uint4 *>(row + j) = make_uint4(0, 0, 0, 0);
@@ -198,10 +203,15 @@ struct Tiles {
             }
             if (i == 0) __syncwarp();
             if (z < 2 && there) {
-                const char *from = a.kv[z] + h * a.st[z][1] + id * a.st[z][0] + in * a.st[z][2];
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"((unsigned int)__cvta_generic_to_shared(row)), "l"(from), "r"(kRowBytes),
-                             "r"((unsigned int)__cvta_generic_to_shared(bar))
-                             : "memory");
+                const int rows = z ? kValueRows : kKeyRows;
+                const unsigned int these = (~0u >> (32 - rows)) << (r - r % rows);
+                const bool all = a.side[z] && (mask & these) == these;
+                if (!all || r % rows == 0) {
+                    const char *from = a.kv[z] + h * a.st[z][1] + id * a.st[z][0] + in * a.st[z][2];
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"((unsigned int)__cvta_generic_to_shared(row)), "l"(from),
+                                 "r"(all ? rows * kRowBytes : kRowBytes), "r"((unsigned int)__cvta_generic_to_shared(bar))
+                                 : "memory");
+                }
             }
         }
         return mask;
@@ -220,8 +230,7 @@ struct Tiles {
 template <typename T, int D, int kN>
 struct Core16 {
     static constexpr int kSub = D == 64 ? 2 : 1, kTile = 16 * kSub, kRows = 8 * kN;  // sixteen slots make a product; shorter rows come in tiles of as many bytes
-    static constexpr int kKeys = D == 64 ? 128 : 2 * D + 64, kValues = 2 * D + 16;  // rows so far apart that eight lanes' 16 bytes are in different banks (keys of 64: two in each)
-    using Tile = Tiles<kTile, 2 * D, kKeys, kValues>;
+    using Tile = Tiles<kTile, 2 * D, 4, 64, 2, 32>;
     static constexpr int kDepth = kN == 2 ? 3 : 2, kWarps = kN == 1 ? 12 : 8, kShared = kDepth * Tile::kBytes;  // of a warp
     static constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = 8.f;
     uint32_t q[kN][D / 32][4];
@@ -244,16 +253,19 @@ struct Core16 {
             l[i][0] = l[i][1] = 0.f;
         }
     }
+    // The slot of a product's i-th row (of eight). With these, and the gaps between rows, the eight lanes that are served together find their 16 bytes in different
+    // banks: keys i = 2j and 2j + 1 are in different fours, values i = 0, 2, 4, 6 (and 1, 3, 5, 7) in different twos.
+    static __device__ __forceinline__ int slot_of(int i) { return 0x37156240 >> (4 * i) & 7; }
     struct Scores { float x[kSub][kN][4]; };
     __device__ __forceinline__ void scores(Scores &y, const char *tile, int lane) const {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const char *key = tile + (16 * u + lane / 4) * kKeys + 16 * (lane % 4);
+            const char *key = tile + Tile::key_at(16 * u + slot_of(lane / 4)) + 16 * (lane % 4);
 #pragma unroll
             for (int i = 0; i < kN; ++i) y.x[u][i][0] = y.x[u][i][1] = y.x[u][i][2] = y.x[u][i][3] = 0.f;
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
-                const uint4 k0 = *reinterpret_cast<const uint4 *>(key + 64 * j), k1 = *reinterpret_cast<const uint4 *>(key + 8 * kKeys + 64 * j);
+                const uint4 k0 = *reinterpret_cast<const uint4 *>(key + 64 * j), k1 = *reinterpret_cast<const uint4 *>(key + Tile::key_at(8) + 64 * j);
 #pragma unroll
                 for (int i = 0; i < kN; ++i) {
                     mma16816<T>(y.x[u][i], k0.x, k1.x, k0.y, k1.y, q[i][j][0], q[i][j][1]);
@@ -269,7 +281,7 @@ struct Core16 {
         bool rise = false;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const bool there0 = mask >> (16 * u + g) & 1, there1 = mask >> (16 * u + g + 8) & 1;
+            const bool there0 = mask >> (16 * u + slot_of(g)) & 1, there1 = mask >> (16 * u + slot_of(g) + 8) & 1;
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 float (&s)[4] = y.x[u][i];
@@ -317,13 +329,15 @@ struct Core16 {
                 lo[i][0] = transpose8(cut2<T>(p0 - r0.x, p1 - r0.y) | 0x00010001u);
                 lo[i][1] = transpose8(cut2<T>(p2 - r1.x, p3 - r1.y) | 0x00010001u);
             }
-            const char *value = tile + kTile * kKeys + (16 * u + 2 * (lane % 4)) * kValues + 16 * g;
+            const char *value[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) value[r] = tile + Tile::value_at(16 * u + slot_of(2 * (lane % 4) + r)) + 16 * g;
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) {
                 uint32_t x[4][4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(value + ((r & 1) + 8 * (r >> 1)) * kValues + 128 * c);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(value[r & 1] + (r >> 1) * (Tile::value_at(8) - Tile::value_at(0)) + 128 * c);
                     x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
                 }
 #pragma unroll
@@ -382,7 +396,7 @@ struct Core32 {
     static constexpr int kTile = 8, kRows = kN;
     static constexpr int kR = kN == 8 ? 2 : 1;  // scores of a lane
     static constexpr int kV = D == 128 ? 8 : 4;  // values' rows of a lane
-    using Tile = Tiles<kTile, 4 * D, 4 * D, 4 * D>;
+    using Tile = Tiles<kTile, 4 * D, 8, 0, 8, 0>;
     static constexpr int kDepth = D == 64 ? 4 : 2, kWarps = kN == 8 ? 10 : 12, kShared = kDepth * Tile::kBytes + 4 * kN * (D + 8);
     static constexpr float kSlack = 8.f;
     float *sq, *sp;  // this warp's queries [kN][D] and weights [8][kN]
@@ -824,6 +838,8 @@ p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStr
     const auto kernel = k_paged_attn<T, D, Core>;
     constexpr int smem = Core::kWarps * Core::kShared;
     if (!allow_shared(kernel, which, smem)) return P8_ERR_CUDA;
+    const int64_t *const strides[2] = {c->k_stride, c->v_stride};
+    for (int z = 0; z < 2; ++z) a.side[z] = (c->page == 1 || strides[z][3] == D) && c->page % Core::Tile::kRowsOf[z] == 0;
     a.pad = attn_units(c, a.heads) <= a.ctas ? kSpan / Core::kTile : 1;  // where every unit can have a CTA, a short one does
     // shares that there can be; in a CTA's share, and in the workspace, places and rows are counted in 32 bits
     const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);
