@@ -393,8 +393,8 @@ typedef struct p8_attn_mass_args {
 } p8_attn_mass_args;
 p8_status p8_attn_mass(const p8_kv *c, const p8_attn_mass_args *a, void *stream);
 
-/* The tree attention and mass kernels are pipelines of warps that wait for one another. A wait that is not over after `ns`
- * nanoseconds gives up: the call ends, once the copies and products that it has started are done, its results are invalid,
+/* The tree attention and mass kernels are pipelines of warps that wait for one another, and p8_paged_attn's warps wait for their
+ * copies. A wait that is not over after `ns` nanoseconds gives up: the call ends, once the copies and products that it has started are done, its results are invalid,
  * and p8_device_error reports bit 7 (128). Two seconds unless set here, for the calls made (or captured) from then on by
  * this process; at most 2^32 - 1. 0: every wait that is not over at its first look gives up, which is how a program's way of
  * dealing with the error can be tried out. */
@@ -554,8 +554,8 @@ p8_status p8_gguf_load_linear(p8_gguf *g, int64_t i, uint8_t *out, size_t out_ca
 
 /* Non-zero if a kernel since the last call gave up (that launch's results are invalid), then clears the word. Bits:
  * 4 GEMM pipeline wait timed out, 8 row-parallel exchange wait timed out, 16 exchange entry with a foreign tag, 64 a
- * cache operator met a length, count, position, row, page or parent out of range and left it out, 128 a tree attention or mass
- * pipeline wait timed out (1, 2 and 32 are unused). Waits for all streams of the current device. */
+ * cache operator met a length, count, position, row, page or parent out of range and left it out, 128 a tree attention, mass
+ * or paged attention wait timed out (1, 2 and 32 are unused). Waits for all streams of the current device. */
 int p8_device_error(void);
 
 const char *p8_status_str(p8_status s);

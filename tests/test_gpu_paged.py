@@ -709,3 +709,90 @@ def test_a_step_in_a_graph_and_two_graphs_with_one_workspace():
         for name in ("tables", "lens", "scores", "tokens", "parents"):
             assert torch.equal(s[name], eager[name]), name
         assert torch.equal(s["k"], eager["k"]) and torch.equal(s["v"], eager["v"])
+
+
+# ------------------------------------------------------------------------------------------------ calls at the edges
+def test_4096_sequences_some_without_a_token():
+    g, B, H, kv, D, P = gen(50), 4096, 4, 2, 64, 16
+    lens_ = [(7 * i) % 90 for i in range(B)]
+    pages = sum(n // P + 1 for n in lens_) + 1
+    kp, vp = make_pages(g, pages, kv, P, D, torch.float16)
+    tables, lens = make_tables(g, lens_, 1, P, pages), ints(*lens_)
+    counts = (torch.arange(B, device="cuda") % 5 != 3).int()
+    q = randn(g, B, H, D, dtype=torch.float16)
+    cos, sin = paged.rotary_tables(100, D, device="cuda")
+    x = randn(g, B, 1, H + 2 * kv, D)
+    before = kp.clone()
+    paged.paged_append(x[:, :, :H], x[:, :, H:H + kv], x[:, :, H + kv:], kp, vp, tables, lens, lens[:, None].contiguous(), cos, sin, counts=counts)
+    at = tables.gather(1, (lens // P).long()[:, None])[:, 0].long()
+    wrote = (kp[at, :, (lens % P).long()] != before[at, :, (lens % P).long()]).flatten(1).any(1)
+    assert torch.equal(wrote, counts.bool())
+    out, lse = torch.full_like(q, 7.0), torch.full((B, H), 7.0, device="cuda")
+    paged.paged_attention(q, kp, vp, tables, lens, counts=counts, out=out, lse=lse)
+    ended()
+    skipped = counts == 0
+    assert (out[skipped] == 7).all() and (lse[skipped] == 7).all()
+    some = torch.arange(0, B, 37, device="cuda")
+    want = attend(q[some], kp, vp, tables[some], lens[some], counts[some], D ** -0.5)
+    live = counts[some] == 1
+    close(out[some][live], want[0][live], want[2][live])
+    close(lse[some][live], want[1][live], want[3][live])
+    none, l0 = torch.full_like(q, 7.0), torch.full((B, H), 7.0, device="cuda")
+    paged.paged_attention(q, kp, vp, tables, lens, counts=torch.zeros_like(counts), out=none, lse=l0)
+    ended()
+    assert (none == 7).all() and (l0 == 7).all()
+
+
+def test_calls_on_two_streams_at_once():
+    g, D, P = gen(51), 128, 16
+    kp, vp = make_pages(g, 700, 8, P, D, torch.bfloat16)
+    sets = []
+    for i in range(2):
+        lens_ = [3000 - 500 * i, 17, 800]
+        tables = make_tables(g, lens_, 1, P, 700)
+        sets.append((randn(g, 3, 32, D, dtype=torch.bfloat16), tables, ints(*lens_), randn(g, 2, 4, 30011), -torch.rand(2, 4, device="cuda", generator=g)))
+    one = [(paged.paged_attention(q, kp, vp, t, n), paged.beam_select(x, s)) for q, t, n, x, s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i, (q, t, n, x, s) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((paged.paged_attention(q, kp, vp, t, n), paged.beam_select(x, s)))
+    ended()
+    for i in range(2):
+        for (a, l), best in got[i]:
+            assert torch.equal(a, one[i][0][0]) and torch.equal(l, one[i][0][1]) and all(torch.equal(x, y) for x, y in zip(best, one[i][1]))
+
+
+def test_a_sequence_over_the_pages_of_another_and_one_page_twice():
+    """the same page in several places of a table, and under several sequences"""
+    g, D, P = gen(52), 64, 8
+    kp, vp = make_pages(g, 4, 2, P, D, torch.float32)
+    tables, lens, q = ints(1, 1, 1, 3, 1, 0).view(2, 3), ints(23, 20), randn(g, 2, 2, D)
+    want = attend(q, kp, vp, tables, lens, None, D ** -0.5)
+    out, lse = paged.paged_attention(q, kp, vp, tables, lens)
+    ended()
+    close(out, want[0], want[2])
+    close(lse, want[1], want[3])
+
+
+def test_select_of_equal_beams_of_an_odd_vocabulary():
+    """two beams that are one another's copy tie in every continuation, wherever their rows begin in memory"""
+    g = gen(53)
+    for name in TYPES:
+        row = randn(g, 1, 1, 20011, dtype=TYPES[name])
+        logits, scores = row.expand(3, 4, 20011).contiguous(), torch.full((3, 4), -2.5, device="cuda")
+        for n in (4, 20):
+            check_select(paged.beam_select(logits, scores, candidates=n), select_ref(logits, scores, None, None, n), 20011)
+    ended()
+
+
+def test_select_of_the_largest_groups():
+    g, W, V = gen(54), 64, 9001
+    logits, scores = randn(g, 2, W, V, dtype=torch.float16, scale=0.1), -torch.rand(2, W, device="cuda", generator=g) * 0.01
+    check_select(paged.beam_select(logits, scores, candidates=64), select_ref(logits, scores, None, None, 64), V)
+    flat = torch.zeros(1, W, V, device="cuda")
+    check_select(paged.beam_select(flat, torch.zeros(1, W, device="cuda"), candidates=64), select_ref(flat, torch.zeros(1, W), None, None, 64), V)
+    done = torch.ones(2, W, dtype=torch.bool, device="cuda")
+    check_select(paged.beam_select(logits, scores, done=done, end=5, candidates=64), select_ref(logits, scores, done, 5, 64), V)
+    ended()
