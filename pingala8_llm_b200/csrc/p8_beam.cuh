@@ -19,7 +19,7 @@ struct SelectArgs {
     unsigned long long *best;  // [rows][splits][n], the best first, 0 behind them
     float2 *sums;              // [rows][splits]: the largest logit m, the sum of exp(x - m)
     long long end;
-    int batch, beams, vocab, n, splits, chunk, deep, wide;  // deep, wide: that many entries of that many lists are n or more
+    int batch, beams, vocab, n, splits, chunk, deep, wide, fold;  // deep, wide: that many entries of that many lists are n or more; fold: so many lists are looked at as one for it
     PageDiv by_splits, by_beam;  // division by the pieces of a row, by the entries of a beam
     int one_row;               // all beams of a group have the same logits: they are read once
     __host__ __device__ int rows() const { return one_row ? batch : batch * beams; }
@@ -206,12 +206,13 @@ __global__ void __launch_bounds__(256, kScanBlocks) k_beam_scan(const __grid_con
     constexpr int kE = R::kE;  // (of a lane, in a round)
     extern __shared__ __align__(16) uint4 s_ring[];
     __shared__ unsigned long long s_list[8][kListSize];
+    __shared__ __align__(16) unsigned long long s_pick[256];
     // logits below s_bar, as order_key, and continuations below s_last are not among the best; 0: not known yet
     __shared__ unsigned long long s_last;
     __shared__ uint32_t s_bar, s_first;
     __shared__ __align__(16) uint32_t s_top[128];
     __shared__ float s_m[8], s_s[8];
-    __shared__ int s_count[8];
+    __shared__ int s_total, s_count[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     after_prior();
     const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits, b = a.one_row ? row : row / a.beams, w = a.one_row ? 0 : row - b * a.beams;
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(256, kScanBlocks) k_beam_scan(const __grid_con
     const auto goes_on = [&](int i) { return i < a.beams && !(a.done && a.done[b * a.beams + i]) && isfinite(a.scores[b * a.beams + i]); };
     if (a.one_row ? !__any_sync(0xffffffffu, goes_on(lane) || goes_on(lane + 32)) : !goes_on(w)) return;  // the whole block
     R logits(x0, s_ring, begin, end);
-    if (threadIdx.x == 0) { s_bar = s_first = 0; s_last = 0; }
+    if (threadIdx.x == 0) { s_bar = s_first = 0; s_last = 0; s_total = 0; }
     __syncthreads();
     unsigned long long *list = s_list[warp];
     int count = 0;
@@ -380,15 +381,22 @@ __global__ void __launch_bounds__(256, kScanBlocks) k_beam_scan(const __grid_con
         }
         if (kVec) logits.ask(r + R::kDepth, stage);
     }
-    // This block's sum, and its best: what the warps' lists have is counted out against one another.
+    // This block's sum, and its best: what the warps' lists have goes to one place, in any order, and is counted out against one another.
+    const auto gather = [&] {
+        int to = 0;
+        if (lane == 0) to = atomicAdd(&s_total, count);
+        to = __shfl_sync(0xffffffffu, to, 0);
+        __syncwarp();
+        for (int i = lane; i < count; i += 32)
+            if (to + i < 256) s_pick[to + i] = list[i];
+    };
+    gather();
     if (sum == 0.f) m = -INFINITY;
-    float peak = m;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+    const float peak = __uint_as_float(order_bits(__reduce_max_sync(0xffffffffu, order_key(__float_as_uint(m + 0.0f)))));
     sum = m == peak ? sum : sum * ex2((m - peak) * kLog2e);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) { s_m[warp] = peak; s_s[warp] = sum; s_count[warp] = count; }
+    if (lane == 0) { s_m[warp] = peak; s_s[warp] = sum; }
     __syncthreads();
     const long long piece = (long long)row * a.splits + split;
     if (threadIdx.x == 0) {
@@ -397,10 +405,10 @@ __global__ void __launch_bounds__(256, kScanBlocks) k_beam_scan(const __grid_con
         for (int o = 0; o < 8; ++o) S += s_m[o] == M ? s_s[o] : s_s[o] * ex2((s_m[o] - M) * kLog2e);
         a.sums[piece] = make_float2(M, S);
     }
-    int have = 0;
-    for (int o = 0; o < 8; ++o) have += s_count[o];
+    int have = s_total;
     if (have > 128 + a.n) {  // a last look at the bar leaves some 1.2 n
         raise_all();
+        if (threadIdx.x == 0) s_total = 0;
         const uint32_t high = s_bar;
         int kept = 0;
         for (int i0 = 0; i0 < count; i0 += 32) {
@@ -411,20 +419,17 @@ __global__ void __launch_bounds__(256, kScanBlocks) k_beam_scan(const __grid_con
             __syncwarp();
         }
         count = kept;
-        if (lane == 0) s_count[warp] = count;
         __syncthreads();
-        have = 0;
-        for (int o = 0; o < 8; ++o) have += s_count[o];
+        gather();
+        __syncthreads();
+        have = s_total;
     }
     if (have <= 256) {
-        for (int i = lane; i < count; i += 32) {
-            const unsigned long long c = list[i];
+        if (threadIdx.x < have) {
+            const unsigned long long c = s_pick[threadIdx.x];
             int rank = 0;
-            for (int o = 0; o < 8; ++o) {
-                const int upto = s_count[o];
 #pragma unroll 4
-                for (int j = 0; j < upto; ++j) rank += s_list[o][j] > c;
-            }
+            for (int o = 0; o < have; ++o) rank += s_pick[o] > c;
             if (rank < a.n) a.best[piece * a.n + rank] = c;
         }
     } else {  // (the logits come in rising order, or nearly so): by the lists' own orders
@@ -466,8 +471,8 @@ constexpr int kMaxLists = 256, kPicked = 1024, kEarly = 4;
 __global__ void __launch_bounds__(256) k_beam_join(const __grid_constant__ SelectArgs a) {
     __shared__ double s_shift[P8_BEAMS_MAX];  // score - log sum
     __shared__ int s_kind[P8_BEAMS_MAX];      // 0: no continuation, 1: from its logits, 2: ended
-    __shared__ __align__(16) uint32_t s_head[kMaxLists];
-    __shared__ unsigned long long s_total[kPicked], s_which[kPicked];
+    __shared__ __align__(16) uint32_t s_head[kMaxLists + 4];
+    __shared__ __align__(16) ulonglong2 s_picked[kPicked];  // total, beam and token
     __shared__ int s_count;
     __shared__ uint32_t s_bar;
     after_prior();
@@ -520,27 +525,37 @@ __global__ void __launch_bounds__(256) k_beam_join(const __grid_constant__ Selec
     } else if (kind == 2 && l == mine * a.splits && a.deep == 1) {
         head = (uint32_t)(total_key(s_shift[mine]) >> 32);
     }
-    s_head[l] = head;
-    __syncthreads();
-    if (l < lists && head) {
-        int above = 0, same = 0;
-        const uint4 *h4 = reinterpret_cast<const uint4 *>(s_head);
+    // Of many lists, the best of two or four side by side: as many of those that are high enough are as many lists. (All on their own where
+    // that leaves too few, as of a first step, where one beam is all there is.)
+    const uint32_t alone = head;
+    for (int fold = a.fold;; fold = 1) {
+        head = alone;
+        if (fold >= 2) head = max(head, __shfl_xor_sync(0xffffffffu, head, 1));
+        if (fold == 4) head = max(head, __shfl_xor_sync(0xffffffffu, head, 2));
+        const int shift = fold == 4 ? 2 : fold == 2 ? 1 : 0, heads = (lists + fold - 1) >> shift;
+        if (threadIdx.x < 4) s_head[heads + threadIdx.x] = 0;  // (read together with the last ones)
+        if (l < lists) s_head[l >> shift] = head;
+        __syncthreads();
+        if (l < lists && head) {
+            int above = 0, same = 0;
+            const uint4 *h4 = reinterpret_cast<const uint4 *>(s_head);
 #pragma unroll 4
-        for (int o = 0; o < (lists + 3) / 4; ++o) {
-            const uint4 y = h4[o];
-            above += (y.x > head) + (y.y > head) + (y.z > head) + (y.w > head);
-            same += (y.x == head) + (y.y == head) + (y.z == head) + (y.w == head);
+            for (int o = 0; o < (heads + 3) / 4; ++o) {
+                const uint4 y = h4[o];
+                above += (y.x > head) + (y.y > head) + (y.z > head) + (y.w > head);
+                same += (y.x == head) + (y.y == head) + (y.z == head) + (y.w == head);
+            }
+            if (above < a.wide && a.wide <= above + same) s_bar = head;  // (all that write, write the same)
         }
-        if (above < a.wide && a.wide <= above + same) s_bar = head;  // (all that write, write the same)
+        __syncthreads();
+        if (s_bar || fold == 1) break;
     }
-    __syncthreads();
     const uint32_t bar = s_bar;
     // What reaches the bar goes to one list; whenever that could overflow, and at the end, it is cut to its n best, in order.
     const auto take = [&](unsigned long long key, unsigned long long which) {
         if ((uint32_t)(key >> 32) < bar) return false;
         const int k = atomicAdd(&s_count, 1);
-        s_total[k] = key;
-        s_which[k] = which;
+        s_picked[k] = make_ulonglong2(key, which);
         return true;
     };
     const auto entry = [&](int w, unsigned long long c) { return c && take(total_of(w, c), (unsigned long long)w << 32 | (0xffffffffu - (unsigned int)c)); };
@@ -559,29 +574,28 @@ __global__ void __launch_bounds__(256) k_beam_join(const __grid_constant__ Selec
         int have = s_count;
         if (have > kPicked / 2 || !go_on) {
             // entry k goes to the place that is the number of entries before it
-            unsigned long long key[kPicked / 256], which[kPicked / 256];
+            ulonglong2 mine_[kPicked / 256];
             int rank[kPicked / 256];
 #pragma unroll
             for (int j = 0; j < kPicked / 256; ++j) {
                 const int k = threadIdx.x + 256 * j;
                 rank[j] = INT_MAX;
                 if (k < have) {
-                    key[j] = s_total[k];
-                    which[j] = s_which[k];
+                    const ulonglong2 x = s_picked[k];
                     int r = 0;
 #pragma unroll 4
                     for (int o = 0; o < have; ++o) {
-                        const unsigned long long y = s_total[o];
-                        r += y > key[j];
-                        if (y == key[j]) r += s_which[o] < which[j];
+                        const ulonglong2 y = s_picked[o];
+                        r += (y.x > x.x) | ((y.x == x.x) & (y.y < x.y));
                     }
+                    mine_[j] = x;
                     rank[j] = r;
                 }
             }
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < kPicked / 256; ++j)
-                if (rank[j] < a.n) { s_total[rank[j]] = key[j]; s_which[rank[j]] = which[j]; }
+                if (rank[j] < a.n) s_picked[rank[j]] = mine_[j];
             have = min(have, a.n);
             if (threadIdx.x == 0) s_count = have;
             __syncthreads();
@@ -605,10 +619,10 @@ __global__ void __launch_bounds__(256) k_beam_join(const __grid_constant__ Selec
         long long token = -1;
         bool ended = false;
         if (there) {
-            const unsigned long long u = s_total[i];
+            const unsigned long long u = s_picked[i].x, which = s_picked[i].y;
             score = (float)__longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u));
-            parent = (int)(s_which[i] >> 32);
-            token = (long long)(s_which[i] & 0xffffffffu);
+            parent = (int)(which >> 32);
+            token = (long long)(which & 0xffffffffu);
             ended = s_kind[parent] == 2 || token == a.end;
         }
         a.out_scores[at] = score;
@@ -641,6 +655,7 @@ p8_status launch_beam_select(const p8_beam_select_args *x, void *workspace, cuda
     const int lists = a.beams * a.splits;
     a.deep = std::min(a.n, (2 * a.n + lists - 1) / lists);
     a.wide = (a.n + a.deep - 1) / a.deep;
+    a.fold = lists >= 8 * a.wide ? 4 : lists >= 4 * a.wide ? 2 : 1;
     a.by_splits = page_div((uint32_t)a.splits);
     a.by_beam = page_div((uint32_t)(a.splits * a.n));
     a.chunk = (int)(((x->vocab + a.splits - 1) / a.splits + 127) / 128 * 128);
