@@ -4,10 +4,16 @@
 // is read once, 4 to 16 operations are done on it, so the memory bounds it (and latency, where there is little to read). The tiles of all
 // sequences and heads form one list, of which every CTA (one an SM) gets an equal contiguous share and every warp of it an equal part:
 // the warps finish together whatever the lengths are. A warp works on its own, with tiles of its own on their way into shared memory:
-// each lane starts the bulk copy of one row, a key or a value, from wherever its page is, and a barrier in shared memory counts
-// the tile's bytes. So 190 KB are in flight on every SM, at one instruction a tile. Each warp keeps the running maximum m, the sum l of 2^(s - m) and
-// the sum of 2^(s - m) v. Where a sequence's head is spread over several warps, their sums meet in shared memory at the end of
-// the CTA, and those of several CTAs in a second launch.
+// each lane starts the bulk copy of one row (or of some that lie side by side), keys or values, from wherever its page is, and a
+// barrier in shared memory counts the tile's bytes. So 190 KB are in flight on every SM, at one instruction a tile. (Loads into registers,
+// three CTAs of four warps, reached 5.3 TB/s: a tile can be asked for only as registers come free; cp.async of 16 bytes 4.2: they and
+// the reads of shared memory stand in one queue.) Each warp keeps the running maximum m, the sum l of 2^(s - m) and the sum of
+// 2^(s - m) v. Where a sequence's head is spread over several warps, their sums meet in shared memory at the end of the CTA, and those of
+// several CTAs in a second launch.
+//
+// Measured (32 query heads over 8 of 128): one sequence of 130 slots 6.0 us, of which the launch is 0.8 and the rest one chain of
+// latencies; four of 2,048 slots in 32 bits 21 us (67 MB: 10.6 of memory, 6 of beginning and end, 3.5 of the second launch); 64 ragged sequences,
+// 1.14 GB, 198 us, 5.8 TB/s; 131,001 slots, 537 MB, 93 us, 5.8 TB/s, where a plain sum over as many bytes takes 92.
 
 struct PagedAttnArgs {
     const char *q;
@@ -125,12 +131,6 @@ struct TileList {
     }
 };
 
-// 16 bytes of the cache, which no one reads again
-__device__ __forceinline__ uint4 ld_once(const char *p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ float ex2(float x) {  // 0 below 2^-126, which is nothing beside the sums here: the largest term of each is 1 or more
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -226,7 +226,8 @@ struct Tiles {
 // type, so that their rounding (2^-14 bf16, 2^-20 fp16) is nothing to that of the result; fp16 has them lifted by 2^7, so
 // that those 2^-31 of the largest still count. The pieces are cut, not rounded, and the second one's last bit is set: neither is negative
 // or nothing, so that an infinite value that is seen comes out as itself. The maximum only moves where a score is 2^8 above it: one vote a tile in place of
-// a reduction and a rescaling.
+// a reduction and a rescaling. The products take no time that shows: one head or eight on each cache head, 51 us for 262 MB; twelve, with
+// two columns of products, 57.
 template <typename T, int D, int kN>
 struct Core16 {
     static constexpr int kSub = D == 64 ? 2 : 1, kTile = 16 * kSub, kRows = 8 * kN;  // sixteen slots make a product; shorter rows come in tiles of as many bytes
@@ -274,8 +275,7 @@ struct Core16 {
             }
         }
     }
-    // scores to weights; their pieces as operands
-    // .. and to what is added: the weights' pieces times the values
+    // scores to weights, and to what is added: the weights' pieces times the values
     __device__ __forceinline__ void weigh_and_add(Scores &y, const char *tile, unsigned int mask, float scale2, int lane) {
         const int g = lane / 4;
         bool rise = false;
@@ -388,7 +388,7 @@ struct Core16 {
 
 // ----------------------------------------------------------------------------------------------------------------
 // 32-bit type: plain multiplications and additions, which the CUDA cores do fast enough for up to eight query heads on each byte
-// (one instruction for a key's element and head), with the rounding, infinities and NaN of 32 bits. Tiles of 8 slots. Scores: eight
+// (one instruction for a key's element and head; eight heads 60 us for 262 MB, four 52), with the rounding, infinities and NaN of 32 bits. Tiles of 8 slots. Scores: eight
 // lanes a key, 16 bytes of it each at a time; their sums for all heads are added up and spread over the eight lanes in one pass
 // (lane j of them ends up with head j). Values: a lane has four columns of all slots; the weights come from shared memory.
 template <int D, int kN>
