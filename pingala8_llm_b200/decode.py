@@ -388,13 +388,13 @@ class BeamDecoder:
         self.k, self.v = (torch.zeros(model.nl, pages, c.kv_heads, page, c.head_dim, dtype=dtype, device=dev) for _ in range(2))
         self._shared, self._own = shared, own
         self.cos, self.sin = rope_tables(c, max_prompt + max_new, dev) if rotary is None else paged.rotary_tables(max_prompt + max_new, c.head_dim, c.rope_theta, device=dev, **rotary)
-        self.tables = torch.zeros(rows, self.columns, dtype=torch.int32, device=dev)
+        self.tables = torch.full((rows, self.columns), -1, dtype=torch.int32, device=dev)  # -1: no page
         self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.scores = torch.zeros(batch, beams, device=dev)
         self.done = None if end is None else torch.zeros(batch, beams, dtype=torch.bool, device=dev)
         self.tokens = torch.zeros(batch, beams, dtype=torch.int64, device=dev)
-        self.said, self.came_from = (torch.zeros(max_new, batch, beams, dtype=torch.int64, device=dev) for _ in range(2))
-        self.at = torch.zeros(1, dtype=torch.int64, device=dev)  # how many tokens every beam has
+        self.said, self.came_from = (torch.zeros(max_new + 1, batch, beams, dtype=torch.int64, device=dev) for _ in range(2))
+        self.at = torch.zeros(1, dtype=torch.int64, device=dev)  # how many tokens every beam has; a step too many writes a row that nothing reads
 
     def _layers(self, x, attend):
         """the layers over x [n, hidden]; attend(layer index, q, k, v) -> [n, heads * head_dim]"""
@@ -422,7 +422,7 @@ class BeamDecoder:
         self.tokens.copy_(best.tokens)
         self.said.index_copy_(0, self.at, best.tokens[None])
         self.came_from.index_copy_(0, self.at, best.parents[None].long())
-        self.at += 1
+        self.at.add_(1).clamp_(max=self.max_new)
         self._paged.beam_reorder(best.parents, self.k, self.v, self.tables, self.lens)
 
     def prefill(self, prompts):
@@ -432,7 +432,7 @@ class BeamDecoder:
             raise ValueError(f"{self.batch} prompts of 1 to {self.max_prompt} tokens")
         lens = [p.numel() for p in prompts]
         first = self.batch * self._shared  # pages from here on belong to one beam each
-        tables = torch.zeros(self.batch * W, self.columns, dtype=torch.int32)
+        tables = torch.full((self.batch * W, self.columns), -1, dtype=torch.int32)
         for b, n in enumerate(lens):
             full = n // P
             tables[b * W:(b + 1) * W, :full] = torch.arange(b * self._shared, b * self._shared + full, dtype=torch.int32)
@@ -463,7 +463,7 @@ class BeamDecoder:
         self._choose(self.logits)
 
     def step(self):
-        """one token for every beam; graph-capturable"""
+        """one token for every beam; graph-capturable. Steps beyond max_new find no room in the cache: device_error() has bit 64 then."""
         rows = self.batch * self.beams
         pos = self.lens[:, None].contiguous()
         tokens = self.tokens.view(-1).clamp(min=0)  # (-1: a beam that is not there)
@@ -491,6 +491,8 @@ class BeamDecoder:
 
     def history(self, n):
         """the beams' tokens so far, int64 [batch, beams, n], the best beam first; -1 where a beam is not there"""
+        if not 1 <= n <= self.max_new:
+            raise ValueError(f"1 to {self.max_new} tokens")
         beam = torch.arange(self.beams, device=self.said.device).expand(self.batch, -1)
         out = []
         for i in range(n - 1, -1, -1):

@@ -125,3 +125,24 @@ def test_stretched_positions(model_and_ref):
     a, b = d.generate(prompts_of(20), 4), plain.generate(prompts_of(20), 4)
     assert not torch.equal(a[1], b[1])  # the angles are others
     assert math.isfinite(float(a[1].sum())) and device_error() == 0
+
+
+@pytest.mark.parametrize("page", [4, 16])
+def test_steps_beyond_the_longest_continuation_are_left_out_and_reported(model_and_ref, page):
+    d = decode.BeamDecoder(model_and_ref[0], 2, 3, 40, 5, page=page)
+    prompts = prompts_of(40, 3)
+    d.generate(prompts, 5, graph=False)
+    tokens, scores = d.generate(prompts, 5)
+    assert device_error() == 0
+    said = d.history(5)
+    pages = d.k[:, :2 * d._shared].clone()  # the prompts'
+    for _ in range(2 * page + 3):
+        d.graph.replay()
+    torch.cuda.synchronize()
+    assert device_error() & 64
+    assert torch.equal(d.k[:, :2 * d._shared], pages)
+    for n in (0, 6):
+        with pytest.raises(ValueError):
+            d.history(n)
+    again = d.generate(prompts, 5)
+    assert torch.equal(said, tokens) and torch.equal(again[0], tokens) and torch.equal(again[1], scores) and device_error() == 0
