@@ -13,7 +13,7 @@
 //
 // Measured (32 query heads over 8 of 128): one sequence of 130 slots 6.0 us, of which the launch is 0.8 and the rest one chain of
 // latencies; four of 2,048 slots in 32 bits 21 us (67 MB: 10.6 of memory, 6 of beginning and end, 3.5 of the second launch); 64 ragged sequences,
-// 1.14 GB, 198 us, 5.8 TB/s; 131,001 slots, 537 MB, 93 us, 5.8 TB/s, where a plain sum over as many bytes takes 92.
+// 1.14 GB, 193 us, 5.9 TB/s; 131,001 slots, 537 MB, 89 us, 6.0 TB/s, where a plain sum over as many bytes takes 92.
 
 struct PagedAttnArgs {
     const char *q;
@@ -228,11 +228,11 @@ struct Tiles {
 // or nothing, so that an infinite value that is seen comes out as itself. The maximum only moves where a score is 2^8 above it: one vote a tile in place of
 // a reduction and a rescaling. The products take no time that shows: one head or eight on each cache head, 51 us for 262 MB; twelve, with
 // two columns of products, 57.
-template <typename T, int D, int kN>
+template <typename T, int D, int kN, int kWarps_>
 struct Core16 {
     static constexpr int kSub = D == 64 ? 2 : 1, kTile = 16 * kSub, kRows = 8 * kN;  // sixteen slots make a product; shorter rows come in tiles of as many bytes
     using Tile = Tiles<kTile, 2 * D, 4, 64, 2, 32>;
-    static constexpr int kDepth = kN == 2 ? 3 : 2, kWarps = kN == 1 ? 12 : 8, kShared = kDepth * Tile::kBytes;  // of a warp
+    static constexpr int kWarps = kWarps_, kDepth = 24 / kWarps, kShared = kDepth * Tile::kBytes;  // of a warp
     static constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = 8.f;
     uint32_t q[kN][D / 32][4];
     float o[kN][D / 16][4], m[kN][2], l[kN][2];
@@ -823,7 +823,7 @@ bool attn_wide(const p8_paged *c, int64_t heads) {  // the larger of the two til
 int attn_rows(const p8_paged *c, int64_t heads) { return (c->type == P8_KV_F32 ? 4 : 8) * (attn_wide(c, heads) ? 2 : 1); }
 int attn_warps(const p8_paged *c, int64_t heads) {
     if (c->type == P8_KV_F32) return attn_wide(c, heads) ? Core32<128, 8>::kWarps : Core32<128, 4>::kWarps;
-    return attn_wide(c, heads) ? Core16<__half, 128, 2>::kWarps : Core16<__half, 128, 1>::kWarps;
+    return attn_wide(c, heads) ? 8 : 12;  // (at most)
 }
 int64_t attn_units(const p8_paged *c, int64_t heads) { return c->rows * c->heads * attn_blocks(c, heads); }
 // Whether a unit can be cut at all: not where each has a CTA's least share to itself and no sequence can be longer.
@@ -833,16 +833,22 @@ size_t attn_part_bytes(const p8_paged *c, int64_t heads) {
 }
 size_t paged_attn_workspace(const p8_paged *c, int64_t heads) { return attn_cuts(c, heads) ? attn_part_bytes(c, heads) + (size_t)attn_units(c, heads) * sizeof(int2) : 0; }
 
+// shares of the least size that the list has, if all sequences are as long as they can be
+int64_t attn_shares(const p8_paged *c, int64_t heads) { return attn_units(c, heads) * ((c->columns * c->page + kSpan - 1) / kSpan); }
+
+// whether a tile's blocks of rows lie side by side: of keys, of values
+template <typename Tile>
+bool side_by_side(const p8_paged *c, int z) { return (c->page == 1 || (z ? c->v_stride : c->k_stride)[3] == c->width) && c->page % Tile::kRowsOf[z] == 0; }
+
 template <typename T, int D, typename Core>
 p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStream_t st) {
     const auto kernel = k_paged_attn<T, D, Core>;
     constexpr int smem = Core::kWarps * Core::kShared;
     if (!allow_shared(kernel, which, smem)) return P8_ERR_CUDA;
-    const int64_t *const strides[2] = {c->k_stride, c->v_stride};
-    for (int z = 0; z < 2; ++z) a.side[z] = (c->page == 1 || strides[z][3] == D) && c->page % Core::Tile::kRowsOf[z] == 0;
+    for (int z = 0; z < 2; ++z) a.side[z] = side_by_side<typename Core::Tile>(c, z);
     a.pad = attn_units(c, a.heads) <= a.ctas ? kSpan / Core::kTile : 1;  // where every unit can have a CTA, a short one does
     // shares that there can be; in a CTA's share, and in the workspace, places and rows are counted in 32 bits
-    const int64_t units = attn_units(c, a.heads), most = units * ((c->columns * c->page + kSpan - 1) / kSpan);
+    const int64_t units = attn_units(c, a.heads), most = attn_shares(c, a.heads);
     if (most / a.ctas >= INT32_MAX / 32 || c->rows * a.heads >= INT32_MAX - 256) return P8_ERR_UNSUPPORTED;
     if (launch_after(kernel, dim3((unsigned int)std::min<int64_t>(a.ctas, most)), dim3(32 * Core::kWarps), (size_t)smem, st, a) != cudaSuccess) return P8_ERR_CUDA;
     if (!a.cut) return P8_OK;
@@ -850,13 +856,26 @@ p8_status run_paged_attn(const p8_paged *c, PagedAttnArgs &a, int which, cudaStr
     if (a.ctas >= 4 * units) return done(launch_after(k_paged_join<T, D, Core, 8>, dim3((unsigned int)rows), dim3(256), 0, st, a));
     return done(launch_after(k_paged_join<T, D, Core, 1>, dim3((unsigned int)((rows + 7) / 8)), dim3(256), 0, st, a));
 }
+// 16-bit caches and up to eight heads a unit: eight warps with three tiles each keep more bytes in flight than twelve with two (which have
+// asked for no other tile than the next while they work on one): 537 MB 90 us and 93, 1.14 GB 195 and 201, one sequence of 4,000 slots 12.0 and
+// 13.7. They need tiles that are asked for quickly, in blocks of rows, and that take one pass of products (pages of one slot 74 us
+// for 262 MB and 61, heads of 64 61 and 54), and units of some tiles (200 sequences of 150 slots 47 us and 46, one of 130 6.8 and 6.1, one of 2,000
+// 10.6 and 10.2).
+template <typename T, int D>
+p8_status run_paged_attn_16(const p8_paged *c, PagedAttnArgs &a, bool wide, int which, cudaStream_t st) {
+    if (wide) return run_paged_attn<T, D, Core16<T, D, 2, 8>>(c, a, which, st);
+    if constexpr (D == 128) {
+        using Eight = Core16<T, D, 1, 8>;
+        if (c->columns * c->page > kSpan && side_by_side<typename Eight::Tile>(c, 0) && side_by_side<typename Eight::Tile>(c, 1) && attn_shares(c, a.heads) > a.ctas) return run_paged_attn<T, D, Eight>(c, a, 12 + which, st);
+    }
+    return run_paged_attn<T, D, Core16<T, D, 1, 12>>(c, a, which, st);
+}
 template <int D>
 p8_status run_paged_attn_d(const p8_paged *c, PagedAttnArgs &a, cudaStream_t st) {
     const bool wide = attn_wide(c, a.heads);
     const int which = 4 * (int)c->type + 2 * wide + (D == 128);
     if (c->type == P8_KV_F32) return wide ? run_paged_attn<float, D, Core32<D, 8>>(c, a, which, st) : run_paged_attn<float, D, Core32<D, 4>>(c, a, which, st);
-    if (c->type == P8_KV_F16) return wide ? run_paged_attn<__half, D, Core16<__half, D, 2>>(c, a, which, st) : run_paged_attn<__half, D, Core16<__half, D, 1>>(c, a, which, st);
-    return wide ? run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 2>>(c, a, which, st) : run_paged_attn<__nv_bfloat16, D, Core16<__nv_bfloat16, D, 1>>(c, a, which, st);
+    return c->type == P8_KV_F16 ? run_paged_attn_16<__half, D>(c, a, wide, which, st) : run_paged_attn_16<__nv_bfloat16, D>(c, a, wide, which, st);
 }
 
 p8_status launch_paged_attn(const p8_paged *c, const p8_paged_attn_args *x, void *workspace, cudaStream_t st) {

@@ -282,6 +282,35 @@ def test_attention(name, case):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+# H, kv, page, lens: heads of 128 whose rows come in blocks, in tables that are longer than the sequences (the eight warps' form),
+# with lengths on either side of its tiles, rounds and shares, rows without a token and pages that are not there
+@pytest.mark.parametrize("name", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("H,kv,page,lens_", [(32, 8, 16, [0, 15, 16, 127, 128, 129, 383, 384, 385, 2000]), (4, 4, 4, [3 * i for i in range(300)]), (16, 2, 64, [9000, 1, 191, 192]), (1, 1, 8, [30000])])
+def test_attention_in_long_tables(name, H, kv, page, lens_):
+    g, dt = gen(H + page), TYPES[name]
+    pages = sum((n + page) // page for n in lens_) + 2
+    kp, vp = make_pages(g, pages, kv, page, 128, dt)
+    B, columns = len(lens_), (max(lens_) + page) // page + 3000 // page
+    tables = torch.full((B, columns), -1, dtype=torch.int32, device="cuda")
+    short = make_tables(g, lens_, 1, page, pages)
+    tables[:, :short.shape[1]] = short
+    lens, q = ints(*lens_), randn(g, B, H, 128, dtype=dt, scale=1.5)
+    counts = torch.ones(B, dtype=torch.int32, device="cuda")
+    if B > 1:
+        counts[B // 2] = 0
+        tables[0, 0], tables[B - 1, 0] = pages, -7  # all of a sequence of one page, and a beginning
+    want = attend(q, kp, vp, tables, lens, counts, 128 ** -0.5)
+    out, lse = paged.paged_attention(q, kp, vp, tables, lens, counts=counts)
+    ended(64 if B > 1 else 0)
+    live = counts.bool()
+    close(out[live], want[0][live], want[2][live], "out")
+    close(lse[live], want[1][live], want[3][live], "lse")
+    assert not out[~live].any() and not lse[~live].any()
+    again, lse2 = paged.paged_attention(q, kp, vp, tables, lens, counts=counts)
+    ended(64 if B > 1 else 0)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
 @pytest.mark.parametrize("name", ["fp32", "fp16", "bf16"])
 def test_attention_rows_without_a_token_and_pages_out_of_range(name):
     g, dt = gen(8), TYPES[name]
