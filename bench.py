@@ -199,6 +199,15 @@ def ref_slots(model, seed=0):
     return _REF_CACHE[key]
 
 
+NO_CPU_REFERENCE = "the reference's CPU core is not built here (oracle/_ref: oracle/build_ref.py needs its sources)"
+
+
+def cpu_reference_built():
+    from oracle.oracle import RefOracle
+
+    return RefOracle.available()
+
+
 def cpu_reference_token(model, reps, warmup, seed=0):
     """The reference's own CPU core (oracle/_ref: vr-native-cpu-core.h with the vrc_tg glue, x16 activations) over one
     decode token: every projection of every layer, 32 x 7 distinct class-3 slots (1.80 GB, far larger than any host
@@ -321,6 +330,9 @@ def gpu_reference_token(model, steps, warmup, seed=0):
 def run_reference(args, rank, world):
     model = LLAMA8B
     if rank != 0:
+        return 0
+    if not cpu_reference_built():
+        print(json.dumps({"impl": "reference", "unavailable": NO_CPU_REFERENCE}), flush=True)
         return 0
     tok_s_time, cores, isa = cpu_reference_token(model, reps=max(1, args.steps), warmup=max(1, args.warmup))
     tok_s = 1.0 / tok_s_time
@@ -1071,7 +1083,9 @@ def run_b200(args, rank, world, local_rank):
                            "config": "512 tokens x 224 projections (32 layers), distinct weights, inputs resident",
                            "c3_per_gemm": {"what": "config C3: each projection alone (p8_mul_mat), per call; tflops of "
                                                    "2 x rows x K x tokens", "tokens": c3}}
-    if world == 1 and not args.no_cpu:
+    if world == 1 and not args.no_cpu and not cpu_reference_built():
+        line["cpu_baseline"] = {"unavailable": NO_CPU_REFERENCE}
+    elif world == 1 and not args.no_cpu:
         tok_time, cores, isa = cpu_reference_token(model, reps=5, warmup=1)
         line["cpu_baseline"] = {"value": round(1.0 / tok_time, 4), "unit": "tok/s", "cores": cores, "kind": "reference",
                                 "sample": f"5 tokens, each all {model['layers'] * 7} projections (distinct slots, 1.80 GB), median; "
