@@ -505,7 +505,7 @@ p8_status p8_paged_attn(const p8_paged *c, const p8_paged_attn_args *a, void *wo
  * parent had ended or the token is `end` (end < 0: there is none, and done must be NULL), 0 for candidates that are not there.
  *
  * Logits of p8_kv_type `type`, element (b, w, t) at b * stride[0] + w * stride[1] + t, strides >= 0 (0: the
- * same for all; 1 <= vocab < 2^31); scores and results are contiguous. Logits of beams that have ended or whose score is not finite are not read.
+ * same for all; 1 <= vocab < 2^31 - 2^16); scores and results are contiguous. Logits of beams that have ended or whose score is not finite are not read.
  * Results overlap neither one another, nor the workspace, nor what is read. Workspace: p8_beam_select_workspace bytes, 256-byte
  * aligned. Deterministic. */
 typedef struct p8_beam_select_args {
